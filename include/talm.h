@@ -31,6 +31,7 @@ extern "C" {
 /* Element types of the tensors whose dtype is a runtime argument. */
 #define TALM_F32 0
 #define TALM_F16 1
+#define TALM_BF16 2 /* the entry points that say so */
 
 /* Message of the last failed call on this thread ("" after a success). */
 const char* talm_last_error(void);
@@ -607,6 +608,117 @@ int talm_head_restore(const float* token_loss, const float* entropy, const int32
                       int32_t* correct_out, int32_t* best_idx_out, uint16_t* grad_out, void* stream);
 int talm_scale_rows(const uint16_t* g, int64_t n, const float* grad_loss, const float* denom,
                     uint16_t* out, void* stream);
+
+/*
+ * talm_attn_fwd in a sliding window: row i of a sequence attends to the keys j <= i with i - j <
+ * window or j < sinks (the sequence's first `sinks` tokens stay visible; 0: none). window >= 1; one
+ * of at least the longest sequence is the causal attention. dtype TALM_F16 or TALM_BF16 (q, k, v
+ * and out); scale positive. Key tiles that no row sees are not read: the work grows with
+ * n_tokens (window + sinks). q, k and v have to be finite (a masked key has weight 0, but 0 times an
+ * infinity is no number). Rows behind the last sequence (cu_seqlens[n_seqs]) are left as they were.
+ * No counterpart in the reference, whose packed rows exclude sliding layers (solution/patches.py:
+ * 173-260).
+ */
+int talm_attn_window_fwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                         const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                         const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
+                         const int32_t* cu_seqlens, int32_t n_seqs, int32_t max_seqlen,
+                         int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim,
+                         float scale, int32_t window, int32_t sinks, int32_t dtype, uint16_t* out,
+                         int64_t o_stride_tok, int64_t o_stride_head, float* lse, void* stream);
+
+/*
+ * Its backward: talm_attn_bwd (cos and sin NULL) or talm_attn_bwd_rope in the window. Rows behind
+ * the last sequence get zero gradients. `workspace` (256-byte aligned) holds
+ * talm_attn_window_bwd_workspace(...) bytes (-1 for arguments the call would reject): the causal
+ * backward's, and partials of the sinks' gradients from the rows past their window (at most 64 MiB,
+ * or one set if that is more). Deterministic. No counterpart in the reference.
+ */
+int64_t talm_attn_window_bwd_workspace(int64_t n_tokens, int32_t n_q_heads, int32_t n_seqs,
+                                       int32_t max_seqlen, int32_t window, int32_t sinks);
+int talm_attn_window_bwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                         const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                         const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
+                         const uint16_t* out, int64_t o_stride_tok, int64_t o_stride_head,
+                         const uint16_t* dout, int64_t do_stride_tok, int64_t do_stride_head,
+                         const float* lse, const int32_t* cu_seqlens, int32_t n_seqs,
+                         int32_t max_seqlen, int64_t n_tokens, int32_t n_q_heads,
+                         int32_t n_kv_heads, int32_t head_dim, float scale, int32_t window,
+                         int32_t sinks, int32_t dtype, const float* cos, const float* sin,
+                         int64_t cs_stride, uint16_t* dq, int64_t dq_stride_tok,
+                         int64_t dq_stride_head, uint16_t* dk, int64_t dk_stride_tok,
+                         int64_t dk_stride_head, uint16_t* dv, int64_t dv_stride_tok,
+                         int64_t dv_stride_head, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+
+/*
+ * Dropout with a mask computed from a counter-based generator and never stored: y = x factor where
+ * the element is kept, 0 elsewhere; the backward is the same call on dy. Element (r, c) of x
+ * [rows, cols] (row stride ldx) has 16 random bits, halfword c % 8 of the Philox-4x32-10 block with
+ * counter (block low, block high, site, low word of key[1]) and key key[0], block = r ceil(cols / 8)
+ * + c / 8; it is kept when they are >= T = round(65536 p) (at most 65535), factor = 65536 / (65536 -
+ * T). key int64 [2] in device memory (read by the kernel, so a captured graph follows its
+ * contents), may be NULL when T = 0; `site` tells a program's dropouts that share a key apart.
+ * dtype TALM_F32, TALM_F16 or TALM_BF16; 0 <= p < 1; y may be x. Replaces native_dropout with a stored or replayed
+ * mask (solution/lora.py:183-186, :209-216).
+ */
+int talm_dropout(const void* x, int64_t ldx, int64_t rows, int64_t cols, int32_t dtype, float p,
+                 const int64_t* key, uint32_t site, void* y, int64_t ldy, void* stream);
+
+/*
+ * The LoRA adapters' products with dropout on x (the mask of talm_dropout on x [n_tokens, k],
+ * adapter g's with site_g), fp16 with fp32 sums, rank 16, 1 or 2 adapters; factor as above.
+ *
+ * talm_lora_down_drop: t[:, 16g:16g+16] = fp16(factor (keep_g x) A_g^T), ts = fp16(scaling_g times the
+ * same sum); A_g f16 [16, k], k a multiple of 32; `workspace` holds
+ * talm_lora_down_drop_workspace bytes (0: may be NULL).
+ *
+ * talm_lora_up: out [n_tokens, cols] = base + sum_g factor keep_g (u[:, 16g:16g+16] M_g^T), one rounding;
+ * M_g f16 [cols, 16], or [16, cols] with m_kmajor; base NULL (0) or f16 [n_tokens, cols], may be out;
+ * the mask on out's elements (p = 0: none). The adapter's output ts B^T, and with A and the masks
+ * the input gradient u A.
+ *
+ * talm_lora_wgrad_drop: dA_g [16, hidden] = factor u_g^T (keep_g x), dB_g [seg_g, 16] = scaling_g
+ * dy[:, lo_g:lo_g+seg_g]^T t_g in grad_dtype (TALM_F32 or TALM_F16), summed in fp32 over the tokens in fixed chunks and those in order
+ * (deterministic); zeros for no tokens. `workspace` holds talm_lora_wgrad_drop_workspace bytes.
+ *
+ * Sizes and strides multiples of 8, operands 16-byte aligned. They replace the adapters' GEMMs
+ * around native_dropout (solution/fused_proj.py:139-153, :188-215, solution/lora.py:183-231).
+ */
+int64_t talm_lora_down_drop_workspace(int64_t n_tokens, int64_t k, int32_t n_adapters);
+int talm_lora_down_drop(const uint16_t* x, int64_t ldx, int64_t n_tokens, int64_t k,
+                        const uint16_t* a0, const uint16_t* a1, int32_t n_adapters, float p,
+                        const int64_t* key, uint32_t site0, uint32_t site1, float scaling0,
+                        float scaling1, uint16_t* t, uint16_t* ts, int64_t ldt, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+int talm_lora_up(const uint16_t* u, int64_t ldu, int64_t n_tokens, int64_t cols, const uint16_t* m0,
+                 const uint16_t* m1, int32_t n_adapters, int32_t m_kmajor, float p,
+                 const int64_t* key, uint32_t site0, uint32_t site1, const uint16_t* base,
+                 int64_t ldb, uint16_t* out, int64_t ldo, void* stream);
+int64_t talm_lora_wgrad_drop_workspace(int64_t n_tokens, int64_t hidden, int32_t n_adapters,
+                                       int64_t seg0, int64_t seg1);
+int talm_lora_wgrad_drop(const uint16_t* x, int64_t ldx, const uint16_t* dy, int64_t ldy,
+                         const uint16_t* u, int64_t ldu, const uint16_t* t, int64_t ldt,
+                         int64_t n_tokens, int64_t hidden, int32_t n_adapters, float p,
+                         const int64_t* key, uint32_t site0, uint32_t site1, int32_t grad_dtype,
+                         int64_t lo0, int64_t seg0, float scaling0, void* da0, void* db0,
+                         int64_t lo1, int64_t seg1, float scaling1, void* da1, void* db1, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/*
+ * Products of a few tokens with a weight W [rows, cols] in the NF4 form of talm_nf4_group_dequant
+ * (packed, absmax8, absmax2, offset2 starting at W's first weight, a multiple of qblock qblock2):
+ * out [n_tokens, rows] = fp16(x [n_tokens, cols] W^T + bias). At most 32 tokens (0: nothing is
+ * done). The fp16 weights are bit-identical to talm_nf4_group_dequant's and never written out;
+ * fp32 sums in a fixed order. qblock 64, qblock2 a power of two; cols a multiple of 64; x and out
+ * fp16 with row strides ldx (a multiple of 8) and ldo; bias f16 [rows] or NULL; x and packed
+ * 16-byte aligned. Replaces the dequantization of the layer plus the projection's GEMM
+ * (solution/qgroup.py:72-99, :346-355) for single-token calls.
+ */
+int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, const uint8_t* packed,
+                  const uint8_t* absmax8, const float* code, const float* absmax2,
+                  const float* offset2, int64_t rows, int64_t cols, int32_t qblock,
+                  int32_t qblock2, const uint16_t* bias, uint16_t* out, int64_t ldo, void* stream);
 
 #ifdef __cplusplus
 }

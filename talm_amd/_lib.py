@@ -10,15 +10,16 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libtalm.so"
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 TALM_OK, TALM_EINVAL, TALM_EHIP = 0, 1, 2
-TALM_F32, TALM_F16 = 0, 1
+TALM_F32, TALM_F16, TALM_BF16 = 0, 1, 2
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
 _F32 = ctypes.c_float
+_U32 = ctypes.c_uint32
 
 # Every exported entry point with its argument types (all return int status).
 SIGNATURES = {
@@ -60,6 +61,21 @@ SIGNATURES = {
     "talm_attn_bwd_rope": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P,
                            _I64, _I64, _P, _P, _I32, _I32, _I64, _I32, _I32, _I32, _F32, _P, _P,
                            _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _P],
+    "talm_attn_window_fwd": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I32, _I32, _I64,
+                             _I32, _I32, _I32, _F32, _I32, _I32, _I32, _P, _I64, _I64, _P, _P],
+    "talm_attn_window_bwd": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P,
+                             _I64, _I64, _P, _P, _I32, _I32, _I64, _I32, _I32, _I32, _F32, _I32,
+                             _I32, _I32, _P, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64,
+                             _I64, _P, _I64, _P],
+    "talm_dropout": [_P, _I64, _I64, _I64, _I32, _F32, _P, _U32, _P, _I64, _P],
+    "talm_lora_down_drop": [_P, _I64, _I64, _I64, _P, _P, _I32, _F32, _P, _U32, _U32, _F32, _F32, _P,
+                            _P, _I64, _P, _I64, _P],
+    "talm_lora_up": [_P, _I64, _I64, _I64, _P, _P, _I32, _I32, _F32, _P, _U32, _U32, _P, _I64, _P,
+                     _I64, _P],
+    "talm_lora_wgrad_drop": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I32, _F32, _P, _U32,
+                             _U32, _I32, _I64, _I64, _F32, _P, _P, _I64, _I64, _F32, _P, _P, _P, _I64,
+                             _P],
+    "talm_nf4_gemv": [_P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _P, _P, _I64, _P],
     "talm_lora_mirror": [_P, _I32, _I64, _P, _P],
     "talm_rope_table": [_P, _I64, _P, _I32, _F32, _P, _P, _P],
     "talm_pack_rows": [_P, _P, _P, _I32, _I32, _I64, _P, _P, _P, _P, _P, _P],
@@ -87,6 +103,9 @@ SIZE_FUNCTIONS = {
     "talm_head_ce_workspace": [_I64, _I64, _I64, _I64, _I64, _I32],
     "talm_lora_wgrad_workspace": [_I64, _I64, _I64, _I64],
     "talm_attn_bwd_workspace": [_I64, _I32],
+    "talm_attn_window_bwd_workspace": [_I64, _I32, _I32, _I32, _I32, _I32],
+    "talm_lora_down_drop_workspace": [_I64, _I64, _I32],
+    "talm_lora_wgrad_drop_workspace": [_I64, _I64, _I32, _I64, _I64],
     "talm_gemm_splitk_workspace": [_I64, _I64, _I64],
     "talm_nf4_gemm_workspace": [_I64, _I64, _I64, _I32],
     "talm_gemm_splitk_parts": [_I64, _I64, _I64],

@@ -7,7 +7,7 @@ are the caller's tensors, annotated as mutated). They are registered for the CUD
 dispatch key only: a CPU tensor raises NotImplementedError from the dispatcher, never a CPU
 fallback. Importing this module loads both libraries or raises (no fallback).
 
-The workspace sizes of head_ce, lora_wgrad, attn_bwd and gemm_splitk are plain functions over the
+The workspace sizes of head_ce, lora_wgrad, attn_bwd, gemm_splitk and their kin are plain functions over the
 C-ABI's size queries.
 """
 
@@ -26,7 +26,8 @@ OPS = ("nf4_group_dequant", "nf4_group_dequant_streaming", "nf4_dequant", "rmsno
        "lora_adamw", "nf4_gemm", "nf4_block_scales", "nf4_group_dequant_t", "gemm_splitk",
        "pack_rows", "row_stats", "head_loss", "scatter_rows", "head_order", "head_restore", "scale_rows",
        "gemm_splitk_partials", "nf4_gemm_partials", "splitk_add_rmsnorm", "splitk_rmsnorm_bwd",
-       "rope_table", "lora_grad_norm", "lora_adamw_clipped")
+       "rope_table", "lora_grad_norm", "lora_adamw_clipped", "attn_window_fwd",
+       "attn_window_bwd", "dropout", "lora_down_drop", "lora_up", "lora_wgrad_drop", "nf4_gemv")
 
 _load_lock = threading.Lock()
 _loaded = False
@@ -75,6 +76,25 @@ def lora_wgrad_workspace_bytes(n_tokens, hidden, seg0, seg1):
 def attn_bwd_workspace_bytes(n_tokens, n_q_heads):
     size = _lib.lib().talm_attn_bwd_workspace(n_tokens, n_q_heads)
     _require(size >= 0, "attn_bwd: unsupported shape")
+    return int(size)
+
+
+def attn_window_bwd_workspace_bytes(n_tokens, n_q_heads, n_seqs, max_seqlen, window, sinks):
+    size = _lib.lib().talm_attn_window_bwd_workspace(n_tokens, n_q_heads, n_seqs, max_seqlen, window,
+                                                     sinks)
+    _require(size >= 0, "attn_window_bwd: unsupported shape")
+    return int(size)
+
+
+def lora_down_drop_workspace_bytes(n_tokens, k, n_adapters):
+    size = _lib.lib().talm_lora_down_drop_workspace(n_tokens, k, n_adapters)
+    _require(size >= 0, "lora_down_drop: unsupported shape")
+    return int(size)
+
+
+def lora_wgrad_drop_workspace_bytes(n_tokens, hidden, n_adapters, seg0, seg1):
+    size = _lib.lib().talm_lora_wgrad_drop_workspace(n_tokens, hidden, n_adapters, seg0, seg1)
+    _require(size >= 0, "lora_wgrad_drop: unsupported shape")
     return int(size)
 
 

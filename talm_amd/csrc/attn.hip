@@ -31,6 +31,16 @@
 //   attn_bwd_reduce the partials of a KV head's query heads summed in head order (deterministic)
 //                   into dK, dV fp16.
 // The dQ and dK / dV bodies run in one launch.
+//
+// The same kernels also run in a sliding window (kWin): row i attends to the keys j <= i with
+// i - j < window or j < sinks, a few first tokens of the sequence that stay visible to every row
+// (sinks = 0: none). Key tiles that no row of a workgroup sees are not visited: its list of tiles is
+// the sinks' tiles, then the window's; the border tiles are masked like the diagonal one. In the
+// backward a key tile's query rows end with the window, but for the sinks, whose rows run to the
+// end of the sequence: rows past the window are separate work items of `far_rows` rows each with
+// partials of their own (attn_bwd_far_kernel adds them in order: deterministic), so that no item's
+// chain is much longer than a window.
+// Operands are fp16 or, in a window, bf16 (the element type E).
 #include "mfma_tile.h"
 
 #include <algorithm>
@@ -50,6 +60,69 @@ constexpr int kKS = kD + 8;     // row stride (halfs) of a [keys][D] tile in LDS
 constexpr float kLn2 = 0.693147180559945309f;
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The operands' element type: fragments and tiles are carried as half8_t / 16-bit words whatever
+// it is; these are the places where it matters.
+struct F16 {
+  static __device__ __forceinline__ f32x16 mfma(half8_t a, half8_t b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ _Float16 cvt(float x) { return static_cast<_Float16>(x); }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack2(lo, hi); }
+  static __device__ __forceinline__ float lo(uint32_t w) { return lo_f(w); }
+  static __device__ __forceinline__ float hi(uint32_t w) { return hi_f(w); }
+};
+struct BF16 {
+  typedef __bf16 x8 __attribute__((ext_vector_type(8)));
+  typedef __bf16 x2 __attribute__((ext_vector_type(2)));
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  static __device__ __forceinline__ f32x16 mfma(half8_t a, half8_t b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(x8, a), __builtin_bit_cast(x8, b), c,
+                                                   0, 0, 0);
+  }
+  static __device__ __forceinline__ _Float16 cvt(float x) {
+    return __builtin_bit_cast(_Float16, static_cast<__bf16>(x));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){lo, hi}, x2));
+  }
+  static __device__ __forceinline__ float lo(uint32_t w) { return __builtin_bit_cast(float, w << 16); }
+  static __device__ __forceinline__ float hi(uint32_t w) {
+    return __builtin_bit_cast(float, w & 0xffff0000u);
+  }
+};
+
+// The rows [s0, s0 + len) of sequence `seq`; in a window kept inside the n_tokens rows whatever
+// `cu` holds.
+struct Rows {
+  int s0, len;
+};
+template <bool kWin>
+__device__ __forceinline__ Rows seq_rows(const int32_t* cu, int seq, int64_t n_tokens) {
+  Rows r{cu[seq], cu[seq + 1]};
+  if constexpr (kWin) {
+    const int n = static_cast<int>(n_tokens);
+    r.s0 = min(max(r.s0, 0), n);
+    r.len = min(max(r.len, r.s0), n);
+  }
+  r.len -= r.s0;
+  return r;
+}
+
+// The key tiles that a workgroup's rows [q0, ..) see, as a list: the sinks' tiles that lie before the
+// window's first one, then the window's up to the diagonal. Without a window every tile from 0.
+template <bool kWin>
+struct KeyTiles {
+  int n_sink = 0, first = 0;  // list index i < n_sink is tile i, else tile i - n_sink + first
+  __device__ __forceinline__ KeyTiles(int q0, int window, int sinks) {
+    if constexpr (kWin) {
+      first = max(q0 - window + 1, 0) / kKeys;
+      n_sink = min((sinks + kKeys - 1) / kKeys, first);
+    }
+  }
+  __device__ __forceinline__ int tile(int i) const { return kWin && i >= n_sink ? i - n_sink + first : i; }
+  __device__ __forceinline__ int count(int n_kt) const { return kWin ? n_kt - first + n_sink : n_kt; }
+};
 
 // The larger of lane l's and lane l ^ 32's value (v_permlane32_swap: the first result holds the
 // lower half's values in both halves, the second the upper half's).
@@ -79,6 +152,7 @@ struct FwdArgs {
   int64_t o_tok, o_head;
   float* lse;         // [Hq, n_tokens]
   int64_t n_tokens;
+  int window, sinks;  // kWin: both at most the longest sequence's length, window >= 1
 };
 
 // K and V tiles of the forward in LDS: [64 keys][128 d] fp16 without padding, 16 chunks of 16
@@ -256,7 +330,7 @@ __device__ __forceinline__ int list_pair(int own, int m_max, unsigned pair, int 
 // for 8 rows of 2048: 253 registers, the same clock), s_setprio around the MFMAs (no change).
 // S = 2 where it does not: the longest workgroup's chain of key tiles sets the time (about 1.1 us
 // per tile), and two groups halve it; their partial results are merged through LDS at the end.
-template <int H, int S>
+template <class E, int H, int S, bool kWin>
 __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
   constexpr int R = 4 / H;           // 32-row blocks per workgroup
   constexpr int kRows = 32 * R;
@@ -270,7 +344,7 @@ __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
   int chunk, seq, tile;
   if (a.list_tiles) {
     const int l = threadIdx.x & 63;
-    const int ll = l < a.n_seqs ? a.cu[l + 1] - a.cu[l] : 0;
+    const int ll = l < a.n_seqs ? seq_rows<kWin>(a.cu, l, a.n_tokens).len : 0;
     const int own = min((max(ll, 0) + kRows - 1) / kRows, a.list_tiles);
     const unsigned pair = blockIdx.x / a.chunks;
     chunk = static_cast<int>(blockIdx.x - pair * a.chunks);
@@ -280,11 +354,12 @@ __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
     const int rank = static_cast<int>(a.rank_x ? blockIdx.x : blockIdx.z);
     chunk = static_cast<int>(a.rank_x ? blockIdx.y : blockIdx.x);
     seq = static_cast<int>(a.rank_x ? blockIdx.z : blockIdx.y);
-    tile = (a.cu[seq + 1] - a.cu[seq] + kRows - 1) / kRows - 1 - rank;  // every sequence's longest tiles first
+    tile = (seq_rows<kWin>(a.cu, seq, a.n_tokens).len + kRows - 1) / kRows - 1 - rank;  // every sequence's longest tiles first
     if (tile < 0) return;  // the whole workgroup, before any barrier
   }
   const int kvh = chunk / a.head_chunks, hc = chunk % a.head_chunks;
-  const int s0 = a.cu[seq], len = a.cu[seq + 1] - s0;
+  const Rows own_rows = seq_rows<kWin>(a.cu, seq, a.n_tokens);
+  const int s0 = own_rows.s0, len = own_rows.len;
   const int q0 = tile * kRows;
   const int tid = threadIdx.x, lane = tid & 63;
   // the wavefront index in a scalar register: everything the branches, loop bounds and the
@@ -304,18 +379,21 @@ __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
 #pragma unroll
     for (int s = 0; s < kD / 16; ++s) qf[s] = *reinterpret_cast<const half8_t*>(qp + 16 * s);
   }
-  const int n_kt = (min(len, q0 + kRows) + kKeys - 1) / kKeys;
+  const KeyTiles<kWin> tiles(q0, a.window, a.sinks);
+  const int n_kt = tiles.count((min(len, q0 + kRows) + kKeys - 1) / kKeys);
   const int n_steps = (n_kt + S - 1) / S;
   // tiles the wavefront's rows see: none where it has no row
   const int my_kt = w0 < row_end ? (min(len, w0 + 32) + kKeys - 1) / kKeys : 0;
+  const int my_lo = w0 - a.window + 1;  // kWin: the first key of its first row's window
   const uint16_t* kbase = a.k + static_cast<int64_t>(s0) * a.k_tok + kvh * a.k_head;
   const uint16_t* vbase = a.v + static_cast<int64_t>(s0) * a.v_tok + kvh * a.v_head;
   TileDma kd, vd;
   kd.init(a.k_tok, wave, lane);
   vd.init(a.v_tok, wave, lane);
   auto issue = [&](int step, int slot) {
-    const int kt = step * S + grp;
-    if (S > 1 && kt >= n_kt) return;
+    const int at = step * S + grp;
+    if (S > 1 && at >= n_kt) return;
+    const int kt = tiles.tile(at);
     unsigned char* dst = smem + grp * kRing + slot * kSlot;
     kd.issue(kbase + static_cast<int64_t>(kt * kKeys) * a.k_tok, len - kt * kKeys, dst, wave);
     vd.issue(vbase + static_cast<int64_t>(kt * kKeys) * a.v_tok, len - kt * kKeys, dst + kTileBytes,
@@ -358,9 +436,10 @@ __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
   }
   auto body = [&](int step, auto slot_) __attribute__((always_inline)) {
     constexpr int kOff = decltype(slot_)::value * kSlot;
-    const int kt = step * S + grp;
+    const int at = step * S + grp, kt = tiles.tile(at);
     if (kt >= my_kt) return;  // every key of the tile is after every row of the wavefront
     const int k0 = kt * kKeys;
+    if (kWin && k0 + kKeys <= my_lo && k0 >= a.sinks) return;  // before every row's window
     // S^T: the second 32 keys' operand reads are issued one by one behind the first block's MFMAs
     f32x16 st[2];
     half8_t kf[kD / 16];
@@ -373,7 +452,7 @@ __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
 #pragma unroll
       for (int s = 0; s < kD / 16; ++s) {
         lgkm_wait(b == 0 ? 7 : 7 - s, kf[s]);
-        st[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[s], qf[s], st[b], 0, 0, 0);
+        st[b] = E::mfma(kf[s], qf[s], st[b]);
         if (b == 0) {
           __builtin_amdgcn_sched_barrier(0);
           kf[s] = read16_untracked(kaddr[s], kOff + 8192);
@@ -389,17 +468,31 @@ __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
         for (int v = 0; v < 16; ++v)
           st[b][v] = 32 * b + 8 * (v >> 2) + (v & 3) > lim ? -INFINITY : st[b][v];
     }
+    if constexpr (kWin) {
+      if (k0 + a.window <= w0 + 31 && k0 + kKeys > a.sinks) {  // uniform: some row's window begins after the tile's first key
+        const int lo = qr - a.window - k0 - 4 * hh, sink = a.sinks - k0 - 4 * hh;
+        asm volatile("");
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int key = 32 * b + 8 * (v >> 2) + (v & 3);
+            st[b][v] = key <= lo && key >= sink ? -INFINITY : st[b][v];
+          }
+      }
+    }
     float mt = -INFINITY;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int v = 0; v < 16; ++v) mt = fmaxf(mt, st[b][v]);
     mt = c * half_max(mt);
-    const bool grow = mt > m + (kt < kEager ? 0.f : kLazy);
+    const bool grow = mt > m + (at < kEager ? 0.f : kLazy);
     if (__ballot(grow)) {  // some row's maximum moved: rescale those rows
       asm volatile("");
       const float m_new = grow ? mt : m;
-      const float alpha = exp2_(m - m_new);  // 0 on the first tile (m = -inf), 1 if unchanged
+      // 0 on the first tile (m = -inf), 1 if unchanged (a row that has seen no key yet: -inf - -inf)
+      const float alpha = kWin && !grow ? 1.f : exp2_(m - m_new);
       m = m_new;
       lsum *= alpha;
 #pragma unroll
@@ -417,11 +510,13 @@ __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
     };
     read_v(0, 0);
     float ps = 0.f;
+    // a row of a window may see no key of its first tiles: its weights are exp2(-inf - 0) = 0 then
+    const float mref = kWin && m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int v = 0; v < 16; ++v) {
-        const float pv = exp2_(__builtin_fmaf(st[b][v], c, -m));
+        const float pv = exp2_(__builtin_fmaf(st[b][v], c, -mref));
         st[b][v] = pv;
         ps += pv;
       }
@@ -433,13 +528,13 @@ __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
       if (g16 < 3) read_v(g16 + 1, buf ^ 1);  // the next group's fly during these MFMAs
       half8_t pb;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) pb[e] = static_cast<_Float16>(st[b][8 * h + e]);
+      for (int e = 0; e < 8; ++e) pb[e] = E::cvt(st[b][8 * h + e]);
 #pragma unroll
       for (int j = 0; j < kD / 32; ++j)
-        o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+        o[j] = E::mfma(
             __builtin_bit_cast(half8_t, __builtin_shufflevector(vt[buf][2 * j], vt[buf][2 * j + 1],
                                                                 0, 1, 2, 3, 4, 5, 6, 7)),
-            pb, o[j], 0, 0, 0);
+            pb, o[j]);
     }
   };
   ring2(n_steps, issue, [&](int step, int slot) __attribute__((always_inline)) {
@@ -462,7 +557,8 @@ __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
     __syncthreads();
     if (grp > 0) return;  // no barrier follows
     const float m2 = pml[2 * lane], l2 = pml[2 * lane + 1];
-    const float m_new = fmaxf(m, m2);  // m is finite: group 0 has key tile 0
+    // finite: group 0 has key tile 0 (in a window one of the groups has a key of every row)
+    const float m_new = fmaxf(m, m2);
     const float a1 = exp2_(m - m_new);
     const float a2 = exp2_(m2 - m_new);  // 0 when group 1 had no tile (m2 = -inf)
     m = m_new;
@@ -482,8 +578,8 @@ __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
     for (int g = 0; g < 4; ++g) {
       const int d0 = 32 * j + 8 * g + 4 * hh;
       uint2 w;
-      w.x = pack2(o[j][4 * g] * inv, o[j][4 * g + 1] * inv);
-      w.y = pack2(o[j][4 * g + 2] * inv, o[j][4 * g + 3] * inv);
+      w.x = E::pack(o[j][4 * g] * inv, o[j][4 * g + 1] * inv);
+      w.y = E::pack(o[j][4 * g + 2] * inv, o[j][4 * g + 3] * inv);
       *reinterpret_cast<uint2*>(&os[l32 * kKS + d0]) = w;
     }
   if (hh == 0 && qrow < row_end)
@@ -545,7 +641,22 @@ struct BwdArgs {
   const float* cos;
   const float* sin;
   int64_t cs_tok;
+  // kWin (window and sinks at most the longest sequence's length): the sinks' rows past their
+  // window in items of far_rows rows (a multiple of 64), far_chunks of them for each (sequence,
+  // 128-key tile of sinks, head); their partials [sequence][head][chunk][sink][D]
+  int window, sinks;
+  int far_rows, far_chunks, far_tiles;
+  unsigned far_items;  // n_seqs x far_chunks x far_tiles x heads
+  float* far_k;
+  float* far_v;
 };
+
+// The query row after the tiles of 64 rows that hold the window of any of a 128-key tile's keys: where
+// the items of its sinks' further rows begin.
+__device__ __forceinline__ int near_end(int k0, int len, int window) {
+  const int rows = min(len, k0 + 127 + window) - k0;
+  return k0 + (rows + 63) / 64 * 64;
+}
 
 // The rotary embedding's backward on one (d, d + 64) pair of four columns each: x = dy at
 // columns d .. d + 3, y at d + 64 .. d + 67, of the token whose cos / sin rows are cr / sr.
@@ -567,6 +678,7 @@ __device__ __forceinline__ void rope_back4(float (&x)[4], float (&y)[4], const f
 
 // Dd[h][t] = sum_d dO[t][h][d] * O[t][h][d] and lse2[h][t] = lse[h][t] log2 e (the exponent offset
 // both backward bodies subtract): 16 lanes per (token, head), 8 columns each.
+template <class E>
 __global__ __launch_bounds__(256) void attn_bwd_dot_kernel(BwdArgs a) {
   const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;  // t * Hq + h
   const int sub = threadIdx.x & 15;
@@ -577,9 +689,9 @@ __global__ __launch_bounds__(256) void attn_bwd_dot_kernel(BwdArgs a) {
   const int h = static_cast<int>(r % a.n_q_heads);
   const u32x4 x = *reinterpret_cast<const u32x4*>(a.o + t * a.o_tok + h * a.o_head + 8 * sub);
   const u32x4 y = *reinterpret_cast<const u32x4*>(a.dout + t * a.do_tok + h * a.do_head + 8 * sub);
-  float acc = lo_f(x.x) * lo_f(y.x) + hi_f(x.x) * hi_f(y.x) + lo_f(x.y) * lo_f(y.y) +
-              hi_f(x.y) * hi_f(y.y) + lo_f(x.z) * lo_f(y.z) + hi_f(x.z) * hi_f(y.z) +
-              lo_f(x.w) * lo_f(y.w) + hi_f(x.w) * hi_f(y.w);
+  float acc = E::lo(x.x) * E::lo(y.x) + E::hi(x.x) * E::hi(y.x) + E::lo(x.y) * E::lo(y.y) +
+              E::hi(x.y) * E::hi(y.y) + E::lo(x.z) * E::lo(y.z) + E::hi(x.z) * E::hi(y.z) +
+              E::lo(x.w) * E::lo(y.w) + E::hi(x.w) * E::hi(y.w);
 #pragma unroll
   for (int off = 8; off >= 1; off >>= 1) acc += __shfl_xor(acc, off, 16);
   if (sub == 0 && row < rows) {
@@ -649,11 +761,12 @@ __device__ __forceinline__ uint32_t slot_step(int slot) {
 
 // dQ: the forward's structure, one query row per lane (S^T = K Q^T, dP^T = V dO^T, then
 // dQ^T += K^T dS^T with K^T read transposed from the K tile); `tile` is the 32W-row query tile.
-template <int W, class Done>
+template <class E, int W, bool kWin, class Done>
 __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head, int tile,
                                             unsigned char* smem, Done&& done) {
   constexpr int kRows = 32 * W;
-  const int s0 = a.cu[seq], len = a.cu[seq + 1] - s0;
+  const Rows own_rows = seq_rows<kWin>(a.cu, seq, a.n_tokens);
+  const int s0 = own_rows.s0, len = own_rows.len;
   const int q0 = tile * kRows;
   if (q0 >= len) return;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -676,8 +789,11 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
   const float ddr = a.dd[static_cast<int64_t>(head) * a.n_tokens + s0 + qr];
   const int wq0 = q0 + 32 * wave;  // the wavefront's first query row
 
-  const int n_kt = (min(len, q0 + kRows) + kKeys - 1) / kKeys;
-  const int my_kt = (min(len, wq0 + 32) + kKeys - 1) / kKeys;  // tiles the wavefront's rows see
+  const KeyTiles<kWin> tiles(q0, a.window, a.sinks);
+  const int n_kt = tiles.count((min(len, q0 + kRows) + kKeys - 1) / kKeys);
+  // tiles the wavefront's rows see (in a window it also takes, masked, the ones that only the
+  // earlier rows of the workgroup see)
+  const int my_kt = tiles.count((min(len, wq0 + 32) + kKeys - 1) / kKeys);
   const int lim = min(qrow, len - 1) - 4 * hh;  // a lane's last key, minus its half's offset
   const uint16_t* kbase = a.k + static_cast<int64_t>(s0) * a.k_tok + kvh * a.k_head;
   const uint16_t* vbase = a.v + static_cast<int64_t>(s0) * a.v_tok + kvh * a.v_head;
@@ -686,7 +802,7 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
   vd.init(a.v_tok, wave, lane);
   auto issue = [&](int kt, int slot) __attribute__((always_inline)) {
     unsigned char* dst = smem + slot * kBwdSlot;
-    const int r0 = kt * kKeys;
+    const int r0 = tiles.tile(kt) * kKeys;
     kd.issue(kbase + static_cast<int64_t>(r0) * a.k_tok, len - r0, dst, wave);
     vd.issue(vbase + static_cast<int64_t>(r0) * a.v_tok, len - r0, dst + kTileBytes, wave);
   };
@@ -703,7 +819,7 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
   // dS^T = P^T (dP^T - Dd), P^T = exp2(S^T scale log2e - lse2): value v of block b
   auto value = [&](int b, int v) __attribute__((always_inline)) {
     const float p = exp2_(__builtin_fmaf(st[b][v], a.scale_log2, -lse2));
-    sb[v >> 3][v & 7] = static_cast<_Float16>(p * (dpt[b][v] - ddr));
+    sb[v >> 3][v & 7] = E::cvt(p * (dpt[b][v] - ddr));
   };
   // ... 0 where masked, for the block whose first key is kb: only on a block that reaches past the
   // wavefront's first row or past the sequence (a uniform branch that holds no MFMA: with two
@@ -715,6 +831,18 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
 #pragma unroll
       for (int v = 0; v < 16; ++v)
         sb[v >> 3][v & 7] = 8 * (v >> 2) + (v & 3) <= last ? sb[v >> 3][v & 7] : static_cast<_Float16>(0.f);
+    }
+    if constexpr (kWin) {
+      if (kb + a.window <= wq0 + 31 && kb + 32 > a.sinks) {  // the block begins before some row's window
+        int lo = lim - a.window - kb;
+        const int sink = a.sinks - kb - 4 * hh;
+        asm volatile("" : "+v"(lo));
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const int key = 8 * (v >> 2) + (v & 3);
+          sb[v >> 3][v & 7] = key <= lo && key >= sink ? static_cast<_Float16>(0.f) : sb[v >> 3][v & 7];
+        }
+      }
     }
   };
   auto read_kt = [&](auto blk, int i) __attribute__((always_inline)) {  // pair i: group i / 4, block i % 4
@@ -741,11 +869,11 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
       // outstanding behind the operand: the other row reads (8 while s < 4) and, from s = 5 on, 4
       // K^T reads per step
       lgkm_wait(s < 4 ? 7 : (7 - 2 * (s - 4)) + (kPrev ? 4 * (s - 4) : 0), f[x]);
-      st[kB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[x], qf[s], st[kB], 0, 0, 0);
+      st[kB] = E::mfma(f[x], qf[s], st[kB]);
       if constexpr (kPrev) value(kB ^ 1, 2 * s);
       __builtin_amdgcn_sched_barrier(0);
       lgkm_wait(s < 4 ? 6 : (6 - 2 * (s - 4)) + (kPrev ? 4 * (s - 4) : 0), f[x + 1]);
-      dpt[kB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[x + 1], df[s], dpt[kB], 0, 0, 0);
+      dpt[kB] = E::mfma(f[x + 1], df[s], dpt[kB]);
       if constexpr (kPrev) value(kB ^ 1, 2 * s + 1);
       __builtin_amdgcn_sched_barrier(0);
       if (s < 4) {
@@ -763,8 +891,7 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       lgkm_wait(14 - 2 * i, kt_[2 * i], kt_[2 * i + 1]);
-      acc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pair8(kt_[2 * i], kt_[2 * i + 1]),
-                                                          sb[i >> 2], acc[i & 3], 0, 0, 0);
+      acc[i & 3] = E::mfma(pair8(kt_[2 * i], kt_[2 * i + 1]), sb[i >> 2], acc[i & 3]);
     }
   };
   using B0 = std::integral_constant<int, 0>;
@@ -783,16 +910,17 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
   arrive(0);
   scores(B0{}, std::false_type{});
   scores(B1{}, std::true_type{});
-  mask(0);
+  mask(tiles.tile(0) * kKeys);
   gather();
   leave();
   for (int t = 1; t < my_kt; ++t) {
     arrive(t);
-    scores(B0{}, std::true_type{});  // block 1 of tile t - 1: never masked, a later tile is live
+    scores(B0{}, std::true_type{});  // block 1 of tile t - 1: not on the diagonal, a later tile is live
+    if constexpr (kWin) mask(tiles.tile(t - 1) * kKeys + 32);
     gather();
     rd.next_t(slot_step(slot == 0 ? 2 : slot - 1));
     scores(B1{}, std::true_type{});
-    mask(t * kKeys);
+    mask(tiles.tile(t) * kKeys);
     gather();
     leave();
   }
@@ -803,7 +931,7 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
   for (int i = 0; i < 8; ++i) read_kt(B1{}, i);
 #pragma unroll
   for (int v = 0; v < 16; ++v) value(1, v);
-  mask((my_kt - 1) * kKeys + 32);
+  mask(tiles.tile(my_kt - 1) * kKeys + 32);
   gather();
   for (int t = my_kt; t < n_kt; ++t) {  // tiles that only later rows of the workgroup see
     arrive(t);
@@ -848,8 +976,8 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
     for (int g = 0; g < 4; ++g) {
       const int d0 = 32 * j + 8 * g + 4 * hh;
       uint2 w;
-      w.x = pack2(dqv[j][4 * g], dqv[j][4 * g + 1]);
-      w.y = pack2(dqv[j][4 * g + 2], dqv[j][4 * g + 3]);
+      w.x = E::pack(dqv[j][4 * g], dqv[j][4 * g + 1]);
+      w.y = E::pack(dqv[j][4 * g + 2], dqv[j][4 * g + 3]);
       *reinterpret_cast<uint2*>(&os[l32 * kKS + d0]) = w;
     }
   // the wavefront reads back its own staging rows: its LDS writes complete first
@@ -874,14 +1002,29 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
 // dP untransposed: keys are accumulator columns), looping over 64-row query tiles: dV^T += dO^T P
 // and dK^T += Q^T dS with Q^T and dO^T read transposed from the row-major tiles. Each slot holds
 // the Q tile, the dO tile, then each wavefront's copy of the tile's 64 lse and 64 Dd values.
-template <int W, class Done>
-__device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int head, int tile,
+// kWin: chunk < 0 is the tile's rows up to the end of its keys' windows, chunk >= 0 that item of its
+// sinks' rows past them.
+template <class E, int W, bool kWin, class Done>
+__device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int head, int tile, int chunk,
                                               unsigned char* smem, Done&& done) {
   constexpr int kCols = 32 * W;  // keys per workgroup
   constexpr int kRowsT = kKeys;  // query rows per tile
-  const int s0 = a.cu[seq], len = a.cu[seq + 1] - s0;
+  const Rows own_rows = seq_rows<kWin>(a.cu, seq, a.n_tokens);
+  const int s0 = own_rows.s0, len = own_rows.len;
   const int k0 = tile * kCols;
   if (k0 >= len) return;
+  // causal: rows below k0 see no key here (k0 is a multiple of 64)
+  int qstart = k0, qstop = len;
+  if constexpr (kWin) {
+    const int end = near_end(k0, len, a.window);
+    if (chunk < 0) {
+      qstop = min(len, end);
+    } else {
+      qstart = end + chunk * a.far_rows;
+      if (qstart >= len) return;
+      qstop = min(len, qstart + a.far_rows);
+    }
+  }
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hh = lane >> 5, l32 = lane & 31;
@@ -889,7 +1032,8 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
   const int key = k0 + 32 * wave + l32;
   const int kr_ = min(key, len - 1);
   const int wk0 = k0 + 32 * wave;  // the wavefront's first key
-  const int q_end = key < len ? len : 0;  // a lane's query rows end here (a key past the sequence: none)
+  // a lane's query rows end here (a key past the sequence: none; in a window, but for the sinks: its window)
+  const int q_end = key >= len ? 0 : kWin && key >= a.sinks ? min(len, key + a.window) : len;
   half8_t kf[kD / 16], vf[kD / 16];
   {
     const uint16_t* kp = a.k + static_cast<int64_t>(s0 + kr_) * a.k_tok + kvh * a.k_head + 8 * hh;
@@ -900,8 +1044,7 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
       vf[s] = *reinterpret_cast<const half8_t*>(vp + 16 * s);
     }
   }
-  const int qstart = k0;  // causal: rows below k0 see no key here (k0 is a multiple of 64)
-  const int n_qt = (len - qstart + kRowsT - 1) / kRowsT;
+  const int n_qt = (qstop - qstart + kRowsT - 1) / kRowsT;
   const uint16_t* qbase = a.q + static_cast<int64_t>(s0) * a.q_tok + head * a.q_head;
   const uint16_t* dbase = a.dout + static_cast<int64_t>(s0) * a.do_tok + head * a.do_head;
   const __amdgpu_buffer_rsrc_t lrs = __builtin_amdgcn_make_buffer_rsrc(
@@ -938,14 +1081,15 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
   // P and dS of value v of the block (row 8 (v / 4) + 4 hh + v % 4 of it)
   auto value = [&](int blk, int v) __attribute__((always_inline)) {
     const float p = exp2_(__builtin_fmaf(sc[v], a.scale_log2, -l4[v >> 2][v & 3]));
-    pb[blk][v >> 3][v & 7] = static_cast<_Float16>(p);
-    sb[blk][v >> 3][v & 7] = static_cast<_Float16>(p * (dp[v] - d4[v >> 2][v & 3]));
+    pb[blk][v >> 3][v & 7] = E::cvt(p);
+    sb[blk][v >> 3][v & 7] = E::cvt(p * (dp[v] - d4[v >> 2][v & 3]));
   };
   // ... 0 where masked, for the block whose first row is q0 (query row < key or past the sequence,
   // key past the sequence): only where some row is masked for some key of the wavefront, a uniform
   // branch that holds no MFMA (with two copies of the products the accumulators were moved)
   auto mask = [&](int blk, int q0) __attribute__((always_inline)) {
-    if (q0 < wk0 + 31 || q0 + 32 > len || wk0 + 32 > len) {
+    if (q0 < wk0 + 31 || q0 + 32 > len || wk0 + 32 > len ||
+        (kWin && q0 + 31 >= wk0 + a.window && wk0 + 32 > a.sinks)) {
       int lo = key - q0 - 4 * hh;
       const int hi = q_end - q0 - 4 * hh;
       asm volatile("" : "+v"(lo));  // a real branch: selects on lo cannot be hoisted out of it
@@ -990,9 +1134,9 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
       // reads and, from s = 5 on, 4 transposed reads per step
       if (s < 4) lgkm_wait(14, f[x], f[x + 1]);
       else lgkm_wait((7 - 2 * (s - 4)) + (kPrev ? 4 * (s - 4) : 0), f[x]);
-      sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[x], kf[s], sc, 0, 0, 0);
+      sc = E::mfma(f[x], kf[s], sc);
       if (s >= 4) lgkm_wait((6 - 2 * (s - 4)) + (kPrev ? 4 * (s - 4) : 0), f[x + 1]);
-      dp = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[x + 1], vf[s], dp, 0, 0, 0);
+      dp = E::mfma(f[x + 1], vf[s], dp);
       __builtin_amdgcn_sched_barrier(0);
       if (s < 4) {
         f[x] = read16_untracked(rd.row[s + 4], kB * 8192);
@@ -1017,9 +1161,9 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
       const int g = u >> 3, i = u & 7, j = i >> 1;
       lgkm_wait(g == 0 ? 14 : 14 - 2 * i, tr[2 * i], tr[2 * i + 1]);
       if (i & 1)
-        dka[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pair8(tr[2 * i], tr[2 * i + 1]), sb[kB][g], dka[j], 0, 0, 0);
+        dka[j] = E::mfma(pair8(tr[2 * i], tr[2 * i + 1]), sb[kB][g], dka[j]);
       else
-        dva[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pair8(tr[2 * i], tr[2 * i + 1]), pb[kB][g], dva[j], 0, 0, 0);
+        dva[j] = E::mfma(pair8(tr[2 * i], tr[2 * i + 1]), pb[kB][g], dva[j]);
       __builtin_amdgcn_sched_barrier(0);
       if (g == 0) read_t(blk, 1, i);
       if constexpr (kNext) value(kB ^ 1, u);
@@ -1028,7 +1172,8 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
   };
   using B0 = std::integral_constant<int, 0>;
   using B1 = std::integral_constant<int, 1>;
-  const int t0 = (wk0 - qstart) / kRowsT;  // the first tile with a row at or past the wavefront's keys
+  // the first tile with a row at or past the wavefront's keys (past the window: none without a sink)
+  const int t0 = !kWin || chunk < 0 ? (wk0 - qstart) / kRowsT : wk0 < a.sinks ? 0 : n_qt;
   int slot = 0;  // of the tile in hand
   issue(0, 0);
   auto arrive = [&](int t) __attribute__((always_inline)) {
@@ -1085,6 +1230,12 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
   __syncthreads();  // every wavefront is done with the ring
   constexpr int kStageLd = kD + 4;
   float* stage = reinterpret_cast<float*>(smem) + wave * 32 * kStageLd;
+  // the partials' rows: the token's, or of an item past the window the sink's in the item's own
+  const bool far = kWin && chunk >= 0;
+  const int64_t row0 =
+      far ? ((static_cast<int64_t>(seq) * a.n_q_heads + head) * a.far_chunks + chunk) * a.sinks + wk0
+          : static_cast<int64_t>(head) * a.n_tokens + s0 + wk0;
+  const int key_end = far ? min(a.sinks, len) : len;
   auto store_rows = [&](const f32x16 (&acc)[kD / 32], float mul, float* part) {
 #pragma unroll
     for (int j = 0; j < kD / 32; ++j)
@@ -1101,18 +1252,57 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
       const int r = 2 * it + (lane >> 5), c = lane & 31;
       x[it] = *reinterpret_cast<const u32x4*>(&stage[r * kStageLd + 4 * c]);
     }
-    const __amdgpu_buffer_rsrc_t prs =
-        store_rsrc(part + (static_cast<int64_t>(head) * a.n_tokens + s0 + wk0) * kD);
+    const __amdgpu_buffer_rsrc_t prs = store_rsrc(part + row0 * kD);
 #pragma unroll
     for (int it = 0; it < 16; ++it) {
       const int r = 2 * it + (lane >> 5), c = lane & 31;
-      store16(prs, wk0 + r < len ? static_cast<uint32_t>((r * kD + 4 * c) * 4) : kOob, x[it]);
+      store16(prs, wk0 + r < key_end ? static_cast<uint32_t>((r * kD + 4 * c) * 4) : kOob, x[it]);
     }
     // the next call overwrites the rows: every read above has returned first
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   };
-  store_rows(dka, a.scale, a.dk_part);
-  store_rows(dva, 1.f, a.dv_part);
+  store_rows(dka, a.scale, far ? a.far_k : a.dk_part);
+  store_rows(dva, 1.f, far ? a.far_v : a.dv_part);
+}
+
+// kWin: item `i` of the sinks' rows past their windows: heads fastest, then 128-key tiles, chunks,
+// sequences. An item without a row returns at once.
+template <class E, int W, class Done>
+__device__ __forceinline__ void attn_bwd_far(const BwdArgs& a, unsigned i, unsigned char* smem,
+                                             Done&& done) {
+  const unsigned heads = static_cast<unsigned>(a.n_q_heads);
+  const unsigned tiles = static_cast<unsigned>(a.far_tiles), chunks = static_cast<unsigned>(a.far_chunks);
+  const unsigned head = i % heads, tile = i / heads % tiles, chunk = i / heads / tiles % chunks;
+  attn_bwd_dkdv<E, W, true>(a, static_cast<int>(i / heads / tiles / chunks), static_cast<int>(head),
+                            static_cast<int>(tile), static_cast<int>(chunk), smem, done);
+}
+
+// kWin: the partials of the sinks' rows past their windows added, in chunk order, to the ones of the
+// rows before: one thread per (sequence, head, sink, four columns).
+__global__ __launch_bounds__(256) void attn_bwd_far_kernel(BwdArgs a) {
+  const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t row = idx / (kD / 4);
+  const int c = static_cast<int>(idx % (kD / 4)) * 4;
+  const int key = static_cast<int>(row % a.sinks);
+  const int64_t sh = row / a.sinks;  // sequence * heads + head
+  if (sh >= static_cast<int64_t>(a.n_seqs) * a.n_q_heads) return;
+  const int seq = static_cast<int>(sh / a.n_q_heads), head = static_cast<int>(sh % a.n_q_heads);
+  const Rows own_rows = seq_rows<true>(a.cu, seq, a.n_tokens);
+  const int s0 = own_rows.s0, len = own_rows.len;
+  if (key >= len) return;
+  const int end = near_end(key / 128 * 128, len, a.window);
+  const int chunks = min(a.far_chunks, (max(len - end, 0) + a.far_rows - 1) / a.far_rows);
+  if (chunks == 0) return;
+  const int64_t at = (static_cast<int64_t>(head) * a.n_tokens + s0 + key) * kD + c;
+  const int64_t from = (sh * a.far_chunks * a.sinks + key) * kD + c, step = static_cast<int64_t>(a.sinks) * kD;
+  f32x4_t k = *reinterpret_cast<const f32x4_t*>(a.dk_part + at);
+  f32x4_t v = *reinterpret_cast<const f32x4_t*>(a.dv_part + at);
+  for (int i = 0; i < chunks; ++i) {
+    k += *reinterpret_cast<const f32x4_t*>(a.far_k + from + i * step);
+    v += *reinterpret_cast<const f32x4_t*>(a.far_v + from + i * step);
+  }
+  *reinterpret_cast<f32x4_t*>(a.dk_part + at) = k;
+  *reinterpret_cast<f32x4_t*>(a.dv_part + at) = v;
 }
 
 // dQ and the dK / dV partials in one launch: they read the same inputs and write disjoint
@@ -1121,17 +1311,28 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
 // 2 x rank): every sequence's longest work is dispatched first, rank by rank, so the workgroups
 // that wait for a free CU are the shortest ones. Rank r of a sequence of n tiles is dQ query tile
 // n - 1 - r (even z) and dK / dV key tile r (odd z); ranks past n exit at once.
-template <int W>
+// kWin: the first far_chunks x far_tiles of the z axis are the items of the sinks' rows past their
+// windows.
+template <class E, int W, bool kWin>
 __global__ __launch_bounds__(64 * W, 1) void attn_bwd_kernel(BwdArgs a) {
   __shared__ __attribute__((aligned(1024))) unsigned char smem[kBwdLds];
-  const int rank = static_cast<int>(blockIdx.z) >> 1;
-  const int len = a.cu[blockIdx.y + 1] - a.cu[blockIdx.y];
+  unsigned z = blockIdx.z;
+  if constexpr (kWin) {
+    const unsigned far = static_cast<unsigned>(a.far_chunks * a.far_tiles);
+    if (z < far) {
+      attn_bwd_far<E, W>(a, (blockIdx.y * far + z) * gridDim.x + blockIdx.x, smem, [] {});
+      return;
+    }
+    z -= far;
+  }
+  const int rank = static_cast<int>(z) >> 1;
+  const int len = seq_rows<kWin>(a.cu, blockIdx.y, a.n_tokens).len;
   const int n_own = (len + 32 * W - 1) / (32 * W);
   if (rank >= n_own) return;  // the whole workgroup, before any barrier
-  if ((blockIdx.z & 1) == 0)
-    attn_bwd_dq<W>(a, blockIdx.y, blockIdx.x, n_own - 1 - rank, smem, [] {});
+  if ((z & 1) == 0)
+    attn_bwd_dq<E, W, kWin>(a, blockIdx.y, blockIdx.x, n_own - 1 - rank, smem, [] {});
   else
-    attn_bwd_dkdv<W>(a, blockIdx.y, blockIdx.x, rank, smem, [] {});
+    attn_bwd_dkdv<E, W, kWin>(a, blockIdx.y, blockIdx.x, rank, -1, smem, [] {});
 }
 
 // The same work from a queue: one workgroup per CU takes items until none is left, the longest
@@ -1142,34 +1343,44 @@ __global__ __launch_bounds__(64 * W, 1) void attn_bwd_kernel(BwdArgs a) {
 //
 // An item is a (sequence, 128-token tile, dK/dV or dQ, head); its length follows the sequence's
 // tiles from there on (dK / dV: the query tiles after its keys; dQ: the key tiles before its
-// rows), the m of list_pair.
-template <int W>
+// rows), the m of list_pair. kWin: the first far_items are the ones of the sinks' rows past their
+// windows; the others' lengths end with the window, and their order matters less.
+template <class E, int W, bool kWin>
 __global__ __launch_bounds__(64 * W, 1) void attn_bwd_queue_kernel(BwdArgs a) {
   // the next item's index behind the ring
   __shared__ __attribute__((aligned(1024))) unsigned char smem[kBwdLds + 16];
   const int lane = threadIdx.x & 63;
-  const int len = lane < a.n_seqs ? a.cu[lane + 1] - a.cu[lane] : 0;
+  const int len = lane < a.n_seqs ? seq_rows<kWin>(a.cu, lane, a.n_tokens).len : 0;
   const int own = min((max(len, 0) + 32 * W - 1) / (32 * W), a.n_tiles);
   const unsigned pairs = static_cast<unsigned>(wave_count(own));
   const unsigned per_pair = 2u * static_cast<unsigned>(a.n_q_heads);
+  const unsigned far = kWin ? a.far_items : 0u;
   unsigned item = blockIdx.x;
   for (;;) {
-    const unsigned pair = item / per_pair;
-    if (pair >= pairs) break;
-    int seq;
-    const int lo = list_pair(own, a.n_tiles, pair, lane, seq);
-    const int rank = __builtin_amdgcn_readlane(own, seq) - lo;
-    const int which = static_cast<int>(item - pair * per_pair);
+    const unsigned pair = item < far ? 0u : (item - far) / per_pair;
+    if (item >= far && pair >= pairs) break;
+    int seq = 0, lo = 0, rank = 0;
+    if (!kWin || item >= far) {
+      lo = list_pair(own, a.n_tiles, pair, lane, seq);
+      rank = __builtin_amdgcn_readlane(own, seq) - lo;
+    }
+    const int which = static_cast<int>(item - far - pair * per_pair);
     // the next item is drawn when this one's products are done, while its results go out (drawn
     // before, the longest items would each hold back one more)
     unsigned next = 0xffffffffu;  // past every item
     auto draw = [&]() __attribute__((always_inline)) {
       if (threadIdx.x == 0) next = atomicAdd(a.counter, 1u);
     };
-    if (which < a.n_q_heads)
-      attn_bwd_dkdv<W>(a, seq, which, rank, smem, draw);
-    else
-      attn_bwd_dq<W>(a, seq, which - a.n_q_heads, lo - 1, smem, draw);
+    if (kWin && item < far) {
+      if constexpr (kWin) {
+        attn_bwd_far<E, W>(a, item, smem, draw);
+        if (threadIdx.x == 0 && next == 0xffffffffu) draw();  // an item without a row returned before its draw
+      }
+    } else if (which < a.n_q_heads) {
+      attn_bwd_dkdv<E, W, kWin>(a, seq, which, rank, -1, smem, draw);
+    } else {
+      attn_bwd_dq<E, W, kWin>(a, seq, which - a.n_q_heads, lo - 1, smem, draw);
+    }
     // the next item's counted waits start from nothing in flight, its ring from idle slots
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -1219,7 +1430,8 @@ __device__ __forceinline__ void sum_heads4(const BwdArgs& a, int kvh, int64_t t,
   }
 }
 
-template <bool kRope>
+// kWin: rows behind the last sequence get zero gradients (dq's too: no query tile holds them).
+template <class E, bool kRope, bool kWin>
 __global__ __launch_bounds__(256) void attn_bwd_reduce_kernel(BwdArgs a) {
   constexpr int kGroups = kRope ? kD / 8 : kD / 4;  // threads per (token, KV head)
   const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
@@ -1235,6 +1447,18 @@ __global__ __launch_bounds__(256) void attn_bwd_reduce_kernel(BwdArgs a) {
   int d[C];
   d[0] = 4 * c4;
   if constexpr (kRope) d[C - 1] = 4 * c4 + kD / 2;
+  if constexpr (kWin) {
+    if (t >= a.cu[a.n_seqs]) {
+      for (int c = 0; c < C; ++c) {
+        *reinterpret_cast<uint2*>(dk + d[c]) = make_uint2(0u, 0u);
+        *reinterpret_cast<uint2*>(dv + d[c]) = make_uint2(0u, 0u);
+        for (int g = 0; g < a.group; ++g)
+          *reinterpret_cast<uint2*>(a.dq + t * a.dq_tok + (kvh * a.group + g) * a.dq_head + d[c]) =
+              make_uint2(0u, 0u);
+      }
+      return;
+    }
+  }
   float kk[C][4], vv[C][4];
   sum_heads4<C>(a, kvh, t, d, kk, vv);
   float(&k1)[4] = kk[0];
@@ -1243,11 +1467,11 @@ __global__ __launch_bounds__(256) void attn_bwd_reduce_kernel(BwdArgs a) {
     float(&k2)[4] = kk[C - 1];
     float(&v2)[4] = vv[C - 1];
     rope_back4(k1, k2, a.cos + t * a.cs_tok, a.sin + t * a.cs_tok, 4 * c4);
-    *reinterpret_cast<uint2*>(dk + 4 * c4 + kD / 2) = make_uint2(pack2(k2[0], k2[1]), pack2(k2[2], k2[3]));
-    *reinterpret_cast<uint2*>(dv + 4 * c4 + kD / 2) = make_uint2(pack2(v2[0], v2[1]), pack2(v2[2], v2[3]));
+    *reinterpret_cast<uint2*>(dk + 4 * c4 + kD / 2) = make_uint2(E::pack(k2[0], k2[1]), E::pack(k2[2], k2[3]));
+    *reinterpret_cast<uint2*>(dv + 4 * c4 + kD / 2) = make_uint2(E::pack(v2[0], v2[1]), E::pack(v2[2], v2[3]));
   }
-  *reinterpret_cast<uint2*>(dk + 4 * c4) = make_uint2(pack2(k1[0], k1[1]), pack2(k1[2], k1[3]));
-  *reinterpret_cast<uint2*>(dv + 4 * c4) = make_uint2(pack2(v1[0], v1[1]), pack2(v1[2], v1[3]));
+  *reinterpret_cast<uint2*>(dk + 4 * c4) = make_uint2(E::pack(k1[0], k1[1]), E::pack(k1[2], k1[3]));
+  *reinterpret_cast<uint2*>(dv + 4 * c4) = make_uint2(E::pack(v1[0], v1[1]), E::pack(v1[2], v1[3]));
 }
 
 }  // namespace
@@ -1255,30 +1479,61 @@ __global__ __launch_bounds__(256) void attn_bwd_reduce_kernel(BwdArgs a) {
 
 using namespace talm;
 
-TALM_API int talm_attn_fwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
-                           const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
-                           const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
-                           const int32_t* cu_seqlens, int32_t n_seqs, int32_t max_seqlen,
-                           int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
-                           int32_t head_dim, float scale, uint16_t* out, int64_t o_stride_tok,
-                           int64_t o_stride_head, float* lse, void* stream) {
+namespace talm {
+namespace {
+
+// The arguments of a sliding window (window = 0: none, the causal entry points).
+struct Window {
+  int32_t window, sinks, dtype;
+};
+
+int check_window(const char* what, const Window& w, float scale) {
+  if (w.dtype != TALM_F16 && w.dtype != TALM_BF16)
+    return fail(TALM_EINVAL, "%s: dtype %d (TALM_F16 or TALM_BF16)", what, w.dtype);
+  if (w.window < 1 || w.sinks < 0)
+    return fail(TALM_EINVAL, "%s: window %d (at least 1), sinks %d (at least 0)", what, w.window, w.sinks);
+  if (!(scale > 0.f) || !(scale < INFINITY))
+    return fail(TALM_EINVAL, "%s: scale %g (positive, finite)", what, static_cast<double>(scale));
+  return TALM_OK;
+}
+
+template <class E, bool kWin>
+void launch_fwd(const FwdArgs& a, int h, bool split, dim3 grid, hipStream_t s) {
+#define TALM_ATTN_FWD(H)                                                                         \
+  if (split)                                                                                     \
+    hipLaunchKernelGGL((attn_fwd_kernel<E, H, 2, kWin>), grid, dim3(512), 0, s, a);              \
+  else                                                                                           \
+    hipLaunchKernelGGL((attn_fwd_kernel<E, H, 1, kWin>), grid, dim3(256), 0, s, a)
+  if (h == 4) { TALM_ATTN_FWD(4); }
+  else if (h == 2) { TALM_ATTN_FWD(2); }
+  else { TALM_ATTN_FWD(1); }
+#undef TALM_ATTN_FWD
+}
+
+int attn_fwd_impl(const char* what, const Window& win, const uint16_t* q, int64_t q_stride_tok,
+                  int64_t q_stride_head, const uint16_t* k, int64_t k_stride_tok,
+                  int64_t k_stride_head, const uint16_t* v, int64_t v_stride_tok,
+                  int64_t v_stride_head, const int32_t* cu_seqlens, int32_t n_seqs,
+                  int32_t max_seqlen, int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                  int32_t head_dim, float scale, uint16_t* out, int64_t o_stride_tok,
+                  int64_t o_stride_head, float* lse, void* stream) {
   if (head_dim != kD)
-    return fail(TALM_EINVAL, "attn_fwd: head_dim %d (only %d)", head_dim, kD);
+    return fail(TALM_EINVAL, "%s: head_dim %d (only %d)", what, head_dim, kD);
   if (n_seqs < 0 || max_seqlen < 0 || n_tokens < 0 || n_q_heads < 1 || n_kv_heads < 1 ||
       n_q_heads % n_kv_heads || n_tokens >= (int64_t{1} << 31))
-    return fail(TALM_EINVAL, "attn_fwd: bad shape (seqs %d, max_seqlen %d, tokens %lld, heads %d/%d)",
+    return fail(TALM_EINVAL, "%s: bad shape (seqs %d, max_seqlen %d, tokens %lld, heads %d/%d)", what,
                 n_seqs, max_seqlen, (long long)n_tokens, n_q_heads, n_kv_heads);
   for (int64_t s : {q_stride_tok, q_stride_head, k_stride_tok, k_stride_head, v_stride_tok,
                     v_stride_head, o_stride_tok, o_stride_head})
     if (s < 0 || s % 8)
-      return fail(TALM_EINVAL, "attn_fwd: strides must be non-negative multiples of 8 elements");
+      return fail(TALM_EINVAL, "%s: strides must be non-negative multiples of 8 elements", what);
   if (k_stride_tok >= (int64_t{1} << 23) || v_stride_tok >= (int64_t{1} << 23) ||
       o_stride_tok >= (int64_t{1} << 23))
-    return fail(TALM_EINVAL, "attn_fwd: k / v / out token strides must be below 2^23 elements");
+    return fail(TALM_EINVAL, "%s: k / v / out token strides must be below 2^23 elements", what);
   if (n_seqs == 0 || max_seqlen == 0 || n_tokens == 0) return ok();
-  if (!q || !k || !v || !cu_seqlens || !out || !lse) return fail(TALM_EINVAL, "attn_fwd: null pointer");
+  if (!q || !k || !v || !cu_seqlens || !out || !lse) return fail(TALM_EINVAL, "%s: null pointer", what);
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16))
-    return fail(TALM_EINVAL, "attn_fwd: q, k, v and out must be 16-byte aligned");
+    return fail(TALM_EINVAL, "%s: q, k, v and out must be 16-byte aligned", what);
   const int group = n_q_heads / n_kv_heads;
   // query heads per workgroup (4 wavefronts): 4, 2 or 1, what divides the group; three with an idle
   // wavefront where a group is a multiple of three and no sequence has more than 64 rows, of which
@@ -1309,7 +1564,16 @@ TALM_API int talm_attn_fwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_st
   // 32.7 us, [4096] 79.7 / 66.8, [900, 700, 333] 21.0 / 18.5; [300, 211] 9.3 / 9.9; 8 rows of
   // 128..512 15.2 / 17.7, 8 of 1024 39.4 / 47.1, [4096, 3001, 2222, 1531] 132 / 139.
   const int64_t wgs = (n_tokens + static_cast<int64_t>(n_seqs) * rows / 2) / rows * chunks;
-  const int64_t cus = device_cus(), chain = (static_cast<int64_t>(max_seqlen) + kKeys - 1) / kKeys;
+  const int64_t cus = device_cus();
+  int64_t chain = (static_cast<int64_t>(max_seqlen) + kKeys - 1) / kKeys;
+  if (win.window) {
+    a.window = std::min(win.window, max_seqlen);
+    a.sinks = std::min(win.sinks, max_seqlen);
+    // a window of any alignment behind the workgroup's rows, and the sinks' tiles
+    const int64_t seen = (static_cast<int64_t>(a.window) + rows + kKeys - 2) / kKeys + 1 +
+                         (a.sinks + kKeys - 1) / kKeys;
+    chain = std::min(chain, seen);
+  }
   const bool split = wgs <= cus ? chain >= 8 : wgs <= 2 * cus && chain >= 16;
   // Workgroups by list_pair's list, longest first over all sequences, where they exceed a round (two
   // per CU) and the sequences differ in length (an eighth of the rectangle empty): round-robin over
@@ -1325,16 +1589,43 @@ TALM_API int talm_attn_fwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_st
     grid = dim3(static_cast<unsigned>(items));
   }
   const hipStream_t s = as_stream(stream);
-#define TALM_ATTN_FWD(H)                                                                         \
-  if (split)                                                                                     \
-    hipLaunchKernelGGL((attn_fwd_kernel<H, 2>), grid, dim3(512), 0, s, a);                       \
-  else                                                                                           \
-    hipLaunchKernelGGL((attn_fwd_kernel<H, 1>), grid, dim3(256), 0, s, a)
-  if (h == 4) { TALM_ATTN_FWD(4); }
-  else if (h == 2) { TALM_ATTN_FWD(2); }
-  else { TALM_ATTN_FWD(1); }
-#undef TALM_ATTN_FWD
-  return check_launch("attn_fwd");
+  if (!win.window) launch_fwd<F16, false>(a, h, split, grid, s);
+  else if (win.dtype == TALM_F16) launch_fwd<F16, true>(a, h, split, grid, s);
+  else launch_fwd<BF16, true>(a, h, split, grid, s);
+  return check_launch(what);
+}
+
+}  // namespace
+}  // namespace talm
+
+TALM_API int talm_attn_fwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                           const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                           const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
+                           const int32_t* cu_seqlens, int32_t n_seqs, int32_t max_seqlen,
+                           int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                           int32_t head_dim, float scale, uint16_t* out, int64_t o_stride_tok,
+                           int64_t o_stride_head, float* lse, void* stream) {
+  return attn_fwd_impl("attn_fwd", Window{0, 0, TALM_F16}, q, q_stride_tok, q_stride_head, k,
+                       k_stride_tok, k_stride_head, v, v_stride_tok, v_stride_head, cu_seqlens,
+                       n_seqs, max_seqlen, n_tokens, n_q_heads, n_kv_heads, head_dim, scale, out,
+                       o_stride_tok, o_stride_head, lse, stream);
+}
+
+TALM_API int talm_attn_window_fwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                                  const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                                  const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
+                                  const int32_t* cu_seqlens, int32_t n_seqs, int32_t max_seqlen,
+                                  int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                                  int32_t head_dim, float scale, int32_t window, int32_t sinks,
+                                  int32_t dtype, uint16_t* out, int64_t o_stride_tok,
+                                  int64_t o_stride_head, float* lse, void* stream) {
+  const Window win{window, sinks, dtype};
+  const int status = check_window("attn_window_fwd", win, scale);
+  if (status != TALM_OK) return status;
+  return attn_fwd_impl("attn_window_fwd", win, q, q_stride_tok, q_stride_head, k, k_stride_tok,
+                       k_stride_head, v, v_stride_tok, v_stride_head, cu_seqlens, n_seqs,
+                       max_seqlen, n_tokens, n_q_heads, n_kv_heads, head_dim, scale, out,
+                       o_stride_tok, o_stride_head, lse, stream);
 }
 
 static constexpr int64_t kQueueBytes = 256;  // the work queue's counter, at the workspace's end
@@ -1350,7 +1641,53 @@ TALM_API int64_t talm_attn_bwd_workspace(int64_t n_tokens, int32_t n_q_heads) {
 namespace talm {
 namespace {
 
-int attn_bwd_impl(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+// How the sinks' rows past their windows are cut: items of at least a window and kFarRows rows, so that
+// none is much longer than a tile's other rows, but few enough that their partials stay within
+// kFarBytes.
+constexpr int64_t kFarRows = 512, kFarBytes = int64_t{64} << 20;
+struct FarPlan {
+  int64_t rows = 64, chunks = 0, tiles = 0, floats = 0;  // floats: of far_k, and again of far_v
+};
+FarPlan far_plan(int64_t n_seqs, int64_t max_seqlen, int64_t n_q_heads, int64_t window, int64_t sinks) {
+  FarPlan f;
+  window = std::min(window, max_seqlen);
+  sinks = std::min(sinks, max_seqlen);
+  const int64_t left = max_seqlen - (127 + window + 63) / 64 * 64;  // of the first key tile
+  if (sinks == 0 || left <= 0 || n_seqs == 0) return f;
+  const int64_t one = n_seqs * n_q_heads * sinks * kD;
+  const int64_t most = std::max<int64_t>(1, kFarBytes / (8 * one));
+  f.rows = std::max(kFarRows, (window + 63) / 64 * 64);
+  f.chunks = std::min((left + f.rows - 1) / f.rows, most);
+  f.rows = std::max(f.rows, ((left + f.chunks - 1) / f.chunks + 63) / 64 * 64);
+  f.tiles = (sinks + 127) / 128;
+  f.floats = one * f.chunks;
+  return f;
+}
+
+template <class E, bool kWin>
+void launch_bwd(const BwdArgs& a, int n_seqs, hipStream_t s) {
+  constexpr int W = 4;
+  const int64_t rows = a.n_tokens * a.n_q_heads;
+  hipLaunchKernelGGL(attn_bwd_dot_kernel<E>, dim3(static_cast<unsigned>((rows * 16 + 255) / 256)),
+                     dim3(256), 0, s, a);
+  if (a.counter) {
+    hipLaunchKernelGGL((attn_bwd_queue_kernel<E, W, kWin>), dim3(a.queue_wgs), dim3(64 * W), 0, s, a);
+  } else {
+    const dim3 grid(static_cast<unsigned>(a.n_q_heads), static_cast<unsigned>(n_seqs),
+                    static_cast<unsigned>(2 * a.n_tiles + a.far_chunks * a.far_tiles));
+    hipLaunchKernelGGL((attn_bwd_kernel<E, W, kWin>), grid, dim3(64 * W), 0, s, a);
+  }
+  if (a.far_items) {
+    const int64_t n = static_cast<int64_t>(n_seqs) * a.n_q_heads * a.sinks * (kD / 4);
+    hipLaunchKernelGGL(attn_bwd_far_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s, a);
+  }
+  const int64_t red = a.n_tokens * a.n_kv_heads * (a.cos ? kD / 8 : kD / 4);
+  const dim3 grid(static_cast<unsigned>((red + 255) / 256));
+  if (a.cos) hipLaunchKernelGGL((attn_bwd_reduce_kernel<E, true, kWin>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((attn_bwd_reduce_kernel<E, false, kWin>), grid, dim3(256), 0, s, a);
+}
+
+int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
                   const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
                   const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
                   const uint16_t* out, int64_t o_stride_tok, int64_t o_stride_head,
@@ -1364,41 +1701,46 @@ int attn_bwd_impl(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head
                   int64_t dv_stride_head, void* workspace, int64_t workspace_bytes,
                   void* stream) {
   if (head_dim != kD)
-    return fail(TALM_EINVAL, "attn_bwd: head_dim %d (only %d)", head_dim, kD);
+    return fail(TALM_EINVAL, "%s: head_dim %d (only %d)", what, head_dim, kD);
   if (n_seqs < 0 || max_seqlen < 0 || n_tokens < 0 || n_q_heads < 1 || n_kv_heads < 1 ||
       n_q_heads % n_kv_heads || n_tokens >= (int64_t{1} << 31))
-    return fail(TALM_EINVAL, "attn_bwd: bad shape (seqs %d, max_seqlen %d, tokens %lld, heads %d/%d)",
+    return fail(TALM_EINVAL, "%s: bad shape (seqs %d, max_seqlen %d, tokens %lld, heads %d/%d)", what,
                 n_seqs, max_seqlen, (long long)n_tokens, n_q_heads, n_kv_heads);
   for (int64_t s : {q_stride_tok, q_stride_head, k_stride_tok, k_stride_head, v_stride_tok,
                     v_stride_head, o_stride_tok, o_stride_head, do_stride_tok, do_stride_head,
                     dq_stride_tok, dq_stride_head, dk_stride_tok, dk_stride_head, dv_stride_tok,
                     dv_stride_head})
     if (s < 0 || s % 8)
-      return fail(TALM_EINVAL, "attn_bwd: strides must be non-negative multiples of 8 elements");
+      return fail(TALM_EINVAL, "%s: strides must be non-negative multiples of 8 elements", what);
   if (q_stride_tok >= (int64_t{1} << 23) || k_stride_tok >= (int64_t{1} << 23) ||
       v_stride_tok >= (int64_t{1} << 23) || do_stride_tok >= (int64_t{1} << 23) ||
       dq_stride_tok >= (int64_t{1} << 23))
-    return fail(TALM_EINVAL, "attn_bwd: q / k / v / dout / dq token strides must be below 2^23 elements");
+    return fail(TALM_EINVAL, "%s: q / k / v / dout / dq token strides must be below 2^23 elements", what);
   if (n_seqs > 65535 || (max_seqlen + 127) / 128 > 32767)
-    return fail(TALM_EINVAL, "attn_bwd: at most 65535 sequences of at most 4194176 tokens");
+    return fail(TALM_EINVAL, "%s: at most 65535 sequences of at most 4194176 tokens", what);
   // (a workspace without the queue's counter is accepted: one workgroup per item then)
-  const int64_t need = talm_attn_bwd_workspace(n_tokens, n_q_heads) - kQueueBytes;
+  const FarPlan far = win.window ? far_plan(n_seqs, max_seqlen, n_q_heads, win.window, win.sinks) : FarPlan{};
+  const int64_t need = talm_attn_bwd_workspace(n_tokens, n_q_heads) - kQueueBytes + 8 * far.floats;
+  if (far.chunks * far.tiles + 2 * ((max_seqlen + 127) / 128) > 65535 ||
+      n_seqs * far.chunks * far.tiles * n_q_heads >= (int64_t{1} << 30) ||
+      n_seqs * static_cast<int64_t>(n_q_heads) * std::min(win.sinks, max_seqlen) >= (int64_t{1} << 31))
+    return fail(TALM_EINVAL, "%s: %d sinks of %d sequences are too many", what, win.sinks, n_seqs);
   if (workspace_bytes < need)
-    return fail(TALM_EINVAL, "attn_bwd: workspace of %lld bytes, %lld needed",
+    return fail(TALM_EINVAL, "%s: workspace of %lld bytes, %lld needed", what,
                 (long long)workspace_bytes, (long long)need);
   const bool rope = cos != nullptr || sin != nullptr;
   if (rope && (cs_stride < kD || cs_stride % 4 || cs_stride >= (int64_t{1} << 24)))
-    return fail(TALM_EINVAL, "attn_bwd: cos / sin row stride %lld (at least %d, a multiple of 4)",
+    return fail(TALM_EINVAL, "%s: cos / sin row stride %lld (at least %d, a multiple of 4)", what,
                 (long long)cs_stride, kD);
   if (n_seqs == 0 || max_seqlen == 0 || n_tokens == 0) return ok();
   if (!q || !k || !v || !out || !dout || !lse || !cu_seqlens || !dq || !dk || !dv || !workspace)
-    return fail(TALM_EINVAL, "attn_bwd: null pointer");
+    return fail(TALM_EINVAL, "%s: null pointer", what);
   if (rope && (!cos || !sin || !aligned(cos, 16) || !aligned(sin, 16)))
-    return fail(TALM_EINVAL, "attn_bwd: cos and sin both given, 16-byte aligned");
+    return fail(TALM_EINVAL, "%s: cos and sin both given, 16-byte aligned", what);
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) ||
       !aligned(dout, 16) || !aligned(dq, 16) || !aligned(dk, 8) || !aligned(dv, 8) ||
       !aligned(workspace, 256))
-    return fail(TALM_EINVAL, "attn_bwd: operands 16-byte aligned (dk, dv 8), workspace 256");
+    return fail(TALM_EINVAL, "%s: operands 16-byte aligned (dk, dv 8), workspace 256", what);
   constexpr int W = 4;
   BwdArgs a{};
   a.q = q; a.q_tok = q_stride_tok; a.q_head = q_stride_head;
@@ -1420,6 +1762,16 @@ int attn_bwd_impl(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head
   a.dq = dq; a.dq_tok = dq_stride_tok; a.dq_head = dq_stride_head;
   a.dk = dk; a.dk_tok = dk_stride_tok; a.dk_head = dk_stride_head;
   a.dv = dv; a.dv_tok = dv_stride_tok; a.dv_head = dv_stride_head;
+  if (win.window) {
+    a.window = std::min(win.window, max_seqlen);
+    a.sinks = std::min(win.sinks, max_seqlen);
+    a.far_rows = static_cast<int>(far.rows);
+    a.far_chunks = static_cast<int>(far.chunks);
+    a.far_tiles = static_cast<int>(far.tiles);
+    a.far_items = static_cast<unsigned>(n_seqs * far.chunks * far.tiles * n_q_heads);
+    a.far_k = a.dv_part + n_tokens * n_q_heads * kD;
+    a.far_v = a.far_k + far.floats;
+  }
   a.cos = rope ? cos : nullptr; a.sin = rope ? sin : nullptr; a.cs_tok = cs_stride;
   // The queue for more than two items per CU (what there is to balance), up to one sequence per lane,
   // where its indices fit 32 bits, and unless the items are all short (one tile per sequence, at most
@@ -1429,34 +1781,20 @@ int attn_bwd_impl(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head
   // tile per sequence, 64 sequences of 33, 64, 96 and 128 tokens with 12 / 2 heads (1536): 46.3 / 52.8,
   // 60.2 / 61.3, 86.2 / 82.6, 105 / 94; 24 sequences, 16 / 16 heads (768): 31.9 / 35.0, 37.5 / 40.6,
   // 51.3 / 53.8, 60.5 / 60.6.
-  const int64_t items = 2 * static_cast<int64_t>(n_q_heads) *
+  const int64_t items = a.far_items + 2 * static_cast<int64_t>(n_q_heads) *
                         std::min<int64_t>(n_tokens / (32 * W) + n_seqs, static_cast<int64_t>(n_seqs) * a.n_tiles);
   a.n_seqs = n_seqs;
   if (n_seqs <= kListSeqs && items > 2 * device_cus() &&
       (a.n_tiles > 1 || n_tokens > 96 * static_cast<int64_t>(n_seqs)) && items < (int64_t{1} << 30) &&
       workspace_bytes >= need + kQueueBytes) {
-    a.counter = reinterpret_cast<unsigned*>(a.dv_part + n_tokens * n_q_heads * kD);
+    a.counter = reinterpret_cast<unsigned*>(a.dv_part + n_tokens * n_q_heads * kD + 2 * far.floats);
     a.queue_wgs = static_cast<unsigned>(std::min<int64_t>(items, device_cus()));
   }
   const hipStream_t s = as_stream(stream);
-  const int64_t rows = n_tokens * n_q_heads;
-  hipLaunchKernelGGL(attn_bwd_dot_kernel, dim3(static_cast<unsigned>((rows * 16 + 255) / 256)),
-                     dim3(256), 0, s, a);
-  if (a.counter) {
-    hipLaunchKernelGGL((attn_bwd_queue_kernel<W>), dim3(a.queue_wgs), dim3(64 * W), 0, s, a);
-  } else {
-    const dim3 grid(static_cast<unsigned>(n_q_heads), static_cast<unsigned>(n_seqs),
-                    static_cast<unsigned>(2 * a.n_tiles));
-    hipLaunchKernelGGL((attn_bwd_kernel<W>), grid, dim3(64 * W), 0, s, a);
-  }
-  const int64_t red = n_tokens * n_kv_heads * (rope ? kD / 8 : kD / 4);
-  if (rope)
-    hipLaunchKernelGGL(attn_bwd_reduce_kernel<true>, dim3(static_cast<unsigned>((red + 255) / 256)),
-                       dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL(attn_bwd_reduce_kernel<false>, dim3(static_cast<unsigned>((red + 255) / 256)),
-                       dim3(256), 0, s, a);
-  return check_launch("attn_bwd");
+  if (!win.window) launch_bwd<F16, false>(a, n_seqs, s);
+  else if (win.dtype == TALM_F16) launch_bwd<F16, true>(a, n_seqs, s);
+  else launch_bwd<BF16, true>(a, n_seqs, s);
+  return check_launch(what);
 }
 
 }  // namespace
@@ -1474,7 +1812,8 @@ TALM_API int talm_attn_bwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_st
                            int64_t dk_stride_tok, int64_t dk_stride_head, uint16_t* dv,
                            int64_t dv_stride_tok, int64_t dv_stride_head, void* workspace,
                            int64_t workspace_bytes, void* stream) {
-  return attn_bwd_impl(q, q_stride_tok, q_stride_head, k, k_stride_tok, k_stride_head, v,
+  return attn_bwd_impl("attn_bwd", Window{0, 0, TALM_F16}, q, q_stride_tok, q_stride_head, k,
+                       k_stride_tok, k_stride_head, v,
                        v_stride_tok, v_stride_head, out, o_stride_tok, o_stride_head, dout,
                        do_stride_tok, do_stride_head, lse, cu_seqlens, n_seqs, max_seqlen,
                        n_tokens, n_q_heads, n_kv_heads, head_dim, scale, nullptr, nullptr, 0, dq,
@@ -1497,10 +1836,45 @@ TALM_API int talm_attn_bwd_rope(const uint16_t* q, int64_t q_stride_tok, int64_t
                                 int64_t dv_stride_head, void* workspace, int64_t workspace_bytes,
                                 void* stream) {
   if (!cos || !sin) return fail(TALM_EINVAL, "attn_bwd_rope: cos and sin are required");
-  return attn_bwd_impl(q, q_stride_tok, q_stride_head, k, k_stride_tok, k_stride_head, v,
+  return attn_bwd_impl("attn_bwd", Window{0, 0, TALM_F16}, q, q_stride_tok, q_stride_head, k,
+                       k_stride_tok, k_stride_head, v,
                        v_stride_tok, v_stride_head, out, o_stride_tok, o_stride_head, dout,
                        do_stride_tok, do_stride_head, lse, cu_seqlens, n_seqs, max_seqlen,
                        n_tokens, n_q_heads, n_kv_heads, head_dim, scale, cos, sin, cs_stride, dq,
                        dq_stride_tok, dq_stride_head, dk, dk_stride_tok, dk_stride_head, dv,
                        dv_stride_tok, dv_stride_head, workspace, workspace_bytes, stream);
+}
+
+TALM_API int64_t talm_attn_window_bwd_workspace(int64_t n_tokens, int32_t n_q_heads, int32_t n_seqs,
+                                                int32_t max_seqlen, int32_t window, int32_t sinks) {
+  if (n_tokens < 0 || n_q_heads < 1 || n_seqs < 0 || max_seqlen < 0 || window < 1 || sinks < 0) return -1;
+  return talm_attn_bwd_workspace(n_tokens, n_q_heads) +
+         8 * far_plan(n_seqs, max_seqlen, n_q_heads, window, sinks).floats;
+}
+
+TALM_API int talm_attn_window_bwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                                  const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                                  const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
+                                  const uint16_t* out, int64_t o_stride_tok, int64_t o_stride_head,
+                                  const uint16_t* dout, int64_t do_stride_tok,
+                                  int64_t do_stride_head, const float* lse,
+                                  const int32_t* cu_seqlens, int32_t n_seqs, int32_t max_seqlen,
+                                  int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                                  int32_t head_dim, float scale, int32_t window, int32_t sinks,
+                                  int32_t dtype, const float* cos, const float* sin,
+                                  int64_t cs_stride, uint16_t* dq, int64_t dq_stride_tok,
+                                  int64_t dq_stride_head, uint16_t* dk, int64_t dk_stride_tok,
+                                  int64_t dk_stride_head, uint16_t* dv, int64_t dv_stride_tok,
+                                  int64_t dv_stride_head, void* workspace, int64_t workspace_bytes,
+                                  void* stream) {
+  const Window win{window, sinks, dtype};
+  const int status = check_window("attn_window_bwd", win, scale);
+  if (status != TALM_OK) return status;
+  return attn_bwd_impl("attn_window_bwd", win, q, q_stride_tok, q_stride_head, k, k_stride_tok,
+                       k_stride_head, v, v_stride_tok, v_stride_head, out, o_stride_tok,
+                       o_stride_head, dout, do_stride_tok, do_stride_head, lse, cu_seqlens, n_seqs,
+                       max_seqlen, n_tokens, n_q_heads, n_kv_heads, head_dim, scale, cos, sin,
+                       cs_stride, dq, dq_stride_tok, dq_stride_head, dk, dk_stride_tok,
+                       dk_stride_head, dv, dv_stride_tok, dv_stride_head, workspace,
+                       workspace_bytes, stream);
 }

@@ -1,0 +1,634 @@
+// Dropout and the LoRA adapters' products with dropout on their input, for gfx950. No mask is
+// stored: every kernel computes it from the generator (philox.h).
+//
+//   dropout        y = keep x factor                       (the gradient: the same on dy)
+//   lora_down_drop t = factor (keep x) A^T, ts = s t       (rank 16; 1 or 2 adapters of one x, each
+//                                                           with a mask of its own)
+//   lora_up        out = base + sum_g factor keep_g (u_g M_g)   (y = ts B^T: no mask; the input
+//                                                           gradient u A under the masks)
+//   lora_wgrad_drop dA_g = factor u_g^T (keep_g x), dB_g = s_g dy_g^T t_g
+// The adapters' arithmetic is PEFT's (solution/lora.py:183-231, solution/fused_proj.py:139-153,
+// :199-215) with x / (1 - p) not rounded on the way: the mask clears fp16 operands exactly and the
+// factor goes on the fp32 sums.
+#include "mfma_tile.h"
+#include "philox.h"
+
+#include <algorithm>
+
+namespace talm {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t half4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kRank = 16;
+constexpr int kMaxAdapters = 2;
+
+__device__ __forceinline__ half8_t h8(uint4 v) { return __builtin_bit_cast(half8_t, v); }
+
+// ------------------------------------------------------------------------------------------
+// Elementwise
+// ------------------------------------------------------------------------------------------
+struct F16Elem {
+  static __device__ __forceinline__ float get(uint16_t v) { return h2f(v); }
+  static __device__ __forceinline__ uint16_t put(float v) { return f2h(v); }
+  typedef uint16_t type;
+};
+struct BF16Elem {
+  static __device__ __forceinline__ float get(uint16_t v) {
+    return __builtin_bit_cast(float, static_cast<uint32_t>(v) << 16);
+  }
+  static __device__ __forceinline__ uint16_t put(float v) {
+    return __builtin_bit_cast(uint16_t, static_cast<__bf16>(v));
+  }
+  typedef uint16_t type;
+};
+struct F32Elem {
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ float put(float v) { return v; }
+  typedef float type;
+};
+
+// One thread per eight columns of a row. kVec: whole chunks, 16-byte aligned rows.
+template <class E, bool kVec>
+__global__ __launch_bounds__(256) void dropout_kernel(const typename E::type* __restrict__ x, int64_t ldx,
+                                                      int64_t rows, int64_t cols, float factor,
+                                                      DropArgs drop, typename E::type* __restrict__ y,
+                                                      int64_t ldy) {
+  typedef typename E::type T;
+  const int64_t per_row = (cols + 7) / 8;
+  const int64_t block = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (block >= rows * per_row) return;
+  const int64_t r = block / per_row, c = (block - r * per_row) * 8;
+  const T* xp = x + r * ldx + c;
+  T* yp = y + r * ldy + c;
+  const int n = kVec ? 8 : static_cast<int>(min(cols - c, static_cast<int64_t>(8)));
+  T v[8];
+  if constexpr (kVec) {
+    *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(xp);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(v + 4) = *reinterpret_cast<const uint4*>(xp + 4);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? xp[e] : T(0);
+  }
+  const DropKey key(drop.key, drop.site, drop.threshold);
+  const uint4 bits = philox_block(static_cast<uint64_t>(block), key);
+  const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t u = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
+    v[e] = u >= key.threshold ? E::put(E::get(v[e]) * factor) : T(0);
+  }
+  if constexpr (kVec) {
+    *reinterpret_cast<uint4*>(yp) = *reinterpret_cast<const uint4*>(v);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(yp + 4) = *reinterpret_cast<const uint4*>(v + 4);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) yp[e] = v[e];
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// t = factor (keep x) A^T
+// ------------------------------------------------------------------------------------------
+struct DownArgs {
+  const uint16_t* x;  // [N][ldx]
+  int64_t ldx;
+  int n_tokens, k, n_adapters, parts;
+  const uint16_t* a[kMaxAdapters];  // [16][k]
+  float scaling[kMaxAdapters];
+  float factor;
+  DropArgs drop;                // adapter g's site: drop.site + site_step g
+  uint32_t site[kMaxAdapters];
+  uint16_t* t;                  // [N][ldt], 16 columns per adapter
+  uint16_t* ts;
+  int64_t ldt;
+  float* part;                  // [parts][N][16 n_adapters] when parts > 1
+};
+
+constexpr int kDownWaves = 8;
+constexpr int kDownBatch = 4;
+
+// One workgroup per 16 tokens and part of the reduction; its wavefronts take the part's 32-deep
+// steps round-robin, the loads of kDownBatch of them before their MFMAs.
+template <int G>
+__global__ __launch_bounds__(64 * kDownWaves) void lora_down_drop_kernel(DownArgs a) {
+  __shared__ float red[kDownWaves][G][16][16 + 1];
+  const int m0 = blockIdx.x * 16;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = lane & 15, kq = 8 * (lane >> 4);
+  const int steps = a.k >> 5, per = (steps + a.parts - 1) / a.parts;
+  const int s_lo = blockIdx.y * per, s_hi = min(steps, s_lo + per);
+  const __amdgpu_buffer_rsrc_t rx = buffer_rsrc(a.x + static_cast<int64_t>(m0) * a.ldx);
+  const uint32_t xoff = m0 + row < a.n_tokens ? static_cast<uint32_t>((row * a.ldx + kq) * 2) : kOob;
+  const uint32_t aoff = static_cast<uint32_t>((row * a.k + kq) * 2);
+  const uint64_t block0 = static_cast<uint64_t>(m0 + row) * (a.k >> 3) + (kq >> 3);
+  f32x4 acc[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) acc[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const DropKey key(a.drop.key, 0, a.drop.threshold);
+  for (int base = s_lo + wave; base < s_hi; base += kDownWaves * kDownBatch) {
+    uint4 xv[kDownBatch], av[kDownBatch][G];
+#pragma unroll
+    for (int j = 0; j < kDownBatch; ++j) {
+      const int c = base + kDownWaves * j;
+      const bool live = c < s_hi;
+      const uint32_t kb = static_cast<uint32_t>(c) * 64;
+      xv[j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rx, live ? xoff + kb : kOob, 0, 0));
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        av[j][g] = __builtin_bit_cast(
+            uint4, __builtin_amdgcn_raw_buffer_load_b128(buffer_rsrc(a.a[g]), live ? aoff + kb : kOob, 0, 0));
+    }
+#pragma unroll
+    for (int j = 0; j < kDownBatch; ++j) {
+      if (base + kDownWaves * j >= s_hi) break;
+      const uint64_t block = block0 + static_cast<uint64_t>(base + kDownWaves * j) * 4;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        DropKey kg = key;
+        kg.site = a.site[g];
+        const uint4 xd = key.threshold ? keep8(xv[j], block, kg) : xv[j];
+        acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8(xd), h8(av[j][g]), acc[g], 0, 0, 0);
+      }
+    }
+  }
+  // accumulator element v of lane l: token 4 (l / 16) + v, rank l % 16
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) red[wave][g][4 * (lane >> 4) + v][lane & 15] = acc[g][v];
+  __syncthreads();
+  for (int e = threadIdx.x; e < G * 256; e += 64 * kDownWaves) {
+    const int g = e >> 8, r = (e >> 4) & 15, i = e & 15;
+    if (m0 + r >= a.n_tokens) continue;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDownWaves; ++w) sum += red[w][g][r][i];
+    if (a.parts > 1) {
+      a.part[(static_cast<int64_t>(blockIdx.y) * a.n_tokens + m0 + r) * (kRank * G) + g * kRank + i] = sum;
+    } else {
+      const int64_t at = static_cast<int64_t>(m0 + r) * a.ldt + g * kRank + i;
+      a.t[at] = f2h(a.factor * sum);
+      a.ts[at] = f2h(a.scaling[g] * (a.factor * sum));
+    }
+  }
+}
+
+// The parts of a split reduction summed in order.
+__global__ __launch_bounds__(256) void lora_down_sum_kernel(DownArgs a) {
+  const int width = kRank * a.n_adapters;
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (e >= static_cast<int64_t>(a.n_tokens) * width) return;
+  const int64_t n = e / width;
+  const int i = static_cast<int>(e - n * width);
+  float sum = 0.f;
+  for (int p = 0; p < a.parts; ++p) sum += a.part[static_cast<int64_t>(p) * a.n_tokens * width + e];
+  a.t[n * a.ldt + i] = f2h(a.factor * sum);
+  a.ts[n * a.ldt + i] = f2h(a.scaling[i / kRank] * (a.factor * sum));
+}
+
+// ------------------------------------------------------------------------------------------
+// out = base + sum_g factor keep_g (u_g M_g)
+// ------------------------------------------------------------------------------------------
+struct UpArgs {
+  const uint16_t* u;  // [N][ldu], 16 columns per adapter
+  int64_t ldu;
+  int n_tokens, cols, n_adapters, m_kmajor;
+  const uint16_t* m[kMaxAdapters];  // [cols][16], or with m_kmajor [16][cols]
+  float factor;
+  DropArgs drop;
+  uint32_t site[kMaxAdapters];
+  const uint16_t* base;  // [N][ldb] or null
+  int64_t ldb;
+  uint16_t* out;         // [N][ldo]; may be base
+  int64_t ldo;
+};
+
+constexpr int kUpTokens = 64;  // per workgroup, in blocks of 32
+
+// One wavefront per 32 columns. C[c][token] = M u^T (v_mfma_f32_32x32x16_f16, K = the rank): a lane
+// owns a token, and with row m of the A operand taken as column c(m) = 16 (m / 4 % 2) + 4 (m / 8) +
+// m % 4 of the block its 16 accumulators are the 16 consecutive columns 16 (lane / 32) .. + 15: two
+// blocks of the generator and two 16-byte stores.
+template <int G>
+__global__ __launch_bounds__(256) void lora_up_kernel(UpArgs a) {
+  const int lane = threadIdx.x & 63, hh = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c0 = blockIdx.x * 128 + 32 * wave;
+  if (c0 >= a.cols) return;  // no barrier follows
+  const int cm = c0 + 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);
+  uint4 mf[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    mf[g] = make_uint4(0u, 0u, 0u, 0u);
+    if (cm < a.cols) {
+      if (a.m_kmajor) {
+        uint32_t h[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = a.m[g][static_cast<int64_t>(8 * hh + e) * a.cols + cm];
+        mf[g] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+      } else {
+        mf[g] = *reinterpret_cast<const uint4*>(a.m[g] + static_cast<int64_t>(cm) * kRank + 8 * hh);
+      }
+    }
+  }
+  const DropKey key(a.drop.key, 0, a.drop.threshold);
+  const int col = c0 + 16 * hh;  // the lane's first column
+#pragma unroll
+  for (int tb = 0; tb < kUpTokens / 32; ++tb) {
+    const int tok = blockIdx.y * kUpTokens + 32 * tb + l32;
+    const bool in = tok < a.n_tokens;
+    const int tk = in ? tok : a.n_tokens - 1;
+    float sum[16];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint4 b = make_uint4(0u, 0u, 0u, 0u);
+      if (a.base && in && col + 8 * q < a.cols)
+        b = *reinterpret_cast<const uint4*>(a.base + static_cast<int64_t>(tk) * a.ldb + col + 8 * q);
+      const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sum[8 * q + 2 * e] = lo_f(w[e]);
+        sum[8 * q + 2 * e + 1] = hi_f(w[e]);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const uint4 uf = *reinterpret_cast<const uint4*>(a.u + static_cast<int64_t>(tk) * a.ldu + kRank * g + 8 * hh);
+      f32x16 acc;
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[v] = 0.f;
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(h8(mf[g]), h8(uf), acc, 0, 0, 0);
+      DropKey kg = key;
+      kg.site = a.site[g];
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint4 bits = make_uint4(0u, 0u, 0u, 0u);
+        if (key.threshold)
+          bits = philox_block(static_cast<uint64_t>(tk) * (a.cols >> 3) + ((col >> 3) + q), kg);
+        const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t r = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
+          sum[8 * q + e] += r >= key.threshold ? a.factor * acc[8 * q + e] : 0.f;
+        }
+      }
+    }
+    if (!in) continue;
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+      if (col + 8 * q < a.cols) {
+        const float* s = sum + 8 * q;
+        *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(tok) * a.ldo + col + 8 * q) =
+            make_uint4(pack2(s[0], s[1]), pack2(s[2], s[3]), pack2(s[4], s[5]), pack2(s[6], s[7]));
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------------------
+// dA_g = factor u_g^T (keep_g x), dB_g = s_g dy_g^T t_g
+// ------------------------------------------------------------------------------------------
+struct WgradArgs {
+  const uint16_t* x;
+  int64_t ldx;
+  const uint16_t* dy;
+  int64_t ldy;
+  const uint16_t* u;
+  int64_t ldu;
+  const uint16_t* t;
+  int64_t ldt;
+  int n_tokens, hidden, n_adapters;
+  int lo[kMaxAdapters], seg[kMaxAdapters];
+  float scaling[kMaxAdapters], factor;
+  DropArgs drop;
+  uint32_t site[kMaxAdapters];
+  // the reductions' columns one after the other: dA of each adapter, then dB of each, every one
+  // padded to whole workgroups of 128
+  int first[2 * kMaxAdapters + 1];
+  int cols;             // first[2 n_adapters]
+  int chunk, chunks;    // tokens per partial (a multiple of 64), partials
+  float* part;          // [chunks][cols][16]
+  int half_out;         // the gradients in fp16, else fp32
+  void* da[kMaxAdapters];
+  void* db[kMaxAdapters];
+};
+
+constexpr int kWgTok = 64;
+constexpr int kWgLd = 128 + 16;  // halves per staged row: rows 32 bytes apart in the banks
+
+// See read_tr_untracked of attn.hip: lane i of a group of 16 gets elements 0..3 = rows 0..3 of column i
+// of the 4 x 16 block whose row j / 4, columns 4 (j % 4) .. + 3 lane j points at.
+__device__ __forceinline__ half4_t read_tr(const uint16_t* p) {
+  const auto r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p));
+  return __builtin_bit_cast(half4_t, r);
+}
+__device__ __forceinline__ half8_t pair(half4_t lo, half4_t hi) {
+  return __builtin_bit_cast(half8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// One workgroup per (128 columns of one reduction, chunk of tokens): 64 tokens at a time staged row
+// by row in LDS (masked on the way), the fragments read transposed; each wavefront 32 columns against
+// the 16 of u or t (v_mfma_f32_16x16x32_f16). The next tokens' loads are in flight meanwhile.
+__global__ __launch_bounds__(256) void lora_wgrad_drop_kernel(WgradArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t xs[kWgTok][kWgLd];
+  __shared__ __attribute__((aligned(16))) uint16_t ms[kWgTok][kRank + 8];
+  const int c0 = blockIdx.x * 128, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int job = 0;
+  while (job + 1 < 2 * a.n_adapters && c0 >= a.first[job + 1]) ++job;
+  const bool is_b = job >= a.n_adapters;
+  const int g = is_b ? job - a.n_adapters : job;
+  const int cb = c0 - a.first[job];                   // first column of the reduction
+  const int width = is_b ? a.seg[g] : a.hidden;
+  const uint16_t* src = is_b ? a.dy + a.lo[g] : a.x;
+  const int64_t ld = is_b ? a.ldy : a.ldx;
+  const uint16_t* mat = (is_b ? a.t : a.u) + kRank * g;
+  const int64_t ldm = is_b ? a.ldt : a.ldu;
+  const DropKey key(a.drop.key, a.site[g], is_b ? 0u : a.drop.threshold);
+  const int r_lo = blockIdx.y * a.chunk, r_hi = min(a.n_tokens, r_lo + a.chunk);
+  // a thread's items: 16-byte chunk tid % 16 of rows tid / 16 + 16 i; of u / t threads 0..127 one chunk
+  const int cc = cb + 8 * (tid & 15);
+  const bool live = cc < width;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  uint4 xv[4], mv;
+  auto load = [&](int r0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r0 + (tid >> 4) + 16 * i;
+      xv[i] = zero;
+      if (live && r < r_hi) xv[i] = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(r) * ld + cc);
+    }
+    mv = zero;
+    const int r = r0 + (tid >> 1);
+    if (tid < 128 && r < r_hi) mv = *reinterpret_cast<const uint4*>(mat + static_cast<int64_t>(r) * ldm + 8 * (tid & 1));
+  };
+  f32x4 acc[2];
+  acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  load(r_lo);
+  const int grp = lane >> 4, j = lane & 15;
+  for (int r0 = r_lo; r0 < r_hi; r0 += kWgTok) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (tid >> 4) + 16 * i;
+      const uint4 v = key.threshold
+                          ? keep8(xv[i], static_cast<uint64_t>(r0 + r) * (a.hidden >> 3) + (cc >> 3), key)
+                          : xv[i];
+      *reinterpret_cast<uint4*>(&xs[r][8 * (tid & 15)]) = v;
+    }
+    if (tid < 128) *reinterpret_cast<uint4*>(&ms[tid >> 1][8 * (tid & 1)]) = mv;
+    __syncthreads();
+    if (r0 + kWgTok < r_hi) load(r0 + kWgTok);
+#pragma unroll
+    for (int ks = 0; ks < kWgTok / 32; ++ks) {
+      const int k0 = 32 * ks + 8 * grp + (j >> 2);  // the lane's row of the first transposed read
+      const half8_t mb = pair(read_tr(&ms[k0][4 * (j & 3)]), read_tr(&ms[k0 + 4][4 * (j & 3)]));
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int c = 32 * wave + 16 * b + 4 * (j & 3);
+        acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pair(read_tr(&xs[k0][c]), read_tr(&xs[k0 + 4][c])), mb,
+                                                       acc[b], 0, 0, 0);
+      }
+    }
+    __syncthreads();
+  }
+  float* out = a.part + (static_cast<int64_t>(blockIdx.y) * a.cols + c0 + 32 * wave) * kRank;
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int v = 0; v < 4; ++v) out[(16 * b + 4 * grp + v) * kRank + j] = acc[b][v];
+}
+
+// The chunks summed in order: one thread per (column, rank).
+__global__ __launch_bounds__(256) void lora_wgrad_sum_kernel(WgradArgs a) {
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (e >= static_cast<int64_t>(a.cols) * kRank) return;
+  const int c = static_cast<int>(e / kRank), i = static_cast<int>(e % kRank);
+  int job = 0;
+  while (job + 1 < 2 * a.n_adapters && c >= a.first[job + 1]) ++job;
+  const bool is_b = job >= a.n_adapters;
+  const int g = is_b ? job - a.n_adapters : job, cj = c - a.first[job];
+  if (cj >= (is_b ? a.seg[g] : a.hidden)) return;
+  const int64_t step = static_cast<int64_t>(a.cols) * kRank;
+  float sum = 0.f;
+  for (int k0 = 0; k0 < a.chunks; k0 += 8) {
+    float v[8];  // eight loads before their adds (selects, so that none is sunk to its add)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = a.part[min(k0 + k, a.chunks - 1) * step + e];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) sum += k0 + k < a.chunks ? v[k] : 0.f;
+  }
+  const float v = (is_b ? a.scaling[g] : a.factor) * sum;
+  const int64_t at = is_b ? static_cast<int64_t>(cj) * kRank + i : static_cast<int64_t>(i) * a.hidden + cj;
+  void* out = is_b ? a.db[g] : a.da[g];
+  if (a.half_out) static_cast<uint16_t*>(out)[at] = f2h(v);
+  else static_cast<float*>(out)[at] = v;
+}
+
+bool fits32(int64_t rows, int64_t ld) { return rows * ld * 2 < (int64_t{1} << 31); }
+
+int check_drop(const char* what, const int64_t* key, float p) {
+  if (!(p >= 0.f && p < 1.f)) return fail(TALM_EINVAL, "%s: p %g (0 <= p < 1)", what, static_cast<double>(p));
+  if (drop_threshold(p) && !key) return fail(TALM_EINVAL, "%s: p %g without a key", what, static_cast<double>(p));
+  if (!aligned(key, 8)) return fail(TALM_EINVAL, "%s: the key must be 8-byte aligned", what);
+  return TALM_OK;
+}
+
+int down_parts(int64_t n_tokens, int64_t k) {
+  (void)n_tokens;
+  (void)k;
+  return 1;
+}
+
+struct WgradPlan {
+  int64_t cols = 0, chunk = 0, chunks = 0;
+};
+WgradPlan wgrad_plan(int64_t n_tokens, int64_t hidden, int64_t n_adapters, int64_t seg0, int64_t seg1) {
+  auto pad = [](int64_t n) { return (n + 127) / 128 * 128; };
+  WgradPlan w;
+  w.cols = n_adapters * pad(hidden) + pad(seg0) + (n_adapters > 1 ? pad(seg1) : 0);
+  w.chunk = 128;
+  w.chunks = std::max<int64_t>(1, (n_tokens + w.chunk - 1) / w.chunk);
+  return w;
+}
+
+}  // namespace
+}  // namespace talm
+
+using namespace talm;
+
+TALM_API int talm_dropout(const void* x, int64_t ldx, int64_t rows, int64_t cols, int32_t dtype, float p,
+                          const int64_t* key, uint32_t site, void* y, int64_t ldy, void* stream) {
+  if (rows < 0 || cols < 0 || ldx < cols || ldy < cols ||
+      (cols > 0 && rows > (int64_t{1} << 38) / ((cols + 7) / 8)))
+    return fail(TALM_EINVAL, "dropout: bad shape (%lld x %lld, row strides %lld / %lld)", (long long)rows,
+                (long long)cols, (long long)ldx, (long long)ldy);
+  if (dtype != TALM_F32 && dtype != TALM_F16 && dtype != TALM_BF16)
+    return fail(TALM_EINVAL, "dropout: dtype %d", dtype);
+  const int status = check_drop("dropout", key, p);
+  if (status != TALM_OK) return status;
+  if (rows == 0 || cols == 0) return ok();
+  if (!x || !y) return fail(TALM_EINVAL, "dropout: null pointer");
+  const DropArgs drop{key, site, drop_threshold(p)};
+  const float factor = drop_factor(drop.threshold);
+  const int64_t n = rows * ((cols + 7) / 8);
+  const dim3 grid(static_cast<unsigned>((n + 255) / 256));
+  const int64_t unit = dtype == TALM_F32 ? 4 : 8;  // elements of 16 bytes
+  const bool vec = cols % 8 == 0 && ldx % unit == 0 && ldy % unit == 0 && aligned(x, 16) && aligned(y, 16);
+  const hipStream_t s = as_stream(stream);
+#define TALM_DROPOUT(E, V)                                                                             \
+  hipLaunchKernelGGL((dropout_kernel<E, V>), grid, dim3(256), 0, s, static_cast<const E::type*>(x), ldx, \
+                     rows, cols, factor, drop, static_cast<E::type*>(y), ldy)
+  if (dtype == TALM_F32) { if (vec) TALM_DROPOUT(F32Elem, true); else TALM_DROPOUT(F32Elem, false); }
+  else if (dtype == TALM_F16) { if (vec) TALM_DROPOUT(F16Elem, true); else TALM_DROPOUT(F16Elem, false); }
+  else { if (vec) TALM_DROPOUT(BF16Elem, true); else TALM_DROPOUT(BF16Elem, false); }
+#undef TALM_DROPOUT
+  return check_launch("dropout");
+}
+
+TALM_API int64_t talm_lora_down_drop_workspace(int64_t n_tokens, int64_t k, int32_t n_adapters) {
+  if (n_tokens < 0 || k < 32 || k % 32 || n_adapters < 1 || n_adapters > kMaxAdapters) return -1;
+  const int parts = down_parts(n_tokens, k);
+  return parts > 1 ? parts * n_tokens * kRank * n_adapters * 4 : 0;
+}
+
+TALM_API int talm_lora_down_drop(const uint16_t* x, int64_t ldx, int64_t n_tokens, int64_t k,
+                                 const uint16_t* a0, const uint16_t* a1, int32_t n_adapters, float p,
+                                 const int64_t* key, uint32_t site0, uint32_t site1, float scaling0,
+                                 float scaling1, uint16_t* t, uint16_t* ts, int64_t ldt, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  const bool two = n_adapters > 1;
+  if (n_tokens < 0 || n_tokens > (1 << 30) || n_adapters < 1 || n_adapters > kMaxAdapters || k < 32 || k % 32 ||
+      ldx < k || ldx % 8 || ldt < kRank * n_adapters || !fits32(16, ldx) || !fits32(16, k))
+    return fail(TALM_EINVAL,
+                "lora_down_drop: bad shape (tokens %lld, k %lld, ldx %lld, adapters %d, ldt %lld): k a "
+                "multiple of 32 inside x's rows of a multiple of 8, 1-2 adapters of rank 16",
+                (long long)n_tokens, (long long)k, (long long)ldx, n_adapters, (long long)ldt);
+  const int status = check_drop("lora_down_drop", key, p);
+  if (status != TALM_OK) return status;
+  if (n_tokens == 0) return ok();
+  if (!x || !a0 || (two && !a1) || !t || !ts) return fail(TALM_EINVAL, "lora_down_drop: null pointer");
+  if (!aligned(x, 16) || !aligned(a0, 16) || (two && !aligned(a1, 16)))
+    return fail(TALM_EINVAL, "lora_down_drop: x and the A matrices must be 16-byte aligned");
+  DownArgs a{};
+  a.x = x; a.ldx = ldx; a.n_tokens = static_cast<int>(n_tokens); a.k = static_cast<int>(k);
+  a.n_adapters = n_adapters; a.parts = down_parts(n_tokens, k);
+  a.a[0] = a0; a.a[1] = two ? a1 : a0;
+  a.scaling[0] = scaling0; a.scaling[1] = scaling1;
+  a.drop = DropArgs{key, 0, drop_threshold(p)};
+  a.site[0] = site0; a.site[1] = site1;
+  a.factor = drop_factor(a.drop.threshold);
+  a.t = t; a.ts = ts; a.ldt = ldt;
+  const int64_t need = talm_lora_down_drop_workspace(n_tokens, k, n_adapters);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail(TALM_EINVAL, "lora_down_drop: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
+  a.part = static_cast<float*>(workspace);
+  const dim3 grid(static_cast<unsigned>((n_tokens + 15) / 16), static_cast<unsigned>(a.parts));
+  const hipStream_t s = as_stream(stream);
+  if (two) hipLaunchKernelGGL(lora_down_drop_kernel<2>, grid, dim3(64 * kDownWaves), 0, s, a);
+  else hipLaunchKernelGGL(lora_down_drop_kernel<1>, grid, dim3(64 * kDownWaves), 0, s, a);
+  if (a.parts > 1) {
+    const int64_t n = n_tokens * kRank * n_adapters;
+    hipLaunchKernelGGL(lora_down_sum_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s, a);
+  }
+  return check_launch("lora_down_drop");
+}
+
+TALM_API int talm_lora_up(const uint16_t* u, int64_t ldu, int64_t n_tokens, int64_t cols, const uint16_t* m0,
+                          const uint16_t* m1, int32_t n_adapters, int32_t m_kmajor, float p, const int64_t* key,
+                          uint32_t site0, uint32_t site1, const uint16_t* base, int64_t ldb, uint16_t* out,
+                          int64_t ldo, void* stream) {
+  const bool two = n_adapters > 1;
+  if (n_tokens < 0 || n_tokens > kUpTokens * int64_t{65535} || n_adapters < 1 || n_adapters > kMaxAdapters || cols < 8 || cols % 8 ||
+      cols > (1 << 30) || ldu < kRank * n_adapters || ldu % 8 || ldo < cols || ldo % 8 ||
+      (base && (ldb < cols || ldb % 8)))
+    return fail(TALM_EINVAL,
+                "lora_up: bad shape (tokens %lld, columns %lld, ldu %lld, ldb %lld, ldo %lld, adapters %d): "
+                "columns and strides multiples of 8, 1-2 adapters of rank 16",
+                (long long)n_tokens, (long long)cols, (long long)ldu, (long long)ldb, (long long)ldo, n_adapters);
+  const int status = check_drop("lora_up", key, p);
+  if (status != TALM_OK) return status;
+  if (n_tokens == 0) return ok();
+  if (!u || !m0 || (two && !m1) || !out) return fail(TALM_EINVAL, "lora_up: null pointer");
+  if (!aligned(u, 16) || !aligned(out, 16) || (base && !aligned(base, 16)) ||
+      (!m_kmajor && (!aligned(m0, 16) || (two && !aligned(m1, 16)))))
+    return fail(TALM_EINVAL, "lora_up: operands must be 16-byte aligned");
+  UpArgs a{};
+  a.u = u; a.ldu = ldu; a.n_tokens = static_cast<int>(n_tokens); a.cols = static_cast<int>(cols);
+  a.n_adapters = n_adapters; a.m_kmajor = m_kmajor;
+  a.m[0] = m0; a.m[1] = two ? m1 : m0;
+  a.drop = DropArgs{key, 0, drop_threshold(p)};
+  a.site[0] = site0; a.site[1] = site1;
+  a.factor = drop_factor(a.drop.threshold);
+  a.base = base; a.ldb = ldb; a.out = out; a.ldo = ldo;
+  const dim3 grid(static_cast<unsigned>((cols + 127) / 128),
+                  static_cast<unsigned>((n_tokens + kUpTokens - 1) / kUpTokens));
+  if (two) hipLaunchKernelGGL(lora_up_kernel<2>, grid, dim3(256), 0, as_stream(stream), a);
+  else hipLaunchKernelGGL(lora_up_kernel<1>, grid, dim3(256), 0, as_stream(stream), a);
+  return check_launch("lora_up");
+}
+
+TALM_API int64_t talm_lora_wgrad_drop_workspace(int64_t n_tokens, int64_t hidden, int32_t n_adapters, int64_t seg0,
+                                                int64_t seg1) {
+  if (n_tokens < 0 || n_tokens > (1 << 30) || hidden < 8 || hidden % 8 || hidden > (1 << 26) || n_adapters < 1 ||
+      n_adapters > kMaxAdapters || seg0 < 8 || seg0 % 8 || seg0 > (1 << 26) ||
+      (n_adapters > 1 && (seg1 < 8 || seg1 % 8 || seg1 > (1 << 26))))
+    return -1;
+  const WgradPlan w = wgrad_plan(n_tokens, hidden, n_adapters, seg0, seg1);
+  return w.chunks > 65535 ? -1 : w.chunks * w.cols * kRank * 4;
+}
+
+TALM_API int talm_lora_wgrad_drop(const uint16_t* x, int64_t ldx, const uint16_t* dy, int64_t ldy,
+                                  const uint16_t* u, int64_t ldu, const uint16_t* t, int64_t ldt,
+                                  int64_t n_tokens, int64_t hidden, int32_t n_adapters, float p,
+                                  const int64_t* key, uint32_t site0, uint32_t site1, int32_t grad_dtype,
+                                  int64_t lo0, int64_t seg0, float scaling0, void* da0, void* db0,
+                                  int64_t lo1, int64_t seg1, float scaling1, void* da1, void* db1, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  const bool two = n_adapters > 1;
+  const int64_t need = talm_lora_wgrad_drop_workspace(n_tokens, hidden, n_adapters, seg0, seg1);
+  if (need < 0 || ldx < hidden || ldx % 8 || ldy % 8 || lo0 < 0 || lo0 % 8 || lo0 + seg0 > ldy ||
+      (two && (lo1 < 0 || lo1 % 8 || lo1 + seg1 > ldy)) || ldu < kRank * n_adapters || ldu % 8 ||
+      ldt < kRank * n_adapters || ldt % 8)
+    return fail(TALM_EINVAL,
+                "lora_wgrad_drop: bad shape (tokens %lld, hidden %lld, segments %lld/%lld at %lld/%lld, strides "
+                "%lld/%lld/%lld/%lld, adapters %d): sizes and strides multiples of 8, 1-2 adapters of rank 16",
+                (long long)n_tokens, (long long)hidden, (long long)seg0, (long long)seg1, (long long)lo0,
+                (long long)lo1, (long long)ldx, (long long)ldy, (long long)ldu, (long long)ldt, n_adapters);
+  if (grad_dtype != TALM_F32 && grad_dtype != TALM_F16)
+    return fail(TALM_EINVAL, "lora_wgrad_drop: gradients of dtype %d", grad_dtype);
+  const int status = check_drop("lora_wgrad_drop", key, p);
+  if (status != TALM_OK) return status;
+  if (!da0 || !db0 || (two && (!da1 || !db1))) return fail(TALM_EINVAL, "lora_wgrad_drop: null pointer");
+  if (n_tokens > 0 && (!x || !dy || !u || !t)) return fail(TALM_EINVAL, "lora_wgrad_drop: null pointer");
+  if (!aligned(x, 16) || !aligned(dy, 16) || !aligned(u, 16) || !aligned(t, 16))
+    return fail(TALM_EINVAL, "lora_wgrad_drop: operands must be 16-byte aligned");
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+    return fail(TALM_EINVAL, "lora_wgrad_drop: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
+  const WgradPlan w = wgrad_plan(n_tokens, hidden, n_adapters, seg0, seg1);
+  WgradArgs a{};
+  a.x = x; a.ldx = ldx; a.dy = dy; a.ldy = ldy; a.u = u; a.ldu = ldu; a.t = t; a.ldt = ldt;
+  a.n_tokens = static_cast<int>(n_tokens); a.hidden = static_cast<int>(hidden); a.n_adapters = n_adapters;
+  a.lo[0] = static_cast<int>(lo0); a.lo[1] = static_cast<int>(lo1);
+  a.seg[0] = static_cast<int>(seg0); a.seg[1] = static_cast<int>(seg1);
+  a.scaling[0] = scaling0; a.scaling[1] = scaling1;
+  a.drop = DropArgs{key, 0, drop_threshold(p)};
+  a.site[0] = site0; a.site[1] = site1;
+  a.factor = drop_factor(a.drop.threshold);
+  auto pad = [](int64_t n) { return static_cast<int>((n + 127) / 128 * 128); };
+  for (int job = 0; job < 2 * n_adapters; ++job)
+    a.first[job + 1] = a.first[job] + pad(job < n_adapters ? a.hidden : a.seg[job - n_adapters]);
+  a.cols = static_cast<int>(w.cols);
+  a.chunk = static_cast<int>(w.chunk); a.chunks = static_cast<int>(w.chunks);
+  a.part = static_cast<float*>(workspace);
+  a.half_out = grad_dtype == TALM_F16;
+  a.da[0] = da0; a.da[1] = da1; a.db[0] = db0; a.db[1] = db1;
+  const hipStream_t s = as_stream(stream);
+  hipLaunchKernelGGL(lora_wgrad_drop_kernel, dim3(static_cast<unsigned>(w.cols / 128), static_cast<unsigned>(w.chunks)),
+                     dim3(256), 0, s, a);
+  hipLaunchKernelGGL(lora_wgrad_sum_kernel, dim3(static_cast<unsigned>((w.cols * kRank + 255) / 256)), dim3(256), 0,
+                     s, a);
+  return check_launch("lora_wgrad_drop");
+}

@@ -20,6 +20,7 @@
 #include <ATen/hip/HIPContext.h>
 #include <hipblaslt/hipblaslt-ext.hpp>
 #include <hipblaslt/hipblaslt.h>
+#include <c10/core/DeviceGuard.h>
 #include <torch/library.h>
 
 #include <atomic>
@@ -672,6 +673,251 @@ void attn_bwd_rope(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
                    double scale, const Tensor& cos, const Tensor& sin, const Tensor& dq,
                    const Tensor& dk, const Tensor& dv, const Tensor& workspace) {
   attn_bwd_any(q, k, v, out, dout, lse, cu, max_seqlen, scale, cos, sin, dq, dk, dv, workspace);
+}
+
+// ------------------------------------------------------------------------------------------
+// Sliding-window attention with sinks (fp16 or bf16 operands)
+// ------------------------------------------------------------------------------------------
+int32_t int32_arg(int64_t v, const char* name) {
+  TORCH_CHECK_VALUE(v >= INT32_MIN && v <= INT32_MAX, name, " ", v, " does not fit 32 bits");
+  return static_cast<int32_t>(v);
+}
+
+void window_operand(const Tensor& t, const Tensor& like, const char* name, int64_t n, int64_t heads) {
+  TORCH_CHECK_VALUE(t.is_cuda() && (t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16) &&
+                        t.scalar_type() == like.scalar_type() && t.device() == like.device() &&
+                        t.dim() == 3 && t.size(0) == n && t.size(1) == heads && t.size(2) == 128 &&
+                        t.stride(2) == 1,
+                    "attn_window: ", name, " must be an fp16 or bf16 [", n, ", ", heads,
+                    ", 128] view with unit column stride, of q's type and device");
+}
+
+int32_t window_dtype(const Tensor& q) { return q.scalar_type() == at::kHalf ? TALM_F16 : TALM_BF16; }
+
+void window_common(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu, const Tensor& out,
+                   const Tensor& lse) {
+  require(q.dim() == 3 && k.dim() == 3, "attn_window: q [N, Hq, 128], k / v [N, Hkv, 128]");
+  const int64_t n = q.size(0), hq = q.size(1), hkv = k.size(1);
+  window_operand(q, q, "q", n, hq);
+  window_operand(k, q, "k", n, hkv);
+  window_operand(v, q, "v", n, hkv);
+  window_operand(out, q, "out", n, hq);
+  attn_cu(cu, q);
+  require(lse.is_cuda() && lse.device() == q.device() && lse.scalar_type() == at::kFloat &&
+              lse.is_contiguous() && same_shape(lse, hq, n),
+          "attn_window: lse float32 [Hq, N]");
+}
+
+void attn_window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
+                     int64_t max_seqlen, double scale, int64_t window, int64_t sinks, const Tensor& out,
+                     const Tensor& lse) {
+  window_common(q, k, v, cu, out, lse);
+  const c10::DeviceGuard guard(q.device());
+  check(talm_attn_window_fwd(as<uint16_t>(q), q.stride(0), q.stride(1), as<uint16_t>(k), k.stride(0),
+                             k.stride(1), as<uint16_t>(v), v.stride(0), v.stride(1), as<int32_t>(cu),
+                             int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_seqlen, "max_seqlen"),
+                             q.size(0), int32_arg(q.size(1), "heads"), int32_arg(k.size(1), "heads"), 128,
+                             static_cast<float>(scale), int32_arg(window, "window"),
+                             int32_arg(sinks, "sinks"), window_dtype(q), as<uint16_t>(out), out.stride(0),
+                             out.stride(1), as<float>(lse), stream_of(q)),
+        "attn_window_fwd");
+}
+
+void attn_window_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& out,
+                     const Tensor& dout, const Tensor& lse, const Tensor& cu, int64_t max_seqlen,
+                     double scale, int64_t window, int64_t sinks, const OptTensor& cos,
+                     const OptTensor& sin, const Tensor& dq, const Tensor& dk, const Tensor& dv,
+                     const Tensor& workspace) {
+  window_common(q, k, v, cu, out, lse);
+  const int64_t n = q.size(0), hq = q.size(1), hkv = k.size(1);
+  window_operand(dout, q, "dout", n, hq);
+  window_operand(dq, q, "dq", n, hq);
+  window_operand(dk, q, "dk", n, hkv);
+  window_operand(dv, q, "dv", n, hkv);
+  require(workspace.is_cuda() && workspace.device() == q.device() && workspace.is_contiguous(),
+          "attn_window_bwd: workspace");
+  require(cos.has_value() == sin.has_value(), "attn_window_bwd: cos and sin both or neither");
+  if (cos.has_value()) {
+    require(cos->device() == q.device() && sin->device() == q.device(), "attn_window_bwd: cos/sin on q's device");
+    cos_sin_rows(cos, sin, n, "attn_window_bwd: cos/sin fp32 [N, >= 128] with one row stride");
+  }
+  const c10::DeviceGuard guard(q.device());
+  check(talm_attn_window_bwd(
+            as<uint16_t>(q), q.stride(0), q.stride(1), as<uint16_t>(k), k.stride(0), k.stride(1),
+            as<uint16_t>(v), v.stride(0), v.stride(1), as<uint16_t>(out), out.stride(0), out.stride(1),
+            as<uint16_t>(dout), dout.stride(0), dout.stride(1), as<float>(lse), as<int32_t>(cu),
+            int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_seqlen, "max_seqlen"), n,
+            int32_arg(hq, "heads"), int32_arg(hkv, "heads"), 128, static_cast<float>(scale),
+            int32_arg(window, "window"), int32_arg(sinks, "sinks"), window_dtype(q), as<float>(cos),
+            as<float>(sin), cos.has_value() ? cos->stride(0) : 0, as<uint16_t>(dq), dq.stride(0),
+            dq.stride(1), as<uint16_t>(dk), dk.stride(0), dk.stride(1), as<uint16_t>(dv), dv.stride(0),
+            dv.stride(1), workspace.data_ptr(),
+            workspace.numel() * static_cast<int64_t>(workspace.element_size()), stream_of(q)),
+        "attn_window_bwd");
+}
+
+// ------------------------------------------------------------------------------------------
+// Dropout from the counter-based generator, and the adapters' products with it
+// ------------------------------------------------------------------------------------------
+const int64_t* drop_key(const OptTensor& key, const Tensor& like) {
+  if (!key.has_value()) return nullptr;
+  TORCH_CHECK_VALUE(key->is_cuda() && key->device() == like.device() && key->scalar_type() == at::kLong &&
+                        key->numel() == 2 && key->is_contiguous(),
+                    "dropout: key int64 [2] on the operands' device");
+  return as<int64_t>(*key);
+}
+
+uint32_t drop_site(int64_t site) {
+  TORCH_CHECK_VALUE(site >= 0 && site <= int64_t{0xffffffff}, "dropout: site ", site, " (0 .. 2^32 - 1)");
+  return static_cast<uint32_t>(site);
+}
+
+// The row stride of a matrix; of a single row (whose stride may be anything) that of a dense one.
+int64_t row_stride(const Tensor& t) { return t.size(0) <= 1 ? (t.size(1) + 7) / 8 * 8 : t.stride(0); }
+
+void half_rows(const Tensor& t, const Tensor& like, const char* name) {
+  TORCH_CHECK_VALUE(t.is_cuda() && t.scalar_type() == at::kHalf && t.device() == like.device() && t.dim() == 2 &&
+                        (t.stride(1) == 1 || t.size(1) == 1),
+                    name, " must be a CUDA float16 matrix with unit column stride on x's device");
+}
+
+void dropout(const Tensor& x, double p, const OptTensor& key, int64_t site, const Tensor& y) {
+  require(x.is_cuda() && x.dim() == 2 && y.dim() == 2 && x.sizes() == y.sizes() && y.device() == x.device() &&
+              y.scalar_type() == x.scalar_type() && (x.size(1) <= 1 || (x.stride(1) == 1 && y.stride(1) == 1)),
+          "dropout: x and y [rows, cols] of one type and device with unit column stride");
+  const int32_t dtype = x.scalar_type() == at::kBFloat16 ? TALM_BF16 : dtype_code(x.scalar_type());
+  const c10::DeviceGuard guard(x.device());
+  check(talm_dropout(ptr(x), row_stride(x), x.size(0), x.size(1), dtype,
+                     static_cast<float>(p), drop_key(key, x), drop_site(site), ptr(y),
+                     row_stride(y), stream_of(x)),
+        "dropout");
+}
+
+// t and ts [N, 16 per adapter] = factor (keep x) A^T, scaling times it.
+void lora_down_drop(const Tensor& x, const Tensor& a0, const OptTensor& a1, double p, const OptTensor& key,
+                    int64_t site0, int64_t site1, double scaling0, double scaling1, const Tensor& t,
+                    const Tensor& ts, const OptTensor& workspace) {
+  const bool two = a1.has_value();
+  half_rows(x, x, "lora_down_drop: x");
+  half_rows(t, x, "lora_down_drop: t");
+  half_rows(ts, x, "lora_down_drop: ts");
+  for (const Tensor* a : {&a0, two ? &*a1 : &a0})
+    require(a->is_cuda() && a->scalar_type() == at::kHalf && a->device() == x.device() && a->is_contiguous() &&
+                same_shape(*a, 16, x.size(1)),
+            "lora_down_drop: A float16 [16, k], contiguous, on x's device");
+  require(same_shape(t, x.size(0), two ? 32 : 16) && ts.sizes() == t.sizes() && row_stride(ts) == row_stride(t),
+          "lora_down_drop: t, ts [N, 16 per adapter] of one layout");
+  if (workspace.has_value())
+    require(workspace->is_cuda() && workspace->is_contiguous() && workspace->device() == x.device(),
+            "lora_down_drop: workspace");
+  const c10::DeviceGuard guard(x.device());
+  check(talm_lora_down_drop(as<uint16_t>(x), row_stride(x), x.size(0), x.size(1), as<uint16_t>(a0),
+                            as<uint16_t>(a1), two ? 2 : 1, static_cast<float>(p), drop_key(key, x),
+                            drop_site(site0), drop_site(site1), static_cast<float>(scaling0),
+                            static_cast<float>(scaling1), as<uint16_t>(t), as<uint16_t>(ts), row_stride(t),
+                            ptr(workspace),
+                            workspace.has_value()
+                                ? workspace->numel() * static_cast<int64_t>(workspace->element_size())
+                                : 0,
+                            stream_of(x)),
+        "lora_down_drop");
+}
+
+// out [N, cols] = base + sum_g factor keep_g (u_g M_g^T); M [cols, 16], or [16, cols] with m_kmajor.
+void lora_up(const Tensor& u, const Tensor& m0, const OptTensor& m1, bool m_kmajor, double p,
+             const OptTensor& key, int64_t site0, int64_t site1, const OptTensor& base, const Tensor& out) {
+  const bool two = m1.has_value();
+  half_rows(u, u, "lora_up: u");
+  half_rows(out, u, "lora_up: out");
+  require(u.size(1) >= (two ? 32 : 16) && u.size(0) == out.size(0), "lora_up: u [N, 16 per adapter], out [N, cols]");
+  const int64_t cols = out.size(1);
+  for (const Tensor* m : {&m0, two ? &*m1 : &m0})
+    require(m->is_cuda() && m->scalar_type() == at::kHalf && m->device() == u.device() && m->is_contiguous() &&
+                (m_kmajor ? same_shape(*m, 16, cols) : same_shape(*m, cols, 16)),
+            "lora_up: M float16 [cols, 16] ([16, cols] with m_kmajor), contiguous, on u's device");
+  if (base.has_value()) {
+    half_rows(*base, u, "lora_up: base");
+    require(base->sizes() == out.sizes(), "lora_up: base of out's shape");
+  }
+  const c10::DeviceGuard guard(u.device());
+  check(talm_lora_up(as<uint16_t>(u), row_stride(u), u.size(0), cols, as<uint16_t>(m0), as<uint16_t>(m1),
+                     two ? 2 : 1, m_kmajor, static_cast<float>(p), drop_key(key, u), drop_site(site0),
+                     drop_site(site1), as<uint16_t>(base), base.has_value() ? row_stride(*base) : 0,
+                     as<uint16_t>(out), row_stride(out), stream_of(u)),
+        "lora_up");
+}
+
+void lora_wgrad_drop(const Tensor& x, const Tensor& dy, const Tensor& u, const Tensor& t, double p,
+                     const OptTensor& key, int64_t site0, int64_t site1, int64_t lo0, int64_t seg0,
+                     double scaling0, const Tensor& da0, const Tensor& db0, int64_t lo1, int64_t seg1,
+                     double scaling1, const OptTensor& da1, const OptTensor& db1, const Tensor& workspace) {
+  const bool two = da1.has_value();
+  require(two == db1.has_value(), "lora_wgrad_drop: dA and dB of the second adapter both or neither");
+  half_rows(x, x, "lora_wgrad_drop: x");
+  half_rows(dy, x, "lora_wgrad_drop: dy");
+  half_rows(u, x, "lora_wgrad_drop: u");
+  half_rows(t, x, "lora_wgrad_drop: t");
+  const int64_t n = x.size(0), hidden = x.size(1), rank = two ? 32 : 16;
+  require(dy.size(0) == n && same_shape(u, n, rank) && same_shape(t, n, rank),
+          "lora_wgrad_drop: dy [N, ..], u and t [N, 16 per adapter]");
+  require(lo0 >= 0 && seg0 >= 0 && lo0 + seg0 <= dy.size(1) &&
+              (!two || (lo1 >= 0 && seg1 >= 0 && lo1 + seg1 <= dy.size(1))),
+          "lora_wgrad_drop: segments inside dy's columns");
+  const at::ScalarType type = da0.scalar_type();
+  auto grad = [&](const Tensor& g, int64_t r, int64_t c) {
+    require(g.is_cuda() && g.device() == x.device() && g.scalar_type() == type && g.is_contiguous() &&
+                same_shape(g, r, c),
+            "lora_wgrad_drop: dA [16, hidden], dB [segment, 16], contiguous, of one type");
+  };
+  grad(da0, 16, hidden);
+  grad(db0, seg0, 16);
+  if (two) {
+    grad(*da1, 16, hidden);
+    grad(*db1, seg1, 16);
+  }
+  require(workspace.is_cuda() && workspace.is_contiguous() && workspace.device() == x.device(),
+          "lora_wgrad_drop: workspace");
+  const c10::DeviceGuard guard(x.device());
+  check(talm_lora_wgrad_drop(as<uint16_t>(x), row_stride(x), as<uint16_t>(dy), row_stride(dy), as<uint16_t>(u),
+                             row_stride(u), as<uint16_t>(t), row_stride(t), n, hidden, two ? 2 : 1,
+                             static_cast<float>(p), drop_key(key, x), drop_site(site0), drop_site(site1),
+                             dtype_code(type), lo0, seg0, static_cast<float>(scaling0), ptr(da0), ptr(db0), lo1,
+                             seg1, static_cast<float>(scaling1), ptr(da1), ptr(db1), workspace.data_ptr(),
+                             workspace.numel() * static_cast<int64_t>(workspace.element_size()), stream_of(x)),
+        "lora_wgrad_drop");
+}
+
+// out [M, rows] = x [M, cols] W^T + bias for a few tokens, W the NF4 weight its buffers start at.
+void nf4_gemv(const Tensor& x, const Tensor& packed, const Tensor& absmax8, const Tensor& code,
+              const Tensor& absmax2, const Tensor& offset2, int64_t rows, int64_t cols, int64_t qblock,
+              int64_t qblock2, const OptTensor& bias, const Tensor& out) {
+  half_rows(x, x, "nf4_gemv: x");
+  half_rows(out, x, "nf4_gemv: out");
+  require(x.size(1) == cols && same_shape(out, x.size(0), rows), "nf4_gemv: x [M, cols], out [M, rows]");
+  for (const Tensor* t : {&packed, &absmax8, &code, &absmax2, &offset2})
+    require(t->is_cuda() && t->device() == x.device() && t->is_contiguous(),
+            "nf4_gemv: the weight's buffers contiguous on x's device");
+  require(packed.scalar_type() == at::kByte && absmax8.scalar_type() == at::kByte &&
+              code.scalar_type() == at::kFloat && absmax2.scalar_type() == at::kFloat &&
+              offset2.scalar_type() == at::kFloat,
+          "nf4_gemv: packed / absmax8 uint8, code / absmax2 / offset2 float32");
+  require(qblock > 0 && qblock2 > 0 && rows > 0 && cols > 0 && rows < (int64_t{1} << 31) &&
+              cols < (int64_t{1} << 31),
+          "nf4_gemv: sizes positive");
+  const int64_t n = rows * cols, blocks = (n + qblock - 1) / qblock, groups = (blocks + qblock2 - 1) / qblock2;
+  require(packed.numel() * 2 >= n && absmax8.numel() >= blocks && code.numel() >= 256 &&
+              absmax2.numel() >= groups && offset2.numel() >= groups,
+          "nf4_gemv: the buffers do not cover W");
+  if (bias.has_value())
+    require(bias->is_cuda() && bias->device() == x.device() && bias->scalar_type() == at::kHalf &&
+                bias->is_contiguous() && bias->numel() == rows,
+            "nf4_gemv: bias float16 [rows]");
+  const c10::DeviceGuard guard(x.device());
+  check(talm_nf4_gemv(as<uint16_t>(x), row_stride(x), x.size(0),
+                      as<uint8_t>(packed), as<uint8_t>(absmax8), as<float>(code), as<float>(absmax2),
+                      as<float>(offset2), rows, cols, int32_arg(qblock, "qblock"), int32_arg(qblock2, "qblock2"),
+                      as<uint16_t>(bias), as<uint16_t>(out), row_stride(out), stream_of(x)),
+        "nf4_gemv");
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1517,6 +1763,21 @@ TORCH_LIBRARY(talm, m) {
   m.def("attn_bwd_rope(Tensor q, Tensor k, Tensor v, Tensor out, Tensor dout, Tensor lse, "
         "Tensor cu_seqlens, int max_seqlen, float scale, Tensor cos, Tensor sin, Tensor(a!) dq, "
         "Tensor(b!) dk, Tensor(c!) dv, Tensor(d!) workspace) -> ()");
+  m.def("attn_window_fwd(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, int max_seqlen, float scale, "
+        "int window, int sinks, Tensor(a!) out, Tensor(b!) lse) -> ()");
+  m.def("attn_window_bwd(Tensor q, Tensor k, Tensor v, Tensor out, Tensor dout, Tensor lse, "
+        "Tensor cu_seqlens, int max_seqlen, float scale, int window, int sinks, Tensor? cos, Tensor? sin, "
+        "Tensor(a!) dq, Tensor(b!) dk, Tensor(c!) dv, Tensor(d!) workspace) -> ()");
+  m.def("dropout(Tensor x, float p, Tensor? key, int site, Tensor(a!) y) -> ()");
+  m.def("lora_down_drop(Tensor x, Tensor a0, Tensor? a1, float p, Tensor? key, int site0, int site1, "
+        "float scaling0, float scaling1, Tensor(a!) t, Tensor(b!) ts, Tensor(c!)? workspace) -> ()");
+  m.def("lora_up(Tensor u, Tensor m0, Tensor? m1, bool m_kmajor, float p, Tensor? key, int site0, "
+        "int site1, Tensor? base, Tensor(a!) out) -> ()");
+  m.def("lora_wgrad_drop(Tensor x, Tensor dy, Tensor u, Tensor t, float p, Tensor? key, int site0, "
+        "int site1, int lo0, int seg0, float scaling0, Tensor(a!) da0, Tensor(b!) db0, int lo1, int seg1, "
+        "float scaling1, Tensor(c!)? da1, Tensor(d!)? db1, Tensor(e!) workspace) -> ()");
+  m.def("nf4_gemv(Tensor x, Tensor packed, Tensor absmax8, Tensor code, Tensor absmax2, Tensor offset2, "
+        "int rows, int cols, int qblock, int qblock2, Tensor? bias, Tensor(a!) out) -> ()");
   m.def("lora_mirror(Tensor table, int n_tensors, int max_numel, Tensor(a!) out) -> ()");
   m.def("pack_rows(Tensor input_ids, Tensor mask, Tensor labels, int n_tokens, Tensor(a!) ids, "
         "Tensor(b!) positions, Tensor(c!) cu, Tensor(d!) targets, Tensor(e!) src) -> ()");
@@ -1584,6 +1845,13 @@ TORCH_LIBRARY_IMPL(talm, CUDA, m) {
   m.impl("attn_fwd", &attn_fwd);
   m.impl("attn_bwd", &attn_bwd);
   m.impl("attn_bwd_rope", &attn_bwd_rope);
+  m.impl("attn_window_fwd", &attn_window_fwd);
+  m.impl("attn_window_bwd", &attn_window_bwd);
+  m.impl("dropout", &dropout);
+  m.impl("lora_down_drop", &lora_down_drop);
+  m.impl("lora_up", &lora_up);
+  m.impl("lora_wgrad_drop", &lora_wgrad_drop);
+  m.impl("nf4_gemv", &nf4_gemv);
   m.impl("lora_mirror", &lora_mirror);
   m.impl("gemm_tune", &gemm_tune);
   m.impl("nf4_gemm", &nf4_gemm);

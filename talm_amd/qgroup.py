@@ -68,6 +68,9 @@ T_BLOCKS = ((0, 1, 2), (3,), (4, 5), (6,))
 # the transposed dequantization.
 W4_BLOCKS = ((4, 5),) if os.environ.get("SOLUTION_DISABLE_W4A16") != "1" else ()
 
+# the most rows of x that talm_nf4_gemv takes
+GEMV_TOKENS = 32
+
 
 def launch(packed, absmax8, code, absmax2, offset2, levels, out, n_rows, qblock, qblock2,
            streaming=False):
@@ -312,6 +315,28 @@ class LayerGroup:
         segs = self.segments[first:last]
         rows, cols = sum(seg.shape[0] for seg in segs), segs[0].shape[1]
         return _ops.nf4_gemm_parts(n_tokens, rows, cols, transpose)
+
+    # -- a few tokens' products on the NF4 codes -------------------------------------------------------
+    def gemv_ok(self, first, last):
+        """Projections first .. last - 1 are one [sum of out, in] matrix talm_nf4_gemv takes."""
+        cols = {seg.shape[1] for seg in self.segments[first:last]}
+        return (self.qblock == 64 and self.qblock2 & (self.qblock2 - 1) == 0 and len(cols) == 1
+                and next(iter(cols)) % 64 == 0)
+
+    def nf4_gemv(self, x, first, last, out):
+        """out [M, sum of out] = x [M, in] W^T + the projections' biases for M <= GEMV_TOKENS rows, W
+        the rows of projections first .. last - 1 read as NF4 codes (the fp16 weights of `span`, never
+        written out). For calls that answer token by token; more rows: `nf4_gemm`, or `span`."""
+        if not self.gemv_ok(first, last):
+            raise ValueError(f"nf4_gemv: projections {first} .. {last - 1} are not one matrix of 64-weight "
+                             "blocks and whole blocks per row")
+        segs = self.segments[first:last]
+        lo, row0 = segs[0].start, segs[0].start // self.qblock
+        torch.ops.talm.nf4_gemv(x, self.packed[lo // 2:], self.absmax8[row0:], self.code,
+                                self.absmax2[row0 // self.qblock2:],
+                                self.offset2[row0 // self.qblock2:],
+                                sum(seg.shape[0] for seg in segs), segs[0].shape[1], self.qblock,
+                                self.qblock2, self.span_bias(first, last), out)
 
     def dequantize_one(self, idx):
         return self.dequantize(idx, idx + 1).view(self.segments[idx].shape)

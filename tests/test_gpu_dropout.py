@@ -1,0 +1,259 @@
+"""Counter-based dropout (dropout.dropout) and the adapters' products with it (lora.adapter_branch,
+torch.ops.talm.lora_*_drop / lora_up), against the oracle's masks and float64 products.
+
+The masks are exact. Tolerances of the products count roundings of at most u = 2^-11 relative (fp16),
+each sum of n products in fp32 adding at most n 2^-24 of the magnitudes summed:
+  t  = x A^T rounded (u); ts = s t rounded (u); y = ts B^T rounded: sum |ts| |B| (u + the sum of t) + u |y|
+  u  = s dy B rounded; dx = u A rounded; dA = u^T x, dB = s dy^T t: of the rounded u and t, (fp16
+  gradients: rounded once more)."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import philox
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -11
+
+
+def _key(*words):
+    return torch.tensor(words, dtype=torch.int64, device="cuda")
+
+
+def _keep(key, rows, cols, p, site=0):
+    return torch.from_numpy(philox.keep(key.tolist(), rows, cols, p, site)).cuda()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols,p", [(1, 1, 0.5), (3, 13, 0.3), (131, 1536, 0.05), (7, 1001, 0.9),
+                                         (64, 8, 0.0), (33, 24, 0.999999)])
+def test_dropout_is_exactly_its_definition(rows, cols, p, dtype):
+    from talm_amd.dropout import dropout
+
+    print(f"[case] dropout {rows} x {cols} p={p} {dtype}", flush=True)
+    g = torch.Generator("cuda").manual_seed(rows)
+    key = _key(-(2 ** 63) + 12345, 2 ** 40 + 6)
+    x = torch.randn(rows, cols, generator=g, device="cuda").to(dtype).requires_grad_()
+    dy = torch.randn(rows, cols, generator=g, device="cuda").to(dtype)
+    y = dropout(x, p, key, 9)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    keep, f = _keep(key, rows, cols, p, 9), float(philox.factor(p))
+    for got, src in ((y, x.detach()), (dx, dy)):
+        want = torch.where(keep, (src.float() * f).to(dtype), torch.zeros((), dtype=dtype, device="cuda"))
+        assert torch.equal(got, want)
+
+
+def test_dropped_values_are_zero_whatever_they_were_and_shapes_stay():
+    from talm_amd.dropout import draw_key, dropout
+
+    torch.manual_seed(3)
+    key = draw_key("cuda")
+    torch.manual_seed(3)
+    assert torch.equal(key, draw_key("cuda")) and not torch.equal(key, draw_key("cuda"))
+    x = torch.full((2, 3, 5, 8), float("nan"), device="cuda")
+    y = dropout(x, 0.5, key)
+    keep = _keep(key, 30, 8, 0.5).view(2, 3, 5, 8)
+    assert y.shape == x.shape and (y[~keep] == 0).all() and torch.isnan(y[keep]).all()
+    for shape in ((0, 8), (4, 0), (0,)):
+        assert dropout(torch.empty(shape, device="cuda"), 0.5, key).shape == shape
+    one = torch.ones((), device="cuda")
+    assert dropout(one, 0.0) == 1 and dropout(one, 0.0).shape == ()
+
+
+def test_strided_rows_and_in_place():
+    from talm_amd import _ops  # noqa: F401
+    from talm_amd.dropout import dropout
+
+    key = _key(1, 2)
+    wide = torch.randn(40, 72, device="cuda").half()
+    for view in (wide[:, 8:40], wide[:, 3:36], wide[::2, :16], wide.t(), wide[:1, :5],
+                 wide[:1].expand(40, 72)):
+        keep = _keep(key, *view.shape, 0.4)
+        want = torch.where(keep, (view.float() * float(philox.factor(0.4))).half(), 0.0)
+        assert torch.equal(dropout(view, 0.4, key), want)
+    x = wide.clone()
+    torch.ops.talm.dropout(x, 0.4, key, 0, x)
+    assert torch.equal(x, dropout(wide, 0.4, key))
+
+
+def test_dropout_refusals_on_the_gpu():
+    from talm_amd.dropout import dropout
+
+    x = torch.ones(4, 8, device="cuda")
+    for args in ((x, 0.5), (x, 1.0, _key(1, 2)), (x, 0.5, torch.tensor([1, 2])), (x, 0.5, _key(1, 2, 3)),
+                 (x, 0.5, _key(1, 2), -1), (x.double(), 0.5, _key(1, 2)), (x.long(), 0.5, _key(1, 2))):
+        with pytest.raises(ValueError):
+            dropout(*args)
+
+
+def test_a_captured_dropout_follows_its_key():
+    from talm_amd.dropout import draw_key, dropout
+
+    x = torch.randn(64, 256, device="cuda").half()
+    key = _key(5, 6)
+    dropout(x, 0.3, key)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = dropout(x, 0.3, key)
+        drawn = draw_key("cuda")
+        z = dropout(x, 0.3, drawn)
+    seen = set()
+    for i in range(4):
+        key.copy_(_key(5, i))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, dropout(x, 0.3, _key(5, i)))
+        assert torch.equal(z, dropout(x, 0.3, drawn.clone()))
+        seen.add(tuple(drawn.tolist()))
+    assert len(seen) == 4  # a replay draws a key of its own
+
+
+# -- the adapters' products ------------------------------------------------------------------------
+
+def _branch(n, size, out, p, dtype, seed, key, site=4, scaling=2.0):
+    g = torch.Generator("cuda").manual_seed(seed)
+    x = torch.randn(n, size, generator=g, device="cuda").half().requires_grad_()
+    a = ((torch.rand(16, size, generator=g, device="cuda") * 2 - 1) * size ** -0.5).to(dtype).requires_grad_()
+    b = (torch.randn(out, 16, generator=g, device="cuda") * 0.05).to(dtype).requires_grad_()
+    dy = torch.randn(n, out, generator=g, device="cuda").half()
+    return x, a, b, dy
+
+
+def _expect(x, a, b, dy, m, scaling, half_grads):
+    """float64 values and tolerances of y, dx, dA, dB; m: the mask times its factor."""
+    x, a, b, dy = (t.detach().half().double() for t in (x, a, b, dy))
+    xd = x * m
+    size, out, n = x.shape[1], b.shape[0], x.shape[0]
+    acc = 2.0 ** -24
+    t, ta = xd @ a.T, xd.abs() @ a.abs().T
+    tol_t = U * t.abs() + (size + 2) * acc * ta + 2.0 ** -25
+    y = scaling * t @ b.T
+    tol_y = scaling * (tol_t + 2.0 ** -25) @ b.abs().T + 16 * acc * scaling * t.abs() @ b.abs().T + U * y.abs() + 2.0 ** -25
+    u = scaling * dy @ b
+    tol_u = U * u.abs() + out * acc * scaling * dy.abs() @ b.abs() + 2.0 ** -25
+    dx = (u @ a) * m
+    tol_dx = (tol_u @ a.abs() + 18 * acc * u.abs() @ a.abs()) * m + U * dx.abs() + 2.0 ** -25
+    da, db = u.T @ xd, scaling * dy.T @ t
+    tol_da = tol_u.T @ xd.abs() + (n + 2) * acc * u.abs().T @ xd.abs()
+    tol_db = scaling * (dy.abs().T @ tol_t + (n + 2) * acc * dy.abs().T @ t.abs())
+    if half_grads:
+        tol_da, tol_db = tol_da + U * da.abs() + 2.0 ** -25, tol_db + U * db.abs() + 2.0 ** -25
+    return (y, dx, da, db), (tol_y, tol_dx, tol_da, tol_db)
+
+
+def _compare(got, want, tols):
+    for name, a, b, tol in zip(("y", "dx", "dA", "dB"), got, want, tols):
+        err = (a.double() - b).abs()
+        worst = (err / tol.clamp_min(1e-30)).max().item() if err.numel() else 0.0
+        print(f"  {name}: max err {err.max().item() if err.numel() else 0:.3e}, {worst:.3f} of its tolerance", flush=True)
+        assert a.shape == b.shape and worst <= 1.0, name
+
+
+@pytest.mark.parametrize("n,size,out", [(1, 32, 32), (17, 96, 160), (64, 1536, 256), (131, 896, 128),
+                                        (200, 256, 1536), (70, 4864, 896)])
+@pytest.mark.parametrize("p,dtype", [(0.0, torch.float32), (0.1, torch.float32), (0.5, torch.float16)])
+def test_adapter_branch_matches_its_formula(n, size, out, p, dtype):
+    from talm_amd.lora import adapter_branch
+
+    print(f"[case] adapter branch {n} x {size} -> {out} p={p} {dtype}", flush=True)
+    key = _key(77, n)
+    x, a, b, dy = _branch(n, size, out, p, dtype, n + size, key)
+    y = adapter_branch(x, a, b, 2.0, p, key if p else None, 4)
+    grads = torch.autograd.grad(y, (x, a, b), dy)
+    assert grads[1].dtype == grads[2].dtype == dtype
+    m = _keep(key, n, size, p, 4).double() / (1 - philox.threshold(p) / 65536)
+    _compare((y, *grads), *_expect(x, a, b, dy, m, 2.0, dtype == torch.float16))
+
+
+def test_adapter_branch_without_rows_and_with_batch_dimensions():
+    from talm_amd.lora import adapter_branch
+
+    key = _key(3, 4)
+    x, a, b, dy = _branch(24, 64, 96, 0.2, torch.float32, 1, key)
+    y = adapter_branch(x, a, b, 2.0, 0.2, key)
+    y3 = adapter_branch(x.view(2, 3, 4, 64), a, b, 2.0, 0.2, key)
+    assert y3.shape == (2, 3, 4, 96) and torch.equal(y3.view(24, 96), y)
+    wide = torch.zeros(24, 80, dtype=torch.float16, device="cuda")
+    wide[:, 4:68] = x.detach()  # rows that are not 16-byte aligned are copied
+    assert torch.equal(adapter_branch(wide[:, 4:68], a, b, 2.0, 0.2, key), y)
+    empty = x.detach()[:0].requires_grad_()
+    out = adapter_branch(empty, a, b, 2.0, 0.2, key)
+    grads = torch.autograd.grad(out.sum(), (empty, a, b))
+    assert out.shape == (0, 96) and (grads[1] == 0).all() and (grads[2] == 0).all()
+
+
+def test_adapter_branch_refusals():
+    from talm_amd.lora import adapter_branch
+
+    x, a, b, _ = _branch(4, 64, 32, 0.2, torch.float32, 1, None)
+    key = _key(1, 2)
+    for args in ((x.float(), a, b, 2.0), (x, a[:8], b[:, :8], 2.0), (x[:, :48], a[:, :48], b, 2.0),
+                 (x, a, b.half(), 2.0), (x, a, b[:24], 2.0), (x, a, b, 2.0, 0.2), (x, a, b, 2.0, 1.5, key),
+                 (x, a.cpu(), b.cpu(), 2.0)):
+        with pytest.raises(ValueError):
+            adapter_branch(*args)
+
+
+def test_two_adapters_have_masks_of_their_own():
+    """The products over two adapters of one x (q and v of a layer): each under its own site."""
+    from talm_amd import _ops
+
+    n, size, lo, seg = 75, 160, (0, 128), (96, 64)
+    p, key, sites = 0.3, _key(8, 9), (0, 1)
+    g = torch.Generator("cuda").manual_seed(2)
+    def rand(*shape):
+        return torch.randn(*shape, generator=g, device="cuda")
+    x = rand(n, size).half()
+    a = [(rand(16, size) * 0.05).half() for _ in range(2)]
+    b = [(rand(s, 16) * 0.05).half() for s in seg]
+    dy = rand(n, 192).half()
+    half = dict(dtype=torch.float16, device="cuda")
+    t, ts = torch.empty(n, 32, **half), torch.empty(n, 32, **half)
+    torch.ops.talm.lora_down_drop(x, a[0], a[1], p, key, *sites, 2.0, 3.0, t, ts, None)
+    u_raw, u = torch.empty(n, 32, **half), torch.empty(n, 32, **half)
+    torch.ops.talm.lora_down(dy, b[0], b[1], seg[0], seg[1], lo[0], lo[1], 1, 2.0, 3.0, u_raw, u)
+    base = rand(n, size).half()
+    dx = base.clone()
+    torch.ops.talm.lora_up(u, a[0], a[1], True, p, key, *sites, dx, dx)
+    da = [torch.empty(16, size, device="cuda") for _ in range(2)]
+    db = [torch.empty(s, 16, device="cuda") for s in seg]
+    ws = torch.full((_ops.lora_wgrad_drop_workspace_bytes(n, size, 2, *seg),), 255, dtype=torch.uint8, device="cuda")
+    torch.ops.talm.lora_wgrad_drop(x, dy, u, t, p, key, *sites, lo[0], seg[0], 2.0, da[0], db[0], lo[1], seg[1],
+                                   3.0, da[1], db[1], ws)
+    total, tol = base.double(), U * base.double().abs() + 2.0 ** -24
+    for i, scaling in enumerate((2.0, 3.0)):
+        m = _keep(key, n, size, p, sites[i]).double() / (1 - philox.threshold(p) / 65536)
+        dyi = dy[:, lo[i]:lo[i] + seg[i]]
+        want, tols = _expect(x, a[i], b[i], dyi, m, scaling, False)
+        _compare((ts[:, 16 * i:16 * i + 16].double() @ b[i].double().T, want[1], da[i], db[i]), want, tols)
+        total, tol = total + want[1], tol + tols[1] + U * want[1].abs()
+    assert ((dx.double() - total).abs() <= tol).all()
+
+
+def test_a_captured_branch_replays():
+    from talm_amd.lora import adapter_branch
+
+    key = _key(1, 1)
+    x, a, b, dy = _branch(96, 256, 128, 0.2, torch.float16, 5, key)
+
+    def step():
+        y = adapter_branch(x, a, b, 2.0, 0.2, key)
+        return (y.detach(), *torch.autograd.grad(y, (x, a, b), dy))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(4):
+        key.copy_(_key(i, 7))
+        with torch.no_grad():
+            x.copy_(torch.randn(96, 256, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(outs, step()):
+            assert torch.equal(got, want)

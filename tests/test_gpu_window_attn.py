@@ -1,0 +1,267 @@
+"""Sliding-window attention with sinks over packed rows (unpad.window_attention) against its formula
+in float64 on the CPU: output, and the gradients of q, k and v.
+
+Tolerances count roundings, each at most half a step u of the operands' type (fp16 2^-11, bf16
+2^-8), elementwise against the magnitudes summed:
+  out     P is rounded (u P, and 2^-25 where fp16 turns subnormal, with a row's sum at least 1:
+          relative to it at most 2^-25), the output is rounded: u (sum P |V| + |out|) + n 2^-25 max |V|
+  dV      u (sum P |dO| + |dV|) + 2^-25 sum |dO| over the rows that see the key
+  dS      = P (dP - D), rounded: u |dS| + 2^-25; D comes from the rounded output, off by at most
+          sum |dO| tol(out)
+  every result's own rounding: u, or 2^-25 where fp16 is subnormal
+  dQ, dK  scale sum tol(dS) |K| (|Q|) + u |dQ|
+and every P carries the fp32 error of its score: a 128-term product (128 2^-24 sum |q k| scale) and of
+exp2, log2 and the scale's product (2^-19 in all for exponents up to 2^5)."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+
+
+def _reference(q, k, v, lengths, scale, window, sinks, dout, half):
+    """float64: (values, tolerances), each (out, dq, dk, dv)."""
+    u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[half]
+    sub = 2.0 ** -25 if half == torch.float16 else 0.0
+    q, k, v, dout = (t.detach().double().cpu().transpose(0, 1) for t in (q, k, v, dout))
+    group = q.shape[0] // k.shape[0]
+    vals = [torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)]
+    tols = [torch.zeros_like(t) for t in vals]
+    s0 = 0
+    for n in lengths:
+        rows = slice(s0, s0 + n)
+        s0 += n
+        i = torch.arange(n)
+        seen = (i[None] <= i[:, None]) & ((i[:, None] - i[None] < window) | (i[None] < sinks))
+        for h in range(q.shape[0]):
+            qh, kh, vh, g = q[h, rows], k[h // group, rows], v[h // group, rows], dout[h, rows]
+            if n == 0:
+                continue
+            s = (scale * qh @ kh.T).masked_fill(~seen, -math.inf)
+            p = torch.softmax(s, -1)
+            rel = 128 * 2.0 ** -24 * (scale * qh.abs() @ kh.abs().T).max().item() + 2.0 ** -19
+            o = p @ vh
+            ds = p * (g @ vh.T - (g * o).sum(-1, keepdim=True))
+            tol_o = (u + 2 * rel) * (p @ vh.abs()) + u * o.abs() + sub * n * vh.abs().max()
+            tol_d = (g.abs() * tol_o).sum(-1, keepdim=True)
+            tol_dp = 128 * 2.0 ** -24 * (g.abs() @ vh.abs().T)
+            tol_ds = ((u + 2 * rel) * ds.abs() + p * (tol_d + tol_dp) + sub) * seen
+            vals[0][h, rows] = o
+            vals[1][h, rows] = scale * ds @ kh
+            vals[2][h // group, rows] += scale * ds.T @ qh
+            vals[3][h // group, rows] += p.T @ g
+            tols[0][h, rows] = tol_o
+            tols[1][h, rows] = scale * tol_ds @ kh.abs()
+            tols[2][h // group, rows] += scale * tol_ds.T @ qh.abs()
+            tols[3][h // group, rows] += (u + 2 * rel) * p.T @ g.abs() + sub * (seen.double().T @ g.abs())
+    # the roundings of the results (out's is in already): u relative, or half of fp16's subnormal
+    # spacing 2^-24 for values below 2^-14, whose rounding is not relative
+    for i, (t, val) in enumerate(zip(tols, vals)):
+        t += (u * val.abs() if i else 0.0) + sub
+    return [t.transpose(0, 1) for t in vals], [t.transpose(0, 1) for t in tols]
+
+
+def _inputs(n, hq, hkv, half, strided, seed):
+    g = torch.Generator("cpu").manual_seed(seed)
+    if strided:  # column views of one [N, q + k + v] buffer
+        qkv = torch.randn(n, (hq + 2 * hkv) * D, generator=g).to(half).cuda()
+        q, k, v = (t.view(n, -1, D) for t in qkv.split([hq * D, hkv * D, hkv * D], 1))
+    else:
+        q, k, v = (torch.randn(n, h, D, generator=g).to(half).cuda() for h in (hq, hkv, hkv))
+    return q, k, v, torch.randn(n, hq, D, generator=g).to(half).cuda()
+
+
+def _call(q, k, v, cu, longest, window, sinks, dout=None, scale=D ** -0.5):
+    from talm_amd.unpad import window_attention
+
+    leaves = [t.transpose(0, 1)[None].detach().requires_grad_() for t in (q, k, v)]
+    out = window_attention(*leaves, cu, longest, scale, window, sinks)
+    if dout is None:
+        return out[0].detach()
+    grads = torch.autograd.grad(out, leaves, dout[None])
+    return [out[0].detach()] + [g[0].transpose(0, 1) for g in grads]
+
+
+def _cu(lengths):
+    return torch.tensor([0] + lengths).cumsum(0).to(torch.int32).cuda()
+
+
+def _check(lengths, window, sinks, hq, hkv, half=torch.float16, strided=True, seed=1):
+    print(f"[case] window lengths={lengths if len(lengths) < 12 else len(lengths)} window={window} "
+          f"sinks={sinks} heads={hq}/{hkv} {half} strided={strided} seed={seed}", flush=True)
+    q, k, v, dout = _inputs(sum(lengths), hq, hkv, half, strided, seed)
+    got = _call(q, k, v, _cu(lengths), max(lengths), window, sinks, dout)
+    vals, tols = _reference(q, k, v, lengths, D ** -0.5, window, sinks, dout, half)
+    for name, a, b, tol in zip(("out", "dq", "dk", "dv"), got, vals, tols):
+        err = (a.double().cpu() - b).abs()
+        ratio = err / tol.clamp_min(1e-30)
+        worst, at = ratio.max().item(), int(ratio.argmax())
+        print(f"  worst at {at}: {a.flatten()[at].item():.9g} for {b.flatten()[at].item():.9g}")
+        print(f"  {name}: max err {err.max():.3e}, {worst:.3f} of its tolerance", flush=True)
+        assert a.dtype == half and worst <= 1.0, name
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (5, 2), (64, 0), (65, 4), (1000, 0), (2 ** 31 - 1, 7)])
+def test_window_short_rows(window, sinks):
+    """From a row of its own token alone to windows wider than every row, at tile borders."""
+    _check([1, 17, 64, 65, 129], window, sinks, 4, 2, strided=False)
+
+
+@pytest.mark.parametrize("lengths,window,sinks,hq,hkv", [
+    ([300, 128, 512, 257], 100, 4, 12, 2),
+    ([700], 33, 65, 4, 1),             # sinks over a tile's border and wider than the window
+    ([700, 650], 20, 200, 2, 1),       # sinks in two key tiles of the backward
+    ([0, 5, 0, 130, 0], 16, 3, 7, 1),  # sequences without a token
+    ([1200], 900, 0, 2, 1),            # few workgroups and a long chain: the key tiles split in two
+    ([1500, 64], 700, 5, 4, 4),
+    ([130, 127, 128, 129], 128, 0, 7, 1),
+    ([40, 64, 16, 33], 9, 1, 12, 4),   # three heads a workgroup
+])
+@pytest.mark.parametrize("half", [torch.float16, torch.bfloat16])
+def test_window_matches_its_formula(lengths, window, sinks, hq, hkv, half):
+    _check(lengths, window, sinks, hq, hkv, half)
+
+
+@pytest.mark.parametrize("window,sinks", [(70, 3), (513, 130)])
+def test_sinks_gradient_over_several_chunks(window, sinks):
+    """Rows far past the window, whose sinks' gradients come from several chunks of rows."""
+    _check([2300, 1000], window, sinks, 2, 1)
+
+
+@pytest.mark.parametrize("sinks", [0, 6])
+def test_window_from_the_work_queue(sinks):
+    """More work items than two per CU: the backward's queue (and its items without a row)."""
+    _check([150 + 7 * (i % 9) for i in range(20)] + [900], 60, sinks, 16, 16, seed=5)
+
+
+def test_many_sequences_one_workgroup_per_item():
+    """More sequences than the queue takes."""
+    _check([30 + i % 50 for i in range(70)], 24, 2, 2, 1, seed=6)
+
+
+def test_a_window_of_the_whole_row_is_the_causal_attention():
+    """Two kernels, each off the formula by at most the tolerance (the compiler contracts their products
+    and sums differently, so not the same bits): apart by at most twice as much."""
+    from talm_amd.unpad import VarlenAttention
+
+    lengths = [300, 77, 513]
+    q, k, v, dout = _inputs(sum(lengths), 12, 2, torch.float16, True, 9)
+    got = _call(q, k, v, _cu(lengths), 513, 513, 0, dout)
+    leaves = [t.transpose(0, 1)[None].detach().requires_grad_() for t in (q, k, v)]
+    out = VarlenAttention.apply(*leaves, _cu(lengths), 513, D ** -0.5)
+    want = [out[0]] + [g[0].transpose(0, 1) for g in torch.autograd.grad(out, leaves, dout[None])]
+    _, tols = _reference(q, k, v, lengths, D ** -0.5, 513, 0, dout, torch.float16)
+    for a, b, tol in zip(got, want, tols):
+        assert ((a.double() - b.double()).abs().cpu() <= 2 * tol).all()
+
+
+def test_gradients_against_differences():
+    """The directional derivative of sum(out g) along a random direction of q, k and v, against a
+    central difference of step h = 2^-4: its truncation is h^2 / 6 of the third derivative, its
+    rounding error that of two fp16 outputs, sqrt(N) 2^-12 |out| |g| / (sqrt(3) h) if independent; both
+    within 2% of the derivative's own scale |grad| |direction| / sqrt(count), taken five times."""
+    lengths, window, sinks = [200, 90], 40, 3
+    q, k, v, dout = _inputs(290, 4, 2, torch.float16, False, 13)
+    cu = _cu(lengths)
+    _, *grads = _call(q, k, v, cu, 200, window, sinks, dout)
+    gen = torch.Generator("cpu").manual_seed(14)
+    for which in range(3):
+        ops = [q, k, v]
+        d = torch.randn(ops[which].shape, generator=gen).cuda()
+        vals, steps = [], []
+        for sign in (1, -1):
+            moved = list(ops)
+            moved[which] = (ops[which].float() + sign * 2.0 ** -4 * d).half()
+            steps.append(moved[which].double())
+            vals.append((_call(*moved, cu, 200, window, sinks).double() * dout.double()).sum())
+        # along the step that was taken (its ends are rounded to fp16)
+        along = (grads[which].double() * (steps[0] - steps[1])).sum()
+        scale = grads[which].double().norm() * (steps[0] - steps[1]).norm() / 1.0
+        assert abs((vals[0] - vals[1]) - along) <= 0.02 * scale, which
+
+
+def test_rows_behind_the_last_sequence():
+    """They are left as they were in an output that the caller gives, and get zero gradients."""
+    from talm_amd import _ops
+
+    q, k, v, dout = _inputs(200, 4, 2, torch.float16, True, 3)
+    cu = _cu([100, 60])
+    out = torch.full((200, 4, D), 7.0, dtype=torch.float16, device="cuda")
+    lse = torch.full((4, 200), 3.0, device="cuda")
+    torch.ops.talm.attn_window_fwd(q, k, v, cu, 100, 0.1, 20, 2, out, lse)
+    assert (out[160:] == 7).all() and (lse[:, 160:] == 3).all() and not (out[:160] == 7).any()
+    dq, dk, dv = (torch.full_like(t, 5.0).contiguous() for t in (q, k, v))
+    ws = torch.full((_ops.attn_window_bwd_workspace_bytes(200, 4, 2, 100, 20, 2),), 255, dtype=torch.uint8,
+                    device="cuda")  # NaN wherever it is read unwritten
+    torch.ops.talm.attn_window_bwd(q, k, v, out, dout, lse, cu, 100, 0.1, 20, 2, None, None, dq, dk, dv, ws)
+    for t in (dq, dk, dv):
+        assert (t[160:] == 0).all() and torch.isfinite(t).all()
+
+
+def test_keys_outside_every_window_tile_are_not_read():
+    """Infinities in k and v where no row of another tile sees them reach no other row."""
+    q, k, v, _ = _inputs(512, 2, 1, torch.float16, False, 8)
+    want = _call(q, k, v, _cu([512]), 512, 32, 0)
+    k, v = k.clone(), v.clone()
+    k[:64], v[:64] = math.inf, math.nan
+    got = _call(q, k, v, _cu([512]), 512, 32, 0)
+    assert torch.equal(got[192:], want[192:])
+
+
+def test_refusals_on_the_gpu():
+    from talm_amd.unpad import window_attention
+
+    q, k, v, _ = _inputs(64, 4, 2, torch.float16, False, 2)
+    a = [t.transpose(0, 1)[None] for t in (q, k, v)]
+    cu = _cu([64])
+    for args in ((a[0], a[1].float(), a[2], cu, 64, 0.1, 4), (a[0][..., :64], a[1][..., :64], a[2][..., :64], cu, 64, 0.1, 4),
+                 (a[0], a[1], a[2][:, :1], cu, 64, 0.1, 4), (*a, cu.long(), 64, 0.1, 4),
+                 (*a, cu.cpu(), 64, 0.1, 4), (*a, cu, 64, 0.1, 0), (*a, cu, 64, 0.0, 4),
+                 (*a, cu, 64, 0.1, 4, -1), (*a, cu, -1, 0.1, 4)):
+        with pytest.raises(ValueError):
+            window_attention(*args)
+
+
+def test_odd_strides_and_another_stream():
+    """Views that the kernels cannot read are copied; the operands' current stream is used."""
+    q, k, v, dout = _inputs(150, 4, 2, torch.float16, False, 4)
+    want = _call(q, k, v, _cu([150]), 150, 33, 1, dout)
+    wide = [torch.empty(150, t.shape[1], D + 1, dtype=t.dtype, device="cuda") for t in (q, k, v)]
+    for w, t in zip(wide, (q, k, v)):
+        w[..., 1:] = t
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _call(*[w[..., 1:] for w in wide], _cu([150]), 150, 33, 1, dout)
+    side.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_captured_forward_and_backward_replay():
+    """Replays follow new inputs and new lengths, with eager work between them."""
+    q, k, v, dout = _inputs(640, 4, 2, torch.float16, True, 21)
+    cu = _cu([300, 200, 140])
+    static = [t.clone() for t in (q, k, v, dout)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        _call(*static[:3], cu, 640, 50, 3, static[3])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = _call(*static[:3], cu, 640, 50, 3, static[3])
+    for seed, lengths in ((31, [640, 0, 0]), (32, [1, 400, 239]), (33, [300, 200, 140]), (34, [64, 512, 64])):
+        fresh = _inputs(640, 4, 2, torch.float16, True, seed)
+        for s, t in zip(static, fresh):
+            s.copy_(t)
+        cu.copy_(_cu(lengths))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = _call(*fresh[:3], _cu(lengths), 640, 50, 3, fresh[3])
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)

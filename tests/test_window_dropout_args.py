@@ -1,0 +1,166 @@
+"""Argument checks of the sliding-window attention, the counter-based dropout with the adapters'
+products, and the few-token 4-bit products: rejected before anything touches a GPU. The
+generator of the oracle against its authors' known answers, the masks' counters and shares."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import philox
+from talm_amd import _lib, _ops, dropout, lora, unpad
+
+PTR = 1 << 12  # a fake address: never dereferenced on rejection
+
+
+def _status(name, *args):
+    lib = _lib.lib()
+    status = getattr(lib, name)(*args)
+    return status, lib.talm_last_error().decode()
+
+
+@pytest.mark.parametrize("counter,key,words", [
+    ((0, 0, 0, 0), (0, 0), (0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8)),
+    ((0xffffffff,) * 4, (0xffffffff,) * 2, (0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd)),
+    ((0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344), (0xa4093822, 0x299f31d0),
+     (0xd16cfe09, 0x94fdcceb, 0x5001e420, 0x24126ea1)),
+])
+def test_oracle_generator_has_the_published_answers(counter, key, words):
+    got = philox.philox4x32([np.array([c]) for c in counter], key)
+    assert tuple(int(w[0]) for w in got) == words
+
+
+def test_masks_differ_by_site_and_key_and_keep_the_stated_share():
+    n, p = 1 << 15, 0.25
+    a = philox.keep((5, 7), 32, n // 32, p, 0)
+    # 2^15 draws of probability 3/4: five standard deviations are 5 sqrt(n p (1 - p)) = 392
+    for other in (philox.keep((5, 7), 32, n // 32, p, 1), philox.keep((6, 7), 32, n // 32, p, 0),
+                  philox.keep((5, 8), 32, n // 32, p, 0)):
+        assert abs(int(other.sum()) - 0.75 * n) < 392
+        # independent masks agree on p^2 + (1 - p)^2 = 0.625 of the elements: sd = sqrt(n .625 .375)
+        assert abs(int((a == other).sum()) - 0.625 * n) < 5 * np.sqrt(n * 0.625 * 0.375)
+    assert philox.keep((5, 7), 3, 13, 0.0).all()
+    assert philox.threshold(0.99999999) == 65535  # never everything
+
+
+# (position of the argument, its bad value, a word of the message) on an otherwise good call
+def _window(**bad):
+    v = dict(tok=256, cu=PTR, seqs=1, longest=8, n=8, hq=2, hkv=1, d=128, scale=1.0, window=4,
+             sinks=0, dtype=_lib.TALM_F16, q=PTR)
+    v.update(bad)
+    return _status("talm_attn_window_fwd", v["q"], v["tok"], 128, PTR, 128, 128, PTR, 128, 128,
+                   v["cu"], v["seqs"], v["longest"], v["n"], v["hq"], v["hkv"], v["d"], v["scale"],
+                   v["window"], v["sinks"], v["dtype"], PTR, 256, 128, PTR, None)
+
+
+@pytest.mark.parametrize("bad,word", [
+    ({"window": 0}, "window"), ({"window": -3}, "window"), ({"sinks": -1}, "sinks"),
+    ({"dtype": _lib.TALM_F32}, "dtype"), ({"scale": 0.0}, "scale"), ({"scale": -1.0}, "scale"),
+    ({"scale": float("inf")}, "scale"), ({"scale": float("nan")}, "scale"), ({"d": 64}, "head_dim"),
+    ({"hq": 3, "hkv": 2}, "shape"), ({"tok": 130}, "multiples of 8"), ({"q": None}, "null"),
+    ({"q": PTR + 8}, "16-byte"), ({"cu": None}, "null"),
+])
+def test_window_forward_rejects(bad, word):
+    status, message = _window(**bad)
+    assert status == _lib.TALM_EINVAL and word in message and "attn_window_fwd" in message
+
+
+def test_window_backward_rejects_a_short_workspace():
+    need = _ops.attn_window_bwd_workspace_bytes(4096, 2, 1, 4096, 64, 4)
+    assert need > _ops.attn_bwd_workspace_bytes(4096, 2)
+    assert _ops.attn_window_bwd_workspace_bytes(4096, 2, 1, 4096, 64, 0) == \
+        _ops.attn_bwd_workspace_bytes(4096, 2)
+    with pytest.raises(ValueError):
+        _ops.attn_window_bwd_workspace_bytes(4096, 2, 1, 4096, 0, 4)
+    rows = [PTR, 256, 128]
+    status, message = _status(
+        "talm_attn_window_bwd", *rows, *[PTR, 128, 128] * 2, *rows, *rows, PTR, PTR, 1, 4096, 4096, 2,
+        1, 128, 1.0, 64, 4, _lib.TALM_F16, None, None, 0, *rows, *[PTR, 128, 128] * 2, PTR,
+        need - 512, None)
+    assert status == _lib.TALM_EINVAL and "workspace" in message
+
+
+def test_window_workspace_of_many_sinks_is_bounded():
+    """The sinks' partials stay within 64 MiB, or one chunk where that alone is more."""
+    for seqs, longest, sinks in ((1, 100000, 4), (64, 4096, 200), (64, 8192, 4), (4, 4096, 4096)):
+        extra = _ops.attn_window_bwd_workspace_bytes(0, 12, seqs, longest, 64, sinks) \
+            - _ops.attn_bwd_workspace_bytes(0, 12)
+        one = seqs * 12 * min(sinks, longest) * 128 * 8
+        assert 0 < extra <= max(64 << 20, one)
+
+
+def test_window_attention_rejects_cpu_tensors_and_bad_arguments():
+    q = torch.zeros(1, 2, 8, 128, dtype=torch.float16)
+    cu = torch.tensor([0, 8], dtype=torch.int32)
+    with pytest.raises(ValueError, match="GPU"):
+        unpad.window_attention(q, q[:, :1], q[:, :1], cu, 8, 1.0, 4)
+
+
+@pytest.mark.parametrize("args,word", [
+    ((PTR, 8, 4, 8, _lib.TALM_F16, 1.0, PTR, 0, PTR, 8), "p 1"),
+    ((PTR, 8, 4, 8, _lib.TALM_F16, -0.1, PTR, 0, PTR, 8), "p -0.1"),
+    ((PTR, 8, 4, 8, _lib.TALM_F16, float("nan"), PTR, 0, PTR, 8), "p nan"),
+    ((PTR, 8, 4, 8, _lib.TALM_F16, 0.5, None, 0, PTR, 8), "key"),
+    ((PTR, 8, 4, 8, _lib.TALM_F16, 0.5, PTR + 4, 0, PTR, 8), "key"),
+    ((PTR, 7, 4, 8, _lib.TALM_F16, 0.5, PTR, 0, PTR, 8), "shape"),
+    ((PTR, 8, 4, 8, 7, 0.5, PTR, 0, PTR, 8), "dtype"),
+    ((None, 8, 4, 8, _lib.TALM_F16, 0.5, PTR, 0, PTR, 8), "null"),
+])
+def test_dropout_rejects(args, word):
+    status, message = _status("talm_dropout", *args, None)
+    assert status == _lib.TALM_EINVAL and word in message
+
+
+def test_dropout_of_nothing_is_no_launch():
+    assert _status("talm_dropout", None, 8, 0, 8, 1, 0.5, PTR, 0, None, 8, None)[0] == _lib.TALM_OK
+
+
+def test_python_entries_reject():
+    x = torch.zeros(4, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="GPU"):
+        dropout.dropout(x, 0.5, torch.zeros(2, dtype=torch.int64))
+    with pytest.raises(ValueError, match="adapter_branch"):
+        lora.adapter_branch(x, torch.zeros(16, 64), torch.zeros(32, 16), 2.0)
+    with pytest.raises(ValueError, match="key is needed"):
+        dropout.check(x, 0.5, None, 0)
+    with pytest.raises(ValueError, match="int64"):
+        dropout.check(x, 0.5, torch.zeros(2), 0)
+    with pytest.raises(ValueError, match="int64"):
+        dropout.check(x, 0.5, torch.zeros(3, dtype=torch.int64), 0)
+    with pytest.raises(ValueError, match="site"):
+        dropout.check(x, 0.5, torch.zeros(2, dtype=torch.int64), 2 ** 32)
+    with pytest.raises(ValueError, match="p 1.0"):
+        dropout.check(x, 1.0, torch.zeros(2, dtype=torch.int64), 0)
+
+
+@pytest.mark.parametrize("k,ldx,adapters,word", [(40, 40, 1, "multiple of 32"), (64, 60, 1, "shape"),
+                                                 (64, 64, 3, "shape"), (64, 66, 1, "shape")])
+def test_adapter_down_rejects(k, ldx, adapters, word):
+    status, message = _status("talm_lora_down_drop", PTR, ldx, 4, k, PTR, PTR, adapters, 0.5, PTR, 0,
+                              1, 1.0, 1.0, PTR, PTR, 32, None, 0, None)
+    assert status == _lib.TALM_EINVAL and word in message
+
+
+@pytest.mark.parametrize("cols,ldo,word", [(12, 16, "multiples of 8"), (16, 12, "shape"), (16, 8, "shape")])
+def test_adapter_up_rejects(cols, ldo, word):
+    status, message = _status("talm_lora_up", PTR, 16, 4, cols, PTR, None, 1, 0, 0.0, None, 0, 0, None,
+                              0, PTR, ldo, None)
+    assert status == _lib.TALM_EINVAL and word in message
+
+
+def test_adapter_weight_gradient_rejects():
+    def call(hidden=64, seg=32, ws=1 << 20, dtype=_lib.TALM_F32, lo=0):
+        return _status("talm_lora_wgrad_drop", PTR, 64, PTR, 32, PTR, 16, PTR, 16, 4, hidden, 1, 0.5,
+                       PTR, 0, 1, dtype, lo, seg, 1.0, PTR, PTR, 0, 0, 0.0, None, None, PTR, ws, None)
+    for kwargs, word in (({"hidden": 60}, "shape"), ({"seg": 40}, "shape"), ({"ws": 64}, "workspace"),
+                         ({"dtype": 2}, "dtype"), ({"lo": 8}, "shape")):
+        status, message = call(**kwargs)
+        assert status == _lib.TALM_EINVAL and word in message, kwargs
+
+
+@pytest.mark.parametrize("tokens,cols,qblock,qblock2,word", [
+    (33, 128, 64, 256, "32 tokens"), (1, 96, 64, 256, "shape"), (1, 128, 32, 256, "blocks"),
+    (1, 128, 64, 200, "blocks"), (-1, 128, 64, 256, "shape")])
+def test_gemv_rejects(tokens, cols, qblock, qblock2, word):
+    status, message = _status("talm_nf4_gemv", PTR, 128, tokens, PTR, PTR, PTR, PTR, PTR, 128, cols,
+                              qblock, qblock2, None, PTR, 128, None)
+    assert status == _lib.TALM_EINVAL and word in message
