@@ -21,6 +21,8 @@
 #include <hipblaslt/hipblaslt-ext.hpp>
 #include <hipblaslt/hipblaslt.h>
 #include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 
 #include <atomic>
@@ -921,6 +923,241 @@ void nf4_gemv(const Tensor& x, const Tensor& packed, const Tensor& absmax8, cons
 }
 
 // ------------------------------------------------------------------------------------------
+// Differentiable forms of the ops above. They are autograd nodes in C++ because their calls are
+// short: a forward and backward through a Python torch.autograd.Function costs 85 to 150 us of host
+// time, several times the kernels' (MI355X, 131 rows: dropout 87 us, an adapter's branch 148 us).
+// ------------------------------------------------------------------------------------------
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// A node's gradients, for a backward that is not itself differentiable: under create_graph a second
+// backward through them is an error, not zeros.
+variable_list once(variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list fake;
+  for (Tensor& g : grads) fake.push_back(g.defined() ? g.detach().requires_grad_() : g);
+  auto error = std::make_shared<torch::autograd::DelayedError>(
+      "this operator is differentiable once: its gradient has no backward", static_cast<int64_t>(fake.size()));
+  error->set_next_edges(torch::autograd::collect_next_edges(fake));
+  return (*error)(std::move(fake));
+}
+
+Tensor byte_workspace(int64_t bytes, const Tensor& like, const char* what) {
+  TORCH_CHECK_VALUE(bytes >= 0, what, ": unsupported shape");
+  return at::empty({bytes}, like.options().dtype(at::kByte));
+}
+
+// [1, H, N, D] -> an [N, H, D] view that the window kernels read (a copy only when it must be).
+Tensor head_rows(const Tensor& t) {
+  Tensor r = t.squeeze(0).transpose(0, 1);
+  if (r.stride(2) != 1 || r.stride(0) % 8 || r.stride(1) % 8 || reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 ||
+      r.stride(0) >= (int64_t{1} << 23))
+    r = r.clone(at::MemoryFormat::Contiguous);
+  return r;
+}
+
+struct WindowAttention : torch::autograd::Function<WindowAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& query, const Tensor& key, const Tensor& value,
+                        const Tensor& cu, int64_t max_len, double scale, int64_t window, int64_t sinks) {
+    const Tensor q = head_rows(query), k = head_rows(key), v = head_rows(value);
+    const Tensor out = at::empty(q.sizes(), q.options());
+    const Tensor lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+    attn_window_fwd(q, k, v, cu, max_len, scale, window, sinks, out, lse);
+    ctx->save_for_backward({q, k, v, out, lse, cu});
+    ctx->saved_data["max_len"] = max_len;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    return out.unsqueeze(0);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4], &cu = saved[5];
+    const int64_t max_len = ctx->saved_data["max_len"].toInt(), window = ctx->saved_data["window"].toInt(),
+                  sinks = ctx->saved_data["sinks"].toInt();
+    variable_list in(8);
+    {
+      at::AutoGradMode off(false);
+      const Tensor g = head_rows(grads[0].transpose(1, 2));
+      const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()),
+                   dv = at::empty(v.sizes(), v.options());
+      const Tensor ws = byte_workspace(
+          talm_attn_window_bwd_workspace(q.size(0), int32_arg(q.size(1), "heads"),
+                                         int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_len, "max_len"),
+                                         int32_arg(window, "window"), int32_arg(sinks, "sinks")),
+          q, "window_attention");
+      attn_window_bwd(q, k, v, out, g, lse, cu, max_len, ctx->saved_data["scale"].toDouble(), window, sinks,
+                      std::nullopt, std::nullopt, dq, dk, dv, ws);
+      in[0] = dq.transpose(0, 1).unsqueeze(0);
+      in[1] = dk.transpose(0, 1).unsqueeze(0);
+      in[2] = dv.transpose(0, 1).unsqueeze(0);
+    }
+    return once(std::move(in));
+  }
+};
+
+// query [1, Hq, N, 128], key / value [1, Hkv, N, 128]; returns [1, N, Hq, 128].
+Tensor window_attention(const Tensor& query, const Tensor& key, const Tensor& value, const Tensor& cu,
+                        int64_t max_len, double scale, int64_t window, int64_t sinks) {
+  const at::ScalarType type = query.scalar_type();
+  auto ok = [&](const Tensor& t) {
+    return t.is_cuda() && t.device() == query.device() && t.scalar_type() == type && t.dim() == 4 &&
+           t.size(0) == 1 && t.size(1) > 0 && t.size(2) == query.size(2) && t.size(3) == 128;
+  };
+  require((type == at::kHalf || type == at::kBFloat16) && query.dim() == 4 && ok(query) && ok(key) && ok(value) &&
+              key.size(1) == value.size(1) && query.size(1) % key.size(1) == 0,
+          "window_attention: query [1, Hq, N, 128], key / value [1, Hkv, N, 128], fp16 or bf16 of one type and "
+          "device on the GPU, Hq a multiple of Hkv");
+  require(cu.is_cuda() && cu.scalar_type() == at::kInt && cu.dim() == 1 && cu.numel() >= 1 && cu.is_contiguous() &&
+              cu.device() == query.device(),
+          "window_attention: cu int32 [sequences + 1] on the operands' device");
+  TORCH_CHECK_VALUE(max_len >= 0 && window >= 1 && sinks >= 0, "window_attention: max_len ", max_len, ", window ",
+                    window, " (at least 1), sinks ", sinks);
+  TORCH_CHECK_VALUE(scale > 0.0 && scale < std::numeric_limits<double>::infinity(), "window_attention: scale ", scale,
+                    " (positive, finite)");
+  // no sequence is longer than the rows: larger values mean the same
+  const int64_t n = query.size(2);
+  return WindowAttention::apply(query, key, value, cu, std::min(max_len, n), scale,
+                                std::min(window, std::max<int64_t>(n, 1)), std::min(sinks, n));
+}
+
+void drop_args(const Tensor& x, double p, const OptTensor& key, int64_t site) {
+  TORCH_CHECK_VALUE(p >= 0.0 && p < 1.0, "dropout: p ", p, " (0 <= p < 1)");
+  require(key.has_value() || p == 0.0, "dropout: a key is needed (draw_key)");
+  drop_key(key, x);
+  drop_site(site);
+}
+
+// x with its dropped elements zero, as rows of its last dimension.
+Tensor dropped(const Tensor& x, double p, const OptTensor& key, int64_t site) {
+  const Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  if (x.numel() == 0) return y;
+  const int64_t cols = x.dim() ? x.size(-1) : 1;
+  Tensor x2 = x.reshape({-1, cols});
+  if ((cols > 1 && x2.stride(1) != 1) || (x2.size(0) > 1 && x2.stride(0) < cols)) x2 = x2.contiguous();
+  dropout(x2, p, key, site, y.view({-1, cols}));
+  return y;
+}
+
+struct CounterDropout : torch::autograd::Function<CounterDropout> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, double p, const OptTensor& key, int64_t site) {
+    ctx->save_for_backward({key.has_value() ? *key : Tensor()});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["site"] = site;
+    return dropped(x, p, key, site);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor key = ctx->get_saved_variables()[0];
+    variable_list in(4);
+    {
+      at::AutoGradMode off(false);
+      in[0] = dropped(grads[0], ctx->saved_data["p"].toDouble(), key.defined() ? OptTensor(key) : OptTensor(),
+                      ctx->saved_data["site"].toInt());
+    }
+    return once(std::move(in));
+  }
+};
+
+Tensor counter_dropout(const Tensor& x, double p, const OptTensor& key, int64_t site) {
+  require(x.is_cuda() && (x.scalar_type() == at::kFloat || x.scalar_type() == at::kHalf ||
+                          x.scalar_type() == at::kBFloat16),
+          "dropout: a float32, float16 or bfloat16 tensor on the GPU");
+  drop_args(x, p, key, site);
+  return CounterDropout::apply(x, p, key, site);
+}
+
+// [..., C] as [N, C] rows that the adapters' kernels read: unit column stride, 16-byte aligned rows.
+Tensor aligned_rows(const Tensor& t) {
+  Tensor r = t.reshape({t.size(-1) ? t.numel() / t.size(-1) : 0, t.size(-1)});
+  if ((r.size(1) > 1 && r.stride(1) != 1) || (r.size(0) > 1 && (r.stride(0) % 8 || r.stride(0) < r.size(1))) ||
+      reinterpret_cast<uintptr_t>(r.data_ptr()) % 16)
+    r = r.clone(at::MemoryFormat::Contiguous);
+  return r;
+}
+
+Tensor adapter_half(const Tensor& w) {
+  const Tensor h = w.to(at::kHalf);
+  return h.is_contiguous() && reinterpret_cast<uintptr_t>(h.data_ptr()) % 16 == 0
+             ? h
+             : h.clone(at::MemoryFormat::Contiguous);
+}
+
+// scaling * B(A(dropout(x))) and its gradients, the mask computed in each product.
+struct AdapterBranch : torch::autograd::Function<AdapterBranch> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& lora_a, const Tensor& lora_b,
+                        const Tensor& a_half, const Tensor& b_half, const OptTensor& key, double scaling, double p,
+                        int64_t site) {
+    const Tensor x2 = aligned_rows(x), a = adapter_half(a_half), b = adapter_half(b_half);
+    const int64_t n = x2.size(0), out = b.size(0);
+    const Tensor t = at::empty({n, 16}, x2.options()), ts = at::empty({n, 16}, x2.options());
+    const Tensor y = at::empty({n, out}, x2.options());
+    const int64_t bytes = talm_lora_down_drop_workspace(n, x2.size(1), 1);
+    lora_down_drop(x2, a, std::nullopt, p, key, site, 0, scaling, 0.0, t, ts,
+                   bytes ? OptTensor(byte_workspace(bytes, x2, "adapter_branch")) : OptTensor());
+    lora_up(ts, b, std::nullopt, false, 0.0, std::nullopt, 0, 0, std::nullopt, y);
+    ctx->save_for_backward({x2, a, b, t, key.has_value() ? *key : Tensor()});
+    ctx->saved_data["scaling"] = scaling;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["site"] = site;
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["type"] = lora_a.scalar_type();
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = out;
+    return y.view(shape);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &a = saved[1], &b = saved[2], &t = saved[3];
+    const OptTensor key = saved[4].defined() ? OptTensor(saved[4]) : OptTensor();
+    const double scaling = ctx->saved_data["scaling"].toDouble(), p = ctx->saved_data["p"].toDouble();
+    const int64_t site = ctx->saved_data["site"].toInt();
+    variable_list in(9);
+    {
+      at::AutoGradMode off(false);
+      const Tensor dy = aligned_rows(grads[0].to(at::kHalf));
+      const int64_t n = x.size(0), size = x.size(1), out = b.size(0);
+      const Tensor u_raw = at::empty(t.sizes(), t.options()), u = at::empty(t.sizes(), t.options());
+      adapter_u(dy, b, scaling, u_raw, u);
+      if (ctx->needs_input_grad(0)) {
+        const Tensor dx = at::empty({n, size}, x.options());
+        lora_up(u, a, std::nullopt, true, p, key, site, 0, std::nullopt, dx);
+        in[0] = dx.view(ctx->saved_data["shape"].toIntVector());
+      }
+      if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
+        const auto options = x.options().dtype(ctx->saved_data["type"].toScalarType());
+        in[1] = at::empty({16, size}, options);
+        in[2] = at::empty({out, 16}, options);
+        lora_wgrad_drop(x, dy, u, t, p, key, site, 0, 0, out, scaling, in[1], in[2], 0, 0, 0.0, std::nullopt,
+                        std::nullopt,
+                        byte_workspace(talm_lora_wgrad_drop_workspace(n, size, 1, out, 0), x, "adapter_branch"));
+      }
+    }
+    return once(std::move(in));
+  }
+  // u = scaling dy B (and B's unscaled product, which the kernel writes too)
+  static void adapter_u(const Tensor& dy, const Tensor& b, double scaling, const Tensor& u_raw, const Tensor& u) {
+    lora_down(dy, b, std::nullopt, b.size(0), 0, 0, 0, 1, scaling, 0.0, u_raw, u);
+  }
+};
+
+// x fp16 [..., in], lora_a [16, in] and lora_b [out, 16] (the leaves), a_half and b_half their fp16 values
+// (or themselves).
+Tensor adapter_branch(const Tensor& x, const Tensor& lora_a, const Tensor& lora_b, const Tensor& a_half,
+                      const Tensor& b_half, double scaling, double p, const OptTensor& key, int64_t site) {
+  const at::ScalarType type = lora_a.scalar_type();
+  require(x.is_cuda() && x.scalar_type() == at::kHalf && x.dim() >= 1 && lora_a.dim() == 2 && lora_b.dim() == 2 &&
+              lora_a.device() == x.device() && lora_b.device() == x.device() && lora_b.scalar_type() == type &&
+              (type == at::kHalf || type == at::kFloat) && lora_a.size(0) == 16 && lora_b.size(1) == 16 &&
+              lora_a.size(1) == x.size(-1) && x.size(-1) % 32 == 0 && lora_b.size(0) % 32 == 0 && x.size(-1) > 0 &&
+              lora_b.size(0) > 0 && a_half.sizes() == lora_a.sizes() && b_half.sizes() == lora_b.sizes() &&
+              a_half.device() == x.device() && b_half.device() == x.device(),
+          "adapter_branch: fp16 x [..., in] on the GPU, A [16, in] and B [out, 16] of one type (fp16 or fp32) "
+          "there, in and out multiples of 32");
+  drop_args(x, p, key, site);
+  return AdapterBranch::apply(x, lora_a, lora_b, a_half.detach(), b_half.detach(), key, scaling, p, site);
+}
+
+// ------------------------------------------------------------------------------------------
 // LoRA adapters: fp16 copies and the fused AdamW step over a device table (9 int64 per tensor,
 // layout in include/talm.h; the addresses in it are the caller's to keep alive).
 // ------------------------------------------------------------------------------------------
@@ -1807,6 +2044,11 @@ TORCH_LIBRARY(talm, m) {
         "Tensor(a!) sum_out, Tensor(b!) h, Tensor(c!) xhat, Tensor(d!) rstd) -> ()");
   m.def("splitk_rmsnorm_bwd(Tensor partials, Tensor xhat, Tensor rstd, Tensor weight, "
         "Tensor? ds, Tensor(a!) dx, Tensor(b!) dbranch) -> ()");
+  m.def("window_attention(Tensor query, Tensor key, Tensor value, Tensor cu, int max_len, float scale, "
+        "int window, int sinks) -> Tensor", &window_attention);
+  m.def("counter_dropout(Tensor x, float p, Tensor? key, int site) -> Tensor", &counter_dropout);
+  m.def("adapter_branch(Tensor x, Tensor lora_a, Tensor lora_b, Tensor a_half, Tensor b_half, float scaling, "
+        "float p, Tensor? key, int site) -> Tensor", &adapter_branch);
   m.def("gemm_algo_table(Tensor rows) -> ()", &gemm_algo_table);
   m.def("gemm_lib_version() -> int", &gemm_lib_version);
   m.def("gemm_tune(Tensor a, int trans_a, Tensor b, int trans_b, Tensor(a!) d, int m, int n, "

@@ -31,49 +31,8 @@ def draw_key(device):
     return torch.randint(-2 ** 63, 2 ** 63 - 1, (2,), dtype=torch.int64, device=device)
 
 
-def check(x, p, key, site):
-    """The arguments' common checks (ValueError)."""
-    if not 0.0 <= p < 1.0:
-        raise ValueError(f"dropout: p {p} (0 <= p < 1)")
-    if key is None and p > 0.0:
-        raise ValueError("dropout: a key is needed (draw_key)")
-    if key is not None and (key.dtype != torch.int64 or key.numel() != 2
-                            or key.device != x.device or not key.is_contiguous()):
-        raise ValueError("dropout: key int64 [2], contiguous, on x's device")
-    if not 0 <= site < 2 ** 32:
-        raise ValueError(f"dropout: site {site} (0 .. 2^32 - 1)")
-
-
-def _apply(x, p, key, site):
-    if x.numel() == 0:
-        return torch.empty_like(x, memory_format=torch.contiguous_format)
-    x2 = x.reshape(-1, x.shape[-1] if x.dim() else 1)
-    if x2.shape[1] > 1 and x2.stride(1) != 1 or x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]:
-        x2 = x2.contiguous()
-    y = torch.empty(x2.shape, dtype=x.dtype, device=x.device)
-    torch.ops.talm.dropout(x2, p, key, site, y)
-    return y.view(x.shape)
-
-
-class Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, p, key, site):
-        ctx.p, ctx.site = p, site
-        ctx.save_for_backward(key)
-        return _apply(x, p, key, site)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        (key,) = ctx.saved_tensors
-        return _apply(grad, ctx.p, key, ctx.site), None, None, None
-
-
 def dropout(x, p, key=None, site=0):
     """x with each element dropped with probability p (in steps of 2^-16) and the others scaled by
-    the reciprocal of the share kept; float32, float16 or bfloat16 on the GPU."""
-    if not x.is_cuda or x.dtype not in (torch.float32, torch.float16, torch.bfloat16):
-        raise ValueError("dropout: a float32, float16 or bfloat16 tensor on the GPU")
-    p, site = float(p), int(site)
-    check(x, p, key, site)
-    return Dropout.apply(x, p, key, site)
+    the reciprocal of the share kept; float32, float16 or bfloat16 on the GPU, of any shape and
+    strides. An autograd node of the C++ op layer, differentiable once."""
+    return torch.ops.talm.counter_dropout(x, p, key, site)

@@ -25,9 +25,8 @@ from collections import namedtuple
 import torch
 import torch.nn as nn
 
-from . import _ops
+from . import _ops  # noqa: F401 - registers torch.ops.talm.*
 from .adapters import COPIES
-from .dropout import check as check_dropout
 from .engaged import FELL_BACK, ON, RAN
 from .state import DISABLED, fallback
 
@@ -182,83 +181,20 @@ def branch_takes(x, lora_a, lora_b):
             and lora_a.shape[1] % 32 == 0 and lora_b.shape[0] % 32 == 0)
 
 
-def _aligned_rows(t):
-    """t [..., C] as [N, C] rows the kernels read: unit column stride, 16-byte aligned rows."""
-    t2 = t.reshape(-1, t.shape[-1])
-    if t2.stride(-1) != 1 or t2.shape[0] > 1 and (t2.stride(0) % 8 or t2.stride(0) < t2.shape[1]) \
-            or t2.data_ptr() % 16:
-        t2 = t2.clone(memory_format=torch.contiguous_format)
-    return t2
-
-
-def _half_weight(w):
-    w = w.detach()
-    w = (COPIES.half(w) if _hooks else w.half()) if w.dtype == torch.float32 else w
-    return w if w.is_contiguous() and w.data_ptr() % 16 == 0 \
-        else w.clone(memory_format=torch.contiguous_format)
-
-
-class AdapterBranch(torch.autograd.Function):
-    """scaling * B(A(dropout(x))) and its gradients on MFMA, the dropout's mask computed in each
-    product from the key (talm_lora_down_drop, talm_lora_up, talm_lora_wgrad_drop): PEFT's branch
-    (solution/lora.py:183-231) without a dropped copy of x or a stored mask."""
-
-    @staticmethod
-    def forward(ctx, x, lora_a, lora_b, scaling, p, key, site):
-        x2, a16, b16 = _aligned_rows(x), _half_weight(lora_a), _half_weight(lora_b)
-        n = x2.shape[0]
-        t = torch.empty(n, 16, dtype=torch.float16, device=x.device)
-        ts = torch.empty_like(t)
-        y = torch.empty(n, b16.shape[0], dtype=torch.float16, device=x.device)
-        torch.ops.talm.lora_down_drop(x2, a16, None, p, key, site, 0, scaling, 0.0, t, ts,
-                                      _down_workspace(x2, 1))
-        torch.ops.talm.lora_up(ts, b16, None, False, 0.0, None, 0, 0, None, y)
-        ctx.save_for_backward(x2, a16, b16, t, key)
-        ctx.scaling, ctx.p, ctx.site, ctx.shape = scaling, p, site, x.shape
-        ctx.grad_dtype = lora_a.dtype
-        return y.view(*x.shape[:-1], b16.shape[0])
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        x2, a16, b16, t, key = ctx.saved_tensors
-        p, site, scaling = ctx.p, ctx.site, ctx.scaling
-        dy = _aligned_rows(grad.to(torch.float16))
-        n, size, out = x2.shape[0], x2.shape[1], b16.shape[0]
-        u_raw = torch.empty_like(t)
-        u = torch.empty_like(t)
-        torch.ops.talm.lora_down(dy, b16, None, out, 0, 0, 0, 1, scaling, 0.0, u_raw, u)
-        dx = da = db = None
-        if ctx.needs_input_grad[0]:
-            dx = torch.empty(n, size, dtype=torch.float16, device=x2.device)
-            torch.ops.talm.lora_up(u, a16, None, True, p, key, site, 0, None, dx)
-            dx = dx.view(ctx.shape)
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            da = torch.empty(16, size, dtype=ctx.grad_dtype, device=x2.device)
-            db = torch.empty(out, 16, dtype=ctx.grad_dtype, device=x2.device)
-            ws = torch.empty(_ops.lora_wgrad_drop_workspace_bytes(n, size, 1, out, 0),
-                             dtype=torch.uint8, device=x2.device)
-            torch.ops.talm.lora_wgrad_drop(x2, dy, u, t, p, key, site, 0, 0, out, scaling, da, db, 0,
-                                           0, 0.0, None, None, ws)
-        return (dx, da if ctx.needs_input_grad[1] else None,
-                db if ctx.needs_input_grad[2] else None, None, None, None, None)
-
-
-def _down_workspace(x2, n_adapters):
-    size = _ops.lora_down_drop_workspace_bytes(x2.shape[0], x2.shape[1], n_adapters)
-    return torch.empty(size, dtype=torch.uint8, device=x2.device) if size else None
+def _half(w):
+    """The fp16 values of an adapter weight that a forward reads (the shared copies of an fp32 one)."""
+    return COPIES.half(w) if _hooks and w.dtype == torch.float32 else w
 
 
 def adapter_branch(x, lora_a, lora_b, scaling, p=0.0, key=None, site=0):
     """A LoRA adapter's branch scaling * (dropout(x) A^T) B^T with gradients for x, A and B: x fp16
     [..., in], A [16, in] and B [out, 16] fp16 or fp32 (fp32 ones are read as fp16 copies, their
-    gradients fp32), in and out multiples of 32; the dropout as `dropout.dropout` on x's rows."""
-    if not branch_takes(x, lora_a, lora_b):
-        raise ValueError("adapter_branch: fp16 x [..., in] on the GPU, A [16, in] and B [out, 16] of one type "
-                         "(fp16 or fp32) there, in and out multiples of 32")
-    p, site = float(p), int(site)
-    check_dropout(x, p, key, site)
-    return AdapterBranch.apply(x, lora_a, lora_b, float(scaling), p, key, site)
+    gradients fp32), in and out multiples of 32; the dropout as `dropout.dropout` on x's rows, its mask
+    computed in each product (talm_lora_down_drop, talm_lora_up, talm_lora_wgrad_drop) and never
+    stored, no dropped copy of x: PEFT's branch (solution/lora.py:183-231) on MFMA. An autograd node
+    of the C++ op layer, differentiable once."""
+    return torch.ops.talm.adapter_branch(x, lora_a, lora_b, _half(lora_a), _half(lora_b), scaling, p,
+                                         key, site)
 
 
 def patch_lora():

@@ -160,6 +160,7 @@ class LayerGroup:
             .expand((seg.stop - seg.start) // span2) for s, seg in zip(states, segments)])
         self.modules = [weakref.ref(m) for m in modules]
         self._bias_spans = {}
+        self._gemv = {}
         self._scales = None
         self.t_layout = self._transposed_layout()
         # the reference's count of backward uses (solution/qgroup.py:179, :536): callers written
@@ -327,16 +328,22 @@ class LayerGroup:
         """out [M, sum of out] = x [M, in] W^T + the projections' biases for M <= GEMV_TOKENS rows, W
         the rows of projections first .. last - 1 read as NF4 codes (the fp16 weights of `span`, never
         written out). For calls that answer token by token; more rows: `nf4_gemm`, or `span`."""
+        args = self._gemv.get((first, last))
+        if args is None:
+            args = self._gemv[(first, last)] = self._gemv_args(first, last)
+        torch.ops.talm.nf4_gemv(x, *args, out)
+
+    def _gemv_args(self, first, last):
+        """talm_nf4_gemv's weight of projections first .. last - 1: views of the packed buffers (made
+        once: a call is as short as its kernel), sizes and the bias."""
         if not self.gemv_ok(first, last):
             raise ValueError(f"nf4_gemv: projections {first} .. {last - 1} are not one matrix of 64-weight "
                              "blocks and whole blocks per row")
         segs = self.segments[first:last]
         lo, row0 = segs[0].start, segs[0].start // self.qblock
-        torch.ops.talm.nf4_gemv(x, self.packed[lo // 2:], self.absmax8[row0:], self.code,
-                                self.absmax2[row0 // self.qblock2:],
-                                self.offset2[row0 // self.qblock2:],
-                                sum(seg.shape[0] for seg in segs), segs[0].shape[1], self.qblock,
-                                self.qblock2, self.span_bias(first, last), out)
+        return (self.packed[lo // 2:], self.absmax8[row0:], self.code, self.absmax2[row0 // self.qblock2:],
+                self.offset2[row0 // self.qblock2:], sum(seg.shape[0] for seg in segs), segs[0].shape[1],
+                self.qblock, self.qblock2, self.span_bias(first, last))
 
     def dequantize_one(self, idx):
         return self.dequantize(idx, idx + 1).view(self.segments[idx].shape)

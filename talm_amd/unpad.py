@@ -313,71 +313,17 @@ def window_takes(query, key, value):
             and query.shape[1] % key.shape[1] == 0 and query.shape[1] > 0)
 
 
-def _head_rows(t):
-    """[1, H, N, D] -> an [N, H, D] view the window kernels read (a copy only when it must be)."""
-    t = t[0].transpose(0, 1)
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16 \
-            or t.stride(0) < 0 or t.stride(0) >= 2 ** 23:
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-class WindowAttention(torch.autograd.Function):
-    """`VarlenAttention` in a sliding window with sinks (talm_attn_window_fwd / _bwd): row i of a
-    sequence sees the keys j <= i with i - j < window or j < sinks."""
-
-    @staticmethod
-    def forward(ctx, query, key, value, cu, max_len, scale, window, sinks):
-        q, k, v = (_head_rows(t) for t in (query, key, value))
-        n, hq = q.shape[0], q.shape[1]
-        out = torch.empty(n, hq, q.shape[2], dtype=q.dtype, device=q.device)
-        lse = torch.empty(hq, n, dtype=torch.float32, device=q.device)
-        torch.ops.talm.attn_window_fwd(q, k, v, cu, max_len, scale, window, sinks, out, lse)
-        ctx.save_for_backward(q, k, v, out, lse, cu)
-        ctx.max_len, ctx.scale, ctx.window, ctx.sinks = max_len, scale, window, sinks
-        RAN["window_attn"] += 1
-        return out[None]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        q, k, v, out, lse, cu = ctx.saved_tensors
-        g = _head_rows(grad.transpose(1, 2))
-        dq = torch.empty_like(out)
-        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-        ws = torch.empty(_ops.attn_window_bwd_workspace_bytes(
-            q.shape[0], q.shape[1], cu.numel() - 1, ctx.max_len, ctx.window, ctx.sinks),
-            dtype=torch.uint8, device=q.device)
-        torch.ops.talm.attn_window_bwd(q, k, v, out, g, lse, cu, ctx.max_len, ctx.scale, ctx.window,
-                                       ctx.sinks, None, None, dq, dk, dv, ws)
-        RAN["window_attn_bwd"] += 1
-        return (dq.transpose(0, 1)[None], dk.transpose(0, 1)[None], dv.transpose(0, 1)[None],
-                None, None, None, None, None)
-
-
 def window_attention(query, key, value, cu, max_len, scale, window, sinks=0):
     """Causal attention of packed rows in a sliding window: query [1, Hq, N, 128], key and value
     [1, Hkv, N, 128] (fp16 or bf16, any strides), cu int32 [sequences + 1] on their device with
     cu[-1] = N, `max_len` at least the longest sequence. Row i of a sequence sees its last `window`
     keys (itself among them) and the sequence's first `sinks` ones, none after itself. Returns
     [1, N, Hq, 128]; gradients for query, key and value. Every operand finite. Rows that no
-    sequence holds (N > cu[-1]) are not written, and get zero gradients."""
-    if not window_takes(query, key, value):
-        raise ValueError("window_attention: query [1, Hq, N, 128], key / value [1, Hkv, N, 128], fp16 or bf16 "
-                         "of one type and device on the GPU, Hq a multiple of Hkv")
-    if not (torch.is_tensor(cu) and cu.dtype == torch.int32 and cu.dim() == 1 and cu.numel() >= 1
-            and cu.device == query.device and cu.is_contiguous()):
-        raise ValueError("window_attention: cu int32 [sequences + 1] on the operands' device")
-    max_len, window, sinks = int(max_len), int(window), int(sinks)
-    if max_len < 0 or window < 1 or sinks < 0:
-        raise ValueError(f"window_attention: max_len {max_len}, window {window} (at least 1), sinks {sinks}")
-    if not 0.0 < scale < float("inf"):
-        raise ValueError(f"window_attention: scale {scale} (positive, finite)")
-    # no sequence is longer than the rows: larger values mean the same
-    n = query.shape[2]
-    return WindowAttention.apply(query, key, value, cu, min(max_len, n), float(scale),
-                                 min(window, max(n, 1)), min(sinks, n))
+    sequence holds (N > cu[-1]) are not written, and get zero gradients. An autograd node of the C++
+    op layer (talm_attn_window_fwd / _bwd), differentiable once."""
+    out = torch.ops.talm.window_attention(query, key, value, cu, max_len, scale, window, sinks)
+    RAN["window_attn"] += 1
+    return out
 
 
 def _varlen_applies(query, key, value, dropout, cu):

@@ -257,3 +257,23 @@ def test_a_captured_branch_replays():
         torch.cuda.synchronize()
         for got, want in zip(outs, step()):
             assert torch.equal(got, want)
+
+
+def test_the_gradients_have_no_backward():
+    """Under create_graph the gradients come out, and a backward through them is an error, not zeros."""
+    from talm_amd.dropout import dropout
+    from talm_amd.lora import adapter_branch
+    from talm_amd.unpad import window_attention
+
+    key = _key(1, 2)
+    x, a, b, _ = _branch(8, 64, 32, 0.2, torch.float32, 1, key)
+    q = torch.randn(1, 2, 8, 128, device="cuda").half().requires_grad_()
+    cu = torch.tensor([0, 8], dtype=torch.int32, device="cuda")
+    for y, leaf in ((dropout(x, 0.2, key), x), (adapter_branch(x, a, b, 2.0, 0.2, key), a),
+                    (window_attention(q, q, q, cu, 8, 0.1, 4), q)):
+        (first,) = torch.autograd.grad(y.float().sum(), leaf, create_graph=True)
+        assert torch.isfinite(first).all()
+        with pytest.raises(RuntimeError):  # the leaf is not reached
+            torch.autograd.grad(first.float().sum(), leaf, retain_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            first.float().sum().backward()

@@ -120,16 +120,6 @@ def test_python_entries_reject():
         dropout.dropout(x, 0.5, torch.zeros(2, dtype=torch.int64))
     with pytest.raises(ValueError, match="adapter_branch"):
         lora.adapter_branch(x, torch.zeros(16, 64), torch.zeros(32, 16), 2.0)
-    with pytest.raises(ValueError, match="key is needed"):
-        dropout.check(x, 0.5, None, 0)
-    with pytest.raises(ValueError, match="int64"):
-        dropout.check(x, 0.5, torch.zeros(2), 0)
-    with pytest.raises(ValueError, match="int64"):
-        dropout.check(x, 0.5, torch.zeros(3, dtype=torch.int64), 0)
-    with pytest.raises(ValueError, match="site"):
-        dropout.check(x, 0.5, torch.zeros(2, dtype=torch.int64), 2 ** 32)
-    with pytest.raises(ValueError, match="p 1.0"):
-        dropout.check(x, 1.0, torch.zeros(2, dtype=torch.int64), 0)
 
 
 @pytest.mark.parametrize("k,ldx,adapters,word", [(40, 40, 1, "multiple of 32"), (64, 60, 1, "shape"),
