@@ -708,8 +708,9 @@ int talm_lora_wgrad_drop(const uint16_t* x, int64_t ldx, const uint16_t* dy, int
 /*
  * Products of a few tokens with a weight W [rows, cols] in the NF4 form of talm_nf4_group_dequant
  * (packed, absmax8, absmax2, offset2 starting at W's first weight, a multiple of qblock qblock2):
- * out [n_tokens, rows] = fp16(x [n_tokens, cols] W^T + bias). At most 32 tokens (0: nothing is
- * done). The fp16 weights are bit-identical to talm_nf4_group_dequant's and never written out;
+ * out [n_tokens, rows] = fp16(x [n_tokens, cols] W^T + bias + sum_g ts[:, 16g:16g+16] B_g^T on
+ * rows [lo_g, hi_g)). ts f16 (row stride ldt) from talm_lora_down or NULL (no adapters), B_g f16
+ * [hi_g - lo_g, 16], b1 NULL with one adapter. At most 32 tokens (0: nothing is done). The fp16 weights are bit-identical to talm_nf4_group_dequant's and never written out;
  * fp32 sums in a fixed order. qblock 64, qblock2 a power of two; cols a multiple of 64; x and out
  * fp16 with row strides ldx (a multiple of 8) and ldo; bias f16 [rows] or NULL; x and packed
  * 16-byte aligned. Replaces the dequantization of the layer plus the projection's GEMM
@@ -718,7 +719,9 @@ int talm_lora_wgrad_drop(const uint16_t* x, int64_t ldx, const uint16_t* dy, int
 int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, const uint8_t* packed,
                   const uint8_t* absmax8, const float* code, const float* absmax2,
                   const float* offset2, int64_t rows, int64_t cols, int32_t qblock,
-                  int32_t qblock2, const uint16_t* bias, uint16_t* out, int64_t ldo, void* stream);
+                  int32_t qblock2, const uint16_t* bias, const uint16_t* ts, int64_t ldt,
+                  const uint16_t* b0, int64_t lo0, int64_t hi0, const uint16_t* b1, int64_t lo1,
+                  int64_t hi1, uint16_t* out, int64_t ldo, void* stream);
 
 #ifdef __cplusplus
 }

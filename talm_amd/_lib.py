@@ -75,7 +75,8 @@ SIGNATURES = {
     "talm_lora_wgrad_drop": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I32, _F32, _P, _U32,
                              _U32, _I32, _I64, _I64, _F32, _P, _P, _I64, _I64, _F32, _P, _P, _P, _I64,
                              _P],
-    "talm_nf4_gemv": [_P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _P, _P, _I64, _P],
+    "talm_nf4_gemv": [_P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _P, _P, _I64, _P,
+                      _I64, _I64, _P, _I64, _I64, _P, _I64, _P],
     "talm_lora_mirror": [_P, _I32, _I64, _P, _P],
     "talm_rope_table": [_P, _I64, _P, _I32, _F32, _P, _P, _P],
     "talm_pack_rows": [_P, _P, _P, _I32, _I32, _I64, _P, _P, _P, _P, _P, _P],

@@ -1,5 +1,5 @@
 // Products of a few tokens (1 .. 32) with a weight W [rows, cols] held in the layer group's NF4 form,
-// for the calls that answer token by token: out = x W^T + bias. Every weight is read once as its
+// for the calls that answer token by token: out = x W^T + bias (+ LoRA adapters, ts B^T). Every weight is read once as its
 // 4-bit code, with its block's absmax code and second-level scale, and never written out; the fp16
 // weights are bit-identical to talm_nf4_group_dequant's (solution/qgroup.py:72-99), the products fp32.
 //
@@ -32,6 +32,10 @@ struct GemvArgs {
   const float* offset2;
   int shift2;            // log2 of the blocks per second-level scale
   const uint16_t* bias;  // [rows] or null
+  const uint16_t* ts;    // [M][ldt]: the scaled down products of up to two LoRA adapters of rank 16, or null
+  int64_t ldt;
+  const uint16_t* b[2];  // [hi - lo][16]: adapter g adds ts_g b_g^T to rows lo .. hi - 1
+  int lo[2], hi[2];
   uint16_t* out;         // [M][ldo]
   int64_t ldo;
   int units;
@@ -110,6 +114,16 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_rows_kernel(GemvA
 #pragma unroll
       for (int p = 0; p < P; ++p) sum += red[w][b][p][r][tok];
     if (a.bias) sum += h2f(a.bias[row]);
+    if (a.ts) {
+#pragma unroll
+      for (int ad = 0; ad < 2; ++ad)
+        if (row >= a.lo[ad] && row < a.hi[ad]) {
+          const uint16_t* tp = a.ts + static_cast<int64_t>(tok + R * b) * a.ldt + 16 * ad;
+          const uint16_t* bp = a.b[ad] + static_cast<int64_t>(row - a.lo[ad]) * 16;
+#pragma unroll
+          for (int q = 0; q < 16; ++q) sum += h2f(tp[q]) * h2f(bp[q]);
+        }
+    }
     a.out[static_cast<int64_t>(tok + R * b) * a.ldo + row] = f2h(sum);
   }
 }
@@ -122,7 +136,9 @@ using namespace talm;
 TALM_API int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, const uint8_t* packed,
                            const uint8_t* absmax8, const float* code, const float* absmax2, const float* offset2,
                            int64_t rows, int64_t cols, int32_t qblock, int32_t qblock2, const uint16_t* bias,
-                           uint16_t* out, int64_t ldo, void* stream) {
+                           const uint16_t* ts, int64_t ldt, const uint16_t* b0, int64_t lo0, int64_t hi0,
+                           const uint16_t* b1, int64_t lo1, int64_t hi1, uint16_t* out, int64_t ldo,
+                           void* stream) {
   if (qblock != 64 || qblock2 < 1 || (qblock2 & (qblock2 - 1)))
     return fail(TALM_EINVAL, "nf4_gemv: blocks of %d weights in groups of %d (64, a power of two)", qblock, qblock2);
   if (n_tokens < 0 || n_tokens > kGemvTokens || rows < 1 || rows > (1 << 30) || cols < 64 || cols % 64 ||
@@ -131,6 +147,10 @@ TALM_API int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, con
                 "nf4_gemv: bad shape (tokens %lld, W [%lld, %lld], ldx %lld, ldo %lld): at most %d tokens, cols "
                 "a multiple of 64, ldx of 8",
                 (long long)n_tokens, (long long)rows, (long long)cols, (long long)ldx, (long long)ldo, kGemvTokens);
+  if (ts && (ldt < (b1 ? 32 : 16) || !b0 || lo0 < 0 || hi0 < lo0 || hi0 > rows ||
+             (b1 && (lo1 < 0 || hi1 < lo1 || hi1 > rows))))
+    return fail(TALM_EINVAL, "nf4_gemv: adapters on rows %lld..%lld / %lld..%lld, ldt %lld", (long long)lo0,
+                (long long)hi0, (long long)lo1, (long long)hi1, (long long)ldt);
   if (n_tokens == 0) return ok();
   if (!x || !packed || !absmax8 || !code || !absmax2 || !offset2 || !out)
     return fail(TALM_EINVAL, "nf4_gemv: null pointer");
@@ -141,6 +161,11 @@ TALM_API int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, con
   a.packed = packed; a.absmax8 = absmax8; a.code = code; a.absmax2 = absmax2; a.offset2 = offset2;
   while ((1 << a.shift2) < qblock2) ++a.shift2;
   a.bias = bias; a.out = out; a.ldo = ldo;
+  if (ts) {
+    a.ts = ts; a.ldt = ldt;
+    a.b[0] = b0; a.lo[0] = static_cast<int>(lo0); a.hi[0] = static_cast<int>(hi0);
+    if (b1) { a.b[1] = b1; a.lo[1] = static_cast<int>(lo1); a.hi[1] = static_cast<int>(hi1); }
+  }
   // parts of the reduction per tile: what the tokens leave room for, fewest idle lanes and CUs
   int best = 1;
   double cost = 0;

@@ -892,7 +892,8 @@ void lora_wgrad_drop(const Tensor& x, const Tensor& dy, const Tensor& u, const T
 // out [M, rows] = x [M, cols] W^T + bias for a few tokens, W the NF4 weight its buffers start at.
 void nf4_gemv(const Tensor& x, const Tensor& packed, const Tensor& absmax8, const Tensor& code,
               const Tensor& absmax2, const Tensor& offset2, int64_t rows, int64_t cols, int64_t qblock,
-              int64_t qblock2, const OptTensor& bias, const Tensor& out) {
+              int64_t qblock2, const OptTensor& bias, const Tensor& out, const OptTensor& ts,
+              const OptTensor& b0, int64_t lo0, int64_t hi0, const OptTensor& b1, int64_t lo1, int64_t hi1) {
   half_rows(x, x, "nf4_gemv: x");
   half_rows(out, x, "nf4_gemv: out");
   require(x.size(1) == cols && same_shape(out, x.size(0), rows), "nf4_gemv: x [M, cols], out [M, rows]");
@@ -914,11 +915,25 @@ void nf4_gemv(const Tensor& x, const Tensor& packed, const Tensor& absmax8, cons
     require(bias->is_cuda() && bias->device() == x.device() && bias->scalar_type() == at::kHalf &&
                 bias->is_contiguous() && bias->numel() == rows,
             "nf4_gemv: bias float16 [rows]");
+  if (ts.has_value()) {
+    half_rows(*ts, x, "nf4_gemv: ts");
+    require(b0.has_value() && ts->size(0) == x.size(0) && ts->size(1) == (b1.has_value() ? 32 : 16),
+            "nf4_gemv: ts [M, 16 per adapter]");
+    auto up = [&](const OptTensor& b, int64_t lo, int64_t hi) {
+      require(!b.has_value() || (b->is_cuda() && b->device() == x.device() && b->scalar_type() == at::kHalf &&
+                                 b->is_contiguous() && lo >= 0 && hi <= rows && same_shape(*b, hi - lo, 16)),
+              "nf4_gemv: B float16 [hi - lo, 16], contiguous, on x's device, its rows inside W's");
+    };
+    up(b0, lo0, hi0);
+    up(b1, lo1, hi1);
+  }
   const c10::DeviceGuard guard(x.device());
   check(talm_nf4_gemv(as<uint16_t>(x), row_stride(x), x.size(0),
                       as<uint8_t>(packed), as<uint8_t>(absmax8), as<float>(code), as<float>(absmax2),
                       as<float>(offset2), rows, cols, int32_arg(qblock, "qblock"), int32_arg(qblock2, "qblock2"),
-                      as<uint16_t>(bias), as<uint16_t>(out), row_stride(out), stream_of(x)),
+                      as<uint16_t>(bias), as<uint16_t>(ts), ts.has_value() ? row_stride(*ts) : 0,
+                      as<uint16_t>(b0), lo0, hi0, as<uint16_t>(b1), lo1, hi1, as<uint16_t>(out), row_stride(out),
+                      stream_of(x)),
         "nf4_gemv");
 }
 
@@ -2014,7 +2029,8 @@ TORCH_LIBRARY(talm, m) {
         "int site1, int lo0, int seg0, float scaling0, Tensor(a!) da0, Tensor(b!) db0, int lo1, int seg1, "
         "float scaling1, Tensor(c!)? da1, Tensor(d!)? db1, Tensor(e!) workspace) -> ()");
   m.def("nf4_gemv(Tensor x, Tensor packed, Tensor absmax8, Tensor code, Tensor absmax2, Tensor offset2, "
-        "int rows, int cols, int qblock, int qblock2, Tensor? bias, Tensor(a!) out) -> ()");
+        "int rows, int cols, int qblock, int qblock2, Tensor? bias, Tensor(a!) out, Tensor? ts=None, "
+        "Tensor? b0=None, int lo0=0, int hi0=0, Tensor? b1=None, int lo1=0, int hi1=0) -> ()");
   m.def("lora_mirror(Tensor table, int n_tensors, int max_numel, Tensor(a!) out) -> ()");
   m.def("pack_rows(Tensor input_ids, Tensor mask, Tensor labels, int n_tokens, Tensor(a!) ids, "
         "Tensor(b!) positions, Tensor(c!) cu, Tensor(d!) targets, Tensor(e!) src) -> ()");

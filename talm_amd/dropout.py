@@ -26,6 +26,11 @@ from . import _ops  # noqa: F401 - registers torch.ops.talm.*
 COUNTER = os.environ.get("SOLUTION_COUNTER_DROPOUT") == "1"
 
 
+def counter_dropout():
+    """Whether the LoRA nodes' dropout comes from this generator now."""
+    return COUNTER or torch.cuda.is_current_stream_capturing()
+
+
 def draw_key(device):
     """A fresh key, int64 [2] on `device`, from PyTorch's generator of the device."""
     return torch.randint(-2 ** 63, 2 ** 63 - 1, (2,), dtype=torch.int64, device=device)

@@ -33,7 +33,7 @@ import os
 
 import torch
 
-from . import _ops
+from . import _ops, few_tokens
 from .engaged import FELL_BACK, ON, RAN
 from .state import DISABLED, fallback
 
@@ -216,11 +216,21 @@ def mlp_plan(mlp, x, component="fused_mlp"):
     return group
 
 
+def _few_mlp(mlp, x):
+    """The MLP of a few tokens without autograd on the NF4 codes (few_tokens.py), or None."""
+    if "swiglu_inplace" not in ON:
+        return None
+    group = mlp_plan(mlp, x)
+    return None if group is None else few_tokens.mlp(x, group, GATE, DOWN)
+
+
 def fused_mlp_forward(mlp, x):
     """FusedMLP when `mlp_plan` takes the layer, else None (the caller's own path runs). The
     node runs in save-up mode when the save-up MLP is installed (mlp_save_up.py) and the call
     records autograd; otherwise in its default mode, which belongs to the in-place MLP patch
     (swiglu_inplace.py)."""
+    if few_tokens.few(x):
+        return _few_mlp(mlp, x)
     save_up = ("mlp_save_up" in ON and "mlp_save_up" not in DISABLED
                and torch.is_grad_enabled() and x.requires_grad)
     if not save_up and "swiglu_inplace" not in ON:

@@ -27,6 +27,8 @@ import os
 import torch
 import torch.nn.functional as F
 
+from . import few_tokens
+from .dropout import counter_dropout, draw_key
 from .engaged import FELL_BACK, ON, RAN
 from .lora import _power_of_two, _to_half, adapters_t, lora_plan
 from .rope import rope_
@@ -110,9 +112,10 @@ class FusedProjections(torch.autograd.Function):
         halves = [_to_half(lora_weights[2 * k], lora_weights[2 * k + 1])
                   for k in range(len(adapters))]
         mfma = None
-        if _mfma_ok(x2, weight, bias, bounds, adapters, halves, rope, head_dim):
+        ctx.key = key = _drop_key(x2, adapters)
+        if _mfma_ok(x2, weight, bias, bounds, adapters, halves, rope, head_dim, key):
             try:
-                mfma = _mfma_forward(x2, weight, bias, bounds, adapters, halves, rope)
+                mfma = _mfma_forward(x2, weight, bias, bounds, adapters, halves, rope, key)
             except Exception as exc:  # noqa: BLE001 - state.py convention
                 if not fallback("qkv_mfma", exc):
                     raise
@@ -142,7 +145,9 @@ class FusedProjections(torch.autograd.Function):
         for k, (seg, scaling, p) in enumerate(adapters):
             a16, b16 = halves[k]
             state = None
-            if p > 0:
+            if p > 0 and key is not None:
+                xd = _dropped(x2, p, key, k)
+            elif p > 0:
                 state = torch.cuda.get_rng_state(x.device)
                 xd = torch.native_dropout(x2, p, True)[0]
             else:
@@ -239,7 +244,10 @@ class FusedProjections(torch.autograd.Function):
             state = ctx.states[k]
             mask = None
             xd = x2
-            if state is not None:
+            keyed = p > 0 and ctx.key is not None
+            if keyed:
+                xd = _dropped(x2, p, ctx.key, k)
+            elif state is not None:
                 device = x2.device
                 current = torch.cuda.get_rng_state(device)
                 torch.cuda.set_rng_state(state, device)
@@ -249,7 +257,9 @@ class FusedProjections(torch.autograd.Function):
             u = torch.mm(g, b16)
             if dx is not None:
                 dx_lora = torch.mm(u, a16)
-                if mask is not None:
+                if keyed:
+                    dx_lora = _dropped(dx_lora, p, ctx.key, k)
+                elif mask is not None:
                     dx_lora = torch.ops.aten.native_dropout_backward(dx_lora, mask, 1.0 / (1.0 - p))
                 dx.add_(dx_lora)
                 del dx_lora
@@ -263,10 +273,31 @@ class FusedProjections(torch.autograd.Function):
                 *_deliver(lora_grads, ctx.lora_params))
 
 
-def _mfma_ok(x2, weight, bias, bounds, adapters, halves, rope, head_dim):
+def _drop_key(x2, adapters):
+    """A key for the node's dropout when it comes from the counter-based generator (dropout.py;
+    adapter k of the node is site k), else None."""
+    if any(p > 0 for _seg, _s, p in adapters) and counter_dropout():
+        RAN["counter_dropout"] += 1
+        return draw_key(x2.device)
+    return None
+
+
+def _dropped(x2, p, key, site):
+    out = torch.empty(x2.shape, dtype=x2.dtype, device=x2.device)
+    torch.ops.talm.dropout(x2, p, key, site, out)
+    return out
+
+
+def _drop_rate(adapters, key):
+    """The adapters' one dropout rate in the MFMA products (0 without a key)."""
+    return max((p for _seg, _s, p in adapters), default=0.0) if key is not None else 0.0
+
+
+def _mfma_ok(x2, weight, bias, bounds, adapters, halves, rope, head_dim, key=None):
     """Whether the q|k|v node's forward can run as talm_lora_down + talm_qkv_lora_fwd: fp16
-    operands with unit column strides and 16-byte rows, at most two adapters of rank 16 without
-    dropout on whole 128-column tiles, the rotary embedding (if any) on 128-wide heads."""
+    operands with unit column strides and 16-byte rows, at most two adapters of rank 16 on whole
+    128-column tiles, without dropout or (a key of the counter-based generator given) with one rate,
+    the rotary embedding (if any) on 128-wide heads."""
     if not QKV_MFMA or "qkv_mfma" in DISABLED or weight is None or len(adapters) > 2:
         return False
     n_out, size = bounds[-1], x2.shape[1]
@@ -281,7 +312,7 @@ def _mfma_ok(x2, weight, bias, bounds, adapters, halves, rope, head_dim):
         return False
     for (seg, _scaling, p), (a16, b16) in zip(adapters, halves):
         lo, hi = bounds[seg], bounds[seg + 1]
-        if p > 0 or tuple(a16.shape) != (16, size) or tuple(b16.shape) != (hi - lo, 16) \
+        if (p > 0 and key is None) or p != adapters[0][2] or tuple(a16.shape) != (16, size) or tuple(b16.shape) != (hi - lo, 16) \
                 or not (a16.is_contiguous() and b16.is_contiguous()) \
                 or lo % 128 or (hi % 128 and hi != n_out):
             return False
@@ -290,9 +321,9 @@ def _mfma_ok(x2, weight, bias, bounds, adapters, halves, rope, head_dim):
     return True
 
 
-def _mfma_forward(x2, weight, bias, bounds, adapters, halves, rope):
+def _mfma_forward(x2, weight, bias, bounds, adapters, halves, rope, key=None):
     """[q|k|v] (+ LoRA, + RoPE on q and k) on MFMA: returns the [N, n_out] output and the
-    adapters' t = x A^T ([N, 16 per adapter], what the backward keeps)."""
+    adapters' t = x A^T ([N, 16 per adapter], what the backward keeps), of dropped x with a key."""
     n, n_out = x2.shape[0], bounds[-1]
     t = ts = None
     a1 = halves[1][0] if len(adapters) > 1 else None
@@ -304,7 +335,8 @@ def _mfma_forward(x2, weight, bias, bounds, adapters, halves, rope):
     cos, sin = rope if rope is not None else (None, None)
     out = torch.empty(n, n_out, dtype=torch.float16, device=x2.device)
     rope_cols = bounds[2] if rope is not None else 0
-    if QKV_FUSED_DOWN:
+    p = _drop_rate(adapters, key)
+    if QKV_FUSED_DOWN and p == 0.0:
         a0 = halves[0][0] if adapters else None
         s0 = adapters[0][1] if adapters else 0.0
         torch.ops.talm.qkv_lora_fwd_down(x2, weight, bias, a0, a1, s0, s1, bs[0], segs[0][0],
@@ -314,8 +346,12 @@ def _mfma_forward(x2, weight, bias, bounds, adapters, halves, rope):
     if adapters:
         ts = torch.empty_like(t)
         size = x2.shape[1]
-        torch.ops.talm.lora_down(x2, halves[0][0], a1, size, size, 0, 0, 0, adapters[0][1], s1,
-                                 t, ts)
+        if p > 0.0:
+            torch.ops.talm.lora_down_drop(x2, halves[0][0], a1, p, key, 0, 1, adapters[0][1], s1, t, ts,
+                                          _down_workspace(x2, len(adapters)))
+        else:
+            torch.ops.talm.lora_down(x2, halves[0][0], a1, size, size, 0, 0, 0, adapters[0][1], s1,
+                                     t, ts)
     torch.ops.talm.qkv_lora_fwd(x2, weight, bias, ts, bs[0], segs[0][0], segs[0][1], bs[1],
                                 segs[1][0], segs[1][1], cos, sin, rope_cols, out)
     return out, t
@@ -362,19 +398,22 @@ def _mfma_backward_ops(ctx, grads, x2, rest, cos, sin, weight, weight_t=None):
     dx, lora_grads = _mfma_backward_core(grads, x2, rest, cos, sin, weight, ctx.sizes,
                                          ctx.adapters, ctx.has_rope, wanted,
                                          getattr(ctx, "a_t", None),
-                                         _grad_targets(ctx.lora_params), weight_t)
+                                         _grad_targets(ctx.lora_params), weight_t, ctx.key)
     dx = None if dx is None else dx.view(ctx.x_shape)
     return (dx, None, None, None, None, None, None, None, *_deliver(lora_grads, ctx.lora_params))
 
 
 def _mfma_backward_core(grads, x2, rest, cos, sin, weight, sizes, adapters, has_rope, wanted,
-                        a_t=None, outs=None, weight_t=None):
+                        a_t=None, outs=None, weight_t=None, key=None):
     """dX [N, H] (None without `weight`) and the adapters' [dA, dB, ...] of the q|k|v node from
     the gradients of its q, k, v outputs (fp16, unit column stride); `rest` holds (t, A16, B16)
     per adapter, `wanted` which adapter gradients to form, `a_t` the adapters' A^T side by side
     ([H, 16 per adapter] fp16; formed here when None); `outs` optional fp32 buffers for the
     adapter gradients (written in place and returned as themselves); `weight_t` the layer
-    group's W^T [H, >= sum of out] when it holds one (then `weight` is not needed)."""
+    group's W^T [H, >= sum of out] when it holds one (then `weight` is not needed); `key` the
+    dropout's key in force in the forward: the adapters' part of dX is then added under their masks
+    by a launch of its own (a mask per element of u A has no place in the GEMM's extra step)."""
+    p = _drop_rate(adapters, key)
     n_tok, size = x2.shape
     bounds = [0]
     for s_ in sizes:
@@ -408,10 +447,15 @@ def _mfma_backward_core(grads, x2, rest, cos, sin, weight, sizes, adapters, has_
         weight_t = transpose_weight_exact(weight)
         del weight
     if weight_t is not None:
-        if a_t is None and adapters:
+        if a_t is None and adapters and p == 0.0:
             a_t = torch.cat([a16 for _t, a16, _b in halves], 0).t().contiguous()
         dx = torch.empty(n_tok, size, dtype=torch.float16, device=x2.device)
-        torch.ops.talm.qkv_lora_bwd_dx(dcat, weight_t, u, a_t, dx)
+        if p > 0.0:
+            torch.ops.talm.qkv_lora_bwd_dx(dcat, weight_t, None, None, dx)
+            torch.ops.talm.lora_up(u, halves[0][1], halves[1][1] if len(adapters) > 1 else None, True, p,
+                                   key, 0, 1, dx, dx)
+        else:
+            torch.ops.talm.qkv_lora_bwd_dx(dcat, weight_t, u, a_t, dx)
         del weight_t
     lora_grads = [None] * (2 * len(adapters))
     if adapters and any(wanted):
@@ -420,7 +464,8 @@ def _mfma_backward_core(grads, x2, rest, cos, sin, weight, sizes, adapters, has_
         t_all = halves[0][0]
         if len(adapters) > 1 and (halves[1][0].data_ptr() != t_all.data_ptr() + 32
                                   or halves[1][0].stride() != t_all.stride()):
-            return dx, _weight_grads_ops(dcat, u, x2, halves, bounds, adapters, wanted)
+            return dx, _weight_grads_ops(dcat, u, x2, halves, bounds, adapters, wanted,
+                                         key if p > 0.0 else None)
         t_cat = torch.as_strided(t_all, (n_tok, 16 * len(adapters)), (t_all.stride(0), 1))
         segs = [(bounds[seg], bounds[seg + 1] - bounds[seg], s_) for seg, s_, _p in adapters]
         shapes = [(16, size) if i % 2 == 0 else (segs[i // 2][1], 16)
@@ -430,6 +475,11 @@ def _mfma_backward_core(grads, x2, rest, cos, sin, weight, sizes, adapters, has_
                   and o.is_contiguous() else torch.empty(shp, dtype=torch.float32, device=x2.device)
                   for o, shp in zip(outs, shapes)]
         pad = segs + [(0, 0, 0.0)]
+        if p > 0.0:
+            ws = torch.empty(_wgrad_drop_ws(n_tok, size, segs), dtype=torch.uint8, device=x2.device)
+            torch.ops.talm.lora_wgrad_drop(x2, dcat, u, t_cat, p, key, 0, 1, *pad[0], grads_[0],
+                                           grads_[1], *pad[1], *(grads_[2:] or [None, None]), ws)
+            return dx, [g if w else None for g, w in zip(grads_, wanted)]
         ws = torch.empty(_ops_ws(n_tok, size, pad[0][1], pad[1][1]), dtype=torch.uint8,
                          device=x2.device)
         torch.ops.talm.lora_wgrad(x2, dcat, u, t_cat, pad[0][0], pad[0][1], pad[0][2], grads_[0],
@@ -440,19 +490,34 @@ def _mfma_backward_core(grads, x2, rest, cos, sin, weight, sizes, adapters, has_
     return dx, lora_grads
 
 
+def _wgrad_drop_ws(n_tok, size, segs):
+    from . import _ops
+
+    return _ops.lora_wgrad_drop_workspace_bytes(n_tok, size, len(segs), segs[0][1],
+                                                segs[1][1] if len(segs) > 1 else 0)
+
+
+def _down_workspace(x2, n_adapters):
+    from . import _ops
+
+    size = _ops.lora_down_drop_workspace_bytes(x2.shape[0], x2.shape[1], n_adapters)
+    return torch.empty(size, dtype=torch.uint8, device=x2.device) if size else None
+
+
 def _ops_ws(n_tok, size, seg0, seg1):
     from . import _ops
 
     return _ops.lora_wgrad_workspace_bytes(n_tok, size, seg0, seg1)
 
 
-def _weight_grads_ops(dcat, u, x2, halves, bounds, adapters, wanted):
+def _weight_grads_ops(dcat, u, x2, halves, bounds, adapters, wanted, key=None):
     """The adapters' dA / dB with the reference's ops (when their t are not one buffer)."""
     lora_grads = []
-    for k, (seg, scaling, _p) in enumerate(adapters):
+    for k, (seg, scaling, p) in enumerate(adapters):
         t, _a16, _b16 = halves[k]
         uk = u[:, 16 * k:16 * (k + 1)]
-        lora_grads.append(torch.mm(uk.t(), x2).float() if wanted[2 * k] else None)
+        xd = x2 if key is None else _dropped(x2, p, key, k)
+        lora_grads.append(torch.mm(uk.t(), xd).float() if wanted[2 * k] else None)
         dy = dcat[:, bounds[seg]:bounds[seg + 1]]
         lora_grads.append(torch.mm((dy * scaling).t(), t).float() if wanted[2 * k + 1] else None)
     return lora_grads
@@ -471,10 +536,11 @@ class AttentionBlock(torch.autograd.Function):
     nodes between them: the step is bound by the host's launch rate. Same kernels, same values,
     except that the backward rotates dq / dk back inside the attention backward
     (torch.ops.talm.attn_bwd_rope) from the fp32 sums, one fp16 rounding instead of two, and
-    hands the projections' backward that output as it is (no separate rotary pass)."""
+    hands the projections' backward that output as it is (no separate rotary pass).
+    `window`: None, or (window, sinks) of a sliding layer (torch.ops.talm.attn_window_fwd / _bwd)."""
 
     @staticmethod
-    def forward(ctx, x, group, adapters, rope, head_dim, n_heads, n_kv, cu, max_len, scale,
+    def forward(ctx, x, group, adapters, rope, head_dim, n_heads, n_kv, cu, max_len, scale, window,
                 *lora_weights):
         x2 = x.reshape(-1, x.shape[-1])
         n_tok = x2.shape[0]
@@ -486,10 +552,11 @@ class AttentionBlock(torch.autograd.Function):
         halves = [_to_half(lora_weights[2 * k], lora_weights[2 * k + 1])
                   for k in range(len(adapters))]
         bias = group.span_bias(Q, V + 1)
-        if not (_mfma_ok(x2, weight, bias, bounds, adapters, halves, rope, head_dim)
+        ctx.key = key = _drop_key(x2, adapters)
+        if not (_mfma_ok(x2, weight, bias, bounds, adapters, halves, rope, head_dim, key)
                 and sizes[0] == n_heads * head_dim and sizes[1] == sizes[2] == n_kv * head_dim):
             raise _NotApplicable()
-        out, t = _mfma_forward(x2, weight, bias, bounds, adapters, halves, rope)
+        out, t = _mfma_forward(x2, weight, bias, bounds, adapters, halves, rope, key)
         del weight
         w_o = group.weight(O)
         q = out[:, :bounds[1]].view(n_tok, n_heads, head_dim)
@@ -497,7 +564,11 @@ class AttentionBlock(torch.autograd.Function):
         v = out[:, bounds[2]:].view(n_tok, n_kv, head_dim)
         o = torch.empty(n_tok, n_heads, head_dim, dtype=torch.float16, device=x.device)
         lse = torch.empty(n_heads, n_tok, dtype=torch.float32, device=x.device)
-        torch.ops.talm.attn_fwd(q, k, v, cu, max_len, scale, o, lse)
+        if window is None:
+            torch.ops.talm.attn_fwd(q, k, v, cu, max_len, scale, o, lse)
+        else:
+            torch.ops.talm.attn_window_fwd(q, k, v, cu, max_len, scale, *window, o, lse)
+            RAN["window_attn"] += 1
         y = torch.empty(n_tok, w_o.shape[0], dtype=torch.float16, device=x.device)
         torch.ops.talm.gemm(o.view(n_tok, -1), w_o, group.biases[O], 1, y)
         del w_o
@@ -508,7 +579,7 @@ class AttentionBlock(torch.autograd.Function):
         ctx.save_for_backward(*saved)
         ctx.group, ctx.adapters, ctx.sizes, ctx.bounds = group, adapters, sizes, bounds
         ctx.head_dim, ctx.n_heads, ctx.n_kv = head_dim, n_heads, n_kv
-        ctx.max_len, ctx.scale, ctx.x_shape = max_len, scale, x.shape
+        ctx.max_len, ctx.scale, ctx.x_shape, ctx.window = max_len, scale, x.shape, window
         ctx.lora_params = tuple(lora_weights)
         # for the backward's dX (forward runs with grad mode off: ask the node's inputs)
         ctx.a_t = adapters_t([lora_weights[2 * k] for k in range(len(adapters))]) \
@@ -550,10 +621,18 @@ class AttentionBlock(torch.autograd.Function):
         dq = dqkv[:, :bounds[1]]
         dk = dqkv[:, bounds[1]:bounds[2]]
         dv = dqkv[:, bounds[2]:]
-        ws = torch.empty(_ops.attn_bwd_workspace_bytes(n_tok, nh), dtype=torch.uint8,
-                         device=x2.device)
+        ws = torch.empty(_ops.attn_bwd_workspace_bytes(n_tok, nh) if ctx.window is None else
+                         _ops.attn_window_bwd_workspace_bytes(n_tok, nh, cu.numel() - 1, ctx.max_len,
+                                                              *ctx.window),
+                         dtype=torch.uint8, device=x2.device)
         views = (dq.view(n_tok, nh, hd), dk.view(n_tok, nkv, hd), dv.view(n_tok, nkv, hd), ws)
-        if _rope_rows(cos, sin):
+        if ctx.window is not None:
+            fused = _rope_rows(cos, sin)
+            torch.ops.talm.attn_window_bwd(q, k, v, o, d_o.view(n_tok, nh, hd), lse, cu, ctx.max_len,
+                                           ctx.scale, *ctx.window, cos if fused else None,
+                                           sin if fused else None, *views)
+            grads = (dqkv,) if fused else (dq, dk, dv)
+        elif _rope_rows(cos, sin):
             # the rotary backward in the attention backward's epilogues: dqkv is the q|k|v
             # gradient before the rotation, the operand of the projections' backward as it is
             torch.ops.talm.attn_bwd_rope(q, k, v, o, d_o.view(n_tok, nh, hd), lse, cu,
@@ -571,14 +650,14 @@ class AttentionBlock(torch.autograd.Function):
                 weight = group.span(Q, V + 1)
                 if weight is None:
                     weight = torch.cat([group.weight(i) for i in (Q, K, V)], 0)
-        wanted = [ctx.needs_input_grad[10 + i] for i in range(2 * len(ctx.adapters))]
+        wanted = [ctx.needs_input_grad[11 + i] for i in range(2 * len(ctx.adapters))]
         dx, lora_grads = _mfma_backward_core(grads, x2, rest, cos, sin, weight,
                                              ctx.sizes, ctx.adapters, True, wanted, ctx.a_t,
-                                             _grad_targets(ctx.lora_params), weight_t)
+                                             _grad_targets(ctx.lora_params), weight_t, ctx.key)
         RAN["attn_kernel_bwd"] += 1
         RAN["qkv_mfma_bwd"] += 1
         dx = None if dx is None else dx.view(ctx.x_shape)
-        return (dx, None, None, None, None, None, None, None, None, None,
+        return (dx, None, None, None, None, None, None, None, None, None, None,
                 *_deliver(lora_grads, ctx.lora_params))
 
 
@@ -721,14 +800,19 @@ def _attention_block(attn, x, group, adapters, weights, rope, n_tok):
     cfg = attn.config
     n_heads = getattr(cfg, "num_attention_heads", None)
     n_kv = getattr(cfg, "num_key_value_heads", None)
-    if total != n_tok or dropout != 0.0 or attn.sliding_window is not None or tag is None \
+    if total != n_tok or dropout != 0.0 or tag is None \
             or tag[0] is not group or tag[1] != O or _linear4bit(o_proj) is not o_proj \
             or attn.head_dim != 128 or not n_heads or not n_kv or n_heads % n_kv \
             or not _no_hooks([o_proj]) or not _rows_attention(cfg):
         return None
+    window = None
+    if attn.sliding_window is not None:
+        # no sequence is longer than max_len: a wider window, or more sinks, mean the same
+        longest = max(int(max_len), 1)
+        window = (min(int(attn.sliding_window), longest), min(unpad.attention_sinks(attn), longest))
     try:
         y = AttentionBlock.apply(x, group, adapters, rope, attn.head_dim, n_heads, n_kv, cu,
-                                 max_len, attn.scaling, *weights)
+                                 max_len, attn.scaling, window, *weights)
     except _NotApplicable:
         return None
     except Exception as exc:  # noqa: BLE001 - state.py convention
@@ -740,6 +824,42 @@ def _attention_block(attn, x, group, adapters, weights, rope, n_tok):
     RAN["varlen_attn"] += 1
     RAN["attn_block"] += 1
     return y
+
+
+def _few_attention(attn, x, position_embeddings, attention_mask, past_key_values, plan, kwargs):
+    """Qwen2Attention.forward for a few tokens without autograd: q|k|v (+ LoRA) as one product on the
+    NF4 codes (few_tokens.py), the rotary embedding in place, then transformers' own steps (the
+    cache, the attention interface, o_proj). None where the product does not take the layer."""
+    from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+    from transformers.models.qwen2 import modeling_qwen2
+
+    group, adapters, weights = plan
+    halves = [_to_half(weights[2 * k], weights[2 * k + 1]) for k in range(len(adapters))]
+    out = few_tokens.linear(x, group, Q, V + 1, adapters, halves)
+    if out is None:
+        return None
+    lead, hd = x.shape[:-1], attn.head_dim
+    n_q, n_k = group.shapes[Q][0], group.shapes[K][0]
+    q, k, v = (t.view(*lead, -1, hd).transpose(1, 2) for t in
+               (out[..., :n_q], out[..., n_q:n_q + n_k], out[..., n_q + n_k:]))
+    cos, sin = position_embeddings
+    rows = out.view(-1, out.shape[-1])
+    if cos.dim() == 3 and cos.dtype == torch.float32 and cos.shape == sin.shape and cos.shape[2] == hd \
+            and hd % 2 == 0 and hd <= 512 and cos.shape[1] == lead[-1] and len(lead) == 2 \
+            and cos.shape[0] in (1, lead[0]) and "rope" not in DISABLED:
+        tables = [t.expand(*lead, hd).reshape(-1, hd) for t in (cos, sin)]
+        rope_(rows[:, :n_q].view(-1, n_q // hd, hd), rows[:, n_q:n_q + n_k].view(-1, n_k // hd, hd), *tables)
+        RAN["rope"] += 1
+    else:
+        q, k = modeling_qwen2.apply_rotary_pos_emb(q, k, cos, sin)
+    if past_key_values is not None:
+        k, v = past_key_values.update(k, v, attn.layer_idx)
+    interface = ALL_ATTENTION_FUNCTIONS.get_interface(attn.config._attn_implementation,
+                                                      modeling_qwen2.eager_attention_forward)
+    y, probs = interface(attn, q, k, v, attention_mask,
+                         dropout=0.0 if not attn.training else attn.attention_dropout,
+                         scaling=attn.scaling, sliding_window=attn.sliding_window, **kwargs)
+    return attn.o_proj(y.reshape(*lead, -1).contiguous()), probs
 
 
 def patch_qwen2_attention():
@@ -758,8 +878,15 @@ def patch_qwen2_attention():
     def forward(self, hidden_states, position_embeddings=None, attention_mask=None,
                 past_key_values=None, **kwargs):
         plan = None
-        if position_embeddings is not None and past_key_values is None:
+        few = position_embeddings is not None and few_tokens.few(hidden_states)
+        if position_embeddings is not None and (past_key_values is None or few):
             plan = qkv_plan(self, hidden_states)
+            if few and plan is not None:
+                out = _few_attention(self, hidden_states, position_embeddings, attention_mask,
+                                     past_key_values, plan, kwargs)
+                if out is not None:
+                    return out
+                plan = plan if past_key_values is None else None
         if plan is None:
             COUNTS["attn_fallback"] += 1
             FELL_BACK["fused_proj"] += 1

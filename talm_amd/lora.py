@@ -25,8 +25,9 @@ from collections import namedtuple
 import torch
 import torch.nn as nn
 
-from . import _ops  # noqa: F401 - registers torch.ops.talm.*
+from . import _ops, few_tokens  # _ops registers torch.ops.talm.*
 from .adapters import COPIES
+from .dropout import counter_dropout, draw_key
 from .engaged import FELL_BACK, ON, RAN
 from .state import DISABLED, fallback
 
@@ -165,6 +166,11 @@ def lora_projection(x, plan):
     """y = x W^T + b + scaling * B(A(dropout(x))) as the q|k|v node on one projection."""
     from .fused_proj import FusedProjections
 
+    if few_tokens.few(x):
+        y = few_tokens.linear(x, plan.group, plan.idx, plan.idx + 1, ((0, plan.scaling, plan.p),),
+                              (_to_half(plan.lora_a, plan.lora_b),))
+        if y is not None:
+            return y
     (y,) = FusedProjections.apply(x, plan.group, plan.idx, plan.idx + 1,
                                   ((0, plan.scaling, plan.p),), (), None, 0, plan.lora_a,
                                   plan.lora_b)
@@ -197,6 +203,33 @@ def adapter_branch(x, lora_a, lora_b, scaling, p=0.0, key=None, site=0):
                                          key, site)
 
 
+def _unpacked_branch(module, x):
+    """The LoRA layer's forward with the branch of `adapter_branch`, its dropout from the
+    counter-based generator, on a base that is not part of a packed layer; None where that does
+    not take the layer or without dropout (the layer's own forward then runs)."""
+    name = _single_adapter(module)
+    if name is None or not x.is_cuda or x.dtype != torch.float16 \
+            or not torch.is_autocast_enabled("cuda") \
+            or torch.get_autocast_dtype("cuda") != torch.float16:
+        return None
+    down, up = module.lora_A[name], module.lora_B[name]
+    p = _dropout_rate(module.lora_dropout[name])
+    if not p or not p < 1.0 or not isinstance(down, nn.Linear) or not isinstance(up, nn.Linear) \
+            or down.bias is not None or up.bias is not None \
+            or not branch_takes(x, down.weight, up.weight):
+        return None
+    base = module.base_layer(x)
+    if base.dtype != torch.float16:
+        return None
+    try:
+        return base + adapter_branch(x, down.weight, up.weight, float(module.scaling[name]), p,
+                                     draw_key(x.device))
+    except Exception as exc:  # noqa: BLE001 - state.py convention
+        if not fallback("lora", exc):
+            raise
+        return None
+
+
 def patch_lora():
     """`LoraLinear.forward` through `lora_projection` when `lora_plan` takes the call; the
     layer's own forward otherwise (a failure turns "lora" off, state.py)."""
@@ -210,6 +243,11 @@ def patch_lora():
         plan = None
         if not (args or kwargs) and "lora" not in DISABLED:
             plan = lora_plan(self, x)
+            if plan is None and counter_dropout():
+                y = _unpacked_branch(self, x)
+                if y is not None:
+                    RAN["lora_branch"] += 1
+                    return y
         if plan is not None:
             try:
                 y = lora_projection(x, plan)

@@ -24,7 +24,7 @@ import os
 
 import torch
 
-from . import _ops, fused_mlp
+from . import _ops, few_tokens, fused_mlp
 from . import rmsnorm as _rms
 from .engaged import FELL_BACK, ON, RAN
 from .fused_mlp import DOWN, GATE
@@ -203,7 +203,7 @@ def mlp_block(layer, x, h, follower):
     partials (the NF4 dequant-GEMM, or the split-K GEMM); else None (the caller runs the separate
     nodes)."""
     if not ENABLED or "mlp_block" in DISABLED or "addnorm" in DISABLED or "splitk" in DISABLED \
-            or not fused_mlp.SPLITK:
+            or not fused_mlp.SPLITK or few_tokens.few(h):
         return None
     norm1 = layer.post_attention_layernorm
     if not (x.is_cuda and h.is_cuda and x.dtype == torch.float32 and h.dtype == torch.float16

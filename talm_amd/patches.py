@@ -59,6 +59,7 @@ def _have_trl():
 
 _unpad = {"enabled": os.environ.get("SOLUTION_DISABLE_UNPAD") != "1", "checked": 0}
 ORIGINAL_FORWARD = {}
+_NO_MASKS = {"full_attention": None, "sliding_attention": None}  # packed rows: the attention masks
 LAST_STEP = []  # the per-token outputs of the last fused forward (Soup's ChunkedStep fields)
 
 
@@ -106,8 +107,8 @@ def _fused_forward(self, input_ids, attention_mask, position_ids, past_key_value
     from .engaged import FELL_BACK, RAN
     from .fused_head import fused_head_loss
     from .rmsnorm import link_next_norms
-    from .unpad import (is_right_padded, rows_context, static_n_tokens, take_prefetched,
-                        unpad_batch)
+    from .unpad import (is_right_padded, packs_sliding, rows_context, static_n_tokens,
+                        take_prefetched, unpad_batch)
 
     stage.clear()
     kwargs.pop("return_dict", None)
@@ -118,7 +119,8 @@ def _fused_forward(self, input_ids, attention_mask, position_ids, past_key_value
              and isinstance(attention_mask, torch.Tensor) and attention_mask.dim() == 2
              and tuple(attention_mask.shape) == (batch, seq)
              and tuple(input_ids.shape) == (batch, seq)
-             and not getattr(self.model, "has_sliding_layers", True))
+             and (not getattr(self.model, "has_sliding_layers", True)
+                  or hasattr(self.model, "has_sliding_layers") and packs_sliding(self.config)))
     counts = None
     n_static = static_n_tokens()
     if n_static is not None:
@@ -153,7 +155,7 @@ def _fused_forward(self, input_ids, attention_mask, position_ids, past_key_value
         shift = shift.to(idx.device)[idx]
         with rows_context(bounds, device=input_ids.device):
             outputs = self.model(input_ids=input_ids.reshape(-1)[idx][None],
-                                 attention_mask={"full_attention": None},
+                                 attention_mask=dict(_NO_MASKS),
                                  position_ids=positions, past_key_values=None,
                                  inputs_embeds=None, use_cache=False, **kwargs)
     else:
@@ -227,7 +229,7 @@ def _static_forward(self, input_ids, mask, labels, n_tokens, num_items, kwargs, 
     link_next_norms(self.model)
     stage.append("unpadded")
     with rows_context_static(cu, static_max_len(seq), n_tokens):
-        outputs = self.model(input_ids=ids[None], attention_mask={"full_attention": None},
+        outputs = self.model(input_ids=ids[None], attention_mask=dict(_NO_MASKS),
                              position_ids=positions, past_key_values=None, inputs_embeds=None,
                              use_cache=False, **kwargs)
     stage.append("head")

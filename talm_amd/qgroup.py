@@ -47,7 +47,7 @@ from collections import namedtuple
 
 import torch
 
-from . import _ops  # noqa: F401 - registers torch.ops.talm.*
+from . import _ops, few_tokens  # _ops registers torch.ops.talm.*
 from .engaged import FELL_BACK, ON, RAN
 from .nf4_dequant import dequantize_4bit
 from .state import DISABLED, fallback
@@ -324,14 +324,20 @@ class LayerGroup:
         return (self.qblock == 64 and self.qblock2 & (self.qblock2 - 1) == 0 and len(cols) == 1
                 and next(iter(cols)) % 64 == 0)
 
-    def nf4_gemv(self, x, first, last, out):
+    def nf4_gemv(self, x, first, last, out, adapters=None):
         """out [M, sum of out] = x [M, in] W^T + the projections' biases for M <= GEMV_TOKENS rows, W
         the rows of projections first .. last - 1 read as NF4 codes (the fp16 weights of `span`, never
-        written out). For calls that answer token by token; more rows: `nf4_gemm`, or `span`."""
+        written out). `adapters`: (ts [M, 16 each], ((B [hi - lo, 16], lo, hi), ..)), one or two whose
+        ts B^T is added to the output columns lo .. hi - 1. For calls that answer token by token; more
+        rows: `nf4_gemm`, or `span`."""
         args = self._gemv.get((first, last))
         if args is None:
             args = self._gemv[(first, last)] = self._gemv_args(first, last)
-        torch.ops.talm.nf4_gemv(x, *args, out)
+        if adapters is None:
+            torch.ops.talm.nf4_gemv.default(x, *args, out)
+            return
+        ts, ups = adapters
+        torch.ops.talm.nf4_gemv.default(x, *args, out, ts, *[v for up in ups for v in up])
 
     def _gemv_args(self, first, last):
         """talm_nf4_gemv's weight of projections first .. last - 1: views of the packed buffers (made
@@ -505,14 +511,15 @@ def setup_layer(layer):
         layer._solution_layer_group = _pack(layer)
 
 
-def enter_layer(layer):
-    """The decoder layer's forward begins: pack on first use, then make its weights resident."""
+def enter_layer(layer, x=None):
+    """The decoder layer's forward on x begins: pack on first use, then make its weights resident,
+    unless a few tokens without autograd read their codes instead (few_tokens.py)."""
     if "qgroup" in DISABLED:
         return
     try:
         setup_layer(layer)
         group = layer._solution_layer_group
-        if group is not None:
+        if group is not None and not (x is not None and few_tokens.serves(group, x)):
             group.begin_forward()
     except Exception as exc:  # noqa: BLE001 - state.py convention
         if not fallback("qgroup", exc):
@@ -533,7 +540,7 @@ def patch_group_dequant():
     ON.add("group")
     if not _in_chain(layer_forward, "_solution_group"):
         def forward(self, *args, **kwargs):
-            enter_layer(self)
+            enter_layer(self, args[0] if args else kwargs.get("hidden_states"))
             return layer_forward(self, *args, **kwargs)
 
         forward._solution_group = True
@@ -549,6 +556,9 @@ def patch_group_dequant():
         if tag is not None and "qgroup" not in DISABLED and x.is_cuda \
                 and x.dtype == torch.float16:
             group, idx = tag
+            y = few_tokens.linear(x, group, idx, idx + 1)
+            if y is not None:
+                return y
             try:
                 return GroupLinear.apply(x, group, idx)
             except Exception as exc:  # noqa: BLE001 - state.py convention

@@ -323,7 +323,7 @@ def patch_qwen2_add_norm():
         if enters_group:  # the layer-group patch below this one would have done it
             from .qgroup import enter_layer
 
-            enter_layer(self)
+            enter_layer(self, hidden_states)
         return _layer_forward(self, hidden_states, dict(
             attention_mask=attention_mask, position_ids=position_ids,
             past_key_values=past_key_values, use_cache=use_cache,

@@ -342,6 +342,43 @@ def _autocast_half(query):
     return dtype if dtype in (torch.float16, torch.bfloat16) else None
 
 
+def attention_sinks(module):
+    """The first tokens of a row that stay visible to a sliding layer's rows (config.attention_sinks;
+    0 when the config names none)."""
+    return int(getattr(module.config, "attention_sinks", 0) or 0)
+
+
+def packs_sliding(config):
+    """Whether a model with sliding layers can run on packed rows: its attention is the wrapped
+    "sdpa" interface, which knows a layer's window from its call."""
+    from .fused_proj import _rows_attention
+
+    return _rows_attention(config)
+
+
+def _window_rows(query, key, value, cu, dropout, scaling, window, sinks):
+    """A sliding layer's attention of the packed rows: `window_attention` in one launch, else one
+    masked SDPA call per row. Returns the attention interface's (output, None)."""
+    scale = scaling if scaling is not None else query.shape[-1] ** -0.5
+    if "varlen_attention" not in DISABLED and cu is not None and dropout == 0.0 \
+            and window_takes(query, key, value) and cu[2] == query.shape[2]:
+        try:
+            return window_attention(query, key, value, cu[0], cu[1], scale, window, sinks), None
+        except Exception as exc:  # noqa: BLE001 - state.py convention
+            if not fallback("varlen_attention", exc):
+                raise
+    outs = []
+    for s, e in _rows[-1]:
+        if e > s:
+            i = torch.arange(e - s, device=query.device)
+            seen = (i[None] <= i[:, None]) & ((i[:, None] - i[None] < window) | (i[None] < sinks))
+            outs.append(F.scaled_dot_product_attention(
+                query[:, :, s:e], key[:, :, s:e], value[:, :, s:e], attn_mask=seen, dropout_p=dropout,
+                scale=scale, enable_gqa=query.shape[1] != key.shape[1]))
+    RAN["rows_attn"] += 1
+    return torch.cat(outs, dim=2).transpose(1, 2).contiguous(), None
+
+
 def patch_sdpa_rows():
     """Wrap transformers' registered "sdpa" attention: per-row causal attention while a flat
     forward runs, the original interface otherwise (solution/unpad.py:338-395)."""
@@ -354,16 +391,20 @@ def patch_sdpa_rows():
 
     def rows_sdpa(module, query, key, value, attention_mask, dropout=0.0, scaling=None,
                   sliding_window=None, **kwargs):
-        if not _rows or query.shape[0] != 1 or sliding_window is not None:
+        sinks = attention_sinks(module) if sliding_window is not None else 0
+        if not _rows or query.shape[0] != 1:
             if _rows:
                 FELL_BACK["rows_attn"] += 1
+            if sinks:
+                raise ValueError("attention sinks (config.attention_sinks) are served for packed training rows "
+                                 "only: this call's mask does not hold them")
             return original(module, query, key, value, attention_mask, dropout=dropout,
                             scaling=scaling, sliding_window=sliding_window, **kwargs)
         half = _autocast_half(query)
         if half is not None:
             query, key, value = query.to(half), key.to(half), value.to(half)
         cu = _cu[-1] if _cu else None
-        if "varlen_attention" not in DISABLED and cu is not None \
+        if "varlen_attention" not in DISABLED and cu is not None and sliding_window is None \
                 and _varlen_applies(query, key, value, dropout, cu[0]) \
                 and cu[2] == query.shape[2]:
             try:
@@ -375,6 +416,8 @@ def patch_sdpa_rows():
             else:
                 RAN["varlen_attn"] += 1
                 return out, None
+        if sliding_window is not None:
+            return _window_rows(query, key, value, cu, dropout, scaling, sliding_window, sinks)
         gqa = query.shape[1] != key.shape[1]
         outs = [F.scaled_dot_product_attention(query[:, :, s:e], key[:, :, s:e], value[:, :, s:e],
                                                dropout_p=dropout, is_causal=True, scale=scaling,

@@ -152,5 +152,15 @@ def test_adapter_weight_gradient_rejects():
     (1, 128, 64, 200, "blocks"), (-1, 128, 64, 256, "shape")])
 def test_gemv_rejects(tokens, cols, qblock, qblock2, word):
     status, message = _status("talm_nf4_gemv", PTR, 128, tokens, PTR, PTR, PTR, PTR, PTR, 128, cols,
-                              qblock, qblock2, None, PTR, 128, None)
+                              qblock, qblock2, None, None, 0, None, 0, 0, None, 0, 0, PTR, 128, None)
     assert status == _lib.TALM_EINVAL and word in message
+
+
+@pytest.mark.parametrize("ldt,b0,lo0,hi0,b1,lo1,hi1", [
+    (15, PTR, 0, 64, None, 0, 0), (31, PTR, 0, 64, PTR, 64, 128), (32, None, 0, 64, None, 0, 0),
+    (32, PTR, -1, 64, None, 0, 0), (32, PTR, 0, 129, None, 0, 0), (32, PTR, 0, 64, PTR, 64, 200),
+    (32, PTR, 0, 64, PTR, 70, 64)])
+def test_gemv_rejects_adapters_outside_the_weight(ldt, b0, lo0, hi0, b1, lo1, hi1):
+    status, message = _status("talm_nf4_gemv", PTR, 128, 1, PTR, PTR, PTR, PTR, PTR, 128, 128, 64, 256,
+                              None, PTR, ldt, b0, lo0, hi0, b1, lo1, hi1, PTR, 128, None)
+    assert status == _lib.TALM_EINVAL and "adapters" in message
