@@ -4,13 +4,25 @@
 // weights are bit-identical to talm_nf4_group_dequant's (solution/qgroup.py:72-99), the products fp32.
 //
 // The weights are the A operand of v_mfma_f32_16x16x32_f16, the tokens the B operand. A lane takes
-// whole 64-weight blocks (32 contiguous bytes of codes, one scale) and looks their weights up in a
-// table of the block's 16 scaled levels kept in its registers (nf4_code.h); the reduction's order is
-// free, so eight MFMAs take a block's eight-weight words as they lie, against the same columns of x.
-// Sixteen operand rows are 16 / P rows of W times P parts of the reduction (unit: 256 P columns); the
+// whole 64-weight blocks (32 contiguous bytes of codes, one scale); the reduction's order is free, so
+// eight MFMAs take a block's eight-weight words as they lie, against the same columns of x. Sixteen
+// operand rows are R = 16 / P rows of W times P parts of the reduction (a unit: 256 P columns); the
 // operand's columns are the tokens times the same P parts, and the blocks of the result where both
-// parts agree are summed: few tokens leave operand columns free, and small P tiles give short rows
-// of W enough workgroups. The wavefronts of a workgroup split the units, joined through LDS in order.
+// parts agree are summed: few tokens leave operand columns free, and small tiles give a W of few
+// rows enough workgroups. The wavefronts of a workgroup split the units, joined through LDS in order.
+//
+// Two ways to look a code up, by the size of W:
+//   rows kernel  a table of the block's 16 scaled levels in the lane's registers (nf4_code.h), 310 VALU
+//                instructions per block, half of them byte permutes;
+//   lut kernel   per byte of codes its two levels from a table in LDS (one ds_read_b64 through an
+//                address made by one byte permute), scaled and packed: 140 instructions per block.
+//                The table stands in 32 copies, lane l reading copy l % 32, so that the 32 lanes of a
+//                read phase meet 32 different bank pairs whatever their codes are; its 64 KiB cost 1 us
+//                to fill and make one workgroup per CU, whose wavefronts walk several tiles.
+// MI355X, us, rows / lut: W [2048, 1536] 1 token 3.3 / 4.6, 32 tokens 7.0 / 7.1; [17920, 1536] 9.4 / 7.2,
+// 18.7 / 13.4; [1536, 8960] 7.3 / 6.6, 38 / 22. What bounds one token: a launch (1.2 us), one memory
+// round trip with the whole of W in flight, the lookups behind it (LDS and VALU 1.4 us each) and the
+// join, one after the other; many tokens: x's operand reads through L2.
 #include "mfma_tile.h"
 #include "nf4_code.h"
 
@@ -39,93 +51,262 @@ struct GemvArgs {
   uint16_t* out;         // [M][ldo]
   int64_t ldo;
   int units;
+  int tiles_per_wg, unit_waves, groups;  // the lut kernel: wavefront w takes units w % unit_waves, .. of
+                                         // tiles w / unit_waves, .. of the workgroup's
 };
 
 constexpr int kGemvMaxWaves = 16;
 constexpr int kGemvTokens = 32;
 
+// A unit's weights of one lane, as loaded: a block's codes and its scale's inputs.
+struct GemvBlock {
+  uint4 lo, hi;
+  uint8_t a8;
+  float s2, o2;
+};
+
+// A lane's place in its operands, and its loads of W from the workgroup's first row on and of x.
 template <int P, int TB>
-__global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_rows_kernel(GemvArgs a) {
-  static_assert(TB == 1 || P == 1, "two token blocks need every operand column");
-  constexpr int R = 16 / P;  // rows of W, and tokens per block
-  __shared__ float table[256];
-  __shared__ float red[kGemvMaxWaves][TB][P][R][R + 1];
-  const int tid = threadIdx.x, lane = tid & 63, waves = blockDim.x >> 6;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int m = lane & 15, g = lane >> 4;
-  const int row0 = blockIdx.x * R;
-  const int wr = m % R, part = m / R;  // this lane's row of W and part (A); its token and part (B)
-  for (int i = tid; i < 256; i += blockDim.x) table[i] = a.code[i];
-  __syncthreads();
-  const bool row_in = row0 + wr < a.rows;
-  const int64_t tile0 = static_cast<int64_t>(row0) * a.cols;  // the tile's first weight
-  const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(a.packed + tile0 / 2), 0, 0x7fffffff, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint8_t*>(a.absmax8 + tile0 / 64), 0, 0x7fffffff, 0x00020000);
-  const __amdgpu_buffer_rsrc_t rx = buffer_rsrc(a.x);
-  f32x4 acc[TB];
-#pragma unroll
-  for (int b = 0; b < TB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int u = wave; u < a.units; u += waves) {
-    const int k = (u * P + part) * 256 + 64 * g;
-    const bool k_in = k < a.cols, in = k_in && row_in;
-    const uint32_t e = static_cast<uint32_t>(wr * a.cols + k);  // weight index inside the tile
-    const uint4 w0 = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rw, in ? e / 2 : kOob, 0, 0));
-    const uint4 w1 =
-        __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rw, in ? e / 2 + 16 : kOob, 0, 0));
-    const uint8_t a8 = __builtin_amdgcn_raw_buffer_load_b8(rs, in ? e / 64 : kOob, 0, 0);
-    const int64_t i2 = in ? ((tile0 + e) >> 6) >> a.shift2 : 0;
-    const float s2 = a.absmax2[i2], o2 = a.offset2[i2];
-    uint4 xv[TB][8];
+struct GemvLane {
+  static constexpr int R = 16 / P;  // rows of W per tile, and tokens per block
+  int row0, wr, part, g;            // wr: the lane's row of a tile (A) and token of a block (B)
+  int64_t first;                    // the workgroup's first weight
+  __amdgpu_buffer_rsrc_t rw, rs, rx;
+  __device__ __forceinline__ GemvLane(const GemvArgs& a, int row, int lane)
+      : row0(row), wr(lane & (R - 1)), part((lane & 15) / R), g(lane >> 4),
+        first(static_cast<int64_t>(row) * a.cols) {
+    rw = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.packed + first / 2), 0, 0x7fffffff, 0x00020000);
+    rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(a.absmax8 + first / 64), 0, 0x7fffffff, 0x00020000);
+    rx = buffer_rsrc(a.x);
+  }
+  __device__ __forceinline__ int column(int unit) const { return (unit * P + part) * 256 + 64 * g; }
+  // A lane outside W reads codes of 0 under some block's scale, against columns of x that read 0, or
+  // for rows that are not stored.
+  __device__ __forceinline__ void load_w(const GemvArgs& a, int tile, int unit, GemvBlock& w) const {
+    const int k = column(unit), row = R * tile + wr;
+    const bool in = k < a.cols && row0 + row < a.rows;
+    const uint32_t e = static_cast<uint32_t>(row * a.cols + k);
+    w.lo = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rw, in ? e / 2 : kOob, 0, 0));
+    w.hi = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rw, in ? e / 2 + 16 : kOob, 0, 0));
+    w.a8 = __builtin_amdgcn_raw_buffer_load_b8(rs, in ? e / 64 : kOob, 0, 0);
+    const int64_t group = in ? ((first + e) >> 6) >> a.shift2 : 0;
+    w.s2 = a.absmax2[group];
+    w.o2 = a.offset2[group];
+  }
+  __device__ __forceinline__ void load_x(const GemvArgs& a, int unit, uint4 (&x)[TB][8]) const {
+    const int k = column(unit);
 #pragma unroll
     for (int b = 0; b < TB; ++b) {
       const int tok = wr + R * b;
-      const uint32_t off = k_in && tok < a.M ? static_cast<uint32_t>((tok * a.ldx + k) * 2) : kOob;
+      const uint32_t off = k < a.cols && tok < a.M ? static_cast<uint32_t>((tok * a.ldx + k) * 2) : kOob;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        xv[b][j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 16 * j, 0));
+        x[b][j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 16 * j, 0));
     }
-    const float scale = in ? block_scale(table[a8], s2, o2) : 0.f;
-    const Nf4Table t = nf4_table(scale);
-    const uint32_t words[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+  }
+  // The lane's accumulators to its wavefront's slot: element v is operand row 4 (lane / 16) + v.
+  __device__ __forceinline__ void leave(const f32x4 (&acc)[TB], float (&slot)[TB][P][R][R + 1]) const {
+#pragma unroll
+    for (int b = 0; b < TB; ++b)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const int r = 4 * g + v;
+        if (r / R == part) slot[b][part][r % R][wr] = acc[b][v];
+      }
+  }
+};
+
+// The sum of the joined parts, bias and adapters, rounded and stored.
+__device__ __forceinline__ void gemv_store(const GemvArgs& a, int row, int token, float sum) {
+  if (a.bias) sum += h2f(a.bias[row]);
+  if (a.ts) {
+#pragma unroll
+    for (int ad = 0; ad < 2; ++ad)
+      if (row >= a.lo[ad] && row < a.hi[ad]) {
+        const uint16_t* tp = a.ts + static_cast<int64_t>(token) * a.ldt + 16 * ad;
+        const uint16_t* bp = a.b[ad] + static_cast<int64_t>(row - a.lo[ad]) * 16;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) sum += h2f(tp[q]) * h2f(bp[q]);
+      }
+  }
+  a.out[static_cast<int64_t>(token) * a.ldo + row] = f2h(sum);
+}
+
+// One workgroup per tile, a wavefront per unit (or several), the next unit's loads in flight.
+template <int P, int TB>
+__global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_rows_kernel(GemvArgs a) {
+  static_assert(TB == 1 || P == 1, "two token blocks need every operand column");
+  constexpr int R = 16 / P;
+  __shared__ float table[256];
+  __shared__ float red[kGemvMaxWaves][TB][P][R][R + 1];
+  const int tid = threadIdx.x, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row0 = blockIdx.x * R;
+  const GemvLane<P, TB> ln(a, row0, tid & 63);
+  f32x4 acc[TB];
+#pragma unroll
+  for (int b = 0; b < TB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // the code table's load first: loads return in order, and its LDS write then waits for none of the
+  // weights', whose first unit's fly meanwhile
+  const float code = tid < 256 ? a.code[tid] : 0.f;
+  GemvBlock w, next;
+  uint4 x[TB][8], x_next[TB][8];
+  int u = wave;
+  if (u < a.units) {
+    ln.load_w(a, 0, u, w);
+    ln.load_x(a, u, x);
+  }
+  if (tid < 256) table[tid] = code;
+  for (int i = tid + blockDim.x; i < 256; i += blockDim.x) table[i] = a.code[i];
+  lds_barrier();
+  for (; u < a.units; u += waves) {
+    const bool more = u + waves < a.units;
+    if (more) {
+      ln.load_w(a, 0, u + waves, next);
+      ln.load_x(a, u + waves, x_next);
+    }
+    const Nf4Table tab = nf4_table(block_scale(table[w.a8], w.s2, w.o2));
+    const uint32_t words[8] = {w.lo.x, w.lo.y, w.lo.z, w.lo.w, w.hi.x, w.hi.y, w.hi.z, w.hi.w};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const half8_t wf = __builtin_bit_cast(half8_t, nf4_lookup_word(words[j], t));
+      const half8_t wf = __builtin_bit_cast(half8_t, nf4_lookup_word(words[j], tab));
 #pragma unroll
       for (int b = 0; b < TB; ++b)
-        acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, __builtin_bit_cast(half8_t, xv[b][j]), acc[b], 0, 0, 0);
+        acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, __builtin_bit_cast(half8_t, x[b][j]), acc[b], 0, 0, 0);
+    }
+    if (more) {
+      w = next;
+#pragma unroll
+      for (int b = 0; b < TB; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[b][j] = x_next[b][j];
     }
   }
-  // element v of lane l: operand row 4 (l / 16) + v, column l % 16
-#pragma unroll
-  for (int b = 0; b < TB; ++b)
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-      const int r = 4 * g + v;
-      if (r / R == part) red[wave][b][part][r % R][wr] = acc[b][v];
-    }
+  ln.leave(acc, red[wave]);
   __syncthreads();
   for (int i = tid; i < TB * R * R; i += blockDim.x) {
-    const int r = i % R, tok = i / R % R, b = i / (R * R), row = row0 + r;
-    if (row >= a.rows || tok + R * b >= a.M) continue;
+    const int r = i % R, tok = i / R % R, b = i / (R * R);
+    if (row0 + r >= a.rows || tok + R * b >= a.M) continue;
     float sum = 0.f;
-    for (int w = 0; w < waves; ++w)
+    for (int v = 0; v < waves; ++v)
 #pragma unroll
-      for (int p = 0; p < P; ++p) sum += red[w][b][p][r][tok];
-    if (a.bias) sum += h2f(a.bias[row]);
-    if (a.ts) {
-#pragma unroll
-      for (int ad = 0; ad < 2; ++ad)
-        if (row >= a.lo[ad] && row < a.hi[ad]) {
-          const uint16_t* tp = a.ts + static_cast<int64_t>(tok + R * b) * a.ldt + 16 * ad;
-          const uint16_t* bp = a.b[ad] + static_cast<int64_t>(row - a.lo[ad]) * 16;
-#pragma unroll
-          for (int q = 0; q < 16; ++q) sum += h2f(tp[q]) * h2f(bp[q]);
-        }
-    }
-    a.out[static_cast<int64_t>(tok + R * b) * a.ldo + row] = f2h(sum);
+      for (int p = 0; p < P; ++p) sum += red[v][b][p][r][tok];
+    gemv_store(a, row0 + r, tok + R * b, sum);
   }
+}
+
+constexpr int kLutBytes = 256 * 256;       // 256 bytes of codes x 32 copies of their two levels
+constexpr int kLutRedFloats = 20 * 1024;   // 80 KiB: the wavefronts' results of every tile
+
+// One workgroup per CU and a.tiles_per_wg tiles. kOne: a wavefront has one unit, whose x it keeps.
+template <int P, int TB, bool kOne>
+__global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_lut_kernel(GemvArgs a) {
+  constexpr int R = 16 / P;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[kLutBytes + 1024 + kLutRedFloats * 4];
+  float* table = reinterpret_cast<float*>(smem + kLutBytes);
+  typedef float Slot[TB][P][R][R + 1];
+  Slot* red = reinterpret_cast<Slot*>(smem + kLutBytes + 1024);  // [tile][unit wavefront]
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int uw = wave % a.unit_waves, grp = wave / a.unit_waves;
+  const int row0 = blockIdx.x * a.tiles_per_wg * R;
+  const int n_tiles = min(a.tiles_per_wg, (a.rows - row0 + R - 1) / R);
+  const GemvLane<P, TB> ln(a, row0, lane);
+  const float code = tid < 256 ? a.code[tid] : 0.f;  // first, as above
+  GemvBlock w;
+  uint4 x[TB][8];
+  int t = grp, u = uw;
+  const bool any = t < n_tiles;
+  if (any) {
+    ln.load_w(a, t, u, w);
+    ln.load_x(a, u, x);
+  }
+  // copy c of byte e's levels at e * 256 + 8 c: a thread writes two copies, a wavefront four bytes of
+  // one high nibble (the levels through scalar loads: no wait for the weights either)
+  for (int e0 = 4 * wave; e0 < 256; e0 += blockDim.x >> 4) {
+    const float* l = kNF4Levels + (e0 & 15);
+    const float hi = kNF4Levels[e0 >> 4], l0 = l[0], l1 = l[1], l2 = l[2], l3 = l[3];
+    const float lo = lane < 32 ? (lane < 16 ? l0 : l1) : (lane < 48 ? l2 : l3);
+    *reinterpret_cast<float4*>(smem + e0 * 256 + lane * 16) = make_float4(hi, lo, hi, lo);
+  }
+  if (tid < 256) table[tid] = code;
+  for (int i = tid + blockDim.x; i < 256; i += blockDim.x) table[i] = a.code[i];
+  lds_barrier();
+  const uint32_t copy = (lane & 31) * 8;
+  if (any) {
+    f32x4 acc[TB];
+#pragma unroll
+    for (int b = 0; b < TB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (;;) {
+      int tn = t, un = u + a.unit_waves;  // the next step: this tile's next unit, or the next tile
+      if (un >= a.units) {
+        un = uw;
+        tn += a.groups;
+      }
+      const bool more = tn < n_tiles;
+      GemvBlock next;
+      if (more) ln.load_w(a, tn, un, next);
+      const float scale = block_scale(table[w.a8], w.s2, w.o2);
+      const uint32_t words[8] = {w.lo.x, w.lo.y, w.lo.z, w.lo.w, w.hi.x, w.hi.y, w.hi.z, w.hi.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint32_t h[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {  // byte q of the word to bits 8..15, the copy below it
+          const uint32_t at = __builtin_amdgcn_perm(words[j], copy, 0x0c0c0400u + (static_cast<uint32_t>(q) << 8));
+          const float2 f = *reinterpret_cast<const float2*>(smem + at);
+          h[q] = __builtin_bit_cast(uint32_t, __builtin_convertvector(
+                                                  (nf4_float2_t){mul_f32(f.x, scale), mul_f32(f.y, scale)}, nf4_half2_t));
+        }
+        const half8_t wf = __builtin_bit_cast(half8_t, make_uint4(h[0], h[1], h[2], h[3]));
+#pragma unroll
+        for (int b = 0; b < TB; ++b)
+          acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, __builtin_bit_cast(half8_t, x[b][j]), acc[b], 0, 0, 0);
+      }
+      if (!more || tn != t) {  // the tile is done
+        ln.leave(acc, red[t * a.unit_waves + uw]);
+#pragma unroll
+        for (int b = 0; b < TB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+      if (!more) break;
+      w = next;
+      t = tn;
+      u = un;
+      if constexpr (!kOne) ln.load_x(a, u, x);
+    }
+  }
+  __syncthreads();
+  const int rows = n_tiles * R;
+  for (int i = tid; i < rows * TB * R; i += blockDim.x) {
+    const int rl = i % rows, token = i / rows, b = token / R;
+    if (row0 + rl >= a.rows || token >= a.M) continue;
+    const Slot* slot = red + rl / R * a.unit_waves;
+    float sum = 0.f;
+    for (int v = 0; v < a.unit_waves; ++v)
+#pragma unroll
+      for (int p = 0; p < P; ++p) sum += slot[v][b][p][rl % R][token % R];
+    gemv_store(a, row0 + rl, token, sum);
+  }
+}
+
+template <int P, int TB>
+void launch_gemv(GemvArgs a, bool lut, hipStream_t s) {
+  constexpr int R = 16 / P;
+  const int tiles = (a.rows + R - 1) / R;
+  a.units = (a.cols + 256 * P - 1) / (256 * P);
+  const int turns = (a.units + kGemvMaxWaves - 1) / kGemvMaxWaves;
+  a.unit_waves = (a.units + turns - 1) / turns;
+  if (!lut) {
+    hipLaunchKernelGGL((nf4_gemv_rows_kernel<P, TB>), dim3(static_cast<unsigned>(tiles)), dim3(64 * a.unit_waves), 0, s, a);
+    return;
+  }
+  const int room = kLutRedFloats / (a.unit_waves * TB * P * R * (R + 1));
+  a.tiles_per_wg = std::min(room, (tiles + device_cus() - 1) / device_cus());
+  a.groups = std::max(1, std::min(a.tiles_per_wg, kGemvMaxWaves / a.unit_waves));
+  const dim3 grid(static_cast<unsigned>((tiles + a.tiles_per_wg - 1) / a.tiles_per_wg));
+  const dim3 block(64 * a.unit_waves * a.groups);
+  if (turns == 1) hipLaunchKernelGGL((nf4_gemv_lut_kernel<P, TB, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((nf4_gemv_lut_kernel<P, TB, false>), grid, block, 0, s, a);
 }
 
 }  // namespace
@@ -166,22 +347,32 @@ TALM_API int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, con
     a.b[0] = b0; a.lo[0] = static_cast<int>(lo0); a.hi[0] = static_cast<int>(hi0);
     if (b1) { a.b[1] = b1; a.lo[1] = static_cast<int>(lo1); a.hi[1] = static_cast<int>(hi1); }
   }
-  // parts of the reduction per tile: what the tokens leave room for, fewest idle lanes and CUs
+  // The table in LDS pays from some size of W on, an earlier one with more tokens. us, rows / lut:
+  // 1 token [1536, 4864] 4.8 / 5.3, [8960, 1024] 5.2 / 5.3, [8960, 1536] 6.4 / 6.1; 16 tokens [4864, 896]
+  // 4.7 / 5.4, [1536, 3584] 8.0 / 7.7, [1536, 4864] 9.7 / 8.9; 32 tokens [2048, 1536] 7.1 / 7.1,
+  // [1792, 2048] 7.9 / 7.7, [1536, 3584] 12.4 / 11.0.
+  const bool lut = rows * cols > (n_tokens <= 8 ? 9 << 20 : n_tokens <= 16 ? 5 << 20 : 3 << 20);
+  // Parts of the reduction per tile: what the tokens leave room for, and
+  //   rows kernel: the fewest idle lanes and CUs (1 token, one / two / four parts: [2048, 1536] 3.8 / 3.2 /
+  //     3.8 us, [4864, 896] 3.7 / 3.8 / 4.0);
+  //   lut kernel: two where whole tiles would leave CUs without one ([1536, 8960] 8.3 / 6.6).
   int best = 1;
-  double cost = 0;
-  for (int p = 1; p <= 4 && p * n_tokens <= 16; p *= 2) {
-    const int64_t units = (cols + 256 * p - 1) / (256 * p), wgs = (rows * p + 15) / 16;
-    const double waste = static_cast<double>(units * 256 * p) / cols, cus = device_cus();
-    const double c = waste * std::max(1.0, cus / static_cast<double>(wgs));
-    if (cost == 0 || c < cost) { cost = c; best = p; }
+  const double cus = device_cus();
+  if (lut) {
+    best = n_tokens <= 8 && (rows + 15) / 16 < device_cus() ? 2 : 1;
+  } else {
+    double cost = 0;
+    for (int p = 1; p <= 4 && p * n_tokens <= 16; p *= 2) {
+      const int64_t units = (cols + 256 * p - 1) / (256 * p), wgs = (rows * p + 15) / 16;
+      const double waste = static_cast<double>(units * 256 * p) / cols;
+      const double c = waste * std::max(1.0, cus / static_cast<double>(wgs));
+      if (cost == 0 || c < cost) { cost = c; best = p; }
+    }
   }
-  a.units = static_cast<int>((cols + 256 * best - 1) / (256 * best));
-  const int turns = (a.units + kGemvMaxWaves - 1) / kGemvMaxWaves, waves = (a.units + turns - 1) / turns;
-  const dim3 grid(static_cast<unsigned>((rows * best + 15) / 16)), block(64 * waves);
   const hipStream_t s = as_stream(stream);
-  if (n_tokens > 16) hipLaunchKernelGGL((nf4_gemv_rows_kernel<1, 2>), grid, block, 0, s, a);
-  else if (best == 1) hipLaunchKernelGGL((nf4_gemv_rows_kernel<1, 1>), grid, block, 0, s, a);
-  else if (best == 2) hipLaunchKernelGGL((nf4_gemv_rows_kernel<2, 1>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((nf4_gemv_rows_kernel<4, 1>), grid, block, 0, s, a);
+  if (n_tokens > 16) launch_gemv<1, 2>(a, lut, s);
+  else if (best == 1) launch_gemv<1, 1>(a, lut, s);
+  else if (best == 2) launch_gemv<2, 1>(a, lut, s);
+  else launch_gemv<4, 1>(a, false, s);
   return check_launch("nf4_gemv");
 }
