@@ -667,43 +667,45 @@ int talm_dropout(const void* x, int64_t ldx, int64_t rows, int64_t cols, int32_t
 
 /*
  * The LoRA adapters' products with dropout on x (the mask of talm_dropout on x [n_tokens, k],
- * adapter g's with site_g), fp16 with fp32 sums, rank 16, 1 or 2 adapters; factor as above.
+ * adapter g's with site_g), fp16 with fp32 sums, rank 16; factor as above.
  *
- * talm_lora_down_drop: t[:, 16g:16g+16] = fp16(factor (keep_g x) A_g^T), ts = fp16(scaling_g times the
- * same sum); A_g f16 [16, k], k a multiple of 32; `workspace` holds
- * talm_lora_down_drop_workspace bytes (0: may be NULL).
+ * talm_lora_down_drop (1 or 2 adapters): t[:, 16g:16g+16] = fp16(factor (keep_g x) A_g^T), ts = fp16(scaling_g
+ * times the same sum); A_g f16 [16, k], k a multiple of 32.
  *
- * talm_lora_up: out [n_tokens, cols] = base + sum_g factor keep_g (u[:, 16g:16g+16] M_g^T), one rounding;
- * M_g f16 [cols, 16], or [16, cols] with m_kmajor; base NULL (0) or f16 [n_tokens, cols], may be out;
- * the mask on out's elements (p = 0: none). The adapter's output ts B^T, and with A and the masks
- * the input gradient u A.
+ * talm_lora_branch_fwd (one adapter): t f16 [n_tokens, 16] as above, y f16 [n_tokens, cols] = fp16(scaling t
+ * B^T), B f16 [cols, 16]; `workspace` holds talm_lora_branch_fwd_workspace bytes.
  *
- * talm_lora_wgrad_drop: dA_g [16, hidden] = factor u_g^T (keep_g x), dB_g [seg_g, 16] = scaling_g
- * dy[:, lo_g:lo_g+seg_g]^T t_g in grad_dtype (TALM_F32 or TALM_F16), summed in fp32 over the tokens in fixed chunks and those in order
- * (deterministic); zeros for no tokens. `workspace` holds talm_lora_wgrad_drop_workspace bytes.
+ * talm_lora_bwd_drop (1 or 2 adapters), u f16 = scaling_g dy_g B_g from talm_lora_down:
+ *   dA_g [16, hidden] = factor u_g^T (keep_g x), dB_g [seg_g, 16] = scaling_g dy[:, lo_g:lo_g+seg_g]^T t_g
+ *     in grad_dtype (TALM_F32 or TALM_F16), summed in fp32 over the tokens in fixed chunks and those in
+ *     order (deterministic), zeros for no tokens; all of them given, or none (NULL);
+ *   dx f16 [n_tokens, hidden] = base + sum_g factor keep_g (u_g A_g), one rounding; base NULL (0) or f16
+ *     [n_tokens, hidden], may be dx; dx NULL: not wanted.
+ * `workspace` holds talm_lora_bwd_drop_workspace bytes.
  *
- * Sizes and strides multiples of 8, operands 16-byte aligned. They replace the adapters' GEMMs
- * around native_dropout (solution/fused_proj.py:139-153, :188-215, solution/lora.py:183-231).
+ * Sizes and strides multiples of 8, operands and workspaces 16-byte aligned. They replace the
+ * adapters' GEMMs around native_dropout (solution/fused_proj.py:139-153, :188-215,
+ * solution/lora.py:183-231).
  */
-int64_t talm_lora_down_drop_workspace(int64_t n_tokens, int64_t k, int32_t n_adapters);
 int talm_lora_down_drop(const uint16_t* x, int64_t ldx, int64_t n_tokens, int64_t k,
                         const uint16_t* a0, const uint16_t* a1, int32_t n_adapters, float p,
                         const int64_t* key, uint32_t site0, uint32_t site1, float scaling0,
-                        float scaling1, uint16_t* t, uint16_t* ts, int64_t ldt, void* workspace,
-                        int64_t workspace_bytes, void* stream);
-int talm_lora_up(const uint16_t* u, int64_t ldu, int64_t n_tokens, int64_t cols, const uint16_t* m0,
-                 const uint16_t* m1, int32_t n_adapters, int32_t m_kmajor, float p,
-                 const int64_t* key, uint32_t site0, uint32_t site1, const uint16_t* base,
-                 int64_t ldb, uint16_t* out, int64_t ldo, void* stream);
-int64_t talm_lora_wgrad_drop_workspace(int64_t n_tokens, int64_t hidden, int32_t n_adapters,
-                                       int64_t seg0, int64_t seg1);
-int talm_lora_wgrad_drop(const uint16_t* x, int64_t ldx, const uint16_t* dy, int64_t ldy,
-                         const uint16_t* u, int64_t ldu, const uint16_t* t, int64_t ldt,
-                         int64_t n_tokens, int64_t hidden, int32_t n_adapters, float p,
-                         const int64_t* key, uint32_t site0, uint32_t site1, int32_t grad_dtype,
-                         int64_t lo0, int64_t seg0, float scaling0, void* da0, void* db0,
-                         int64_t lo1, int64_t seg1, float scaling1, void* da1, void* db1, void* workspace,
+                        float scaling1, uint16_t* t, uint16_t* ts, int64_t ldt, void* stream);
+int64_t talm_lora_branch_fwd_workspace(int64_t n_tokens, int64_t k);
+int talm_lora_branch_fwd(const uint16_t* x, int64_t ldx, int64_t n_tokens, int64_t k, int64_t cols,
+                         const uint16_t* a, const uint16_t* b, float p, const int64_t* key,
+                         uint32_t site, float scaling, uint16_t* t, uint16_t* y, void* workspace,
                          int64_t workspace_bytes, void* stream);
+int64_t talm_lora_bwd_drop_workspace(int64_t n_tokens, int64_t hidden, int32_t n_adapters,
+                                     int64_t seg0, int64_t seg1);
+int talm_lora_bwd_drop(const uint16_t* x, int64_t ldx, const uint16_t* dy, int64_t ldy,
+                       const uint16_t* u, int64_t ldu, const uint16_t* t, int64_t ldt,
+                       int64_t n_tokens, int64_t hidden, int32_t n_adapters, float p,
+                       const int64_t* key, uint32_t site0, uint32_t site1, int32_t grad_dtype,
+                       int64_t lo0, int64_t seg0, float scaling0, void* da0, void* db0, int64_t lo1,
+                       int64_t seg1, float scaling1, void* da1, void* db1, const uint16_t* a0,
+                       const uint16_t* a1, const uint16_t* base, int64_t ldb, uint16_t* dx,
+                       int64_t ldd, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Products of a few tokens with a weight W [rows, cols] in the NF4 form of talm_nf4_group_dequant

@@ -69,12 +69,12 @@ SIGNATURES = {
                              _I64, _P, _I64, _P],
     "talm_dropout": [_P, _I64, _I64, _I64, _I32, _F32, _P, _U32, _P, _I64, _P],
     "talm_lora_down_drop": [_P, _I64, _I64, _I64, _P, _P, _I32, _F32, _P, _U32, _U32, _F32, _F32, _P,
-                            _P, _I64, _P, _I64, _P],
-    "talm_lora_up": [_P, _I64, _I64, _I64, _P, _P, _I32, _I32, _F32, _P, _U32, _U32, _P, _I64, _P,
-                     _I64, _P],
-    "talm_lora_wgrad_drop": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I32, _F32, _P, _U32,
-                             _U32, _I32, _I64, _I64, _F32, _P, _P, _I64, _I64, _F32, _P, _P, _P, _I64,
+                            _P, _I64, _P],
+    "talm_lora_branch_fwd": [_P, _I64, _I64, _I64, _I64, _P, _P, _F32, _P, _U32, _F32, _P, _P, _P, _I64,
                              _P],
+    "talm_lora_bwd_drop": [_P, _I64, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I32, _F32, _P, _U32,
+                           _U32, _I32, _I64, _I64, _F32, _P, _P, _I64, _I64, _F32, _P, _P, _P, _P, _P,
+                           _I64, _P, _I64, _P, _I64, _P],
     "talm_nf4_gemv": [_P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _P, _P, _I64, _P,
                       _I64, _I64, _P, _I64, _I64, _P, _I64, _P],
     "talm_lora_mirror": [_P, _I32, _I64, _P, _P],
@@ -105,8 +105,8 @@ SIZE_FUNCTIONS = {
     "talm_lora_wgrad_workspace": [_I64, _I64, _I64, _I64],
     "talm_attn_bwd_workspace": [_I64, _I32],
     "talm_attn_window_bwd_workspace": [_I64, _I32, _I32, _I32, _I32, _I32],
-    "talm_lora_down_drop_workspace": [_I64, _I64, _I32],
-    "talm_lora_wgrad_drop_workspace": [_I64, _I64, _I32, _I64, _I64],
+    "talm_lora_branch_fwd_workspace": [_I64, _I64],
+    "talm_lora_bwd_drop_workspace": [_I64, _I64, _I32, _I64, _I64],
     "talm_gemm_splitk_workspace": [_I64, _I64, _I64],
     "talm_nf4_gemm_workspace": [_I64, _I64, _I64, _I32],
     "talm_gemm_splitk_parts": [_I64, _I64, _I64],

@@ -27,7 +27,7 @@ OPS = ("nf4_group_dequant", "nf4_group_dequant_streaming", "nf4_dequant", "rmsno
        "pack_rows", "row_stats", "head_loss", "scatter_rows", "head_order", "head_restore", "scale_rows",
        "gemm_splitk_partials", "nf4_gemm_partials", "splitk_add_rmsnorm", "splitk_rmsnorm_bwd",
        "rope_table", "lora_grad_norm", "lora_adamw_clipped", "attn_window_fwd",
-       "attn_window_bwd", "dropout", "lora_down_drop", "lora_up", "lora_wgrad_drop", "nf4_gemv")
+       "attn_window_bwd", "dropout", "lora_down_drop", "lora_bwd_drop", "nf4_gemv")
 
 _load_lock = threading.Lock()
 _loaded = False
@@ -86,15 +86,9 @@ def attn_window_bwd_workspace_bytes(n_tokens, n_q_heads, n_seqs, max_seqlen, win
     return int(size)
 
 
-def lora_down_drop_workspace_bytes(n_tokens, k, n_adapters):
-    size = _lib.lib().talm_lora_down_drop_workspace(n_tokens, k, n_adapters)
-    _require(size >= 0, "lora_down_drop: unsupported shape")
-    return int(size)
-
-
-def lora_wgrad_drop_workspace_bytes(n_tokens, hidden, n_adapters, seg0, seg1):
-    size = _lib.lib().talm_lora_wgrad_drop_workspace(n_tokens, hidden, n_adapters, seg0, seg1)
-    _require(size >= 0, "lora_wgrad_drop: unsupported shape")
+def lora_bwd_drop_workspace_bytes(n_tokens, hidden, n_adapters, seg0, seg1):
+    size = _lib.lib().talm_lora_bwd_drop_workspace(n_tokens, hidden, n_adapters, seg0, seg1)
+    _require(size >= 0, "lora_bwd_drop: unsupported shape")
     return int(size)
 
 

@@ -651,10 +651,13 @@ struct BwdArgs {
   float* far_v;
 };
 
-// The query row after the tiles of 64 rows that hold the window of any of a 128-key tile's keys: where
-// the items of its sinks' further rows begin.
-__device__ __forceinline__ int near_end(int k0, int len, int window) {
-  const int rows = min(len, k0 + 127 + window) - k0;
+// The query row after the tiles of 64 rows that hold the window of any of a 128-key tile's keys and, of
+// a tile with sinks, kFarSlack rows more: where the items of its sinks' further rows begin (rows that
+// are few more than a window get no item, no partial and no launch of their own).
+constexpr int kFarSlack = 512;
+__device__ __forceinline__ int near_end(int k0, int len, int window, int sinks) {
+  const int64_t end = static_cast<int64_t>(k0) + 127 + window + (k0 < sinks ? kFarSlack : 0);
+  const int rows = static_cast<int>(end < len ? end : len) - k0;
   return k0 + (rows + 63) / 64 * 64;
 }
 
@@ -1016,7 +1019,7 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
   // causal: rows below k0 see no key here (k0 is a multiple of 64)
   int qstart = k0, qstop = len;
   if constexpr (kWin) {
-    const int end = near_end(k0, len, a.window);
+    const int end = near_end(k0, len, a.window, a.sinks);
     if (chunk < 0) {
       qstop = min(len, end);
     } else {
@@ -1290,7 +1293,7 @@ __global__ __launch_bounds__(256) void attn_bwd_far_kernel(BwdArgs a) {
   const Rows own_rows = seq_rows<true>(a.cu, seq, a.n_tokens);
   const int s0 = own_rows.s0, len = own_rows.len;
   if (key >= len) return;
-  const int end = near_end(key / 128 * 128, len, a.window);
+  const int end = near_end(key / 128 * 128, len, a.window, a.sinks);
   const int chunks = min(a.far_chunks, (max(len - end, 0) + a.far_rows - 1) / a.far_rows);
   if (chunks == 0) return;
   const int64_t at = (static_cast<int64_t>(head) * a.n_tokens + s0 + key) * kD + c;
@@ -1652,7 +1655,7 @@ FarPlan far_plan(int64_t n_seqs, int64_t max_seqlen, int64_t n_q_heads, int64_t 
   FarPlan f;
   window = std::min(window, max_seqlen);
   sinks = std::min(sinks, max_seqlen);
-  const int64_t left = max_seqlen - (127 + window + 63) / 64 * 64;  // of the first key tile
+  const int64_t left = max_seqlen - (127 + window + kFarSlack + 63) / 64 * 64;  // of the first key tile
   if (sinks == 0 || left <= 0 || n_seqs == 0) return f;
   const int64_t one = n_seqs * n_q_heads * sinks * kD;
   const int64_t most = std::max<int64_t>(1, kFarBytes / (8 * one));

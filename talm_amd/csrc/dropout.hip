@@ -1,14 +1,14 @@
 // Dropout and the LoRA adapters' products with dropout on their input, for gfx950. No mask is
 // stored: every kernel computes it from the generator (philox.h).
 //
-//   dropout        y = keep x factor                       (the gradient: the same on dy)
-//   lora_down_drop t = factor (keep x) A^T, ts = s t       (rank 16; 1 or 2 adapters of one x, each
-//                                                           with a mask of its own)
-//   lora_up        out = base + sum_g factor keep_g (u_g M_g)   (y = ts B^T: no mask; the input
-//                                                           gradient u A under the masks)
-//   lora_wgrad_drop dA_g = factor u_g^T (keep_g x), dB_g = s_g dy_g^T t_g
+//   dropout          y = keep x factor                      (the gradient: the same on dy)
+//   lora_down_drop   t = factor (keep x) A^T, ts = s t      (rank 16; 1 or 2 adapters of one x, each
+//                                                            with a mask of its own)
+//   lora_branch_fwd  t, then y = s t B^T                    (one adapter)
+//   lora_bwd_drop    dA_g = factor u_g^T (keep_g x), dB_g = s_g dy_g^T t_g,
+//                    dx = base + sum_g factor keep_g (u_g A_g)
 // The adapters' arithmetic is PEFT's (solution/lora.py:183-231, solution/fused_proj.py:139-153,
-// :199-215) with x / (1 - p) not rounded on the way: the mask clears fp16 operands exactly and the
+// :188-215) with x / (1 - p) not rounded on the way: the mask clears fp16 operands exactly and the
 // factor goes on the fp32 sums.
 #include "mfma_tile.h"
 #include "philox.h"
@@ -99,16 +99,18 @@ struct DownArgs {
   const uint16_t* a[kMaxAdapters];  // [16][k]
   float scaling[kMaxAdapters];
   float factor;
-  DropArgs drop;                // adapter g's site: drop.site + site_step g
+  DropArgs drop;
   uint32_t site[kMaxAdapters];
   uint16_t* t;                  // [N][ldt], 16 columns per adapter
   uint16_t* ts;
   int64_t ldt;
-  float* part;                  // [parts][N][16 n_adapters] when parts > 1
+  float* part;                  // one adapter's sums [parts][N][16] instead (no factor), or null
 };
 
 constexpr int kDownWaves = 8;
 constexpr int kDownBatch = 4;
+constexpr int kDownMaxParts = 4;
+constexpr int64_t kDownCus = 256;  // the chip's CUs, for plans that a size query makes without a device
 
 // One workgroup per 16 tokens and part of the reduction; its wavefronts take the part's 32-deep
 // steps round-robin, the loads of kDownBatch of them before their MFMAs.
@@ -150,7 +152,7 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_drop_kernel(DownArg
       for (int g = 0; g < G; ++g) {
         DropKey kg = key;
         kg.site = a.site[g];
-        const uint4 xd = key.threshold ? keep8(xv[j], block, kg) : xv[j];
+        const uint4 xd = key.threshold ? keep8(xv[j], philox_block(block, kg), key.threshold) : xv[j];
         acc[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8(xd), h8(av[j][g]), acc[g], 0, 0, 0);
       }
     }
@@ -167,8 +169,8 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_drop_kernel(DownArg
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kDownWaves; ++w) sum += red[w][g][r][i];
-    if (a.parts > 1) {
-      a.part[(static_cast<int64_t>(blockIdx.y) * a.n_tokens + m0 + r) * (kRank * G) + g * kRank + i] = sum;
+    if (G == 1 && a.part) {
+      a.part[(static_cast<int64_t>(blockIdx.y) * a.n_tokens + m0 + r) * kRank + i] = sum;
     } else {
       const int64_t at = static_cast<int64_t>(m0 + r) * a.ldt + g * kRank + i;
       a.t[at] = f2h(a.factor * sum);
@@ -177,126 +179,84 @@ __global__ __launch_bounds__(64 * kDownWaves) void lora_down_drop_kernel(DownArg
   }
 }
 
-// The parts of a split reduction summed in order.
-__global__ __launch_bounds__(256) void lora_down_sum_kernel(DownArgs a) {
-  const int width = kRank * a.n_adapters;
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (e >= static_cast<int64_t>(a.n_tokens) * width) return;
-  const int64_t n = e / width;
-  const int i = static_cast<int>(e - n * width);
-  float sum = 0.f;
-  for (int p = 0; p < a.parts; ++p) sum += a.part[static_cast<int64_t>(p) * a.n_tokens * width + e];
-  a.t[n * a.ldt + i] = f2h(a.factor * sum);
-  a.ts[n * a.ldt + i] = f2h(a.scaling[i / kRank] * (a.factor * sum));
-}
-
 // ------------------------------------------------------------------------------------------
-// out = base + sum_g factor keep_g (u_g M_g)
+// y = s t B^T, t = factor times the parts of the down product
 // ------------------------------------------------------------------------------------------
 struct UpArgs {
-  const uint16_t* u;  // [N][ldu], 16 columns per adapter
-  int64_t ldu;
-  int n_tokens, cols, n_adapters, m_kmajor;
-  const uint16_t* m[kMaxAdapters];  // [cols][16], or with m_kmajor [16][cols]
-  float factor;
-  DropArgs drop;
-  uint32_t site[kMaxAdapters];
-  const uint16_t* base;  // [N][ldb] or null
-  int64_t ldb;
-  uint16_t* out;         // [N][ldo]; may be base
-  int64_t ldo;
+  const float* part;  // [parts][N][16]
+  int parts, n_tokens, cols;
+  float factor, scaling;
+  uint16_t* t;        // [N][16]: what the backward keeps
+  const uint16_t* b;  // [cols][16]
+  uint16_t* y;        // [N][cols]
 };
 
 constexpr int kUpTokens = 64;  // per workgroup, in blocks of 32
 
-// One wavefront per 32 columns. C[c][token] = M u^T (v_mfma_f32_32x32x16_f16, K = the rank): a lane
-// owns a token, and with row m of the A operand taken as column c(m) = 16 (m / 4 % 2) + 4 (m / 8) +
-// m % 4 of the block its 16 accumulators are the 16 consecutive columns 16 (lane / 32) .. + 15: two
-// blocks of the generator and two 16-byte stores.
-template <int G>
+// Column of a 32-column block that row m of the A operand holds, so that a lane's 16 accumulators (rows
+// 8 (v / 4) + 4 (lane / 32) + v % 4) are the 16 consecutive columns 16 (lane / 32) .. + 15.
+__device__ __forceinline__ int up_column(int m) { return 16 * ((m >> 2) & 1) + 4 * (m >> 3) + (m & 3); }
+
+// One wavefront per 32 columns: C[c][token] = B t^T (v_mfma_f32_32x32x16_f16, K = the rank), a lane owns
+// a token and 16 consecutive columns: two 16-byte stores. The parts (at most kDownMaxParts) are summed
+// here, in order, by every workgroup that reads them: one launch less than a sum of their own.
 __global__ __launch_bounds__(256) void lora_up_kernel(UpArgs a) {
   const int lane = threadIdx.x & 63, hh = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int c0 = blockIdx.x * 128 + 32 * wave;
   if (c0 >= a.cols) return;  // no barrier follows
-  const int cm = c0 + 16 * ((l32 >> 2) & 1) + 4 * (l32 >> 3) + (l32 & 3);
-  uint4 mf[G];
-#pragma unroll
-  for (int g = 0; g < G; ++g) {
-    mf[g] = make_uint4(0u, 0u, 0u, 0u);
-    if (cm < a.cols) {
-      if (a.m_kmajor) {
-        uint32_t h[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = a.m[g][static_cast<int64_t>(8 * hh + e) * a.cols + cm];
-        mf[g] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-      } else {
-        mf[g] = *reinterpret_cast<const uint4*>(a.m[g] + static_cast<int64_t>(cm) * kRank + 8 * hh);
-      }
-    }
-  }
-  const DropKey key(a.drop.key, 0, a.drop.threshold);
-  const int col = c0 + 16 * hh;  // the lane's first column
+  const int cm = min(c0 + up_column(l32), a.cols - 1), col = c0 + 16 * hh;
+  const uint4 bf = *reinterpret_cast<const uint4*>(a.b + static_cast<int64_t>(cm) * kRank + 8 * hh);
 #pragma unroll
   for (int tb = 0; tb < kUpTokens / 32; ++tb) {
     const int tok = blockIdx.y * kUpTokens + 32 * tb + l32;
     const bool in = tok < a.n_tokens;
-    const int tk = in ? tok : a.n_tokens - 1;
-    float sum[16];
+    const float* p = a.part + static_cast<int64_t>(in ? tok : a.n_tokens - 1) * kRank + 8 * hh;
+    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    // every part's loads before their adds: a part past the last is the last one again, adding 0
+    float4 lo[kDownMaxParts], hi[kDownMaxParts];
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      uint4 b = make_uint4(0u, 0u, 0u, 0u);
-      if (a.base && in && col + 8 * q < a.cols)
-        b = *reinterpret_cast<const uint4*>(a.base + static_cast<int64_t>(tk) * a.ldb + col + 8 * q);
-      const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sum[8 * q + 2 * e] = lo_f(w[e]);
-        sum[8 * q + 2 * e + 1] = hi_f(w[e]);
-      }
+    for (int i = 0; i < kDownMaxParts; ++i) {
+      const float* q = p + static_cast<int64_t>(min(i, a.parts - 1)) * a.n_tokens * kRank;
+      lo[i] = reinterpret_cast<const float4*>(q)[0];
+      hi[i] = reinterpret_cast<const float4*>(q)[1];
     }
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-      const uint4 uf = *reinterpret_cast<const uint4*>(a.u + static_cast<int64_t>(tk) * a.ldu + kRank * g + 8 * hh);
-      f32x16 acc;
-#pragma unroll
-      for (int v = 0; v < 16; ++v) acc[v] = 0.f;
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(h8(mf[g]), h8(uf), acc, 0, 0, 0);
-      DropKey kg = key;
-      kg.site = a.site[g];
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        uint4 bits = make_uint4(0u, 0u, 0u, 0u);
-        if (key.threshold)
-          bits = philox_block(static_cast<uint64_t>(tk) * (a.cols >> 3) + ((col >> 3) + q), kg);
-        const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t r = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
-          sum[8 * q + e] += r >= key.threshold ? a.factor * acc[8 * q + e] : 0.f;
-        }
-      }
+    for (int i = 0; i < kDownMaxParts; ++i) {
+      const float f = i < a.parts ? 1.f : 0.f;
+      s[0] += f * lo[i].x; s[1] += f * lo[i].y; s[2] += f * lo[i].z; s[3] += f * lo[i].w;
+      s[4] += f * hi[i].x; s[5] += f * hi[i].y; s[6] += f * hi[i].z; s[7] += f * hi[i].w;
     }
+    const float f = a.factor;
+    const uint4 tf = make_uint4(pack2(f * s[0], f * s[1]), pack2(f * s[2], f * s[3]), pack2(f * s[4], f * s[5]),
+                                pack2(f * s[6], f * s[7]));
+    if (c0 == 0 && in) *reinterpret_cast<uint4*>(a.t + static_cast<int64_t>(tok) * kRank + 8 * hh) = tf;
+    f32x16 acc;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[v] = 0.f;
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(h8(bf), h8(tf), acc, 0, 0, 0);
     if (!in) continue;
 #pragma unroll
     for (int q = 0; q < 2; ++q)
       if (col + 8 * q < a.cols) {
-        const float* s = sum + 8 * q;
-        *reinterpret_cast<uint4*>(a.out + static_cast<int64_t>(tok) * a.ldo + col + 8 * q) =
-            make_uint4(pack2(s[0], s[1]), pack2(s[2], s[3]), pack2(s[4], s[5]), pack2(s[6], s[7]));
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = a.scaling * acc[8 * q + e];
+        *reinterpret_cast<uint4*>(a.y + static_cast<int64_t>(tok) * a.cols + col + 8 * q) =
+            make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
       }
   }
 }
 
 // ------------------------------------------------------------------------------------------
-// dA_g = factor u_g^T (keep_g x), dB_g = s_g dy_g^T t_g
+// dA_g = factor u_g^T (keep_g x), dB_g = s_g dy_g^T t_g, dx = base + sum_g factor keep_g (u_g A_g)
 // ------------------------------------------------------------------------------------------
-struct WgradArgs {
+struct BwdArgs {
   const uint16_t* x;
   int64_t ldx;
   const uint16_t* dy;
   int64_t ldy;
-  const uint16_t* u;
+  const uint16_t* u;  // [N][ldu], 16 columns per adapter
   int64_t ldu;
   const uint16_t* t;
   int64_t ldt;
@@ -305,6 +265,11 @@ struct WgradArgs {
   float scaling[kMaxAdapters], factor;
   DropArgs drop;
   uint32_t site[kMaxAdapters];
+  const uint16_t* a[kMaxAdapters];  // [16][hidden]: for dx
+  const uint16_t* base;             // [N][ldb] or null
+  int64_t ldb;
+  uint16_t* dx;                     // [N][ldd] or null; may be base
+  int64_t ldd;
   // the reductions' columns one after the other: dA of each adapter, then dB of each, every one
   // padded to whole workgroups of 128
   int first[2 * kMaxAdapters + 1];
@@ -316,8 +281,8 @@ struct WgradArgs {
   void* db[kMaxAdapters];
 };
 
-constexpr int kWgTok = 64;
-constexpr int kWgLd = 128 + 16;  // halves per staged row: rows 32 bytes apart in the banks
+constexpr int kBwTok = 64;
+constexpr int kBwLd = 128 + 16;  // halves per staged row: rows 32 bytes apart in the banks
 
 // See read_tr_untracked of attn.hip: lane i of a group of 16 gets elements 0..3 = rows 0..3 of column i
 // of the 4 x 16 block whose row j / 4, columns 4 (j % 4) .. + 3 lane j points at.
@@ -329,31 +294,43 @@ __device__ __forceinline__ half8_t pair(half4_t lo, half4_t hi) {
   return __builtin_bit_cast(half8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// One workgroup per (128 columns of one reduction, chunk of tokens): 64 tokens at a time staged row
-// by row in LDS (masked on the way), the fragments read transposed; each wavefront 32 columns against
-// the 16 of u or t (v_mfma_f32_16x16x32_f16). The next tokens' loads are in flight meanwhile.
-__global__ __launch_bounds__(256) void lora_wgrad_drop_kernel(WgradArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t xs[kWgTok][kWgLd];
-  __shared__ __attribute__((aligned(16))) uint16_t ms[kWgTok][kRank + 8];
-  const int c0 = blockIdx.x * 128, tid = threadIdx.x, lane = tid & 63;
+// One workgroup per (128 columns, chunk of tokens); columns of x for every adapter, or of one adapter's
+// dy. 64 tokens at a time: the rows staged in LDS (x under each adapter's mask, computed once for the
+// weight gradient and dx), the next tokens' loads in flight meanwhile. Weight gradients: the fragments
+// read transposed, each wavefront 32 columns against the 16 of u or t (v_mfma_f32_16x16x32_f16). dx:
+// each wavefront 32 columns, C[c][token] = A^T u^T as in lora_up_kernel, its A fragment gathered once.
+template <int G>
+__global__ __launch_bounds__(256) void lora_bwd_drop_kernel(BwdArgs a) {
+  __shared__ __attribute__((aligned(16))) uint16_t xs[G][kBwTok][kBwLd];
+  __shared__ __attribute__((aligned(16))) uint16_t ms[G][kBwTok][kRank + 8];
+  __shared__ __attribute__((aligned(16))) uint8_t bits[G][kBwTok][16];
+  const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int job = 0;
-  while (job + 1 < 2 * a.n_adapters && c0 >= a.first[job + 1]) ++job;
-  const bool is_b = job >= a.n_adapters;
-  const int g = is_b ? job - a.n_adapters : job;
-  const int cb = c0 - a.first[job];                   // first column of the reduction
-  const int width = is_b ? a.seg[g] : a.hidden;
-  const uint16_t* src = is_b ? a.dy + a.lo[g] : a.x;
+  // x's column blocks come first (first[1] is one adapter's width), then each adapter's dy
+  const int x_blocks = a.first[1] >> 7;
+  const bool is_b = static_cast<int>(blockIdx.x) >= x_blocks;
+  int job = 0, c0 = blockIdx.x * 128;  // the reduction, and its first column here
+  if (is_b) {
+    c0 += (G - 1) * a.first[1];
+    job = G;
+    while (job + 1 < 2 * G && c0 >= a.first[job + 1]) ++job;
+  }
+  const int gb = is_b ? job - G : 0;       // the adapter of a dB block
+  const int n_g = is_b ? 1 : G;
+  const int cb = c0 - a.first[job];
+  const int width = is_b ? a.seg[gb] : a.hidden;
+  const uint16_t* src = is_b ? a.dy + a.lo[gb] : a.x;
   const int64_t ld = is_b ? a.ldy : a.ldx;
-  const uint16_t* mat = (is_b ? a.t : a.u) + kRank * g;
+  const uint16_t* mat = is_b ? a.t + kRank * gb : a.u;
   const int64_t ldm = is_b ? a.ldt : a.ldu;
-  const DropKey key(a.drop.key, a.site[g], is_b ? 0u : a.drop.threshold);
+  const uint32_t threshold = is_b ? 0u : a.drop.threshold;
+  const DropKey key(a.drop.key, 0, threshold);
   const int r_lo = blockIdx.y * a.chunk, r_hi = min(a.n_tokens, r_lo + a.chunk);
   // a thread's items: 16-byte chunk tid % 16 of rows tid / 16 + 16 i; of u / t threads 0..127 one chunk
   const int cc = cb + 8 * (tid & 15);
   const bool live = cc < width;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-  uint4 xv[4], mv;
+  uint4 xv[4], mv[G];
   auto load = [&](int r0) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -361,48 +338,129 @@ __global__ __launch_bounds__(256) void lora_wgrad_drop_kernel(WgradArgs a) {
       xv[i] = zero;
       if (live && r < r_hi) xv[i] = *reinterpret_cast<const uint4*>(src + static_cast<int64_t>(r) * ld + cc);
     }
-    mv = zero;
     const int r = r0 + (tid >> 1);
-    if (tid < 128 && r < r_hi) mv = *reinterpret_cast<const uint4*>(mat + static_cast<int64_t>(r) * ldm + 8 * (tid & 1));
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      mv[g] = zero;
+      if (g < n_g && tid < 128 && r < r_hi)
+        mv[g] = *reinterpret_cast<const uint4*>(mat + static_cast<int64_t>(r) * ldm + kRank * g + 8 * (tid & 1));
+    }
   };
-  f32x4 acc[2];
-  acc[0] = acc[1] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // dx: the adapters' A fragments, lane row l % 32 the column up_column of the wavefront's 32
+  const int l32 = lane & 31, hh = lane >> 5;
+  const bool has_dx = !is_b && a.dx != nullptr;
+  uint4 af[G];
+#pragma unroll
+  for (int g = 0; g < G; ++g) {
+    af[g] = zero;
+    const int c = cb + 32 * wave + up_column(l32);
+    if (has_dx && c < a.hidden) {
+      uint32_t h[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = a.a[g][static_cast<int64_t>(8 * hh + e) * a.hidden + c];
+      af[g] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+    }
+  }
+  f32x4 acc[G][2];
+#pragma unroll
+  for (int g = 0; g < G; ++g) acc[g][0] = acc[g][1] = f32x4{0.f, 0.f, 0.f, 0.f};
   load(r_lo);
   const int grp = lane >> 4, j = lane & 15;
-  for (int r0 = r_lo; r0 < r_hi; r0 += kWgTok) {
+  for (int r0 = r_lo; r0 < r_hi; r0 += kBwTok) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = (tid >> 4) + 16 * i;
-      const uint4 v = key.threshold
-                          ? keep8(xv[i], static_cast<uint64_t>(r0 + r) * (a.hidden >> 3) + (cc >> 3), key)
-                          : xv[i];
-      *reinterpret_cast<uint4*>(&xs[r][8 * (tid & 15)]) = v;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        if (g >= n_g) break;
+        uint4 v = xv[i];
+        if (threshold) {
+          DropKey kg = key;
+          kg.site = a.site[g];
+          const uint4 rnd = philox_block(static_cast<uint64_t>(r0 + r) * (a.hidden >> 3) + (cc >> 3), kg);
+          v = keep8(v, rnd, threshold);
+          if (has_dx) bits[g][r][tid & 15] = static_cast<uint8_t>(keep_bits(rnd, threshold));
+        }
+        *reinterpret_cast<uint4*>(&xs[g][r][8 * (tid & 15)]) = v;
+      }
     }
-    if (tid < 128) *reinterpret_cast<uint4*>(&ms[tid >> 1][8 * (tid & 1)]) = mv;
+    if (tid < 128)
+#pragma unroll
+      for (int g = 0; g < G; ++g) *reinterpret_cast<uint4*>(&ms[g][tid >> 1][8 * (tid & 1)]) = mv[g];
     __syncthreads();
-    if (r0 + kWgTok < r_hi) load(r0 + kWgTok);
+    if (r0 + kBwTok < r_hi) load(r0 + kBwTok);
+    if (has_dx) {
+      const int lc = 32 * wave + 16 * hh, col = cb + lc;  // the lane's 16 columns
 #pragma unroll
-    for (int ks = 0; ks < kWgTok / 32; ++ks) {
+      for (int tb = 0; tb < kBwTok / 32; ++tb) {
+        const int rl = 32 * tb + l32, tok = r0 + rl;
+        float sum[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sum[e] = 0.f;
+        if (a.base && tok < r_hi)
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            if (col + 8 * q < a.hidden) {
+              const uint4 b = *reinterpret_cast<const uint4*>(a.base + static_cast<int64_t>(tok) * a.ldb + col + 8 * q);
+              const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                sum[8 * q + 2 * e] = lo_f(w[e]);
+                sum[8 * q + 2 * e + 1] = hi_f(w[e]);
+              }
+            }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const uint4 uf = *reinterpret_cast<const uint4*>(&ms[g][rl][8 * hh]);
+          f32x16 d;
+#pragma unroll
+          for (int v = 0; v < 16; ++v) d[v] = 0.f;
+          d = __builtin_amdgcn_mfma_f32_32x32x16_f16(h8(af[g]), h8(uf), d, 0, 0, 0);
+          uint32_t keep = 0xffffu;
+          if (threshold) keep = *reinterpret_cast<const uint16_t*>(&bits[g][rl][lc >> 3]);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) sum[e] += keep >> e & 1 ? a.factor * d[e] : 0.f;
+        }
+        if (tok < r_hi)
+#pragma unroll
+          for (int q = 0; q < 2; ++q)
+            if (col + 8 * q < a.hidden) {
+              const float* s = sum + 8 * q;
+              *reinterpret_cast<uint4*>(a.dx + static_cast<int64_t>(tok) * a.ldd + col + 8 * q) =
+                  make_uint4(pack2(s[0], s[1]), pack2(s[2], s[3]), pack2(s[4], s[5]), pack2(s[6], s[7]));
+            }
+      }
+    }
+#pragma unroll
+    for (int ks = 0; ks < kBwTok / 32; ++ks) {
       const int k0 = 32 * ks + 8 * grp + (j >> 2);  // the lane's row of the first transposed read
-      const half8_t mb = pair(read_tr(&ms[k0][4 * (j & 3)]), read_tr(&ms[k0 + 4][4 * (j & 3)]));
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const int c = 32 * wave + 16 * b + 4 * (j & 3);
-        acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pair(read_tr(&xs[k0][c]), read_tr(&xs[k0 + 4][c])), mb,
-                                                       acc[b], 0, 0, 0);
+      for (int g = 0; g < G; ++g) {
+        if (g >= n_g) break;
+        const half8_t mb = pair(read_tr(&ms[g][k0][4 * (j & 3)]), read_tr(&ms[g][k0 + 4][4 * (j & 3)]));
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int c = 32 * wave + 16 * b + 4 * (j & 3);
+          acc[g][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pair(read_tr(&xs[g][k0][c]), read_tr(&xs[g][k0 + 4][c])),
+                                                            mb, acc[g][b], 0, 0, 0);
+        }
       }
     }
     __syncthreads();
   }
-  float* out = a.part + (static_cast<int64_t>(blockIdx.y) * a.cols + c0 + 32 * wave) * kRank;
 #pragma unroll
-  for (int b = 0; b < 2; ++b)
+  for (int g = 0; g < G; ++g) {
+    if (g >= n_g) break;
+    float* out = a.part + (static_cast<int64_t>(blockIdx.y) * a.cols + c0 + g * a.first[1] + 32 * wave) * kRank;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) out[(16 * b + 4 * grp + v) * kRank + j] = acc[b][v];
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) out[(16 * b + 4 * grp + v) * kRank + j] = acc[g][b][v];
+  }
 }
 
 // The chunks summed in order: one thread per (column, rank).
-__global__ __launch_bounds__(256) void lora_wgrad_sum_kernel(WgradArgs a) {
+__global__ __launch_bounds__(256) void lora_wgrad_sum_kernel(BwdArgs a) {
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (e >= static_cast<int64_t>(a.cols) * kRank) return;
   const int c = static_cast<int>(e / kRank), i = static_cast<int>(e % kRank);
@@ -436,20 +494,26 @@ int check_drop(const char* what, const int64_t* key, float p) {
   return TALM_OK;
 }
 
+// Parts of the branch's down product: about two workgroups per CU, at least two 32-deep steps for each
+// of a workgroup's wavefronts.
 int down_parts(int64_t n_tokens, int64_t k) {
-  (void)n_tokens;
-  (void)k;
-  return 1;
+  const int64_t blocks = std::max<int64_t>(1, (n_tokens + 15) / 16), steps = k / 32;
+  const int64_t most = std::min<int64_t>(kDownMaxParts, steps / (2 * kDownWaves));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(most, 2 * kDownCus / blocks)));
 }
 
-struct WgradPlan {
-  int64_t cols = 0, chunk = 0, chunks = 0;
+struct BwdPlan {
+  int64_t cols = 0, x_blocks = 0, chunk = 0, chunks = 0;
 };
-WgradPlan wgrad_plan(int64_t n_tokens, int64_t hidden, int64_t n_adapters, int64_t seg0, int64_t seg1) {
+BwdPlan bwd_plan(int64_t n_tokens, int64_t hidden, int64_t n_adapters, int64_t seg0, int64_t seg1) {
   auto pad = [](int64_t n) { return (n + 127) / 128 * 128; };
-  WgradPlan w;
+  BwdPlan w;
+  w.x_blocks = pad(hidden) / 128;
   w.cols = n_adapters * pad(hidden) + pad(seg0) + (n_adapters > 1 ? pad(seg1) : 0);
-  w.chunk = 128;
+  // 128 tokens to a partial while that gives the chip three rounds of workgroups at most, whole multiples
+  // of it from there on: fewer partials to write and sum
+  const int64_t blocks = w.cols / 128 - (n_adapters - 1) * w.x_blocks;
+  w.chunk = 128 * std::max<int64_t>(1, (n_tokens + 127) / 128 * blocks / (3 * kDownCus));
   w.chunks = std::max<int64_t>(1, (n_tokens + w.chunk - 1) / w.chunk);
   return w;
 }
@@ -488,17 +552,22 @@ TALM_API int talm_dropout(const void* x, int64_t ldx, int64_t rows, int64_t cols
   return check_launch("dropout");
 }
 
-TALM_API int64_t talm_lora_down_drop_workspace(int64_t n_tokens, int64_t k, int32_t n_adapters) {
-  if (n_tokens < 0 || k < 32 || k % 32 || n_adapters < 1 || n_adapters > kMaxAdapters) return -1;
-  const int parts = down_parts(n_tokens, k);
-  return parts > 1 ? parts * n_tokens * kRank * n_adapters * 4 : 0;
+namespace talm {
+namespace {
+
+void launch_down(const DownArgs& a, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>((a.n_tokens + 15) / 16), static_cast<unsigned>(a.parts));
+  if (a.n_adapters > 1) hipLaunchKernelGGL(lora_down_drop_kernel<2>, grid, dim3(64 * kDownWaves), 0, s, a);
+  else hipLaunchKernelGGL(lora_down_drop_kernel<1>, grid, dim3(64 * kDownWaves), 0, s, a);
 }
+
+}  // namespace
+}  // namespace talm
 
 TALM_API int talm_lora_down_drop(const uint16_t* x, int64_t ldx, int64_t n_tokens, int64_t k,
                                  const uint16_t* a0, const uint16_t* a1, int32_t n_adapters, float p,
                                  const int64_t* key, uint32_t site0, uint32_t site1, float scaling0,
-                                 float scaling1, uint16_t* t, uint16_t* ts, int64_t ldt, void* workspace,
-                                 int64_t workspace_bytes, void* stream) {
+                                 float scaling1, uint16_t* t, uint16_t* ts, int64_t ldt, void* stream) {
   const bool two = n_adapters > 1;
   if (n_tokens < 0 || n_tokens > (1 << 30) || n_adapters < 1 || n_adapters > kMaxAdapters || k < 32 || k % 32 ||
       ldx < k || ldx % 8 || ldt < kRank * n_adapters || !fits32(16, ldx) || !fits32(16, k))
@@ -514,101 +583,107 @@ TALM_API int talm_lora_down_drop(const uint16_t* x, int64_t ldx, int64_t n_token
     return fail(TALM_EINVAL, "lora_down_drop: x and the A matrices must be 16-byte aligned");
   DownArgs a{};
   a.x = x; a.ldx = ldx; a.n_tokens = static_cast<int>(n_tokens); a.k = static_cast<int>(k);
-  a.n_adapters = n_adapters; a.parts = down_parts(n_tokens, k);
+  a.n_adapters = n_adapters; a.parts = 1;
   a.a[0] = a0; a.a[1] = two ? a1 : a0;
   a.scaling[0] = scaling0; a.scaling[1] = scaling1;
   a.drop = DropArgs{key, 0, drop_threshold(p)};
   a.site[0] = site0; a.site[1] = site1;
   a.factor = drop_factor(a.drop.threshold);
   a.t = t; a.ts = ts; a.ldt = ldt;
-  const int64_t need = talm_lora_down_drop_workspace(n_tokens, k, n_adapters);
-  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
-    return fail(TALM_EINVAL, "lora_down_drop: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
-  a.part = static_cast<float*>(workspace);
-  const dim3 grid(static_cast<unsigned>((n_tokens + 15) / 16), static_cast<unsigned>(a.parts));
-  const hipStream_t s = as_stream(stream);
-  if (two) hipLaunchKernelGGL(lora_down_drop_kernel<2>, grid, dim3(64 * kDownWaves), 0, s, a);
-  else hipLaunchKernelGGL(lora_down_drop_kernel<1>, grid, dim3(64 * kDownWaves), 0, s, a);
-  if (a.parts > 1) {
-    const int64_t n = n_tokens * kRank * n_adapters;
-    hipLaunchKernelGGL(lora_down_sum_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s, a);
-  }
+  launch_down(a, as_stream(stream));
   return check_launch("lora_down_drop");
 }
 
-TALM_API int talm_lora_up(const uint16_t* u, int64_t ldu, int64_t n_tokens, int64_t cols, const uint16_t* m0,
-                          const uint16_t* m1, int32_t n_adapters, int32_t m_kmajor, float p, const int64_t* key,
-                          uint32_t site0, uint32_t site1, const uint16_t* base, int64_t ldb, uint16_t* out,
-                          int64_t ldo, void* stream) {
-  const bool two = n_adapters > 1;
-  if (n_tokens < 0 || n_tokens > kUpTokens * int64_t{65535} || n_adapters < 1 || n_adapters > kMaxAdapters || cols < 8 || cols % 8 ||
-      cols > (1 << 30) || ldu < kRank * n_adapters || ldu % 8 || ldo < cols || ldo % 8 ||
-      (base && (ldb < cols || ldb % 8)))
-    return fail(TALM_EINVAL,
-                "lora_up: bad shape (tokens %lld, columns %lld, ldu %lld, ldb %lld, ldo %lld, adapters %d): "
-                "columns and strides multiples of 8, 1-2 adapters of rank 16",
-                (long long)n_tokens, (long long)cols, (long long)ldu, (long long)ldb, (long long)ldo, n_adapters);
-  const int status = check_drop("lora_up", key, p);
-  if (status != TALM_OK) return status;
-  if (n_tokens == 0) return ok();
-  if (!u || !m0 || (two && !m1) || !out) return fail(TALM_EINVAL, "lora_up: null pointer");
-  if (!aligned(u, 16) || !aligned(out, 16) || (base && !aligned(base, 16)) ||
-      (!m_kmajor && (!aligned(m0, 16) || (two && !aligned(m1, 16)))))
-    return fail(TALM_EINVAL, "lora_up: operands must be 16-byte aligned");
-  UpArgs a{};
-  a.u = u; a.ldu = ldu; a.n_tokens = static_cast<int>(n_tokens); a.cols = static_cast<int>(cols);
-  a.n_adapters = n_adapters; a.m_kmajor = m_kmajor;
-  a.m[0] = m0; a.m[1] = two ? m1 : m0;
-  a.drop = DropArgs{key, 0, drop_threshold(p)};
-  a.site[0] = site0; a.site[1] = site1;
-  a.factor = drop_factor(a.drop.threshold);
-  a.base = base; a.ldb = ldb; a.out = out; a.ldo = ldo;
-  const dim3 grid(static_cast<unsigned>((cols + 127) / 128),
-                  static_cast<unsigned>((n_tokens + kUpTokens - 1) / kUpTokens));
-  if (two) hipLaunchKernelGGL(lora_up_kernel<2>, grid, dim3(256), 0, as_stream(stream), a);
-  else hipLaunchKernelGGL(lora_up_kernel<1>, grid, dim3(256), 0, as_stream(stream), a);
-  return check_launch("lora_up");
+TALM_API int64_t talm_lora_branch_fwd_workspace(int64_t n_tokens, int64_t k) {
+  if (n_tokens < 0 || n_tokens > (1 << 30) || k < 32 || k % 32) return -1;
+  return down_parts(n_tokens, k) * n_tokens * kRank * 4;
 }
 
-TALM_API int64_t talm_lora_wgrad_drop_workspace(int64_t n_tokens, int64_t hidden, int32_t n_adapters, int64_t seg0,
-                                                int64_t seg1) {
+TALM_API int talm_lora_branch_fwd(const uint16_t* x, int64_t ldx, int64_t n_tokens, int64_t k, int64_t cols,
+                                  const uint16_t* a_, const uint16_t* b, float p, const int64_t* key,
+                                  uint32_t site, float scaling, uint16_t* t, uint16_t* y, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  const int64_t need = talm_lora_branch_fwd_workspace(n_tokens, k);
+  if (need < 0 || n_tokens > kUpTokens * int64_t{65535} || ldx < k || ldx % 8 || cols < 8 || cols % 8 ||
+      cols > (1 << 30) || !fits32(16, ldx) || !fits32(16, k))
+    return fail(TALM_EINVAL,
+                "lora_branch_fwd: bad shape (tokens %lld, k %lld, ldx %lld, columns %lld): k a multiple of 32 "
+                "inside x's rows of a multiple of 8, columns a multiple of 8",
+                (long long)n_tokens, (long long)k, (long long)ldx, (long long)cols);
+  const int status = check_drop("lora_branch_fwd", key, p);
+  if (status != TALM_OK) return status;
+  if (n_tokens == 0) return ok();
+  if (!x || !a_ || !b || !t || !y) return fail(TALM_EINVAL, "lora_branch_fwd: null pointer");
+  if (!aligned(x, 16) || !aligned(a_, 16) || !aligned(b, 16) || !aligned(t, 16) || !aligned(y, 16))
+    return fail(TALM_EINVAL, "lora_branch_fwd: operands must be 16-byte aligned");
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
+    return fail(TALM_EINVAL, "lora_branch_fwd: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
+  DownArgs d{};
+  d.x = x; d.ldx = ldx; d.n_tokens = static_cast<int>(n_tokens); d.k = static_cast<int>(k);
+  d.n_adapters = 1; d.parts = down_parts(n_tokens, k);
+  d.a[0] = d.a[1] = a_;
+  d.drop = DropArgs{key, 0, drop_threshold(p)};
+  d.site[0] = site;
+  d.part = static_cast<float*>(workspace);
+  const hipStream_t s = as_stream(stream);
+  launch_down(d, s);
+  UpArgs u{};
+  u.part = d.part; u.parts = d.parts; u.n_tokens = d.n_tokens; u.cols = static_cast<int>(cols);
+  u.factor = drop_factor(d.drop.threshold); u.scaling = scaling;
+  u.t = t; u.b = b; u.y = y;
+  hipLaunchKernelGGL(lora_up_kernel,
+                     dim3(static_cast<unsigned>((cols + 127) / 128),
+                          static_cast<unsigned>((n_tokens + kUpTokens - 1) / kUpTokens)),
+                     dim3(256), 0, s, u);
+  return check_launch("lora_branch_fwd");
+}
+
+TALM_API int64_t talm_lora_bwd_drop_workspace(int64_t n_tokens, int64_t hidden, int32_t n_adapters, int64_t seg0,
+                                              int64_t seg1) {
   if (n_tokens < 0 || n_tokens > (1 << 30) || hidden < 8 || hidden % 8 || hidden > (1 << 26) || n_adapters < 1 ||
       n_adapters > kMaxAdapters || seg0 < 8 || seg0 % 8 || seg0 > (1 << 26) ||
       (n_adapters > 1 && (seg1 < 8 || seg1 % 8 || seg1 > (1 << 26))))
     return -1;
-  const WgradPlan w = wgrad_plan(n_tokens, hidden, n_adapters, seg0, seg1);
+  const BwdPlan w = bwd_plan(n_tokens, hidden, n_adapters, seg0, seg1);
   return w.chunks > 65535 ? -1 : w.chunks * w.cols * kRank * 4;
 }
 
-TALM_API int talm_lora_wgrad_drop(const uint16_t* x, int64_t ldx, const uint16_t* dy, int64_t ldy,
-                                  const uint16_t* u, int64_t ldu, const uint16_t* t, int64_t ldt,
-                                  int64_t n_tokens, int64_t hidden, int32_t n_adapters, float p,
-                                  const int64_t* key, uint32_t site0, uint32_t site1, int32_t grad_dtype,
-                                  int64_t lo0, int64_t seg0, float scaling0, void* da0, void* db0,
-                                  int64_t lo1, int64_t seg1, float scaling1, void* da1, void* db1, void* workspace,
-                                  int64_t workspace_bytes, void* stream) {
+TALM_API int talm_lora_bwd_drop(const uint16_t* x, int64_t ldx, const uint16_t* dy, int64_t ldy,
+                                const uint16_t* u, int64_t ldu, const uint16_t* t, int64_t ldt,
+                                int64_t n_tokens, int64_t hidden, int32_t n_adapters, float p,
+                                const int64_t* key, uint32_t site0, uint32_t site1, int32_t grad_dtype,
+                                int64_t lo0, int64_t seg0, float scaling0, void* da0, void* db0, int64_t lo1,
+                                int64_t seg1, float scaling1, void* da1, void* db1, const uint16_t* a0,
+                                const uint16_t* a1, const uint16_t* base, int64_t ldb, uint16_t* dx, int64_t ldd,
+                                void* workspace, int64_t workspace_bytes, void* stream) {
   const bool two = n_adapters > 1;
-  const int64_t need = talm_lora_wgrad_drop_workspace(n_tokens, hidden, n_adapters, seg0, seg1);
+  const int64_t need = talm_lora_bwd_drop_workspace(n_tokens, hidden, n_adapters, seg0, seg1);
   if (need < 0 || ldx < hidden || ldx % 8 || ldy % 8 || lo0 < 0 || lo0 % 8 || lo0 + seg0 > ldy ||
       (two && (lo1 < 0 || lo1 % 8 || lo1 + seg1 > ldy)) || ldu < kRank * n_adapters || ldu % 8 ||
-      ldt < kRank * n_adapters || ldt % 8)
+      ldt < kRank * n_adapters || ldt % 8 ||
+      (dx && (ldd < hidden || ldd % 8 || (base && (ldb < hidden || ldb % 8)))))
     return fail(TALM_EINVAL,
-                "lora_wgrad_drop: bad shape (tokens %lld, hidden %lld, segments %lld/%lld at %lld/%lld, strides "
+                "lora_bwd_drop: bad shape (tokens %lld, hidden %lld, segments %lld/%lld at %lld/%lld, strides "
                 "%lld/%lld/%lld/%lld, adapters %d): sizes and strides multiples of 8, 1-2 adapters of rank 16",
                 (long long)n_tokens, (long long)hidden, (long long)seg0, (long long)seg1, (long long)lo0,
                 (long long)lo1, (long long)ldx, (long long)ldy, (long long)ldu, (long long)ldt, n_adapters);
   if (grad_dtype != TALM_F32 && grad_dtype != TALM_F16)
-    return fail(TALM_EINVAL, "lora_wgrad_drop: gradients of dtype %d", grad_dtype);
-  const int status = check_drop("lora_wgrad_drop", key, p);
+    return fail(TALM_EINVAL, "lora_bwd_drop: gradients of dtype %d", grad_dtype);
+  const int status = check_drop("lora_bwd_drop", key, p);
   if (status != TALM_OK) return status;
-  if (!da0 || !db0 || (two && (!da1 || !db1))) return fail(TALM_EINVAL, "lora_wgrad_drop: null pointer");
-  if (n_tokens > 0 && (!x || !dy || !u || !t)) return fail(TALM_EINVAL, "lora_wgrad_drop: null pointer");
-  if (!aligned(x, 16) || !aligned(dy, 16) || !aligned(u, 16) || !aligned(t, 16))
-    return fail(TALM_EINVAL, "lora_wgrad_drop: operands must be 16-byte aligned");
+  const bool grads = da0 != nullptr;
+  if (grads ? !db0 || (two && (!da1 || !db1)) : db0 || da1 || db1)
+    return fail(TALM_EINVAL, "lora_bwd_drop: the weight gradients are given all or none");
+  if (!grads && !dx) return ok();
+  if (n_tokens > 0 && (!x || !dy || !u || !t || (dx && (!a0 || (two && !a1)))))
+    return fail(TALM_EINVAL, "lora_bwd_drop: null pointer");
+  if (!aligned(x, 16) || !aligned(dy, 16) || !aligned(u, 16) || !aligned(t, 16) || !aligned(base, 16) ||
+      !aligned(dx, 16))
+    return fail(TALM_EINVAL, "lora_bwd_drop: operands must be 16-byte aligned");
   if (!workspace || workspace_bytes < need || !aligned(workspace, 16))
-    return fail(TALM_EINVAL, "lora_wgrad_drop: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
-  const WgradPlan w = wgrad_plan(n_tokens, hidden, n_adapters, seg0, seg1);
-  WgradArgs a{};
+    return fail(TALM_EINVAL, "lora_bwd_drop: a 16-byte aligned workspace of %lld bytes is needed", (long long)need);
+  const BwdPlan w = bwd_plan(n_tokens, hidden, n_adapters, seg0, seg1);
+  BwdArgs a{};
   a.x = x; a.ldx = ldx; a.dy = dy; a.ldy = ldy; a.u = u; a.ldu = ldu; a.t = t; a.ldt = ldt;
   a.n_tokens = static_cast<int>(n_tokens); a.hidden = static_cast<int>(hidden); a.n_adapters = n_adapters;
   a.lo[0] = static_cast<int>(lo0); a.lo[1] = static_cast<int>(lo1);
@@ -617,6 +692,8 @@ TALM_API int talm_lora_wgrad_drop(const uint16_t* x, int64_t ldx, const uint16_t
   a.drop = DropArgs{key, 0, drop_threshold(p)};
   a.site[0] = site0; a.site[1] = site1;
   a.factor = drop_factor(a.drop.threshold);
+  a.a[0] = a0; a.a[1] = two ? a1 : a0;
+  a.base = base; a.ldb = ldb; a.dx = dx; a.ldd = ldd;
   auto pad = [](int64_t n) { return static_cast<int>((n + 127) / 128 * 128); };
   for (int job = 0; job < 2 * n_adapters; ++job)
     a.first[job + 1] = a.first[job] + pad(job < n_adapters ? a.hidden : a.seg[job - n_adapters]);
@@ -626,9 +703,12 @@ TALM_API int talm_lora_wgrad_drop(const uint16_t* x, int64_t ldx, const uint16_t
   a.half_out = grad_dtype == TALM_F16;
   a.da[0] = da0; a.da[1] = da1; a.db[0] = db0; a.db[1] = db1;
   const hipStream_t s = as_stream(stream);
-  hipLaunchKernelGGL(lora_wgrad_drop_kernel, dim3(static_cast<unsigned>(w.cols / 128), static_cast<unsigned>(w.chunks)),
-                     dim3(256), 0, s, a);
-  hipLaunchKernelGGL(lora_wgrad_sum_kernel, dim3(static_cast<unsigned>((w.cols * kRank + 255) / 256)), dim3(256), 0,
-                     s, a);
-  return check_launch("lora_wgrad_drop");
+  const int64_t blocks = w.cols / 128 - (n_adapters - 1) * w.x_blocks;  // x's blocks serve every adapter
+  const dim3 grid(static_cast<unsigned>(grads ? blocks : w.x_blocks), static_cast<unsigned>(w.chunks));
+  if (two) hipLaunchKernelGGL(lora_bwd_drop_kernel<2>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(lora_bwd_drop_kernel<1>, grid, dim3(256), 0, s, a);
+  if (grads)
+    hipLaunchKernelGGL(lora_wgrad_sum_kernel, dim3(static_cast<unsigned>((w.cols * kRank + 255) / 256)), dim3(256), 0,
+                       s, a);
+  return check_launch("lora_bwd_drop");
 }

@@ -38,15 +38,19 @@ struct DropKey {
   }
 };
 
+__device__ __forceinline__ uint32_t xor3(uint32_t a, uint32_t b, uint32_t c) {
+  return __builtin_amdgcn_bitop3_b32(a, b, c, 0x96);  // v_bitop3_b32 with the table of a ^ b ^ c
+}
+
 __device__ __forceinline__ uint4 philox_block(uint64_t block, const DropKey& d) {
   uint32_t c0 = static_cast<uint32_t>(block), c1 = static_cast<uint32_t>(block >> 32), c2 = d.site,
            c3 = d.word3, k0 = d.k0, k1 = d.k1;
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t a = static_cast<uint64_t>(c0) * 0xD2511F53u, b = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
-    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
+    c0 = xor3(static_cast<uint32_t>(b >> 32), c1, k0);
     c1 = static_cast<uint32_t>(b);
-    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
+    c2 = xor3(static_cast<uint32_t>(a >> 32), c3, k1);
     c3 = static_cast<uint32_t>(a);
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
@@ -60,11 +64,19 @@ __device__ __forceinline__ uint32_t keep2(uint32_t x, uint32_t bits, uint32_t th
   const uint32_t hi = (bits >> 16) >= threshold ? 0xffff0000u : 0u;
   return x & (lo | hi);
 }
-// Eight of them, columns 8 b .. 8 b + 7 of the row whose blocks begin at `row_block`.
-__device__ __forceinline__ uint4 keep8(uint4 x, uint64_t block, const DropKey& d) {
-  const uint4 r = philox_block(block, d);
-  return make_uint4(keep2(x.x, r.x, d.threshold), keep2(x.y, r.y, d.threshold),
-                    keep2(x.z, r.z, d.threshold), keep2(x.w, r.w, d.threshold));
+// Eight of them: the columns of block `r`.
+__device__ __forceinline__ uint4 keep8(uint4 x, uint4 r, uint32_t threshold) {
+  return make_uint4(keep2(x.x, r.x, threshold), keep2(x.y, r.y, threshold), keep2(x.z, r.z, threshold),
+                    keep2(x.w, r.w, threshold));
+}
+// Bit e: column e of the block is kept.
+__device__ __forceinline__ uint32_t keep_bits(uint4 r, uint32_t threshold) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  uint32_t bits = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    bits |= ((e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu) >= threshold ? 1u : 0u) << e;
+  return bits;
 }
 
 inline uint32_t drop_threshold(float p) {

@@ -798,7 +798,7 @@ void dropout(const Tensor& x, double p, const OptTensor& key, int64_t site, cons
 // t and ts [N, 16 per adapter] = factor (keep x) A^T, scaling times it.
 void lora_down_drop(const Tensor& x, const Tensor& a0, const OptTensor& a1, double p, const OptTensor& key,
                     int64_t site0, int64_t site1, double scaling0, double scaling1, const Tensor& t,
-                    const Tensor& ts, const OptTensor& workspace) {
+                    const Tensor& ts) {
   const bool two = a1.has_value();
   half_rows(x, x, "lora_down_drop: x");
   half_rows(t, x, "lora_down_drop: t");
@@ -809,84 +809,64 @@ void lora_down_drop(const Tensor& x, const Tensor& a0, const OptTensor& a1, doub
             "lora_down_drop: A float16 [16, k], contiguous, on x's device");
   require(same_shape(t, x.size(0), two ? 32 : 16) && ts.sizes() == t.sizes() && row_stride(ts) == row_stride(t),
           "lora_down_drop: t, ts [N, 16 per adapter] of one layout");
-  if (workspace.has_value())
-    require(workspace->is_cuda() && workspace->is_contiguous() && workspace->device() == x.device(),
-            "lora_down_drop: workspace");
   const c10::DeviceGuard guard(x.device());
   check(talm_lora_down_drop(as<uint16_t>(x), row_stride(x), x.size(0), x.size(1), as<uint16_t>(a0),
                             as<uint16_t>(a1), two ? 2 : 1, static_cast<float>(p), drop_key(key, x),
                             drop_site(site0), drop_site(site1), static_cast<float>(scaling0),
                             static_cast<float>(scaling1), as<uint16_t>(t), as<uint16_t>(ts), row_stride(t),
-                            ptr(workspace),
-                            workspace.has_value()
-                                ? workspace->numel() * static_cast<int64_t>(workspace->element_size())
-                                : 0,
                             stream_of(x)),
         "lora_down_drop");
 }
 
-// out [N, cols] = base + sum_g factor keep_g (u_g M_g^T); M [cols, 16], or [16, cols] with m_kmajor.
-void lora_up(const Tensor& u, const Tensor& m0, const OptTensor& m1, bool m_kmajor, double p,
-             const OptTensor& key, int64_t site0, int64_t site1, const OptTensor& base, const Tensor& out) {
-  const bool two = m1.has_value();
-  half_rows(u, u, "lora_up: u");
-  half_rows(out, u, "lora_up: out");
-  require(u.size(1) >= (two ? 32 : 16) && u.size(0) == out.size(0), "lora_up: u [N, 16 per adapter], out [N, cols]");
-  const int64_t cols = out.size(1);
-  for (const Tensor* m : {&m0, two ? &*m1 : &m0})
-    require(m->is_cuda() && m->scalar_type() == at::kHalf && m->device() == u.device() && m->is_contiguous() &&
-                (m_kmajor ? same_shape(*m, 16, cols) : same_shape(*m, cols, 16)),
-            "lora_up: M float16 [cols, 16] ([16, cols] with m_kmajor), contiguous, on u's device");
-  if (base.has_value()) {
-    half_rows(*base, u, "lora_up: base");
-    require(base->sizes() == out.sizes(), "lora_up: base of out's shape");
-  }
-  const c10::DeviceGuard guard(u.device());
-  check(talm_lora_up(as<uint16_t>(u), row_stride(u), u.size(0), cols, as<uint16_t>(m0), as<uint16_t>(m1),
-                     two ? 2 : 1, m_kmajor, static_cast<float>(p), drop_key(key, u), drop_site(site0),
-                     drop_site(site1), as<uint16_t>(base), base.has_value() ? row_stride(*base) : 0,
-                     as<uint16_t>(out), row_stride(out), stream_of(u)),
-        "lora_up");
-}
-
-void lora_wgrad_drop(const Tensor& x, const Tensor& dy, const Tensor& u, const Tensor& t, double p,
-                     const OptTensor& key, int64_t site0, int64_t site1, int64_t lo0, int64_t seg0,
-                     double scaling0, const Tensor& da0, const Tensor& db0, int64_t lo1, int64_t seg1,
-                     double scaling1, const OptTensor& da1, const OptTensor& db1, const Tensor& workspace) {
-  const bool two = da1.has_value();
-  require(two == db1.has_value(), "lora_wgrad_drop: dA and dB of the second adapter both or neither");
-  half_rows(x, x, "lora_wgrad_drop: x");
-  half_rows(dy, x, "lora_wgrad_drop: dy");
-  half_rows(u, x, "lora_wgrad_drop: u");
-  half_rows(t, x, "lora_wgrad_drop: t");
-  const int64_t n = x.size(0), hidden = x.size(1), rank = two ? 32 : 16;
+// The adapters' dA, dB and (with dx) their input gradient under the masks, added to base.
+void lora_bwd_drop(const Tensor& x, const Tensor& dy, const Tensor& u, const Tensor& t, double p,
+                   const OptTensor& key, int64_t site0, int64_t site1, int64_t lo0, int64_t seg0,
+                   double scaling0, const OptTensor& da0, const OptTensor& db0, int64_t lo1, int64_t seg1,
+                   double scaling1, const OptTensor& da1, const OptTensor& db1, const OptTensor& a0,
+                   const OptTensor& a1, const OptTensor& base, const OptTensor& dx, const Tensor& workspace) {
+  const int64_t n = x.size(0), hidden = x.size(1), rank = u.size(1);
+  const bool two = rank == 32;
+  half_rows(x, x, "lora_bwd_drop: x");
+  half_rows(dy, x, "lora_bwd_drop: dy");
+  half_rows(u, x, "lora_bwd_drop: u");
+  half_rows(t, x, "lora_bwd_drop: t");
+  require(rank == 16 || rank == 32, "lora_bwd_drop: u [N, 16 per adapter], one or two adapters");
   require(dy.size(0) == n && same_shape(u, n, rank) && same_shape(t, n, rank),
-          "lora_wgrad_drop: dy [N, ..], u and t [N, 16 per adapter]");
+          "lora_bwd_drop: dy [N, ..], u and t [N, 16 per adapter]");
   require(lo0 >= 0 && seg0 >= 0 && lo0 + seg0 <= dy.size(1) &&
               (!two || (lo1 >= 0 && seg1 >= 0 && lo1 + seg1 <= dy.size(1))),
-          "lora_wgrad_drop: segments inside dy's columns");
-  const at::ScalarType type = da0.scalar_type();
-  auto grad = [&](const Tensor& g, int64_t r, int64_t c) {
-    require(g.is_cuda() && g.device() == x.device() && g.scalar_type() == type && g.is_contiguous() &&
-                same_shape(g, r, c),
-            "lora_wgrad_drop: dA [16, hidden], dB [segment, 16], contiguous, of one type");
+          "lora_bwd_drop: segments inside dy's columns");
+  const at::ScalarType type = da0.has_value() ? da0->scalar_type() : at::kFloat;
+  auto grad = [&](const OptTensor& g, int64_t r, int64_t c) {
+    require(!g.has_value() || (g->is_cuda() && g->device() == x.device() && g->scalar_type() == type &&
+                               g->is_contiguous() && same_shape(*g, r, c)),
+            "lora_bwd_drop: dA [16, hidden], dB [segment, 16], contiguous, of one type");
   };
   grad(da0, 16, hidden);
   grad(db0, seg0, 16);
-  if (two) {
-    grad(*da1, 16, hidden);
-    grad(*db1, seg1, 16);
-  }
+  grad(da1, 16, hidden);
+  grad(db1, seg1, 16);
+  for (const OptTensor* a : {&a0, &a1})
+    require(!a->has_value() || ((*a)->is_cuda() && (*a)->scalar_type() == at::kHalf && (*a)->device() == x.device() &&
+                                (*a)->is_contiguous() && same_shape(**a, 16, hidden)),
+            "lora_bwd_drop: A float16 [16, hidden], contiguous, on x's device");
+  for (const OptTensor* m : {&base, &dx})
+    if (m->has_value()) {
+      half_rows(**m, x, "lora_bwd_drop: base / dx");
+      require((*m)->sizes() == x.sizes(), "lora_bwd_drop: base and dx of x's shape");
+    }
   require(workspace.is_cuda() && workspace.is_contiguous() && workspace.device() == x.device(),
-          "lora_wgrad_drop: workspace");
+          "lora_bwd_drop: workspace");
   const c10::DeviceGuard guard(x.device());
-  check(talm_lora_wgrad_drop(as<uint16_t>(x), row_stride(x), as<uint16_t>(dy), row_stride(dy), as<uint16_t>(u),
-                             row_stride(u), as<uint16_t>(t), row_stride(t), n, hidden, two ? 2 : 1,
-                             static_cast<float>(p), drop_key(key, x), drop_site(site0), drop_site(site1),
-                             dtype_code(type), lo0, seg0, static_cast<float>(scaling0), ptr(da0), ptr(db0), lo1,
-                             seg1, static_cast<float>(scaling1), ptr(da1), ptr(db1), workspace.data_ptr(),
-                             workspace.numel() * static_cast<int64_t>(workspace.element_size()), stream_of(x)),
-        "lora_wgrad_drop");
+  check(talm_lora_bwd_drop(as<uint16_t>(x), row_stride(x), as<uint16_t>(dy), row_stride(dy), as<uint16_t>(u),
+                           row_stride(u), as<uint16_t>(t), row_stride(t), n, hidden, two ? 2 : 1,
+                           static_cast<float>(p), drop_key(key, x), drop_site(site0), drop_site(site1),
+                           dtype_code(type), lo0, seg0, static_cast<float>(scaling0), ptr(da0), ptr(db0), lo1, seg1,
+                           static_cast<float>(scaling1), ptr(da1), ptr(db1), as<uint16_t>(a0), as<uint16_t>(a1),
+                           as<uint16_t>(base), base.has_value() ? row_stride(*base) : 0, as<uint16_t>(dx),
+                           dx.has_value() ? row_stride(*dx) : 0, workspace.data_ptr(),
+                           workspace.numel() * static_cast<int64_t>(workspace.element_size()), stream_of(x)),
+        "lora_bwd_drop");
 }
 
 // out [M, rows] = x [M, cols] W^T + bias for a few tokens, W the NF4 weight its buffers start at.
@@ -1103,13 +1083,15 @@ struct AdapterBranch : torch::autograd::Function<AdapterBranch> {
                         const Tensor& a_half, const Tensor& b_half, const OptTensor& key, double scaling, double p,
                         int64_t site) {
     const Tensor x2 = aligned_rows(x), a = adapter_half(a_half), b = adapter_half(b_half);
-    const int64_t n = x2.size(0), out = b.size(0);
-    const Tensor t = at::empty({n, 16}, x2.options()), ts = at::empty({n, 16}, x2.options());
-    const Tensor y = at::empty({n, out}, x2.options());
-    const int64_t bytes = talm_lora_down_drop_workspace(n, x2.size(1), 1);
-    lora_down_drop(x2, a, std::nullopt, p, key, site, 0, scaling, 0.0, t, ts,
-                   bytes ? OptTensor(byte_workspace(bytes, x2, "adapter_branch")) : OptTensor());
-    lora_up(ts, b, std::nullopt, false, 0.0, std::nullopt, 0, 0, std::nullopt, y);
+    const int64_t n = x2.size(0), size = x2.size(1), out = b.size(0);
+    const Tensor t = at::empty({n, 16}, x2.options()), y = at::empty({n, out}, x2.options());
+    const Tensor ws = byte_workspace(talm_lora_branch_fwd_workspace(n, size), x2, "adapter_branch");
+    const c10::DeviceGuard guard(x2.device());
+    check(talm_lora_branch_fwd(as<uint16_t>(x2), row_stride(x2), n, size, out, as<uint16_t>(a), as<uint16_t>(b),
+                               static_cast<float>(p), drop_key(key, x2), drop_site(site),
+                               static_cast<float>(scaling), as<uint16_t>(t), as<uint16_t>(y), ws.data_ptr(),
+                               ws.numel(), stream_of(x2)),
+          "lora_branch_fwd");
     ctx->save_for_backward({x2, a, b, t, key.has_value() ? *key : Tensor()});
     ctx->saved_data["scaling"] = scaling;
     ctx->saved_data["p"] = p;
@@ -1131,27 +1113,24 @@ struct AdapterBranch : torch::autograd::Function<AdapterBranch> {
       at::AutoGradMode off(false);
       const Tensor dy = aligned_rows(grads[0].to(at::kHalf));
       const int64_t n = x.size(0), size = x.size(1), out = b.size(0);
-      const Tensor u_raw = at::empty(t.sizes(), t.options()), u = at::empty(t.sizes(), t.options());
-      adapter_u(dy, b, scaling, u_raw, u);
+      // u = scaling dy B (lora_down writes the unscaled product too), and the weight gradients' partials
+      const Tensor u2 = at::empty({2, n, 16}, t.options()), u_raw = u2.select(0, 0), u = u2.select(0, 1);
+      lora_down(dy, b, std::nullopt, out, 0, 0, 0, 1, scaling, 0.0, u_raw, u);
+      OptTensor dx, da, db;
       if (ctx->needs_input_grad(0)) {
-        const Tensor dx = at::empty({n, size}, x.options());
-        lora_up(u, a, std::nullopt, true, p, key, site, 0, std::nullopt, dx);
-        in[0] = dx.view(ctx->saved_data["shape"].toIntVector());
+        dx = at::empty({n, size}, x.options());
+        in[0] = dx->view(ctx->saved_data["shape"].toIntVector());
       }
       if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
         const auto options = x.options().dtype(ctx->saved_data["type"].toScalarType());
-        in[1] = at::empty({16, size}, options);
-        in[2] = at::empty({out, 16}, options);
-        lora_wgrad_drop(x, dy, u, t, p, key, site, 0, 0, out, scaling, in[1], in[2], 0, 0, 0.0, std::nullopt,
-                        std::nullopt,
-                        byte_workspace(talm_lora_wgrad_drop_workspace(n, size, 1, out, 0), x, "adapter_branch"));
+        da = in[1] = at::empty({16, size}, options);
+        db = in[2] = at::empty({out, 16}, options);
       }
+      lora_bwd_drop(x, dy, u, t, p, key, site, 0, 0, out, scaling, da, db, 0, 0, 0.0, std::nullopt, std::nullopt, a,
+                    std::nullopt, std::nullopt, dx,
+                    byte_workspace(talm_lora_bwd_drop_workspace(n, size, 1, out, 0), x, "adapter_branch"));
     }
     return once(std::move(in));
-  }
-  // u = scaling dy B (and B's unscaled product, which the kernel writes too)
-  static void adapter_u(const Tensor& dy, const Tensor& b, double scaling, const Tensor& u_raw, const Tensor& u) {
-    lora_down(dy, b, std::nullopt, b.size(0), 0, 0, 0, 1, scaling, 0.0, u_raw, u);
   }
 };
 
@@ -2022,12 +2001,11 @@ TORCH_LIBRARY(talm, m) {
         "Tensor(a!) dq, Tensor(b!) dk, Tensor(c!) dv, Tensor(d!) workspace) -> ()");
   m.def("dropout(Tensor x, float p, Tensor? key, int site, Tensor(a!) y) -> ()");
   m.def("lora_down_drop(Tensor x, Tensor a0, Tensor? a1, float p, Tensor? key, int site0, int site1, "
-        "float scaling0, float scaling1, Tensor(a!) t, Tensor(b!) ts, Tensor(c!)? workspace) -> ()");
-  m.def("lora_up(Tensor u, Tensor m0, Tensor? m1, bool m_kmajor, float p, Tensor? key, int site0, "
-        "int site1, Tensor? base, Tensor(a!) out) -> ()");
-  m.def("lora_wgrad_drop(Tensor x, Tensor dy, Tensor u, Tensor t, float p, Tensor? key, int site0, "
-        "int site1, int lo0, int seg0, float scaling0, Tensor(a!) da0, Tensor(b!) db0, int lo1, int seg1, "
-        "float scaling1, Tensor(c!)? da1, Tensor(d!)? db1, Tensor(e!) workspace) -> ()");
+        "float scaling0, float scaling1, Tensor(a!) t, Tensor(b!) ts) -> ()");
+  m.def("lora_bwd_drop(Tensor x, Tensor dy, Tensor u, Tensor t, float p, Tensor? key, int site0, int site1, "
+        "int lo0, int seg0, float scaling0, Tensor(a!)? da0, Tensor(b!)? db0, int lo1, int seg1, "
+        "float scaling1, Tensor(c!)? da1, Tensor(d!)? db1, Tensor? a0, Tensor? a1, Tensor? base, "
+        "Tensor(e!)? dx, Tensor(f!) workspace) -> ()");
   m.def("nf4_gemv(Tensor x, Tensor packed, Tensor absmax8, Tensor code, Tensor absmax2, Tensor offset2, "
         "int rows, int cols, int qblock, int qblock2, Tensor? bias, Tensor(a!) out, Tensor? ts=None, "
         "Tensor? b0=None, int lo0=0, int hi0=0, Tensor? b1=None, int lo1=0, int hi1=0) -> ()");
@@ -2107,8 +2085,7 @@ TORCH_LIBRARY_IMPL(talm, CUDA, m) {
   m.impl("attn_window_bwd", &attn_window_bwd);
   m.impl("dropout", &dropout);
   m.impl("lora_down_drop", &lora_down_drop);
-  m.impl("lora_up", &lora_up);
-  m.impl("lora_wgrad_drop", &lora_wgrad_drop);
+  m.impl("lora_bwd_drop", &lora_bwd_drop);
   m.impl("nf4_gemv", &nf4_gemv);
   m.impl("lora_mirror", &lora_mirror);
   m.impl("gemm_tune", &gemm_tune);

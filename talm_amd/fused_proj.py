@@ -347,8 +347,7 @@ def _mfma_forward(x2, weight, bias, bounds, adapters, halves, rope, key=None):
         ts = torch.empty_like(t)
         size = x2.shape[1]
         if p > 0.0:
-            torch.ops.talm.lora_down_drop(x2, halves[0][0], a1, p, key, 0, 1, adapters[0][1], s1, t, ts,
-                                          _down_workspace(x2, len(adapters)))
+            torch.ops.talm.lora_down_drop(x2, halves[0][0], a1, p, key, 0, 1, adapters[0][1], s1, t, ts)
         else:
             torch.ops.talm.lora_down(x2, halves[0][0], a1, size, size, 0, 0, 0, adapters[0][1], s1,
                                      t, ts)
@@ -452,11 +451,11 @@ def _mfma_backward_core(grads, x2, rest, cos, sin, weight, sizes, adapters, has_
         dx = torch.empty(n_tok, size, dtype=torch.float16, device=x2.device)
         if p > 0.0:
             torch.ops.talm.qkv_lora_bwd_dx(dcat, weight_t, None, None, dx)
-            torch.ops.talm.lora_up(u, halves[0][1], halves[1][1] if len(adapters) > 1 else None, True, p,
-                                   key, 0, 1, dx, dx)
         else:
             torch.ops.talm.qkv_lora_bwd_dx(dcat, weight_t, u, a_t, dx)
         del weight_t
+    if p > 0.0:
+        return dx, _dropped_grads(dx, x2, dcat, u, halves, bounds, adapters, wanted, outs, p, key)
     lora_grads = [None] * (2 * len(adapters))
     if adapters and any(wanted):
         # all adapters' dA, dB in fp32 in one call (t of each adapter is a column view of one
@@ -464,22 +463,11 @@ def _mfma_backward_core(grads, x2, rest, cos, sin, weight, sizes, adapters, has_
         t_all = halves[0][0]
         if len(adapters) > 1 and (halves[1][0].data_ptr() != t_all.data_ptr() + 32
                                   or halves[1][0].stride() != t_all.stride()):
-            return dx, _weight_grads_ops(dcat, u, x2, halves, bounds, adapters, wanted,
-                                         key if p > 0.0 else None)
+            return dx, _weight_grads_ops(dcat, u, x2, halves, bounds, adapters, wanted)
         t_cat = torch.as_strided(t_all, (n_tok, 16 * len(adapters)), (t_all.stride(0), 1))
         segs = [(bounds[seg], bounds[seg + 1] - bounds[seg], s_) for seg, s_, _p in adapters]
-        shapes = [(16, size) if i % 2 == 0 else (segs[i // 2][1], 16)
-                  for i in range(2 * len(adapters))]
-        outs = outs or [None] * len(shapes)
-        grads_ = [o if o is not None and tuple(o.shape) == shp and o.dtype == torch.float32
-                  and o.is_contiguous() else torch.empty(shp, dtype=torch.float32, device=x2.device)
-                  for o, shp in zip(outs, shapes)]
+        grads_ = _weight_grad_buffers(segs, size, outs, x2.device)
         pad = segs + [(0, 0, 0.0)]
-        if p > 0.0:
-            ws = torch.empty(_wgrad_drop_ws(n_tok, size, segs), dtype=torch.uint8, device=x2.device)
-            torch.ops.talm.lora_wgrad_drop(x2, dcat, u, t_cat, p, key, 0, 1, *pad[0], grads_[0],
-                                           grads_[1], *pad[1], *(grads_[2:] or [None, None]), ws)
-            return dx, [g if w else None for g, w in zip(grads_, wanted)]
         ws = torch.empty(_ops_ws(n_tok, size, pad[0][1], pad[1][1]), dtype=torch.uint8,
                          device=x2.device)
         torch.ops.talm.lora_wgrad(x2, dcat, u, t_cat, pad[0][0], pad[0][1], pad[0][2], grads_[0],
@@ -490,18 +478,35 @@ def _mfma_backward_core(grads, x2, rest, cos, sin, weight, sizes, adapters, has_
     return dx, lora_grads
 
 
-def _wgrad_drop_ws(n_tok, size, segs):
+def _weight_grad_buffers(segs, size, outs, device):
+    """fp32 dA [16, size], dB [segment, 16] per adapter: the caller's buffers where they fit."""
+    shapes = [(16, size) if i % 2 == 0 else (segs[i // 2][1], 16) for i in range(2 * len(segs))]
+    outs = outs or [None] * len(shapes)
+    return [o if o is not None and tuple(o.shape) == shp and o.dtype == torch.float32
+            and o.is_contiguous() else torch.empty(shp, dtype=torch.float32, device=device)
+            for o, shp in zip(outs, shapes)]
+
+
+def _dropped_grads(dx, x2, dcat, u, halves, bounds, adapters, wanted, outs, p, key):
+    """The adapters' weight gradients from dropped x, and their part of dx added to it under their masks
+    (talm_lora_bwd_drop: one mask computed for both)."""
     from . import _ops
 
-    return _ops.lora_wgrad_drop_workspace_bytes(n_tok, size, len(segs), segs[0][1],
-                                                segs[1][1] if len(segs) > 1 else 0)
-
-
-def _down_workspace(x2, n_adapters):
-    from . import _ops
-
-    size = _ops.lora_down_drop_workspace_bytes(x2.shape[0], x2.shape[1], n_adapters)
-    return torch.empty(size, dtype=torch.uint8, device=x2.device) if size else None
+    n_tok, size = x2.shape
+    two = len(adapters) > 1
+    grads = any(wanted)
+    if dx is None and not grads:
+        return [None] * len(wanted)
+    t = torch.cat([h[0] for h in halves], 1) if two else halves[0][0]
+    segs = [(bounds[seg], bounds[seg + 1] - bounds[seg], s_) for seg, s_, _p in adapters]
+    bufs = _weight_grad_buffers(segs, size, outs, x2.device) if grads else [None] * (2 * len(segs))
+    ws = torch.empty(_ops.lora_bwd_drop_workspace_bytes(n_tok, size, len(segs), segs[0][1],
+                                                        segs[1][1] if two else 0),
+                     dtype=torch.uint8, device=x2.device)
+    torch.ops.talm.lora_bwd_drop(x2, dcat, u, t, p, key, 0, 1, *segs[0], bufs[0], bufs[1],
+                                 *(segs[1] if two else (0, 0, 0.0)), *(bufs[2:] if two else (None, None)),
+                                 halves[0][1], halves[1][1] if two else None, dx, dx, ws)
+    return [g if w else None for g, w in zip(bufs, wanted)]
 
 
 def _ops_ws(n_tok, size, seg0, seg1):
@@ -510,14 +515,13 @@ def _ops_ws(n_tok, size, seg0, seg1):
     return _ops.lora_wgrad_workspace_bytes(n_tok, size, seg0, seg1)
 
 
-def _weight_grads_ops(dcat, u, x2, halves, bounds, adapters, wanted, key=None):
+def _weight_grads_ops(dcat, u, x2, halves, bounds, adapters, wanted):
     """The adapters' dA / dB with the reference's ops (when their t are not one buffer)."""
     lora_grads = []
-    for k, (seg, scaling, p) in enumerate(adapters):
+    for k, (seg, scaling, _p) in enumerate(adapters):
         t, _a16, _b16 = halves[k]
         uk = u[:, 16 * k:16 * (k + 1)]
-        xd = x2 if key is None else _dropped(x2, p, key, k)
-        lora_grads.append(torch.mm(uk.t(), xd).float() if wanted[2 * k] else None)
+        lora_grads.append(torch.mm(uk.t(), x2).float() if wanted[2 * k] else None)
         dy = dcat[:, bounds[seg]:bounds[seg + 1]]
         lora_grads.append(torch.mm((dy * scaling).t(), t).float() if wanted[2 * k + 1] else None)
     return lora_grads

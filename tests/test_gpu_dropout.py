@@ -1,9 +1,10 @@
 """Counter-based dropout (dropout.dropout) and the adapters' products with it (lora.adapter_branch,
-torch.ops.talm.lora_*_drop / lora_up), against the oracle's masks and float64 products.
+torch.ops.talm.lora_down_drop / lora_bwd_drop), against the oracle's masks and float64 products.
 
 The masks are exact. Tolerances of the products count roundings of at most u = 2^-11 relative (fp16),
 each sum of n products in fp32 adding at most n 2^-24 of the magnitudes summed:
-  t  = x A^T rounded (u); ts = s t rounded (u); y = ts B^T rounded: sum |ts| |B| (u + the sum of t) + u |y|
+  t  = x A^T rounded (u), a second time as ts = s t where two products share it; y = s t B^T rounded:
+       s sum |t| |B| (u + the sum of t) + u |y|
   u  = s dy B rounded; dx = u A rounded; dA = u^T x, dB = s dy^T t: of the rounded u and t, (fp16
   gradients: rounded once more)."""
 
@@ -211,17 +212,20 @@ def test_two_adapters_have_masks_of_their_own():
     dy = rand(n, 192).half()
     half = dict(dtype=torch.float16, device="cuda")
     t, ts = torch.empty(n, 32, **half), torch.empty(n, 32, **half)
-    torch.ops.talm.lora_down_drop(x, a[0], a[1], p, key, *sites, 2.0, 3.0, t, ts, None)
+    torch.ops.talm.lora_down_drop(x, a[0], a[1], p, key, *sites, 2.0, 3.0, t, ts)
     u_raw, u = torch.empty(n, 32, **half), torch.empty(n, 32, **half)
     torch.ops.talm.lora_down(dy, b[0], b[1], seg[0], seg[1], lo[0], lo[1], 1, 2.0, 3.0, u_raw, u)
     base = rand(n, size).half()
     dx = base.clone()
-    torch.ops.talm.lora_up(u, a[0], a[1], True, p, key, *sites, dx, dx)
     da = [torch.empty(16, size, device="cuda") for _ in range(2)]
     db = [torch.empty(s, 16, device="cuda") for s in seg]
-    ws = torch.full((_ops.lora_wgrad_drop_workspace_bytes(n, size, 2, *seg),), 255, dtype=torch.uint8, device="cuda")
-    torch.ops.talm.lora_wgrad_drop(x, dy, u, t, p, key, *sites, lo[0], seg[0], 2.0, da[0], db[0], lo[1], seg[1],
-                                   3.0, da[1], db[1], ws)
+    ws = torch.full((_ops.lora_bwd_drop_workspace_bytes(n, size, 2, *seg),), 255, dtype=torch.uint8, device="cuda")
+    torch.ops.talm.lora_bwd_drop(x, dy, u, t, p, key, *sites, lo[0], seg[0], 2.0, da[0], db[0], lo[1], seg[1], 3.0,
+                                 da[1], db[1], a[0], a[1], dx, dx, ws)
+    alone = torch.empty_like(dx)  # dx without the weight gradients, into another tensor than its base
+    torch.ops.talm.lora_bwd_drop(x, dy, u, t, p, key, *sites, lo[0], seg[0], 2.0, None, None, lo[1], seg[1], 3.0,
+                                 None, None, a[0], a[1], base, alone, ws)
+    assert torch.equal(alone, dx)
     total, tol = base.double(), U * base.double().abs() + 2.0 ** -24
     for i, scaling in enumerate((2.0, 3.0)):
         m = _keep(key, n, size, p, sites[i]).double() / (1 - philox.threshold(p) / 65536)

@@ -126,25 +126,31 @@ def test_python_entries_reject():
                                                  (64, 64, 3, "shape"), (64, 66, 1, "shape")])
 def test_adapter_down_rejects(k, ldx, adapters, word):
     status, message = _status("talm_lora_down_drop", PTR, ldx, 4, k, PTR, PTR, adapters, 0.5, PTR, 0,
-                              1, 1.0, 1.0, PTR, PTR, 32, None, 0, None)
+                              1, 1.0, 1.0, PTR, PTR, 32, None)
     assert status == _lib.TALM_EINVAL and word in message
 
 
-@pytest.mark.parametrize("cols,ldo,word", [(12, 16, "multiples of 8"), (16, 12, "shape"), (16, 8, "shape")])
-def test_adapter_up_rejects(cols, ldo, word):
-    status, message = _status("talm_lora_up", PTR, 16, 4, cols, PTR, None, 1, 0, 0.0, None, 0, 0, None,
-                              0, PTR, ldo, None)
+@pytest.mark.parametrize("k,cols,ws,p,word", [
+    (40, 32, 1 << 20, 0.5, "multiple of 32"), (64, 12, 1 << 20, 0.5, "columns"), (64, 32, 64, 0.5, "workspace"),
+    (64, 32, 1 << 20, 1.0, "p 1"), (0, 32, 1 << 20, 0.5, "shape")])
+def test_adapter_branch_forward_rejects(k, cols, ws, p, word):
+    status, message = _status("talm_lora_branch_fwd", PTR, 64, 4, k, cols, PTR, PTR, p, PTR, 0, 2.0, PTR,
+                              PTR, PTR, ws, None)
     assert status == _lib.TALM_EINVAL and word in message
 
 
-def test_adapter_weight_gradient_rejects():
-    def call(hidden=64, seg=32, ws=1 << 20, dtype=_lib.TALM_F32, lo=0):
-        return _status("talm_lora_wgrad_drop", PTR, 64, PTR, 32, PTR, 16, PTR, 16, 4, hidden, 1, 0.5,
-                       PTR, 0, 1, dtype, lo, seg, 1.0, PTR, PTR, 0, 0, 0.0, None, None, PTR, ws, None)
+def test_adapter_backward_rejects():
+    def call(hidden=64, seg=32, ws=1 << 20, dtype=_lib.TALM_F32, lo=0, da=PTR, db=PTR, a0=PTR, dx=PTR, ldd=64,
+             p=0.5):
+        return _status("talm_lora_bwd_drop", PTR, 64, PTR, 32, PTR, 16, PTR, 16, 4, hidden, 1, p, PTR, 0, 1, dtype,
+                       lo, seg, 1.0, da, db, 0, 0, 0.0, None, None, a0, None, None, 0, dx, ldd, PTR, ws, None)
     for kwargs, word in (({"hidden": 60}, "shape"), ({"seg": 40}, "shape"), ({"ws": 64}, "workspace"),
-                         ({"dtype": 2}, "dtype"), ({"lo": 8}, "shape")):
+                         ({"dtype": 2}, "dtype"), ({"lo": 8}, "shape"), ({"db": None}, "all or none"),
+                         ({"da": None}, "all or none"), ({"a0": None}, "null"), ({"ldd": 60}, "shape"),
+                         ({"dx": PTR + 8}, "16-byte"), ({"p": 1.5}, "p 1.5")):
         status, message = call(**kwargs)
         assert status == _lib.TALM_EINVAL and word in message, kwargs
+    assert call(da=None, db=None, dx=None)[0] == _lib.TALM_OK  # nothing wanted: no launch
 
 
 @pytest.mark.parametrize("tokens,cols,qblock,qblock2,word", [
