@@ -634,8 +634,9 @@ int talm_attn_window_fwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_stri
  * backward's, and partials of the sinks' gradients from the rows past their window (at most 64 MiB,
  * or one set if that is more). Deterministic. No counterpart in the reference.
  */
-int64_t talm_attn_window_bwd_workspace(int64_t n_tokens, int32_t n_q_heads, int32_t n_seqs,
-                                       int32_t max_seqlen, int32_t window, int32_t sinks);
+int64_t talm_attn_window_bwd_workspace(int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                                       int32_t n_seqs, int32_t max_seqlen, int32_t window,
+                                       int32_t sinks);
 int talm_attn_window_bwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
                          const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
                          const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,

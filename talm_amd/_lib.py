@@ -104,7 +104,7 @@ SIZE_FUNCTIONS = {
     "talm_head_ce_workspace": [_I64, _I64, _I64, _I64, _I64, _I32],
     "talm_lora_wgrad_workspace": [_I64, _I64, _I64, _I64],
     "talm_attn_bwd_workspace": [_I64, _I32],
-    "talm_attn_window_bwd_workspace": [_I64, _I32, _I32, _I32, _I32, _I32],
+    "talm_attn_window_bwd_workspace": [_I64, _I32, _I32, _I32, _I32, _I32, _I32],
     "talm_lora_branch_fwd_workspace": [_I64, _I64],
     "talm_lora_bwd_drop_workspace": [_I64, _I64, _I32, _I64, _I64],
     "talm_gemm_splitk_workspace": [_I64, _I64, _I64],

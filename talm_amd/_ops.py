@@ -79,9 +79,9 @@ def attn_bwd_workspace_bytes(n_tokens, n_q_heads):
     return int(size)
 
 
-def attn_window_bwd_workspace_bytes(n_tokens, n_q_heads, n_seqs, max_seqlen, window, sinks):
-    size = _lib.lib().talm_attn_window_bwd_workspace(n_tokens, n_q_heads, n_seqs, max_seqlen, window,
-                                                     sinks)
+def attn_window_bwd_workspace_bytes(n_tokens, n_q_heads, n_kv_heads, n_seqs, max_seqlen, window, sinks):
+    size = _lib.lib().talm_attn_window_bwd_workspace(n_tokens, n_q_heads, n_kv_heads, n_seqs, max_seqlen,
+                                                     window, sinks)
     _require(size >= 0, "attn_window_bwd: unsupported shape")
     return int(size)
 

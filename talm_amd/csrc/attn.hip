@@ -619,6 +619,7 @@ struct BwdArgs {
   const float* lse;    // [Hq, n_tokens], natural log
   const int32_t* cu;
   int group, n_q_heads, n_kv_heads;
+  int kv_parts;        // dK / dV partials per KV head: group, or (kWin) group / item_heads
   int n_tiles;         // tiles per sequence (of the longest)
   float scale, scale_log2;
   int64_t n_tokens;
@@ -643,20 +644,19 @@ struct BwdArgs {
   int64_t cs_tok;
   // kWin (window and sinks at most the longest sequence's length): the sinks' rows past their
   // window in items of far_rows rows (a multiple of 64), far_chunks of them for each (sequence,
-  // 128-key tile of sinks, head); their partials [sequence][head][chunk][sink][D]
+  // 128-key tile of sinks, item_heads heads); their partials [sequence][heads][chunk][sink][D]
   int window, sinks;
-  int far_rows, far_chunks, far_tiles;
-  unsigned far_items;  // n_seqs x far_chunks x far_tiles x heads
+  int item_heads;      // query heads of a KV head that a dK / dV item takes one after the other
+  int far_rows, far_chunks, far_tiles, far_slack;
+  unsigned far_items;  // n_seqs x far_chunks x far_tiles x heads / item_heads
   float* far_k;
   float* far_v;
 };
 
 // The query row after the tiles of 64 rows that hold the window of any of a 128-key tile's keys and, of
-// a tile with sinks, kFarSlack rows more: where the items of its sinks' further rows begin (rows that
-// are few more than a window get no item, no partial and no launch of their own).
-constexpr int kFarSlack = 512;
-__device__ __forceinline__ int near_end(int k0, int len, int window, int sinks) {
-  const int64_t end = static_cast<int64_t>(k0) + 127 + window + (k0 < sinks ? kFarSlack : 0);
+// a tile with sinks, `slack` rows more: where the items of its sinks' further rows begin.
+__device__ __forceinline__ int near_end(int k0, int len, int window, int sinks, int slack) {
+  const int64_t end = static_cast<int64_t>(k0) + 127 + window + (k0 < sinks ? slack : 0);
   const int rows = static_cast<int>(end < len ? end : len) - k0;
   return k0 + (rows + 63) / 64 * 64;
 }
@@ -1006,9 +1006,11 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
 // and dK^T += Q^T dS with Q^T and dO^T read transposed from the row-major tiles. Each slot holds
 // the Q tile, the dO tile, then each wavefront's copy of the tile's 64 lse and 64 Dd values.
 // kWin: chunk < 0 is the tile's rows up to the end of its keys' windows, chunk >= 0 that item of its
-// sinks' rows past them.
+// sinks' rows past them; the item takes a.item_heads heads of one KV head, its tiles one after the other
+// in one pipeline, into one partial: fewer partials to write and sum where the windows are short and
+// the items many.
 template <class E, int W, bool kWin, class Done>
-__device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int head, int tile, int chunk,
+__device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int part, int tile, int chunk,
                                               unsigned char* smem, Done&& done) {
   constexpr int kCols = 32 * W;  // keys per workgroup
   constexpr int kRowsT = kKeys;  // query rows per tile
@@ -1019,7 +1021,7 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
   // causal: rows below k0 see no key here (k0 is a multiple of 64)
   int qstart = k0, qstop = len;
   if constexpr (kWin) {
-    const int end = near_end(k0, len, a.window, a.sinks);
+    const int end = near_end(k0, len, a.window, a.sinks, a.far_slack);
     if (chunk < 0) {
       qstop = min(len, end);
     } else {
@@ -1031,6 +1033,7 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hh = lane >> 5, l32 = lane & 31;
+  const int n_heads = kWin ? a.item_heads : 1, head = part * n_heads;  // its first head
   const int kvh = head / a.group;
   const int key = k0 + 32 * wave + l32;
   const int kr_ = min(key, len - 1);
@@ -1048,18 +1051,32 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
     }
   }
   const int n_qt = (qstop - qstart + kRowsT - 1) / kRowsT;
+  const int n_t = n_heads * n_qt;  // the item's tiles: head by head
   const uint16_t* qbase = a.q + static_cast<int64_t>(s0) * a.q_tok + head * a.q_head;
   const uint16_t* dbase = a.dout + static_cast<int64_t>(s0) * a.do_tok + head * a.do_head;
-  const __amdgpu_buffer_rsrc_t lrs = __builtin_amdgcn_make_buffer_rsrc(
+  int iq = 0, ih = head;  // kWin: the next tile to issue, and its head
+  __amdgpu_buffer_rsrc_t lrs = __builtin_amdgcn_make_buffer_rsrc(
       a.lse2 + static_cast<int64_t>(head) * a.n_tokens + s0, 0, len * 4, 0x00020000);
-  const __amdgpu_buffer_rsrc_t drs = __builtin_amdgcn_make_buffer_rsrc(
+  __amdgpu_buffer_rsrc_t drs = __builtin_amdgcn_make_buffer_rsrc(
       a.dd + static_cast<int64_t>(head) * a.n_tokens + s0, 0, len * 4, 0x00020000);
   TileDma qd, od;
   qd.init(a.q_tok, wave, lane);
   od.init(a.do_tok, wave, lane);
-  auto issue = [&](int qt, int slot) __attribute__((always_inline)) {
+  auto issue = [&](int t, int slot) __attribute__((always_inline)) {
     unsigned char* dst = smem + slot * kBwdSlot;
-    const int r0 = qstart + qt * kRowsT;
+    if constexpr (kWin) {
+      if (iq == n_qt) {  // the next head's rows
+        iq = 0;
+        ++ih;
+        qbase += a.q_head;
+        dbase += a.do_head;
+        lrs = __builtin_amdgcn_make_buffer_rsrc(a.lse2 + static_cast<int64_t>(ih) * a.n_tokens + s0, 0, len * 4,
+                                                0x00020000);
+        drs = __builtin_amdgcn_make_buffer_rsrc(a.dd + static_cast<int64_t>(ih) * a.n_tokens + s0, 0, len * 4,
+                                                0x00020000);
+      }
+    }
+    const int r0 = qstart + (kWin ? iq++ : t) * kRowsT;
     qd.issue(qbase + static_cast<int64_t>(r0) * a.q_tok, len - r0, dst, wave);
     od.issue(dbase + static_cast<int64_t>(r0) * a.do_tok, len - r0, dst + kTileBytes, wave);
     // the tile's 64 lse and 64 Dd values, one 4-byte load per lane (rows past len read 0), into
@@ -1176,26 +1193,29 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
   using B0 = std::integral_constant<int, 0>;
   using B1 = std::integral_constant<int, 1>;
   // the first tile with a row at or past the wavefront's keys (past the window: none without a sink)
-  const int t0 = !kWin || chunk < 0 ? (wk0 - qstart) / kRowsT : wk0 < a.sinks ? 0 : n_qt;
+  const int t0 = !kWin || chunk < 0 ? (wk0 - qstart) / kRowsT : wk0 < a.sinks ? 0 : n_t;
   int slot = 0;  // of the tile in hand
   issue(0, 0);
   auto arrive = [&](int t) __attribute__((always_inline)) {
     wait_vmcnt<0>();
     lds_barrier();  // tile t has landed; everyone is done with tile t - 2, whose slot takes t + 1
-    if (t + 1 < n_qt) issue(t + 1, slot == 2 ? 0 : slot + 1);
+    if (t + 1 < n_t) issue(t + 1, slot == 2 ? 0 : slot + 1);
   };
   auto leave = [&]() __attribute__((always_inline)) {
     rd.next_row(slot_step(slot));
     lrow += slot_step(slot);
     slot = slot == 2 ? 0 : slot + 1;
   };
-  for (int t = 0; t < t0 && t < n_qt; ++t) {
+  for (int t = 0; t < t0 && t < n_t; ++t) {
     arrive(t);
     rd.next_t(slot_step(slot));
     leave();
   }
-  if (t0 < n_qt) {
-    const int q0 = qstart + t0 * kRowsT;
+  if (t0 < n_t) {
+    // kWin: the tile of its head that is in hand (a wavefront whose keys begin later skips the first
+    // head's first tiles, and takes the next heads' masked)
+    int cq = kWin ? t0 % n_qt : t0;
+    const int q0 = qstart + cq * kRowsT;
     arrive(t0);
     scores(B0{}, std::false_type{});
 #pragma unroll
@@ -1205,8 +1225,10 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
     gather(B0{}, std::true_type{});
     mask(1, q0 + 32);
     leave();
-    for (int t = t0 + 1; t < n_qt; ++t) {
-      const int r0 = qstart + t * kRowsT;
+    for (int t = t0 + 1; t < n_t; ++t) {
+      ++cq;
+      if (kWin && cq == n_qt) cq = 0;
+      const int r0 = qstart + cq * kRowsT;
       arrive(t);
       scores(B0{}, std::true_type{});
       gather(B1{}, std::true_type{});
@@ -1236,8 +1258,8 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
   // the partials' rows: the token's, or of an item past the window the sink's in the item's own
   const bool far = kWin && chunk >= 0;
   const int64_t row0 =
-      far ? ((static_cast<int64_t>(seq) * a.n_q_heads + head) * a.far_chunks + chunk) * a.sinks + wk0
-          : static_cast<int64_t>(head) * a.n_tokens + s0 + wk0;
+      far ? ((static_cast<int64_t>(seq) * (a.n_q_heads / n_heads) + part) * a.far_chunks + chunk) * a.sinks + wk0
+          : static_cast<int64_t>(part) * a.n_tokens + s0 + wk0;
   const int key_end = far ? min(a.sinks, len) : len;
   auto store_rows = [&](const f32x16 (&acc)[kD / 32], float mul, float* part) {
 #pragma unroll
@@ -1268,12 +1290,12 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int hea
   store_rows(dva, 1.f, far ? a.far_v : a.dv_part);
 }
 
-// kWin: item `i` of the sinks' rows past their windows: heads fastest, then 128-key tiles, chunks,
-// sequences. An item without a row returns at once.
+// kWin: item `i` of the sinks' rows past their windows: parts (item_heads heads) fastest, then 128-key
+// tiles, chunks, sequences. An item without a row returns at once.
 template <class E, int W, class Done>
 __device__ __forceinline__ void attn_bwd_far(const BwdArgs& a, unsigned i, unsigned char* smem,
                                              Done&& done) {
-  const unsigned heads = static_cast<unsigned>(a.n_q_heads);
+  const unsigned heads = static_cast<unsigned>(a.n_q_heads / a.item_heads);
   const unsigned tiles = static_cast<unsigned>(a.far_tiles), chunks = static_cast<unsigned>(a.far_chunks);
   const unsigned head = i % heads, tile = i / heads % tiles, chunk = i / heads / tiles % chunks;
   attn_bwd_dkdv<E, W, true>(a, static_cast<int>(i / heads / tiles / chunks), static_cast<int>(head),
@@ -1281,22 +1303,23 @@ __device__ __forceinline__ void attn_bwd_far(const BwdArgs& a, unsigned i, unsig
 }
 
 // kWin: the partials of the sinks' rows past their windows added, in chunk order, to the ones of the
-// rows before: one thread per (sequence, head, sink, four columns).
+// rows before: one thread per (sequence, part, sink, four columns).
 __global__ __launch_bounds__(256) void attn_bwd_far_kernel(BwdArgs a) {
   const int64_t idx = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t row = idx / (kD / 4);
   const int c = static_cast<int>(idx % (kD / 4)) * 4;
   const int key = static_cast<int>(row % a.sinks);
-  const int64_t sh = row / a.sinks;  // sequence * heads + head
-  if (sh >= static_cast<int64_t>(a.n_seqs) * a.n_q_heads) return;
-  const int seq = static_cast<int>(sh / a.n_q_heads), head = static_cast<int>(sh % a.n_q_heads);
+  const int64_t sh = row / a.sinks;  // sequence * parts + part
+  const int parts = a.n_q_heads / a.item_heads;
+  if (sh >= static_cast<int64_t>(a.n_seqs) * parts) return;
+  const int seq = static_cast<int>(sh / parts), part = static_cast<int>(sh % parts);
   const Rows own_rows = seq_rows<true>(a.cu, seq, a.n_tokens);
   const int s0 = own_rows.s0, len = own_rows.len;
   if (key >= len) return;
-  const int end = near_end(key / 128 * 128, len, a.window, a.sinks);
+  const int end = near_end(key / 128 * 128, len, a.window, a.sinks, a.far_slack);
   const int chunks = min(a.far_chunks, (max(len - end, 0) + a.far_rows - 1) / a.far_rows);
   if (chunks == 0) return;
-  const int64_t at = (static_cast<int64_t>(head) * a.n_tokens + s0 + key) * kD + c;
+  const int64_t at = (static_cast<int64_t>(part) * a.n_tokens + s0 + key) * kD + c;
   const int64_t from = (sh * a.far_chunks * a.sinks + key) * kD + c, step = static_cast<int64_t>(a.sinks) * kD;
   f32x4_t k = *reinterpret_cast<const f32x4_t*>(a.dk_part + at);
   f32x4_t v = *reinterpret_cast<const f32x4_t*>(a.dv_part + at);
@@ -1322,10 +1345,12 @@ __global__ __launch_bounds__(64 * W, 1) void attn_bwd_kernel(BwdArgs a) {
   unsigned z = blockIdx.z;
   if constexpr (kWin) {
     const unsigned far = static_cast<unsigned>(a.far_chunks * a.far_tiles);
+    const unsigned parts = gridDim.x / static_cast<unsigned>(a.item_heads);
     if (z < far) {
-      attn_bwd_far<E, W>(a, (blockIdx.y * far + z) * gridDim.x + blockIdx.x, smem, [] {});
+      if (blockIdx.x < parts) attn_bwd_far<E, W>(a, (blockIdx.y * far + z) * parts + blockIdx.x, smem, [] {});
       return;
     }
+    if ((z - far & 1) && blockIdx.x >= parts) return;  // a dK / dV item takes item_heads heads
     z -= far;
   }
   const int rank = static_cast<int>(z) >> 1;
@@ -1346,8 +1371,9 @@ __global__ __launch_bounds__(64 * W, 1) void attn_bwd_kernel(BwdArgs a) {
 //
 // An item is a (sequence, 128-token tile, dK/dV or dQ, head); its length follows the sequence's
 // tiles from there on (dK / dV: the query tiles after its keys; dQ: the key tiles before its
-// rows), the m of list_pair. kWin: the first far_items are the ones of the sinks' rows past their
-// windows; the others' lengths end with the window, and their order matters less.
+// rows), the m of list_pair. kWin: first the far_items, of the sinks' rows past their windows, then the
+// dK / dV items (of item_heads heads, the longest ones), then dQ's: the windows end their lengths, and
+// the order of the pairs matters less.
 template <class E, int W, bool kWin>
 __global__ __launch_bounds__(64 * W, 1) void attn_bwd_queue_kernel(BwdArgs a) {
   // the next item's index behind the ring
@@ -1358,16 +1384,28 @@ __global__ __launch_bounds__(64 * W, 1) void attn_bwd_queue_kernel(BwdArgs a) {
   const unsigned pairs = static_cast<unsigned>(wave_count(own));
   const unsigned per_pair = 2u * static_cast<unsigned>(a.n_q_heads);
   const unsigned far = kWin ? a.far_items : 0u;
+  const unsigned parts = kWin ? static_cast<unsigned>(a.n_q_heads / a.item_heads) : 0u;
   unsigned item = blockIdx.x;
   for (;;) {
-    const unsigned pair = item < far ? 0u : (item - far) / per_pair;
-    if (item >= far && pair >= pairs) break;
+    unsigned pair, in_pair;  // in_pair: dK / dV's parts first, then dQ's heads
+    if constexpr (kWin) {
+      const unsigned heads = static_cast<unsigned>(a.n_q_heads), first_dq = far + pairs * parts;
+      const bool dq = item >= first_dq;
+      const unsigned i = item - (dq ? first_dq : far), per = dq ? heads : parts;
+      pair = item < far ? 0u : i / per;
+      in_pair = i - pair * per + (dq ? heads : 0u);
+      if (item >= far && pair >= pairs) break;
+    } else {
+      pair = item / per_pair;
+      in_pair = item - pair * per_pair;
+      if (pair >= pairs) break;
+    }
     int seq = 0, lo = 0, rank = 0;
     if (!kWin || item >= far) {
       lo = list_pair(own, a.n_tiles, pair, lane, seq);
       rank = __builtin_amdgcn_readlane(own, seq) - lo;
     }
-    const int which = static_cast<int>(item - far - pair * per_pair);
+    const int which = static_cast<int>(in_pair);
     // the next item is drawn when this one's products are done, while its results go out (drawn
     // before, the longest items would each hold back one more)
     unsigned next = 0xffffffffu;  // past every item
@@ -1406,14 +1444,14 @@ __device__ __forceinline__ void sum_heads4(const BwdArgs& a, int kvh, int64_t t,
 #pragma unroll
     for (int e = 0; e < 4; ++e) k[c][e] = v[c][e] = 0.f;
   const int64_t head_stride = a.n_tokens * kD;
-  const int64_t off0 = (static_cast<int64_t>(kvh) * a.group * a.n_tokens + t) * kD;
-  for (int g0 = 0; g0 < a.group; g0 += 8) {
+  const int64_t off0 = (static_cast<int64_t>(kvh) * a.kv_parts * a.n_tokens + t) * kD;
+  for (int g0 = 0; g0 < a.kv_parts; g0 += 8) {
     float4 xk[8][C], xv[8][C];
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int64_t off = off0 + (g0 + j < a.group ? g0 + j : 0) * head_stride + d[c];
+        const int64_t off = off0 + (g0 + j < a.kv_parts ? g0 + j : 0) * head_stride + d[c];
         xk[j][c] = *reinterpret_cast<const float4*>(a.dk_part + off);
         xv[j][c] = *reinterpret_cast<const float4*>(a.dv_part + off);
       }
@@ -1421,7 +1459,7 @@ __device__ __forceinline__ void sum_heads4(const BwdArgs& a, int kvh, int64_t t,
     // each load to its add, one round trip per head (heads past the group add +0)
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const bool in = g0 + j < a.group;
+      const bool in = g0 + j < a.kv_parts;
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         k[c][0] += in ? xk[j][c].x : 0.f; k[c][1] += in ? xk[j][c].y : 0.f;
@@ -1644,22 +1682,45 @@ TALM_API int64_t talm_attn_bwd_workspace(int64_t n_tokens, int32_t n_q_heads) {
 namespace talm {
 namespace {
 
-// How the sinks' rows past their windows are cut: items of at least a window and kFarRows rows, so that
-// none is much longer than a tile's other rows, but few enough that their partials stay within
-// kFarBytes.
+// Query heads of a KV head per dK / dV item in a window: as many of the group as keep the item's chain of
+// 64-row steps within a CU's share of all the work (a step of dQ is two thirds of one of dK / dV; a key
+// sees on the average w - w^2 / 2 L rows, w the window, L the mean length). An item writes one partial for
+// its heads, 128 KiB a tile of keys, and loads its keys once. Backward, us, one head / so: lengths [4096,
+// 3001, 2222, 1531] with 12 / 2 heads, window 1000 351 / 317 (three heads; all six 317), 256 206 / 165
+// (six), 4096 546 / 504 (two; six 977); 16 rows of 128..512, window 256 89 / 77 (two; six 123); [2048], 1000
+// 79 (one; two 102).
+int window_item_heads(int64_t n_tokens, int64_t n_seqs, int64_t max_seqlen, int64_t n_q_heads, int64_t group,
+                      int64_t window) {
+  if (n_tokens == 0 || n_seqs == 0) return 1;
+  const int64_t n_tiles = (max_seqlen + 127) / 128, tiles = std::min(n_tokens / 128 + n_seqs / 2, n_seqs * n_tiles);
+  const int64_t steps = std::min(2 * n_tiles, (std::min(window, max_seqlen) + 127 + 63) / 64);
+  const double mean = static_cast<double>(n_tokens) / n_seqs, w = std::min<double>(window, mean);
+  const double share = tiles * n_q_heads * ((w - w * w / (2 * mean) + 127) / 64) * 5 / 3 / device_cus();
+  int heads = 1;
+  for (int64_t d = 2; d <= group; ++d)
+    if (group % d == 0 && d * steps <= share) heads = static_cast<int>(d);
+  return heads;
+}
+
+// How the sinks' rows past their windows are cut: items of a window's or kFarRows rows over their heads,
+// so that none is much longer than a tile's other rows, but few enough that their partials stay within
+// kFarBytes. Where an item has one head, kFarRows rows more than a window stay with the tile (no item,
+// partial or launch for a few rows).
 constexpr int64_t kFarRows = 512, kFarBytes = int64_t{64} << 20;
 struct FarPlan {
-  int64_t rows = 64, chunks = 0, tiles = 0, floats = 0;  // floats: of far_k, and again of far_v
+  int64_t rows = 64, chunks = 0, tiles = 0, slack = 0, floats = 0;  // floats: of far_k, and again of far_v
 };
-FarPlan far_plan(int64_t n_seqs, int64_t max_seqlen, int64_t n_q_heads, int64_t window, int64_t sinks) {
+FarPlan far_plan(int64_t n_seqs, int64_t max_seqlen, int64_t n_q_heads, int64_t item_heads, int64_t window,
+                 int64_t sinks) {
   FarPlan f;
   window = std::min(window, max_seqlen);
   sinks = std::min(sinks, max_seqlen);
-  const int64_t left = max_seqlen - (127 + window + kFarSlack + 63) / 64 * 64;  // of the first key tile
+  if (item_heads == 1) f.slack = kFarRows;
+  const int64_t left = max_seqlen - (127 + window + f.slack + 63) / 64 * 64;  // of the first tile
   if (sinks == 0 || left <= 0 || n_seqs == 0) return f;
-  const int64_t one = n_seqs * n_q_heads * sinks * kD;
+  const int64_t one = n_seqs * (n_q_heads / item_heads) * sinks * kD;
   const int64_t most = std::max<int64_t>(1, kFarBytes / (8 * one));
-  f.rows = std::max(kFarRows, (window + 63) / 64 * 64);
+  f.rows = (std::max(kFarRows, window) / item_heads + 63) / 64 * 64;
   f.chunks = std::min((left + f.rows - 1) / f.rows, most);
   f.rows = std::max(f.rows, ((left + f.chunks - 1) / f.chunks + 63) / 64 * 64);
   f.tiles = (sinks + 127) / 128;
@@ -1681,7 +1742,7 @@ void launch_bwd(const BwdArgs& a, int n_seqs, hipStream_t s) {
     hipLaunchKernelGGL((attn_bwd_kernel<E, W, kWin>), grid, dim3(64 * W), 0, s, a);
   }
   if (a.far_items) {
-    const int64_t n = static_cast<int64_t>(n_seqs) * a.n_q_heads * a.sinks * (kD / 4);
+    const int64_t n = static_cast<int64_t>(n_seqs) * (a.n_q_heads / a.item_heads) * a.sinks * (kD / 4);
     hipLaunchKernelGGL(attn_bwd_far_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s, a);
   }
   const int64_t red = a.n_tokens * a.n_kv_heads * (a.cos ? kD / 8 : kD / 4);
@@ -1722,7 +1783,10 @@ int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
   if (n_seqs > 65535 || (max_seqlen + 127) / 128 > 32767)
     return fail(TALM_EINVAL, "%s: at most 65535 sequences of at most 4194176 tokens", what);
   // (a workspace without the queue's counter is accepted: one workgroup per item then)
-  const FarPlan far = win.window ? far_plan(n_seqs, max_seqlen, n_q_heads, win.window, win.sinks) : FarPlan{};
+  const int item_heads = win.window ? window_item_heads(n_tokens, n_seqs, max_seqlen, n_q_heads,
+                                                        n_q_heads / n_kv_heads, win.window) : 1;
+  const FarPlan far =
+      win.window ? far_plan(n_seqs, max_seqlen, n_q_heads, item_heads, win.window, win.sinks) : FarPlan{};
   const int64_t need = talm_attn_bwd_workspace(n_tokens, n_q_heads) - kQueueBytes + 8 * far.floats;
   if (far.chunks * far.tiles + 2 * ((max_seqlen + 127) / 128) > 65535 ||
       n_seqs * far.chunks * far.tiles * n_q_heads >= (int64_t{1} << 30) ||
@@ -1752,7 +1816,8 @@ int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
   a.o = out; a.o_tok = o_stride_tok; a.o_head = o_stride_head;
   a.dout = dout; a.do_tok = do_stride_tok; a.do_head = do_stride_head;
   a.lse = lse; a.cu = cu_seqlens;
-  a.group = n_q_heads / n_kv_heads; a.n_q_heads = n_q_heads; a.n_kv_heads = n_kv_heads;
+  a.group = a.kv_parts = n_q_heads / n_kv_heads; a.n_q_heads = n_q_heads; a.n_kv_heads = n_kv_heads;
+  a.item_heads = 1;
   a.n_tiles = (max_seqlen + 32 * W - 1) / (32 * W);
   a.scale = scale; a.scale_log2 = scale * 1.44269504088896341f;
   a.n_tokens = n_tokens;
@@ -1771,7 +1836,10 @@ int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
     a.far_rows = static_cast<int>(far.rows);
     a.far_chunks = static_cast<int>(far.chunks);
     a.far_tiles = static_cast<int>(far.tiles);
-    a.far_items = static_cast<unsigned>(n_seqs * far.chunks * far.tiles * n_q_heads);
+    a.far_slack = static_cast<int>(far.slack);
+    a.item_heads = item_heads;
+    a.kv_parts = a.group / item_heads;
+    a.far_items = static_cast<unsigned>(n_seqs * far.chunks * far.tiles * (n_q_heads / item_heads));
     a.far_k = a.dv_part + n_tokens * n_q_heads * kD;
     a.far_v = a.far_k + far.floats;
   }
@@ -1784,7 +1852,7 @@ int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
   // tile per sequence, 64 sequences of 33, 64, 96 and 128 tokens with 12 / 2 heads (1536): 46.3 / 52.8,
   // 60.2 / 61.3, 86.2 / 82.6, 105 / 94; 24 sequences, 16 / 16 heads (768): 31.9 / 35.0, 37.5 / 40.6,
   // 51.3 / 53.8, 60.5 / 60.6.
-  const int64_t items = a.far_items + 2 * static_cast<int64_t>(n_q_heads) *
+  const int64_t items = a.far_items + (n_q_heads + n_q_heads / item_heads) *
                         std::min<int64_t>(n_tokens / (32 * W) + n_seqs, static_cast<int64_t>(n_seqs) * a.n_tiles);
   a.n_seqs = n_seqs;
   if (n_seqs <= kListSeqs && items > 2 * device_cus() &&
@@ -1848,11 +1916,15 @@ TALM_API int talm_attn_bwd_rope(const uint16_t* q, int64_t q_stride_tok, int64_t
                        dv_stride_tok, dv_stride_head, workspace, workspace_bytes, stream);
 }
 
-TALM_API int64_t talm_attn_window_bwd_workspace(int64_t n_tokens, int32_t n_q_heads, int32_t n_seqs,
-                                                int32_t max_seqlen, int32_t window, int32_t sinks) {
-  if (n_tokens < 0 || n_q_heads < 1 || n_seqs < 0 || max_seqlen < 0 || window < 1 || sinks < 0) return -1;
+TALM_API int64_t talm_attn_window_bwd_workspace(int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                                                int32_t n_seqs, int32_t max_seqlen, int32_t window,
+                                                int32_t sinks) {
+  if (n_tokens < 0 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads % n_kv_heads || n_seqs < 0 || max_seqlen < 0 ||
+      window < 1 || sinks < 0)
+    return -1;
+  const int heads = window_item_heads(n_tokens, n_seqs, max_seqlen, n_q_heads, n_q_heads / n_kv_heads, window);
   return talm_attn_bwd_workspace(n_tokens, n_q_heads) +
-         8 * far_plan(n_seqs, max_seqlen, n_q_heads, window, sinks).floats;
+         8 * far_plan(n_seqs, max_seqlen, n_q_heads, heads, window, sinks).floats;
 }
 
 TALM_API int talm_attn_window_bwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,

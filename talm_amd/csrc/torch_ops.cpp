@@ -973,11 +973,12 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     variable_list in(8);
     {
       at::AutoGradMode off(false);
+      const c10::DeviceGuard guard(q.device());
       const Tensor g = head_rows(grads[0].transpose(1, 2));
       const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()),
                    dv = at::empty(v.sizes(), v.options());
       const Tensor ws = byte_workspace(
-          talm_attn_window_bwd_workspace(q.size(0), int32_arg(q.size(1), "heads"),
+          talm_attn_window_bwd_workspace(q.size(0), int32_arg(q.size(1), "heads"), int32_arg(k.size(1), "heads"),
                                          int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_len, "max_len"),
                                          int32_arg(window, "window"), int32_arg(sinks, "sinks")),
           q, "window_attention");

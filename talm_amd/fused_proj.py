@@ -626,7 +626,7 @@ class AttentionBlock(torch.autograd.Function):
         dk = dqkv[:, bounds[1]:bounds[2]]
         dv = dqkv[:, bounds[2]:]
         ws = torch.empty(_ops.attn_bwd_workspace_bytes(n_tok, nh) if ctx.window is None else
-                         _ops.attn_window_bwd_workspace_bytes(n_tok, nh, cu.numel() - 1, ctx.max_len,
+                         _ops.attn_window_bwd_workspace_bytes(n_tok, nh, nkv, cu.numel() - 1, ctx.max_len,
                                                               *ctx.window),
                          dtype=torch.uint8, device=x2.device)
         views = (dq.view(n_tok, nh, hd), dk.view(n_tok, nkv, hd), dv.view(n_tok, nkv, hd), ws)

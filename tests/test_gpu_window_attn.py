@@ -195,7 +195,7 @@ def test_rows_behind_the_last_sequence():
     torch.ops.talm.attn_window_fwd(q, k, v, cu, 100, 0.1, 20, 2, out, lse)
     assert (out[160:] == 7).all() and (lse[:, 160:] == 3).all() and not (out[:160] == 7).any()
     dq, dk, dv = (torch.full_like(t, 5.0).contiguous() for t in (q, k, v))
-    ws = torch.full((_ops.attn_window_bwd_workspace_bytes(200, 4, 2, 100, 20, 2),), 255, dtype=torch.uint8,
+    ws = torch.full((_ops.attn_window_bwd_workspace_bytes(200, 4, 2, 2, 100, 20, 2),), 255, dtype=torch.uint8,
                     device="cuda")  # NaN wherever it is read unwritten
     torch.ops.talm.attn_window_bwd(q, k, v, out, dout, lse, cu, 100, 0.1, 20, 2, None, None, dq, dk, dv, ws)
     for t in (dq, dk, dv):

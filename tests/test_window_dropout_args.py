@@ -65,12 +65,12 @@ def test_window_forward_rejects(bad, word):
 
 
 def test_window_backward_rejects_a_short_workspace():
-    need = _ops.attn_window_bwd_workspace_bytes(4096, 2, 1, 4096, 64, 4)
+    need = _ops.attn_window_bwd_workspace_bytes(4096, 2, 1, 1, 4096, 64, 4)
     assert need > _ops.attn_bwd_workspace_bytes(4096, 2)
-    assert _ops.attn_window_bwd_workspace_bytes(4096, 2, 1, 4096, 64, 0) == \
+    assert _ops.attn_window_bwd_workspace_bytes(4096, 2, 1, 1, 4096, 64, 0) == \
         _ops.attn_bwd_workspace_bytes(4096, 2)
     with pytest.raises(ValueError):
-        _ops.attn_window_bwd_workspace_bytes(4096, 2, 1, 4096, 0, 4)
+        _ops.attn_window_bwd_workspace_bytes(4096, 2, 1, 1, 4096, 0, 4)
     rows = [PTR, 256, 128]
     status, message = _status(
         "talm_attn_window_bwd", *rows, *[PTR, 128, 128] * 2, *rows, *rows, PTR, PTR, 1, 4096, 4096, 2,
@@ -82,8 +82,9 @@ def test_window_backward_rejects_a_short_workspace():
 def test_window_workspace_of_many_sinks_is_bounded():
     """The sinks' partials stay within 64 MiB, or one chunk where that alone is more."""
     for seqs, longest, sinks in ((1, 100000, 4), (64, 4096, 200), (64, 8192, 4), (4, 4096, 4096)):
-        extra = _ops.attn_window_bwd_workspace_bytes(0, 12, seqs, longest, 64, sinks) \
-            - _ops.attn_bwd_workspace_bytes(0, 12)
+        n = seqs * longest // 2
+        extra = _ops.attn_window_bwd_workspace_bytes(n, 12, 2, seqs, longest, 64, sinks) \
+            - _ops.attn_bwd_workspace_bytes(n, 12)
         one = seqs * 12 * min(sinks, longest) * 128 * 8
         assert 0 < extra <= max(64 << 20, one)
 
