@@ -70,7 +70,7 @@ template <int P, int TB>
 struct GemvLane {
   static constexpr int R = 16 / P;  // rows of W per tile, and tokens per block
   int row0, wr, part, g;            // wr: the lane's row of a tile (A) and token of a block (B)
-  int64_t first;                    // the workgroup's first weight
+  int64_t first;                    // the workgroup's first weight (its at most 128 rows fit 32 bits: cols <= 2^24)
   __amdgpu_buffer_rsrc_t rw, rs, rx;
   __device__ __forceinline__ GemvLane(const GemvArgs& a, int row, int lane)
       : row0(row), wr(lane & (R - 1)), part((lane & 15) / R), g(lane >> 4),
@@ -80,8 +80,8 @@ struct GemvLane {
     rx = buffer_rsrc(a.x);
   }
   __device__ __forceinline__ int column(int unit) const { return (unit * P + part) * 256 + 64 * g; }
-  // A lane outside W reads codes of 0 under some block's scale, against columns of x that read 0, or
-  // for rows that are not stored.
+  // A lane outside W reads codes and scales of 0, against columns of x that read 0, or for rows that
+  // are not stored.
   __device__ __forceinline__ void load_w(const GemvArgs& a, int tile, int unit, GemvBlock& w) const {
     const int k = column(unit), row = R * tile + wr;
     const bool in = k < a.cols && row0 + row < a.rows;
@@ -90,8 +90,8 @@ struct GemvLane {
     w.hi = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rw, in ? e / 2 + 16 : kOob, 0, 0));
     w.a8 = __builtin_amdgcn_raw_buffer_load_b8(rs, in ? e / 64 : kOob, 0, 0);
     const int64_t group = in ? ((first + e) >> 6) >> a.shift2 : 0;
-    w.s2 = a.absmax2[group];
-    w.o2 = a.offset2[group];
+    w.s2 = in ? a.absmax2[group] : 0.f;
+    w.o2 = in ? a.offset2[group] : 0.f;
   }
   __device__ __forceinline__ void load_x(const GemvArgs& a, int unit, uint4 (&x)[TB][8]) const {
     const int k = column(unit);
@@ -323,7 +323,7 @@ TALM_API int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, con
   if (qblock != 64 || qblock2 < 1 || (qblock2 & (qblock2 - 1)))
     return fail(TALM_EINVAL, "nf4_gemv: blocks of %d weights in groups of %d (64, a power of two)", qblock, qblock2);
   if (n_tokens < 0 || n_tokens > kGemvTokens || rows < 1 || rows > (1 << 30) || cols < 64 || cols % 64 ||
-      cols > (1 << 26) || ldx < cols || ldx % 8 || ldx > (1 << 24) || ldo < rows)
+      cols > (1 << 24) || ldx < cols || ldx % 8 || ldx > (1 << 24) || ldo < rows)
     return fail(TALM_EINVAL,
                 "nf4_gemv: bad shape (tokens %lld, W [%lld, %lld], ldx %lld, ldo %lld): at most %d tokens, cols "
                 "a multiple of 64, ldx of 8",

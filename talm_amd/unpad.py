@@ -367,6 +367,8 @@ def _window_rows(query, key, value, cu, dropout, scaling, window, sinks):
         except Exception as exc:  # noqa: BLE001 - state.py convention
             if not fallback("varlen_attention", exc):
                 raise
+    if _rows[-1] is None:  # fixed-shape packing: no host row bounds
+        raise RuntimeError("sliding layers under fixed-shape packing need fp16 or bf16 heads of 128")
     outs = []
     for s, e in _rows[-1]:
         if e > s:

@@ -23,11 +23,11 @@ pytestmark = pytest.mark.gpu
 D = 128
 
 
-def _reference(q, k, v, lengths, scale, window, sinks, dout, half):
-    """float64: (values, tolerances), each (out, dq, dk, dv)."""
+def _reference(q, k, v, lengths, scale, window, sinks, dout, half, device="cpu"):
+    """float64 (on the GPU for the larger cases): (values, tolerances), each (out, dq, dk, dv)."""
     u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[half]
     sub = 2.0 ** -25 if half == torch.float16 else 0.0
-    q, k, v, dout = (t.detach().double().cpu().transpose(0, 1) for t in (q, k, v, dout))
+    q, k, v, dout = (t.detach().to(device).double().transpose(0, 1) for t in (q, k, v, dout))
     group = q.shape[0] // k.shape[0]
     vals = [torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)]
     tols = [torch.zeros_like(t) for t in vals]
@@ -35,7 +35,7 @@ def _reference(q, k, v, lengths, scale, window, sinks, dout, half):
     for n in lengths:
         rows = slice(s0, s0 + n)
         s0 += n
-        i = torch.arange(n)
+        i = torch.arange(n, device=device)
         seen = (i[None] <= i[:, None]) & ((i[:, None] - i[None] < window) | (i[None] < sinks))
         for h in range(q.shape[0]):
             qh, kh, vh, g = q[h, rows], k[h // group, rows], v[h // group, rows], dout[h, rows]
@@ -62,7 +62,7 @@ def _reference(q, k, v, lengths, scale, window, sinks, dout, half):
     # spacing 2^-24 for values below 2^-14, whose rounding is not relative
     for i, (t, val) in enumerate(zip(tols, vals)):
         t += (u * val.abs() if i else 0.0) + sub
-    return [t.transpose(0, 1) for t in vals], [t.transpose(0, 1) for t in tols]
+    return [t.transpose(0, 1).cpu() for t in vals], [t.transpose(0, 1).cpu() for t in tols]
 
 
 def _inputs(n, hq, hkv, half, strided, seed):
@@ -90,12 +90,12 @@ def _cu(lengths):
     return torch.tensor([0] + lengths).cumsum(0).to(torch.int32).cuda()
 
 
-def _check(lengths, window, sinks, hq, hkv, half=torch.float16, strided=True, seed=1):
+def _check(lengths, window, sinks, hq, hkv, half=torch.float16, strided=True, seed=1, device="cpu"):
     print(f"[case] window lengths={lengths if len(lengths) < 12 else len(lengths)} window={window} "
           f"sinks={sinks} heads={hq}/{hkv} {half} strided={strided} seed={seed}", flush=True)
     q, k, v, dout = _inputs(sum(lengths), hq, hkv, half, strided, seed)
     got = _call(q, k, v, _cu(lengths), max(lengths), window, sinks, dout)
-    vals, tols = _reference(q, k, v, lengths, D ** -0.5, window, sinks, dout, half)
+    vals, tols = _reference(q, k, v, lengths, D ** -0.5, window, sinks, dout, half, device)
     for name, a, b, tol in zip(("out", "dq", "dk", "dv"), got, vals, tols):
         err = (a.double().cpu() - b).abs()
         ratio = err / tol.clamp_min(1e-30)
@@ -136,6 +136,17 @@ def test_sinks_gradient_over_several_chunks(window, sinks):
 def test_window_from_the_work_queue(sinks):
     """More work items than two per CU: the backward's queue (and its items without a row)."""
     _check([150 + 7 * (i % 9) for i in range(20)] + [900], 60, sinks, 16, 16, seed=5)
+
+
+@pytest.mark.parametrize("lengths,window,sinks,hq,hkv,half", [
+    ([1300] * 16, 60, 6, 6, 1, torch.float16),        # all six heads an item, sinks' rows in chunks
+    ([1300] * 16, 60, 0, 6, 1, torch.float16),
+    ([700, 1, 65, 1500, 0, 900, 128, 2000] * 2, 300, 130, 12, 2, torch.bfloat16),   # some of the heads
+    ([1111, 800] * 6, 1000, 3, 4, 2, torch.float16),
+])
+def test_several_heads_per_item(lengths, window, sinks, hq, hkv, half):
+    """Enough work that a dK / dV item takes several heads of its KV head one after the other."""
+    _check(lengths, window, sinks, hq, hkv, half, seed=7, device="cuda")
 
 
 def test_many_sequences_one_workgroup_per_item():

@@ -156,7 +156,7 @@ def test_adapter_backward_rejects():
 
 @pytest.mark.parametrize("tokens,cols,qblock,qblock2,word", [
     (33, 128, 64, 256, "32 tokens"), (1, 96, 64, 256, "shape"), (1, 128, 32, 256, "blocks"),
-    (1, 128, 64, 200, "blocks"), (-1, 128, 64, 256, "shape")])
+    (1, 128, 64, 200, "blocks"), (-1, 128, 64, 256, "shape"), (1, (1 << 24) + 64, 64, 256, "shape")])
 def test_gemv_rejects(tokens, cols, qblock, qblock2, word):
     status, message = _status("talm_nf4_gemv", PTR, 128, tokens, PTR, PTR, PTR, PTR, PTR, 128, cols,
                               qblock, qblock2, None, None, 0, None, 0, 0, None, 0, 0, PTR, 128, None)
