@@ -51,7 +51,7 @@ struct GemvArgs {
   uint16_t* out;         // [M][ldo]
   int64_t ldo;
   int units;
-  int tiles_per_wg, unit_waves, groups;  // the lut kernel: wavefront w takes units w % unit_waves, .. of
+  int tiles_per_wg, round, unit_waves, groups;  // the lut kernel: wavefront w takes units w % unit_waves, .. of
                                          // tiles w / unit_waves, .. of the workgroup's
 };
 
@@ -65,12 +65,21 @@ struct GemvBlock {
   float s2, o2;
 };
 
+// LDS operations of a wavefront complete in order: its lanes see each other's once the compiler keeps theirs.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+constexpr int kStageBytes = 4096;
+
 // A lane's place in its operands, and its loads of W from the workgroup's first row on and of x.
 template <int P, int TB>
 struct GemvLane {
   static constexpr int R = 16 / P;  // rows of W per tile, and tokens per block
   int row0, wr, part, g;            // wr: the lane's row of a tile (A) and token of a block (B)
-  int64_t first;                    // the workgroup's first weight (its at most 128 rows fit 32 bits: cols <= 2^24)
+  int64_t first;                    // the workgroup's first weight (those after it fit 31 bits)
   __amdgpu_buffer_rsrc_t rw, rs, rx;
   __device__ __forceinline__ GemvLane(const GemvArgs& a, int row, int lane)
       : row0(row), wr(lane & (R - 1)), part((lane & 15) / R), g(lane >> 4),
@@ -102,6 +111,35 @@ struct GemvLane {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         x[b][j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 16 * j, 0));
+    }
+  }
+  // The same operand (P = 1), its global loads in pieces of 64 bytes: half `p` of a token's four blocks by 16
+  // lanes, four tokens at a time, then through the wavefront's kStageBytes of LDS, 16 tokens' halves at a
+  // time. Chunk c (16 bytes) of token n lies at chunk c ^ n: the lanes of a read phase take 16 different.
+  __device__ __forceinline__ void fetch_rows(const GemvArgs& a, int b, int unit, int lane, uint4 (&raw)[8]) const {
+    static_assert(P == 1, "an operand row is one token's");
+    const int c = lane & 15, k = unit * 256 + 64 * (c >> 2) + 8 * (c & 3);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int tok = 16 * b + 4 * (i & 3) + (lane >> 4);
+      const uint32_t off = k < a.cols && tok < a.M ? static_cast<uint32_t>((tok * a.ldx + k) * 2) : kOob;
+      raw[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 64 * (i >> 2), 0));
+    }
+  }
+  __device__ __forceinline__ void stage_rows(unsigned char* slice, int lane, const uint4 (&raw)[8], uint4 (&x)[8]) const {
+    const int n = lane & 15;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      wave_sync();  // the reads of the pass before
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 4 * i + (lane >> 4);
+        *reinterpret_cast<uint4*>(slice + row * 256 + ((n ^ row) << 4)) = raw[4 * p + i];
+      }
+      wave_sync();
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x[4 * p + j] = *reinterpret_cast<const uint4*>(slice + n * 256 + (((4 * g + j) ^ n) << 4));
     }
   }
   // The lane's accumulators to its wavefront's slot: element v is operand row 4 (lane / 16) + v.
@@ -150,7 +188,8 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_rows_kernel(GemvA
   // weights', whose first unit's fly meanwhile
   const float code = tid < 256 ? a.code[tid] : 0.f;
   GemvBlock w, next;
-  uint4 x[TB][8], x_next[TB][8];
+  constexpr bool kAhead = TB == 1;  // x too (two blocks of tokens would spill)
+  uint4 x[TB][8], x_next[kAhead ? TB : 1][8];
   int u = wave;
   if (u < a.units) {
     ln.load_w(a, 0, u, w);
@@ -163,7 +202,7 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_rows_kernel(GemvA
     const bool more = u + waves < a.units;
     if (more) {
       ln.load_w(a, 0, u + waves, next);
-      ln.load_x(a, u + waves, x_next);
+      if constexpr (kAhead) ln.load_x(a, u + waves, x_next);
     }
     const Nf4Table tab = nf4_table(block_scale(table[w.a8], w.s2, w.o2));
     const uint32_t words[8] = {w.lo.x, w.lo.y, w.lo.z, w.lo.w, w.hi.x, w.hi.y, w.hi.z, w.hi.w};
@@ -176,8 +215,9 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_rows_kernel(GemvA
     }
     if (more) {
       w = next;
+      if constexpr (!kAhead) ln.load_x(a, u + waves, x);
 #pragma unroll
-      for (int b = 0; b < TB; ++b)
+      for (int b = 0; b < (kAhead ? TB : 0); ++b)
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[b][j] = x_next[b][j];
     }
@@ -198,8 +238,13 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_rows_kernel(GemvA
 constexpr int kLutBytes = 256 * 256;       // 256 bytes of codes x 32 copies of their two levels
 constexpr int kLutRedFloats = 20 * 1024;   // 80 KiB: the wavefronts' results of every tile
 
-// One workgroup per CU and a.tiles_per_wg tiles. kOne: a wavefront has one unit, whose x it keeps.
-template <int P, int TB, bool kOne>
+// One workgroup per CU and a.tiles_per_wg tiles, joined a.round tiles at a time.
+enum LutX {
+  kEachUnit,  // a wavefront walks several units, and loads the x of each
+  kOneUnit,   // it has one, whose x it keeps
+  kOneStaged  // the same, x loaded through LDS (into the results' room, which has 16 wavefronts' slices)
+};
+template <int P, int TB, LutX kX>
 __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_lut_kernel(GemvArgs a) {
   constexpr int R = 16 / P;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[kLutBytes + 1024 + kLutRedFloats * 4];
@@ -217,9 +262,11 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_lut_kernel(GemvAr
   uint4 x[TB][8];
   int t = grp, u = uw;
   const bool any = t < n_tiles;
+  uint4 raw[8];
   if (any) {
     ln.load_w(a, t, u, w);
-    ln.load_x(a, u, x);
+    if constexpr (kX == kOneStaged) ln.fetch_rows(a, 0, u, lane, raw);
+    else ln.load_x(a, u, x);
   }
   // copy c of byte e's levels at e * 256 + 8 c: a thread writes two copies, a wavefront four bytes of
   // one high nibble (the levels through scalar loads: no wait for the weights either)
@@ -231,13 +278,24 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_lut_kernel(GemvAr
   }
   if (tid < 256) table[tid] = code;
   for (int i = tid + blockDim.x; i < 256; i += blockDim.x) table[i] = a.code[i];
+  if constexpr (kX == kOneStaged)
+    if (any) {
+      unsigned char* slice = reinterpret_cast<unsigned char*>(red) + wave * kStageBytes;
+      ln.stage_rows(slice, lane, raw, x[0]);
+#pragma unroll
+      for (int b = 1; b < TB; ++b) {  // not with the first 16 tokens' loads: 32 registers would be spilled
+        ln.fetch_rows(a, b, u, lane, raw);
+        ln.stage_rows(slice, lane, raw, x[b]);
+      }
+    }
   lds_barrier();
   const uint32_t copy = (lane & 31) * 8;
-  if (any) {
-    f32x4 acc[TB];
+  f32x4 acc[TB];
 #pragma unroll
-    for (int b = 0; b < TB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (;;) {
+  for (int b = 0; b < TB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int first = 0; first < n_tiles; first += a.round) {
+    const int end = min(n_tiles, first + a.round);
+    while (t < end) {
       int tn = t, un = u + a.unit_waves;  // the next step: this tile's next unit, or the next tile
       if (un >= a.units) {
         un = uw;
@@ -263,29 +321,31 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_lut_kernel(GemvAr
         for (int b = 0; b < TB; ++b)
           acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, __builtin_bit_cast(half8_t, x[b][j]), acc[b], 0, 0, 0);
       }
-      if (!more || tn != t) {  // the tile is done
-        ln.leave(acc, red[t * a.unit_waves + uw]);
+      if (tn != t) {  // the tile is done
+        ln.leave(acc, red[(t - first) * a.unit_waves + uw]);
 #pragma unroll
         for (int b = 0; b < TB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
-      if (!more) break;
-      w = next;
       t = tn;
       u = un;
-      if constexpr (!kOne) ln.load_x(a, u, x);
+      if (more) {
+        w = next;
+        if constexpr (kX == kEachUnit) ln.load_x(a, u, x);
+      }
     }
-  }
-  __syncthreads();
-  const int rows = n_tiles * R;
-  for (int i = tid; i < rows * TB * R; i += blockDim.x) {
-    const int rl = i % rows, token = i / rows, b = token / R;
-    if (row0 + rl >= a.rows || token >= a.M) continue;
-    const Slot* slot = red + rl / R * a.unit_waves;
-    float sum = 0.f;
-    for (int v = 0; v < a.unit_waves; ++v)
+    lds_barrier();
+    const int rows = (end - first) * R, row1 = row0 + first * R;
+    for (int i = tid; i < rows * TB * R; i += blockDim.x) {
+      const int rl = i % rows, token = i / rows, b = token / R;
+      if (row1 + rl >= a.rows || token >= a.M) continue;
+      const Slot* slot = red + rl / R * a.unit_waves;
+      float sum = 0.f;
+      for (int v = 0; v < a.unit_waves; ++v)
 #pragma unroll
-      for (int p = 0; p < P; ++p) sum += slot[v][b][p][rl % R][token % R];
-    gemv_store(a, row0 + rl, token, sum);
+        for (int p = 0; p < P; ++p) sum += slot[v][b][p][rl % R][token % R];
+      gemv_store(a, row1 + rl, token, sum);
+    }
+    if (end < n_tiles) lds_barrier();
   }
 }
 
@@ -301,12 +361,22 @@ void launch_gemv(GemvArgs a, bool lut, hipStream_t s) {
     return;
   }
   const int room = kLutRedFloats / (a.unit_waves * TB * P * R * (R + 1));
-  a.tiles_per_wg = std::min(room, (tiles + device_cus() - 1) / device_cus());
-  a.groups = std::max(1, std::min(a.tiles_per_wg, kGemvMaxWaves / a.unit_waves));
+  a.tiles_per_wg = std::min((tiles + device_cus() - 1) / device_cus(), 0x7fffffff / (R * a.cols));  // 32-bit offsets
+  a.groups = std::max(1, std::min(std::min(a.tiles_per_wg, room), kGemvMaxWaves / a.unit_waves));
+  a.round = room / a.groups * a.groups;
   const dim3 grid(static_cast<unsigned>((tiles + a.tiles_per_wg - 1) / a.tiles_per_wg));
   const dim3 block(64 * a.unit_waves * a.groups);
-  if (turns == 1) hipLaunchKernelGGL((nf4_gemv_lut_kernel<P, TB, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((nf4_gemv_lut_kernel<P, TB, false>), grid, block, 0, s, a);
+  if constexpr (P == 1)
+    if (turns == 1 && (TB > 1 || a.M > 8)) {
+      hipLaunchKernelGGL((nf4_gemv_lut_kernel<P, TB, kOneStaged>), grid, block, 0, s, a);
+      return;
+    }
+  if constexpr (TB == 1)
+    if (turns == 1) {
+      hipLaunchKernelGGL((nf4_gemv_lut_kernel<P, TB, kOneUnit>), grid, block, 0, s, a);
+      return;
+    }
+  hipLaunchKernelGGL((nf4_gemv_lut_kernel<P, TB, kEachUnit>), grid, block, 0, s, a);
 }
 
 }  // namespace
