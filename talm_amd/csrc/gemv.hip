@@ -1,7 +1,7 @@
 // Products of a few tokens (1 .. 32) with a weight W [rows, cols] held in the layer group's NF4 form,
-// for the calls that answer token by token: out = x W^T + bias (+ LoRA adapters, ts B^T). Every weight is read once as its
-// 4-bit code, with its block's absmax code and second-level scale, and never written out; the fp16
-// weights are bit-identical to talm_nf4_group_dequant's (solution/qgroup.py:72-99), the products fp32.
+// for the calls that answer token by token: out = x W^T + bias (+ LoRA adapters, ts B^T). Every weight is
+// read once as its 4-bit code, with its block's absmax code and second-level scale, and never written out;
+// the fp16 weights are bit-identical to talm_nf4_group_dequant's (solution/qgroup.py:72-99), the products fp32.
 //
 // The weights are the A operand of v_mfma_f32_16x16x32_f16, the tokens the B operand. A lane takes
 // whole 64-weight blocks (32 contiguous bytes of codes, one scale); the reduction's order is free, so
@@ -18,11 +18,19 @@
 //                address made by one byte permute), scaled and packed: 140 instructions per block.
 //                The table stands in 32 copies, lane l reading copy l % 32, so that the 32 lanes of a
 //                read phase meet 32 different bank pairs whatever their codes are; its 64 KiB cost 1 us
-//                to fill and make one workgroup per CU, whose wavefronts walk several tiles.
-// MI355X, us, rows / lut: W [2048, 1536] 1 token 3.3 / 4.6, 32 tokens 7.0 / 7.1; [17920, 1536] 9.4 / 7.2,
-// 18.7 / 13.4; [1536, 8960] 7.3 / 6.6, 38 / 22. What bounds one token: a launch (1.2 us), one memory
+//                to fill and make one workgroup per CU, whose wavefronts walk all of its tiles, joined as
+//                many at a time as the LDS has room for.
+// A lane's share of x is 16 bytes of 64 columns from the next lane group's: loaded straight, a load
+// instruction of many tokens touches 64 cache lines, and the eight that share them run behind each other
+// through a smaller cache. With many tokens x comes in pieces of 64 bytes and changes places in LDS
+// (us, straight / through LDS: W [17920, 1536] 16 tokens 9.7 / 8.3, 32 tokens 13.5 / 10.1; [1536, 8960] 16
+// tokens 14.3 / 10.1, 32 tokens 21.8 / 13.3; several units per wavefront, [3584, 18944]: 2 tokens 16.9 / 18.5,
+// 4 20.4 / 18.6, 8 27.7 / 20.0; [1536, 8960] 5 tokens 7.7 / 8.0, 6 8.3 / 8.0).
+// MI355X, us, rows / lut: W [2048, 1536] 1 token 3.1 / 5.6, 32 tokens 6.0 / 6.1; [8960, 1536] 7.2 / 6.0,
+// 14.3 / 8.6; lut: [17920, 1536] 7.1 and 10.1 (2.0 TB/s of codes and scales), [1536, 8960] 6.8 and 13.3,
+// [152064, 1536] 28 and 42 (4.3 TB/s, 2.9). What bounds one token: a launch (1.2 us), one memory
 // round trip with the whole of W in flight, the lookups behind it (LDS and VALU 1.4 us each) and the
-// join, one after the other; many tokens: x's operand reads through L2.
+// join, one after the other; many tokens: x's way through L2 and LDS, and the lookups.
 #include "mfma_tile.h"
 #include "nf4_code.h"
 
@@ -113,34 +121,30 @@ struct GemvLane {
         x[b][j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 16 * j, 0));
     }
   }
-  // The same operand (P = 1), its global loads in pieces of 64 bytes: half `p` of a token's four blocks by 16
+  // The same operand, its global loads in pieces of 64 bytes: half `p` of a token's four blocks by 16
   // lanes, four tokens at a time, then through the wavefront's kStageBytes of LDS, 16 tokens' halves at a
   // time. Chunk c (16 bytes) of token n lies at chunk c ^ n: the lanes of a read phase take 16 different.
   __device__ __forceinline__ void fetch_rows(const GemvArgs& a, int b, int unit, int lane, uint4 (&raw)[8]) const {
-    static_assert(P == 1, "an operand row is one token's");
-    const int c = lane & 15, k = unit * 256 + 64 * (c >> 2) + 8 * (c & 3);
+    const int c = lane & 15;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int tok = 16 * b + 4 * (i & 3) + (lane >> 4);
+      const int n = 4 * (i & 3) + (lane >> 4), tok = R * b + (n & (R - 1));
+      const int k = (unit * P + n / R) * 256 + 64 * (c >> 2) + 8 * (c & 3);
       const uint32_t off = k < a.cols && tok < a.M ? static_cast<uint32_t>((tok * a.ldx + k) * 2) : kOob;
       raw[i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rx, off, 64 * (i >> 2), 0));
     }
   }
-  __device__ __forceinline__ void stage_rows(unsigned char* slice, int lane, const uint4 (&raw)[8], uint4 (&x)[8]) const {
+  __device__ __forceinline__ void stage_half(unsigned char* slice, int lane, const uint4* raw, uint4* x) const {
     const int n = lane & 15;
+    wave_sync();  // the reads of the half before
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      wave_sync();  // the reads of the pass before
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 4 * i + (lane >> 4);
-        *reinterpret_cast<uint4*>(slice + row * 256 + ((n ^ row) << 4)) = raw[4 * p + i];
-      }
-      wave_sync();
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        x[4 * p + j] = *reinterpret_cast<const uint4*>(slice + n * 256 + (((4 * g + j) ^ n) << 4));
+    for (int i = 0; i < 4; ++i) {
+      const int row = 4 * i + (lane >> 4);
+      *reinterpret_cast<uint4*>(slice + row * 256 + ((n ^ row) << 4)) = raw[i];
     }
+    wave_sync();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = *reinterpret_cast<const uint4*>(slice + n * 256 + (((4 * g + j) ^ n) << 4));
   }
   // The lane's accumulators to its wavefront's slot: element v is operand row 4 (lane / 16) + v.
   __device__ __forceinline__ void leave(const f32x4 (&acc)[TB], float (&slot)[TB][P][R][R + 1]) const {
@@ -153,6 +157,24 @@ struct GemvLane {
       }
   }
 };
+
+// The sum of element (row, token) over `n` wavefronts' slots, in order; four slots' loads at a time.
+template <int P, int R, class Slot>
+__device__ __forceinline__ float gemv_join(const Slot* slot, int n, int b, int row, int token) {
+  float sum = 0.f;
+  for (int v0 = 0; v0 < n; v0 += 4) {
+    float f[4][P];
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int p = 0; p < P; ++p) f[v][p] = slot[min(v0 + v, n - 1)][b][p][row][token];
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+#pragma unroll
+      for (int p = 0; p < P; ++p) sum += v0 + v < n ? f[v][p] : 0.f;
+  }
+  return sum;
+}
 
 // The sum of the joined parts, bias and adapters, rounded and stored.
 __device__ __forceinline__ void gemv_store(const GemvArgs& a, int row, int token, float sum) {
@@ -173,7 +195,6 @@ __device__ __forceinline__ void gemv_store(const GemvArgs& a, int row, int token
 // One workgroup per tile, a wavefront per unit (or several), the next unit's loads in flight.
 template <int P, int TB>
 __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_rows_kernel(GemvArgs a) {
-  static_assert(TB == 1 || P == 1, "two token blocks need every operand column");
   constexpr int R = 16 / P;
   __shared__ float table[256];
   __shared__ float red[kGemvMaxWaves][TB][P][R][R + 1];
@@ -227,30 +248,36 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_rows_kernel(GemvA
   for (int i = tid; i < TB * R * R; i += blockDim.x) {
     const int r = i % R, tok = i / R % R, b = i / (R * R);
     if (row0 + r >= a.rows || tok + R * b >= a.M) continue;
-    float sum = 0.f;
-    for (int v = 0; v < waves; ++v)
-#pragma unroll
-      for (int p = 0; p < P; ++p) sum += red[v][b][p][r][tok];
-    gemv_store(a, row0 + r, tok + R * b, sum);
+    gemv_store(a, row0 + r, tok + R * b, gemv_join<P, R>(red, waves, b, r, tok));
   }
 }
 
-constexpr int kLutBytes = 256 * 256;       // 256 bytes of codes x 32 copies of their two levels
-constexpr int kLutRedFloats = 20 * 1024;   // 80 KiB: the wavefronts' results of every tile
+constexpr int kLutBytes = 256 * 256;  // 256 bytes of codes x 32 copies of their two levels
 
 // One workgroup per CU and a.tiles_per_wg tiles, joined a.round tiles at a time.
 enum LutX {
-  kEachUnit,  // a wavefront walks several units, and loads the x of each
-  kOneUnit,   // it has one, whose x it keeps
-  kOneStaged  // the same, x loaded through LDS (into the results' room, which has 16 wavefronts' slices)
+  kEachUnit,   // a wavefront walks several units, and loads the x of each
+  kOneUnit,    // it has one, whose x it keeps
+  kOneStaged,  // the same, x loaded through LDS, where the results go later
+  kEachStaged  // several, the x of each through LDS, half by half where the products take it
+};
+template <LutX kX>
+struct LutRoom {  // wavefronts, and LDS: 160 KiB or less of the lookup table, absmax's, the x slices and
+                  // the wavefronts' results of a round of tiles
+  static constexpr int kWaves = kX == kEachStaged ? 12 : kGemvMaxWaves;
+  static constexpr int kSlices = kX == kEachStaged ? kWaves * kStageBytes : 0;
+  static constexpr int kRedFloats = kX == kEachStaged ? 11 * 1024 : 20 * 1024;
+  static_assert(kX != kOneStaged || kWaves * kStageBytes <= kRedFloats * 4, "the slices lie in the results' room");
+  static constexpr int kBytes = kLutBytes + 1024 + kSlices + kRedFloats * 4;
+  static_assert(kBytes <= 160 * 1024, "LDS");
 };
 template <int P, int TB, LutX kX>
-__global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_lut_kernel(GemvArgs a) {
+__global__ __launch_bounds__(64 * LutRoom<kX>::kWaves) void nf4_gemv_lut_kernel(GemvArgs a) {
   constexpr int R = 16 / P;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[kLutBytes + 1024 + kLutRedFloats * 4];
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[LutRoom<kX>::kBytes];
   float* table = reinterpret_cast<float*>(smem + kLutBytes);
   typedef float Slot[TB][P][R][R + 1];
-  Slot* red = reinterpret_cast<Slot*>(smem + kLutBytes + 1024);  // [tile][unit wavefront]
+  Slot* red = reinterpret_cast<Slot*>(smem + kLutBytes + 1024 + LutRoom<kX>::kSlices);  // [tile][unit wavefront]
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int uw = wave % a.unit_waves, grp = wave / a.unit_waves;
@@ -258,14 +285,20 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_lut_kernel(GemvAr
   const int n_tiles = min(a.tiles_per_wg, (a.rows - row0 + R - 1) / R);
   const GemvLane<P, TB> ln(a, row0, lane);
   const float code = tid < 256 ? a.code[tid] : 0.f;  // first, as above
+  unsigned char* slice = smem + kLutBytes + 1024 + wave * kStageBytes;
   GemvBlock w;
-  uint4 x[TB][8];
+  uint4 x[kX == kEachStaged ? 1 : TB][8], raw[kX == kEachStaged ? TB : 1][8];
   int t = grp, u = uw;
   const bool any = t < n_tiles;
-  uint4 raw[8];
+  auto fetch = [&](int unit) __attribute__((always_inline)) {
+    if constexpr (kX == kEachStaged)
+#pragma unroll
+      for (int b = 0; b < TB; ++b) ln.fetch_rows(a, b, unit, lane, raw[b]);
+  };
   if (any) {
     ln.load_w(a, t, u, w);
-    if constexpr (kX == kOneStaged) ln.fetch_rows(a, 0, u, lane, raw);
+    if constexpr (kX == kOneStaged) ln.fetch_rows(a, 0, u, lane, raw[0]);
+    else if constexpr (kX == kEachStaged) fetch(u);
     else ln.load_x(a, u, x);
   }
   // copy c of byte e's levels at e * 256 + 8 c: a thread writes two copies, a wavefront four bytes of
@@ -280,15 +313,17 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_lut_kernel(GemvAr
   for (int i = tid + blockDim.x; i < 256; i += blockDim.x) table[i] = a.code[i];
   if constexpr (kX == kOneStaged)
     if (any) {
-      unsigned char* slice = reinterpret_cast<unsigned char*>(red) + wave * kStageBytes;
-      ln.stage_rows(slice, lane, raw, x[0]);
 #pragma unroll
-      for (int b = 1; b < TB; ++b) {  // not with the first 16 tokens' loads: 32 registers would be spilled
-        ln.fetch_rows(a, b, u, lane, raw);
-        ln.stage_rows(slice, lane, raw, x[b]);
+      for (int b = 0; b < TB; ++b) {
+        if (b) ln.fetch_rows(a, b, u, lane, raw[0]);  // not with the first 16 tokens': 32 registers would be spilled
+        ln.stage_half(slice, lane, raw[0], x[b]);
+        ln.stage_half(slice, lane, raw[0] + 4, x[b] + 4);
       }
     }
   lds_barrier();
+  // The first step needs all of its loads anyway; without this wait the compiler, which sees a path that skipped
+  // their uses, would wait for them inside the loop, and so for the next step's.
+  if constexpr (kX != kEachUnit) __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
   const uint32_t copy = (lane & 31) * 8;
   f32x4 acc[TB];
 #pragma unroll
@@ -306,20 +341,39 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_lut_kernel(GemvAr
       if (more) ln.load_w(a, tn, un, next);
       const float scale = block_scale(table[w.a8], w.s2, w.o2);
       const uint32_t words[8] = {w.lo.x, w.lo.y, w.lo.z, w.lo.w, w.hi.x, w.hi.y, w.hi.z, w.hi.w};
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      auto levels = [&](uint32_t word) __attribute__((always_inline)) {
         uint32_t h[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {  // byte q of the word to bits 8..15, the copy below it
-          const uint32_t at = __builtin_amdgcn_perm(words[j], copy, 0x0c0c0400u + (static_cast<uint32_t>(q) << 8));
+          const uint32_t at = __builtin_amdgcn_perm(word, copy, 0x0c0c0400u + (static_cast<uint32_t>(q) << 8));
           const float2 f = *reinterpret_cast<const float2*>(smem + at);
           h[q] = __builtin_bit_cast(uint32_t, __builtin_convertvector(
                                                   (nf4_float2_t){mul_f32(f.x, scale), mul_f32(f.y, scale)}, nf4_half2_t));
         }
-        const half8_t wf = __builtin_bit_cast(half8_t, make_uint4(h[0], h[1], h[2], h[3]));
+        return __builtin_bit_cast(half8_t, make_uint4(h[0], h[1], h[2], h[3]));
+      };
+      if constexpr (kX == kEachStaged) {
 #pragma unroll
-        for (int b = 0; b < TB; ++b)
-          acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, __builtin_bit_cast(half8_t, x[b][j]), acc[b], 0, 0, 0);
+        for (int p = 0; p < 2; ++p) {
+          half8_t wf[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) wf[j] = levels(words[4 * p + j]);
+#pragma unroll
+          for (int b = 0; b < TB; ++b) {
+            ln.stage_half(slice, lane, raw[b] + 4 * p, x[0]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[j], __builtin_bit_cast(half8_t, x[0][j]), acc[b], 0, 0, 0);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const half8_t wf = levels(words[j]);
+#pragma unroll
+          for (int b = 0; b < TB; ++b)
+            acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf, __builtin_bit_cast(half8_t, x[b][j]), acc[b], 0, 0, 0);
+        }
       }
       if (tn != t) {  // the tile is done
         ln.leave(acc, red[(t - first) * a.unit_waves + uw]);
@@ -330,7 +384,8 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_lut_kernel(GemvAr
       u = un;
       if (more) {
         w = next;
-        if constexpr (kX == kEachUnit) ln.load_x(a, u, x);
+        if constexpr (kX == kEachStaged) fetch(u);
+        else if constexpr (kX == kEachUnit) ln.load_x(a, u, x);
       }
     }
     lds_barrier();
@@ -339,44 +394,43 @@ __global__ __launch_bounds__(64 * kGemvMaxWaves) void nf4_gemv_lut_kernel(GemvAr
       const int rl = i % rows, token = i / rows, b = token / R;
       if (row1 + rl >= a.rows || token >= a.M) continue;
       const Slot* slot = red + rl / R * a.unit_waves;
-      float sum = 0.f;
-      for (int v = 0; v < a.unit_waves; ++v)
-#pragma unroll
-        for (int p = 0; p < P; ++p) sum += slot[v][b][p][rl % R][token % R];
-      gemv_store(a, row1 + rl, token, sum);
+      gemv_store(a, row1 + rl, token, gemv_join<P, R>(slot, a.unit_waves, b, rl % R, token % R));
     }
     if (end < n_tiles) lds_barrier();
   }
 }
 
+template <int P, int TB, LutX kX>
+void launch_lut(GemvArgs a, hipStream_t s) {
+  constexpr int R = 16 / P, most = LutRoom<kX>::kWaves;
+  const int tiles = (a.rows + R - 1) / R, turns = (a.units + most - 1) / most;
+  a.unit_waves = (a.units + turns - 1) / turns;
+  const int room = LutRoom<kX>::kRedFloats / (a.unit_waves * TB * P * R * (R + 1));
+  a.tiles_per_wg = std::min((tiles + device_cus() - 1) / device_cus(), 0x7fffffff / (R * a.cols));  // 32-bit offsets
+  a.groups = std::max(1, std::min(std::min(a.tiles_per_wg, room), most / a.unit_waves));
+  a.round = room / a.groups * a.groups;
+  hipLaunchKernelGGL((nf4_gemv_lut_kernel<P, TB, kX>),
+                     dim3(static_cast<unsigned>((tiles + a.tiles_per_wg - 1) / a.tiles_per_wg)),
+                     dim3(64 * a.unit_waves * a.groups), 0, s, a);
+}
+
 template <int P, int TB>
 void launch_gemv(GemvArgs a, bool lut, hipStream_t s) {
   constexpr int R = 16 / P;
-  const int tiles = (a.rows + R - 1) / R;
   a.units = (a.cols + 256 * P - 1) / (256 * P);
-  const int turns = (a.units + kGemvMaxWaves - 1) / kGemvMaxWaves;
-  a.unit_waves = (a.units + turns - 1) / turns;
+  const bool one = a.units <= kGemvMaxWaves;
   if (!lut) {
-    hipLaunchKernelGGL((nf4_gemv_rows_kernel<P, TB>), dim3(static_cast<unsigned>(tiles)), dim3(64 * a.unit_waves), 0, s, a);
+    const int turns = (a.units + kGemvMaxWaves - 1) / kGemvMaxWaves, waves = (a.units + turns - 1) / turns;
+    hipLaunchKernelGGL((nf4_gemv_rows_kernel<P, TB>), dim3(static_cast<unsigned>((a.rows + R - 1) / R)), dim3(64 * waves),
+                       0, s, a);
     return;
   }
-  const int room = kLutRedFloats / (a.unit_waves * TB * P * R * (R + 1));
-  a.tiles_per_wg = std::min((tiles + device_cus() - 1) / device_cus(), 0x7fffffff / (R * a.cols));  // 32-bit offsets
-  a.groups = std::max(1, std::min(std::min(a.tiles_per_wg, room), kGemvMaxWaves / a.unit_waves));
-  a.round = room / a.groups * a.groups;
-  const dim3 grid(static_cast<unsigned>((tiles + a.tiles_per_wg - 1) / a.tiles_per_wg));
-  const dim3 block(64 * a.unit_waves * a.groups);
-  if constexpr (P == 1)
-    if (turns == 1 && (TB > 1 || a.M > 8)) {
-      hipLaunchKernelGGL((nf4_gemv_lut_kernel<P, TB, kOneStaged>), grid, block, 0, s, a);
-      return;
-    }
-  if constexpr (TB == 1)
-    if (turns == 1) {
-      hipLaunchKernelGGL((nf4_gemv_lut_kernel<P, TB, kOneUnit>), grid, block, 0, s, a);
-      return;
-    }
-  hipLaunchKernelGGL((nf4_gemv_lut_kernel<P, TB, kEachUnit>), grid, block, 0, s, a);
+  if constexpr (P < 4)
+    if (a.M > (one ? 8 : 5)) return one ? launch_lut<P, TB, kOneStaged>(a, s) : launch_lut<P, TB, kEachStaged>(a, s);
+  if constexpr (TB == 1 && P < 4) {
+    if (one) launch_lut<P, TB, kOneUnit>(a, s);
+    else launch_lut<P, TB, kEachUnit>(a, s);
+  }
 }
 
 }  // namespace
@@ -418,18 +472,21 @@ TALM_API int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, con
     if (b1) { a.b[1] = b1; a.lo[1] = static_cast<int>(lo1); a.hi[1] = static_cast<int>(hi1); }
   }
   // The table in LDS pays from some size of W on, an earlier one with more tokens. us, rows / lut:
-  // 1 token [1536, 4864] 4.8 / 5.3, [8960, 1024] 5.2 / 5.3, [8960, 1536] 6.4 / 6.1; 16 tokens [4864, 896]
-  // 4.7 / 5.4, [1536, 3584] 8.0 / 7.7, [1536, 4864] 9.7 / 8.9; 32 tokens [2048, 1536] 7.1 / 7.1,
-  // [1792, 2048] 7.9 / 7.7, [1536, 3584] 12.4 / 11.0.
+  // 1 token [1536, 4864] 5.0 / 5.3, [8960, 1024] 5.1 / 5.2, [8960, 1536] 7.2 / 6.0; 16 tokens [4864, 896]
+  // 4.6 / 5.2, [1536, 3584] 7.9 / 6.0, [1536, 4864] 9.7 / 6.8; 32 tokens [2048, 1536] 6.1 / 6.1,
+  // [1792, 2048] 7.1 / 6.0, [1536, 3584] 11.5 / 7.5.
   const bool lut = rows * cols > (n_tokens <= 8 ? 9 << 20 : n_tokens <= 16 ? 5 << 20 : 3 << 20);
   // Parts of the reduction per tile: what the tokens leave room for, and
   //   rows kernel: the fewest idle lanes and CUs (1 token, one / two / four parts: [2048, 1536] 3.8 / 3.2 /
   //     3.8 us, [4864, 896] 3.7 / 3.8 / 4.0);
-  //   lut kernel: two where whole tiles would leave CUs without one ([1536, 8960] 8.3 / 6.6).
+  //   lut kernel: two where whole tiles would leave CUs without one (1 token, one / two parts: [1536, 8960]
+  //     8.3 / 6.8, [2048, 8192] 8.2 / 6.2), of 9 tokens on, which then are two blocks, where the halves
+  //     leave no CU with two (16 tokens: [2048, 8192] 10.3 / 8.6; [3584, 18944] 20 / 27).
   int best = 1;
   const double cus = device_cus();
   if (lut) {
-    best = n_tokens <= 8 && (rows + 15) / 16 < device_cus() ? 2 : 1;
+    const int64_t tiles = (rows + 15) / 16;
+    best = n_tokens <= 8 ? (tiles < device_cus() ? 2 : 1) : (n_tokens <= 16 && 2 * tiles <= device_cus() ? 2 : 1);
   } else {
     double cost = 0;
     for (int p = 1; p <= 4 && p * n_tokens <= 16; p *= 2) {
@@ -441,6 +498,7 @@ TALM_API int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, con
   }
   const hipStream_t s = as_stream(stream);
   if (n_tokens > 16) launch_gemv<1, 2>(a, lut, s);
+  else if (best == 2 && n_tokens > 8) launch_gemv<2, 2>(a, lut, s);
   else if (best == 1) launch_gemv<1, 1>(a, lut, s);
   else if (best == 2) launch_gemv<2, 1>(a, lut, s);
   else launch_gemv<4, 1>(a, false, s);

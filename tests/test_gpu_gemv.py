@@ -73,6 +73,38 @@ def test_gemv_of_the_layer_shapes():
             _check(group, x, first, last)
 
 
+@pytest.mark.parametrize("rows,cols", [
+    (9092, 4096),    # more tiles per workgroup than the LDS joins at a time, x through LDS; a partial tile
+    (20612, 4096),   # the same, x straight
+    (9088, 4352),    # several units per wavefront
+    (33088, 4352),
+    (2044, 4096),    # two parts per tile, one unit
+    (1536, 16640),   # and several
+    (1536, 704),     # a table in registers
+])
+def test_gemv_over_tiles(rows, cols):
+    print(f"[case] gemv over tiles W {rows} x {cols}", flush=True)
+    group = _group(SHAPES[:6] + ((rows, cols),), seed=rows)
+    g = torch.Generator("cuda").manual_seed(rows)
+    for tokens in (1, 5, 6, 8, 9, 13, 16, 17, 27, 32):
+        _check(group, torch.randn(tokens, cols, generator=g, device="cuda").half(), 6, 7)
+
+
+def test_gemv_keeps_nan_and_infinity_to_their_token():
+    """x's rows do not mix, whichever way they are loaded."""
+    for cols in (512, 4096, 8960):
+        group = _group(SHAPES[:6] + ((1536, cols),), seed=cols)
+        for tokens in (2, 8, 12, 32):
+            x = torch.randn(tokens, cols, device="cuda").half()
+            out, bad = (torch.empty(tokens, 1536, dtype=torch.float16, device="cuda") for _ in range(2))
+            group.nf4_gemv(x, 6, 7, out)
+            x[1, cols - 1], x[tokens - 1, 3] = float("nan"), float("inf")
+            group.nf4_gemv(x, 6, 7, bad)
+            kept = [t for t in range(tokens) if t not in (1, tokens - 1)]
+            assert torch.equal(out[kept], bad[kept])
+            assert bad[1].isnan().all() and not bad[tokens - 1].isfinite().any()
+
+
 def test_gemv_rows_of_a_wider_buffer_and_refusals():
     group = _group()
     wide = torch.randn(5, 1024, device="cuda").half()
