@@ -196,8 +196,8 @@ def adapter_branch(x, lora_a, lora_b, scaling, p=0.0, key=None, site=0):
     """A LoRA adapter's branch scaling * (dropout(x) A^T) B^T with gradients for x, A and B: x fp16
     [..., in], A [16, in] and B [out, 16] fp16 or fp32 (fp32 ones are read as fp16 copies, their
     gradients fp32), in and out multiples of 32; the dropout as `dropout.dropout` on x's rows, its mask
-    computed in each product (talm_lora_down_drop, talm_lora_up, talm_lora_wgrad_drop) and never
-    stored, no dropped copy of x: PEFT's branch (solution/lora.py:183-231) on MFMA. An autograd node
+    computed in each product (talm_lora_branch_fwd, talm_lora_bwd_drop) and never stored, no dropped
+    copy of x: PEFT's branch (solution/lora.py:183-231) on MFMA. An autograd node
     of the C++ op layer, differentiable once."""
     return torch.ops.talm.adapter_branch(x, lora_a, lora_b, _half(lora_a), _half(lora_b), scaling, p,
                                          key, site)

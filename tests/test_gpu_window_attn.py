@@ -276,3 +276,65 @@ def test_captured_forward_and_backward_replay():
         want = _call(*fresh[:3], _cu(lengths), 640, 50, 3, fresh[3])
         for a, b in zip(outs, want):
             assert torch.equal(a, b)
+
+
+def test_broadcast_operands_and_gradients():
+    """A KV head and gradients given as expanded views: the copies' results, a shared head's gradient the sum of
+    what its copies get (two roundings of each, one of their sum: three half steps of the magnitudes)."""
+    q, k, v, dout = _inputs(300, 4, 1, torch.float16, True, 9)
+    cu = _cu([170, 130])
+    want = _call(q, k.expand(300, 2, D).contiguous(), v.expand(300, 2, D).contiguous(), cu, 170, 40, 2, dout)
+    from talm_amd.unpad import window_attention
+
+    leaves = [t.transpose(0, 1)[None].detach().requires_grad_() for t in (q, k, v)]
+    out = window_attention(leaves[0], *(t.expand(1, 2, 300, D) for t in leaves[1:]), cu, 170, D ** -0.5, 40, 2)
+    grads = torch.autograd.grad(out, leaves, dout[None])
+    assert torch.equal(out[0].detach(), want[0]) and torch.equal(grads[0][0].transpose(0, 1), want[1])
+    for got, copies in zip(grads[1:], want[2:]):
+        copies = copies.double()
+        tol = 3 * 2.0 ** -11 * copies.abs().sum(1) + 2.0 ** -24
+        assert ((got[0, 0].double() - copies.sum(1)).abs() <= tol).all()
+    for shape in ((1, 1, 4, D), (1, 300, 1, D), (1, 300, 4, 1), (1, 1, 1, 1)):
+        part = torch.randn(shape, device="cuda").half()
+        dense = part.expand(1, 300, 4, D).contiguous()
+        leaf = q.transpose(0, 1)[None].detach().requires_grad_()
+        kv = [t.transpose(0, 1)[None] for t in (k, v)]
+        for full in (part.expand(1, 300, 4, D), dense):
+            out = window_attention(leaf, *kv, cu, 170, D ** -0.5, 40, 2)
+            (g,) = torch.autograd.grad(out, leaf, full)
+            first = g if full is not dense else first
+        assert torch.equal(first, g)
+
+
+def test_two_calls_at_once():
+    """Calls on two streams, their workspaces their own: each one's results are those it has alone."""
+    cases = [(_inputs(2000, 6, 1, torch.float16, True, s), [900, 1100], w, n) for s, w, n in ((3, 100, 5), (4, 300, 0))]
+    want = [_call(*t[:3], _cu(ls), 1100, w, n, t[3]) for t, ls, w, n in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    cus = [_cu(ls) for _, ls, _, _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for stream, cu, (t, _, w, n) in zip(streams, cus, cases):
+            with torch.cuda.stream(stream):
+                got.append(_call(*t[:3], cu, 1100, w, n, t[3]))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_in_inference_mode():
+    from talm_amd.dropout import dropout
+    from talm_amd.lora import adapter_branch
+
+    q, k, v, _ = _inputs(100, 4, 2, torch.float16, True, 2)
+    key = torch.tensor([5, 6], device="cuda")
+    x, a, b = torch.randn(9, 64, device="cuda").half(), torch.randn(16, 64, device="cuda"), \
+        torch.randn(32, 16, device="cuda")
+    want = _call(q, k, v, _cu([100]), 100, 20, 1), dropout(x, 0.3, key), adapter_branch(x, a, b, 1.0, 0.3, key)
+    with torch.inference_mode():
+        from talm_amd.unpad import window_attention
+
+        out = window_attention(*(t.transpose(0, 1)[None] for t in (q, k, v)), _cu([100]), 100, D ** -0.5, 20, 1)
+        got = out[0], dropout(x, 0.3, key), adapter_branch(x, a, b, 1.0, 0.3, key)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
