@@ -49,48 +49,67 @@ struct F32Elem {
   typedef float type;
 };
 
-// One thread per eight columns of a row (or several such, one grid apart, of more than 2^30 of them).
-// kVec: whole chunks, 16-byte aligned rows. Bound by memory: fp16 or bf16 [2048, 8960] 13.1 us, 5.6 TB/s (a
-// large copy reaches 4.9); the generator, about 70 VALU instructions per chunk with 20 of them at a quarter
-// of the rate, runs beside the loads.
+// n / d of n < 2^31 as (mulhi(mul, n) + n) >> shift; shift -1: the division itself.
+struct Divider {
+  uint32_t mul;
+  int shift;
+};
+Divider divider(int64_t most, int64_t d) {
+  if (most >= int64_t{1} << 31) return Divider{0, -1};
+  int s = 0;
+  while ((int64_t{1} << s) < d) ++s;
+  return Divider{static_cast<uint32_t>((((uint64_t{1} << s) - d) << 32) / d + 1), s};
+}
+
+// One thread per eight columns of a row, `first` those of the launches before. kVec: whole chunks, 16-byte
+// aligned rows. The generator, about 70 VALU instructions per chunk with 20 of them at a quarter of the rate,
+// runs beside other wavefronts' loads: the thread's own load is issued before the key's (16.8 us for bf16
+// [2048, 8960] the other way round).
+// Bound by memory: bf16 [2048, 8960] 14.2 us (5.2 TB/s; a large copy reaches 4.9), [40000, 4096] 107 (6.1);
+// fp32 [2048, 8960] 31.2 (4.7).
 template <class E, bool kVec>
 __global__ __launch_bounds__(256) void dropout_kernel(const typename E::type* __restrict__ x, int64_t ldx,
                                                       int64_t rows, int64_t cols, float factor,
                                                       DropArgs drop, typename E::type* __restrict__ y,
-                                                      int64_t ldy) {
+                                                      int64_t ldy, int64_t first, Divider div) {
   typedef typename E::type T;
-  const int64_t per_row = (cols + 7) / 8, blocks = rows * per_row, step = static_cast<int64_t>(gridDim.x) * 256;
+  const int64_t per_row = (cols + 7) / 8;
+  const int64_t block = first + static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (block >= rows * per_row) return;
+  int64_t r;
+  if (div.shift >= 0) {
+    const uint32_t n = static_cast<uint32_t>(block);
+    r = (__umulhi(div.mul, n) + n) >> div.shift;
+  } else {
+    r = block / per_row;
+  }
+  const int64_t c = (block - r * per_row) * 8;
+  const T* xp = x + r * ldx + c;
+  T* yp = y + r * ldy + c;
+  const int n = kVec ? 8 : static_cast<int>(min(cols - c, static_cast<int64_t>(8)));
+  T v[8];
+  if constexpr (kVec) {
+    *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(xp);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(v + 4) = *reinterpret_cast<const uint4*>(xp + 4);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? xp[e] : T(0);
+  }
   const DropKey key(drop.key, drop.site, drop.threshold);
-  for (int64_t block = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; block < blocks; block += step) {
-    // one 64-bit division where 32 bits do not hold the index
-    const int64_t r = blocks <= 0xffffffffll ? static_cast<uint32_t>(block) / static_cast<uint32_t>(per_row) : block / per_row;
-    const int64_t c = (block - r * per_row) * 8;
-    const T* xp = x + r * ldx + c;
-    T* yp = y + r * ldy + c;
-    const int n = kVec ? 8 : static_cast<int>(min(cols - c, static_cast<int64_t>(8)));
-    T v[8];
-    if constexpr (kVec) {
-      *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(xp);
-      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(v + 4) = *reinterpret_cast<const uint4*>(xp + 4);
-    } else {
+  const uint4 bits = philox_block(static_cast<uint64_t>(block), key);
+  const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = e < n ? xp[e] : T(0);
-    }
-    const uint4 bits = philox_block(static_cast<uint64_t>(block), key);
-    const uint32_t w[4] = {bits.x, bits.y, bits.z, bits.w};
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t u = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
+    v[e] = u >= key.threshold ? E::put(E::get(v[e]) * factor) : T(0);
+  }
+  if constexpr (kVec) {
+    *reinterpret_cast<uint4*>(yp) = *reinterpret_cast<const uint4*>(v);
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(yp + 4) = *reinterpret_cast<const uint4*>(v + 4);
+  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t u = e & 1 ? w[e >> 1] >> 16 : w[e >> 1] & 0xffffu;
-      v[e] = u >= key.threshold ? E::put(E::get(v[e]) * factor) : T(0);
-    }
-    if constexpr (kVec) {
-      *reinterpret_cast<uint4*>(yp) = *reinterpret_cast<const uint4*>(v);
-      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(yp + 4) = *reinterpret_cast<const uint4*>(v + 4);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < n) yp[e] = v[e];
-    }
+    for (int e = 0; e < 8; ++e)
+      if (e < n) yp[e] = v[e];
   }
 }
 
@@ -543,16 +562,20 @@ TALM_API int talm_dropout(const void* x, int64_t ldx, int64_t rows, int64_t cols
   const DropArgs drop{key, site, drop_threshold(p)};
   const float factor = drop_factor(drop.threshold);
   const int64_t n = rows * ((cols + 7) / 8);
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((n + 255) / 256, 1 << 22)));
+  const Divider div = divider(n, (cols + 7) / 8);
   const int64_t unit = dtype == TALM_F32 ? 4 : 8;  // elements of 16 bytes
   const bool vec = cols % 8 == 0 && ldx % unit == 0 && ldy % unit == 0 && aligned(x, 16) && aligned(y, 16);
   const hipStream_t s = as_stream(stream);
 #define TALM_DROPOUT(E, V)                                                                             \
   hipLaunchKernelGGL((dropout_kernel<E, V>), grid, dim3(256), 0, s, static_cast<const E::type*>(x), ldx, \
-                     rows, cols, factor, drop, static_cast<E::type*>(y), ldy)
-  if (dtype == TALM_F32) { if (vec) TALM_DROPOUT(F32Elem, true); else TALM_DROPOUT(F32Elem, false); }
-  else if (dtype == TALM_F16) { if (vec) TALM_DROPOUT(F16Elem, true); else TALM_DROPOUT(F16Elem, false); }
-  else { if (vec) TALM_DROPOUT(BF16Elem, true); else TALM_DROPOUT(BF16Elem, false); }
+                     rows, cols, factor, drop, static_cast<E::type*>(y), ldy, first, div)
+  constexpr int64_t kMost = int64_t{1} << 30;  // a launch's threads stay below 2^32
+  for (int64_t first = 0; first < n; first += kMost) {
+    const dim3 grid(static_cast<unsigned>((std::min(kMost, n - first) + 255) / 256));
+    if (dtype == TALM_F32) { if (vec) TALM_DROPOUT(F32Elem, true); else TALM_DROPOUT(F32Elem, false); }
+    else if (dtype == TALM_F16) { if (vec) TALM_DROPOUT(F16Elem, true); else TALM_DROPOUT(F16Elem, false); }
+    else { if (vec) TALM_DROPOUT(BF16Elem, true); else TALM_DROPOUT(BF16Elem, false); }
+  }
 #undef TALM_DROPOUT
   return check_launch("dropout");
 }
