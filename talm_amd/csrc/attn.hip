@@ -7,7 +7,7 @@
 // reference's per-KV-head memory-efficient attention launches (solution/unpad.py:199-294), whose
 // semantics are per-row causal SDPA (solution/unpad.py:121-134).
 //
-// The forward is a flash-attention pass per (sequence, query tile, query heads of one KV head),
+// The forward is one pass with a running maximum and sum per (sequence, query tile, query heads of one KV head),
 // 32 query rows of a head per wavefront, its key tiles of 64 streamed with direct-to-LDS loads and,
 // where few workgroups leave the chip idle, split between two groups of wavefronts. Scores are
 // computed transposed, S^T = K Q^T (v_mfma_f32_32x32x16_f16), so each lane owns one query row (its
@@ -18,7 +18,7 @@
 // row statistics are kept in base 2 (scores times scale * log2 e); lse is written in natural-log
 // units, [Hq, N].
 //
-// The backward (FlashAttention-2's recurrences: P = exp(S - lse), dV = P^T dO, dP = dO V^T,
+// The backward (P = exp(S - lse), dV = P^T dO, dP = dO V^T,
 // dS = P (dP - rowsum(dO O)), dQ = scale dS K, dK = scale dS^T Q) runs as
 //   attn_bwd_dot    Dd[h][t] = sum_d dO O (fp32);
 //   attn_bwd_dq     per (sequence, query head, 128-row query tile): the forward's loop with
@@ -41,6 +41,11 @@
 // partials of their own (attn_bwd_far_kernel adds them in order: deterministic), so that no item's
 // chain is much longer than a window.
 // Operands are fp16 or, in a window, bf16 (the element type E).
+// A window's times (MI355X, 12 / 2 heads): [8192] in bf16, window 2047, 128 sinks, forward 111 us (95 GFLOP
+// of visible pairs, 860 TF/s); [4096, 3001, 2222, 1531], window 1000, 4 sinks, forward 79 us (690 TF/s),
+// backward 317 (430 TF/s; the causal kernels on whole rows: 770 and 550); 16 rows of 128..512, window 256,
+// 18 and 77 us. Bound as the causal kernels are (below); a window adds its border: a 128-row tile's
+// list of keys, and a key tile's of rows, is window + 127 long, of which half a tile at either end is masked.
 #include "mfma_tile.h"
 
 #include <algorithm>
@@ -681,6 +686,9 @@ __device__ __forceinline__ void rope_back4(float (&x)[4], float (&y)[4], const f
 
 // Dd[h][t] = sum_d dO[t][h][d] * O[t][h][d] and lse2[h][t] = lse[h][t] log2 e (the exponent offset
 // both backward bodies subtract): 16 lanes per (token, head), 8 columns each.
+// Dd from the rounded output, the only one that is kept: beside the rounding of dS for its products, 2^-11
+// relative in fp16, its error is small (relative L2 of dq and dk against 64 bits, one row of 200 in a window
+// of 64: 2.1e-4 with fp32 throughout, 2.95e-4 with dS rounded, 3.1e-4 with both).
 template <class E>
 __global__ __launch_bounds__(256) void attn_bwd_dot_kernel(BwdArgs a) {
   const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;  // t * Hq + h

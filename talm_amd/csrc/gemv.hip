@@ -347,8 +347,8 @@ __global__ __launch_bounds__(64 * LutRoom<kX>::kWaves) void nf4_gemv_lut_kernel(
         for (int q = 0; q < 4; ++q) {  // byte q of the word to bits 8..15, the copy below it
           const uint32_t at = __builtin_amdgcn_perm(word, copy, 0x0c0c0400u + (static_cast<uint32_t>(q) << 8));
           const float2 f = *reinterpret_cast<const float2*>(smem + at);
-          h[q] = __builtin_bit_cast(uint32_t, __builtin_convertvector(
-                                                  (nf4_float2_t){mul_f32(f.x, scale), mul_f32(f.y, scale)}, nf4_half2_t));
+          const nf4_float2_t wq = {mul_f32(f.x, scale), mul_f32(f.y, scale)};
+          h[q] = __builtin_bit_cast(uint32_t, __builtin_convertvector(wq, nf4_half2_t));
         }
         return __builtin_bit_cast(half8_t, make_uint4(h[0], h[1], h[2], h[3]));
       };
@@ -363,7 +363,8 @@ __global__ __launch_bounds__(64 * LutRoom<kX>::kWaves) void nf4_gemv_lut_kernel(
             ln.stage_half(slice, lane, raw[b] + 4 * p, x[0]);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[j], __builtin_bit_cast(half8_t, x[0][j]), acc[b], 0, 0, 0);
+              acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wf[j], __builtin_bit_cast(half8_t, x[0][j]), acc[b], 0,
+                                                              0, 0);
           }
         }
       } else {
@@ -421,8 +422,8 @@ void launch_gemv(GemvArgs a, bool lut, hipStream_t s) {
   const bool one = a.units <= kGemvMaxWaves;
   if (!lut) {
     const int turns = (a.units + kGemvMaxWaves - 1) / kGemvMaxWaves, waves = (a.units + turns - 1) / turns;
-    hipLaunchKernelGGL((nf4_gemv_rows_kernel<P, TB>), dim3(static_cast<unsigned>((a.rows + R - 1) / R)), dim3(64 * waves),
-                       0, s, a);
+    hipLaunchKernelGGL((nf4_gemv_rows_kernel<P, TB>), dim3(static_cast<unsigned>((a.rows + R - 1) / R)),
+                       dim3(64 * waves), 0, s, a);
     return;
   }
   if constexpr (P < 4)
