@@ -942,51 +942,71 @@ Tensor byte_workspace(int64_t bytes, const Tensor& like, const char* what) {
   return at::empty({bytes}, like.options().dtype(at::kByte));
 }
 
-// [1, H, N, D] -> an [N, H, D] view that the window kernels read (a copy only when it must be).
+// The nodes hand the C entries their operands' pointers and strides without views of them: a view costs the host
+// about as much as an allocation, and these calls are short.
+
+// Whether the window kernels read rows of these token, head and column strides where they lie.
+bool window_reads(const Tensor& t, int64_t tok, int64_t head, int64_t col) {
+  return col == 1 && tok % 8 == 0 && head % 8 == 0 && tok < (int64_t{1} << 23) &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+// A [1, H, N, D] operand, or a copy of its rows where it must be.
 Tensor head_rows(const Tensor& t) {
-  Tensor r = t.squeeze(0).transpose(0, 1);
-  if (r.stride(2) != 1 || r.stride(0) % 8 || r.stride(1) % 8 || reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 ||
-      r.stride(0) >= (int64_t{1} << 23))
-    r = r.clone(at::MemoryFormat::Contiguous);
-  return r;
+  if (window_reads(t, t.stride(2), t.stride(1), t.stride(3))) return t;
+  return t.transpose(1, 2).clone(at::MemoryFormat::Contiguous).transpose(1, 2);
 }
 
 struct WindowAttention : torch::autograd::Function<WindowAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& query, const Tensor& key, const Tensor& value,
                         const Tensor& cu, int64_t max_len, double scale, int64_t window, int64_t sinks) {
     const Tensor q = head_rows(query), k = head_rows(key), v = head_rows(value);
-    const Tensor out = at::empty(q.sizes(), q.options());
-    const Tensor lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
-    attn_window_fwd(q, k, v, cu, max_len, scale, window, sinks, out, lse);
+    const int64_t hq = q.size(1), n = q.size(2);
+    const Tensor out = at::empty({1, n, hq, 128}, q.options());
+    const Tensor lse = at::empty({hq, n}, q.options().dtype(at::kFloat));
+    const c10::DeviceGuard guard(q.device());
+    check(talm_attn_window_fwd(as<uint16_t>(q), q.stride(2), q.stride(1), as<uint16_t>(k), k.stride(2), k.stride(1),
+                               as<uint16_t>(v), v.stride(2), v.stride(1), as<int32_t>(cu),
+                               int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_len, "max_len"), n,
+                               int32_arg(hq, "heads"), int32_arg(k.size(1), "heads"), 128, static_cast<float>(scale),
+                               int32_arg(window, "window"), int32_arg(sinks, "sinks"), window_dtype(q),
+                               as<uint16_t>(out), hq * 128, 128, as<float>(lse), stream_of(q)),
+          "attn_window_fwd");
     ctx->save_for_backward({q, k, v, out, lse, cu});
-    ctx->saved_data["max_len"] = max_len;
+    ctx->saved_data["args"] = std::vector<int64_t>{max_len, window, sinks};
     ctx->saved_data["scale"] = scale;
-    ctx->saved_data["window"] = window;
-    ctx->saved_data["sinks"] = sinks;
-    return out.unsqueeze(0);
+    return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4], &cu = saved[5];
-    const int64_t max_len = ctx->saved_data["max_len"].toInt(), window = ctx->saved_data["window"].toInt(),
-                  sinks = ctx->saved_data["sinks"].toInt();
+    const std::vector<int64_t> args = ctx->saved_data["args"].toIntVector();
     variable_list in(8);
     {
       at::AutoGradMode off(false);
       const c10::DeviceGuard guard(q.device());
-      const Tensor g = head_rows(grads[0].transpose(1, 2));
-      const Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()),
-                   dv = at::empty(v.sizes(), v.options());
+      const int64_t hq = q.size(1), hkv = k.size(1), n = q.size(2);
+      const int32_t n_seqs = int32_arg(cu.numel() - 1, "sequences"), longest = int32_arg(args[0], "max_len"),
+                    window = int32_arg(args[1], "window"), sinks = int32_arg(args[2], "sinks");
+      Tensor g = grads[0];
+      if (!window_reads(g, g.stride(1), g.stride(2), g.stride(3))) g = g.clone(at::MemoryFormat::Contiguous);
+      // [1, H, N, 128] of [N, H, 128] rows
+      auto rows = [&](int64_t heads) {
+        return at::empty_strided({1, heads, n, 128}, {n * heads * 128, 128, heads * 128, 1}, q.options());
+      };
+      const Tensor dq = in[0] = rows(hq), dk = in[1] = rows(hkv), dv = in[2] = rows(hkv);
       const Tensor ws = byte_workspace(
-          talm_attn_window_bwd_workspace(q.size(0), int32_arg(q.size(1), "heads"), int32_arg(k.size(1), "heads"),
-                                         int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_len, "max_len"),
-                                         int32_arg(window, "window"), int32_arg(sinks, "sinks")),
+          talm_attn_window_bwd_workspace(n, int32_arg(hq, "heads"), int32_arg(hkv, "heads"), n_seqs, longest, window,
+                                         sinks),
           q, "window_attention");
-      attn_window_bwd(q, k, v, out, g, lse, cu, max_len, ctx->saved_data["scale"].toDouble(), window, sinks,
-                      std::nullopt, std::nullopt, dq, dk, dv, ws);
-      in[0] = dq.transpose(0, 1).unsqueeze(0);
-      in[1] = dk.transpose(0, 1).unsqueeze(0);
-      in[2] = dv.transpose(0, 1).unsqueeze(0);
+      check(talm_attn_window_bwd(
+                as<uint16_t>(q), q.stride(2), q.stride(1), as<uint16_t>(k), k.stride(2), k.stride(1), as<uint16_t>(v),
+                v.stride(2), v.stride(1), as<uint16_t>(out), hq * 128, 128, as<uint16_t>(g), g.stride(1), g.stride(2),
+                as<float>(lse), as<int32_t>(cu), n_seqs, longest, n, static_cast<int32_t>(hq),
+                static_cast<int32_t>(hkv), 128, static_cast<float>(ctx->saved_data["scale"].toDouble()), window, sinks,
+                window_dtype(q), nullptr, nullptr, 0, as<uint16_t>(dq), hq * 128, 128, as<uint16_t>(dk), hkv * 128,
+                128, as<uint16_t>(dv), hkv * 128, 128, ws.data_ptr(), ws.numel(), stream_of(q)),
+            "attn_window_bwd");
     }
     return once(std::move(in));
   }
@@ -1028,10 +1048,19 @@ void drop_args(const Tensor& x, double p, const OptTensor& key, int64_t site) {
 Tensor dropped(const Tensor& x, double p, const OptTensor& key, int64_t site) {
   const Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
   if (x.numel() == 0) return y;
-  const int64_t cols = x.dim() ? x.size(-1) : 1;
-  Tensor x2 = x.reshape({-1, cols});
-  if ((cols > 1 && x2.stride(1) != 1) || (x2.size(0) > 1 && x2.stride(0) < cols)) x2 = x2.contiguous();
-  dropout(x2, p, key, site, y.view({-1, cols}));
+  const int64_t cols = x.dim() ? x.size(-1) : 1, rows = x.numel() / cols;
+  Tensor x2 = x;
+  int64_t ldx = rows <= 1 ? (cols + 7) / 8 * 8 : cols, ldy = ldx;
+  if (!x.is_contiguous()) {
+    x2 = x.reshape({-1, cols});
+    if ((cols > 1 && x2.stride(1) != 1) || (x2.size(0) > 1 && x2.stride(0) < cols)) x2 = x2.contiguous();
+    ldx = row_stride(x2);
+  }
+  const int32_t dtype = x.scalar_type() == at::kBFloat16 ? TALM_BF16 : dtype_code(x.scalar_type());
+  const c10::DeviceGuard guard(x.device());
+  check(talm_dropout(ptr(x2), ldx, rows, cols, dtype, static_cast<float>(p), drop_key(key, x), drop_site(site), ptr(y),
+                     ldy, stream_of(x)),
+        "dropout");
   return y;
 }
 
@@ -1062,14 +1091,22 @@ Tensor counter_dropout(const Tensor& x, double p, const OptTensor& key, int64_t 
   return CounterDropout::apply(x, p, key, site);
 }
 
-// [..., C] as [N, C] rows that the adapters' kernels read: unit column stride, 16-byte aligned rows.
-Tensor aligned_rows(const Tensor& t) {
-  Tensor r = t.reshape({t.size(-1) ? t.numel() / t.size(-1) : 0, t.size(-1)});
-  if ((r.size(1) > 1 && r.stride(1) != 1) || (r.size(0) > 1 && (r.stride(0) % 8 || r.stride(0) < r.size(1))) ||
-      reinterpret_cast<uintptr_t>(r.data_ptr()) % 16)
-    r = r.clone(at::MemoryFormat::Contiguous);
-  return r;
-}
+// [..., C] as N rows of C columns that the adapters' kernels read: unit column stride, 16-byte aligned rows.
+struct AlignedRows {
+  Tensor t;
+  int64_t n, ld;
+  explicit AlignedRows(const Tensor& x) : t(x), n(0), ld(x.size(-1)) {
+    const int64_t size = ld;
+    n = size ? x.numel() / size : 0;
+    const bool aligned = reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+    if (x.is_contiguous() && aligned && size % 8 == 0) return;
+    t = x.reshape({n, size});
+    if ((size > 1 && t.stride(1) != 1) || (n > 1 && (t.stride(0) % 8 || t.stride(0) < size)) ||
+        reinterpret_cast<uintptr_t>(t.data_ptr()) % 16)
+      t = t.clone(at::MemoryFormat::Contiguous);
+    ld = row_stride(t);
+  }
+};
 
 Tensor adapter_half(const Tensor& w) {
   const Tensor h = w.to(at::kHalf);
@@ -1083,53 +1120,62 @@ struct AdapterBranch : torch::autograd::Function<AdapterBranch> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& lora_a, const Tensor& lora_b,
                         const Tensor& a_half, const Tensor& b_half, const OptTensor& key, double scaling, double p,
                         int64_t site) {
-    const Tensor x2 = aligned_rows(x), a = adapter_half(a_half), b = adapter_half(b_half);
-    const int64_t n = x2.size(0), size = x2.size(1), out = b.size(0);
-    const Tensor t = at::empty({n, 16}, x2.options()), y = at::empty({n, out}, x2.options());
-    const Tensor ws = byte_workspace(talm_lora_branch_fwd_workspace(n, size), x2, "adapter_branch");
-    const c10::DeviceGuard guard(x2.device());
-    check(talm_lora_branch_fwd(as<uint16_t>(x2), row_stride(x2), n, size, out, as<uint16_t>(a), as<uint16_t>(b),
-                               static_cast<float>(p), drop_key(key, x2), drop_site(site),
-                               static_cast<float>(scaling), as<uint16_t>(t), as<uint16_t>(y), ws.data_ptr(),
-                               ws.numel(), stream_of(x2)),
-          "lora_branch_fwd");
-    ctx->save_for_backward({x2, a, b, t, key.has_value() ? *key : Tensor()});
-    ctx->saved_data["scaling"] = scaling;
-    ctx->saved_data["p"] = p;
-    ctx->saved_data["site"] = site;
-    ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->saved_data["type"] = lora_a.scalar_type();
+    const AlignedRows rows(x);
+    const Tensor a = adapter_half(a_half), b = adapter_half(b_half);
+    const int64_t n = rows.n, size = x.size(-1), out = b.size(0);
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = out;
-    return y.view(shape);
+    const Tensor t = at::empty({n, 16}, x.options()), y = at::empty(shape, x.options());
+    const Tensor ws = byte_workspace(talm_lora_branch_fwd_workspace(n, size), x, "adapter_branch");
+    const c10::DeviceGuard guard(x.device());
+    check(talm_lora_branch_fwd(as<uint16_t>(rows.t), rows.ld, n, size, out, as<uint16_t>(a), as<uint16_t>(b),
+                               static_cast<float>(p), drop_key(key, x), drop_site(site), static_cast<float>(scaling),
+                               as<uint16_t>(t), as<uint16_t>(y), ws.data_ptr(), ws.numel(), stream_of(x)),
+          "lora_branch_fwd");
+    ctx->save_for_backward({rows.t, a, b, t, key.has_value() ? *key : Tensor()});
+    shape.back() = size;
+    ctx->saved_data["shape"] = std::move(shape);
+    ctx->saved_data["rates"] = std::vector<double>{scaling, p};
+    ctx->saved_data["site"] = site;
+    ctx->saved_data["type"] = lora_a.scalar_type();
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &a = saved[1], &b = saved[2], &t = saved[3];
+    const Tensor &a = saved[1], &b = saved[2], &t = saved[3];
     const OptTensor key = saved[4].defined() ? OptTensor(saved[4]) : OptTensor();
-    const double scaling = ctx->saved_data["scaling"].toDouble(), p = ctx->saved_data["p"].toDouble();
-    const int64_t site = ctx->saved_data["site"].toInt();
+    const std::vector<double> rates = ctx->saved_data["rates"].toDoubleVector();
+    const float scaling = static_cast<float>(rates[0]), p = static_cast<float>(rates[1]);
     variable_list in(9);
     {
       at::AutoGradMode off(false);
-      const Tensor dy = aligned_rows(grads[0].to(at::kHalf));
-      const int64_t n = x.size(0), size = x.size(1), out = b.size(0);
-      // u = scaling dy B (lora_down writes the unscaled product too), and the weight gradients' partials
-      const Tensor u2 = at::empty({2, n, 16}, t.options()), u_raw = u2.select(0, 0), u = u2.select(0, 1);
-      lora_down(dy, b, std::nullopt, out, 0, 0, 0, 1, scaling, 0.0, u_raw, u);
-      OptTensor dx, da, db;
-      if (ctx->needs_input_grad(0)) {
-        dx = at::empty({n, size}, x.options());
-        in[0] = dx->view(ctx->saved_data["shape"].toIntVector());
-      }
+      const c10::DeviceGuard guard(t.device());
+      const AlignedRows x(saved[0]), dy(grads[0]);
+      const int64_t n = x.n, size = saved[0].size(-1), out = b.size(0), up = (n * 32 + 255) / 256 * 256;
+      Tensor dx, da, db;
+      if (ctx->needs_input_grad(0))
+        dx = in[0] = at::empty(ctx->saved_data["shape"].toIntVector(), t.options());
+      const at::ScalarType type = ctx->saved_data["type"].toScalarType();
       if (ctx->needs_input_grad(1) || ctx->needs_input_grad(2)) {
-        const auto options = x.options().dtype(ctx->saved_data["type"].toScalarType());
+        const auto options = t.options().dtype(type);
         da = in[1] = at::empty({16, size}, options);
         db = in[2] = at::empty({out, 16}, options);
       }
-      lora_bwd_drop(x, dy, u, t, p, key, site, 0, 0, out, scaling, da, db, 0, 0, 0.0, std::nullopt, std::nullopt, a,
-                    std::nullopt, std::nullopt, dx,
-                    byte_workspace(talm_lora_bwd_drop_workspace(n, size, 1, out, 0), x, "adapter_branch"));
+      // u = scaling dy B behind the unscaled product, which lora_down writes too, and the partials
+      const int64_t need = talm_lora_bwd_drop_workspace(n, size, 1, out, 0);
+      const Tensor scratch = byte_workspace(need < 0 ? need : need + 2 * up, t, "adapter_branch");
+      uint8_t* base = as<uint8_t>(scratch);
+      uint16_t *raw = reinterpret_cast<uint16_t*>(base), *u = reinterpret_cast<uint16_t*>(base + up);
+      check(talm_lora_down(as<uint16_t>(dy.t), dy.ld, n, out, 0, 0, 0, as<uint16_t>(b), nullptr, 1, 1, scaling, 0.f, raw,
+                           u, 16, stream_of(t)),
+            "lora_down");
+      auto grad = [](const Tensor& g) { return g.defined() ? g.data_ptr() : nullptr; };
+      check(talm_lora_bwd_drop(as<uint16_t>(x.t), x.ld, as<uint16_t>(dy.t), dy.ld, u, 16, as<uint16_t>(t), 16, n, size,
+                               1, p, drop_key(key, t), drop_site(ctx->saved_data["site"].toInt()), 0,
+                               dtype_code(type), 0, out, scaling, grad(da), grad(db), 0, 0, 0.f, nullptr, nullptr,
+                               as<uint16_t>(a), nullptr, nullptr, 0, static_cast<uint16_t*>(grad(dx)), size,
+                               base + 2 * up, need, stream_of(t)),
+            "lora_bwd_drop");
     }
     return once(std::move(in));
   }
