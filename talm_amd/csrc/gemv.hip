@@ -31,6 +31,8 @@
 // [152064, 1536] 28 and 42 (4.3 TB/s, 2.9). What bounds one token: a launch (1.2 us), one memory
 // round trip with the whole of W in flight, the lookups behind it (LDS and VALU 1.4 us each) and the
 // join, one after the other; many tokens: x's way through L2 and LDS, and the lookups.
+// Not kept: three tiles' weights ahead in registers, the body three times (1 token: [17920, 1536] 8.4 us, and 7.6
+// for 6.3 at [2048, 8192], whose workgroups have one tile): a launch finds its code cold, and longer code costs more.
 #include "mfma_tile.h"
 #include "nf4_code.h"
 
