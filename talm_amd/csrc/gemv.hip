@@ -31,8 +31,8 @@
 // [152064, 1536] 28 and 42 (4.3 TB/s, 2.9). What bounds one token: a launch (1.2 us), one memory
 // round trip with the whole of W in flight, the lookups behind it (LDS and VALU 1.4 us each) and the
 // join, one after the other; many tokens: x's way through L2 and LDS, and the lookups.
-// Not kept: three tiles' weights ahead in registers, the body three times (1 token: [17920, 1536] 8.4 us, and 7.6
-// for 6.3 at [2048, 8192], whose workgroups have one tile): a launch finds its code cold, and longer code costs more.
+// Not kept: three tiles' weights ahead in registers (1 token, [17920, 1536] 8.4 us, [2048, 8192] 7.6 for 6.3); the
+// rows kernel's lookups as a loop (3.3 us for 3.15).
 #include "mfma_tile.h"
 #include "nf4_code.h"
 
@@ -418,21 +418,31 @@ void launch_lut(GemvArgs a, hipStream_t s) {
 }
 
 template <int P, int TB>
-void launch_gemv(GemvArgs a, bool lut, hipStream_t s) {
+void launch_rows(GemvArgs a, hipStream_t s) {
   constexpr int R = 16 / P;
   a.units = (a.cols + 256 * P - 1) / (256 * P);
+  const int turns = (a.units + kGemvMaxWaves - 1) / kGemvMaxWaves, waves = (a.units + turns - 1) / turns;
+  hipLaunchKernelGGL((nf4_gemv_rows_kernel<P, TB>), dim3(static_cast<unsigned>((a.rows + R - 1) / R)),
+                     dim3(64 * waves), 0, s, a);
+}
+
+// The way of x: through LDS from 9 tokens on (which two parts hold as two blocks), from 6 on where a wavefront
+// has several units (figures above).
+template <int P, int TB>
+void launch_lut_form(GemvArgs a, hipStream_t s) {
+  a.units = (a.cols + 256 * P - 1) / (256 * P);
   const bool one = a.units <= kGemvMaxWaves;
-  if (!lut) {
-    const int turns = (a.units + kGemvMaxWaves - 1) / kGemvMaxWaves, waves = (a.units + turns - 1) / turns;
-    hipLaunchKernelGGL((nf4_gemv_rows_kernel<P, TB>), dim3(static_cast<unsigned>((a.rows + R - 1) / R)),
-                       dim3(64 * waves), 0, s, a);
-    return;
-  }
-  if constexpr (P < 4)
-    if (a.M > (one ? 8 : 5)) return one ? launch_lut<P, TB, kOneStaged>(a, s) : launch_lut<P, TB, kEachStaged>(a, s);
-  if constexpr (TB == 1 && P < 4) {
-    if (one) launch_lut<P, TB, kOneUnit>(a, s);
-    else launch_lut<P, TB, kEachUnit>(a, s);
+  if constexpr (TB == 2) {
+    if (one) launch_lut<P, TB, kOneStaged>(a, s);
+    else launch_lut<P, TB, kEachStaged>(a, s);
+  } else if (one) {
+    if constexpr (P == 1)
+      if (a.M > 8) return launch_lut<P, TB, kOneStaged>(a, s);
+    launch_lut<P, TB, kOneUnit>(a, s);
+  } else if (a.M > 5) {
+    launch_lut<P, TB, kEachStaged>(a, s);
+  } else {
+    launch_lut<P, TB, kEachUnit>(a, s);
   }
 }
 
@@ -500,10 +510,19 @@ TALM_API int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, con
     }
   }
   const hipStream_t s = as_stream(stream);
-  if (n_tokens > 16) launch_gemv<1, 2>(a, lut, s);
-  else if (best == 2 && n_tokens > 8) launch_gemv<2, 2>(a, lut, s);
-  else if (best == 1) launch_gemv<1, 1>(a, lut, s);
-  else if (best == 2) launch_gemv<2, 1>(a, lut, s);
-  else launch_gemv<4, 1>(a, false, s);
+  if (lut) {
+    if (n_tokens > 16) launch_lut_form<1, 2>(a, s);
+    else if (best == 1) launch_lut_form<1, 1>(a, s);
+    else if (n_tokens > 8) launch_lut_form<2, 2>(a, s);
+    else launch_lut_form<2, 1>(a, s);
+  } else if (n_tokens > 16) {
+    launch_rows<1, 2>(a, s);
+  } else if (best == 1) {
+    launch_rows<1, 1>(a, s);
+  } else if (best == 2) {
+    launch_rows<2, 1>(a, s);
+  } else {
+    launch_rows<4, 1>(a, s);
+  }
   return check_launch("nf4_gemv");
 }
