@@ -63,6 +63,30 @@ def test_dropped_values_are_zero_whatever_they_were_and_shapes_stay():
     assert dropout(one, 0.0) == 1 and dropout(one, 0.0).shape == ()
 
 
+@pytest.mark.parametrize("rows", [2 ** 21 + 3, 2 ** 22 + 3])
+def test_dropout_of_more_blocks_than_a_launch_holds(rows):
+    """Blocks past 2^30 (further launches) and past 2^31 (a 64-bit division), in place."""
+    from talm_amd import _ops  # noqa: F401 - registers torch.ops.talm.*
+
+    cols, p = 4096, 0.25
+    if torch.cuda.mem_get_info()[0] < 2 * rows * cols + (4 << 30):
+        pytest.skip("not enough free device memory")
+    print(f"[case] dropout {rows} x {cols}", flush=True)
+    key = _key(77, 88)
+    x = torch.ones(rows, cols, dtype=torch.float16, device="cuda")
+    torch.ops.talm.dropout(x, p, key, 3, x)
+    f = torch.tensor(float(philox.factor(p))).half()
+    for r in (0, 1, 2 ** 21 - 1, 2 ** 21, 2 ** 21 + 2, rows - 4, rows - 1):
+        block = np.arange(cols // 8, dtype=np.uint64) + np.uint64(r * (cols // 8))
+        words = philox.philox4x32((block, block >> np.uint64(32), np.full_like(block, 3), np.full_like(block, 88)),
+                                  (77, 0))
+        bits = np.stack(words, 1).astype("<u4").view("<u2").reshape(-1)
+        keep = torch.from_numpy(bits.astype(np.int64) >= philox.threshold(p))
+        assert torch.equal(x[r].cpu(), torch.where(keep, f, torch.zeros((), dtype=torch.float16)))
+    del x
+    torch.cuda.empty_cache()
+
+
 def test_strided_rows_and_in_place():
     from talm_amd import _ops  # noqa: F401
     from talm_amd.dropout import dropout
@@ -166,6 +190,32 @@ def test_adapter_branch_matches_its_formula(n, size, out, p, dtype):
     assert grads[1].dtype == grads[2].dtype == dtype
     m = _keep(key, n, size, p, 4).double() / (1 - philox.threshold(p) / 65536)
     _compare((y, *grads), *_expect(x, a, b, dy, m, 2.0, dtype == torch.float16))
+
+
+def test_adapter_branch_past_32_bit_offsets():
+    """x of more than 2^31 elements; only the last rows have a gradient, so that theirs are the weights' too."""
+    from talm_amd.lora import adapter_branch
+
+    n, size, out, tail, p = 300000, 8960, 32, 64, 0.25
+    if torch.cuda.mem_get_info()[0] < 32 << 30:
+        pytest.skip("not enough free device memory")
+    print(f"[case] adapter branch {n} x {size}", flush=True)
+    key = _key(41, 42)
+    _, a, b, _ = _branch(1, size, out, p, torch.float32, 3, key)
+    x = torch.empty(n, size, dtype=torch.float16, device="cuda").normal_().requires_grad_()
+    dy = torch.zeros(n, out, dtype=torch.float16, device="cuda")
+    dy[-tail:] = torch.randn(tail, out, device="cuda").half()
+    y = adapter_branch(x, a, b, 2.0, p, key, 4)
+    dx, da, db = torch.autograd.grad(y, (x, a, b), dy)
+    block = np.arange((n - tail) * size // 8, n * size // 8, dtype=np.uint64)
+    words = philox.philox4x32((block, block >> np.uint64(32), np.full_like(block, 4), np.full_like(block, 42)), (41, 0))
+    bits = np.stack(words, 1).astype("<u4").view("<u2").reshape(tail, size)
+    m = torch.from_numpy(bits.astype(np.int64) >= philox.threshold(p)).cuda().double() * float(philox.factor(p))
+    want, tols = _expect(x[-tail:], a, b, dy[-tail:], m, 2.0, False)
+    assert not dx[:-tail].any()
+    _compare((y[-tail:].detach(), dx[-tail:], da, db), want, tols)
+    del x, dx, y
+    torch.cuda.empty_cache()
 
 
 def test_adapter_branch_without_rows_and_with_batch_dimensions():

@@ -90,6 +90,34 @@ def test_gemv_over_tiles(rows, cols):
         _check(group, torch.randn(tokens, cols, generator=g, device="cuda").half(), 6, 7)
 
 
+def test_gemv_past_32_bit_offsets():
+    """W of more than 2^31 weights: its last rows against a call on their buffers alone. Both round the same fp32
+    sums, taken in another order: (cols / 32 + 96) 2^-24 of the magnitudes summed (at most 0.03 |x|) each."""
+    from talm_amd import _ops  # noqa: F401 - registers torch.ops.talm.*
+
+    rows, cols, tail = 1500000, 1536, 128
+    print(f"[case] gemv W {rows} x {cols}", flush=True)
+    n, at = rows * cols, (rows - tail) * cols
+    assert n > 2 ** 31 and at % (64 * 256) == 0
+    g = torch.Generator("cuda").manual_seed(4)
+    packed = torch.randint(0, 256, (n // 2,), dtype=torch.uint8, device="cuda", generator=g)
+    absmax8 = torch.randint(0, 256, (n // 64,), dtype=torch.uint8, device="cuda", generator=g)
+    code = torch.linspace(-1, 1, 256, device="cuda")
+    absmax2 = torch.rand(n // 16384, device="cuda", generator=g) * 0.01
+    offset2 = torch.rand(n // 16384, device="cuda", generator=g) * 0.01 + 0.01
+    for tokens in (1, 12, 32):
+        x = torch.randn(tokens, cols, device="cuda", generator=g).half()
+        out = torch.empty(tokens, rows, dtype=torch.float16, device="cuda")
+        last = torch.empty(tokens, tail, dtype=torch.float16, device="cuda")
+        torch.ops.talm.nf4_gemv(x, packed, absmax8, code, absmax2, offset2, rows, cols, 64, 256, None, out)
+        torch.ops.talm.nf4_gemv(x, packed[at // 2:], absmax8[at // 64:], code, absmax2[at // 16384:],
+                                offset2[at // 16384:], tail, cols, 64, 256, None, last)
+        err = (out[:, -tail:].double() - last.double()).abs()
+        mag = 0.03 * x.double().abs().sum(1, keepdim=True)
+        tol = 2 * (2.0 ** -11 * last.double().abs() + (cols / 32 + 96) * 2.0 ** -24 * mag + 2.0 ** -25)
+        assert last.abs().max() > 0.1 and (err <= tol).all()
+
+
 def test_gemv_keeps_nan_and_infinity_to_their_token():
     """x's rows do not mix, whichever way they are loaded."""
     for cols in (512, 4096, 8960):

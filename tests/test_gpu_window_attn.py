@@ -149,6 +149,27 @@ def test_several_heads_per_item(lengths, window, sinks, hq, hkv, half):
     _check(lengths, window, sinks, hq, hkv, half, seed=7, device="cuda")
 
 
+def test_rows_past_32_bit_offsets():
+    """Operands of more than 2^31 elements: the last sequences' results and gradients."""
+    lengths, tail, hq, hkv = [4096] * 299 + [700, 77], 777, 12, 2
+    n = sum(lengths)
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("not enough free device memory")
+    print(f"[case] window, {n} rows of {(hq + 2 * hkv) * D} columns", flush=True)
+    g = torch.Generator("cuda").manual_seed(8)
+    qkv = torch.empty(n, (hq + 2 * hkv) * D, dtype=torch.float16, device="cuda").normal_(generator=g)
+    assert qkv.numel() > 2 ** 31
+    q, k, v = (t.view(n, -1, D) for t in qkv.split([hq * D, hkv * D, hkv * D], 1))
+    dout = torch.empty(n, hq, D, dtype=torch.float16, device="cuda").normal_(generator=g)
+    got = [t[-tail:].clone() for t in _call(q, k, v, _cu(lengths), max(lengths), 100, 4, dout)]
+    vals, tols = _reference(q[-tail:], k[-tail:], v[-tail:], [700, 77], D ** -0.5, 100, 4, dout[-tail:],
+                            torch.float16, "cuda")
+    for name, a, b, tol in zip(("out", "dq", "dk", "dv"), got, vals, tols):
+        assert ((a.double().cpu() - b).abs() <= tol).all(), name
+    del qkv, q, k, v, dout
+    torch.cuda.empty_cache()
+
+
 def test_many_sequences_one_workgroup_per_item():
     """More sequences than the queue takes."""
     _check([30 + i % 50 for i in range(70)], 24, 2, 2, 1, seed=6)
