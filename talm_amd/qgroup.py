@@ -49,6 +49,7 @@ import torch
 
 from . import _ops, few_tokens  # _ops registers torch.ops.talm.*
 from .engaged import FELL_BACK, ON, RAN
+from .few_tokens import GEMV_TOKENS  # noqa: F401 - LayerGroup.nf4_gemv's limit
 from .nf4_dequant import dequantize_4bit
 from .state import DISABLED, fallback
 
@@ -67,9 +68,6 @@ T_BLOCKS = ((0, 1, 2), (3,), (4, 5), (6,))
 # where that GEMM is faster than the split-K GEMM on the transposed weights plus their share of
 # the transposed dequantization.
 W4_BLOCKS = ((4, 5),) if os.environ.get("SOLUTION_DISABLE_W4A16") != "1" else ()
-
-# the most rows of x that talm_nf4_gemv takes
-GEMV_TOKENS = 32
 
 
 def launch(packed, absmax8, code, absmax2, offset2, levels, out, n_rows, qblock, qblock2,
@@ -160,7 +158,7 @@ class LayerGroup:
             .expand((seg.stop - seg.start) // span2) for s, seg in zip(states, segments)])
         self.modules = [weakref.ref(m) for m in modules]
         self._bias_spans = {}
-        self._gemv = {}
+        self._gemv, self._gemv_ok = {}, {}
         self._scales = None
         self.t_layout = self._transposed_layout()
         # the reference's count of backward uses (solution/qgroup.py:179, :536): callers written
@@ -320,9 +318,13 @@ class LayerGroup:
     # -- a few tokens' products on the NF4 codes -------------------------------------------------------
     def gemv_ok(self, first, last):
         """Projections first .. last - 1 are one [sum of out, in] matrix talm_nf4_gemv takes."""
-        cols = {seg.shape[1] for seg in self.segments[first:last]}
-        return (self.qblock == 64 and self.qblock2 & (self.qblock2 - 1) == 0 and len(cols) == 1
+        ok = self._gemv_ok.get((first, last))
+        if ok is None:
+            cols = {seg.shape[1] for seg in self.segments[first:last]}
+            ok = self._gemv_ok[(first, last)] = (
+                self.qblock == 64 and self.qblock2 & (self.qblock2 - 1) == 0 and len(cols) == 1
                 and next(iter(cols)) % 64 == 0)
+        return ok
 
     def nf4_gemv(self, x, first, last, out, adapters=None):
         """out [M, sum of out] = x [M, in] W^T + the projections' biases for M <= GEMV_TOKENS rows, W
