@@ -312,7 +312,8 @@ def _mfma_ok(x2, weight, bias, bounds, adapters, halves, rope, head_dim, key=Non
         return False
     for (seg, _scaling, p), (a16, b16) in zip(adapters, halves):
         lo, hi = bounds[seg], bounds[seg + 1]
-        if (p > 0 and key is None) or p != adapters[0][2] or tuple(a16.shape) != (16, size) or tuple(b16.shape) != (hi - lo, 16) \
+        if (p > 0 and key is None) or p != adapters[0][2] \
+                or tuple(a16.shape) != (16, size) or tuple(b16.shape) != (hi - lo, 16) \
                 or not (a16.is_contiguous() and b16.is_contiguous()) \
                 or lo % 128 or (hi % 128 and hi != n_out):
             return False
