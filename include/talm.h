@@ -629,10 +629,11 @@ int talm_attn_window_fwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_stri
 
 /*
  * Its backward: talm_attn_bwd (cos and sin NULL) or talm_attn_bwd_rope in the window. Rows behind
- * the last sequence get zero gradients. `workspace` (256-byte aligned) holds
- * talm_attn_window_bwd_workspace(...) bytes (-1 for arguments the call would reject): the causal
- * backward's, and partials of the sinks' gradients from the rows past their window (at most 64 MiB,
- * or one set if that is more). Deterministic. No counterpart in the reference.
+ * the last sequence get zero gradients, all rows where no sequence has a token (n_seqs or
+ * max_seqlen 0). `workspace` (256-byte aligned) holds talm_attn_window_bwd_workspace(...) bytes (-1
+ * for arguments the call would reject): the causal backward's, and partials of the sinks'
+ * gradients from the rows past their window (at most 64 MiB, or one set if that is more).
+ * Deterministic. No counterpart in the reference.
  */
 int64_t talm_attn_window_bwd_workspace(int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
                                        int32_t n_seqs, int32_t max_seqlen, int32_t window,

@@ -1481,7 +1481,8 @@ __device__ __forceinline__ void sum_heads4(const BwdArgs& a, int kvh, int64_t t,
   }
 }
 
-// kWin: rows behind the last sequence get zero gradients (dq's too: no query tile holds them).
+// kWin: rows behind the last sequence get zero gradients (dq's too: no query tile holds them), every row
+// where no sequence has a token (n_tiles 0).
 template <class E, bool kRope, bool kWin>
 __global__ __launch_bounds__(256) void attn_bwd_reduce_kernel(BwdArgs a) {
   constexpr int kGroups = kRope ? kD / 8 : kD / 4;  // threads per (token, KV head)
@@ -1499,7 +1500,7 @@ __global__ __launch_bounds__(256) void attn_bwd_reduce_kernel(BwdArgs a) {
   d[0] = 4 * c4;
   if constexpr (kRope) d[C - 1] = 4 * c4 + kD / 2;
   if constexpr (kWin) {
-    if (t >= a.cu[a.n_seqs]) {
+    if (t >= (a.n_tiles ? a.cu[a.n_seqs] : 0)) {
       for (int c = 0; c < C; ++c) {
         *reinterpret_cast<uint2*>(dk + d[c]) = make_uint2(0u, 0u);
         *reinterpret_cast<uint2*>(dv + d[c]) = make_uint2(0u, 0u);
@@ -1761,6 +1762,13 @@ void launch_bwd(const BwdArgs& a, int n_seqs, hipStream_t s) {
   else hipLaunchKernelGGL((attn_bwd_reduce_kernel<E, false, kWin>), grid, dim3(256), 0, s, a);
 }
 
+// kWin: zero gradients for all rows (the words are the same in both types, rotated or not).
+void launch_zero(const BwdArgs& a, hipStream_t s) {
+  const int64_t n = a.n_tokens * a.n_kv_heads * (kD / 4);
+  hipLaunchKernelGGL((attn_bwd_reduce_kernel<F16, false, true>), dim3(static_cast<unsigned>((n + 255) / 256)),
+                     dim3(256), 0, s, a);
+}
+
 int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
                   const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
                   const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
@@ -1809,8 +1817,10 @@ int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
   if (rope && (cs_stride < kD || cs_stride % 4 || cs_stride >= (int64_t{1} << 24)))
     return fail(TALM_EINVAL, "%s: cos / sin row stride %lld (at least %d, a multiple of 4)", what,
                 (long long)cs_stride, kD);
-  if (n_seqs == 0 || max_seqlen == 0 || n_tokens == 0) return ok();
-  if (!q || !k || !v || !out || !dout || !lse || !cu_seqlens || !dq || !dk || !dv || !workspace)
+  // no sequence has a token: in a window every row is one behind the last sequence
+  const bool none = n_seqs == 0 || max_seqlen == 0;
+  if (n_tokens == 0 || (none && !win.window)) return ok();
+  if (!dq || !dk || !dv || (!none && (!q || !k || !v || !out || !dout || !lse || !cu_seqlens || !workspace)))
     return fail(TALM_EINVAL, "%s: null pointer", what);
   if (rope && (!cos || !sin || !aligned(cos, 16) || !aligned(sin, 16)))
     return fail(TALM_EINVAL, "%s: cos and sin both given, 16-byte aligned", what);
@@ -1828,7 +1838,7 @@ int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
   a.lse = lse; a.cu = cu_seqlens;
   a.group = a.kv_parts = n_q_heads / n_kv_heads; a.n_q_heads = n_q_heads; a.n_kv_heads = n_kv_heads;
   a.item_heads = 1;
-  a.n_tiles = (max_seqlen + 32 * W - 1) / (32 * W);
+  a.n_tiles = none ? 0 : (max_seqlen + 32 * W - 1) / (32 * W);
   a.scale = scale; a.scale_log2 = scale * 1.44269504088896341f;
   a.n_tokens = n_tokens;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
@@ -1872,7 +1882,8 @@ int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
     a.queue_wgs = static_cast<unsigned>(std::min<int64_t>(items, device_cus()));
   }
   const hipStream_t s = as_stream(stream);
-  if (!win.window) launch_bwd<F16, false>(a, n_seqs, s);
+  if (none) launch_zero(a, s);
+  else if (!win.window) launch_bwd<F16, false>(a, n_seqs, s);
   else if (win.dtype == TALM_F16) launch_bwd<F16, true>(a, n_seqs, s);
   else launch_bwd<BF16, true>(a, n_seqs, s);
   return check_launch(what);

@@ -359,3 +359,35 @@ def test_in_inference_mode():
         out = window_attention(*(t.transpose(0, 1)[None] for t in (q, k, v)), _cu([100]), 100, D ** -0.5, 20, 1)
         got = out[0], dropout(x, 0.3, key), adapter_branch(x, a, b, 1.0, 0.3, key)
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def _poison(like):
+    """Leaves NaN in the memory that the next tensors of these sizes get."""
+    held = [torch.full((t.numel(),), math.nan, dtype=t.dtype, device="cuda") for t in like for _ in range(4)]
+    del held
+
+
+@pytest.mark.parametrize("half", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lengths", [[], [0], [0, 0, 0]])
+def test_gradients_are_zero_without_a_token_in_a_sequence(lengths, half):
+    """No sequence at all, or none with a token: every row lies behind the last one."""
+    from talm_amd import _ops
+
+    print(f"[case] window without tokens, lengths={lengths} {half}", flush=True)
+    q, k, v, dout = _inputs(70, 4, 2, half, False, 5)
+    cu = _cu(lengths) if lengths else torch.zeros(1, dtype=torch.int32, device="cuda")
+    for longest in (0, 16):
+        _poison((q, k, v))
+        _, *grads = _call(q, k, v, cu, longest, 8, 2, dout)
+        for g, t in zip(grads, (q, k, v)):
+            assert g.shape == t.shape and (g == 0).all()
+        out, lse = torch.zeros_like(q), torch.zeros(4, 70, device="cuda")
+        angles = torch.rand(70, D, device="cuda")
+        for rotated in (False, True):
+            dq, dk, dv = (torch.full_like(t, 5.0) for t in (q, k, v))
+            ws = torch.full((_ops.attn_window_bwd_workspace_bytes(70, 4, 2, len(lengths), longest, 8, 2),), 255,
+                            dtype=torch.uint8, device="cuda")
+            torch.ops.talm.attn_window_bwd(q, k, v, out, dout, lse, cu, longest, 0.1, 8, 2,
+                                           angles.cos() if rotated else None, angles.sin() if rotated else None,
+                                           dq, dk, dv, ws)
+            assert not dq.any() and not dk.any() and not dv.any()
