@@ -245,7 +245,8 @@ __global__ __launch_bounds__(256) void lora_up_kernel(UpArgs a) {
     const bool in = tok < a.n_tokens;
     const float* p = a.part + static_cast<int64_t>(in ? tok : a.n_tokens - 1) * kRank + 8 * hh;
     float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    // every part's loads before their adds: a part past the last is the last one again, adding 0
+    // every part's loads before their adds: a part past the last is the last one again, not added (selects:
+    // a product with 0 would turn an infinity into NaN)
     float4 lo[kDownMaxParts], hi[kDownMaxParts];
 #pragma unroll
     for (int i = 0; i < kDownMaxParts; ++i) {
@@ -255,9 +256,9 @@ __global__ __launch_bounds__(256) void lora_up_kernel(UpArgs a) {
     }
 #pragma unroll
     for (int i = 0; i < kDownMaxParts; ++i) {
-      const float f = i < a.parts ? 1.f : 0.f;
-      s[0] += f * lo[i].x; s[1] += f * lo[i].y; s[2] += f * lo[i].z; s[3] += f * lo[i].w;
-      s[4] += f * hi[i].x; s[5] += f * hi[i].y; s[6] += f * hi[i].z; s[7] += f * hi[i].w;
+      const bool is = i < a.parts;
+      s[0] += is ? lo[i].x : 0.f; s[1] += is ? lo[i].y : 0.f; s[2] += is ? lo[i].z : 0.f; s[3] += is ? lo[i].w : 0.f;
+      s[4] += is ? hi[i].x : 0.f; s[5] += is ? hi[i].y : 0.f; s[6] += is ? hi[i].z : 0.f; s[7] += is ? hi[i].w : 0.f;
     }
     const float f = a.factor;
     const uint4 tf = make_uint4(pack2(f * s[0], f * s[1]), pack2(f * s[2], f * s[3]), pack2(f * s[4], f * s[5]),

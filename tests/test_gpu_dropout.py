@@ -331,3 +331,37 @@ def test_the_gradients_have_no_backward():
             torch.autograd.grad(first.float().sum(), leaf, retain_graph=True)
         with pytest.raises(RuntimeError, match="differentiable once"):
             first.float().sum().backward()
+
+
+@pytest.mark.parametrize("size", [96, 1536, 2048])
+def test_an_infinity_reaches_its_own_token_as_the_formula_has_it(size):
+    """x holds an infinity where A is positive: t and, B positive, y are infinite for that token, whatever the
+    reduction's number of parts, and the others are what they are without it."""
+    from talm_amd import _lib
+
+    n, out = 40, 64
+    half = dict(dtype=torch.float16, device="cuda")
+    g = torch.Generator("cuda").manual_seed(size)
+    x = torch.randn(n, size, generator=g, device="cuda").half()
+    a = (torch.rand(16, size, generator=g, device="cuda") * 0.02 + 0.01).half()
+    b = (torch.rand(out, 16, generator=g, device="cuda") + 0.5).half()
+    lib = _lib.lib()
+
+    def branch(x):
+        t, y = torch.empty(n, 16, **half), torch.empty(n, out, **half)
+        ws = torch.empty(lib.talm_lora_branch_fwd_workspace(n, size), dtype=torch.uint8, device="cuda")
+        status = lib.talm_lora_branch_fwd(x.data_ptr(), size, n, size, out, a.data_ptr(), b.data_ptr(), 0.0, None, 0,
+                                          2.0, t.data_ptr(), y.data_ptr(), ws.data_ptr(), ws.numel(),
+                                          torch.cuda.current_stream().cuda_stream)
+        assert status == _lib.TALM_OK
+        torch.cuda.synchronize()
+        return t, y
+    want = branch(x)
+    others = [i for i in range(n) if i != 7]
+    for column in (0, size // 2, size - 1):
+        for value in (float("inf"), -float("inf")):
+            print(f"[case] branch of {size} columns, {value} at {column}", flush=True)
+            bad = x.clone()
+            bad[7, column] = value
+            for got, without in zip(branch(bad), want):
+                assert (got[7] == value).all() and torch.equal(got[others], without[others])
