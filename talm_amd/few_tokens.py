@@ -96,10 +96,15 @@ def _linear(x, group, first, last, adapters, halves):
     return out.view(*x.shape[:-1], out.shape[1])
 
 
+def mlp_takes(x, group, gate, down):
+    """Whether `mlp` takes fp16 x."""
+    return takes(x, group, gate, down) and group.gemv_ok(down, down + 1)
+
+
 def mlp(x, group, gate, down):
     """down(silu(gate(x)) * up(x)), gate and up adjacent projections, in three launches; None as
     `linear`."""
-    if not group.gemv_ok(down, down + 1):
+    if not mlp_takes(x, group, gate, down):
         return None
     gu = linear(x, group, gate, down)
     if gu is None:

@@ -225,12 +225,15 @@ def _few_mlp(mlp, x):
 
 
 def fused_mlp_forward(mlp, x):
-    """FusedMLP when `mlp_plan` takes the layer, else None (the caller's own path runs). The
-    node runs in save-up mode when the save-up MLP is installed (mlp_save_up.py) and the call
+    """A few tokens without autograd on the NF4 codes where the layer's group is served there, else
+    FusedMLP when `mlp_plan` takes the layer, else None (the caller's own path runs). The node
+    runs in save-up mode when the save-up MLP is installed (mlp_save_up.py) and the call
     records autograd; otherwise in its default mode, which belongs to the in-place MLP patch
     (swiglu_inplace.py)."""
     if few_tokens.few(x):
-        return _few_mlp(mlp, x)
+        y = _few_mlp(mlp, x)
+        if y is not None:
+            return y
     save_up = ("mlp_save_up" in ON and "mlp_save_up" not in DISABLED
                and torch.is_grad_enabled() and x.requires_grad)
     if not save_up and "swiglu_inplace" not in ON:

@@ -200,10 +200,10 @@ def mlp_block(layer, x, h, follower):
     residual stream, h the attention's fp16 output of x's shape, both norms on the kernel with
     fp16 outputs, rows of at most MAX_WIDTH columns, the MLP a packed layer group in FusedMLP's
     default mode (`fused_mlp.mlp_plan`) whose gate|up input gradient can be left as K-part
-    partials (the NF4 dequant-GEMM, or the split-K GEMM); else None (the caller runs the separate
-    nodes)."""
+    partials (the NF4 dequant-GEMM, or the split-K GEMM), not for the few tokens that run on the
+    NF4 codes; else None (the caller runs the separate nodes)."""
     if not ENABLED or "mlp_block" in DISABLED or "addnorm" in DISABLED or "splitk" in DISABLED \
-            or not fused_mlp.SPLITK or few_tokens.few(h):
+            or not fused_mlp.SPLITK:
         return None
     norm1 = layer.post_attention_layernorm
     if not (x.is_cuda and h.is_cuda and x.dtype == torch.float32 and h.dtype == torch.float16
@@ -214,7 +214,7 @@ def mlp_block(layer, x, h, follower):
     if "swiglu_inplace" not in ON or ("mlp_save_up" in ON and "mlp_save_up" not in DISABLED):
         return None
     group = fused_mlp.mlp_plan(layer.mlp, h)
-    if group is None:
+    if group is None or few_tokens.mlp_takes(h, group, GATE, DOWN):
         return None
     inter = group.shapes[GATE][0]
     if inter < fused_mlp.SPLITK_MIN_K or inter % 8:

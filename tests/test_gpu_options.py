@@ -292,3 +292,24 @@ def test_mlp_alone(patched):
         want = (torch.nn.functional.silu(a @ gate.T) * (a @ up.T)) @ group.dequantize_one(6).double().T
     # gate, up, the activation and y rounded: a few 2^-11 of the magnitudes
     assert y.shape == x.shape and (y.double() - want).norm() <= 4 * 2.0 ** -11 * want.norm()
+
+
+def test_few_tokens_of_a_layer_the_codes_do_not_serve_keep_the_mlp_node(monkeypatch, patched):
+    """A group that the few-token products refuse (other NF4 blocks, other widths): the MLP stays the node
+    that longer calls run, the results too."""
+    model = _model(hidden_size=1024, intermediate_size=4096, num_hidden_layers=2).eval()
+    patches.apply()
+    ids = torch.randint(0, 1000, (1, 8), device="cuda")
+
+    def run():
+        engaged.reset()
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.float16):
+            logits = model(input_ids=ids).logits
+        return logits, {name: engaged.RAN[name] for name in ("fused_mlp", "mlp_block", "gemv")}
+    with monkeypatch.context() as m:
+        m.setattr(few_tokens, "ENABLED", False)
+        want, ran = run()
+    assert ran["fused_mlp"] == 2 and ran["gemv"] == 0
+    monkeypatch.setattr(qgroup.LayerGroup, "gemv_ok", lambda *a: False)
+    got, now = run()
+    assert now == ran and torch.equal(got, want)
