@@ -24,8 +24,8 @@ from .state import DISABLED, fallback
 
 ENABLED = os.environ.get("SOLUTION_DISABLE_GEMV") != "1"
 
-# the most rows of x that talm_nf4_gemv takes
-GEMV_TOKENS = 32
+# the most rows of x that talm_nf4_gemv takes, and the most elements from one to the next
+GEMV_TOKENS, MAX_STRIDE = 32, 1 << 24
 
 
 def few(x):
@@ -49,7 +49,9 @@ def serves(group, x):
 
 def _rows(x):
     x2 = x.reshape(-1, x.shape[-1])
-    if x2.stride(1) != 1 or x2.shape[0] > 1 and x2.stride(0) % 8 or x2.data_ptr() % 16:
+    (n, cols), (step, unit) = x2.shape, x2.stride()
+    # the kernel's rows do not overlap, and lie at most MAX_STRIDE elements apart
+    if unit != 1 or x2.data_ptr() % 16 or n > 1 and (step % 8 or not cols <= step <= MAX_STRIDE):
         x2 = x2.clone(memory_format=torch.contiguous_format)
     return x2
 

@@ -313,3 +313,16 @@ def test_few_tokens_of_a_layer_the_codes_do_not_serve_keep_the_mlp_node(monkeypa
     monkeypatch.setattr(qgroup.LayerGroup, "gemv_ok", lambda *a: False)
     got, now = run()
     assert now == ran and torch.equal(got, want)
+
+def test_rows_that_share_memory_stay_on_the_codes(patched):
+    """x given as an expanded row, or as overlapping ones: copied, not refused."""
+    model = _model().eval()
+    patches.apply()
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.float16):
+        model(input_ids=torch.zeros(1, 40, dtype=torch.int64, device="cuda"))  # packs the layers
+        flat = torch.randn(1024, device="cuda").half()
+        for x in (flat[:512].expand(4, 512), flat[:512].expand(2, 3, 512), flat.as_strided((4, 512), (8, 1))):
+            ran = engaged.RAN["gemv"]
+            got = model.model.layers[0].self_attn.o_proj(x)
+            assert engaged.RAN["gemv"] == ran + 1
+            assert torch.equal(got, model.model.layers[0].self_attn.o_proj(x.contiguous()))

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import philox
-from talm_amd import _lib, _ops, dropout, lora, unpad
+from talm_amd import _lib, _ops, dropout, few_tokens, lora, unpad
 
 PTR = 1 << 12  # a fake address: never dereferenced on rejection
 
@@ -171,3 +171,24 @@ def test_gemv_rejects_adapters_outside_the_weight(ldt, b0, lo0, hi0, b1, lo1, hi
     status, message = _status("talm_nf4_gemv", PTR, 128, 1, PTR, PTR, PTR, PTR, PTR, 128, 128, 64, 256,
                               None, PTR, ldt, b0, lo0, hi0, b1, lo1, hi1, PTR, 128, None)
     assert status == _lib.TALM_EINVAL and "adapters" in message
+
+
+@pytest.mark.parametrize("x", [
+    torch.zeros(64, dtype=torch.float16).expand(4, 64), torch.zeros(64, dtype=torch.float16).expand(2, 3, 64),
+    torch.zeros(256, dtype=torch.float16).as_strided((4, 64), (8, 1)),
+    torch.zeros(256, dtype=torch.float16).as_strided((4, 64), (56, 1)),
+    torch.zeros(4, 68, dtype=torch.float16)[:, :64], torch.zeros(4, 80, dtype=torch.float16)[:, 4:68],
+    torch.zeros(64, 4, dtype=torch.float16).t(),
+    torch.zeros((1 << 25) + 64, dtype=torch.float16).as_strided((2, 64), (1 << 25, 1))])
+def test_gemv_rows_are_ones_the_product_reads(x):
+    """Rows that share memory, are not 16-byte aligned or lie further apart than the kernel's offsets reach
+    are copied; others are taken where they lie."""
+    rows = few_tokens._rows(x)
+    assert rows.shape == (x.numel() // 64, 64) and rows.stride(1) == 1 and torch.equal(rows, x.reshape(-1, 64))
+    assert 64 <= rows.stride(0) <= 1 << 24 and rows.stride(0) % 8 == 0 and rows.data_ptr() % 16 == 0
+
+
+def test_gemv_rows_of_a_wider_buffer_stay():
+    wide = torch.zeros(4, 128, dtype=torch.float16)
+    assert few_tokens._rows(wide[:, 64:]).data_ptr() == wide[:, 64:].data_ptr()
+    assert few_tokens._rows(wide[:1, 8:72]).data_ptr() == wide[:1, 8:72].data_ptr()
