@@ -218,16 +218,14 @@ def _unpacked_branch(module, x):
             or down.bias is not None or up.bias is not None \
             or not branch_takes(x, down.weight, up.weight):
         return None
-    base = module.base_layer(x)
-    if base.dtype != torch.float16:
-        return None
     try:
-        return base + adapter_branch(x, down.weight, up.weight, float(module.scaling[name]), p,
-                                     draw_key(x.device))
+        branch = adapter_branch(x, down.weight, up.weight, float(module.scaling[name]), p,
+                                draw_key(x.device))
     except Exception as exc:  # noqa: BLE001 - state.py convention
         if not fallback("lora", exc):
             raise
         return None
+    return module.base_layer(x) + branch
 
 
 def patch_lora():

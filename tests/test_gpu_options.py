@@ -326,3 +326,28 @@ def test_rows_that_share_memory_stay_on_the_codes(patched):
             got = model.model.layers[0].self_attn.o_proj(x)
             assert engaged.RAN["gemv"] == ran + 1
             assert torch.equal(got, model.model.layers[0].self_attn.o_proj(x.contiguous()))
+
+def test_unpacked_adapter_on_a_base_of_another_type(monkeypatch, patched):
+    """A base that answers in float32 (it leaves autocast): run once, its output kept in that type."""
+    calls = []
+
+    class Base(torch.nn.Linear):
+        def forward(self, x):
+            calls.append(1)
+            with torch.autocast("cuda", enabled=False):
+                return super().forward(x.float())
+
+    torch.manual_seed(0)
+    layer = lora.LoraLinear(Base(256, 128, device="cuda"), 16, 32, 0.25).cuda().train()
+    with torch.no_grad():
+        layer.lora_B["default"].weight.normal_(0, 0.05)
+    x = torch.randn(9, 256, device="cuda").half()
+    patches.apply()
+    monkeypatch.setattr(dropout, "COUNTER", True)
+    key = _fixed_key(monkeypatch, 42, 43)
+    with torch.autocast("cuda", dtype=torch.float16):
+        y = layer(x)
+    assert len(calls) == 1 and y.dtype == torch.float32 and engaged.RAN["lora_branch"] == 1
+    params = (layer.lora_A["default"].weight, layer.lora_B["default"].weight)
+    branch = lora.adapter_branch(x, *params, 2.0, 0.25, key)
+    assert torch.equal(y, layer.base_layer(x) + branch)
