@@ -28,7 +28,7 @@ COUNTER = os.environ.get("SOLUTION_COUNTER_DROPOUT") == "1"
 
 def counter_dropout():
     """Whether the LoRA nodes' dropout comes from this generator now."""
-    return COUNTER or torch.cuda.is_current_stream_capturing()
+    return COUNTER or torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing()
 
 
 def draw_key(device):

@@ -241,7 +241,7 @@ def patch_lora():
         plan = None
         if not (args or kwargs) and "lora" not in DISABLED:
             plan = lora_plan(self, x)
-            if plan is None and counter_dropout():
+            if plan is None and x.is_cuda and counter_dropout():
                 y = _unpacked_branch(self, x)
                 if y is not None:
                     RAN["lora_branch"] += 1

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from oracle import philox
-from talm_amd import _lib, _ops, dropout, few_tokens, lora, unpad
+from talm_amd import _lib, _ops, dropout, few_tokens, lora, patches, unpad
 
 PTR = 1 << 12  # a fake address: never dereferenced on rejection
 
@@ -192,3 +192,21 @@ def test_gemv_rows_of_a_wider_buffer_stay():
     wide = torch.zeros(4, 128, dtype=torch.float16)
     assert few_tokens._rows(wide[:, 64:]).data_ptr() == wide[:, 64:].data_ptr()
     assert few_tokens._rows(wide[:1, 8:72]).data_ptr() == wide[:1, 8:72].data_ptr()
+
+
+def test_dropout_is_native_where_no_gpu_is_in_use(monkeypatch):
+    """A process without a GPU is not asked whether it captures a graph: a patched adapter layer on the CPU
+    runs its own forward."""
+    monkeypatch.setattr(dropout, "COUNTER", False)
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: pytest.fail("asked"))
+    assert not dropout.counter_dropout()
+    layer = lora.LoraLinear(torch.nn.Linear(64, 32), 16, 32, 0.5).eval()
+    x = torch.randn(3, 64)
+    want = layer(x)
+    monkeypatch.setattr(lora, "install_cast_cache", lambda: None)
+    lora.patch_lora()
+    try:
+        assert torch.equal(layer(x), want)
+    finally:
+        patches.unapply()
