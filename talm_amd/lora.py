@@ -187,20 +187,14 @@ def branch_takes(x, lora_a, lora_b):
             and lora_a.shape[1] % 32 == 0 and lora_b.shape[0] % 32 == 0)
 
 
-def _half(w):
-    """The fp16 values of an adapter weight that a forward reads (the shared copies of an fp32 one)."""
-    return COPIES.half(w) if _hooks and w.dtype == torch.float32 else w
-
-
 def adapter_branch(x, lora_a, lora_b, scaling, p=0.0, key=None, site=0):
     """A LoRA adapter's branch scaling * (dropout(x) A^T) B^T with gradients for x, A and B: x fp16
-    [..., in], A [16, in] and B [out, 16] fp16 or fp32 (fp32 ones are read as fp16 copies, their
-    gradients fp32), in and out multiples of 32; the dropout as `dropout.dropout` on x's rows, its mask
+    [..., in], A [16, in] and B [out, 16] fp16 or fp32 (fp32 ones are read as fp16 copies made in the
+    call, their gradients fp32), in and out multiples of 32; the dropout as `dropout.dropout` on x's rows, its mask
     computed in each product (talm_lora_branch_fwd, talm_lora_bwd_drop) and never stored, no dropped
     copy of x: PEFT's branch (solution/lora.py:183-231) on MFMA. An autograd node
     of the C++ op layer, differentiable once."""
-    return torch.ops.talm.adapter_branch(x, lora_a, lora_b, _half(lora_a), _half(lora_b), scaling, p,
-                                         key, site)
+    return torch.ops.talm.adapter_branch(x, lora_a, lora_b, lora_a, lora_b, scaling, p, key, site)
 
 
 def _unpacked_branch(module, x):
@@ -218,9 +212,13 @@ def _unpacked_branch(module, x):
             or down.bias is not None or up.bias is not None \
             or not branch_takes(x, down.weight, up.weight):
         return None
+    weights = down.weight, up.weight
     try:
-        branch = adapter_branch(x, down.weight, up.weight, float(module.scaling[name]), p,
-                                draw_key(x.device))
+        # the shared fp16 copies, whose launch reads the parameters as dense fp32 matrices
+        halves = _to_half(*weights) if all(w.is_contiguous() and w.dtype == torch.float32 for w in weights) \
+            else weights
+        branch = torch.ops.talm.adapter_branch(x, *weights, *halves, float(module.scaling[name]), p,
+                                               draw_key(x.device), 0)
     except Exception as exc:  # noqa: BLE001 - state.py convention
         if not fallback("lora", exc):
             raise

@@ -351,3 +351,27 @@ def test_unpacked_adapter_on_a_base_of_another_type(monkeypatch, patched):
     params = (layer.lora_A["default"].weight, layer.lora_B["default"].weight)
     branch = lora.adapter_branch(x, *params, 2.0, 0.25, key)
     assert torch.equal(y, layer.base_layer(x) + branch)
+
+
+def test_adapter_branch_reads_its_weights_as_they_are(patched):
+    """In a patched process, whose parameters have shared fp16 copies: weights that are views of other
+    memory, that change through .data, and that are temporaries."""
+    patches.apply()
+    g = torch.Generator("cuda").manual_seed(3)
+    x = torch.randn(12, 64, device="cuda", generator=g).half()
+    key = torch.tensor([3, 4], device="cuda")
+    a = torch.randn(16, 64, device="cuda", generator=g)
+    b = torch.randn(32, 16, device="cuda", generator=g)
+
+    def check(a, b):
+        want = lora.adapter_branch(x, a.half().contiguous(), b.half().contiguous(), 2.0, 0.3, key)
+        assert torch.equal(lora.adapter_branch(x, a, b, 2.0, 0.3, key), want)
+        return want
+    for views in ((a, b), (a.t().contiguous().t(), b.t().contiguous().t()), (a[:1].expand(16, 64), b[:1].expand(32, 16)),
+                  (torch.randn(32, 128, device="cuda")[::2, ::2], b)):
+        first = check(*views)
+        views[0].data.mul_(2.0) if views[0].stride(0) else views[0][:1].data.mul_(2.0)
+        second = check(*views)
+        assert not torch.equal(first, second)
+    for i in range(3):
+        check(a * i, b + i)

@@ -210,3 +210,13 @@ def test_dropout_is_native_where_no_gpu_is_in_use(monkeypatch):
         assert torch.equal(layer(x), want)
     finally:
         patches.unapply()
+
+
+def test_adapter_branch_keeps_nothing_of_its_weights(monkeypatch):
+    """The shared fp16 copies belong to a model's contiguous parameters, kept by identity until an optimizer
+    steps: any tensor may be given here, a view or one that changes through .data."""
+    monkeypatch.setattr(lora, "_hooks", [None])  # as in a patched process
+    monkeypatch.setattr(lora.COPIES, "half", lambda w: pytest.fail("kept"))
+    with pytest.raises(ValueError, match="adapter_branch"):  # the refusal of CPU operands
+        lora.adapter_branch(torch.zeros(4, 64, dtype=torch.float16), torch.zeros(1, 64).expand(16, 64),
+                            torch.zeros(32, 16), 2.0)
