@@ -344,8 +344,8 @@ def _autocast_half(query):
 
 def attention_sinks(module):
     """The first tokens of a row that stay visible to a sliding layer's rows (config.attention_sinks;
-    0 when the config names none)."""
-    return int(getattr(module.config, "attention_sinks", 0) or 0)
+    0 when the module has no config, or one that names none)."""
+    return int(getattr(getattr(module, "config", None), "attention_sinks", 0) or 0)
 
 
 def packs_sliding(config):

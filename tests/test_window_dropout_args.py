@@ -220,3 +220,28 @@ def test_adapter_branch_keeps_nothing_of_its_weights(monkeypatch):
     with pytest.raises(ValueError, match="adapter_branch"):  # the refusal of CPU operands
         lora.adapter_branch(torch.zeros(4, 64, dtype=torch.float16), torch.zeros(1, 64).expand(16, 64),
                             torch.zeros(32, 16), 2.0)
+
+
+def test_windowed_calls_of_modules_without_a_config_pass(monkeypatch):
+    """The "sdpa" interface is the process's: a module that names no config has no sinks, one whose config
+    does is refused off the packed rows."""
+    from types import SimpleNamespace
+
+    from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+
+    q = torch.randn(1, 2, 5, 16, generator=torch.Generator().manual_seed(0))
+    plain = ALL_ATTENTION_FUNCTIONS["sdpa"]
+    unpad.patch_sdpa_rows()
+    try:
+        call = ALL_ATTENTION_FUNCTIONS["sdpa"]
+        assert call is not plain
+        for module in (SimpleNamespace(is_causal=True), SimpleNamespace(is_causal=True, config=None),
+                       SimpleNamespace(is_causal=True, config=SimpleNamespace()),
+                       SimpleNamespace(is_causal=True, config=SimpleNamespace(attention_sinks=None))):
+            want = plain(module, q, q, q, None, sliding_window=3)[0]
+            assert torch.equal(call(module, q, q, q, None, sliding_window=3)[0], want)
+        module = SimpleNamespace(is_causal=True, config=SimpleNamespace(attention_sinks=2))
+        with pytest.raises(ValueError, match="sinks"):
+            call(module, q, q, q, None, sliding_window=3)
+    finally:
+        patches.unapply()
