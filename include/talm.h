@@ -613,9 +613,10 @@ int talm_scale_rows(const uint16_t* g, int64_t n, const float* grad_loss, const 
  * talm_attn_fwd in a sliding window: row i of a sequence attends to the keys j <= i with i - j <
  * window or j < sinks (the sequence's first `sinks` tokens stay visible; 0: none). window >= 1; one
  * of at least the longest sequence is the causal attention. dtype TALM_F16 or TALM_BF16 (q, k, v
- * and out); scale positive. Key tiles that no row sees are not read: the work grows with
- * n_tokens (window + sinks). q, k and v have to be finite (a masked key has weight 0, but 0 times an
- * infinity is no number). Rows behind the last sequence (cu_seqlens[n_seqs]) are left as they were.
+ * and out); scale positive; fewer than 2^30 rows. Key tiles that no row sees are not read: the work
+ * grows with n_tokens (window + sinks). q, k and v have to be finite (a masked key has weight 0,
+ * but 0 times an infinity is no number). Rows behind the last sequence (cu_seqlens[n_seqs]) are
+ * left as they were.
  * No counterpart in the reference, whose packed rows exclude sliding layers (solution/patches.py:
  * 173-260).
  */

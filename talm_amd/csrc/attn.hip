@@ -1539,6 +1539,13 @@ struct Window {
   int32_t window, sinks, dtype;
 };
 
+// No sequence is longer than the rows, of which a window takes fewer than 2^30: the kernels' sums of a row and
+// a window or sinks, at most this long, fit 32 bits.
+constexpr int64_t kWindowRows = int64_t{1} << 30;
+int32_t longest_of(int32_t max_seqlen, int64_t n_tokens) {
+  return static_cast<int32_t>(std::min<int64_t>(max_seqlen, n_tokens));
+}
+
 int check_window(const char* what, const Window& w, float scale) {
   if (w.dtype != TALM_F16 && w.dtype != TALM_BF16)
     return fail(TALM_EINVAL, "%s: dtype %d (TALM_F16 or TALM_BF16)", what, w.dtype);
@@ -1572,7 +1579,7 @@ int attn_fwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
   if (head_dim != kD)
     return fail(TALM_EINVAL, "%s: head_dim %d (only %d)", what, head_dim, kD);
   if (n_seqs < 0 || max_seqlen < 0 || n_tokens < 0 || n_q_heads < 1 || n_kv_heads < 1 ||
-      n_q_heads % n_kv_heads || n_tokens >= (int64_t{1} << 31))
+      n_q_heads % n_kv_heads || n_tokens >= (win.window ? kWindowRows : int64_t{1} << 31))
     return fail(TALM_EINVAL, "%s: bad shape (seqs %d, max_seqlen %d, tokens %lld, heads %d/%d)", what,
                 n_seqs, max_seqlen, (long long)n_tokens, n_q_heads, n_kv_heads);
   for (int64_t s : {q_stride_tok, q_stride_head, k_stride_tok, k_stride_head, v_stride_tok,
@@ -1582,6 +1589,7 @@ int attn_fwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
   if (k_stride_tok >= (int64_t{1} << 23) || v_stride_tok >= (int64_t{1} << 23) ||
       o_stride_tok >= (int64_t{1} << 23))
     return fail(TALM_EINVAL, "%s: k / v / out token strides must be below 2^23 elements", what);
+  if (win.window) max_seqlen = longest_of(max_seqlen, n_tokens);
   if (n_seqs == 0 || max_seqlen == 0 || n_tokens == 0) return ok();
   if (!q || !k || !v || !cu_seqlens || !out || !lse) return fail(TALM_EINVAL, "%s: null pointer", what);
   if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16))
@@ -1785,7 +1793,7 @@ int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
   if (head_dim != kD)
     return fail(TALM_EINVAL, "%s: head_dim %d (only %d)", what, head_dim, kD);
   if (n_seqs < 0 || max_seqlen < 0 || n_tokens < 0 || n_q_heads < 1 || n_kv_heads < 1 ||
-      n_q_heads % n_kv_heads || n_tokens >= (int64_t{1} << 31))
+      n_q_heads % n_kv_heads || n_tokens >= (win.window ? kWindowRows : int64_t{1} << 31))
     return fail(TALM_EINVAL, "%s: bad shape (seqs %d, max_seqlen %d, tokens %lld, heads %d/%d)", what,
                 n_seqs, max_seqlen, (long long)n_tokens, n_q_heads, n_kv_heads);
   for (int64_t s : {q_stride_tok, q_stride_head, k_stride_tok, k_stride_head, v_stride_tok,
@@ -1798,7 +1806,8 @@ int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
       v_stride_tok >= (int64_t{1} << 23) || do_stride_tok >= (int64_t{1} << 23) ||
       dq_stride_tok >= (int64_t{1} << 23))
     return fail(TALM_EINVAL, "%s: q / k / v / dout / dq token strides must be below 2^23 elements", what);
-  if (n_seqs > 65535 || (max_seqlen + 127) / 128 > 32767)
+  if (win.window) max_seqlen = longest_of(max_seqlen, n_tokens);
+  if (n_seqs > 65535 || max_seqlen > 128 * 32767)
     return fail(TALM_EINVAL, "%s: at most 65535 sequences of at most 4194176 tokens", what);
   // (a workspace without the queue's counter is accepted: one workgroup per item then)
   const int item_heads = win.window ? window_item_heads(n_tokens, n_seqs, max_seqlen, n_q_heads,
@@ -1941,8 +1950,9 @@ TALM_API int64_t talm_attn_window_bwd_workspace(int64_t n_tokens, int32_t n_q_he
                                                 int32_t n_seqs, int32_t max_seqlen, int32_t window,
                                                 int32_t sinks) {
   if (n_tokens < 0 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads % n_kv_heads || n_seqs < 0 || max_seqlen < 0 ||
-      window < 1 || sinks < 0)
+      window < 1 || sinks < 0 || n_tokens >= kWindowRows)
     return -1;
+  max_seqlen = longest_of(max_seqlen, n_tokens);
   const int heads = window_item_heads(n_tokens, n_seqs, max_seqlen, n_q_heads, n_q_heads / n_kv_heads, window);
   return talm_attn_bwd_workspace(n_tokens, n_q_heads) +
          8 * far_plan(n_seqs, max_seqlen, n_q_heads, heads, window, sinks).floats;

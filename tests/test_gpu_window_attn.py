@@ -391,3 +391,25 @@ def test_gradients_are_zero_without_a_token_in_a_sequence(lengths, half):
                                            angles.cos() if rotated else None, angles.sin() if rotated else None,
                                            dq, dk, dv, ws)
             assert not dq.any() and not dk.any() and not dv.any()
+
+
+@pytest.mark.parametrize("window,sinks", [(40, 2 ** 31 - 1), (2 ** 31 - 1, 3), (2 ** 31 - 1, 2 ** 31 - 1), (70, 5)])
+def test_the_largest_arguments_mean_the_whole_rows(window, sinks):
+    """The ops with the largest 32-bit longest length, window and sinks: the results of the rows' own sizes."""
+    from talm_amd import _ops
+
+    print(f"[case] window={window} sinks={sinks} of a longest length of 2^31 - 1", flush=True)
+    lengths = [500, 77, 130]
+    n, cu = sum(lengths), _cu(lengths)
+    q, k, v, dout = _inputs(n, 4, 2, torch.float16, True, 6)
+
+    def call(longest, window, sinks):
+        out, lse = torch.empty_like(dout), torch.empty(4, n, device="cuda")
+        torch.ops.talm.attn_window_fwd(q, k, v, cu, longest, 0.1, window, sinks, out, lse)
+        grads = [torch.empty(t.shape, dtype=t.dtype, device="cuda") for t in (q, k, v)]
+        ws = torch.empty(_ops.attn_window_bwd_workspace_bytes(n, 4, 2, 3, longest, window, sinks), dtype=torch.uint8,
+                         device="cuda")
+        torch.ops.talm.attn_window_bwd(q, k, v, out, dout, lse, cu, longest, 0.1, window, sinks, None, None, *grads, ws)
+        return [out, lse, *grads]
+    for a, b in zip(call(2 ** 31 - 1, window, sinks), call(n, min(window, n), min(sinks, n))):
+        assert torch.equal(a, b)

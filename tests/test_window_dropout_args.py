@@ -245,3 +245,16 @@ def test_windowed_calls_of_modules_without_a_config_pass(monkeypatch):
             call(module, q, q, q, None, sliding_window=3)
     finally:
         patches.unapply()
+
+
+def test_a_longest_length_beyond_the_rows_is_the_rows():
+    """The kernels add rows, windows and sinks in 32 bits: none may count as longer than all rows."""
+    for window in (64, 2 ** 31 - 1):
+        for sinks in (0, 4, 4096, 2 ** 31 - 1):
+            want = _ops.attn_window_bwd_workspace_bytes(4096, 2, 1, 1, 4096, window, sinks)
+            for longest in (5000, 2 ** 31 - 1):
+                assert _ops.attn_window_bwd_workspace_bytes(4096, 2, 1, 1, longest, window, sinks) == want
+    with pytest.raises(ValueError):
+        _ops.attn_window_bwd_workspace_bytes(1 << 30, 1, 1, 1, 4096, 64, 0)
+    status, message = _window(n=1 << 30)
+    assert status == _lib.TALM_EINVAL and "shape" in message
