@@ -1747,6 +1747,24 @@ FarPlan far_plan(int64_t n_seqs, int64_t max_seqlen, int64_t n_q_heads, int64_t 
   return f;
 }
 
+constexpr int kMostSeqs = 65535, kLongestBwd = 128 * 32767;  // a grid's second axis, half of its third
+
+struct WindowPlan {
+  int item_heads = 1;
+  FarPlan far;
+};
+// A window's backward for at most kMostSeqs sequences of at most kLongestBwd rows; false where the launches or
+// the partials' 32-bit indices do not hold its heads or sinks.
+bool window_plan(int64_t n_tokens, int64_t n_seqs, int64_t max_seqlen, int64_t n_q_heads, int64_t group,
+                 const Window& win, WindowPlan& p) {
+  if (n_q_heads > 65535 || n_seqs * n_q_heads * std::min<int64_t>(win.sinks, max_seqlen) >= (int64_t{1} << 31))
+    return false;
+  p.item_heads = window_item_heads(n_tokens, n_seqs, max_seqlen, n_q_heads, group, win.window);
+  p.far = far_plan(n_seqs, max_seqlen, n_q_heads, p.item_heads, win.window, win.sinks);
+  return p.far.chunks * p.far.tiles + 2 * ((max_seqlen + 127) / 128) <= 65535 &&
+         n_seqs * p.far.chunks * p.far.tiles * n_q_heads < (int64_t{1} << 30);
+}
+
 template <class E, bool kWin>
 void launch_bwd(const BwdArgs& a, int n_seqs, hipStream_t s) {
   constexpr int W = 4;
@@ -1807,18 +1825,16 @@ int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
       dq_stride_tok >= (int64_t{1} << 23))
     return fail(TALM_EINVAL, "%s: q / k / v / dout / dq token strides must be below 2^23 elements", what);
   if (win.window) max_seqlen = longest_of(max_seqlen, n_tokens);
-  if (n_seqs > 65535 || max_seqlen > 128 * 32767)
-    return fail(TALM_EINVAL, "%s: at most 65535 sequences of at most 4194176 tokens", what);
+  if (n_seqs > kMostSeqs || max_seqlen > kLongestBwd)
+    return fail(TALM_EINVAL, "%s: at most %d sequences of at most %d tokens", what, kMostSeqs, kLongestBwd);
   // (a workspace without the queue's counter is accepted: one workgroup per item then)
-  const int item_heads = win.window ? window_item_heads(n_tokens, n_seqs, max_seqlen, n_q_heads,
-                                                        n_q_heads / n_kv_heads, win.window) : 1;
-  const FarPlan far =
-      win.window ? far_plan(n_seqs, max_seqlen, n_q_heads, item_heads, win.window, win.sinks) : FarPlan{};
+  WindowPlan plan;
+  if (win.window && !window_plan(n_tokens, n_seqs, max_seqlen, n_q_heads, n_q_heads / n_kv_heads, win, plan))
+    return fail(TALM_EINVAL, "%s: %d sinks of %d sequences with %d heads are too many", what, win.sinks, n_seqs,
+                n_q_heads);
+  const int item_heads = plan.item_heads;
+  const FarPlan& far = plan.far;
   const int64_t need = talm_attn_bwd_workspace(n_tokens, n_q_heads) - kQueueBytes + 8 * far.floats;
-  if (far.chunks * far.tiles + 2 * ((max_seqlen + 127) / 128) > 65535 ||
-      n_seqs * far.chunks * far.tiles * n_q_heads >= (int64_t{1} << 30) ||
-      n_seqs * static_cast<int64_t>(n_q_heads) * std::min(win.sinks, max_seqlen) >= (int64_t{1} << 31))
-    return fail(TALM_EINVAL, "%s: %d sinks of %d sequences are too many", what, win.sinks, n_seqs);
   if (workspace_bytes < need)
     return fail(TALM_EINVAL, "%s: workspace of %lld bytes, %lld needed", what,
                 (long long)workspace_bytes, (long long)need);
@@ -1953,9 +1969,12 @@ TALM_API int64_t talm_attn_window_bwd_workspace(int64_t n_tokens, int32_t n_q_he
       window < 1 || sinks < 0 || n_tokens >= kWindowRows)
     return -1;
   max_seqlen = longest_of(max_seqlen, n_tokens);
-  const int heads = window_item_heads(n_tokens, n_seqs, max_seqlen, n_q_heads, n_q_heads / n_kv_heads, window);
-  return talm_attn_bwd_workspace(n_tokens, n_q_heads) +
-         8 * far_plan(n_seqs, max_seqlen, n_q_heads, heads, window, sinks).floats;
+  WindowPlan plan;
+  if (n_seqs > kMostSeqs || max_seqlen > kLongestBwd ||
+      !window_plan(n_tokens, n_seqs, max_seqlen, n_q_heads, n_q_heads / n_kv_heads, Window{window, sinks, TALM_F16},
+                   plan))
+    return -1;
+  return talm_attn_bwd_workspace(n_tokens, n_q_heads) + 8 * plan.far.floats;
 }
 
 TALM_API int talm_attn_window_bwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,

@@ -258,3 +258,21 @@ def test_a_longest_length_beyond_the_rows_is_the_rows():
         _ops.attn_window_bwd_workspace_bytes(1 << 30, 1, 1, 1, 4096, 64, 0)
     status, message = _window(n=1 << 30)
     assert status == _lib.TALM_EINVAL and "shape" in message
+
+
+@pytest.mark.parametrize("tokens,heads,kv,seqs,longest,window,sinks", [
+    (1 << 30, 1, 1, 1, 4096, 64, 4),           # rows
+    (1 << 20, 2, 1, 65536, 64, 64, 4),         # sequences
+    (1 << 29, 1, 1, 1, 4194177, 64, 0),        # a longer sequence than the tiles' axis holds
+    (1 << 29, 1, 1, 2, 4194176, 64, 4194176),  # sinks' tiles beside the others
+    (1 << 29, 64, 64, 65535, 4096, 64, 4096),  # sinks' partials
+    (1 << 20, 1 << 16, 1, 1, 4096, 64, 0),     # heads
+])
+def test_window_workspace_of_a_call_that_would_be_rejected(tokens, heads, kv, seqs, longest, window, sinks):
+    """The size query answers -1 exactly where the call says TALM_EINVAL for its sizes."""
+    assert _lib.lib().talm_attn_window_bwd_workspace(tokens, heads, kv, seqs, longest, window, sinks) == -1
+    rows = [PTR, 256, 128]
+    status, message = _status(
+        "talm_attn_window_bwd", *rows, *rows, *rows, *rows, *rows, PTR, PTR, seqs, longest, tokens, heads, kv, 128,
+        1.0, window, sinks, _lib.TALM_F16, None, None, 0, *rows, *rows, *rows, PTR, 0, None)
+    assert status == _lib.TALM_EINVAL and "workspace" not in message
