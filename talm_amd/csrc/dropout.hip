@@ -713,6 +713,7 @@ TALM_API int talm_lora_bwd_drop(const uint16_t* x, int64_t ldx, const uint16_t* 
   const bool grads = da0 != nullptr;
   if (grads ? !db0 || (two && (!da1 || !db1)) : db0 || da1 || db1)
     return fail(TALM_EINVAL, "lora_bwd_drop: the weight gradients are given all or none");
+  if (n_tokens == 0) dx = nullptr;  // no element, and A may be null
   if (!grads && !dx) return ok();
   if (n_tokens > 0 && (!x || !dy || !u || !t || (dx && (!a0 || (two && !a1)))))
     return fail(TALM_EINVAL, "lora_bwd_drop: null pointer");

@@ -365,3 +365,19 @@ def test_an_infinity_reaches_its_own_token_as_the_formula_has_it(size):
             bad[7, column] = value
             for got, without in zip(branch(bad), want):
                 assert (got[7] == value).all() and torch.equal(got[others], without[others])
+
+
+def test_adapter_gradients_of_no_tokens_are_zero_without_a():
+    """dx is given for no tokens, A is not: the weight gradients are zeros."""
+    from talm_amd import _lib
+
+    lib = _lib.lib()
+    da, db = torch.full((16, 64), 5.0, device="cuda"), torch.full((32, 16), 5.0, device="cuda")
+    dx = torch.full((1, 64), 5.0, dtype=torch.float16, device="cuda")
+    ws = torch.empty(max(lib.talm_lora_bwd_drop_workspace(0, 64, 1, 32, 0), 1), dtype=torch.uint8, device="cuda")
+    status = lib.talm_lora_bwd_drop(None, 64, None, 32, None, 16, None, 16, 0, 64, 1, 0.5, _key(1, 2).data_ptr(), 0, 1,
+                                    _lib.TALM_F32, 0, 32, 1.0, da.data_ptr(), db.data_ptr(), 0, 0, 0.0, None, None,
+                                    None, None, None, 0, dx.data_ptr(), 64, ws.data_ptr(), ws.numel(),
+                                    torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert status == _lib.TALM_OK and (da == 0).all() and (db == 0).all() and (dx == 5).all()

@@ -276,3 +276,11 @@ def test_window_workspace_of_a_call_that_would_be_rejected(tokens, heads, kv, se
         "talm_attn_window_bwd", *rows, *rows, *rows, *rows, *rows, PTR, PTR, seqs, longest, tokens, heads, kv, 128,
         1.0, window, sinks, _lib.TALM_F16, None, None, 0, *rows, *rows, *rows, PTR, 0, None)
     assert status == _lib.TALM_EINVAL and "workspace" not in message
+
+
+def test_adapter_backward_of_no_tokens_wants_nothing_for_dx():
+    """dx of no tokens has no element, and A may be absent: without weight gradients nothing is launched."""
+    status, message = _status("talm_lora_bwd_drop", None, 64, None, 32, None, 16, None, 16, 0, 64, 1, 0.5, PTR, 0, 1,
+                              _lib.TALM_F32, 0, 32, 1.0, None, None, 0, 0, 0.0, None, None, None, None, None, 0, PTR,
+                              64, PTR, 1 << 20, None)
+    assert status == _lib.TALM_OK, message
