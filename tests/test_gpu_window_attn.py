@@ -413,3 +413,37 @@ def test_the_largest_arguments_mean_the_whole_rows(window, sinks):
         return [out, lse, *grads]
     for a, b in zip(call(2 ** 31 - 1, window, sinks), call(n, min(window, n), min(sinks, n))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("half,h", [(torch.float16, 2.0 ** -4), (torch.bfloat16, 2.0 ** -3)])
+def test_gradients_against_differences_along_them(half, h, which):
+    """A central difference of sum(out g) along the gradient itself of q, k or v, whose derivative is of the
+    size |gradient| |step|. By the triangle inequality it is off <gradient, step> by at most the two outputs'
+    tolerances against |g|, the float64 difference's own distance from the float64 derivative (its
+    truncation), and the gradient's tolerance against |step|. A negated, doubled, missing or shifted gradient is
+    further off (1.9 to 47 times the bound where float64 stands for the kernels)."""
+    print(f"[case] difference along the gradient of {'qkv'[which]} {half}", flush=True)
+    lengths, window, sinks, scale = [200, 90], 40, 3, D ** -0.5
+    ops = list(_inputs(290, 4, 2, half, False, 13))
+    dout, cu = ops.pop(), _cu(lengths)
+    grad = _call(*ops, cu, 200, window, sinks, dout)[1 + which].double().cpu()
+    vals, tols = _reference(*ops, lengths, scale, window, sinks, dout, half)
+    true, tol = vals[1 + which], tols[1 + which]
+    direction = h * math.sqrt(true.numel()) * true / true.norm()
+    weight, ends = dout.double().cpu(), []
+    for sign in (1, -1):
+        moved = list(ops)
+        moved[which] = (ops[which].double().cpu() + sign * direction).to(half).cuda()
+        out = _call(*moved, cu, 200, window, sinks).double().cpu()
+        exact, slack = (t[0] for t in _reference(*moved, lengths, scale, window, sinks, dout, half))
+        ends.append((moved[which].double().cpu(), out, exact, slack))
+    (at, out, exact, slack), (at_, out_, exact_, slack_) = ends
+    step = at - at_
+    diff = ((out - out_) * weight).sum()
+    bound = ((slack + slack_) * weight.abs()).sum() + (tol * step.abs()).sum() \
+        + abs(((exact - exact_) * weight).sum() - (true * step).sum())
+    print(f"  difference {diff:.1f}, derivative {(grad * step).sum():.1f}, bound {bound:.1f}", flush=True)
+    assert abs(diff - (grad * step).sum()) <= bound
+    for wrong in (-grad, 2 * grad, 0 * grad, grad.roll(1, 0)):
+        assert abs(diff - (wrong * step).sum()) > bound
