@@ -167,3 +167,80 @@ def test_gemv_replays_from_a_graph():
         want = torch.empty_like(out)
         group.nf4_gemv(x, 4, 6, want)
         assert torch.equal(out, want)
+
+
+# -- buffers of any number of rows, and adapters, straight through the op ------------------------------
+
+def _weight(rows, cols, seed):
+    """The op's buffers of a W [rows, cols], and W in float64."""
+    from oracle import nf4
+
+    g = torch.Generator().manual_seed(seed)
+    n = rows * cols
+    blocks, groups = n // 64, (n // 64 + 255) // 256
+    packed = torch.randint(0, 256, (n // 2,), generator=g, dtype=torch.uint8)
+    absmax8 = torch.randint(0, 256, (blocks,), generator=g, dtype=torch.uint8)
+    code = torch.linspace(-1, 1, 256)
+    absmax2 = torch.rand(groups, generator=g) * 0.05
+    offset2 = torch.rand(groups, generator=g) * 0.05 + 0.05
+    # the oracle takes whole second-level groups
+    bits = nf4.group_dequant(*(torch.nn.functional.pad(t, (0, size - t.numel())).numpy() for t, size in (
+        (packed, groups * 8192), (absmax8, groups * 256), (code, 256), (absmax2, groups), (offset2, groups))))
+    w = torch.from_numpy(bits.view("float16")[:n].astype("float32")).view(rows, cols)
+    return [t.cuda() for t in (packed, absmax8, code, absmax2, offset2)], w.cuda().double()
+
+
+def _check_op(rows, cols, tokens, segments, biased, buffers, w, pad=0):
+    """segments: the adapters' (lo, hi). 16 products of an adapter are exact in fp32 and added one by one: 32
+    additions more than the tolerance above counts, and the bias."""
+    print(f"[case] W {rows} x {cols} tokens={tokens} adapters={segments} bias={biased}", flush=True)
+    g = torch.Generator("cuda").manual_seed(rows + tokens)
+
+    def rand(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").half()
+    x = rand(tokens, cols + pad)[:, :cols]
+    bias = rand(rows) if biased else None
+    ts = rand(tokens, 16 * len(segments) + pad)[:, :16 * len(segments)] if segments else None
+    ups = [rand(hi - lo, 16) for lo, hi in segments]
+    wide = torch.full((tokens, rows + 16), 3.0, dtype=torch.float16, device="cuda")
+    out = wide[:, 8:8 + rows]
+    extra = [] if ts is None else [ts, *[v for b, (lo, hi) in zip(ups, segments) for v in (b, lo, hi)]]
+    torch.ops.talm.nf4_gemv(x, *buffers, rows, cols, 64, 256, bias, out, *extra)
+    y, mag = x.double() @ w.T, x.double().abs() @ w.abs().T
+    if biased:
+        y, mag = y + bias.double(), mag + bias.double().abs()
+    for i, (b, (lo, hi)) in enumerate(zip(ups, segments)):
+        t = ts[:, 16 * i:16 * i + 16].double()
+        y[:, lo:hi] += t @ b.double().T
+        mag[:, lo:hi] += t.abs() @ b.double().abs().T
+    tol = 2.0 ** -11 * y.abs() + (cols / 32 + 96 + 33) * 2.0 ** -24 * mag + 2.0 ** -25
+    worst = ((out.double() - y).abs() / tol).max().item()
+    print(f"  {worst:.3f} of the tolerance", flush=True)
+    assert worst <= 1.0
+    assert (wide[:, :8] == 3).all() and (wide[:, 8 + rows:] == 3).all()
+
+
+@pytest.mark.parametrize("cols", [64, 320, 896])
+@pytest.mark.parametrize("rows", [1, 7, 13, 250])
+def test_gemv_of_odd_rows_and_reductions(rows, cols):
+    """Row tiles and reduction units that are both partial, down to a weight of one row."""
+    buffers, w = _weight(rows, cols, rows + cols)
+    for tokens in (1, 2, 3, 5, 9, 17, 32):
+        _check_op(rows, cols, tokens, (), tokens % 2 == 1, buffers, w, pad=8 * (tokens % 3))
+
+
+@pytest.mark.parametrize("rows,cols", [
+    (250, 896), (2048, 1536),      # a table in registers
+    (6203, 1600),                  # a table in LDS: one unit a wavefront
+    (2051, 4672),                  # two parts per tile
+    (4101, 4352), (1540, 8960),    # several units per wavefront, in one part and in two
+    (20612, 4096),                 # tiles joined in several rounds
+])
+def test_gemv_with_adapters_matches_its_formula(rows, cols):
+    """One and two adapters whose rows begin and end inside tiles, lie in the last one, or share some."""
+    buffers, w = _weight(rows, cols, rows)
+    third, last = rows // 3 | 1, rows - 5
+    for tokens in (1, 5, 9, 17, 32):
+        for segments in ([(0, rows)], [(third, last)], [(3, third), (last, rows)], [(third, rows), (1, last)],
+                         [(last, last + 1), (0, 1)]):
+            _check_op(rows, cols, tokens, segments, tokens != 5, buffers, w, pad=8 * (tokens & 1))

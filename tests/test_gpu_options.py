@@ -375,3 +375,35 @@ def test_adapter_branch_reads_its_weights_as_they_are(patched):
         assert not torch.equal(first, second)
     for i in range(3):
         check(a * i, b + i)
+
+
+@pytest.mark.parametrize("batch", [1, 9])
+def test_adapters_of_single_projections_join_their_products(monkeypatch, patched, batch):
+    """Generation with adapters on o_proj and down_proj beside q's and v's: each is added by its projection's
+    product. Logits against the same patched model without the few-token products, as above."""
+    print(f"[case] generation with adapters on o and down, batch={batch}", flush=True)
+    torch.manual_seed(4)
+    model = _model()
+    for layer in model.model.layers:
+        for owner, name in ((layer.self_attn, "o_proj"), (layer.mlp, "down_proj")):
+            wrapped = lora.LoraLinear(getattr(owner, name), 16, 32)
+            torch.nn.init.normal_(wrapped.lora_B["default"].weight, 0, 0.02)
+            setattr(owner, name, wrapped)
+    model.eval()
+    patches.apply()
+    ids = torch.randint(0, 1000, (batch, 70), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    with monkeypatch.context() as m:
+        m.setattr(few_tokens, "ENABLED", False)
+        want = _logits(model, ids, 3)
+        assert engaged.RAN["gemv"] == 0
+        for layer in model.model.layers:  # the adapters matter
+            layer.mlp.down_proj.scaling["default"] = 0.0
+        without = _logits(model, ids, 3)
+        for layer in model.model.layers:
+            layer.mlp.down_proj.scaling["default"] = 2.0
+    assert (without - want).norm() > 0.05 * want.norm()
+    engaged.reset()
+    got = _logits(model, ids, 3)
+    # per layer and token: q|k|v, o, gate, up, down
+    assert engaged.RAN["gemv"] == 3 * 3 * 5
+    assert (got - want).norm() <= 5e-3 * want.norm()
