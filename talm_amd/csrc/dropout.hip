@@ -244,9 +244,8 @@ __global__ __launch_bounds__(256) void lora_up_kernel(UpArgs a) {
     const int tok = blockIdx.y * kUpTokens + 32 * tb + l32;
     const bool in = tok < a.n_tokens;
     const float* p = a.part + static_cast<int64_t>(in ? tok : a.n_tokens - 1) * kRank + 8 * hh;
-    float s[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    // every part's loads before their adds: a part past the last is the last one again, not added (selects:
-    // a product with 0 would turn an infinity into NaN)
+    // every part's loads before their adds: a part past the last is the last one again, its bits cleared
+    // (a product with 0 would turn an infinity into NaN; a select would be a branch before the loads)
     float4 lo[kDownMaxParts], hi[kDownMaxParts];
 #pragma unroll
     for (int i = 0; i < kDownMaxParts; ++i) {
@@ -254,11 +253,13 @@ __global__ __launch_bounds__(256) void lora_up_kernel(UpArgs a) {
       lo[i] = reinterpret_cast<const float4*>(q)[0];
       hi[i] = reinterpret_cast<const float4*>(q)[1];
     }
+    float s[8] = {lo[0].x, lo[0].y, lo[0].z, lo[0].w, hi[0].x, hi[0].y, hi[0].z, hi[0].w};
 #pragma unroll
-    for (int i = 0; i < kDownMaxParts; ++i) {
-      const bool is = i < a.parts;
-      s[0] += is ? lo[i].x : 0.f; s[1] += is ? lo[i].y : 0.f; s[2] += is ? lo[i].z : 0.f; s[3] += is ? lo[i].w : 0.f;
-      s[4] += is ? hi[i].x : 0.f; s[5] += is ? hi[i].y : 0.f; s[6] += is ? hi[i].z : 0.f; s[7] += is ? hi[i].w : 0.f;
+    for (int i = 1; i < kDownMaxParts; ++i) {
+      const uint32_t is = i < a.parts ? 0xffffffffu : 0u;
+      const float v[8] = {lo[i].x, lo[i].y, lo[i].z, lo[i].w, hi[i].x, hi[i].y, hi[i].z, hi[i].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v[e]) & is);
     }
     const float f = a.factor;
     const uint4 tf = make_uint4(pack2(f * s[0], f * s[1]), pack2(f * s[2], f * s[3]), pack2(f * s[4], f * s[5]),
