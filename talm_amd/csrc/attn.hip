@@ -18,7 +18,8 @@
 // row statistics are kept in base 2 (scores times scale * log2 e); lse is written in natural-log
 // units, [Hq, N].
 //
-// The backward (P = exp(S - lse), dV = P^T dO, dP = dO V^T,
+// The backward (the recurrences of Dao, "FlashAttention-2: Faster Attention with Better Parallelism and
+// Work Partitioning", 2023: P = exp(S - lse), dV = P^T dO, dP = dO V^T,
 // dS = P (dP - rowsum(dO O)), dQ = scale dS K, dK = scale dS^T Q) runs as
 //   attn_bwd_dot    Dd[h][t] = sum_d dO O (fp32);
 //   attn_bwd_dq     per (sequence, query head, 128-row query tile): the forward's loop with
@@ -41,11 +42,13 @@
 // partials of their own (attn_bwd_far_kernel adds them in order: deterministic), so that no item's
 // chain is much longer than a window.
 // Operands are fp16 or, in a window, bf16 (the element type E).
-// A window's times (MI355X, 12 / 2 heads): [8192] in bf16, window 2047, 128 sinks, forward 111 us (95 GFLOP
-// of visible pairs, 860 TF/s); [4096, 3001, 2222, 1531], window 1000, 4 sinks, forward 79 us (690 TF/s),
-// backward 317 (430 TF/s; the causal kernels on whole rows: 770 and 550); 16 rows of 128..512, window 256,
-// 18 and 77 us. Bound as the causal kernels are (below); a window adds its border: a 128-row tile's
-// list of keys, and a key tile's of rows, is window + 127 long, of which half a tile at either end is masked.
+// A window's times (MI355X, 12 / 2 heads, replayed from a graph): [8192] in bf16, window 2047, 128 sinks,
+// forward 111 us (95 GFLOP of visible pairs, 860 TF/s), backward 476 (500); [4096, 3001, 2222, 1531], window
+// 1000, 4 sinks, forward 75-81 us (55 GFLOP, 670-730 TF/s), backward 340 (400 TF/s; without sinks 316; the
+// causal kernels on whole rows: 770 and 550); 16 rows of 128..512, window 256, 17 and 77 us. With the rotary
+// embedding's backward 488, 359 and 87. Bound as the causal kernels are (below); a window adds its border: a
+// 128-row tile's list of keys, and a key tile's of rows, is window + 127 long, of which half a tile at either
+// end is masked.
 #include "mfma_tile.h"
 
 #include <algorithm>
@@ -533,7 +536,7 @@ __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
       if (g16 < 3) read_v(g16 + 1, buf ^ 1);  // the next group's fly during these MFMAs
       half8_t pb;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) pb[e] = E::cvt(st[b][8 * h + e]);
+      for (int e = 0; e < 8; ++e) pb[e] = E::cvt(st[b][8 * h + e]);  // P in the operands' type, as MFMA takes it
 #pragma unroll
       for (int j = 0; j < kD / 32; ++j)
         o[j] = E::mfma(
@@ -690,7 +693,7 @@ __device__ __forceinline__ void rope_back4(float (&x)[4], float (&y)[4], const f
 // relative in fp16, its error is small (relative L2 of dq and dk against 64 bits, one row of 200 in a window
 // of 64: 2.1e-4 with fp32 throughout, 2.95e-4 with dS rounded, 3.1e-4 with both; in a window of 2, where dP
 // and Dd nearly cancel, 4.8e-4). Without it Dd would take the scores and dP once more, two of the
-// forward's products: 79 us of the 417 at the long lengths above.
+// forward's products: 79 us of the 413 (forward and backward) at the long lengths above.
 template <class E>
 __global__ __launch_bounds__(256) void attn_bwd_dot_kernel(BwdArgs a) {
   const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;  // t * Hq + h
@@ -829,7 +832,8 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
     for (int v = 0; v < 16; ++v) acc[j][v] = 0.f;
   half8_t sb[2];     // dS^T of the block in hand, packed: 16 keys each
   half4_t kt_[16];   // its K^T operands: [16-key group][column block][8-key halves]
-  // dS^T = P^T (dP^T - Dd), P^T = exp2(S^T scale log2e - lse2): value v of block b
+  // dS^T = P^T (dP^T - Dd), P^T = exp2(S^T scale log2e - lse2): value v of block b, rounded to the operands'
+  // type for the product with K^T, whose sums are fp32
   auto value = [&](int b, int v) __attribute__((always_inline)) {
     const float p = exp2_(__builtin_fmaf(st[b][v], a.scale_log2, -lse2));
     sb[v >> 3][v & 7] = E::cvt(p * (dpt[b][v] - ddr));
@@ -1108,7 +1112,8 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int par
   half8_t pb[2][2], sb[2][2];  // [block][16-row group]: P and dS, packed
   f32x4_t l4[4], d4[4];        // the block's rows' lse and Dd
   half4_t tr[16];              // transposed operands of a 16-row group: [column block][dO, Q][halves]
-  // P and dS of value v of the block (row 8 (v / 4) + 4 hh + v % 4 of it)
+  // P and dS of value v of the block (row 8 (v / 4) + 4 hh + v % 4 of it), rounded to the operands' type for
+  // their products, whose sums are fp32
   auto value = [&](int blk, int v) __attribute__((always_inline)) {
     const float p = exp2_(__builtin_fmaf(sc[v], a.scale_log2, -l4[v >> 2][v & 3]));
     pb[blk][v >> 3][v & 7] = E::cvt(p);
@@ -1705,9 +1710,9 @@ namespace {
 // 64-row steps within a CU's share of all the work (a step of dQ is two thirds of one of dK / dV; a key
 // sees on the average w - w^2 / 2 L rows, w the window, L the mean length). An item writes one partial for
 // its heads, 128 KiB a tile of keys, and loads its keys once. Backward, us, one head / so: lengths [4096,
-// 3001, 2222, 1531] with 12 / 2 heads, window 1000 351 / 317 (three heads; all six 317), 256 206 / 165
-// (six), 4096 546 / 504 (two; six 977); 16 rows of 128..512, window 256 89 / 77 (two; six 123); [2048], 1000
-// 79 (one; two 102).
+// 3001, 2222, 1531] with 12 / 2 heads, window 1000 348 / 316 (three heads; all six 315), 256 205 / 166
+// (six), 4096 508 / 490 (two; six 974); 16 rows of 128..512, window 256 88 / 77 (two; six 124); [2048], 1000
+// 73 (one; two 94).
 int window_item_heads(int64_t n_tokens, int64_t n_seqs, int64_t max_seqlen, int64_t n_q_heads, int64_t group,
                       int64_t window) {
   if (n_tokens == 0 || n_seqs == 0) return 1;

@@ -11,9 +11,15 @@
 // :188-215) with x / (1 - p) not rounded on the way: the mask clears fp16 operands exactly and the
 // factor goes on the fp32 sums.
 //
+// t and u enter their second products in fp16, like every MFMA operand: as the reference's adapters keep them
+// under autocast. Relative L2 of the gradients against 64 bits 2.9e-4, 2.1e-4 from the results' rounding alone.
+//
 // An adapter of 8960 inputs and 1536 outputs on 2048 tokens, us (MI355X): down 13.2, up 5.0; u 5.6 (the plain
 // down product on dy), backward 21.7, its sums 4.2: 50 for 124 MB that have to move (25 at 4.93 TB/s). On 1312 tokens
 // of 1536 inputs: 4.3, 3.7, 5.6, 8.2, 3.0.
+// In a packed layer (lora_down_drop, lora_bwd_drop onto the base product's dx, its sums included): q and v of 1312
+// tokens, two masks of x, down 7.6, u 5.2, backward 15.6; of 2048 tokens 7.7, 5.2, 20.3; down_proj's 8960 inputs on
+// 2048 tokens 18.5 (lora_down_drop does not split its reduction), 4.9, 31.9.
 #include "mfma_tile.h"
 #include "philox.h"
 
@@ -67,10 +73,10 @@ Divider divider(int64_t most, int64_t d) {
 
 // One thread per eight columns of a row, `first` those of the launches before. kVec: whole chunks, 16-byte
 // aligned rows. The generator, about 70 VALU instructions per chunk with 20 of them at a quarter of the rate,
-// runs beside other wavefronts' loads: the thread's own load is issued before the key's (16.8 us for bf16
-// [2048, 8960] the other way round).
-// Bound by memory: bf16 [2048, 8960] 14.2 us (5.2 TB/s; a large copy reaches 4.9), [40000, 4096] 107 (6.1);
-// fp32 [2048, 8960] 31.2 (4.7).
+// runs beside other wavefronts' loads: the thread's own load is issued before the key's (the other way round
+// bf16 [2048, 8960] took 16.8 us for 14.2).
+// Bound by memory: bf16 [2048, 8960] 13.4 us (5.5 TB/s) with four x and y in turn, 12.2 (6.0) where one pair stays
+// in the last-level cache, [40000, 4096] 107 (6.1; a large copy reaches 4.9); fp32 [2048, 8960] 31.1 (4.7), 23.9.
 template <class E, bool kVec>
 __global__ __launch_bounds__(256) void dropout_kernel(const typename E::type* __restrict__ x, int64_t ldx,
                                                       int64_t rows, int64_t cols, float factor,
@@ -144,7 +150,7 @@ constexpr int64_t kDownCus = 256;  // the chip's CUs, for plans that a size quer
 // steps round-robin, the loads of kDownBatch of them before their MFMAs. Bound by the generator: 2.3 million
 // blocks of x [2048, 8960] take the VALU about 7.6 of the 13.2 us, the 37 MB of x as long (4.93 TB/s), half
 // behind each other (not kept, no faster: two adjacent steps per wavefront; the next batch's loads
-// ahead of this one's masks). The reduction in one part: 20 us.
+// ahead of this one's masks). The reduction in one part, as talm_lora_down_drop runs it: 18.5 us.
 template <int G>
 __global__ __launch_bounds__(64 * kDownWaves) void lora_down_drop_kernel(DownArgs a) {
   __shared__ float red[kDownWaves][G][16][16 + 1];
