@@ -106,7 +106,7 @@ def mlp_takes(x, group, gate, down):
 def mlp(x, group, gate, down):
     """down(silu(gate(x)) * up(x)), gate and up adjacent projections, in three launches; None as
     `linear`."""
-    if not mlp_takes(x, group, gate, down):
+    if not group.gemv_ok(down, down + 1):
         return None
     gu = linear(x, group, gate, down)
     if gu is None:

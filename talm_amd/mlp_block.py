@@ -205,6 +205,9 @@ def mlp_block(layer, x, h, follower):
     if not ENABLED or "mlp_block" in DISABLED or "addnorm" in DISABLED or "splitk" in DISABLED \
             or not fused_mlp.SPLITK:
         return None
+    group = getattr(layer, "_solution_layer_group", None)
+    if group is not None and few_tokens.mlp_takes(h, group, GATE, DOWN):
+        return None
     norm1 = layer.post_attention_layernorm
     if not (x.is_cuda and h.is_cuda and x.dtype == torch.float32 and h.dtype == torch.float16
             and h.shape == x.shape and x.shape[-1] % 8 == 0 and x.shape[-1] <= MAX_WIDTH
@@ -214,7 +217,7 @@ def mlp_block(layer, x, h, follower):
     if "swiglu_inplace" not in ON or ("mlp_save_up" in ON and "mlp_save_up" not in DISABLED):
         return None
     group = fused_mlp.mlp_plan(layer.mlp, h)
-    if group is None or few_tokens.mlp_takes(h, group, GATE, DOWN):
+    if group is None:
         return None
     inter = group.shapes[GATE][0]
     if inter < fused_mlp.SPLITK_MIN_K or inter % 8:
