@@ -31,9 +31,10 @@
 // [152064, 1536] 28 and 42 (4.3 TB/s, 2.9). What bounds one token: a launch (1.2 us), one memory
 // round trip with the whole of W in flight, the lookups behind it (LDS and VALU 1.4 us each) and the
 // join, one after the other; many tokens: x's way through L2 and LDS, and the lookups.
-// These read one W again and again, which then lies in the caches. With the W of 28 layers in turn (650 MB in all,
-// from memory), one token / 32: q|k|v [2048, 1536] 4.0 / 6.9 us, o 3.6 / 6.5, gate|up 8.0 / 11.5, down 6.8 / 13.2; a
-// layer's four products behind each other 23.6 / 40.7, eight tokens 26.9. An adapter's sum in the store adds 0.1 to
+// These read one W again and again, which then lies in the L2. With the W of 28 layers in turn (45, 33, 400 and 200 MB:
+// from the last-level cache, gate|up's from memory), one token / 32: q|k|v [2048, 1536] 4.0 / 6.9 us, o 3.6 / 6.5,
+// gate|up 8.0 / 11.5, down 6.8 / 13.2; all of a model's products behind each other, 650 MB from memory, 23.6 / 40.7 a
+// layer, eight tokens 26.9. An adapter's sum in the store adds 0.1 to
 // 0.6 us (1.2 at gate|up of 32 tokens); its down product is a launch in front: q|k|v with q's and v's adapters 8.3
 // and 13.0 us, 9.3 and 14.0 over 28 layers.
 // Not kept: three tiles' weights ahead in registers (1 token, [17920, 1536] 8.4 us, [2048, 8192] 7.6 for 6.3); the
