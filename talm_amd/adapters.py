@@ -83,7 +83,10 @@ class AdapterCopies:
             h_off.append(size)
             size += _pad(w.numel())
         t_of = [(-1, 0)] * len(weights)
-        for pair in self.pairs:
+        # a weight's transpose has one place: of sets that share a weight the larger, first registered one's
+        for pair in sorted(self.pairs, key=len, reverse=True):
+            if any(t_of[p][0] >= 0 for p in pair):
+                continue  # copied on its own at each use after a change
             width = sum(weights[p].shape[0] for p in pair)
             col = 0
             for p in pair:
@@ -187,17 +190,29 @@ class AdapterCopies:
         else:
             if not all(self._current(pos, p) for pos, p in zip(positions, params)):
                 self.refresh(params[0].device)
-            t_off, width = self.layout[1][positions[0]]
-            if t_off >= 0 and all(self._current(pos, p) for pos, p in zip(positions, params)):
-                cols = params[0].shape[1]
+            t_off = self.layout[1][positions[0]][0]
+            if self._laid_out(positions, params) \
+                    and all(self._current(pos, p) for pos, p in zip(positions, params)):
+                cols, width = params[0].shape[1], sum(p.shape[0] for p in params)
                 return self.buffer[t_off:t_off + cols * width].view(cols, width)
+        if params[0].is_cuda and torch.cuda.is_current_stream_capturing():
+            return self._transposes(params)  # a replay makes them from the weights as they are then
         keys = tuple(_key(p) for p in params)
         hit = self.loose.get(ids)
         if hit is None or any(r() is not p for r, p in zip(hit[0], params)) or hit[1] != keys:
-            hit = (tuple(weakref.ref(p) for p in params), keys,
-                   torch.cat([p.detach() for p in params], 0).t().to(torch.float16).contiguous())
+            hit = (tuple(weakref.ref(p) for p in params), keys, self._transposes(params))
             self.loose[ids] = hit
         return hit[2]
+
+    @staticmethod
+    def _transposes(params):
+        return torch.cat([p.detach() for p in params], 0).t().to(torch.float16).contiguous()
+
+    def _laid_out(self, positions, params):
+        """Whether the weights' transposes lie side by side, in this order, in a block of their own."""
+        places, rows = [self.layout[1][pos] for pos in positions], [p.shape[0] for p in params]
+        t_off, width = places[0]
+        return t_off >= 0 and places == [(t_off + sum(rows[:i]), sum(rows)) for i in range(len(rows))]
 
 
 COPIES = AdapterCopies()

@@ -166,3 +166,70 @@ def test_fused_tail_matches_unscale_clip_step(case):
         torch.testing.assert_close(b, a, rtol=1e-6, atol=1e-9)
     for a, b in zip(v0, v1):
         torch.testing.assert_close(b, a, rtol=1e-5, atol=1e-20)
+
+
+@pytest.mark.parametrize("order", [((0, 1), (0,), (1,)), ((0,), (1,), (0, 1)), ((1,), (0, 1), (2, 0), (0,))])
+def test_a_weight_of_several_transposed_sets(order):
+    """Nodes over q and v, and over one of them (an evaluation with a cache, between training steps): each gets
+    its own weights' transposes, before and after a change, and from a captured graph."""
+    copies = adapters.AdapterCopies()
+    ws = [torch.randn(16, 96, device="cuda") for _ in range(3)]
+
+    def check(picks):
+        want = torch.cat([ws[i] for i in picks], 0).t().half()
+        got = copies.pair_t(tuple(ws[i] for i in picks))
+        assert got.shape == want.shape and torch.equal(got, want), picks
+    for _ in range(3):
+        for picks in order:
+            check(picks)
+            for i in picks:
+                assert torch.equal(copies.half(ws[i]), ws[i].half())
+        with torch.no_grad():
+            for w in ws:
+                w.mul_(0.5)
+    copies.in_place = True
+    for picks in order:
+        check(picks)
+    for picks in order:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            seen = copies.pair_t(tuple(ws[i] for i in picks)).clone()
+        for _ in range(3):
+            with torch.no_grad():
+                for w in ws:
+                    w.add_(1.0)
+            copies.refresh(ws[0].device)  # as the optimizer's step leaves the copies
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(seen, torch.cat([ws[i] for i in picks], 0).t().half()), picks
+
+
+def test_a_model_asked_for_gradients_with_a_cache_between_steps():
+    """A training step's q|k|v node reads q's and v's transposes side by side; the evaluation's projections, each a
+    node of its own, read one of them: the same copies serve both, in either order."""
+    from talm_amd import patches, qgroup, qlora_model
+
+    config = qlora_model.qwen2_config(vocab_size=1000, hidden_size=512, intermediate_size=1024, num_hidden_layers=2,
+                                      num_attention_heads=4, num_key_value_heads=2, head_dim=128)
+    model = qlora_model.build_model(config, seed=3)
+    params = qlora_model.lora_parameters(model)
+    with torch.no_grad():
+        for p in params:
+            if not p.any():
+                p.normal_(0, 0.02)
+    batch = qlora_model.make_batch(seed=5, step=0, vocab=1000, seq=128, lo=64, hi=128)
+
+    def grads(mode):
+        getattr(model, mode)()
+        with torch.autocast("cuda", dtype=torch.float16):
+            loss = model(**batch).loss
+        return torch.autograd.grad(loss * 1024, params)
+    want = {mode: grads(mode) for mode in ("train", "eval")}
+    try:
+        patches.apply()
+        for mode in ("train", "eval", "train", "eval"):
+            for got, ref in zip(grads(mode), want[mode]):
+                assert (got - ref).norm() <= 0.02 * ref.norm(), mode
+    finally:
+        patches.unapply()
+        qgroup.release()
