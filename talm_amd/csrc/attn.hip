@@ -661,6 +661,11 @@ struct BwdArgs {
   float* far_v;
 };
 
+// kWin: every row sees itself alone (as a sequence's first row does in any window). Its softmax is 1 whatever
+// the score, dS exactly 0, and so are dQ and, where all rows are such, dK. They are taken as such: dP and Dd, equal
+// then, are summed in different orders, and their difference would be rounding noise in the place of zeros.
+__device__ __forceinline__ bool one_key(const BwdArgs& a) { return a.window == 1 && a.sinks == 0; }
+
 // The query row after the tiles of 64 rows that hold the window of any of a 128-key tile's keys and, of
 // a tile with sinks, `slack` rows more: where the items of its sinks' further rows begin.
 __device__ __forceinline__ int near_end(int k0, int len, int window, int sinks, int slack) {
@@ -801,7 +806,8 @@ __device__ __forceinline__ void attn_bwd_dq(const BwdArgs& a, int seq, int head,
       df[s] = *reinterpret_cast<const half8_t*>(dp + 16 * s);
     }
   }
-  const float lse2 = a.lse2[static_cast<int64_t>(head) * a.n_tokens + s0 + qr];
+  float lse2 = a.lse2[static_cast<int64_t>(head) * a.n_tokens + s0 + qr];
+  if (kWin) lse2 = qr == 0 || one_key(a) ? INFINITY : lse2;  // P 0 here, so that dS is (one_key)
   const float ddr = a.dd[static_cast<int64_t>(head) * a.n_tokens + s0 + qr];
   const int wq0 = q0 + 32 * wave;  // the wavefront's first query row
 
@@ -1301,7 +1307,8 @@ __device__ __forceinline__ void attn_bwd_dkdv(const BwdArgs& a, int seq, int par
     // the next call overwrites the rows: every read above has returned first
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   };
-  store_rows(dka, a.scale, far ? a.far_k : a.dk_part);
+  // where every row sees one key dK is 0 (one_key): not so in the loop, whose blocks it made 2 to 4% longer
+  store_rows(dka, kWin && (len == 1 || one_key(a)) ? 0.f : a.scale, far ? a.far_k : a.dk_part);
   store_rows(dva, 1.f, far ? a.far_v : a.dv_part);
 }
 

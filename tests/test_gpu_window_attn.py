@@ -447,3 +447,45 @@ def test_gradients_against_differences_along_them(half, h, which):
     assert abs(diff - (grad * step).sum()) <= bound
     for wrong in (-grad, 2 * grad, 0 * grad, grad.roll(1, 0)):
         assert abs(diff - (wrong * step).sum()) > bound
+
+
+@pytest.mark.parametrize("half", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lengths,window,sinks", [
+    ([1] * 9, 5, 0), ([1] * 200, 5, 3), ([1, 0, 1], 1, 1),  # rows of one token
+    ([300, 65, 1], 1, 0), ([150] * 40, 1, 0),               # a window of one
+    ([1300] * 16, 1, 0),                                    # several heads an item
+])
+def test_rows_that_see_one_key_have_no_gradient_of_their_scores(lengths, window, sinks, half):
+    """A softmax over one key is 1 whatever its score: dq and dk are exactly zero, out is v, and dv the sum of
+    the group's dO (four products of 1, in fp32, rounded once)."""
+    print(f"[case] one key a row: {len(lengths)} sequences, window={window} {half}", flush=True)
+    n, hq, hkv = sum(lengths), 8, 2
+    q, k, v, dout = _inputs(n, hq, hkv, half, True, 7)
+    out, dq, dk, dv = _call(q, k, v, _cu(lengths), max(lengths), window, sinks, dout)
+    assert torch.equal(out, v.repeat_interleave(hq // hkv, 1))
+    assert not dq.any() and not dk.any()
+    want = dout.double().view(n, hkv, hq // hkv, D)
+    u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[half]
+    tol = u * want.sum(2).abs() + 4 * 2.0 ** -24 * want.abs().sum(2) + 2.0 ** -25
+    assert ((dv.double() - want.sum(2)).abs() <= tol).all()
+
+
+def test_first_rows_have_no_gradient_of_their_scores():
+    """The first row of a sequence sees itself alone, whatever the window; with and without the rotation."""
+    from talm_amd import _ops
+
+    lengths, hq, hkv = [200, 1, 77, 130], 4, 2
+    n, cu = sum(lengths), _cu(lengths)
+    q, k, v, dout = _inputs(n, hq, hkv, torch.float16, True, 8)
+    angles = torch.rand(n, D, device="cuda")
+    for window, sinks, turned in ((40, 3, False), (1000, 0, True)):
+        out, lse = torch.empty_like(dout), torch.empty(hq, n, device="cuda")
+        torch.ops.talm.attn_window_fwd(q, k, v, cu, 200, 0.1, window, sinks, out, lse)
+        dq, dk, dv = (torch.full(t.shape, 5.0, dtype=t.dtype, device="cuda") for t in (q, k, v))
+        ws = torch.empty(_ops.attn_window_bwd_workspace_bytes(n, hq, hkv, 4, 200, window, sinks), dtype=torch.uint8,
+                         device="cuda")
+        torch.ops.talm.attn_window_bwd(q, k, v, out, dout, lse, cu, 200, 0.1, window, sinks,
+                                       angles.cos() if turned else None, angles.sin() if turned else None, dq, dk, dv, ws)
+        for first in (0, 200, 201, 278):
+            assert not dq[first].any()
+        assert not dk[200].any() and dq[1].any() and dk[0].any()
