@@ -655,6 +655,36 @@ int talm_attn_window_bwd(const uint16_t* q, int64_t q_stride_tok, int64_t q_stri
                          void* stream);
 
 /*
+ * The same two calls with what out's rounding left off: out_lo [n_tokens, n_q_heads, head_dim] dense,
+ * of out's type, 16-byte aligned, is the unrounded output less out (rows behind the last sequence are
+ * left as they were). The backward then takes rowsum(dout (out + out_lo)): without it, of out alone, the
+ * gradients of q and k are off by up to twice as much where a row sees few keys. out_lo NULL: the calls
+ * above.
+ */
+int talm_attn_window_fwd_lo(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                            const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                            const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
+                            const int32_t* cu_seqlens, int32_t n_seqs, int32_t max_seqlen,
+                            int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                            int32_t head_dim, float scale, int32_t window, int32_t sinks,
+                            int32_t dtype, uint16_t* out, int64_t o_stride_tok,
+                            int64_t o_stride_head, uint16_t* out_lo, float* lse, void* stream);
+int talm_attn_window_bwd_lo(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                            const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                            const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
+                            const uint16_t* out, int64_t o_stride_tok, int64_t o_stride_head,
+                            const uint16_t* out_lo, const uint16_t* dout, int64_t do_stride_tok,
+                            int64_t do_stride_head, const float* lse, const int32_t* cu_seqlens,
+                            int32_t n_seqs, int32_t max_seqlen, int64_t n_tokens,
+                            int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, float scale,
+                            int32_t window, int32_t sinks, int32_t dtype, const float* cos,
+                            const float* sin, int64_t cs_stride, uint16_t* dq,
+                            int64_t dq_stride_tok, int64_t dq_stride_head, uint16_t* dk,
+                            int64_t dk_stride_tok, int64_t dk_stride_head, uint16_t* dv,
+                            int64_t dv_stride_tok, int64_t dv_stride_head, void* workspace,
+                            int64_t workspace_bytes, void* stream);
+
+/*
  * Dropout with a mask computed from a counter-based generator and never stored: y = x factor where
  * the element is kept, 0 elsewhere; the backward is the same call on dy. Element (r, c) of x
  * [rows, cols] (row stride ldx) has 16 random bits, halfword c % 8 of the Philox-4x32-10 block with

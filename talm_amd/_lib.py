@@ -10,7 +10,7 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libtalm.so"
-ABI_VERSION = 21
+ABI_VERSION = 22
 
 TALM_OK, TALM_EINVAL, TALM_EHIP = 0, 1, 2
 TALM_F32, TALM_F16, TALM_BF16 = 0, 1, 2
@@ -67,6 +67,12 @@ SIGNATURES = {
                              _I64, _I64, _P, _P, _I32, _I32, _I64, _I32, _I32, _I32, _F32, _I32,
                              _I32, _I32, _P, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64,
                              _I64, _P, _I64, _P],
+    "talm_attn_window_fwd_lo": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I32, _I32, _I64,
+                                _I32, _I32, _I32, _F32, _I32, _I32, _I32, _P, _I64, _I64, _P, _P, _P],
+    "talm_attn_window_bwd_lo": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P,
+                                _I64, _I64, _P, _P, _I32, _I32, _I64, _I32, _I32, _I32, _F32, _I32,
+                                _I32, _I32, _P, _P, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64,
+                                _I64, _P, _I64, _P],
     "talm_dropout": [_P, _I64, _I64, _I64, _I32, _F32, _P, _U32, _P, _I64, _P],
     "talm_lora_down_drop": [_P, _I64, _I64, _I64, _P, _P, _I32, _F32, _P, _U32, _U32, _F32, _F32, _P,
                             _P, _I64, _P],

@@ -43,12 +43,12 @@
 // chain is much longer than a window.
 // Operands are fp16 or, in a window, bf16 (the element type E).
 // A window's times (MI355X, 12 / 2 heads, replayed from a graph): [8192] in bf16, window 2047, 128 sinks,
-// forward 111 us (95 GFLOP of visible pairs, 860 TF/s), backward 476 (500); [4096, 3001, 2222, 1531], window
-// 1000, 4 sinks, forward 75-81 us (55 GFLOP, 670-730 TF/s), backward 340 (400 TF/s; without sinks 316; the
-// causal kernels on whole rows: 770 and 550); 16 rows of 128..512, window 256, 17 and 77 us. With the rotary
-// embedding's backward 488, 359 and 87. Bound as the causal kernels are (below); a window adds its border: a
-// 128-row tile's list of keys, and a key tile's of rows, is window + 127 long, of which half a tile at either
-// end is masked.
+// forward 111-115 us (95 GFLOP of visible pairs, 830-860 TF/s), backward 476 (500); [4096, 3001, 2222, 1531],
+// window 1000, 4 sinks, forward 75-78 us (55 GFLOP, 700-730 TF/s), 82 with out_lo, backward 347 (390 TF/s; the
+// causal kernels on whole rows: 770 and 550); 16 rows of 128..512, window 256, 17, 19-20 and 80 us. With the
+// rotary embedding's backward 489, 366 and 90. Bound as the causal kernels are (below); a window adds its
+// border: a 128-row tile's list of keys, and a key tile's of rows, is window + 127 long, of which half a tile
+// at either end is masked.
 #include "mfma_tile.h"
 
 #include <algorithm>
@@ -161,6 +161,8 @@ struct FwdArgs {
   float* lse;         // [Hq, n_tokens]
   int64_t n_tokens;
   int window, sinks;  // kWin: both at most the longest sequence's length, window >= 1
+  uint16_t* out_lo;   // kWin: what out's rounding left off, dense rows of lo_tok = Hq D, or null
+  int64_t lo_tok;
 };
 
 // K and V tiles of the forward in LDS: [64 keys][128 d] fp16 without padding, 16 chunks of 16
@@ -608,6 +610,35 @@ __global__ __launch_bounds__(256 * S, 2) void attn_fwd_kernel(FwdArgs a) {
     const int cc16 = it * 64 + lane, r = cc16 / (kD / 8), cc = cc16 % (kD / 8);
     store16(ors, w0 + r < row_end ? static_cast<uint32_t>((r * a.o_tok + 8 * cc) * 2) : kOob, ov[it]);
   }
+  if constexpr (kWin) {
+    if (!a.out_lo) return;
+    // the same way once more with the rounding's remainders: what Dd of the backward needs beside out
+#pragma unroll
+    for (int j = 0; j < kD / 32; ++j)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d0 = 32 * j + 8 * g + 4 * hh;
+        const float x[4] = {o[j][4 * g] * inv, o[j][4 * g + 1] * inv, o[j][4 * g + 2] * inv, o[j][4 * g + 3] * inv};
+        const uint32_t lo = E::pack(x[0], x[1]), hi = E::pack(x[2], x[3]);
+        uint2 w;
+        w.x = E::pack(x[0] - E::lo(lo), x[1] - E::hi(lo));
+        w.y = E::pack(x[2] - E::lo(hi), x[3] - E::hi(hi));
+        *reinterpret_cast<uint2*>(&os[l32 * kKS + d0]) = w;
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int it = 0; it < kOut; ++it) {
+      const int cc16 = it * 64 + lane, r = cc16 / (kD / 8), cc = cc16 % (kD / 8);
+      ov[it] = *reinterpret_cast<const u32x4*>(&os[r * kKS + 8 * cc]);
+    }
+    const __amdgpu_buffer_rsrc_t lrs =
+        store_rsrc(a.out_lo + static_cast<int64_t>(s0 + w0) * a.lo_tok + static_cast<int64_t>(head) * kD);
+#pragma unroll
+    for (int it = 0; it < kOut; ++it) {
+      const int cc16 = it * 64 + lane, r = cc16 / (kD / 8), cc = cc16 % (kD / 8);
+      store16(lrs, w0 + r < row_end ? static_cast<uint32_t>((r * a.lo_tok + 8 * cc) * 2) : kOob, ov[it]);
+    }
+  }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -622,6 +653,7 @@ struct BwdArgs {
   int64_t v_tok, v_head;
   const uint16_t* o;
   int64_t o_tok, o_head;
+  const uint16_t* o_lo;  // kWin: [n_tokens][Hq][D], what o's rounding left off, or null
   const uint16_t* dout;
   int64_t do_tok, do_head;
   const float* lse;    // [Hq, n_tokens], natural log
@@ -694,12 +726,14 @@ __device__ __forceinline__ void rope_back4(float (&x)[4], float (&y)[4], const f
 
 // Dd[h][t] = sum_d dO[t][h][d] * O[t][h][d] and lse2[h][t] = lse[h][t] log2 e (the exponent offset
 // both backward bodies subtract): 16 lanes per (token, head), 8 columns each.
-// Dd from the rounded output, the only one that is kept: beside the rounding of dS for its products, 2^-11
-// relative in fp16, its error is small (relative L2 of dq and dk against 64 bits, one row of 200 in a window
-// of 64: 2.1e-4 with fp32 throughout, 2.95e-4 with dS rounded, 3.1e-4 with both; in a window of 2, where dP
-// and Dd nearly cancel, 4.8e-4). Without it Dd would take the scores and dP once more, two of the
-// forward's products: 79 us of the 413 (forward and backward) at the long lengths above.
-template <class E>
+// kWin: with out_lo Dd is that of the unrounded output. Of the rounded one alone it would be the largest error
+// where a row sees few keys, and dP and Dd nearly cancel (relative L2 of dq and dk against 64 bits, of out alone /
+// with out_lo, in units of the type's half step 2^-11 or 2^-8: rows of 2 and 3 tokens 0.92 / 0.65, single rows of
+// two tokens up to 2.5 / 0.95; rows of 100 tokens and more 0.65 / 0.61, of which the rounding of dS for its
+// products leaves 0.6 and the result's own 0.43). It costs the forward one more store of the output's size and
+// this kernel its read: 413 -> 430 us forward and backward at the long lengths above, 94 -> 99 at the short ones.
+// The causal entries, which have no out_lo, take out as it is.
+template <class E, bool kWin>
 __global__ __launch_bounds__(256) void attn_bwd_dot_kernel(BwdArgs a) {
   const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;  // t * Hq + h
   const int sub = threadIdx.x & 15;
@@ -710,9 +744,15 @@ __global__ __launch_bounds__(256) void attn_bwd_dot_kernel(BwdArgs a) {
   const int h = static_cast<int>(r % a.n_q_heads);
   const u32x4 x = *reinterpret_cast<const u32x4*>(a.o + t * a.o_tok + h * a.o_head + 8 * sub);
   const u32x4 y = *reinterpret_cast<const u32x4*>(a.dout + t * a.do_tok + h * a.do_head + 8 * sub);
-  float acc = E::lo(x.x) * E::lo(y.x) + E::hi(x.x) * E::hi(y.x) + E::lo(x.y) * E::lo(y.y) +
-              E::hi(x.y) * E::hi(y.y) + E::lo(x.z) * E::lo(y.z) + E::hi(x.z) * E::hi(y.z) +
-              E::lo(x.w) * E::lo(y.w) + E::hi(x.w) * E::hi(y.w);
+  u32x4 z{0u, 0u, 0u, 0u};
+  if (kWin && a.o_lo) z = *reinterpret_cast<const u32x4*>(a.o_lo + r * kD + 8 * sub);
+  auto dot = [&](const u32x4& u) __attribute__((always_inline)) {
+    return E::lo(u.x) * E::lo(y.x) + E::hi(u.x) * E::hi(y.x) + E::lo(u.y) * E::lo(y.y) +
+           E::hi(u.y) * E::hi(y.y) + E::lo(u.z) * E::lo(y.z) + E::hi(u.z) * E::hi(y.z) +
+           E::lo(u.w) * E::lo(y.w) + E::hi(u.w) * E::hi(y.w);
+  };
+  float acc = dot(x);
+  if (kWin && a.o_lo) acc += dot(z);
 #pragma unroll
   for (int off = 8; off >= 1; off >>= 1) acc += __shfl_xor(acc, off, 16);
   if (sub == 0 && row < rows) {
@@ -1549,6 +1589,7 @@ namespace {
 // The arguments of a sliding window (window = 0: none, the causal entry points).
 struct Window {
   int32_t window, sinks, dtype;
+  uint16_t* out_lo = nullptr;  // what out's rounding left off (written by the forward, read by the backward)
 };
 
 // No sequence is longer than the rows, of which a window takes fewer than 2^30: the kernels' sums of a row and
@@ -1561,6 +1602,7 @@ int32_t longest_of(int32_t max_seqlen, int64_t n_tokens) {
 int check_window(const char* what, const Window& w, float scale) {
   if (w.dtype != TALM_F16 && w.dtype != TALM_BF16)
     return fail(TALM_EINVAL, "%s: dtype %d (TALM_F16 or TALM_BF16)", what, w.dtype);
+  if (!aligned(w.out_lo, 16)) return fail(TALM_EINVAL, "%s: out_lo must be 16-byte aligned", what);
   if (w.window < 1 || w.sinks < 0)
     return fail(TALM_EINVAL, "%s: window %d (at least 1), sinks %d (at least 0)", what, w.window, w.sinks);
   if (!(scale > 0.f) || !(scale < INFINITY))
@@ -1641,6 +1683,8 @@ int attn_fwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
   if (win.window) {
     a.window = std::min(win.window, max_seqlen);
     a.sinks = std::min(win.sinks, max_seqlen);
+    a.out_lo = win.out_lo;
+    a.lo_tok = static_cast<int64_t>(n_q_heads) * kD;
     // a window of any alignment behind the workgroup's rows, and the sinks' tiles
     const int64_t seen = (static_cast<int64_t>(a.window) + rows + kKeys - 2) / kKeys + 1 +
                          (a.sinks + kKeys - 1) / kKeys;
@@ -1691,7 +1735,22 @@ TALM_API int talm_attn_window_fwd(const uint16_t* q, int64_t q_stride_tok, int64
                                   int32_t head_dim, float scale, int32_t window, int32_t sinks,
                                   int32_t dtype, uint16_t* out, int64_t o_stride_tok,
                                   int64_t o_stride_head, float* lse, void* stream) {
-  const Window win{window, sinks, dtype};
+  return talm_attn_window_fwd_lo(q, q_stride_tok, q_stride_head, k, k_stride_tok, k_stride_head, v,
+                                 v_stride_tok, v_stride_head, cu_seqlens, n_seqs, max_seqlen, n_tokens,
+                                 n_q_heads, n_kv_heads, head_dim, scale, window, sinks, dtype, out,
+                                 o_stride_tok, o_stride_head, nullptr, lse, stream);
+}
+
+TALM_API int talm_attn_window_fwd_lo(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                                     const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                                     const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
+                                     const int32_t* cu_seqlens, int32_t n_seqs, int32_t max_seqlen,
+                                     int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                                     int32_t head_dim, float scale, int32_t window, int32_t sinks,
+                                     int32_t dtype, uint16_t* out, int64_t o_stride_tok,
+                                     int64_t o_stride_head, uint16_t* out_lo, float* lse,
+                                     void* stream) {
+  const Window win{window, sinks, dtype, out_lo};
   const int status = check_window("attn_window_fwd", win, scale);
   if (status != TALM_OK) return status;
   return attn_fwd_impl("attn_window_fwd", win, q, q_stride_tok, q_stride_head, k, k_stride_tok,
@@ -1781,7 +1840,7 @@ template <class E, bool kWin>
 void launch_bwd(const BwdArgs& a, int n_seqs, hipStream_t s) {
   constexpr int W = 4;
   const int64_t rows = a.n_tokens * a.n_q_heads;
-  hipLaunchKernelGGL(attn_bwd_dot_kernel<E>, dim3(static_cast<unsigned>((rows * 16 + 255) / 256)),
+  hipLaunchKernelGGL((attn_bwd_dot_kernel<E, kWin>), dim3(static_cast<unsigned>((rows * 16 + 255) / 256)),
                      dim3(256), 0, s, a);
   if (a.counter) {
     hipLaunchKernelGGL((attn_bwd_queue_kernel<E, W, kWin>), dim3(a.queue_wgs), dim3(64 * W), 0, s, a);
@@ -1890,6 +1949,7 @@ int attn_bwd_impl(const char* what, const Window& win, const uint16_t* q, int64_
   if (win.window) {
     a.window = std::min(win.window, max_seqlen);
     a.sinks = std::min(win.sinks, max_seqlen);
+    a.o_lo = win.out_lo;
     a.far_rows = static_cast<int>(far.rows);
     a.far_chunks = static_cast<int>(far.chunks);
     a.far_tiles = static_cast<int>(far.tiles);
@@ -2004,7 +2064,31 @@ TALM_API int talm_attn_window_bwd(const uint16_t* q, int64_t q_stride_tok, int64
                                   int64_t dk_stride_head, uint16_t* dv, int64_t dv_stride_tok,
                                   int64_t dv_stride_head, void* workspace, int64_t workspace_bytes,
                                   void* stream) {
-  const Window win{window, sinks, dtype};
+  return talm_attn_window_bwd_lo(q, q_stride_tok, q_stride_head, k, k_stride_tok, k_stride_head, v,
+                                 v_stride_tok, v_stride_head, out, o_stride_tok, o_stride_head, nullptr,
+                                 dout, do_stride_tok, do_stride_head, lse, cu_seqlens, n_seqs,
+                                 max_seqlen, n_tokens, n_q_heads, n_kv_heads, head_dim, scale, window,
+                                 sinks, dtype, cos, sin, cs_stride, dq, dq_stride_tok, dq_stride_head,
+                                 dk, dk_stride_tok, dk_stride_head, dv, dv_stride_tok, dv_stride_head,
+                                 workspace, workspace_bytes, stream);
+}
+
+TALM_API int talm_attn_window_bwd_lo(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                                     const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                                     const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head,
+                                     const uint16_t* out, int64_t o_stride_tok, int64_t o_stride_head,
+                                     const uint16_t* out_lo, const uint16_t* dout,
+                                     int64_t do_stride_tok, int64_t do_stride_head, const float* lse,
+                                     const int32_t* cu_seqlens, int32_t n_seqs, int32_t max_seqlen,
+                                     int64_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                                     int32_t head_dim, float scale, int32_t window, int32_t sinks,
+                                     int32_t dtype, const float* cos, const float* sin,
+                                     int64_t cs_stride, uint16_t* dq, int64_t dq_stride_tok,
+                                     int64_t dq_stride_head, uint16_t* dk, int64_t dk_stride_tok,
+                                     int64_t dk_stride_head, uint16_t* dv, int64_t dv_stride_tok,
+                                     int64_t dv_stride_head, void* workspace,
+                                     int64_t workspace_bytes, void* stream) {
+  const Window win{window, sinks, dtype, const_cast<uint16_t*>(out_lo)};
   const int status = check_window("attn_window_bwd", win, scale);
   if (status != TALM_OK) return status;
   return attn_bwd_impl("attn_window_bwd", win, q, q_stride_tok, q_stride_head, k, k_stride_tok,

@@ -710,18 +710,27 @@ void window_common(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
           "attn_window: lse float32 [Hq, N]");
 }
 
+// out's rounding error: dense, of out's shape
+void window_rest(const OptTensor& out_lo, const Tensor& out) {
+  require(!out_lo.has_value() || (out_lo->is_cuda() && out_lo->device() == out.device() &&
+                                  out_lo->scalar_type() == out.scalar_type() && out_lo->sizes() == out.sizes() &&
+                                  out_lo->is_contiguous()),
+          "attn_window: out_lo contiguous, of out's shape, type and device");
+}
+
 void attn_window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu,
                      int64_t max_seqlen, double scale, int64_t window, int64_t sinks, const Tensor& out,
-                     const Tensor& lse) {
+                     const Tensor& lse, const OptTensor& out_lo) {
   window_common(q, k, v, cu, out, lse);
+  window_rest(out_lo, out);
   const c10::DeviceGuard guard(q.device());
-  check(talm_attn_window_fwd(as<uint16_t>(q), q.stride(0), q.stride(1), as<uint16_t>(k), k.stride(0),
+  check(talm_attn_window_fwd_lo(as<uint16_t>(q), q.stride(0), q.stride(1), as<uint16_t>(k), k.stride(0),
                              k.stride(1), as<uint16_t>(v), v.stride(0), v.stride(1), as<int32_t>(cu),
                              int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_seqlen, "max_seqlen"),
                              q.size(0), int32_arg(q.size(1), "heads"), int32_arg(k.size(1), "heads"), 128,
                              static_cast<float>(scale), int32_arg(window, "window"),
                              int32_arg(sinks, "sinks"), window_dtype(q), as<uint16_t>(out), out.stride(0),
-                             out.stride(1), as<float>(lse), stream_of(q)),
+                             out.stride(1), as<uint16_t>(out_lo), as<float>(lse), stream_of(q)),
         "attn_window_fwd");
 }
 
@@ -729,8 +738,9 @@ void attn_window_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Te
                      const Tensor& dout, const Tensor& lse, const Tensor& cu, int64_t max_seqlen,
                      double scale, int64_t window, int64_t sinks, const OptTensor& cos,
                      const OptTensor& sin, const Tensor& dq, const Tensor& dk, const Tensor& dv,
-                     const Tensor& workspace) {
+                     const Tensor& workspace, const OptTensor& out_lo) {
   window_common(q, k, v, cu, out, lse);
+  window_rest(out_lo, out);
   const int64_t n = q.size(0), hq = q.size(1), hkv = k.size(1);
   window_operand(dout, q, "dout", n, hq);
   window_operand(dq, q, "dq", n, hq);
@@ -744,10 +754,10 @@ void attn_window_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Te
     cos_sin_rows(cos, sin, n, "attn_window_bwd: cos/sin fp32 [N, >= 128] with one row stride");
   }
   const c10::DeviceGuard guard(q.device());
-  check(talm_attn_window_bwd(
+  check(talm_attn_window_bwd_lo(
             as<uint16_t>(q), q.stride(0), q.stride(1), as<uint16_t>(k), k.stride(0), k.stride(1),
             as<uint16_t>(v), v.stride(0), v.stride(1), as<uint16_t>(out), out.stride(0), out.stride(1),
-            as<uint16_t>(dout), dout.stride(0), dout.stride(1), as<float>(lse), as<int32_t>(cu),
+            as<uint16_t>(out_lo), as<uint16_t>(dout), dout.stride(0), dout.stride(1), as<float>(lse), as<int32_t>(cu),
             int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_seqlen, "max_seqlen"), n,
             int32_arg(hq, "heads"), int32_arg(hkv, "heads"), 128, static_cast<float>(scale),
             int32_arg(window, "window"), int32_arg(sinks, "sinks"), window_dtype(q), as<float>(cos),
@@ -959,20 +969,22 @@ Tensor head_rows(const Tensor& t) {
 
 struct WindowAttention : torch::autograd::Function<WindowAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& query, const Tensor& key, const Tensor& value,
-                        const Tensor& cu, int64_t max_len, double scale, int64_t window, int64_t sinks) {
+                        const Tensor& cu, int64_t max_len, double scale, int64_t window, int64_t sinks, bool train) {
     const Tensor q = head_rows(query), k = head_rows(key), v = head_rows(value);
     const int64_t hq = q.size(1), n = q.size(2);
     const Tensor out = at::empty({1, n, hq, 128}, q.options());
     const Tensor lse = at::empty({hq, n}, q.options().dtype(at::kFloat));
+    const Tensor lo = train ? at::empty({n, hq, 128}, q.options()) : Tensor();
     const c10::DeviceGuard guard(q.device());
-    check(talm_attn_window_fwd(as<uint16_t>(q), q.stride(2), q.stride(1), as<uint16_t>(k), k.stride(2), k.stride(1),
+    check(talm_attn_window_fwd_lo(as<uint16_t>(q), q.stride(2), q.stride(1), as<uint16_t>(k), k.stride(2), k.stride(1),
                                as<uint16_t>(v), v.stride(2), v.stride(1), as<int32_t>(cu),
                                int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_len, "max_len"), n,
                                int32_arg(hq, "heads"), int32_arg(k.size(1), "heads"), 128, static_cast<float>(scale),
                                int32_arg(window, "window"), int32_arg(sinks, "sinks"), window_dtype(q),
-                               as<uint16_t>(out), hq * 128, 128, as<float>(lse), stream_of(q)),
+                               as<uint16_t>(out), hq * 128, 128, train ? as<uint16_t>(lo) : nullptr, as<float>(lse),
+                               stream_of(q)),
           "attn_window_fwd");
-    ctx->save_for_backward({q, k, v, out, lse, cu});
+    if (train) ctx->save_for_backward({q, k, v, out, lse, cu, lo});
     ctx->saved_data["args"] = std::vector<int64_t>{max_len, window, sinks};
     ctx->saved_data["scale"] = scale;
     return out;
@@ -980,8 +992,9 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &out = saved[3], &lse = saved[4], &cu = saved[5];
+    const Tensor& lo = saved[6];
     const std::vector<int64_t> args = ctx->saved_data["args"].toIntVector();
-    variable_list in(8);
+    variable_list in(9);
     {
       at::AutoGradMode off(false);
       const c10::DeviceGuard guard(q.device());
@@ -999,10 +1012,10 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
           talm_attn_window_bwd_workspace(n, int32_arg(hq, "heads"), int32_arg(hkv, "heads"), n_seqs, longest, window,
                                          sinks),
           q, "window_attention");
-      check(talm_attn_window_bwd(
+      check(talm_attn_window_bwd_lo(
                 as<uint16_t>(q), q.stride(2), q.stride(1), as<uint16_t>(k), k.stride(2), k.stride(1), as<uint16_t>(v),
-                v.stride(2), v.stride(1), as<uint16_t>(out), hq * 128, 128, as<uint16_t>(g), g.stride(1), g.stride(2),
-                as<float>(lse), as<int32_t>(cu), n_seqs, longest, n, static_cast<int32_t>(hq),
+                v.stride(2), v.stride(1), as<uint16_t>(out), hq * 128, 128, as<uint16_t>(lo), as<uint16_t>(g), g.stride(1),
+                g.stride(2), as<float>(lse), as<int32_t>(cu), n_seqs, longest, n, static_cast<int32_t>(hq),
                 static_cast<int32_t>(hkv), 128, static_cast<float>(ctx->saved_data["scale"].toDouble()), window, sinks,
                 window_dtype(q), nullptr, nullptr, 0, as<uint16_t>(dq), hq * 128, 128, as<uint16_t>(dk), hkv * 128,
                 128, as<uint16_t>(dv), hkv * 128, 128, ws.data_ptr(), ws.numel(), stream_of(q)),
@@ -1033,8 +1046,10 @@ Tensor window_attention(const Tensor& query, const Tensor& key, const Tensor& va
                     " (positive, finite)");
   // no sequence is longer than the rows: larger values mean the same
   const int64_t n = query.size(2);
+  const bool train =
+      at::GradMode::is_enabled() && (query.requires_grad() || key.requires_grad() || value.requires_grad());
   return WindowAttention::apply(query, key, value, cu, std::min(max_len, n), scale,
-                                std::min(window, std::max<int64_t>(n, 1)), std::min(sinks, n));
+                                std::min(window, std::max<int64_t>(n, 1)), std::min(sinks, n), train);
 }
 
 void drop_args(const Tensor& x, double p, const OptTensor& key, int64_t site) {
@@ -2042,10 +2057,10 @@ TORCH_LIBRARY(talm, m) {
         "Tensor cu_seqlens, int max_seqlen, float scale, Tensor cos, Tensor sin, Tensor(a!) dq, "
         "Tensor(b!) dk, Tensor(c!) dv, Tensor(d!) workspace) -> ()");
   m.def("attn_window_fwd(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, int max_seqlen, float scale, "
-        "int window, int sinks, Tensor(a!) out, Tensor(b!) lse) -> ()");
+        "int window, int sinks, Tensor(a!) out, Tensor(b!) lse, Tensor(c!)? out_lo=None) -> ()");
   m.def("attn_window_bwd(Tensor q, Tensor k, Tensor v, Tensor out, Tensor dout, Tensor lse, "
         "Tensor cu_seqlens, int max_seqlen, float scale, int window, int sinks, Tensor? cos, Tensor? sin, "
-        "Tensor(a!) dq, Tensor(b!) dk, Tensor(c!) dv, Tensor(d!) workspace) -> ()");
+        "Tensor(a!) dq, Tensor(b!) dk, Tensor(c!) dv, Tensor(d!) workspace, Tensor? out_lo=None) -> ()");
   m.def("dropout(Tensor x, float p, Tensor? key, int site, Tensor(a!) y) -> ()");
   m.def("lora_down_drop(Tensor x, Tensor a0, Tensor? a1, float p, Tensor? key, int site0, int site1, "
         "float scaling0, float scaling1, Tensor(a!) t, Tensor(b!) ts) -> ()");

@@ -569,15 +569,18 @@ class AttentionBlock(torch.autograd.Function):
         v = out[:, bounds[2]:].view(n_tok, n_kv, head_dim)
         o = torch.empty(n_tok, n_heads, head_dim, dtype=torch.float16, device=x.device)
         lse = torch.empty(n_heads, n_tok, dtype=torch.float32, device=x.device)
+        o_lo = None  # a window's, with a backward: what o's rounding left off
         if window is None:
             torch.ops.talm.attn_fwd(q, k, v, cu, max_len, scale, o, lse)
         else:
-            torch.ops.talm.attn_window_fwd(q, k, v, cu, max_len, scale, *window, o, lse)
+            if any(ctx.needs_input_grad):
+                o_lo = torch.empty_like(o)
+            torch.ops.talm.attn_window_fwd(q, k, v, cu, max_len, scale, *window, o, lse, o_lo)
             RAN["window_attn"] += 1
         y = torch.empty(n_tok, w_o.shape[0], dtype=torch.float16, device=x.device)
         torch.ops.talm.gemm(o.view(n_tok, -1), w_o, group.biases[O], 1, y)
         del w_o
-        saved = [x2, out, o, lse, cu]
+        saved = [x2, out, o, o_lo, lse, cu]
         for k_ in range(len(adapters)):
             saved += [t[:, 16 * k_:16 * (k_ + 1)], halves[k_][0], halves[k_][1]]
         saved += list(rope)
@@ -598,7 +601,7 @@ class AttentionBlock(torch.autograd.Function):
     def backward(ctx, grad):
         from . import _ops
 
-        x2, out, o, lse, cu, *rest = ctx.saved_tensors
+        x2, out, o, o_lo, lse, cu, *rest = ctx.saved_tensors
         cos, sin = rest[-2:]
         rest = rest[:-2]
         group, bounds = ctx.group, ctx.bounds
@@ -635,7 +638,7 @@ class AttentionBlock(torch.autograd.Function):
             fused = _rope_rows(cos, sin)
             torch.ops.talm.attn_window_bwd(q, k, v, o, d_o.view(n_tok, nh, hd), lse, cu, ctx.max_len,
                                            ctx.scale, *ctx.window, cos if fused else None,
-                                           sin if fused else None, *views)
+                                           sin if fused else None, *views, o_lo)
             grads = (dqkv,) if fused else (dq, dk, dv)
         elif _rope_rows(cos, sin):
             # the rotary backward in the attention backward's epilogues: dqkv is the q|k|v

@@ -320,7 +320,8 @@ def window_attention(query, key, value, cu, max_len, scale, window, sinks=0):
     keys (itself among them) and the sequence's first `sinks` ones, none after itself. Returns
     [1, N, Hq, 128]; gradients for query, key and value. Every operand finite. Rows that no
     sequence holds (N > cu[-1]) are not written, and get zero gradients. An autograd node of the C++
-    op layer (talm_attn_window_fwd / _bwd), differentiable once."""
+    op layer (talm_attn_window_fwd_lo / _bwd_lo: with a gradient to come the output's rounding error is
+    kept too, for rowsum(dO O)), differentiable once."""
     out = torch.ops.talm.window_attention(query, key, value, cu, max_len, scale, window, sinks)
     RAN["window_attn"] += 1
     return out

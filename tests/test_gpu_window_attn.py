@@ -489,3 +489,116 @@ def test_first_rows_have_no_gradient_of_their_scores():
         for first in (0, 200, 201, 278):
             assert not dq[first].any()
         assert not dk[200].any() and dq[1].any() and dk[0].any()
+
+
+def _forward(q, k, v, lengths, window, sinks, low=True, scale=D ** -0.5):
+    from talm_amd import _ops  # noqa: F401 - registers torch.ops.talm.*
+
+    cu = _cu(lengths)
+    out, lse = torch.empty_like(q, memory_format=torch.contiguous_format), torch.empty(q.shape[1], q.shape[0], device="cuda")
+    lo = torch.full_like(out, 9.0) if low else None
+    torch.ops.talm.attn_window_fwd(q, k, v, cu, max(lengths), scale, window, sinks, out, lse, lo)
+    return cu, out, lse, lo
+
+
+def _backward(q, k, v, out, lo, dout, lse, cu, lengths, window, sinks, scale=D ** -0.5):
+    from talm_amd import _ops
+
+    grads = [torch.empty(t.shape, dtype=t.dtype, device="cuda") for t in (q, k, v)]
+    ws = torch.empty(_ops.attn_window_bwd_workspace_bytes(q.shape[0], q.shape[1], k.shape[1], len(lengths), max(lengths),
+                                                          window, sinks), dtype=torch.uint8, device="cuda")
+    torch.ops.talm.attn_window_bwd(q, k, v, out, dout, lse, cu, max(lengths), scale, window, sinks, None, None, *grads,
+                                   ws, lo)
+    return grads
+
+
+@pytest.mark.parametrize("half", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lengths,hq,hkv", [([300, 1, 65], 12, 2), ([700], 4, 1), ([40, 64, 16], 12, 4), ([130] * 9, 7, 7)])
+def test_the_outputs_remainder(lengths, hq, hkv, half):
+    """out_lo is what out's rounding to nearest left off: at most half of out's spacing (2^-8 or 2^-11 of the power
+    of two at or below |out|, 2^-25 below fp16's normals), itself rounded once more; out is the same with and without
+    it. Rows behind the last sequence are left as they were."""
+    print(f"[case] remainder {lengths} {hq}/{hkv} {half}", flush=True)
+    n = sum(lengths)
+    q, k, v, _ = _inputs(n + 5, hq, hkv, half, True, 12)
+    _, out, lse, lo = _forward(q, k, v, lengths, 50, 3)
+    _, alone, lse2, _ = _forward(q, k, v, lengths, 50, 3, low=False)
+    assert torch.equal(out[:n], alone[:n]) and torch.equal(lse[:, :n], lse2[:, :n]) and (lo[n:] == 9).all()
+    out, lo = out[:n].double(), lo[:n].double()
+    step = torch.exp2(torch.floor(torch.log2(out.abs().clamp_min(2.0 ** -14 if half == torch.float16 else 2.0 ** -120))))
+    u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[half]
+    assert (lo.abs() <= u * step).all() and (lo != 0).double().mean() > 0.9
+    # the remainder fills its range: uniform over it, its mean square would be a third of the bound's
+    share = (lo ** 2).sum() / ((u * step) ** 2).sum()
+    assert 0.2 < share < 0.5, share
+
+
+@pytest.mark.parametrize("half", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lengths,window,sinks", [([150, 65], 40, 3), ([2] * 50, 5, 0)])
+def test_the_backward_takes_out_and_its_remainder(lengths, window, sinks, half):
+    """rowsum(dO (out + out_lo)) of the given tensors, whatever they hold: with an out_lo as large as out the
+    gradients are P (dP - that) through K and Q. dS is rounded (u), P carries the fp32 error of its score, the sums of
+    128 products 2^-17 of their magnitudes, the result is rounded (u)."""
+    print(f"[case] given remainder {lengths[:3]} {half}", flush=True)
+    hq, hkv, scale = 4, 2, D ** -0.5
+    q, k, v, dout = _inputs(sum(lengths), hq, hkv, half, False, 15)
+    cu, out, lse, _ = _forward(q, k, v, lengths, window, sinks)
+    g = torch.Generator("cuda").manual_seed(1)
+    lo = torch.randn(out.shape, generator=g, device="cuda").to(half)
+    got = _backward(q, k, v, out, lo, dout, lse, cu, lengths, window, sinks)
+    u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[half]
+    s0 = 0
+    want = [torch.zeros(t.shape, dtype=torch.float64) for t in (q, k)]
+    tols = [torch.zeros_like(t) for t in want]
+    ops = [t.cpu().double() for t in (q, k, v, dout, out, lo)]
+    for n in lengths:
+        i, rows = torch.arange(n), slice(s0, s0 + n)
+        s0 += n
+        seen = (i[None] <= i[:, None]) & ((i[:, None] - i[None] < window) | (i[None] < sinks))
+        single = seen.sum(1) == 1  # a row that sees one key has no gradient of its score
+        for h in range(hq):
+            qh, gh, oh, lh = (ops[j][rows, h] for j in (0, 3, 4, 5))
+            kh, vh = (ops[j][rows, h // 2] for j in (1, 2))
+            s = (scale * qh @ kh.T).masked_fill(~seen, -math.inf)
+            p = torch.softmax(s, -1)
+            rel = 128 * 2.0 ** -24 * (scale * qh.abs() @ kh.abs().T).max().item() + 2.0 ** -19
+            dd = (gh * (oh + lh)).sum(1, keepdim=True)
+            mag = (gh.abs() * (oh.abs() + lh.abs())).sum(1, keepdim=True) + gh.abs() @ vh.abs().T
+            ds = p * (gh @ vh.T - dd)
+            tol = ((u + 2 * rel) * ds.abs() + p * 2.0 ** -16 * mag + 2.0 ** -25) * seen
+            dq_row = torch.where(single[:, None], torch.zeros(()), ds)
+            want[0][rows, h] = scale * dq_row @ kh
+            tols[0][rows, h] = scale * tol @ kh.abs()
+            want[1][rows, h // 2] += scale * ds.T @ qh
+            tols[1][rows, h // 2] += scale * tol.T @ qh.abs()
+    for name, a, b, tol in zip(("dq", "dk"), got, want, tols):
+        worst = ((a.cpu().double() - b).abs() / (tol + u * b.abs() + 2.0 ** -25)).max().item()
+        print(f"  {name}: {worst:.3f} of its tolerance", flush=True)
+        assert worst <= 1.0, name
+
+
+@pytest.mark.parametrize("half", [torch.float16, torch.bfloat16])
+def test_gradients_of_rows_that_see_few_keys(half):
+    """Where dO V^T and rowsum(dO O) nearly cancel, the rounding of O would be the gradients' largest error: the
+    differentiable call keeps its remainder, and is nearer to 64 bits than the ops on out alone."""
+    lengths = [2, 3] * 120
+    q, k, v, dout = _inputs(sum(lengths), 8, 2, half, False, 16)
+    vals, _ = _reference(q, k, v, lengths, D ** -0.5, 9, 0, dout, half)
+    _, *near = _call(q, k, v, _cu(lengths), 3, 9, 0, dout)
+    cu, out, lse, _ = _forward(q, k, v, lengths, 9, 0, low=False)
+    far = _backward(q, k, v, out, None, dout, lse, cu, lengths, 9, 0)
+    u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[half]
+    for name, a, b, want in zip(("dq", "dk"), near, far, vals[1:]):
+        e, e_out = (((t.cpu().double() - want).norm() / want.norm()).item() for t in (a, b))
+        print(f"  {name}: {e / u:.3f} u, {e_out / u:.3f} u of out alone", flush=True)
+        assert e <= 0.85 * e_out
+
+
+def test_the_remainder_is_checked():
+    q, k, v, dout = _inputs(64, 4, 2, torch.float16, False, 2)
+    cu, out, lse, lo = _forward(q, k, v, [64], 9, 0)
+    for bad in (lo.float(), lo[:, :2], lo.transpose(0, 1).contiguous().transpose(0, 1), lo.cpu()):
+        with pytest.raises(ValueError):
+            torch.ops.talm.attn_window_fwd(q, k, v, cu, 64, 0.1, 9, 0, out, lse, bad)
+        with pytest.raises(ValueError):
+            _backward(q, k, v, out, bad, dout, lse, cu, [64], 9, 0)

@@ -284,3 +284,14 @@ def test_adapter_backward_of_no_tokens_wants_nothing_for_dx():
                               _lib.TALM_F32, 0, 32, 1.0, None, None, 0, 0, 0.0, None, None, None, None, None, 0, PTR,
                               64, PTR, 1 << 20, None)
     assert status == _lib.TALM_OK, message
+
+
+def test_window_remainder_has_to_be_aligned():
+    rows = [PTR, 256, 128]
+    status, message = _status("talm_attn_window_fwd_lo", *rows, *rows, *rows, PTR, 1, 8, 8, 2, 2, 128, 1.0, 4, 0,
+                              _lib.TALM_F16, PTR, 256, 128, PTR + 8, PTR, None)
+    assert status == _lib.TALM_EINVAL and "out_lo" in message
+    status, message = _status("talm_attn_window_bwd_lo", *rows, *rows, *rows, PTR, 256, 128, PTR + 8, *rows, PTR, PTR, 1,
+                              8, 8, 2, 2, 128, 1.0, 4, 0, _lib.TALM_F16, None, None, 0, *rows, *rows, *rows, PTR,
+                              1 << 20, None)
+    assert status == _lib.TALM_EINVAL and "out_lo" in message
