@@ -725,12 +725,12 @@ void attn_window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Te
   window_rest(out_lo, out);
   const c10::DeviceGuard guard(q.device());
   check(talm_attn_window_fwd_lo(as<uint16_t>(q), q.stride(0), q.stride(1), as<uint16_t>(k), k.stride(0),
-                             k.stride(1), as<uint16_t>(v), v.stride(0), v.stride(1), as<int32_t>(cu),
-                             int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_seqlen, "max_seqlen"),
-                             q.size(0), int32_arg(q.size(1), "heads"), int32_arg(k.size(1), "heads"), 128,
-                             static_cast<float>(scale), int32_arg(window, "window"),
-                             int32_arg(sinks, "sinks"), window_dtype(q), as<uint16_t>(out), out.stride(0),
-                             out.stride(1), as<uint16_t>(out_lo), as<float>(lse), stream_of(q)),
+                                k.stride(1), as<uint16_t>(v), v.stride(0), v.stride(1), as<int32_t>(cu),
+                                int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_seqlen, "max_seqlen"),
+                                q.size(0), int32_arg(q.size(1), "heads"), int32_arg(k.size(1), "heads"), 128,
+                                static_cast<float>(scale), int32_arg(window, "window"),
+                                int32_arg(sinks, "sinks"), window_dtype(q), as<uint16_t>(out), out.stride(0),
+                                out.stride(1), as<uint16_t>(out_lo), as<float>(lse), stream_of(q)),
         "attn_window_fwd");
 }
 
@@ -977,12 +977,12 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     const Tensor lo = train ? at::empty({n, hq, 128}, q.options()) : Tensor();
     const c10::DeviceGuard guard(q.device());
     check(talm_attn_window_fwd_lo(as<uint16_t>(q), q.stride(2), q.stride(1), as<uint16_t>(k), k.stride(2), k.stride(1),
-                               as<uint16_t>(v), v.stride(2), v.stride(1), as<int32_t>(cu),
-                               int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_len, "max_len"), n,
-                               int32_arg(hq, "heads"), int32_arg(k.size(1), "heads"), 128, static_cast<float>(scale),
-                               int32_arg(window, "window"), int32_arg(sinks, "sinks"), window_dtype(q),
-                               as<uint16_t>(out), hq * 128, 128, train ? as<uint16_t>(lo) : nullptr, as<float>(lse),
-                               stream_of(q)),
+                                  as<uint16_t>(v), v.stride(2), v.stride(1), as<int32_t>(cu),
+                                  int32_arg(cu.numel() - 1, "sequences"), int32_arg(max_len, "max_len"), n,
+                                  int32_arg(hq, "heads"), int32_arg(k.size(1), "heads"), 128, static_cast<float>(scale),
+                                  int32_arg(window, "window"), int32_arg(sinks, "sinks"), window_dtype(q),
+                                  as<uint16_t>(out), hq * 128, 128, train ? as<uint16_t>(lo) : nullptr, as<float>(lse),
+                                  stream_of(q)),
           "attn_window_fwd");
     if (train) ctx->save_for_backward({q, k, v, out, lse, cu, lo});
     ctx->saved_data["args"] = std::vector<int64_t>{max_len, window, sinks};
