@@ -758,6 +758,65 @@ int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, const uint8_
                   const uint16_t* b0, int64_t lo0, int64_t hi0, const uint16_t* b1, int64_t lo1,
                   int64_t hi1, uint16_t* out, int64_t ldo, void* stream);
 
+/*
+ * A layer's 8-bit key and value cache (no counterpart in the reference). A sequence's tokens form blocks
+ * of 64; a complete block is a page of a pool, the tokens behind the last complete block lie in 16 bits
+ * in the tail:
+ *   codes   u8  [n_pages, 2, n_kv, 64 D]  keys, then values: e4m3 codes; a page's keys in the order [tile of 16
+ *               tokens 4][64 columns D/64][quarter of them 4][token 16][column 16], its values [tile of 16
+ *               columns D/16][g 4][column 16][tile of tokens 4][r 4], token = 16 tile + 4 g + r
+ *   scales  f32 [n_pages, 2, n_kv]        a value is code * scale; scale = 2^e, the smallest with the block's
+ *               largest finite magnitude at most 448 scale (1 for zeros; e >= -100)
+ *   tail    f16 or bf16 [n_seqs, 2, n_kv, 64 D]  keys [64, D], values [D, 64]
+ *   table   i32 [n_seqs, width]           the page of each of a sequence's blocks; what is no page of the
+ *               pool holds none: writes to it are dropped, it reads as zeros and is not attended to
+ * D = head_dim, 64 or 128; dtype TALM_F16 or TALM_BF16, of the tail and every 16-bit operand.
+ * A call's new tokens are rows of packed operands: sequence b's are rows bounds[2b] .. bounds[2b + 1] - 1, the
+ * i-th of them token past[b] + i. bounds and past lie in device memory; rows outside the operands, past the
+ * first max_new of a sequence or behind its width blocks are left out (nothing of them is written). Two sequences
+ * may share complete pages. Strides in elements, multiples of 8; 16-byte aligned buffers (scales, table, bounds
+ * and past 4). Non-finite values are held as NaN in a page.
+ *
+ * talm_cache_write puts k, v [n_rows, n_kv, D] into the cache. With cos and sin (f32 [n_rows, D], row stride
+ * cs_stride, a multiple of 4; NULL both: without) the keys are turned by them first (as talm_rope does, rounded
+ * to 16 bits), and the queries q [n_rows, n_q, D] into q_out [n_rows, n_q, D] dense (n_q may be 0).
+ * It reads the open block from the tail: calls that write one sequence must be in order.
+ *
+ * talm_cache_read puts tokens past[b] + i back into k, v [n_rows, n_kv, D] dense, of a cache whose sequences
+ * hold length[b] tokens; tokens behind them read as zeros. A magnitude that a code rounded past the largest
+ * fp16 number reads as that number.
+ *
+ * talm_cache_attn: out [n_rows, n_q, D] dense, row i of sequence b = softmax(scale q K^T) V over the cached tokens
+ * j <= past[b] + i, with a window (> 0) only those with past[b] + i - j < window or j < sinks; zeros where it sees
+ * none. The cache holds the rows' own tokens already: past[b] + (rows of b) tokens in all, of which max_len at
+ * least as many. Codes enter the products exactly; the keys' scale multiplies the fp32 scores, the values' the
+ * fp32 sums. Values of tokens that a row's window leaves out must be finite. `workspace` holds
+ * talm_cache_attn_workspace bytes (-1: rejected shape). Deterministic.
+ */
+int talm_cache_write(const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,
+                     const uint16_t* v, int64_t v_stride_tok, int64_t v_stride_head, int64_t n_rows,
+                     int32_t n_kv_heads, int32_t head_dim, int32_t dtype, const int32_t* bounds,
+                     const int32_t* past, int32_t n_seqs, int32_t max_new, uint8_t* codes,
+                     float* scales, uint16_t* tail, const int32_t* table, int64_t n_pages,
+                     int32_t width, const float* cos, const float* sin, int64_t cs_stride,
+                     const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head,
+                     int32_t n_q_heads, uint16_t* q_out, void* stream);
+int talm_cache_read(const uint8_t* codes, const float* scales, const uint16_t* tail,
+                    const int32_t* table, int64_t n_pages, int32_t width, int32_t n_seqs,
+                    int32_t n_kv_heads, int32_t head_dim, int32_t dtype, const int32_t* length,
+                    const int32_t* bounds, const int32_t* past, int32_t max_new, int64_t n_rows,
+                    uint16_t* k, uint16_t* v, void* stream);
+int64_t talm_cache_attn_workspace(int64_t n_rows, int32_t n_q_heads, int32_t n_kv_heads,
+                                  int32_t head_dim, int32_t n_seqs, int32_t max_new,
+                                  int32_t max_len, int32_t window, int32_t sinks);
+int talm_cache_attn(const uint16_t* q, int64_t q_stride_tok, int64_t q_stride_head, int64_t n_rows,
+                    int32_t n_q_heads, int32_t n_kv_heads, int32_t head_dim, int32_t dtype,
+                    const int32_t* bounds, const int32_t* past, int32_t n_seqs, int32_t max_new,
+                    int32_t max_len, const uint8_t* codes, const float* scales,
+                    const uint16_t* tail, const int32_t* table, int64_t n_pages, int32_t width,
+                    float scale, int32_t window, int32_t sinks, uint16_t* out, void* workspace,
+                    int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

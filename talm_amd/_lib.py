@@ -10,7 +10,7 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libtalm.so"
-ABI_VERSION = 22
+ABI_VERSION = 23
 
 TALM_OK, TALM_EINVAL, TALM_EHIP = 0, 1, 2
 TALM_F32, TALM_F16, TALM_BF16 = 0, 1, 2
@@ -83,6 +83,12 @@ SIGNATURES = {
                            _I64, _P, _I64, _P, _I64, _P],
     "talm_nf4_gemv": [_P, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _P, _P, _I64, _P,
                       _I64, _I64, _P, _I64, _I64, _P, _I64, _P],
+    "talm_cache_write": [_P, _I64, _I64, _P, _I64, _I64, _I64, _I32, _I32, _I32, _P, _P, _I32, _I32, _P,
+                         _P, _P, _P, _I64, _I32, _P, _P, _I64, _P, _I64, _I64, _I32, _P, _P],
+    "talm_cache_read": [_P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _P, _P, _I32, _I64, _P, _P,
+                        _P],
+    "talm_cache_attn": [_P, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _P, _P, _I32, _I32, _I32, _P, _P, _P,
+                        _P, _I64, _I32, _F32, _I32, _I32, _P, _P, _I64, _P],
     "talm_lora_mirror": [_P, _I32, _I64, _P, _P],
     "talm_rope_table": [_P, _I64, _P, _I32, _F32, _P, _P, _P],
     "talm_pack_rows": [_P, _P, _P, _I32, _I32, _I64, _P, _P, _P, _P, _P, _P],
@@ -113,6 +119,7 @@ SIZE_FUNCTIONS = {
     "talm_attn_window_bwd_workspace": [_I64, _I32, _I32, _I32, _I32, _I32, _I32],
     "talm_lora_branch_fwd_workspace": [_I64, _I64],
     "talm_lora_bwd_drop_workspace": [_I64, _I64, _I32, _I64, _I64],
+    "talm_cache_attn_workspace": [_I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32],
     "talm_gemm_splitk_workspace": [_I64, _I64, _I64],
     "talm_nf4_gemm_workspace": [_I64, _I64, _I64, _I32],
     "talm_gemm_splitk_parts": [_I64, _I64, _I64],

@@ -1052,6 +1052,161 @@ Tensor window_attention(const Tensor& query, const Tensor& key, const Tensor& va
                                 std::min(window, std::max<int64_t>(n, 1)), std::min(sinks, n), train);
 }
 
+// ------------------------------------------------------------------------------------------
+// The 8-bit key and value cache. Functional forms that allocate their outputs and workspaces here: a
+// step's calls are short, and each allocation from Python costs the host as much as one of them.
+// ------------------------------------------------------------------------------------------
+struct CacheSizes {
+  int64_t pages, kv, dim, seqs, width;
+};
+
+CacheSizes cache_buffers(const Tensor& codes, const Tensor& scales, const Tensor& tail, const Tensor& table) {
+  require(codes.is_cuda() && codes.scalar_type() == at::kFloat8_e4m3fn && codes.dim() == 4 && codes.size(1) == 2 &&
+              codes.is_contiguous() && (codes.size(3) == 64 * 64 || codes.size(3) == 64 * 128),
+          "cache: codes float8_e4m3fn [pages, 2, Hkv, 64 D] on the GPU, contiguous, D 64 or 128");
+  require(scales.device() == codes.device() && scales.scalar_type() == at::kFloat && scales.is_contiguous() &&
+              scales.dim() == 3 && scales.size(0) == codes.size(0) && scales.size(1) == 2 &&
+              scales.size(2) == codes.size(2),
+          "cache: scales float32 [pages, 2, Hkv] on the codes' device, contiguous");
+  require(tail.device() == codes.device() &&
+              (tail.scalar_type() == at::kHalf || tail.scalar_type() == at::kBFloat16) && tail.is_contiguous() &&
+              tail.dim() == 4 && tail.size(1) == 2 && tail.size(2) == codes.size(2) && tail.size(3) == codes.size(3),
+          "cache: tail float16 or bfloat16 [sequences, 2, Hkv, 64 D] on the codes' device, contiguous");
+  require(table.device() == codes.device() && table.scalar_type() == at::kInt && table.is_contiguous() &&
+              table.dim() == 2 && table.size(0) == tail.size(0),
+          "cache: table int32 [sequences, width] on the codes' device, contiguous");
+  return CacheSizes{codes.size(0), codes.size(2), codes.size(3) / 64, tail.size(0), table.size(1)};
+}
+
+void cache_spans(const Tensor& bounds, const Tensor& past, int64_t seqs, const Tensor& like) {
+  require(bounds.device() == like.device() && bounds.scalar_type() == at::kInt && bounds.is_contiguous() &&
+              bounds.dim() == 2 && bounds.size(0) == seqs && bounds.size(1) == 2,
+          "cache: bounds int32 [sequences, 2] on the cache's device, contiguous");
+  require(past.device() == like.device() && past.scalar_type() == at::kInt && past.is_contiguous() &&
+              past.dim() == 1 && past.size(0) == seqs,
+          "cache: past int32 [sequences] on the cache's device");
+}
+
+// [1, H, N, D] rows of the cache's type, read where they lie if their strides suit the kernels.
+Tensor cache_rows(const Tensor& t, const Tensor& tail, int64_t dim, const char* what) {
+  TORCH_CHECK_VALUE(t.device() == tail.device() && t.scalar_type() == tail.scalar_type() && t.dim() == 4 &&
+                        t.size(0) == 1 && t.size(3) == dim,
+                    "cache: ", what, " must be [1, H, N, ", dim, "] of the tail's type on the cache's device");
+  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()), "cache: ", what,
+                    " requires a gradient, and the cache's operators have none: call them without autograd");
+  return head_rows(t);
+}
+
+int64_t cache_count(int64_t n, const char* what) {
+  TORCH_CHECK_VALUE(n >= 0 && n <= (int64_t{1} << 30), "cache: ", what, " ", n, " (0 to 2^30)");
+  return n;
+}
+
+// key, value [1, Hkv, N, D]; returns the turned query [1, Hq, N, D], if there is one.
+OptTensor cache_write(const Tensor& key, const Tensor& value, const Tensor& bounds, const Tensor& past,
+                      int64_t max_new, const Tensor& codes, const Tensor& scales, const Tensor& tail,
+                      const Tensor& table, const OptTensor& query, const OptTensor& cos, const OptTensor& sin) {
+  const CacheSizes c = cache_buffers(codes, scales, tail, table);
+  cache_spans(bounds, past, c.seqs, codes);
+  const Tensor k = cache_rows(key, tail, c.dim, "key"), v = cache_rows(value, tail, c.dim, "value");
+  const int64_t n = k.size(2);
+  require(k.size(1) == c.kv && v.size(1) == c.kv && v.size(2) == n, "cache_write: key and value [1, Hkv, N, D]");
+  require(cos.has_value() == sin.has_value() && (cos.has_value() || !query.has_value()),
+          "cache_write: cos and sin both or neither, a query only with them");
+  Tensor cs, sn, q, q_out;
+  if (cos.has_value()) {
+    auto rows = [&](const Tensor& t) {
+      require(t.device() == codes.device() && t.scalar_type() == at::kFloat && same_shape(t, n, c.dim),
+              "cache_write: cos and sin float32 [N, D] on the cache's device");
+      return t;
+    };
+    cs = rows(*cos);
+    sn = rows(*sin);
+    auto good = [&](const Tensor& t) {
+      return t.stride(1) == 1 && t.stride(0) >= c.dim && t.stride(0) % 4 == 0 &&
+             reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+    };
+    if (!good(cs) || !good(sn) || cs.stride(0) != sn.stride(0)) {
+      cs = cs.clone(at::MemoryFormat::Contiguous);
+      sn = sn.clone(at::MemoryFormat::Contiguous);
+    }
+  }
+  const c10::DeviceGuard guard(codes.device());
+  int64_t hq = 0;
+  if (query.has_value()) {
+    q = cache_rows(*query, tail, c.dim, "query");
+    hq = q.size(1);
+    require(q.size(2) == n, "cache_write: query [1, Hq, N, D] of as many rows as the key");
+    q_out = at::empty_strided({1, hq, n, c.dim}, {n * hq * c.dim, c.dim, hq * c.dim, 1}, q.options());
+  }
+  const bool turn = cs.defined(), ask = q.defined();
+  if (n == 0) return ask ? OptTensor(q_out) : std::nullopt;
+  check(talm_cache_write(as<uint16_t>(k), k.stride(2), k.stride(1), as<uint16_t>(v), v.stride(2), v.stride(1), n,
+                         int32_arg(c.kv, "heads"), static_cast<int32_t>(c.dim), window_dtype(tail),
+                         as<int32_t>(bounds), as<int32_t>(past), int32_arg(c.seqs, "sequences"),
+                         static_cast<int32_t>(cache_count(max_new, "max_new")), static_cast<uint8_t*>(codes.data_ptr()),
+                         as<float>(scales), as<uint16_t>(tail), as<int32_t>(table), c.pages,
+                         int32_arg(c.width, "table width"), turn ? as<float>(cs) : nullptr,
+                         turn ? as<float>(sn) : nullptr, turn ? cs.stride(0) : 0, ask ? as<uint16_t>(q) : nullptr,
+                         ask ? q.stride(2) : 0, ask ? q.stride(1) : 0, int32_arg(hq, "heads"),
+                         ask ? as<uint16_t>(q_out) : nullptr, stream_of(codes)),
+        "cache_write");
+  return ask ? OptTensor(q_out) : std::nullopt;
+}
+
+void cache_read(const Tensor& codes, const Tensor& scales, const Tensor& tail, const Tensor& table,
+                const Tensor& length, const Tensor& bounds, const Tensor& past, int64_t max_new, const Tensor& key,
+                const Tensor& value) {
+  const CacheSizes c = cache_buffers(codes, scales, tail, table);
+  cache_spans(bounds, past, c.seqs, codes);
+  require(length.device() == codes.device() && length.scalar_type() == at::kInt && length.is_contiguous() &&
+              length.dim() == 1 && length.size(0) == c.seqs,
+          "cache_read: length int32 [sequences] on the cache's device");
+  for (const Tensor* t : {&key, &value})
+    require(t->device() == codes.device() && t->scalar_type() == tail.scalar_type() && t->is_contiguous() &&
+                t->dim() == 3 && t->size(0) == key.size(0) && t->size(1) == c.kv && t->size(2) == c.dim,
+            "cache_read: key and value [N, Hkv, D] of the tail's type on the cache's device, contiguous");
+  const c10::DeviceGuard guard(codes.device());
+  check(talm_cache_read(static_cast<const uint8_t*>(codes.data_ptr()), as<float>(scales), as<uint16_t>(tail),
+                        as<int32_t>(table), c.pages, int32_arg(c.width, "table width"), int32_arg(c.seqs, "sequences"),
+                        int32_arg(c.kv, "heads"), static_cast<int32_t>(c.dim), window_dtype(tail), as<int32_t>(length),
+                        as<int32_t>(bounds), as<int32_t>(past), static_cast<int32_t>(cache_count(max_new, "max_new")),
+                        key.size(0), as<uint16_t>(key), as<uint16_t>(value), stream_of(codes)),
+        "cache_read");
+}
+
+// query [1, Hq, N, D]; returns [1, N, Hq, D].
+Tensor cache_attention(const Tensor& query, const Tensor& bounds, const Tensor& past, int64_t max_new, int64_t max_len,
+                       const Tensor& codes, const Tensor& scales, const Tensor& tail, const Tensor& table,
+                       double scale, int64_t window, int64_t sinks) {
+  const CacheSizes c = cache_buffers(codes, scales, tail, table);
+  cache_spans(bounds, past, c.seqs, codes);
+  const Tensor q = cache_rows(query, tail, c.dim, "query");
+  const int64_t hq = q.size(1), n = q.size(2);
+  require(hq > 0 && c.kv > 0 && hq % c.kv == 0, "cache_attention: query heads a multiple of the KV heads");
+  TORCH_CHECK_VALUE(window >= 0 && sinks >= 0, "cache_attention: window ", window, " and sinks ", sinks,
+                    " not negative");
+  // no sequence is longer than the table's blocks: larger values mean the same
+  const int64_t most = std::min(cache_count(max_len, "max_len"), c.width * 64);
+  window = window >= most ? 0 : window;
+  sinks = window ? std::min(sinks, most) : 0;
+  const int32_t heads = int32_arg(hq, "heads"), kv = int32_arg(c.kv, "heads"), dim = static_cast<int32_t>(c.dim),
+                seqs = int32_arg(c.seqs, "sequences"),
+                rows = static_cast<int32_t>(cache_count(max_new, "max_new")),
+                len = int32_arg(most, "max_len"), win = static_cast<int32_t>(window), snk = static_cast<int32_t>(sinks);
+  const c10::DeviceGuard guard(codes.device());
+  const Tensor out = at::empty({1, n, hq, c.dim}, q.options());
+  const int64_t bytes = talm_cache_attn_workspace(n, heads, kv, dim, seqs, rows, len, win, snk);
+  const Tensor ws = bytes ? byte_workspace(bytes, q, "cache_attention") : Tensor();
+  check(talm_cache_attn(as<uint16_t>(q), q.stride(2), q.stride(1), n, heads, kv, dim, window_dtype(tail),
+                        as<int32_t>(bounds), as<int32_t>(past), seqs, rows, len,
+                        static_cast<const uint8_t*>(codes.data_ptr()), as<float>(scales), as<uint16_t>(tail),
+                        as<int32_t>(table), c.pages, int32_arg(c.width, "table width"), static_cast<float>(scale), win,
+                        snk, as<uint16_t>(out), bytes ? ws.data_ptr() : nullptr, bytes, stream_of(codes)),
+        "cache_attn");
+  return out;
+}
+
 void drop_args(const Tensor& x, double p, const OptTensor& key, int64_t site) {
   TORCH_CHECK_VALUE(p >= 0.0 && p < 1.0, "dropout: p ", p, " (0 <= p < 1)");
   require(key.has_value() || p == 0.0, "dropout: a key is needed (draw_key)");
@@ -2102,6 +2257,13 @@ TORCH_LIBRARY(talm, m) {
         "Tensor? ds, Tensor(a!) dx, Tensor(b!) dbranch) -> ()");
   m.def("window_attention(Tensor query, Tensor key, Tensor value, Tensor cu, int max_len, float scale, "
         "int window, int sinks) -> Tensor", &window_attention);
+  m.def("cache_write(Tensor key, Tensor value, Tensor bounds, Tensor past, int max_new, Tensor(a!) codes, "
+        "Tensor(b!) scales, Tensor(c!) tail, Tensor table, Tensor? query, Tensor? cos, Tensor? sin) -> Tensor?",
+        &cache_write);
+  m.def("cache_read(Tensor codes, Tensor scales, Tensor tail, Tensor table, Tensor length, Tensor bounds, "
+        "Tensor past, int max_new, Tensor(a!) key, Tensor(b!) value) -> ()", &cache_read);
+  m.def("cache_attention(Tensor query, Tensor bounds, Tensor past, int max_new, int max_len, Tensor codes, "
+        "Tensor scales, Tensor tail, Tensor table, float scale, int window, int sinks) -> Tensor", &cache_attention);
   m.def("counter_dropout(Tensor x, float p, Tensor? key, int site) -> Tensor", &counter_dropout);
   m.def("adapter_branch(Tensor x, Tensor lora_a, Tensor lora_b, Tensor a_half, Tensor b_half, float scaling, "
         "float p, Tensor? key, int site) -> Tensor", &adapter_branch);
