@@ -18,6 +18,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -433,109 +434,33 @@ struct Visits {
   __device__ __forceinline__ int page(int i) const { return i < sinks ? i : i - sinks + first; }
 };
 
-__device__ __forceinline__ float rows_max(float x) {  // over the lanes of one query column
-  x = fmaxf(x, __shfl_xor(x, 16, kWave));
-  return fmaxf(x, __shfl_xor(x, 32, kWave));
+// Over the four lanes of one query column, 16 apart.
+__device__ __forceinline__ float rows_max(float x) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+  const uint32_t w = __builtin_bit_cast(uint32_t, x);
+  const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(q[0])), __builtin_bit_cast(float, static_cast<uint32_t>(q[1])));
 }
 __device__ __forceinline__ float rows_sum(float x) {
   x += __shfl_xor(x, 16, kWave);
   return x + __shfl_xor(x, 32, kWave);
 }
 
-// A workgroup: 16 (token, head) rows of one sequence and KV head against one part of its pages, a
-// page per wavefront at a time, each with its own running maximum and sum; joined through LDS.
-template <class T, int D>
-__global__ __launch_bounds__(kThreads) void cache_attn_kernel(AttnArgs a) {
-  constexpr int kC = D / 64, kN = D / 16, kPitch = D + 4;
-  __shared__ float part[kWaves][16][kPitch];
-  __shared__ float stat[2][kWaves][16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid / kWave, col = lane & 15, g = lane >> 4;
-  const int split = static_cast<int>(blockIdx.x % a.splits);
-  int rest = static_cast<int>(blockIdx.x / a.splits);
-  const int tile = rest % a.tiles;
-  rest /= a.tiles;
-  const int head = rest % a.c.kv, seq = rest / a.c.kv;
-  const Span s = span_of(a.bounds, a.past, seq, a.n_rows, a.max_new, a.max_len);
-  const int rows = s.n * a.group, r0 = tile * 16;
-  if (r0 >= rows) return;
-  const int len = s.past + s.n;
-  const int row = min(r0 + col, rows - 1);  // the columns behind the last row repeat it
-  const int at = row / a.group, place = s.past + at;
-  const int lo_place = s.past + r0 / a.group, hi_place = s.past + min(r0 + 15, rows - 1) / a.group;
-  const Visits visits(lo_place, hi_place, a.window, a.sinks);
-  const int begin = split * a.per, end = min(visits.count, begin + a.per);
-  if (begin >= end) return;
-  const int qh = head * a.group + row % a.group;
-
-  half8 q[kC][2];
-  {
-    const uint16_t* p = a.q + (s.row0 + at) * a.q_tok + qh * a.q_head + g * 16;
-#pragma unroll
-    for (int c = 0; c < kC; ++c)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) q[c][h] = *reinterpret_cast<const half8*>(p + c * 64 + h * 8);
-  }
-  f32x4 acc[kN];
-#pragma unroll
-  for (int n = 0; n < kN; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+// The 16 scores of a lane (tokens first + 16 t + 4 g + r) become weights exp2(c s - m) of a running
+// maximum m; returns what the sums so far are multiplied by. kMask: tokens that the row does not see.
+struct Softmax {
   float m = -__builtin_inff(), l = 0.f;
-
-  for (int i = begin + wave; i < end; i += kWaves) {
-    const int block = visits.page(i);
-    const bool whole = block < len / kBlock;
-    const int64_t page = whole ? a.c.page(seq, block) : 0;
-    if (page < 0) continue;  // no page: nothing to see
-    f32x4 st[4];
-    u32x4 vw[kN];
-    float k_scale = 1.f, v_scale = 1.f;
-    const uint16_t* tail = a.c.tail + (static_cast<int64_t>(seq) * 2 * a.c.kv + head) * (kBlock * D);
-    if (whole) {
-      const int64_t kp = page * 2 * a.c.kv + head, vp = kp + a.c.kv;
-      const u32x4* ks = reinterpret_cast<const u32x4*>(a.c.codes + kp * (kBlock * D));
-      const u32x4* vs = reinterpret_cast<const u32x4*>(a.c.codes + vp * (kBlock * D));
-      u32x4 kw[4 * kC];
-#pragma unroll
-      for (int t = 0; t < 4 * kC; ++t) kw[t] = ks[t * kWave + lane];
-#pragma unroll
-      for (int n = 0; n < kN; ++n) vw[n] = vs[n * kWave + lane];
-      k_scale = a.c.scales[kp];
-      v_scale = a.c.scales[vp];
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < kC; ++c) {
-          const u32x4 w = kw[t * kC + c];
-          st[t] = T::mfma(T::codes(u32x2{w.x, w.y}), q[c][0], st[t]);
-          st[t] = T::mfma(T::codes(u32x2{w.z, w.w}), q[c][1], st[t]);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < kC; ++c)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const half8 w =
-                *reinterpret_cast<const half8*>(tail + (t * 16 + col) * D + c * 64 + g * 16 + h * 8);
-            st[t] = T::mfma(w, q[c][h], st[t]);
-          }
-      }
-    }
-    const float c = a.scale_log2 * k_scale;
-    const int first = block * kBlock;
-    // every key of the page seen by every row?
-    const bool all = first + kBlock - 1 <= lo_place &&
-                     (a.window == 0 || hi_place - first < a.window || first + kBlock <= a.sinks);
-    if (!all) {
+  __device__ __forceinline__ float step(f32x4 (&st)[4], float c, bool mask, int first, int g, int place, int window,
+                                        int sinks) {
+    if (mask) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int key = first + t * 16 + g * 4 + r;
-          const bool seen = key <= place && (a.window == 0 || place - key < a.window || key < a.sinks);
+          const bool seen = key <= place && (window == 0 || place - key < window || key < sinks);
           st[t][r] = seen ? st[t][r] : -__builtin_inff();
         }
     }
@@ -558,10 +483,110 @@ __global__ __launch_bounds__(kThreads) void cache_attn_kernel(AttnArgs a) {
         sum += st[t][r];
       }
     l = l * alpha + sum;
-    // P in fp16 whatever the operands' type: the values' codes are exact in it (the tail of a
-    // bfloat16 cache takes P as two bfloat16 parts). The error is that of a rounding to 11 bits,
-    // below the output's own.
-    if (whole) {
+    return alpha;
+  }
+};
+
+// A workgroup: 16 (token, head) rows of one sequence and KV head against one part of its pages, a
+// page per wavefront at a time, each with its own running maximum and sum; joined through LDS.
+template <class T, int D>
+__global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(AttnArgs a) {
+  constexpr int kC = D / 64, kN = D / 16, kPitch = D + 4;
+  __shared__ float part[kWaves][16][kPitch];
+  __shared__ float stat[2][kWaves][16];
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int split = static_cast<int>(blockIdx.x % a.splits);
+  int rest = static_cast<int>(blockIdx.x / a.splits);
+  const int tile = rest % a.tiles;
+  rest /= a.tiles;
+  const int head = rest % a.c.kv, seq = rest / a.c.kv;
+  const Span s = span_of(a.bounds, a.past, seq, a.n_rows, a.max_new, a.max_len);
+  const int rows = s.n * a.group, r0 = tile * 16;
+  if (r0 >= rows) return;
+  const int len = s.past + s.n;
+  const int row = min(r0 + col, rows - 1);  // the columns behind the last row repeat it
+  const int at = row / a.group, place = s.past + at;
+  const int lo_place = s.past + r0 / a.group, hi_place = s.past + min(r0 + 15, rows - 1) / a.group;
+  const Visits visits(lo_place, hi_place, a.window, a.sinks);
+  const int begin = split * a.per, end = min(visits.count, begin + a.per);
+  if (begin >= end) return;
+  const int qh = head * a.group + row % a.group;
+  // the last visit is the open block, whose tokens are in the tail, where the rows reach it
+  const bool open = hi_place / kBlock == len / kBlock;
+  const int code_end = a.c.n_pages > 0 ? min(end, visits.count - (open ? 1 : 0)) : begin;
+
+  half8 q[kC][2];
+  {
+    const uint16_t* p = a.q + (s.row0 + at) * a.q_tok + qh * a.q_head + g * 16;
+#pragma unroll
+    for (int c = 0; c < kC; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) q[c][h] = *reinterpret_cast<const half8*>(p + c * 64 + h * 8);
+  }
+  f32x4 acc[kN];
+#pragma unroll
+  for (int n = 0; n < kN; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Softmax soft;
+  u32x4 kw[4 * kC], vw[kN];
+  auto load_k = [&](int page) {
+    const u32x4* src = reinterpret_cast<const u32x4*>(
+                           a.c.codes + (static_cast<int64_t>(page) * 2 * a.c.kv + head) * (kBlock * D)) + lane;
+#pragma unroll
+    for (int t = 0; t < 4 * kC; ++t) kw[t] = __builtin_nontemporal_load(src + t * kWave);
+  };
+  auto load_v = [&](int page) {
+    const u32x4* src = reinterpret_cast<const u32x4*>(
+                           a.c.codes + ((static_cast<int64_t>(page) * 2 + 1) * a.c.kv + head) * (kBlock * D)) + lane;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) vw[n] = __builtin_nontemporal_load(src + n * kWave);
+  };
+
+  // 64 of the wavefront's pages at a time: lane l holds the l-th one's place and scales
+  for (int base = begin + wave; base < code_end; base += kWaves * kWave) {
+    const int mine = base + kWaves * lane;
+    int page_l = -1;
+    float ks_l = 1.f, vs_l = 1.f;
+    if (mine < code_end) {
+      page_l = static_cast<int>(a.c.page(seq, visits.page(mine)));
+      if (page_l >= 0) {
+        ks_l = a.c.scales[static_cast<int64_t>(page_l) * 2 * a.c.kv + head];
+        vs_l = a.c.scales[(static_cast<int64_t>(page_l) * 2 + 1) * a.c.kv + head];
+      }
+    }
+    const int count = min((code_end - base + kWaves - 1) / kWaves, kWave);
+    // what is no page is read as the pool's first one and seen by no row
+    int page = __builtin_amdgcn_readlane(page_l, 0);
+    load_k(max(page, 0));
+    load_v(max(page, 0));
+    auto step = [&](int i, auto more) {
+      const float k_scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks_l), i));
+      const float v_scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs_l), i));
+      const int next = decltype(more)::value ? __builtin_amdgcn_readlane(page_l, i + 1) : 0;
+      f32x4 st[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < kC; ++c) {
+          const u32x4 w = kw[t * kC + c];
+          st[t] = T::mfma(T::codes(u32x2{w.x, w.y}), q[c][0], st[t]);
+          st[t] = T::mfma(T::codes(u32x2{w.z, w.w}), q[c][1], st[t]);
+        }
+      }
+      // the next page's keys are on their way while this one's weights and values are worked on, its
+      // values during the next one's scores (the last page is a copy of its own without them: a
+      // condition here would make every wait one for all loads)
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (decltype(more)::value) load_k(max(next, 0));
+      __builtin_amdgcn_sched_barrier(0);
+      const int first = visits.page(base + kWaves * i) * kBlock;
+      const bool all = page >= 0 && first + kBlock - 1 <= lo_place &&
+                       (a.window == 0 || hi_place - first < a.window || first + kBlock <= a.sinks);
+      const float alpha = soft.step(st, a.scale_log2 * k_scale, !all, page >= 0 ? first : 0x7fff0000, g, place,
+                                    a.window, a.sinks);
+      // P in fp16 whatever the operands' type: the values' codes are exact in it. The error is that of
+      // a rounding to 11 bits, below the output's own.
       half8 p[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -570,6 +595,10 @@ __global__ __launch_bounds__(kThreads) void cache_attn_kernel(AttnArgs a) {
           p[u][r] = static_cast<_Float16>(st[2 * u][r]);
           p[u][4 + r] = static_cast<_Float16>(st[2 * u + 1][r]);
         }
+      if (page < 0) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) vw[n] = u32x4{0, 0, 0, 0};
+      }
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -577,41 +606,69 @@ __global__ __launch_bounds__(kThreads) void cache_attn_kernel(AttnArgs a) {
         o = F16::mfma(F16::codes(u32x2{vw[n].z, vw[n].w}), p[1], o);
         // the scale of the page's values in fp32: it may be past what fp16 holds
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[n][r] = __builtin_fmaf(acc[n][r], alpha, o[r] * v_scale);
+        for (int r = 0; r < 4; ++r) acc[n][r] = __builtin_fmaf(o[r], v_scale, acc[n][r] * alpha);
       }
-    } else {
-      const uint16_t* tv = tail + static_cast<int64_t>(a.c.kv) * (kBlock * D);
-      const int left = len - first;  // tokens in the tail; what lies behind them is no value
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (decltype(more)::value) load_v(max(next, 0));
+      __builtin_amdgcn_sched_barrier(0);
+      page = next;
+    };
+    for (int i = 0; i < count - 1; ++i) step(i, std::true_type{});
+    step(count - 1, std::false_type{});
+  }
+
+  // the tail, by the wavefront whose turn it is
+  if (open && visits.count - 1 >= begin && visits.count - 1 < end && (visits.count - 1 - begin) % kWaves == wave) {
+    const uint16_t* tk = a.c.tail + (static_cast<int64_t>(seq) * 2 * a.c.kv + head) * (kBlock * D);
+    const uint16_t* tv = tk + static_cast<int64_t>(a.c.kv) * (kBlock * D);
+    const int first = len / kBlock * kBlock, left = len - first;
+    f32x4 st[4];
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
+    for (int t = 0; t < 4; ++t) {
+      st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[n][r] *= alpha;
+      for (int c = 0; c < kC; ++c)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint64_t w[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int t = (2 * u + e) * 16 + g * 4, there = min(max(left - t, 0), 4);
-            w[e] = *reinterpret_cast<const uint64_t*>(tv + (n * 16 + col) * kBlock + t);
-            w[e] &= there == 4 ? ~uint64_t{0} : (uint64_t{1} << (16 * there)) - 1;
-          }
-          struct Two { uint64_t x, y; };
-          const half8 v = __builtin_bit_cast(half8, Two{w[0], w[1]});
-          half8 hi, lo;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float x = st[2 * u + e / 4][e % 4];
-            const uint16_t b = T::down(x);
-            hi[e] = __builtin_bit_cast(_Float16, b);
-            lo[e] = __builtin_bit_cast(_Float16, T::down(x - T::up(b)));
-          }
-          acc[n] = T::mfma(v, hi, acc[n]);
-          if constexpr (__is_same(T, BF16)) acc[n] = T::mfma(v, lo, acc[n]);
+        for (int h = 0; h < 2; ++h) {
+          const half8 w = *reinterpret_cast<const half8*>(tk + (t * 16 + col) * D + c * 64 + g * 16 + h * 8);
+          st[t] = T::mfma(w, q[c][h], st[t]);
         }
+    }
+    const float alpha = soft.step(st, a.scale_log2, true, first, g, place, a.window, a.sinks);
+    // the weights in the tail's type; for bfloat16 as two parts, so that they keep 16 bits
+    half8 hi[2], lo[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = st[2 * u + e / 4][e % 4];
+        const uint16_t b = T::down(x);
+        hi[u][e] = __builtin_bit_cast(_Float16, b);
+        lo[u][e] = __builtin_bit_cast(_Float16, T::down(x - T::up(b)));
+      }
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[n][r] *= alpha;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint64_t w[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          // what lies behind the sequence's tokens is no value
+          const int t = (2 * u + e) * 16 + g * 4, there = min(max(left - t, 0), 4);
+          w[e] = *reinterpret_cast<const uint64_t*>(tv + (n * 16 + col) * kBlock + t);
+          w[e] &= there == 4 ? ~uint64_t{0} : (uint64_t{1} << (16 * there)) - 1;
+        }
+        struct Two { uint64_t x, y; };
+        const half8 v = __builtin_bit_cast(half8, Two{w[0], w[1]});
+        acc[n] = T::mfma(v, hi[u], acc[n]);
+        if constexpr (__is_same(T, BF16)) acc[n] = T::mfma(v, lo[u], acc[n]);
       }
     }
   }
 
+  float m = soft.m, l = soft.l;
   l = rows_sum(l);
   if (g == 0) {
     stat[0][wave][col] = m;
@@ -657,51 +714,95 @@ __global__ __launch_bounds__(kThreads) void cache_attn_kernel(AttnArgs a) {
   }
 }
 
-// The parts of one row and head, joined in their order.
-template <class T, int D>
+// Sum and maximum over a wavefront in every lane, through VALU operands.
+__device__ __forceinline__ float lanes_max(float x) {
+  return __builtin_bit_cast(float, lanes_reduce(__builtin_bit_cast(uint32_t, x), [](uint32_t p, uint32_t q) {
+    return __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, p), __builtin_bit_cast(float, q)));
+  }));
+}
+__device__ __forceinline__ float lanes_sum(float x) {
+  return __builtin_bit_cast(float, lanes_reduce(__builtin_bit_cast(uint32_t, x), [](uint32_t p, uint32_t q) {
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, p) + __builtin_bit_cast(float, q));
+  }));
+}
+
+// The parts of one row and head, joined in their order: 4 kLanes columns a workgroup, its groups of
+// kLanes threads take every so many-th part, all loads on their way before the weights are known.
+template <class T, int D, int kLanes>
 __global__ __launch_bounds__(kThreads) void cache_join_kernel(AttnArgs a) {
+  constexpr int kGroups = kThreads / kLanes, kEach = 8, kSlices = D / (4 * kLanes);
   __shared__ float weight[kSplits];
-  __shared__ float red[2][kWaves];
-  __shared__ float sums[kThreads];
-  const int tid = threadIdx.x;
-  const int qh = static_cast<int>(blockIdx.x % a.n_q);
-  const int rest = static_cast<int>(blockIdx.x / a.n_q);
+  __shared__ f32x4 sums[kGroups][kLanes];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int slice = static_cast<int>(blockIdx.x % kSlices);
+  int rest = static_cast<int>(blockIdx.x / kSlices);
+  const int qh = rest % a.n_q;
+  rest /= a.n_q;
   const int at = rest % a.max_new, seq = rest / a.max_new;
   const Span s = span_of(a.bounds, a.past, seq, a.n_rows, a.max_new, a.max_len);
   if (at >= s.n) return;
   const int rows = s.n * a.group, r0 = (at * a.group + qh % a.group) / 16 * 16;
   const Visits visits(s.past + r0 / a.group, s.past + min(r0 + 15, rows - 1) / a.group, a.window, a.sinks);
   const int parts = (visits.count + a.per - 1) / a.per;
-  if (parts <= 1) return;
+  if (parts <= 1) return;  // written by its one part
   const int64_t to = (s.row0 + at) * a.n_q + qh;
-  float2 ml = make_float2(-__builtin_inff(), 0.f);
-  if (tid < parts) ml = a.part_ml[to * a.splits + tid];
-  float top = wave_max(ml.x);
-  if ((tid & 63) == 0) red[0][tid / kWave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  const float w = ml.x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
-  weight[tid] = w;
-  const float part_sum = wave_sum(ml.y * w);
-  if ((tid & 63) == 0) red[1][tid / kWave] = part_sum;
-  __syncthreads();
-  const float sum = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-  constexpr int kGroups = kThreads / D;
-  const int d = tid % D, grp = tid / D;
+  const int grp = tid / kLanes, d = slice * 4 * kLanes + (tid % kLanes) * 4;
   const float* p = a.part_o + to * a.splits * D + d;
-  float o = 0.f;
-#pragma unroll 8
-  for (int i = grp; i < parts; i += kGroups) o += weight[i] * p[static_cast<int64_t>(i) * D];
-  sums[tid] = o;
+  f32x4 o[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int j = grp + i * kGroups;
+    o[i] = j < parts ? *reinterpret_cast<const f32x4*>(p + static_cast<int64_t>(j) * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // every wavefront takes all weights
+  constexpr int kPer = kSplits / kWave;
+  float2 ml[kPer];
+  float top = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int j = lane + i * kWave;
+    ml[i] = j < parts ? a.part_ml[to * a.splits + j] : make_float2(-__builtin_inff(), 0.f);
+    top = fmaxf(top, ml[i].x);
+  }
+  top = lanes_max(top);
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const float w = ml[i].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - top);
+    sum += ml[i].y * w;
+    if (tid < kWave) weight[lane + i * kWave] = w;
+  }
+  sum = lanes_sum(sum);
+  __syncthreads();
+  f32x4 total = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    const int j = grp + i * kGroups;
+    if (j < parts) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) total[e] += weight[j] * o[i][e];
+    }
+  }
+  sums[grp][tid % kLanes] = total;
   __syncthreads();
   if (grp != 0) return;
+  const int used = min(kGroups, parts);
+  for (int i = 1; i < used; ++i) {
+    const f32x4 x = sums[i][tid];
 #pragma unroll
-  for (int i = 1; i < kGroups; ++i) o += sums[i * D + d];
-  a.out[to * D + d] = T::down(sum > 0.f ? o / sum : sum == 0.f ? 0.f : sum);
+    for (int e = 0; e < 4; ++e) total[e] += x[e];
+  }
+  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  u32x2 w;
+  w.x = T::down(total[0] * inv) | static_cast<uint32_t>(T::down(total[1] * inv)) << 16;
+  w.y = T::down(total[2] * inv) | static_cast<uint32_t>(T::down(total[3] * inv)) << 16;
+  *reinterpret_cast<u32x2*>(a.out + to * D + d) = w;
 }
 
-// How an attention call splits its pages: enough workgroups for every CU to hold four, parts of at
-// least a page per wavefront.
+constexpr int kPerCu = 3;  // workgroups of the attention that a CU holds
+
+// How an attention call splits its pages: enough workgroups to fill every CU, parts of at least a page
+// per wavefront.
 struct Plan {
   int64_t tiles, splits, per;
 };
@@ -713,7 +814,7 @@ Plan plan_of(int64_t n_seqs, int64_t kv, int64_t group, int64_t max_new, int64_t
   int64_t visits = (max_len + kBlock - 1) / kBlock;
   if (window > 0) visits = std::min(visits, (window + 15 + 63) / kBlock + 1 + (sinks + kBlock - 1) / kBlock);
   const int64_t base = n_seqs * kv * p.tiles;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kSplits, 4 * device_cus() / std::max<int64_t>(base, 1)));
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kSplits, kPerCu * device_cus() / std::max<int64_t>(base, 1)));
   p.per = std::max<int64_t>((visits + want - 1) / want, kWaves);
   p.splits = std::max<int64_t>((visits + p.per - 1) / p.per, 1);
   return p;
@@ -868,15 +969,24 @@ TALM_API int talm_cache_attn(const uint16_t* q, int64_t q_stride_tok, int64_t q_
              reinterpret_cast<float2*>(part_o ? part_o + n_rows * n_q_heads * p.splits * head_dim : nullptr)};
   const int64_t items = static_cast<int64_t>(n_seqs) * n_kv_heads * p.tiles * p.splits;
   const int64_t joins = p.splits > 1 ? static_cast<int64_t>(n_seqs) * max_new * n_q_heads : 0;
-  if (items > 0x7fffffff || joins > 0x7fffffff) return fail(TALM_EINVAL, "cache_attn: too many rows");
+  if (items > 0x7fffffff || joins * (head_dim / 32) > 0x7fffffff) return fail(TALM_EINVAL, "cache_attn: too many rows");
   const hipStream_t st = as_stream(stream);
 #define LAUNCH(T, D, grid, block, args) hipLaunchKernelGGL((cache_attn_kernel<T, D>), grid, block, 0, st, args)
   TALM_CACHE_KERNEL(LAUNCH, items, a);
 #undef LAUNCH
   if (const int status = check_launch("cache_attn")) return status;
   if (joins == 0) return TALM_OK;
-#define LAUNCH(T, D, grid, block, args) hipLaunchKernelGGL((cache_join_kernel<T, D>), grid, block, 0, st, args)
-  TALM_CACHE_KERNEL(LAUNCH, joins, a);
+  // a whole head's columns a workgroup where its groups reach the parts in eight steps, else 32
+  const bool few = p.splits <= 8 * (kThreads / (head_dim / 4));
+  const int64_t slices = few ? 1 : head_dim / 32;
+#define LAUNCH(T, D, grid, block, args)                                                  \
+  do {                                                                                   \
+    if (few)                                                                             \
+      hipLaunchKernelGGL((cache_join_kernel<T, D, D / 4>), grid, block, 0, st, args);    \
+    else                                                                                 \
+      hipLaunchKernelGGL((cache_join_kernel<T, D, 8>), grid, block, 0, st, args);        \
+  } while (0)
+  TALM_CACHE_KERNEL(LAUNCH, joins * slices, a);
 #undef LAUNCH
   return check_launch("cache_attn");
 }
