@@ -30,7 +30,9 @@ typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half2_ __attribute__((ext_vector_type(2)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
@@ -56,17 +58,17 @@ struct Cache {
 // A sequence's new rows [row0, row0 + n) behind `past` tokens, kept inside the buffers' rows, the
 // caller's longest counts and the table whatever the device arrays hold.
 struct Span {
-  int64_t row0;
-  int past, n;
+  int row0, past, n;
 };
+__device__ __forceinline__ Span span_of(int lo, int hi, int past, int n_rows, int max_new, int max_len) {
+  lo = max(0, min(lo, n_rows));
+  hi = max(lo, min(hi, n_rows));
+  if (past < 0 || past >= max_len) return Span{lo, 0, 0};
+  return Span{lo, past, min(min(hi - lo, max_new), max_len - past)};
+}
 __device__ __forceinline__ Span span_of(const int32_t* bounds, const int32_t* past, int seq, int64_t n_rows,
                                         int max_new, int max_len) {
-  const int64_t lo = max(int64_t{0}, min(static_cast<int64_t>(bounds[2 * seq]), n_rows));
-  const int64_t hi = max(lo, min(static_cast<int64_t>(bounds[2 * seq + 1]), n_rows));
-  Span s{lo, past[seq], static_cast<int>(min(hi - lo, static_cast<int64_t>(max_new)))};
-  if (s.past < 0 || s.past >= max_len) return Span{lo, 0, 0};
-  s.n = min(s.n, max_len - s.past);
-  return s;
+  return span_of(bounds[2 * seq], bounds[2 * seq + 1], past[seq], static_cast<int>(n_rows), max_new, max_len);
 }
 
 struct F16 {
@@ -83,6 +85,9 @@ struct F16 {
   static __device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
+  static __device__ __forceinline__ f32x16 mfma(half8 a, half8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
 };
 struct BF16 {
   static __device__ __forceinline__ float up(uint32_t bits) { return __builtin_bit_cast(float, bits << 16); }
@@ -98,6 +103,10 @@ struct BF16 {
   }
   static __device__ __forceinline__ f32x4 mfma(half8 a, half8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0,
+                                                   0);
+  }
+  static __device__ __forceinline__ f32x16 mfma(half8 a, half8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0,
                                                    0);
   }
 };
@@ -239,7 +248,7 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(WriteArgs a) {
   const bool turn = kTurn && which == 0;
   // the 8 columns from d on of the sequence's token `t`, a new one
   auto fresh = [&](int t, int d, uint32_t (&w)[4]) {
-    const int64_t row = s.row0 + (t - s.past);
+    const int64_t row = s.row0 + (t - s.past);  // of the operands
     row8<T, D>(src + row * tok, kTurn ? a.cos + row * a.cs_tok : nullptr, kTurn ? a.sin + row * a.cs_tok : nullptr,
                d, turn, w);
   };
@@ -358,7 +367,7 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(ReadArgs a) {
   const int block = s.past / kBlock + j;
   const int lo = max(block * kBlock, s.past), hi = min((block + 1) * kBlock, s.past + s.n);
   if (lo >= hi) return;
-  uint16_t* dst = (which ? a.v : a.k) + (s.row0 - s.past) * (a.c.kv * D) + head * D;
+  uint16_t* dst = (which ? a.v : a.k) + static_cast<int64_t>(s.row0 - s.past) * (a.c.kv * D) + head * D;
   const int64_t pitch = static_cast<int64_t>(a.c.kv) * D;
   const int64_t page = block < len / kBlock ? a.c.page(seq, block) : -1;
   const bool open = block == len / kBlock;  // the tail's tokens, up to len
@@ -407,19 +416,27 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(ReadArgs a) {
 
 struct AttnArgs {
   Cache c;
-  const uint16_t* q;
-  int64_t q_tok, q_head;
-  int64_t n_rows;
-  int n_q, group;
   const int32_t* bounds;
   const int32_t* past;
-  int max_new, max_len;
-  float scale_log2;
+  int n_rows, max_new, max_len;
+  int n_q, group, group_magic, group_shift;  // query heads per KV head; row / group is over() of them
+  int cols, splits, per;  // rows of a tile; parts of the pages, pages of a part
+  int turn;               // 2^n - 1 below both 8 and `splits`
+  bool listed;            // the grid's first axis: the sequences' tiles in a row, else one tile each
   int window, sinks;  // window 0: every key
-  int tiles, splits, per;  // tiles of rows per sequence and KV head; parts of the pages, pages of a part
+  float scale_log2;
+  const uint16_t* q;
+  int64_t q_tok, q_head;
   uint16_t* out;      // [n_rows, n_q, D]
   float* part_o;      // [n_rows, n_q, splits, D]
   float2* part_ml;    // [n_rows, n_q, splits]: maximum, sum
+  // n / group of 0 <= n < 2^30: the integer division would be some thirty instructions in front of the
+  // first load
+  __device__ __forceinline__ int over(int n) const {
+    return group == 1 ? n
+                      : static_cast<int>(__umulhi(static_cast<uint32_t>(n), static_cast<uint32_t>(group_magic)) >>
+                                         group_shift);
+  }
 };
 
 // The pages that rows at places [lo, hi] see, as a list: the sinks', then the window's.
@@ -434,179 +451,293 @@ struct Visits {
   __device__ __forceinline__ int page(int i) const { return i < sinks ? i : i - sinks + first; }
 };
 
-// Over the four lanes of one query column, 16 apart.
-__device__ __forceinline__ float rows_max(float x) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, x);
-  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  x = fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
-  const uint32_t w = __builtin_bit_cast(uint32_t, x);
-  const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-  return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(q[0])), __builtin_bit_cast(float, static_cast<uint32_t>(q[1])));
-}
-__device__ __forceinline__ float rows_sum(float x) {
-  x += __shfl_xor(x, 16, kWave);
-  return x + __shfl_xor(x, 32, kWave);
-}
-
-// The 16 scores of a lane (tokens first + 16 t + 4 g + r) become weights exp2(c s - m) of a running
-// maximum m; returns what the sums so far are multiplied by. kMask: tokens that the row does not see.
-struct Softmax {
-  float m = -__builtin_inff(), l = 0.f;
-  __device__ __forceinline__ float step(f32x4 (&st)[4], float c, bool mask, int first, int g, int place, int window,
-                                        int sinks) {
-    if (mask) {
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = first + t * 16 + g * 4 + r;
-          const bool seen = key <= place && (window == 0 || place - key < window || key < sinks);
-          st[t][r] = seen ? st[t][r] : -__builtin_inff();
-        }
+// How S^T = K Q^T and O^T = V^T P^T of one page lie in a wavefront with kCol query columns, 16
+// (v_mfma_*_16x16x32) or 32 (v_mfma_*_32x32x16; half as many instructions for the same products, each of
+// which takes the VALU's issue for about 8 cycles). Lane l is column l % kCol, quarter or half g = l / kCol.
+// Its scores in order, i = 0, 1, ..: token kStep (i / 4) + 4 g + i % 4; its output columns likewise.
+template <int D, int kCol>
+struct Lay {
+  static constexpr int kStep = kCol == 16 ? 16 : 8;
+  static constexpr int kLane = kBlock * kCol / kWave;  // scores of a lane
+  static constexpr int kTiles = kBlock / kCol;         // tiles of scores
+  static constexpr int kEach = kLane / kTiles;         // and numbers of one
+  static constexpr int kOuts = D / kCol;               // tiles of outputs, kEach numbers each
+  static constexpr int kFrags = D * kCol / 512;        // operands of 8 of a row's columns
+  static constexpr int kPs = kLane / 8;                // operands of P
+  using Tile = typename std::conditional<kCol == 16, f32x4, f32x16>::type;
+  // first column of a lane's f-th operand of a query or key row
+  static __device__ __forceinline__ int column(int f, int g) {
+    return kCol == 16 ? f / 2 * 64 + g * 16 + f % 2 * 8 : f / 4 * 64 + f / 2 % 2 * 32 + g * 16 + f % 2 * 8;
+  }
+  // places of a lane's 16 bytes in a page, without the lane's own part: the i-th load of the keys belongs
+  // to tile i / (kFrags / 2) and to operands 2 (i % (kFrags / 2)) and one behind it
+  static __device__ __forceinline__ int key_at(int i) {
+    if (kCol == 16) return i * 64;
+    constexpr int kC = D / 64;
+    const int tile = i / (2 * kC), rest = i % (2 * kC);
+    return (2 * tile * kC + rest / 2) * 64 + rest % 2 * 32;
+  }
+  static __device__ __forceinline__ int key_lane(int lane) {
+    return kCol == 16 ? lane : (lane >> 4 & 1) * (D / 64) * 64 + (lane >> 5) * 16 + (lane & 15);
+  }
+  static __device__ __forceinline__ int value_at(int i) { return kCol == 16 ? i * 64 : i / 2 * 128 + i % 2 * 32; }
+  static __device__ __forceinline__ int value_lane(int lane) {
+    return kCol == 16 ? lane : (lane >> 4 & 1) * 64 + (lane >> 5) * 16 + (lane & 15);
+  }
+  // the codes of output tile n that meet the u-th operand of P
+  static __device__ __forceinline__ u32x2 value_codes(const u32x4 (&w)[D / 16], int n, int u) {
+    if constexpr (kCol == 16) return u32x2{w[n][2 * u], w[n][2 * u + 1]};
+    else return u32x2{w[2 * n][u], w[2 * n + 1][u]};
+  }
+  // over the lanes of one column
+  static __device__ __forceinline__ float max_of(float x) {
+    if (kCol == 16) {
+      const uint32_t u = __builtin_bit_cast(uint32_t, x);
+      const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+      x = fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])),
+                __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
     }
-    float top = st[0][0];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) top = fmaxf(top, st[t][r]);
-    const float m_new = fmaxf(m, rows_max(top) * c);
-    // a row that has seen no key yet keeps -inf, its weights are exp2(-inf - 0) = 0
-    const float ref = m_new == -__builtin_inff() ? 0.f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m - ref);
-    m = m_new;
-    float sum = 0.f;
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        st[t][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[t][r], c, -ref));
-        sum += st[t][r];
-      }
-    l = l * alpha + sum;
-    return alpha;
+    const uint32_t w = __builtin_bit_cast(uint32_t, x);
+    const auto q = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(q[0])),
+                 __builtin_bit_cast(float, static_cast<uint32_t>(q[1])));
+  }
+  static __device__ __forceinline__ float sum_of(float x) {
+    if (kCol == 16) x += __shfl_xor(x, 16, kWave);
+    return x + __shfl_xor(x, 32, kWave);
   }
 };
 
-// A workgroup: 16 (token, head) rows of one sequence and KV head against one part of its pages, a
-// page per wavefront at a time, each with its own running maximum and sum; joined through LDS.
-template <class T, int D>
-__global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(AttnArgs a) {
-  constexpr int kC = D / 64, kN = D / 16, kPitch = D + 4;
-  __shared__ float part[kWaves][16][kPitch];
-  __shared__ float stat[2][kWaves][16];
-  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int split = static_cast<int>(blockIdx.x % a.splits);
-  int rest = static_cast<int>(blockIdx.x / a.splits);
-  const int tile = rest % a.tiles;
-  rest /= a.tiles;
-  const int head = rest % a.c.kv, seq = rest / a.c.kv;
-  const Span s = span_of(a.bounds, a.past, seq, a.n_rows, a.max_new, a.max_len);
-  const int rows = s.n * a.group, r0 = tile * 16;
+// A workgroup: kCols = kCol kWide (token, head) rows of one sequence and KV head, the columns of S^T =
+// K Q^T, against one part of its pages. Each of kWide groups of wavefronts has kCol of the columns; the
+// wavefronts of a group take a page each at a time, with a running reference and sums of their own, joined
+// through LDS.
+//
+// Weights are exp2(c s - ref) of a reference that follows the running maximum only where a score passes it
+// by more than 2^8: they stay below 2^8, far inside fp16, and nearly every page leaves the sums so far as
+// they are.
+template <class T, int D, int kCol, int kWide>
+__global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kernel(AttnArgs a) {
+  using L = Lay<D, kCol>;
+  using Tile = typename L::Tile;
+  constexpr int kPitch = D + 4, kCols = kCol * kWide, kDeep = kWaves / kWide, kLoads = D / 16;
+  constexpr bool kUnits = __is_same(T, F16);
+  __shared__ float part[kDeep][kCols][kPitch];
+  __shared__ float stat[2][kDeep][kCols];
+  const int tid = threadIdx.x, lane = tid & 63, col = lane % kCol, g = lane / kCol;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave), wide = wave % kWide, deep = wave / kWide;
+  const int head = blockIdx.y;
+  int tile = 0, seq = blockIdx.z, split = blockIdx.x;
+  if (a.listed) {
+    tile = split / a.splits;
+    split -= tile * a.splits;
+  }
+  // Workgroups go to the eight dies in turn: without this a die would have the same part of every sequence,
+  // and later parts are those that short sequences lack.
+  split += (head + seq + tile) & a.turn;
+  if (split >= a.splits) split -= a.splits;
+  // A workgroup begins with a chain of cache misses; all arguments in one, the sequence's numbers and its
+  // pages' places (without a window known from the part alone) in the next, then the pages.
+  asm volatile("" ::"s"(a.c.codes), "s"(a.c.scales), "s"(a.c.tail), "s"(a.c.table), "s"(a.c.width), "s"(a.c.kv),
+               "s"(a.bounds), "s"(a.past), "s"(a.n_rows), "s"(a.max_new), "s"(a.max_len), "s"(a.group),
+               "s"(a.group_magic), "s"(a.group_shift), "s"(a.window), "s"(a.sinks), "s"(a.q), "s"(a.q_tok),
+               "s"(a.q_head));
+  const bool alone = kCol == 16 || a.c.n_seqs == 1;  // the sequence is known from the grid
+  int early = -1;
+  if (alone && a.window == 0) {
+    const int mine = split * a.per + deep + kDeep * lane;
+    if (mine < a.c.width) early = a.c.table[static_cast<int64_t>(seq) * a.c.width + mine];
+  }
+  Span s;
+  if (alone) {
+    const int lo_row = a.bounds[2 * seq], hi_row = a.bounds[2 * seq + 1], held = a.past[seq];
+    asm volatile("" ::"s"(lo_row), "s"(hi_row), "s"(held));
+    s = span_of(lo_row, hi_row, held, a.n_rows, a.max_new, a.max_len);
+  } else {
+    // Tile `tile` of the sequences' tiles in a row, of every 64 sequences those with the most pages first: a
+    // long one that began last would be the call's tail. Lane l has sequence l's tiles.
+    for (seq = 0;; seq += kWave) {
+      if (seq >= a.c.n_seqs) return;
+      Span mine{0, 0, 0};
+      if (seq + lane < a.c.n_seqs) mine = span_of(a.bounds, a.past, seq + lane, a.n_rows, a.max_new, a.max_len);
+      const int count = (mine.n * a.group + kCols - 1) / kCols, size = mine.past + mine.n;
+      int before = 0, all = 0;
+      for (int l = 0; l < min(kWave, a.c.n_seqs - seq); ++l) {
+        const int c = __builtin_amdgcn_readlane(count, l), n = __builtin_amdgcn_readlane(size, l);
+        all += c;
+        if (n > size || (n == size && l < lane)) before += c;
+      }
+      if (tile >= all) {
+        tile -= all;
+        continue;
+      }
+      const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(before <= tile && tile < before + count));
+      tile -= __builtin_amdgcn_readlane(before, l);
+      seq += l;
+      s = Span{__builtin_amdgcn_readlane(mine.row0, l), __builtin_amdgcn_readlane(mine.past, l),
+               __builtin_amdgcn_readlane(mine.n, l)};
+      break;
+    }
+  }
+  const int rows = s.n * a.group, r0 = tile * kCols;
   if (r0 >= rows) return;
   const int len = s.past + s.n;
-  const int row = min(r0 + col, rows - 1);  // the columns behind the last row repeat it
-  const int at = row / a.group, place = s.past + at;
-  const int lo_place = s.past + r0 / a.group, hi_place = s.past + min(r0 + 15, rows - 1) / a.group;
-  const Visits visits(lo_place, hi_place, a.window, a.sinks);
+  const int last_place = s.past + a.over(min(r0 + kCols, rows) - 1);
+  const Visits visits(s.past + a.over(r0), last_place, a.window, a.sinks);
   const int begin = split * a.per, end = min(visits.count, begin + a.per);
   if (begin >= end) return;
-  const int qh = head * a.group + row % a.group;
-  // the last visit is the open block, whose tokens are in the tail, where the rows reach it
-  const bool open = hi_place / kBlock == len / kBlock;
-  const int code_end = a.c.n_pages > 0 ? min(end, visits.count - (open ? 1 : 0)) : begin;
+  // the wavefront's columns; those behind the last row repeat it
+  const int c0 = r0 + wide * kCol;
+  const bool idle = c0 >= rows;
+  const int lo_place = s.past + a.over(min(c0, rows - 1)), hi_place = s.past + a.over(min(c0 + kCol, rows) - 1);
+  // the last visit is the open block, whose tokens are in the tail, where the workgroup's rows reach it
+  const bool open = last_place / kBlock == len / kBlock;
+  const int code_end = a.c.n_pages > 0 && !idle ? min(end, visits.count - (open ? 1 : 0)) : begin;
 
-  half8 q[kC][2];
+  const int row = min(c0 + col, rows - 1), row_token = a.over(row), place = s.past + row_token;
+  half8 q[L::kFrags];
   {
-    const uint16_t* p = a.q + (s.row0 + at) * a.q_tok + qh * a.q_head + g * 16;
+    const uint16_t* p = a.q + (s.row0 + row_token) * a.q_tok + (head * a.group + row - row_token * a.group) * a.q_head;
 #pragma unroll
-    for (int c = 0; c < kC; ++c)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) q[c][h] = *reinterpret_cast<const half8*>(p + c * 64 + h * 8);
+    for (int f = 0; f < L::kFrags; ++f) q[f] = *reinterpret_cast<const half8*>(p + L::column(f, g));
   }
-  f32x4 acc[kN];
+  Tile acc[L::kOuts], st[L::kTiles];
 #pragma unroll
-  for (int n = 0; n < kN; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-  Softmax soft;
-  u32x4 kw[4 * kC], vw[kN];
-  auto load_k = [&](int page) {
+  for (int n = 0; n < L::kOuts; ++n) acc[n] = Tile(0.f);
+  float ref = -__builtin_inff(), l = 0.f;
+  // fp16: acc is in units of the last page's scale. Such scales lie between 2^-33 and 2^8, so the sums
+  // stay inside fp32's range whatever follows; bfloat16's do not, and there each page's sums are scaled.
+  float unit = 1.f;
+  u32x4 kw[kLoads], vw[kLoads];
+  // what one wavefront alone reads passes by the caches
+  auto load = [&](const u32x4* p) { return kWide == 1 ? __builtin_nontemporal_load(p) : *p; };
+  auto load_k = [&](int page) __attribute__((always_inline)) {
     const u32x4* src = reinterpret_cast<const u32x4*>(
-                           a.c.codes + (static_cast<int64_t>(page) * 2 * a.c.kv + head) * (kBlock * D)) + lane;
+                           a.c.codes + (static_cast<int64_t>(page) * 2 * a.c.kv + head) * (kBlock * D)) +
+                       L::key_lane(lane);
 #pragma unroll
-    for (int t = 0; t < 4 * kC; ++t) kw[t] = __builtin_nontemporal_load(src + t * kWave);
+    for (int i = 0; i < kLoads; ++i) kw[i] = load(src + L::key_at(i));
   };
-  auto load_v = [&](int page) {
+  auto load_v = [&](int page) __attribute__((always_inline)) {
     const u32x4* src = reinterpret_cast<const u32x4*>(
-                           a.c.codes + ((static_cast<int64_t>(page) * 2 + 1) * a.c.kv + head) * (kBlock * D)) + lane;
+                           a.c.codes + ((static_cast<int64_t>(page) * 2 + 1) * a.c.kv + head) * (kBlock * D)) +
+                       L::value_lane(lane);
 #pragma unroll
-    for (int n = 0; n < kN; ++n) vw[n] = __builtin_nontemporal_load(src + n * kWave);
+    for (int i = 0; i < kLoads; ++i) vw[i] = load(src + L::value_at(i));
+  };
+  // Weights of a page's (or the tail's) scores; the sums so far follow a new reference and unit.
+  auto weigh = [&](float c, bool mask, int first, float ratio) __attribute__((always_inline)) {
+    if (mask) {
+#pragma unroll
+      for (int i = 0; i < L::kLane; ++i) {
+        const int key = first + L::kStep * (i / 4) + 4 * g + i % 4;
+        const bool seen = (key <= place) & ((a.window == 0) | (place - key < a.window) | (key < a.sinks));
+        st[i / L::kEach][i % L::kEach] = seen ? st[i / L::kEach][i % L::kEach] : -__builtin_inff();
+      }
+    }
+    float top = st[0][0];
+#pragma unroll
+    for (int i = 1; i < L::kLane; ++i) top = fmaxf(top, st[i / L::kEach][i % L::kEach]);
+    top = L::max_of(top) * c;
+    if (__builtin_amdgcn_ballot_w64(top > ref + 8.f) || ratio != 1.f) {
+      const float next = fmaxf(ref, top);
+      // a row that has seen no key yet keeps -inf
+      const float grow = next == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ref - next);
+      ref = next;
+      l *= grow;
+#pragma unroll
+      for (int n = 0; n < L::kOuts; ++n)
+#pragma unroll
+        for (int e = 0; e < L::kEach; ++e) acc[n][e] *= grow * ratio;
+    }
+    const float base = ref == -__builtin_inff() ? 0.f : ref;  // its weights are exp2(-inf - 0) = 0
+#pragma unroll
+    for (int i = 0; i < L::kLane; ++i) {
+      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i / L::kEach][i % L::kEach], c, -base));
+      st[i / L::kEach][i % L::kEach] = x;
+      l += x;
+    }
   };
 
   // 64 of the wavefront's pages at a time: lane l holds the l-th one's place and scales
-  for (int base = begin + wave; base < code_end; base += kWaves * kWave) {
-    const int mine = base + kWaves * lane;
+  for (int base = begin + deep; base < code_end; base += kDeep * kWave) {
+    const int mine = base + kDeep * lane;
     int page_l = -1;
     float ks_l = 1.f, vs_l = 1.f;
     if (mine < code_end) {
-      page_l = static_cast<int>(a.c.page(seq, visits.page(mine)));
+      if (alone && a.window == 0 && base == begin + deep)
+        page_l = early < a.c.n_pages ? early : -1;
+      else
+        page_l = static_cast<int>(a.c.page(seq, visits.page(mine)));
       if (page_l >= 0) {
         ks_l = a.c.scales[static_cast<int64_t>(page_l) * 2 * a.c.kv + head];
         vs_l = a.c.scales[(static_cast<int64_t>(page_l) * 2 + 1) * a.c.kv + head];
       }
     }
-    const int count = min((code_end - base + kWaves - 1) / kWaves, kWave);
+    const int count = min((code_end - base + kDeep - 1) / kDeep, kWave);
     // what is no page is read as the pool's first one and seen by no row
     int page = __builtin_amdgcn_readlane(page_l, 0);
     load_k(max(page, 0));
     load_v(max(page, 0));
-    auto step = [&](int i, auto more) {
+    auto step = [&](int i, auto more) __attribute__((always_inline)) {
       const float k_scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ks_l), i));
       const float v_scale = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, vs_l), i));
       const int next = decltype(more)::value ? __builtin_amdgcn_readlane(page_l, i + 1) : 0;
-      f32x4 st[4];
+      const int first = visits.page(base + kDeep * i) * kBlock;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < L::kTiles; ++t) st[t] = Tile(0.f);
 #pragma unroll
-        for (int c = 0; c < kC; ++c) {
-          const u32x4 w = kw[t * kC + c];
-          st[t] = T::mfma(T::codes(u32x2{w.x, w.y}), q[c][0], st[t]);
-          st[t] = T::mfma(T::codes(u32x2{w.z, w.w}), q[c][1], st[t]);
+      for (int f = 0; f < L::kFrags; ++f)
+#pragma unroll
+        for (int t = 0; t < L::kTiles; ++t) {
+          const u32x4 w = kw[t * (L::kFrags / 2) + f / 2];
+          st[t] = T::mfma(T::codes(f % 2 ? u32x2{w.z, w.w} : u32x2{w.x, w.y}), q[f], st[t]);
         }
-      }
       // the next page's keys are on their way while this one's weights and values are worked on, its
       // values during the next one's scores (the last page is a copy of its own without them: a
       // condition here would make every wait one for all loads)
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (decltype(more)::value) load_k(max(next, 0));
       __builtin_amdgcn_sched_barrier(0);
-      const int first = visits.page(base + kWaves * i) * kBlock;
       const bool all = page >= 0 && first + kBlock - 1 <= lo_place &&
                        (a.window == 0 || hi_place - first < a.window || first + kBlock <= a.sinks);
-      const float alpha = soft.step(st, a.scale_log2 * k_scale, !all, page >= 0 ? first : 0x7fff0000, g, place,
-                                    a.window, a.sinks);
+      weigh(a.scale_log2 * k_scale, !all, page >= 0 ? first : 0x7fff0000, kUnits ? unit * inverse(v_scale) : 1.f);
+      if constexpr (kUnits) unit = v_scale;
       // P in fp16 whatever the operands' type: the values' codes are exact in it. The error is that of
       // a rounding to 11 bits, below the output's own.
-      half8 p[2];
+      half8 p[L::kPs];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < L::kPs; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          p[u][r] = static_cast<_Float16>(st[2 * u][r]);
-          p[u][4 + r] = static_cast<_Float16>(st[2 * u + 1][r]);
+        for (int e = 0; e < 8; e += 2) {
+          const int i0 = 8 * u + e;
+          const half2_ w = __builtin_convertvector(
+              (f32x2{st[i0 / L::kEach][i0 % L::kEach], st[i0 / L::kEach][i0 % L::kEach + 1]}), half2_);
+          p[u][e] = w.x;
+          p[u][e + 1] = w.y;
         }
       if (page < 0) {
 #pragma unroll
-        for (int n = 0; n < kN; ++n) vw[n] = u32x4{0, 0, 0, 0};
+        for (int k = 0; k < kLoads; ++k) vw[k] = u32x4{0, 0, 0, 0};
       }
 #pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        f32x4 o = {0.f, 0.f, 0.f, 0.f};
-        o = F16::mfma(F16::codes(u32x2{vw[n].x, vw[n].y}), p[0], o);
-        o = F16::mfma(F16::codes(u32x2{vw[n].z, vw[n].w}), p[1], o);
-        // the scale of the page's values in fp32: it may be past what fp16 holds
+      for (int n = 0; n < L::kOuts; n += 2) {
+        Tile o[2];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[n][r] = __builtin_fmaf(o[r], v_scale, acc[n][r] * alpha);
+        for (int k = 0; k < 2; ++k) o[k] = kUnits ? acc[n + k] : Tile(0.f);
+#pragma unroll
+        for (int u = 0; u < L::kPs; ++u)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) o[k] = F16::mfma(F16::codes(L::value_codes(vw, n + k, u)), p[u], o[k]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if constexpr (kUnits) {
+            acc[n + k] = o[k];
+          } else {
+#pragma unroll
+            for (int e = 0; e < L::kEach; ++e) acc[n + k][e] = __builtin_fmaf(o[k][e], v_scale, acc[n + k][e]);
+          }
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (decltype(more)::value) load_v(max(next, 0));
@@ -617,90 +748,54 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(AttnArgs a) {
     step(count - 1, std::false_type{});
   }
 
-  // the tail, by the wavefront whose turn it is
-  if (open && visits.count - 1 >= begin && visits.count - 1 < end && (visits.count - 1 - begin) % kWaves == wave) {
+  // the tail, by the wavefronts whose turn it is
+  if (open && !idle && visits.count - 1 >= begin && visits.count - 1 < end &&
+      (visits.count - 1 - begin) % kDeep == deep) {
     const uint16_t* tk = a.c.tail + (static_cast<int64_t>(seq) * 2 * a.c.kv + head) * (kBlock * D);
     const uint16_t* tv = tk + static_cast<int64_t>(a.c.kv) * (kBlock * D);
     const int first = len / kBlock * kBlock, left = len - first;
-    f32x4 st[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < L::kTiles; ++t) {
+      st[t] = Tile(0.f);
 #pragma unroll
-      for (int c = 0; c < kC; ++c)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const half8 w = *reinterpret_cast<const half8*>(tk + (t * 16 + col) * D + c * 64 + g * 16 + h * 8);
-          st[t] = T::mfma(w, q[c][h], st[t]);
-        }
+      for (int f = 0; f < L::kFrags; ++f)
+        st[t] = T::mfma(*reinterpret_cast<const half8*>(tk + (t * kCol + col) * D + L::column(f, g)), q[f], st[t]);
     }
-    const float alpha = soft.step(st, a.scale_log2, true, first, g, place, a.window, a.sinks);
+    weigh(a.scale_log2, true, first, unit);
+    unit = 1.f;
     // the weights in the tail's type; for bfloat16 as two parts, so that they keep 16 bits
-    half8 hi[2], lo[2];
+    half8 hi[L::kPs], lo[L::kPs];
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int i = 0; i < L::kLane; ++i) {
+      const float x = st[i / L::kEach][i % L::kEach];
+      const uint16_t b = T::down(x);
+      hi[i / 8][i % 8] = __builtin_bit_cast(_Float16, b);
+      lo[i / 8][i % 8] = __builtin_bit_cast(_Float16, T::down(x - T::up(b)));
+    }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x = st[2 * u + e / 4][e % 4];
-        const uint16_t b = T::down(x);
-        hi[u][e] = __builtin_bit_cast(_Float16, b);
-        lo[u][e] = __builtin_bit_cast(_Float16, T::down(x - T::up(b)));
-      }
+    for (int n = 0; n < L::kOuts; ++n)
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[n][r] *= alpha;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < L::kPs; ++u) {
         uint64_t w[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           // what lies behind the sequence's tokens is no value
-          const int t = (2 * u + e) * 16 + g * 4, there = min(max(left - t, 0), 4);
-          w[e] = *reinterpret_cast<const uint64_t*>(tv + (n * 16 + col) * kBlock + t);
+          const int t = L::kStep * (2 * u + e) + g * 4, there = min(max(left - t, 0), 4);
+          w[e] = *reinterpret_cast<const uint64_t*>(tv + (n * kCol + col) * kBlock + t);
           w[e] &= there == 4 ? ~uint64_t{0} : (uint64_t{1} << (16 * there)) - 1;
         }
         struct Two { uint64_t x, y; };
         const half8 v = __builtin_bit_cast(half8, Two{w[0], w[1]});
         acc[n] = T::mfma(v, hi[u], acc[n]);
-        if constexpr (__is_same(T, BF16)) acc[n] = T::mfma(v, lo[u], acc[n]);
+        if constexpr (!kUnits) acc[n] = T::mfma(v, lo[u], acc[n]);
       }
-    }
   }
 
-  float m = soft.m, l = soft.l;
-  l = rows_sum(l);
-  if (g == 0) {
-    stat[0][wave][col] = m;
-    stat[1][wave][col] = l;
-  }
-  __syncthreads();
-  float top = stat[0][0][col];
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) top = fmaxf(top, stat[0][w][col]);
-  const float mine = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - top);
-#pragma unroll
-  for (int n = 0; n < kN; ++n)
-    *reinterpret_cast<f32x4*>(&part[wave][col][n * 16 + g * 4]) =
-        f32x4{acc[n][0] * mine, acc[n][1] * mine, acc[n][2] * mine, acc[n][3] * mine};
-  __syncthreads();
+  // 4 columns of one row, from its sums over the part
   const bool only = visits.count <= a.per;
-  for (int i = tid; i < 16 * D / 4; i += kThreads) {
-    const int c = i / (D / 4), d = (i % (D / 4)) * 4, r = r0 + c;
-    if (r >= rows) break;
-    float best = stat[0][0][c], sum = 0.f;
-#pragma unroll
-    for (int w = 1; w < kWaves; ++w) best = fmaxf(best, stat[0][w][c]);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float x = stat[0][w][c];
-      sum += x == -__builtin_inff() ? 0.f : stat[1][w][c] * __builtin_amdgcn_exp2f(x - best);
-      const f32x4 y = *reinterpret_cast<const f32x4*>(&part[w][c][d]);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += y[e];
-    }
-    const int64_t to = (s.row0 + r / a.group) * a.n_q + head * a.group + r % a.group;
+  auto store = [&](int r, int d, f32x4 o, float top, float sum) __attribute__((always_inline)) {
+    const int token = a.over(r);
+    const int64_t to = static_cast<int64_t>(s.row0 + token) * a.n_q + head * a.group + r - token * a.group;
     if (only) {
       const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // a sum that is NaN stays one
       u32x2 w;
@@ -709,8 +804,48 @@ __global__ __launch_bounds__(kThreads, 3) void cache_attn_kernel(AttnArgs a) {
       *reinterpret_cast<u32x2*>(a.out + to * D + d) = w;
     } else {
       *reinterpret_cast<f32x4*>(a.part_o + (to * a.splits + split) * D + d) = o;
-      if (d == 0) a.part_ml[to * a.splits + split] = make_float2(best, sum);
+      if (d == 0) a.part_ml[to * a.splits + split] = make_float2(top, sum);
     }
+  };
+  // the i-th four output columns of a lane, of D / (4 wavefronts' lanes a column)
+  auto out4 = [&](int i, float by) __attribute__((always_inline)) {
+    constexpr int kFours = L::kEach / 4;
+    const Tile& o = acc[i / kFours];
+    const int e = i % kFours * 4;
+    return f32x4{o[e] * by, o[e + 1] * by, o[e + 2] * by, o[e + 3] * by};
+  };
+  constexpr int kFours = L::kOuts * L::kEach / 4;
+  auto out_at = [&](int i) { return kCol == 16 ? i * 16 + g * 4 : i * 8 + g * 4; };
+  l = L::sum_of(l);
+  const int mine = wide * kCol + col;
+  if (g == 0) {
+    stat[0][deep][mine] = ref;
+    stat[1][deep][mine] = l;
+  }
+  __syncthreads();
+  float best = stat[0][0][mine];
+#pragma unroll
+  for (int w = 1; w < kDeep; ++w) best = fmaxf(best, stat[0][w][mine]);
+  const float by = ref == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ref - best) * unit;
+#pragma unroll
+  for (int i = 0; i < kFours; ++i) *reinterpret_cast<f32x4*>(&part[deep][mine][out_at(i)]) = out4(i, by);
+  __syncthreads();
+  for (int i = tid; i < kCols * D / 4; i += kThreads) {
+    const int c = i / (D / 4), d = (i % (D / 4)) * 4, r = r0 + c;
+    if (r >= rows) break;
+    float top = stat[0][0][c], sum = 0.f;
+#pragma unroll
+    for (int w = 1; w < kDeep; ++w) top = fmaxf(top, stat[0][w][c]);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kDeep; ++w) {
+      const float x = stat[0][w][c];
+      sum += x == -__builtin_inff() ? 0.f : stat[1][w][c] * __builtin_amdgcn_exp2f(x - top);
+      const f32x4 y = *reinterpret_cast<const f32x4*>(&part[w][c][d]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += y[e];
+    }
+    store(r, d, o, top, sum);
   }
 }
 
@@ -726,96 +861,159 @@ __device__ __forceinline__ float lanes_sum(float x) {
   }));
 }
 
-// The parts of one row and head, joined in their order: 4 kLanes columns a workgroup, its groups of
-// kLanes threads take every so many-th part, all loads on their way before the weights are known.
-template <class T, int D, int kLanes>
+// The parts of a row and head, joined in their order. kRows = 0: a workgroup has 32 columns of one, its
+// 32 groups of 8 threads take every 32nd part (up to 256). Else a wavefront has all D columns of kRows of
+// them, its groups of D / 4 lanes take every second part (fourth with 64 columns), kEach each. All loads are
+// on their way before the weights are known.
+template <class T, int D, int kRows, int kEach>
 __global__ __launch_bounds__(kThreads) void cache_join_kernel(AttnArgs a) {
-  constexpr int kGroups = kThreads / kLanes, kEach = 8, kSlices = D / (4 * kLanes);
-  __shared__ float weight[kSplits];
-  __shared__ f32x4 sums[kGroups][kLanes];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int slice = static_cast<int>(blockIdx.x % kSlices);
-  int rest = static_cast<int>(blockIdx.x / kSlices);
-  const int qh = rest % a.n_q;
-  rest /= a.n_q;
-  const int at = rest % a.max_new, seq = rest / a.max_new;
-  const Span s = span_of(a.bounds, a.past, seq, a.n_rows, a.max_new, a.max_len);
-  if (at >= s.n) return;
-  const int rows = s.n * a.group, r0 = (at * a.group + qh % a.group) / 16 * 16;
-  const Visits visits(s.past + r0 / a.group, s.past + min(r0 + 15, rows - 1) / a.group, a.window, a.sinks);
-  const int parts = (visits.count + a.per - 1) / a.per;
-  if (parts <= 1) return;  // written by its one part
-  const int64_t to = (s.row0 + at) * a.n_q + qh;
+  constexpr bool kWide = kRows == 0;
+  constexpr int kLanes = kWide ? 8 : D / 4, kGroups = (kWide ? kThreads : kWave) / kLanes, kR = kWide ? 1 : kRows;
+  constexpr int kSlices = kWide ? D / 32 : 1, kPer = kWide ? kSplits / kWave : 1;
+  __shared__ float weight[kWide ? kSplits : 1];
+  __shared__ f32x4 sums[kWide ? kGroups : 1][kLanes];
+  const int lane = threadIdx.x & 63, tid = kWide ? threadIdx.x : lane;
+  uint32_t item = kWide ? blockIdx.x : blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int slice = static_cast<int>(item % kSlices);
+  item = item / kSlices * kR;
   const int grp = tid / kLanes, d = slice * 4 * kLanes + (tid % kLanes) * 4;
-  const float* p = a.part_o + to * a.splits * D + d;
-  f32x4 o[kEach];
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int j = grp + i * kGroups;
-    o[i] = j < parts ? *reinterpret_cast<const f32x4*>(p + static_cast<int64_t>(j) * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+  int seq, at, qh;
+  {
+    const uint32_t rest = item / a.n_q;
+    qh = static_cast<int>(item - rest * a.n_q);
+    seq = static_cast<int>(rest / a.max_new);
+    at = static_cast<int>(rest) - seq * a.max_new;
   }
-  // every wavefront takes all weights
-  constexpr int kPer = kSplits / kWave;
-  float2 ml[kPer];
-  float top = -__builtin_inff();
+  int64_t to[kR];
+  int parts[kR];
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int j = lane + i * kWave;
-    ml[i] = j < parts ? a.part_ml[to * a.splits + j] : make_float2(-__builtin_inff(), 0.f);
-    top = fmaxf(top, ml[i].x);
-  }
-  top = lanes_max(top);
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const float w = ml[i].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - top);
-    sum += ml[i].y * w;
-    if (tid < kWave) weight[lane + i * kWave] = w;
-  }
-  sum = lanes_sum(sum);
-  __syncthreads();
-  f32x4 total = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const int j = grp + i * kGroups;
-    if (j < parts) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) total[e] += weight[j] * o[i][e];
+  for (int k = 0; k < kR; ++k) {
+    to[k] = parts[k] = 0;
+    if (seq < a.c.n_seqs) {
+      const Span s = span_of(a.bounds, a.past, seq, a.n_rows, a.max_new, a.max_len);
+      if (at < s.n) {
+        const int rows = s.n * a.group, r0 = (at * a.group + qh - a.over(qh) * a.group) & ~(a.cols - 1);
+        const Visits visits(s.past + a.over(r0), s.past + a.over(min(r0 + a.cols, rows) - 1), a.window, a.sinks);
+        parts[k] = (visits.count + a.per - 1) / a.per;
+        to[k] = static_cast<int64_t>(s.row0 + at) * a.n_q + qh;
+      }
+    }
+    if (++qh == a.n_q) {
+      qh = 0;
+      if (++at == a.max_new) {
+        at = 0;
+        ++seq;
+      }
     }
   }
-  sums[grp][tid % kLanes] = total;
-  __syncthreads();
-  if (grp != 0) return;
-  const int used = min(kGroups, parts);
-  for (int i = 1; i < used; ++i) {
-    const f32x4 x = sums[i][tid];
+  f32x4 o[kR][kEach];
+  float2 ml[kR][kPer];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) total[e] += x[e];
+  for (int k = 0; k < kR; ++k) {
+    if (parts[k] <= 1) continue;  // nothing, or written by its one part
+    const float* p = a.part_o + to[k] * a.splits * D + d;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int j = grp + i * kGroups;
+      o[k][i] = j < parts[k] ? *reinterpret_cast<const f32x4*>(p + static_cast<int64_t>(j) * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    // every wavefront takes all weights
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int j = lane + i * kWave;
+      ml[k][i] = j < parts[k] ? a.part_ml[to[k] * a.splits + j] : make_float2(-__builtin_inff(), 0.f);
+    }
   }
-  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-  u32x2 w;
-  w.x = T::down(total[0] * inv) | static_cast<uint32_t>(T::down(total[1] * inv)) << 16;
-  w.y = T::down(total[2] * inv) | static_cast<uint32_t>(T::down(total[3] * inv)) << 16;
-  *reinterpret_cast<u32x2*>(a.out + to * D + d) = w;
+#pragma unroll
+  for (int k = 0; k < kR; ++k) {
+    if (parts[k] <= 1) continue;
+    float top = -__builtin_inff(), w[kPer], sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) top = fmaxf(top, ml[k][i].x);
+    top = lanes_max(top);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      w[i] = ml[k][i].x == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ml[k][i].x - top);
+      sum += ml[k][i].y * w[i];
+    }
+    sum = lanes_sum(sum);
+    f32x4 total = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (kWide) {
+      if (threadIdx.x < kWave) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) weight[lane + i * kWave] = w[i];
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int j = grp + i * kGroups;
+      const float by = kWide ? weight[kWide ? j : 0] : __shfl(w[0], j & 63, kWave);
+      if (j < parts[k]) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) total[e] += by * o[k][i][e];
+      }
+    }
+    if constexpr (kWide) {
+      sums[grp][tid % kLanes] = total;
+      __syncthreads();
+      if (grp != 0) return;
+      const int used = min(kGroups, parts[k]);
+      for (int i = 1; i < used; ++i) {
+        const f32x4 x = sums[i][tid];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) total[e] += x[e];
+      }
+    } else {
+#pragma unroll
+      for (int off = kLanes; off < kWave; off *= 2)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) total[e] += __shfl_xor(total[e], off, kWave);
+    }
+    if (grp == 0) {
+      const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+      u32x2 out;
+      out.x = T::down(total[0] * inv) | static_cast<uint32_t>(T::down(total[1] * inv)) << 16;
+      out.y = T::down(total[2] * inv) | static_cast<uint32_t>(T::down(total[3] * inv)) << 16;
+      *reinterpret_cast<u32x2*>(a.out + to[k] * D + d) = out;
+    }
+  }
 }
 
-constexpr int kPerCu = 3;  // workgroups of the attention that a CU holds
+constexpr int kMost = 10;
 
-// How an attention call splits its pages: enough workgroups to fill every CU, parts of at least a page
-// per wavefront.
+// How an attention call is cut: rows of a tile, tiles of a KV head at most, parts of the pages and pages of
+// a part.
 struct Plan {
-  int64_t tiles, splits, per;
+  int wide;  // 0: 16 rows a workgroup, one tile a sequence; 1, 2: kWide of 32 each
+  int64_t cols, tiles, splits, per;
 };
-Plan plan_of(int64_t n_seqs, int64_t kv, int64_t group, int64_t max_new, int64_t max_len, int64_t window,
-             int64_t sinks) {
+Plan plan_of(int64_t n_rows, int64_t n_seqs, int64_t kv, int64_t group, int64_t max_new, int64_t max_len,
+             int64_t window, int64_t sinks) {
   Plan p;
   sinks = std::min(sinks, max_len);
-  p.tiles = (max_new * group + 15) / 16;
-  int64_t visits = (max_len + kBlock - 1) / kBlock;
-  if (window > 0) visits = std::min(visits, (window + 15 + 63) / kBlock + 1 + (sinks + kBlock - 1) / kBlock);
-  const int64_t base = n_seqs * kv * p.tiles;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kSplits, kPerCu * device_cus() / std::max<int64_t>(base, 1)));
-  p.per = std::max<int64_t>((visits + want - 1) / want, kWaves);
+  const int64_t rows = max_new * group, cus = device_cus();
+  // a sequence's last tile may be part of one; no more rows than there are
+  auto tiles_of = [&](int64_t cols) {
+    return std::min(n_seqs * ((rows + cols - 1) / cols), (n_rows * group + cols - 1) / cols + n_seqs);
+  };
+  auto visits_of = [&](int64_t cols) {
+    const int64_t all = (max_len + kBlock - 1) / kBlock;
+    return window > 0 ? std::min(all, (window + cols - 1 + kBlock - 1) / kBlock + 1 + (sinks + kBlock - 1) / kBlock)
+                      : all;
+  };
+  // Rows past 16: tiles of 64, whose pages come through the L1 for two wavefronts, where the pages' way from
+  // the L2 sets the time; tiles of 32 below that, which spread over more CUs
+  p.wide = rows <= 16 ? 0 : rows <= 32 || kv * tiles_of(64) * visits_of(64) < 24 * cus ? 1 : 2;
+  p.cols = p.wide ? 32 * p.wide : 16;
+  p.tiles = p.wide ? tiles_of(p.cols) : n_seqs;
+  const int64_t visits = visits_of(p.cols), base = std::max<int64_t>(kv * p.tiles, 1);
+  // Two workgroups a CU, parts of at least a page per wavefront. Parts of 16-row tiles have at most kMost
+  // pages: sequences of other lengths than the longest leave CUs idle at the end, a short part less.
+  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kSplits, 2 * cus / base));
+  p.per = (visits + want - 1) / want;
+  if (!p.wide) p.per = std::max(std::min<int64_t>(p.per, kMost), (visits + kSplits - 1) / kSplits);
+  p.per = std::max<int64_t>(p.per, kWaves);
   p.splits = std::max<int64_t>((visits + p.per - 1) / p.per, 1);
   return p;
 }
@@ -836,7 +1034,7 @@ using namespace talm;
 
 #define TALM_CACHE_KERNEL(name, grid, args)                                                                   \
   do {                                                                                                        \
-    const dim3 g_(static_cast<unsigned>(grid)), b_(kThreads);                                                 \
+    const dim3 g_(grid), b_(kThreads);                                                 \
     if (dtype == TALM_F16 && head_dim == 128) name(F16, 128, g_, b_, args);                                   \
     else if (dtype == TALM_F16) name(F16, 64, g_, b_, args);                                                  \
     else if (head_dim == 128) name(BF16, 128, g_, b_, args);                                                  \
@@ -886,7 +1084,7 @@ TALM_API int talm_cache_write(const uint16_t* k, int64_t k_stride_tok, int64_t k
     else                                                                                    \
       hipLaunchKernelGGL((cache_write_kernel<T, D, false>), grid, block, 0, st, args);      \
   } while (0)
-  TALM_CACHE_KERNEL(LAUNCH, a.kv_items + turns, a);
+  TALM_CACHE_KERNEL(LAUNCH, static_cast<unsigned>(a.kv_items + turns), a);
 #undef LAUNCH
   return check_launch("cache_write");
 }
@@ -911,7 +1109,7 @@ TALM_API int talm_cache_read(const uint8_t* codes, const float* scales, const ui
   if (items > 0x7fffffff) return fail(TALM_EINVAL, "cache_read: too many tokens");
   const hipStream_t st = as_stream(stream);
 #define LAUNCH(T, D, grid, block, args) hipLaunchKernelGGL((cache_read_kernel<T, D>), grid, block, 0, st, args)
-  TALM_CACHE_KERNEL(LAUNCH, items, a);
+  TALM_CACHE_KERNEL(LAUNCH, static_cast<unsigned>(items), a);
 #undef LAUNCH
   return check_launch("cache_read");
 }
@@ -931,7 +1129,7 @@ TALM_API int64_t talm_cache_attn_workspace(int64_t n_rows, int32_t n_q_heads, in
                                            int32_t sinks) {
   if (!attn_shape(n_rows, n_q_heads, n_kv_heads, head_dim, n_seqs, max_new, max_len, window, sinks)) return -1;
   max_new = static_cast<int32_t>(std::min<int64_t>(max_new, n_rows));
-  const Plan p = plan_of(n_seqs, n_kv_heads, n_q_heads / n_kv_heads, max_new, max_len, window, sinks);
+  const Plan p = plan_of(n_rows, n_seqs, n_kv_heads, n_q_heads / n_kv_heads, max_new, max_len, window, sinks);
   return p.splits > 1 ? n_rows * n_q_heads * p.splits * (head_dim + 2) * static_cast<int64_t>(sizeof(float)) : 0;
 }
 
@@ -960,33 +1158,57 @@ TALM_API int talm_cache_attn(const uint16_t* q, int64_t q_stride_tok, int64_t q_
     return fail(TALM_EINVAL, "cache_attn: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                 (long long)need);
   max_new = static_cast<int32_t>(std::min<int64_t>(max_new, n_rows));
-  const Plan p = plan_of(n_seqs, n_kv_heads, n_q_heads / n_kv_heads, max_new, max_len, window, sinks);
+  const Plan p = plan_of(n_rows, n_seqs, n_kv_heads, n_q_heads / n_kv_heads, max_new, max_len, window, sinks);
   float* part_o = static_cast<float*>(workspace);
-  AttnArgs a{Cache{codes, scales, tail, table, n_pages, width, n_seqs, n_kv_heads}, q, q_stride_tok, q_stride_head,
-             n_rows, n_q_heads, n_q_heads / n_kv_heads, bounds, past, max_new, std::min(max_len, width * kBlock),
-             scale * 1.44269504088896340736f, window, std::min(sinks, max_len), static_cast<int>(p.tiles), static_cast<int>(p.splits),
-             static_cast<int>(p.per), out, part_o,
+  // n / group for n < 2^30 as (n magic) >> e, magic = ceil(2^e / group), e = 30 + ceil(log2 group), both
+  // shifted up to a product's upper half (group is at most 2^16, so magic is below 2^32)
+  const int64_t group = n_q_heads / n_kv_heads;
+  int e = 30;
+  while ((int64_t{1} << (e - 30)) < group) ++e;
+  uint64_t magic = ((uint64_t{1} << e) + group - 1) / group;
+  while (e < 32) {
+    magic <<= 1;
+    ++e;
+  }
+  AttnArgs a{Cache{codes, scales, tail, table, n_pages, width, n_seqs, n_kv_heads}, bounds, past,
+             static_cast<int>(n_rows), max_new, std::min(max_len, width * kBlock), n_q_heads, static_cast<int>(group),
+             static_cast<int>(static_cast<uint32_t>(magic)), e - 32, static_cast<int>(p.cols),
+             static_cast<int>(p.splits), static_cast<int>(p.per),
+             p.splits >= 8 ? 7 : p.splits >= 4 ? 3 : p.splits >= 2 ? 1 : 0, p.wide != 0, window,
+             std::min(sinks, max_len), scale * 1.44269504088896340736f, q, q_stride_tok, q_stride_head, out, part_o,
              reinterpret_cast<float2*>(part_o ? part_o + n_rows * n_q_heads * p.splits * head_dim : nullptr)};
-  const int64_t items = static_cast<int64_t>(n_seqs) * n_kv_heads * p.tiles * p.splits;
+  const int64_t items = (p.wide ? p.tiles : 1) * p.splits;
   const int64_t joins = p.splits > 1 ? static_cast<int64_t>(n_seqs) * max_new * n_q_heads : 0;
-  if (items > 0x7fffffff || joins * (head_dim / 32) > 0x7fffffff) return fail(TALM_EINVAL, "cache_attn: too many rows");
+  if (items > 0x7fffffff || joins * (head_dim / 32) > 0x7fffffff || (!p.wide && n_seqs > 65535))
+    return fail(TALM_EINVAL, "cache_attn: too many rows, or more than 65535 sequences of few");
   const hipStream_t st = as_stream(stream);
-#define LAUNCH(T, D, grid, block, args) hipLaunchKernelGGL((cache_attn_kernel<T, D>), grid, block, 0, st, args)
-  TALM_CACHE_KERNEL(LAUNCH, items, a);
+#define LAUNCH(T, D, grid, block, args)                                                    \
+  do {                                                                                     \
+    if (p.wide == 0)                                                                       \
+      hipLaunchKernelGGL((cache_attn_kernel<T, D, 16, 1>), grid, block, 0, st, args);       \
+    else if (p.wide == 1)                                                                  \
+      hipLaunchKernelGGL((cache_attn_kernel<T, D, 32, 1>), grid, block, 0, st, args);       \
+    else                                                                                   \
+      hipLaunchKernelGGL((cache_attn_kernel<T, D, 32, 2>), grid, block, 0, st, args);       \
+  } while (0)
+  TALM_CACHE_KERNEL(LAUNCH, dim3(static_cast<unsigned>(items), n_kv_heads, p.wide ? 1 : n_seqs), a);
 #undef LAUNCH
   if (const int status = check_launch("cache_attn")) return status;
   if (joins == 0) return TALM_OK;
-  // a whole head's columns a workgroup where its groups reach the parts in eight steps, else 32
-  const bool few = p.splits <= 8 * (kThreads / (head_dim / 4));
-  const int64_t slices = few ? 1 : head_dim / 32;
-#define LAUNCH(T, D, grid, block, args)                                                  \
-  do {                                                                                   \
-    if (few)                                                                             \
-      hipLaunchKernelGGL((cache_join_kernel<T, D, D / 4>), grid, block, 0, st, args);    \
-    else                                                                                 \
-      hipLaunchKernelGGL((cache_join_kernel<T, D, 8>), grid, block, 0, st, args);        \
+  // groups of D / 4 lanes in a wavefront; one row's few parts are too little work for it
+  const int lanes = kWave * 4 / head_dim;
+  const int rows = p.splits <= 2 * lanes ? 4 : p.splits <= 8 * lanes ? 1 : 0;
+  const int64_t groups = rows ? (joins + rows * kWaves - 1) / (rows * kWaves) : joins * (head_dim / 32);
+#define LAUNCH(T, D, grid, block, args)                                                   \
+  do {                                                                                    \
+    if (rows == 4)                                                                        \
+      hipLaunchKernelGGL((cache_join_kernel<T, D, 4, 2>), grid, block, 0, st, args);      \
+    else if (rows == 1)                                                                   \
+      hipLaunchKernelGGL((cache_join_kernel<T, D, 1, 8>), grid, block, 0, st, args);      \
+    else                                                                                  \
+      hipLaunchKernelGGL((cache_join_kernel<T, D, 0, 8>), grid, block, 0, st, args);      \
   } while (0)
-  TALM_CACHE_KERNEL(LAUNCH, joins * slices, a);
+  TALM_CACHE_KERNEL(LAUNCH, static_cast<unsigned>(groups), a);
 #undef LAUNCH
   return check_launch("cache_attn");
 }
