@@ -1,5 +1,10 @@
 """An attention layer's keys and values in 8 bits, for a model that answers token by token.
 
+`QuantizedCache` is a model's cache: given as `past_key_values` to a patched Qwen2 (`generate`, or its
+forward), which then keeps its keys and values in 8 bits and attends to them with the kernels here;
+sliding layers with sinks (config.attention_sinks), which transformers' own masks do not know, are
+answered with it too.
+
 `CacheLayer` holds the buffers of one layer and has three operators on the HIP kernels (kvcache.hip,
 talm_cache_write / _read / _attn): new tokens' keys and values are written, quantized block by block
 and turned by their rotary positions on the way; tokens are read back in 16 bits; new tokens' queries
@@ -13,10 +18,14 @@ page of each of a sequence's blocks: pages may lie in any order, and sequences w
 beginning may share complete ones.
 """
 
-import torch
+import contextlib
+import functools
 
-from . import _ops  # noqa: F401 - registers torch.ops.talm.*
-from .engaged import RAN
+import torch
+from transformers import Cache
+
+from . import _ops, unpad  # noqa: F401 - _ops registers torch.ops.talm.*
+from .engaged import ON, RAN
 
 BLOCK = 64
 
@@ -98,3 +107,216 @@ class CacheLayer:
                                              self.tail, self.table, scale, window or 0, sinks)
         RAN["cache_attn"] += 1
         return out
+
+
+def _packed(x):
+    """[B, H, T, D] -> its rows as [1, H, B T, D], a view where the strides allow one."""
+    b, h, t, d = x.shape
+    return x.transpose(1, 2).reshape(b * t, h, d).transpose(0, 1)[None]
+
+
+class QuantizedCache(Cache):
+    """The keys and values of a patched Qwen2 in 8 bits, for `batch` sequences of up to `capacity` tokens:
+
+        cache = QuantizedCache(model.config, batch=4, capacity=4096)
+        model.generate(**inputs, past_key_values=cache)
+
+    Each call's new tokens are those that its attention mask names, one run per sequence (left-padded
+    prompts, as generation has them); padding is neither stored nor attended to. A first call attends to
+    its own 16-bit keys and values where the packed rows' kernels take them (fp16 or bfloat16 heads of
+    128), later ones, and first ones of heads of 64, to the cache. It needs solution.apply(), the "sdpa"
+    attention, and no gradient; it does not reorder, repeat or crop its sequences (beam search, assisted
+    generation), and its calls run eagerly (a step to capture in a HIP graph takes CacheLayer)."""
+
+    is_compileable = False
+
+    def __init__(self, config, batch, capacity, dtype=torch.float16, device="cuda"):
+        super().__init__(layers=[])
+        heads = config.num_attention_heads
+        dim = getattr(config, "head_dim", None) or config.hidden_size // heads
+        self.cache_layers = [CacheLayer.allocate(batch, config.num_key_value_heads, dim, capacity, dtype, device)
+                             for _ in range(config.num_hidden_layers)]
+        self.batch, self.capacity, self.dtype = batch, capacity, dtype
+        self.device = torch.device(device)
+        self.lengths, self.columns = [0] * batch, 0
+        self._step = self._broken = None
+
+    # -- what transformers asks of a cache
+
+    def get_seq_length(self, layer_idx=0):
+        """Columns of the attention mask so far, padding among them."""
+        return self.columns
+
+    def get_mask_sizes(self, query_length, layer_idx=0):
+        return self.columns + int(query_length), 0
+
+    def get_max_length(self, layer_idx=0):
+        return self.capacity
+
+    get_max_cache_shape = get_max_length
+
+    def reset(self):
+        """Empty again, also after a call that failed part-way."""
+        self.lengths, self.columns = [0] * self.batch, 0
+        self._step = self._broken = None
+
+    def _unsupported(self, *args, **kwargs):
+        raise NotImplementedError("QuantizedCache does not reorder, repeat, select, crop or offload its sequences")
+
+    reorder_cache = crop = batch_repeat_interleave = batch_select_indices = offload = _unsupported
+
+    # -- one call of the model
+
+    @contextlib.contextmanager
+    def step(self, config, batch, rows, mask=None):
+        """One forward of `rows` new columns a sequence; `mask` [batch, columns so far + rows] or None (all
+        of them tokens). The sequences grow when it ends; one that fails part-way leaves the cache unusable
+        until `reset`, since some layers hold its tokens."""
+        from .fused_proj import _rows_attention
+
+        if self._broken:
+            raise RuntimeError("QuantizedCache: a call failed part-way, reset() empties the cache")
+        if self._step is not None:
+            raise RuntimeError("QuantizedCache: one call of the model at a time")
+        if torch.is_grad_enabled():
+            raise ValueError("QuantizedCache: the cache has no gradient, call the model under torch.no_grad()")
+        if not _rows_attention(config):
+            raise ValueError('QuantizedCache: the model must be patched (solution.apply()) and use "sdpa" attention')
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("QuantizedCache: its calls run eagerly; capture CacheLayer's operators")
+        if batch != self.batch or rows < 1:
+            raise ValueError(f"QuantizedCache: {rows} tokens of {batch} sequences, made for {self.batch}")
+        runs, padded = _runs(mask, batch, self.columns, rows)
+        new = [end - start for start, end in runs]
+        lengths = [n + m for n, m in zip(self.lengths, new)]
+        if max(lengths) > self.capacity:
+            raise ValueError(f"QuantizedCache: a sequence of {max(lengths)} tokens, made for {self.capacity}")
+        first = not any(self.lengths)
+        # one copy: bounds, past, and for a first call the rows' sequences, padding as sequences of its own
+        bounds = [b * rows + at for b, run in enumerate(runs) for at in run]
+        values = bounds + self.lengths + ([0] + bounds + [batch * rows] if first else [])
+        device = torch.tensor(values, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
+        self._step = _Step(device[:2 * batch].view(batch, 2), device[2 * batch:3 * batch], max(new), max(lengths),
+                           device[3 * batch:] if first else None, rows,
+                           _real(runs, rows, self.device) if padded and not first else None)
+        unpad._cached.append(self)
+        try:
+            yield
+        except BaseException:
+            self._broken = True
+            raise
+        finally:
+            unpad._cached.pop()
+            self._step = None
+        self.lengths, self.columns = lengths, self.columns + rows
+
+    def _layer(self, layer_idx):
+        if self._step is None:
+            raise RuntimeError("QuantizedCache: outside of a patched Qwen2 model's forward (solution.apply())")
+        return self.cache_layers[layer_idx]
+
+    def update(self, key_states, value_states, layer_idx, *args, **kwargs):
+        """New keys and values [B, Hkv, T, D] of one layer; returns them (the attention reads the cache)."""
+        layer, s = self._layer(layer_idx), self._step
+        key_states, value_states = key_states.to(self.dtype), value_states.to(self.dtype)
+        layer.write(_packed(key_states), _packed(value_states), s.bounds, s.past, s.max_new)
+        return key_states, value_states
+
+    def takes(self, query, tables):
+        """Whether `answer` serves the call: not a first one (its keys are needed in 16 bits), of the
+        cache's type, with tables that the write turns by."""
+        return (self._step is not None and self._step.cu is None and query.dtype == self.dtype
+                and tables[0].shape[-1] == query.shape[-1])
+
+    def answer(self, query, key, value, layer_idx, tables, scale, window, sinks):
+        """Attention of new rows [1, H, N, D] that are not turned yet, tables (cos, sin) float32 [N, D]: written
+        with their rotary positions in one launch, then attended. Returns [1, N, Hq, D]."""
+        layer, s = self._layer(layer_idx), self._step
+        turned = layer.write(key, value, s.bounds, s.past, s.max_new, query, tables)
+        return self._clean(layer.attention(turned, s.bounds, s.past, s.max_new, s.max_len, scale, window, sinks))
+
+    def attend(self, module, query, key, value, dropout, scaling, window):
+        """The attention interface of a call with this cache: query [B, Hq, T, D] against the layer's tokens;
+        returns [B, T, Hq, D]."""
+        if dropout:
+            raise ValueError("QuantizedCache: no dropout of attention weights")
+        layer, s = self._layer(module.layer_idx), self._step
+        b, heads, t, d = query.shape
+        scale = scaling if scaling is not None else d ** -0.5
+        sinks = unpad.attention_sinks(module) if window is not None else 0
+        q = _packed(query.to(self.dtype))
+        if s.cu is not None:
+            k, v = _packed(key), _packed(value)
+            if unpad.window_takes(q, k, v):
+                # without a window: one that no sequence is longer than, or the fp16 kernels of training
+                out = unpad.VarlenAttention.apply(q, k, v, s.cu, s.rows, scale) \
+                    if window is None and q.dtype == torch.float16 \
+                    else unpad.window_attention(q, k, v, s.cu, s.rows, scale, window or s.rows, sinks)
+                return out.view(b, t, heads, d)
+        out = layer.attention(q, s.bounds, s.past, s.max_new, s.max_len, scale, window, sinks)
+        return self._clean(out).view(b, t, heads, d)
+
+    def _clean(self, out):
+        """Padding's rows, which no sequence holds, as zeros."""
+        real = self._step.real
+        return out if real is None else torch.where(real, out, 0.0)
+
+
+class _Step:
+    """What the layers of one call share."""
+
+    def __init__(self, bounds, past, max_new, max_len, cu, rows, real):
+        self.bounds, self.past, self.max_new, self.max_len = bounds, past, max_new, max_len
+        self.cu, self.rows, self.real = cu, rows, real
+
+
+def _runs(mask, batch, columns, rows):
+    """Where each sequence's new tokens lie among its `rows` new columns, [(start, end)], and whether any
+    column is padding. Reads the mask on the host."""
+    if mask is None:
+        return [(0, rows)] * batch, False
+    if not isinstance(mask, torch.Tensor) or tuple(mask.shape) != (batch, columns + rows):
+        raise ValueError(f"QuantizedCache: an attention mask [{batch}, {columns + rows}] of the tokens so far and "
+                         "the new ones, or none")
+    new = mask[:, columns:] != 0
+    count = new.sum(1)
+    start = new.to(torch.int8).argmax(1)
+    # a run: as many tokens between the first and the last as there are
+    span = torch.where(count > 0, rows - new.flip(1).to(torch.int8).argmax(1) - start, 0)
+    values = torch.stack((count, start, span)).tolist()
+    if values[0] != values[2]:
+        raise ValueError("QuantizedCache: a sequence's new tokens must be one run of its mask")
+    return [(lo, lo + n) for n, lo in zip(values[0], values[1])], any(n < rows for n in values[0])
+
+
+def _real(runs, rows, device):
+    """[1, B T, 1, 1]: the rows that are tokens."""
+    at = torch.arange(rows)
+    lo, hi = torch.tensor(runs).unbind(1)
+    return ((at >= lo[:, None]) & (at < hi[:, None])).view(1, -1, 1, 1).to(device)
+
+
+def patch_qwen2_cache():
+    """`Qwen2Model.forward` opens the step of a QuantizedCache that it is given, and makes no masks then."""
+    from transformers.models.qwen2 import modeling_qwen2
+
+    cls = modeling_qwen2.Qwen2Model
+    forward = cls.forward
+    ON.add("kv_cache")
+    if getattr(forward, "_talm_cache", False):
+        return
+
+    @functools.wraps(forward)
+    def forward_cached(self, input_ids=None, attention_mask=None, position_ids=None, past_key_values=None,
+                       inputs_embeds=None, **kwargs):
+        if not isinstance(past_key_values, QuantizedCache):
+            return forward(self, input_ids=input_ids, attention_mask=attention_mask, position_ids=position_ids,
+                           past_key_values=past_key_values, inputs_embeds=inputs_embeds, **kwargs)
+        tokens = input_ids if input_ids is not None else inputs_embeds
+        with past_key_values.step(self.config, tokens.shape[0], tokens.shape[1], attention_mask):
+            return forward(self, input_ids=input_ids, attention_mask={"full_attention": None, "sliding_attention": None},
+                           position_ids=position_ids, past_key_values=past_key_values, inputs_embeds=inputs_embeds,
+                           **kwargs)
+
+    forward_cached._talm_cache = True
+    cls.forward = forward_cached

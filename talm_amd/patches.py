@@ -10,6 +10,7 @@ the original code outside the exact situation it was written for. Installed here
   (mlp_save_up.py, opt-in SOLUTION_MLP_SAVE_UP=1);
 - grouped NF4 dequantization of the 4-bit projections (qgroup.py), the LoRA node (lora.py) and
   q|k|v as one projection node with the rotary embedding in place (fused_proj.py);
+- the 8-bit key and value cache of a generating model (kv_cache.py);
 - padding removal with per-row attention (unpad.py) and the fused LM head + cross-entropy of
   the causal LM (fused_head.py, `patch_qwen2_causal_lm` below);
 - the measured hipBLASLt solution table of the decoder's GEMMs (gemm_tuning.py);
@@ -352,6 +353,10 @@ def apply():
 
             patch_sdpa_rows()
             patch_qwen2_causal_lm()
+        with installing("kv_cache"):
+            from .kv_cache import patch_qwen2_cache
+
+            patch_qwen2_cache()
         if _have_trl():
             with installing("fused_head"):
                 from .sft_loss import patch_sft_compute_loss
@@ -387,8 +392,9 @@ def unapply():
                 Linear4bit, LoraLinear):
         cls.forward = _root(cls.forward)
     forward = modeling_qwen2.Qwen2Model.forward
-    if getattr(forward, "_solution_link_norms", False):
-        modeling_qwen2.Qwen2Model.forward = forward.__wrapped__
+    while getattr(forward, "_solution_link_norms", False) or getattr(forward, "_talm_cache", False):
+        forward = forward.__wrapped__
+    modeling_qwen2.Qwen2Model.forward = forward
     modeling_qwen2.apply_rotary_pos_emb = _root(modeling_qwen2.apply_rotary_pos_emb)
     trl = sys.modules.get("trl")
     if trl is not None and hasattr(trl, "SFTTrainer") \

@@ -41,6 +41,7 @@ COMPONENTS = {
     "fused_mlp": "the MLP as one node on the layer group -> the per-projection MLP",
     "attn_block": "q|k|v, attention and o_proj as one node -> the per-node attention",
     "gemv": "a few tokens' products on the NF4 codes -> the dequantized products",
+    "kv_cache": "the 8-bit cache in Qwen2Model's forward -> transformers' caches alone",
     "gemm_table": "measured hipBLASLt solutions (gemm_tuning.py) -> hipBLASLt's heuristic",
 }
 

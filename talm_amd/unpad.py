@@ -23,6 +23,7 @@ from .state import DISABLED, fallback
 
 _rows = []
 _cu = []
+_cached = []  # the 8-bit cache (kv_cache.QuantizedCache) whose model's forward runs
 _ahead = {}  # batch key -> (mask ref, labels ref, pinned host values, event): row statistics
              # copied ahead of time
 _AHEAD_MAX = 4
@@ -394,13 +395,15 @@ def patch_sdpa_rows():
 
     def rows_sdpa(module, query, key, value, attention_mask, dropout=0.0, scaling=None,
                   sliding_window=None, **kwargs):
+        if _cached:
+            return _cached[-1].attend(module, query, key, value, dropout, scaling, sliding_window), None
         sinks = attention_sinks(module) if sliding_window is not None else 0
         if not _rows or query.shape[0] != 1:
             if _rows:
                 FELL_BACK["rows_attn"] += 1
             if sinks:
                 raise ValueError("attention sinks (config.attention_sinks) are served for packed training rows "
-                                 "only: this call's mask does not hold them")
+                                 "and with a QuantizedCache: this call's mask does not hold them")
             return original(module, query, key, value, attention_mask, dropout=dropout,
                             scaling=scaling, sliding_window=sliding_window, **kwargs)
         half = _autocast_half(query)
