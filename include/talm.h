@@ -783,8 +783,8 @@ int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, const uint8_
  * It reads the open block from the tail: calls that write one sequence must be in order.
  *
  * talm_cache_read puts tokens past[b] + i back into k, v [n_rows, n_kv, D] dense, of a cache whose sequences
- * hold length[b] tokens; tokens behind them read as zeros. A magnitude that a code rounded past the largest
- * fp16 number reads as that number.
+ * hold length[b] tokens; tokens behind them read as zeros. A magnitude that a code rounded past the type's
+ * largest number reads as that number.
  *
  * talm_cache_attn: out [n_rows, n_q, D] dense, row i of sequence b = softmax(scale q K^T) V over the cached tokens
  * j <= past[b] + i, with a window (> 0) only those with past[b] + i - j < window or j < sinks; zeros where it sees

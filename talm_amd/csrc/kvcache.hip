@@ -234,10 +234,15 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(WriteArgs a) {
     *reinterpret_cast<u32x4*>(a.q_out + rh * D + d) = u32x4{w[0], w[1], w[2], w[3]};
     return;
   }
-  const int j = static_cast<int>(blockIdx.x % a.chunks);
-  const int rest = static_cast<int>(blockIdx.x / a.chunks);
-  const int which = rest & 1, head = (rest >> 1) % a.c.kv, seq = (rest >> 1) / a.c.kv;
-  const Span s = span_of(a.bounds, a.past, seq, a.n_rows, a.max_new, a.max_len);
+  const int rest = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.chunks));
+  const int j = static_cast<int>(blockIdx.x) - rest * a.chunks;
+  const int seq = (rest >> 1) / a.c.kv, head = (rest >> 1) - seq * a.c.kv, which = rest & 1;
+  // the arguments in one cache miss, the sequence's numbers in the next
+  asm volatile("" ::"s"(a.bounds), "s"(a.past), "s"(a.n_rows), "s"(a.max_new), "s"(a.max_len), "s"(a.tail),
+               "s"(a.k), "s"(a.k_tok), "s"(a.k_head), "s"(a.v), "s"(a.v_tok), "s"(a.v_head));
+  const int lo_row = a.bounds[2 * seq], hi_row = a.bounds[2 * seq + 1], held = a.past[seq];
+  asm volatile("" ::"s"(lo_row), "s"(hi_row), "s"(held));
+  const Span s = span_of(lo_row, hi_row, held, static_cast<int>(a.n_rows), a.max_new, a.max_len);
   const int len = s.past + s.n;
   const int block = s.past / kBlock + j, last = len / kBlock;  // last: the open block, perhaps empty
   if (s.n == 0 || (j > 0 && block >= last)) return;
@@ -254,28 +259,49 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(WriteArgs a) {
   };
   if (block < last) {
     const int64_t page = a.c.page(seq, block);
-    // the block to LDS: pieces of 8 columns, a row's behind each other
+    // the block to LDS: what the tail has of it in 16-byte pieces (8 columns of a key, 8 tokens of a
+    // column of the values), then the new tokens in pieces of 8 columns
     float top = 0.f;
-    for (int i = tid; i < kBlock * kPer; i += kThreads) {
-      const int t = i / kPer, d = (i % kPer) * 8, at = block * kBlock + t;
+    const int old = max(s.past - block * kBlock, 0);
+    u32x4 x[kBlock * kPer / kThreads];
+    if (old > 0) {
+#pragma unroll
+      for (int n = 0; n < kBlock * kPer / kThreads; ++n)
+        x[n] = reinterpret_cast<const u32x4*>(tail)[n * kThreads + tid];
+    }
+    for (int i = old * kPer + tid; i < kBlock * kPer; i += kThreads) {
+      const int t = i / kPer, d = (i % kPer) * 8;
       uint32_t w[4];
-      if (at < s.past) {
-        if (which == 0) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(tail + t * D + d);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = x[e];
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w[e] = tail[(d + 2 * e) * kBlock + t] |
-                   static_cast<uint32_t>(tail[(d + 2 * e + 1) * kBlock + t]) << 16;
-        }
-      } else {
-        fresh(at, d, w);
-      }
+      fresh(block * kBlock + t, d, w);
       top = top_of<T>(w, top);
 #pragma unroll
       for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(&tile[t][d + 2 * e]) = w[e];
+    }
+    if (old > 0) {
+#pragma unroll
+      for (int n = 0; n < kBlock * kPer / kThreads; ++n) {
+        const int i = n * kThreads + tid;
+        if (which == 0) {
+          const int t = i / kPer, d = (i % kPer) * 8;
+          uint32_t w[4] = {x[n].x, x[n].y, x[n].z, x[n].w};
+          if (t < old) {
+            top = top_of<T>(w, top);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<uint32_t*>(&tile[t][d + 2 * e]) = w[e];
+          }
+        } else {
+          const int d = i / (kBlock / 8), t = (i % (kBlock / 8)) * 8;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const uint16_t y = static_cast<uint16_t>(x[n][e / 2] >> (16 * (e % 2)));
+            if (t + e < old) {
+              const float z = fabsf(T::up(y));
+              if (z < __builtin_inff()) top = fmaxf(top, z);
+              tile[t + e][d] = y;
+            }
+          }
+        }
+      }
     }
     top = wave_max(top);
     if (lane == 0) tops[tid / kWave] = top;
@@ -342,71 +368,92 @@ struct ReadArgs {
   uint16_t* v;
 };
 
-// code * scale in 16 bits. In fp16 a value just under 65504 may have been rounded up to 65536, which
-// the type does not hold: its largest number stands for it.
+// A lane's 16 codes times their scale in 16 bits. A value near the type's largest number may have been rounded
+// up to a power of two that the type does not hold (with the largest scale only): its largest number
+// stands for it.
 template <class T>
-__device__ __forceinline__ uint16_t held(float code, float scale) {
-  float x = code * scale;
-  if constexpr (__is_same(T, F16)) {
-    if (fabsf(x) > 65504.f) x = copysignf(65504.f, x);
+__device__ __forceinline__ void held(u32x4 w, float scale, uint32_t (&out)[8]) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (__is_same(T, F16)) {
+      out[2 * e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[e], scale, false));
+      out[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[e], scale, true));
+    } else {
+      out[2 * e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[e], scale, false));
+      out[2 * e + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[e], scale, true));
+    }
   }
-  return T::down(x);
+  constexpr uint32_t kInf = __is_same(T, F16) ? 0x7c00u : 0x7f80u;
+  if (scale >= (__is_same(T, F16) ? 0x1p8f : 0x1p120f)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if ((out[e] & 0x7fffu) == kInf) out[e] -= 1;
+      if ((out[e] & 0x7fff0000u) == kInf << 16) out[e] -= 0x10000u;
+    }
+  }
 }
 
-// One workgroup: one block of one sequence, one KV head, keys or values.
+// One workgroup: one block of one sequence, one KV head, keys or values. A lane's 16 keys are one token's
+// columns and go where they belong; its values are 16 tokens of one column and are turned in LDS.
 template <class T, int D>
 __global__ __launch_bounds__(kThreads) void cache_read_kernel(ReadArgs a) {
-  constexpr int kPer = D / 8;
-  __shared__ alignas(16) uint16_t tile[kBlock][D + 2];
+  constexpr int kPer = D / 8, kEach = kBlock * D / 16 / kThreads;
+  __shared__ alignas(16) uint16_t tile[kBlock][D + 8];
   const int tid = threadIdx.x;
   const int j = static_cast<int>(blockIdx.x % a.chunks);
   const int rest = static_cast<int>(blockIdx.x / a.chunks);
   const int which = rest & 1, head = (rest >> 1) % a.c.kv, seq = (rest >> 1) / a.c.kv;
   const Span s = span_of(a.bounds, a.past, seq, a.n_rows, a.max_new, a.max_len);
   const int len = min(max(a.length[seq], 0), a.max_len);
-  const int block = s.past / kBlock + j;
-  const int lo = max(block * kBlock, s.past), hi = min((block + 1) * kBlock, s.past + s.n);
+  const int block = s.past / kBlock + j, first = block * kBlock;
+  const int lo = max(first, s.past), hi = min(first + kBlock, s.past + s.n);
   if (lo >= hi) return;
-  uint16_t* dst = (which ? a.v : a.k) + static_cast<int64_t>(s.row0 - s.past) * (a.c.kv * D) + head * D;
   const int64_t pitch = static_cast<int64_t>(a.c.kv) * D;
+  // token t's row
+  uint16_t* dst = (which ? a.v : a.k) + static_cast<int64_t>(s.row0 - s.past) * pitch + head * D;
   const int64_t page = block < len / kBlock ? a.c.page(seq, block) : -1;
-  const bool open = block == len / kBlock;  // the tail's tokens, up to len
-  const uint16_t* tail = a.c.tail + ((static_cast<int64_t>(seq) * 2 + which) * a.c.kv + head) * (kBlock * D);
   if (page >= 0) {
     const int64_t place = (page * 2 + which) * a.c.kv + head;
     const float scale = a.c.scales[place];
     const u32x4* src = reinterpret_cast<const u32x4*>(a.c.codes + place * (kBlock * D));
-    for (int i = tid; i < kBlock * D / 16; i += kThreads) {
-      const int row = i & 15, g = (i >> 4) & 3, outer = i >> 6;
-      const u32x4 w = src[i];
-      constexpr int kC = D / 64;
+    u32x4 w[kEach];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+    for (int n = 0; n < kEach; ++n) w[n] = __builtin_nontemporal_load(src + n * kThreads + tid);
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          // the byte selector is an immediate
-          const float x = b == 0   ? __builtin_amdgcn_cvt_f32_fp8(w[e], 0)
-                          : b == 1 ? __builtin_amdgcn_cvt_f32_fp8(w[e], 1)
-                          : b == 2 ? __builtin_amdgcn_cvt_f32_fp8(w[e], 2)
-                                   : __builtin_amdgcn_cvt_f32_fp8(w[e], 3);
-          const int t = which ? e * 16 + g * 4 + b : (outer / kC) * 16 + row;
-          const int d = which ? outer * 16 + row : (outer % kC) * 64 + g * 16 + 4 * e + b;
-          tile[t][d] = held<T>(x, scale);
+    for (int n = 0; n < kEach; ++n) {
+      const int i = n * kThreads + tid, row = i & 15, g = (i >> 4) & 3, outer = i >> 6;
+      uint32_t x[8];
+      held<T>(w[n], scale, x);
+      if (which == 0) {
+        constexpr int kC = D / 64;
+        const int at = first + (outer / kC) * 16 + row, d = (outer % kC) * 64 + g * 16;
+        if (at >= lo && at < hi) {
+          u32x4* to = reinterpret_cast<u32x4*>(dst + at * pitch + d);
+          to[0] = u32x4{x[0], x[1], x[2], x[3]};
+          to[1] = u32x4{x[4], x[5], x[6], x[7]};
         }
+      } else {
+        const int d = outer * 16 + row;
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          tile[e / 4 * 16 + g * 4 + e % 4][d] = static_cast<uint16_t>(x[e / 2] >> (16 * (e % 2)));
       }
     }
+    if (which == 0) return;
   } else {
+    // the open block's tokens from the tail (the keys in the order of the tile, the values transposed),
+    // zeros behind them and where there is no page
+    const bool open = block == len / kBlock;
+    const uint16_t* tail = a.c.tail + ((static_cast<int64_t>(seq) * 2 + which) * a.c.kv + head) * (kBlock * D);
     for (int i = tid; i < kBlock * D; i += kThreads) {
-      // the keys' tail is in the order of the tile, the values' is transposed
       const int t = which ? i % kBlock : i / D, d = which ? i / kBlock : i % D;
-      tile[t][d] = open && block * kBlock + t < len ? tail[i] : 0;
+      tile[t][d] = open && first + t < len ? tail[i] : 0;
     }
   }
   __syncthreads();
   for (int i = tid; i < (hi - lo) * kPer; i += kThreads) {
     const int at = lo + i / kPer, d = (i % kPer) * 8;
-    const uint32_t* x = reinterpret_cast<const uint32_t*>(&tile[at - block * kBlock][d]);
-    *reinterpret_cast<u32x4*>(dst + at * pitch + d) = u32x4{x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<u32x4*>(dst + at * pitch + d) = *reinterpret_cast<const u32x4*>(&tile[at - first][d]);
   }
 }
 

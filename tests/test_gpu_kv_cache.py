@@ -159,31 +159,40 @@ def test_contents_do_not_depend_on_the_calls():
         assert torch.equal(x, y)
 
 
-@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_codes_of_every_magnitude(dtype):
-    """Blocks of zeros, of subnormals, of the type's largest numbers, with one loud value, on the border of
-    a scale, and every value of a code and halfway between two."""
-    c = Case(1, 1, 64, 64 * 16, dtype)
-    k = torch.randn(64 * 10, 64, generator=c.g)
+def _magnitudes(dtype, g):
+    """Ten blocks [640, 64]: of zeros, of subnormals, of the type's largest numbers, with one loud value, on
+    the border of a scale, and every value of a code and halfway between two."""
+    k = torch.randn(64 * 10, 64, generator=g)
     big = torch.finfo(dtype).max
     k[0:64] = 0
     k[64:128] *= 2.0 ** -20 if dtype == torch.float16 else 2.0 ** -120
     k[128:192] = big * torch.linspace(-1, 1, 64)
     k[192:256] *= 2.0 ** -6
     k[200, 5] = 300.0
-    k[256:320] = 448.0 * torch.rand(64, 64, generator=c.g)  # a scale of 1 exactly
+    k[256:320] = 448.0 * torch.rand(64, 64, generator=g)  # a scale of 1 exactly
     k[256, 0] = 448.0
     k[320:384] = k[256:320]
-    k[330, 1] = 448.5 if dtype == torch.float16 else 450.0   # the next scale
+    k[330, 1] = 448.5 if dtype == torch.float16 else 450.0  # the next scale
     codes = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).float()
     codes = codes[codes.isfinite()].sort().values
-    k[384:448].view(-1)[:254] = codes                        # every code, and the ties between them
+    k[384:448].view(-1)[:254] = codes                       # every code, and the ties between them
     k[384:448].view(-1)[300:553] = (codes[1:] + codes[:-1]) / 2
     k[448:512] = -0.0
-    k[512:576] = torch.finfo(dtype).smallest_normal * torch.rand(64, 64, generator=c.g)
-    k = k.to(dtype).cuda()[None, None]
-    c.append([640], k=k, v=k.flip(2).contiguous())
+    k[512:576] = torch.finfo(dtype).smallest_normal * torch.rand(64, 64, generator=g)
+    return k.to(dtype).cuda()[None, None]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_codes_of_every_magnitude(dtype):
+    c = Case(1, 1, 64, 64 * 16, dtype)
+    k = _magnitudes(dtype, c.g)
+    v = k.flip(2).contiguous()
+    c.append([640], k=k, v=v)
     c.check_held()
+    one = torch.tensor([640], dtype=torch.int32).cuda()
+    got = c.layer.read(one, torch.tensor([[0, 640]], dtype=torch.int32).cuda(), one * 0, 640, 640)
+    for x, want in zip(got, c.values(0, torch.finfo(dtype).max)):
+        np.testing.assert_array_equal(x[0].double().cpu().numpy(), want)
 
 
 def test_values_that_are_not_finite_are_nan_in_a_page():
@@ -274,12 +283,13 @@ def test_read_back(kv, dim, dtype):
         assert all((o[torch.from_numpy(free).cuda()] == 7.0).all() for o in out)
 
 
-def test_read_saturates_at_the_largest_number():
-    c = Case(1, 1, 64, 64)
-    c.append([64], k=torch.full((1, 1, 64, 64), 65504.0, dtype=torch.float16, device="cuda"))
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_read_saturates_at_the_largest_number(dtype):
+    c, most = Case(1, 1, 64, 64, dtype), torch.finfo(dtype).max
+    c.append([64], k=torch.full((1, 1, 64, 64), most, dtype=dtype, device="cuda"))
     one = torch.tensor([64], dtype=torch.int32).cuda()
     k, _ = c.layer.read(one, torch.tensor([[0, 64]], dtype=torch.int32).cuda(), one * 0, 64, 64)
-    assert (k == 65504.0).all()
+    assert (k == most).all()
 
 
 @pytest.mark.parametrize("heads,kv,dim,dtype", [
