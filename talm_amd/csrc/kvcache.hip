@@ -700,9 +700,8 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
     const float base = ref == -__builtin_inff() ? 0.f : ref;  // its weights are exp2(-inf - 0) = 0
 #pragma unroll
     for (int i = 0; i < L::kLane; ++i) {
-      const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(st[i / L::kEach][i % L::kEach], c, -base));
-      st[i / L::kEach][i % L::kEach] = x;
-      l += x;
+      st[i / L::kEach][i % L::kEach] =
+          __builtin_amdgcn_exp2f(__builtin_fmaf(st[i / L::kEach][i % L::kEach], c, -base));
     }
   };
 
@@ -751,7 +750,8 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
       weigh(a.scale_log2 * k_scale, !all, page >= 0 ? first : 0x7fff0000, kUnits ? unit * inverse(v_scale) : 1.f);
       if constexpr (kUnits) unit = v_scale;
       // P in fp16 whatever the operands' type: the values' codes are exact in it. The error is that of
-      // a rounding to 11 bits, below the output's own.
+      // a rounding to 11 bits, and its sum is that of the rounded weights, so a token that has nearly all
+      // of it keeps its values exactly.
       half8 p[L::kPs];
 #pragma unroll
       for (int u = 0; u < L::kPs; ++u)
@@ -762,6 +762,7 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
               (f32x2{st[i0 / L::kEach][i0 % L::kEach], st[i0 / L::kEach][i0 % L::kEach + 1]}), half2_);
           p[u][e] = w.x;
           p[u][e + 1] = w.y;
+          l = __builtin_amdgcn_fdot2(w, half2_{static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)}, l, false);
         }
       if (page < 0) {
 #pragma unroll
@@ -818,6 +819,7 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
       const uint16_t b = T::down(x);
       hi[i / 8][i % 8] = __builtin_bit_cast(_Float16, b);
       lo[i / 8][i % 8] = __builtin_bit_cast(_Float16, T::down(x - T::up(b)));
+      l += kUnits ? T::up(b) : x;
     }
 #pragma unroll
     for (int n = 0; n < L::kOuts; ++n)

@@ -3,11 +3,12 @@ bit for bit, what is read back, and attention over it in float64.
 
 Attention's tolerance counts roundings, u half a step of the operands' type (fp16 2^-11, bf16 2^-8):
 P enters its product in fp16 (2^-11 relative, or 2^-25 where it is subnormal; a row's sum is at least 1
-where P is formed), the tail's in two bfloat16 parts or fp16, no coarser; the output is rounded (u, or
-2^-25 where fp16 is subnormal); a score is an fp32 sum of D products (D 2^-24 of the sum of their
-magnitudes, and P relatively so much) with exp2 and the scale's product (2^-19 for exponents up to 2^5);
-P V sums at most T tokens (T 2^-24): (2^-11 + 2 (D 2^-24 max sum |q k| scale + 2^-19) + T 2^-24) P|V| +
-u |out| + 2^-25 T max|V| + 2^-25."""
+where P is formed), the tail's in two bfloat16 parts or fp16, no coarser, and so does its sum: with weights
+p (1 + d), |d| <= 2^-11, the output is off by (sum p d v - out sum p d) / sum p (1 + d), at most
+2^-11 (P|V| + |out|) (1 + 2^-10); the output is rounded (u, or 2^-25 where fp16 is subnormal); a score is
+an fp32 sum of D products (D 2^-24 of the sum of their magnitudes, and P relatively so much) with exp2 and
+the scale's product (2^-19 for exponents up to 2^5); P V sums at most T tokens (T 2^-24):
+(2^-11 + 2 (D 2^-24 max sum |q k| scale + 2^-19) + T 2^-24) (P|V| + |out|) + u |out| + 2^-25 T max|V| + 2^-25."""
 
 import numpy as np
 import pytest
@@ -115,7 +116,7 @@ class Case:
                 want, size, score = oracle.attention(x, k[j], v[j], past[b], scale, window, sinks)
                 length = k.shape[1]
                 rel = 2.0 ** -11 + 2 * (self.dim * 2.0 ** -24 * score + 2.0 ** -19) + length * 2.0 ** -24
-                tol = rel * size + U[self.dtype] * np.abs(want) \
+                tol = rel * (size + np.abs(want)) + U[self.dtype] * np.abs(want) \
                     + sub * (length * np.abs(v[j]).max(initial=0.0) + 1)
                 err = np.abs(got[lo:hi, h] - want)
                 assert not np.isnan(err).any()
