@@ -773,8 +773,8 @@ int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, const uint8_
  * D = head_dim, 64 or 128; dtype TALM_F16 or TALM_BF16, of the tail and every 16-bit operand.
  * A call's new tokens are rows of packed operands: sequence b's are rows bounds[2b] .. bounds[2b + 1] - 1, the
  * i-th of them token past[b] + i. bounds and past lie in device memory; rows outside the operands, past the
- * first max_new of a sequence or behind its width blocks are left out (nothing of them is written). Two sequences
- * may share complete pages. Strides in elements, multiples of 8; 16-byte aligned buffers (scales, table, bounds
+ * first max_new of a sequence or behind its width blocks are left out (nothing of them is written). The
+ * sequences' rows do not overlap. Two sequences may share complete pages. Strides in elements, multiples of 8; 16-byte aligned buffers (scales, table, bounds
  * and past 4). Non-finite values are held as NaN in a page.
  *
  * talm_cache_write puts k, v [n_rows, n_kv, D] into the cache. With cos and sin (f32 [n_rows, D], row stride

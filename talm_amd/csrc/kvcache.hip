@@ -674,6 +674,7 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
   };
   // Weights of a page's (or the tail's) scores; the sums so far follow a new reference and unit.
   auto weigh = [&](float c, bool mask, int first, float ratio) __attribute__((always_inline)) {
+    c = fmaxf(c, 1e-37f);  // never 0: c times a hidden score's -inf is one
     if (mask) {
 #pragma unroll
       for (int i = 0; i < L::kLane; ++i) {
@@ -1058,11 +1059,13 @@ Plan plan_of(int64_t n_rows, int64_t n_seqs, int64_t kv, int64_t group, int64_t 
   p.tiles = p.wide ? tiles_of(p.cols) : n_seqs;
   const int64_t visits = visits_of(p.cols), base = std::max<int64_t>(kv * p.tiles, 1);
   // Two workgroups a CU, parts of at least a page per wavefront. Parts of 16-row tiles have at most kMost
-  // pages: sequences of other lengths than the longest leave CUs idle at the end, a short part less.
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kSplits, 2 * cus / base));
-  p.per = (visits + want - 1) / want;
-  if (!p.wide) p.per = std::max(std::min<int64_t>(p.per, kMost), (visits + kSplits - 1) / kSplits);
-  p.per = std::max<int64_t>(p.per, kWaves);
+  // pages: sequences of other lengths than the longest leave CUs idle at the end, a short part less. All
+  // within 8192 workgroups (those of parts that a sequence lacks cost a start each) and 128 MB of parts.
+  const int64_t most = std::min<int64_t>({kSplits, 8192 / base, (int64_t{1} << 27) / (n_rows * kv * group * 520 + 1)});
+  int64_t want = 2 * cus / base;
+  if (!p.wide) want = std::max(want, (visits + kMost - 1) / kMost);
+  want = std::max<int64_t>(1, std::min(want, most));
+  p.per = std::max<int64_t>((visits + want - 1) / want, kWaves);
   p.splits = std::max<int64_t>((visits + p.per - 1) / p.per, 1);
   return p;
 }

@@ -199,15 +199,14 @@ class QuantizedCache(Cache):
         self._step = _Step(device[:2 * batch].view(batch, 2), device[2 * batch:3 * batch], max(new), max(lengths),
                            device[3 * batch:] if first else None, rows,
                            _real(runs, rows, self.device) if padded and not first else None)
-        unpad._cached.append(self)
+        outer, unpad._cached.step = getattr(unpad._cached, "step", None), self
         try:
             yield
         except BaseException:
             self._broken = True
             raise
         finally:
-            unpad._cached.pop()
-            self._step = None
+            unpad._cached.step, self._step = outer, None
         self.lengths, self.columns = lengths, self.columns + rows
 
     def _layer(self, layer_idx):

@@ -12,6 +12,7 @@ call per row.
 """
 
 import contextlib
+import threading
 import weakref
 
 import torch
@@ -23,7 +24,7 @@ from .state import DISABLED, fallback
 
 _rows = []
 _cu = []
-_cached = []  # the 8-bit cache (kv_cache.QuantizedCache) whose model's forward runs
+_cached = threading.local()  # .step: the 8-bit cache (kv_cache.QuantizedCache) whose model's forward runs here
 _ahead = {}  # batch key -> (mask ref, labels ref, pinned host values, event): row statistics
              # copied ahead of time
 _AHEAD_MAX = 4
@@ -395,8 +396,9 @@ def patch_sdpa_rows():
 
     def rows_sdpa(module, query, key, value, attention_mask, dropout=0.0, scaling=None,
                   sliding_window=None, **kwargs):
-        if _cached:
-            return _cached[-1].attend(module, query, key, value, dropout, scaling, sliding_window), None
+        cache = getattr(_cached, "step", None)
+        if cache is not None:
+            return cache.attend(module, query, key, value, dropout, scaling, sliding_window), None
         sinks = attention_sinks(module) if sliding_window is not None else 0
         if not _rows or query.shape[0] != 1:
             if _rows:

@@ -325,14 +325,38 @@ def test_attention_in_a_window(window, sinks, new):
     c.check_attention([new, new, 3, new], window, sinks)
 
 
-def test_attention_of_one_long_sequence():
-    """Its keys are split over many workgroups and joined."""
-    c = Case(1, 1, 64, 20001, heads=2)
-    c.append([20000])
-    c.append([1])
-    a = c.check_attention([1])
-    c.check_attention([1], window=9000, sinks=100)
-    del a
+@pytest.mark.parametrize("length,dim,dtype", [
+    (500, 128, torch.float16), (3000, 128, torch.bfloat16), (3000, 64, torch.float16), (20000, 128, torch.float16),
+    (20000, 64, torch.bfloat16)])
+def test_attention_of_long_sequences(length, dim, dtype):
+    """Keys split over a few, over some and over many workgroups, whose parts are joined in three ways."""
+    c = Case(2, 1, dim, length + 1, dtype, heads=3)
+    c.append([length, length // 5])
+    c.append([1, 1])
+    c.check_attention([1, 1])
+    c.check_attention([1, 1], window=length // 2, sinks=100)
+
+
+@pytest.mark.parametrize("heads,kv,dim,dtype", [
+    (16, 8, 64, torch.float16), (16, 8, 128, torch.bfloat16), (12, 2, 128, torch.float16)])
+def test_attention_of_long_pieces(heads, kv, dim, dtype):
+    """Tiles of 64 rows, two sequences, the second without new tokens; masks of windows inside a tile."""
+    c = Case(3, kv, dim, 9400, dtype, heads=heads)
+    c.append([2000, 300, 8700])
+    new = [130, 0, 650 if kv == 2 else 450]
+    c.append(new)
+    c.check_attention(new)
+    c.check_attention([3, 1, new[2]], window=700, sinks=5)
+
+
+@pytest.mark.parametrize("new", [1, 9])
+def test_attention_of_more_sequences_than_a_wavefront_counts(new):
+    c = Case(131, 1, 64, 200, heads=4)
+    c.append([(i * 37) % 150 for i in range(131)])
+    rows = [0 if i % 7 == 3 else 1 + i % new for i in range(131)]
+    c.append(rows)
+    c.check_held()
+    c.check_attention(rows)
 
 
 def test_attention_of_loud_keys_and_quiet_values():

@@ -88,7 +88,8 @@ def _attn(**bad):
     ({"scale": -1.0}, "scale"), ({"scale": float("nan")}, "scale"), ({"scale": float("inf")}, "scale"),
     ({"q": None}, "null"), ({"out": None}, "null"), ({"tail": None}, "null"), ({"qs": 4}, "strides"),
     ({"q": PTR + 8}, "16-byte"), ({"ws": PTR + 4}, "16-byte"), ({"bytes": 100}, "workspace"),
-    ({"ws": None, "bytes": 0}, "workspace"), ({"ws": None}, "workspace")])
+    ({"ws": None, "bytes": 0}, "workspace"), ({"ws": None}, "workspace"),
+    ({"rows": 70000, "seqs": 65536, "len": 64}, "sequences")])
 def test_attention_rejects(bad, word):
     status, message = _attn(**bad)
     assert status == _lib.TALM_EINVAL and word in message, message
@@ -105,6 +106,10 @@ def test_workspace_is_what_the_parts_need():
     # a window's keys, not the whole length's; windows and sinks past every length are no larger
     assert 0 < size(1, 12, 2, 128, 1, 1, 131072, 4096, 4) < size(1, 12, 2, 128, 1, 1, 131072, 0, 0)
     assert size(1, 12, 2, 128, 1, 1, 9000, 2 ** 31 - 1, 2 ** 31 - 1) == size(1, 12, 2, 128, 1, 1, 9000, 0, 0)
+    # many sequences: bounded, and so are the workgroups (8192 over the KV heads)
+    for rows in (64, 1000, 20000):
+        assert size(rows, 64, 8, 128, rows, 1, 131072, 0, 0) <= 1 << 27
+    assert size(2000, 12, 2, 128, 2000, 1, 131072, 0, 0) == 2000 * 12 * 2 * 130 * 4
     # counts of new tokens past the rows mean the rows
     assert size(1, 12, 2, 128, 1, 1 << 20, 9000, 0, 0) == size(1, 12, 2, 128, 1, 1, 9000, 0, 0)
 
