@@ -1154,25 +1154,35 @@ OptTensor cache_write(const Tensor& key, const Tensor& value, const Tensor& boun
   return ask ? OptTensor(q_out) : std::nullopt;
 }
 
-void cache_read(const Tensor& codes, const Tensor& scales, const Tensor& tail, const Tensor& table,
-                const Tensor& length, const Tensor& bounds, const Tensor& past, int64_t max_new, const Tensor& key,
-                const Tensor& value) {
+// (key, value), each [1, Hkv, rows, D] of [rows, Hkv, D] storage: new, or the two given buffers.
+std::tuple<Tensor, Tensor> cache_read(const Tensor& codes, const Tensor& scales, const Tensor& tail,
+                                      const Tensor& table, const Tensor& length, const Tensor& bounds,
+                                      const Tensor& past, int64_t max_new, int64_t rows, const OptTensor& out_key,
+                                      const OptTensor& out_value) {
   const CacheSizes c = cache_buffers(codes, scales, tail, table);
   cache_spans(bounds, past, c.seqs, codes);
   require(length.device() == codes.device() && length.scalar_type() == at::kInt && length.is_contiguous() &&
               length.dim() == 1 && length.size(0) == c.seqs,
           "cache_read: length int32 [sequences] on the cache's device");
-  for (const Tensor* t : {&key, &value})
-    require(t->device() == codes.device() && t->scalar_type() == tail.scalar_type() && t->is_contiguous() &&
-                t->dim() == 3 && t->size(0) == key.size(0) && t->size(1) == c.kv && t->size(2) == c.dim,
-            "cache_read: key and value [N, Hkv, D] of the tail's type on the cache's device, contiguous");
+  TORCH_CHECK_VALUE(rows >= 0, "cache_read: ", rows, " rows");
+  require(out_key.has_value() == out_value.has_value(), "cache_read: both buffers or neither");
   const c10::DeviceGuard guard(codes.device());
+  const std::vector<int64_t> sizes{1, c.kv, rows, c.dim}, strides{rows * c.kv * c.dim, c.dim, c.kv * c.dim, 1};
+  auto buffer = [&](const OptTensor& out) {
+    if (!out.has_value()) return at::empty_strided(sizes, strides, tail.options());
+    require(out->device() == codes.device() && out->scalar_type() == tail.scalar_type() && out->is_contiguous() &&
+                out->dim() == 3 && out->size(0) == rows && out->size(1) == c.kv && out->size(2) == c.dim,
+            "cache_read: out [rows, Hkv, D] of the tail's type on the cache's device, contiguous");
+    return out->as_strided(sizes, strides);
+  };
+  const Tensor key = buffer(out_key), value = buffer(out_value);
   check(talm_cache_read(static_cast<const uint8_t*>(codes.data_ptr()), as<float>(scales), as<uint16_t>(tail),
                         as<int32_t>(table), c.pages, int32_arg(c.width, "table width"), int32_arg(c.seqs, "sequences"),
                         int32_arg(c.kv, "heads"), static_cast<int32_t>(c.dim), window_dtype(tail), as<int32_t>(length),
                         as<int32_t>(bounds), as<int32_t>(past), static_cast<int32_t>(cache_count(max_new, "max_new")),
-                        key.size(0), as<uint16_t>(key), as<uint16_t>(value), stream_of(codes)),
+                        rows, as<uint16_t>(key), as<uint16_t>(value), stream_of(codes)),
         "cache_read");
+  return {key, value};
 }
 
 // query [1, Hq, N, D]; returns [1, N, Hq, D].
@@ -2261,7 +2271,8 @@ TORCH_LIBRARY(talm, m) {
         "Tensor(b!) scales, Tensor(c!) tail, Tensor table, Tensor? query, Tensor? cos, Tensor? sin) -> Tensor?",
         &cache_write);
   m.def("cache_read(Tensor codes, Tensor scales, Tensor tail, Tensor table, Tensor length, Tensor bounds, "
-        "Tensor past, int max_new, Tensor(a!) key, Tensor(b!) value) -> ()", &cache_read);
+        "Tensor past, int max_new, int rows, Tensor(a!)? out_key, Tensor(b!)? out_value) -> (Tensor, Tensor)",
+        &cache_read);
   m.def("cache_attention(Tensor query, Tensor bounds, Tensor past, int max_new, int max_len, Tensor codes, "
         "Tensor scales, Tensor tail, Tensor table, float scale, int window, int sinks) -> Tensor", &cache_attention);
   m.def("counter_dropout(Tensor x, float p, Tensor? key, int site) -> Tensor", &counter_dropout);

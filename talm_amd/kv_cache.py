@@ -85,15 +85,11 @@ class CacheLayer:
         bounds[b, 0] + i of (key, value), each [1, Hkv, rows, D] in the tail's type. `out`: two contiguous
         [rows, Hkv, D] buffers to take them (rows that no sequence holds keep their contents there, and
         are undefined without it). Tokens behind a sequence's length read as zeros."""
-        if out is None:
-            shape = (rows, self.codes.shape[2], self.codes.shape[3] // BLOCK)
-            out = (self.tail.new_empty(shape), self.tail.new_empty(shape))
-        elif any(t.shape[0] != rows for t in out):
-            raise ValueError(f"cache_read: out of {[t.shape[0] for t in out]} rows, {rows} asked")
-        torch.ops.talm.cache_read(self.codes, self.scales, self.tail, self.table, length, bounds, past, max_new,
-                                  *out)
+        key, value = out if out is not None else (None, None)
+        out = torch.ops.talm.cache_read(self.codes, self.scales, self.tail, self.table, length, bounds, past, max_new,
+                                        rows, key, value)
         RAN["cache_read"] += 1
-        return tuple(t.transpose(0, 1)[None] for t in out)
+        return out
 
     def attention(self, query, bounds, past, max_new, max_len, scale, window=None, sinks=0):
         """softmax(scale q K^T) V of query [1, Hq, N, D] over the cache, which holds the rows' own tokens

@@ -569,22 +569,43 @@ def test_captured_steps_replay():
     c.check_held()
 
 
-def test_calls_on_other_streams_are_the_same():
-    c = Case(2, 2, 128, 5000, heads=12)
-    c.append([4500, 300])
-    c.append([1, 1])
-    bounds, _ = c.spans([1, 1])
-    q, past = c.rows(2, 12), torch.tensor([4500, 300], dtype=torch.int32).cuda()
-    want = c.layer.attention(q, bounds, past, 1, 4501, 0.1)
+@pytest.mark.parametrize("dim,dtype", [(128, torch.float16), (64, torch.bfloat16)])
+def test_calls_on_other_streams_and_in_graphs_are_the_same(dim, dtype):
+    """Many calls on several streams at once, and in two graphs that are replayed beside each other and
+    beside an eager call: the same bits."""
+    c = Case(5, 2, dim, 5000, dtype, heads=12)
+    c.append([4500, 300, 2000, 0, 64])
+    c.append([1, 1, 1, 0, 1])
+    bounds, n = c.spans([1, 1, 1, 0, 1])
+    q, past = c.rows(n, 12), torch.tensor([4500, 300, 2000, 0, 64], dtype=torch.int32).cuda()
+
+    def call():
+        return c.layer.attention(q, bounds, past, 1, 4501, 0.1)
+
+    want = call()
     streams = [torch.cuda.Stream() for _ in range(3)]
     torch.cuda.synchronize()
     outs = []
-    for _ in range(4):
+    for _ in range(20):
         for s in streams:
             with torch.cuda.stream(s):
-                outs.append(c.layer.attention(q, bounds, past, 1, 4501, 0.1))
+                outs.append(call())
+    outs += [call() for _ in range(20)]
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((graph, out))
+    for _ in range(3):
+        for (graph, _), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        eager = call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in (eager, *(out for _, out in graphs)))
 
 
 def test_operands_that_are_refused():
@@ -621,6 +642,12 @@ def test_operands_that_are_refused():
         c.layer.read(past, bounds, past, 1, 2, (k[0], k[0]))
     with pytest.raises(ValueError):
         c.layer.read(past[:1], bounds, past, 1, 2)
+    good = torch.empty(2, 2, 64, dtype=torch.float16, device="cuda")
+    for out in ((good, good[:1]), (good, None), (good.float(), good), (good, good.expand(2, 2, 64)[:, :, :32])):
+        with pytest.raises(ValueError):
+            c.layer.read(past, bounds, past, 1, 2, out)
+    with pytest.raises(ValueError):
+        c.layer.read(past, bounds, past, 1, -1)
     layer = c.layer
     for name, value in (("codes", layer.codes.view(torch.uint8)), ("scales", layer.scales[:-1]),
                         ("tail", layer.tail.float()), ("table", layer.table.long()), ("table", layer.table[:1])):
