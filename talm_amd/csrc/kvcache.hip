@@ -1030,8 +1030,6 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(AttnArgs a) {
   }
 }
 
-constexpr int kMost = 10;
-
 // How an attention call is cut: rows of a tile, tiles of a KV head at most, parts of the pages and pages of
 // a part.
 struct Plan {
@@ -1058,12 +1056,23 @@ Plan plan_of(int64_t n_rows, int64_t n_seqs, int64_t kv, int64_t group, int64_t 
   p.cols = p.wide ? 32 * p.wide : 16;
   p.tiles = p.wide ? tiles_of(p.cols) : n_seqs;
   const int64_t visits = visits_of(p.cols), base = std::max<int64_t>(kv * p.tiles, 1);
-  // Two workgroups a CU, parts of at least a page per wavefront. Parts of 16-row tiles have at most kMost
-  // pages: sequences of other lengths than the longest leave CUs idle at the end, a short part less. All
-  // within 8192 workgroups (those of parts that a sequence lacks cost a start each) and 128 MB of parts.
+  // Parts cost their join: a launch, and 520 bytes a row written and read again. Two workgroups a CU, parts of
+  // at least a page per wavefront. No parts where one's pages in turn take no longer than the join: 16 pages,
+  // 32 where 16-row tiles fill half of the CUs, 48 where larger ones fill a quarter (one token of 64
+  // sequences over 1001 and 2001 tokens 16.5 and 20.8 us in parts, 10.6 and 16.2 without; of 128 over 2001
+  // 34.6 and 29). Else 16-row tiles have short parts where there are few sequences, since those of other
+  // lengths than the longest leave CUs idle at the end (64 sequences of 201 to 8191: 36 us in parts of 10
+  // pages, 40 in 32), and long ones where there are many (256 over 2001: 64 in 10, 51 in 32). All within
+  // 8192 workgroups (a part that a sequence lacks costs a start) and 128 MB of parts.
   const int64_t most = std::min<int64_t>({kSplits, 8192 / base, (int64_t{1} << 27) / (n_rows * kv * group * 520 + 1)});
+  const bool filled = base >= (p.wide ? cus / 4 : cus / 2);
   int64_t want = 2 * cus / base;
-  if (!p.wide) want = std::max(want, (visits + kMost - 1) / kMost);
+  if (visits <= (!filled ? 16 : p.wide ? 48 : 32)) {
+    want = 1;
+  } else if (!p.wide) {
+    const int64_t pages = base < cus ? 10 : base < 2 * cus ? 32 : 64;
+    want = std::max(want, (visits + pages - 1) / pages);
+  }
   want = std::max<int64_t>(1, std::min(want, most));
   p.per = std::max<int64_t>((visits + want - 1) / want, kWaves);
   p.splits = std::max<int64_t>((visits + p.per - 1) / p.per, 1);

@@ -326,7 +326,7 @@ def test_attention_in_a_window(window, sinks, new):
 
 
 @pytest.mark.parametrize("length,dim,dtype", [
-    (500, 128, torch.float16), (3000, 128, torch.bfloat16), (3000, 64, torch.float16), (20000, 128, torch.float16),
+    (500, 128, torch.float16), (1100, 64, torch.float16), (3000, 128, torch.bfloat16), (3000, 64, torch.float16), (20000, 128, torch.float16),
     (20000, 64, torch.bfloat16)])
 def test_attention_of_long_sequences(length, dim, dtype):
     """Keys split over a few, over some and over many workgroups, whose parts are joined in three ways."""
