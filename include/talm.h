@@ -774,8 +774,9 @@ int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, const uint8_
  * A call's new tokens are rows of packed operands: sequence b's are rows bounds[2b] .. bounds[2b + 1] - 1, the
  * i-th of them token past[b] + i. bounds and past lie in device memory; rows outside the operands, past the
  * first max_new of a sequence or behind its width blocks are left out (nothing of them is written). The
- * sequences' rows do not overlap. Two sequences may share complete pages. Strides in elements, multiples of 8; 16-byte aligned buffers (scales, table, bounds
- * and past 4). Non-finite values are held as NaN in a page.
+ * sequences' rows do not overlap. Two sequences may share complete pages; a page that a call writes belongs to
+ * one block of one sequence. n_seqs at most 2^24. Strides in elements, multiples of 8; 16-byte aligned buffers
+ * (scales, table, bounds and past 4). Non-finite values are held as NaN in a page.
  *
  * talm_cache_write puts k, v [n_rows, n_kv, D] into the cache. With cos and sin (f32 [n_rows, D], row stride
  * cs_stride, a multiple of 4; NULL both: without) the keys are turned by them first (as talm_rope does, rounded
@@ -790,7 +791,7 @@ int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, const uint8_
  * j <= past[b] + i, with a window (> 0) only those with past[b] + i - j < window or j < sinks; zeros where it sees
  * none. The cache holds the rows' own tokens already: past[b] + (rows of b) tokens in all, of which max_len at
  * least as many. Codes enter the products exactly; the keys' scale multiplies the fp32 scores, the values' the
- * fp32 sums. Values of tokens that a row's window leaves out must be finite. `workspace` holds
+ * fp32 sums. Values of tokens that a row does not see must be finite (its keys may be anything). `workspace` holds
  * talm_cache_attn_workspace bytes (-1: rejected shape). Deterministic.
  */
 int talm_cache_write(const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,

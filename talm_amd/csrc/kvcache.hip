@@ -1082,8 +1082,8 @@ Plan plan_of(int64_t n_rows, int64_t n_seqs, int64_t kv, int64_t group, int64_t 
 bool cache_shape(int32_t n_kv, int32_t head_dim, int32_t dtype, int32_t n_seqs, int64_t n_pages, int32_t width,
                  int64_t n_rows) {
   return n_kv >= 1 && n_kv <= 1024 && (head_dim == 64 || head_dim == 128) &&
-         (dtype == TALM_F16 || dtype == TALM_BF16) && n_seqs >= 0 && n_pages >= 0 && n_pages < (int64_t{1} << 31) &&
-         width >= 0 && width <= (1 << 24) && n_rows >= 0 && n_rows < (int64_t{1} << 31);
+         (dtype == TALM_F16 || dtype == TALM_BF16) && n_seqs >= 0 && n_seqs <= (1 << 24) && n_pages >= 0 &&
+         n_pages < (int64_t{1} << 31) && width >= 0 && width <= (1 << 24) && n_rows >= 0 && n_rows < (int64_t{1} << 31);
 }
 
 bool strides_fit(int64_t tok, int64_t head) { return tok % 8 == 0 && head % 8 == 0 && tok >= 0 && head >= 0; }

@@ -45,7 +45,8 @@ class CacheLayer:
     [sequences] lie on the device, `max_new` is at least the largest count of rows. Rows that no sequence
     holds, that lie past max_new or do not fit the table are not written. The operators run on the
     current stream, wait for nothing and can be captured in a HIP graph; they have no gradient and
-    refuse operands that need one."""
+    refuse operands that need one. A row belongs to one sequence, and a page that a call writes to one
+    block of one sequence."""
 
     def __init__(self, codes, scales, tail, table):
         self.codes, self.scales, self.tail, self.table = codes, scales, tail, table
@@ -95,8 +96,9 @@ class CacheLayer:
         """softmax(scale q K^T) V of query [1, Hq, N, D] over the cache, which holds the rows' own tokens
         already: the row of token p sees the tokens up to p, in a `window` only the last `window` ones
         (itself among them) and the sequence's first `sinks`. `max_len` is at least the longest sequence
-        with its new tokens. Returns [1, N, Hq, D]; a row that sees nothing is zero, a row that no
-        sequence holds undefined."""
+        with its new tokens (in a graph: with those of any replay). Values of tokens that a row does not
+        see must be finite, since a weight of 0 does not hide NaN; its keys may be anything. Returns
+        [1, N, Hq, D]; a row that sees nothing is zero, a row that no sequence holds undefined."""
         if window is not None and window < 1:
             raise ValueError(f"cache_attention: window {window} (at least 1, or None)")
         out = torch.ops.talm.cache_attention(query, bounds, past, max_new, max_len, self.codes, self.scales,
@@ -194,7 +196,7 @@ class QuantizedCache(Cache):
         device = torch.tensor(values, dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
         self._step = _Step(device[:2 * batch].view(batch, 2), device[2 * batch:3 * batch], max(new), max(lengths),
                            device[3 * batch:] if first else None, rows,
-                           _real(runs, rows, self.device) if padded and not first else None)
+                           _real(runs, rows, self.device) if padded else None)
         outer, unpad._cached.step = getattr(unpad._cached, "step", None), self
         try:
             yield
@@ -232,7 +234,7 @@ class QuantizedCache(Cache):
 
     def attend(self, module, query, key, value, dropout, scaling, window):
         """The attention interface of a call with this cache: query [B, Hq, T, D] against the layer's tokens;
-        returns [B, T, Hq, D]."""
+        returns [B, T, Hq, D] in the query's type."""
         if dropout:
             raise ValueError("QuantizedCache: no dropout of attention weights")
         layer, s = self._layer(module.layer_idx), self._step
@@ -247,9 +249,9 @@ class QuantizedCache(Cache):
                 out = unpad.VarlenAttention.apply(q, k, v, s.cu, s.rows, scale) \
                     if window is None and q.dtype == torch.float16 \
                     else unpad.window_attention(q, k, v, s.cu, s.rows, scale, window or s.rows, sinks)
-                return out.view(b, t, heads, d)
+                return out.view(b, t, heads, d).to(query.dtype)
         out = layer.attention(q, s.bounds, s.past, s.max_new, s.max_len, scale, window, sinks)
-        return self._clean(out).view(b, t, heads, d)
+        return self._clean(out).view(b, t, heads, d).to(query.dtype)
 
     def _clean(self, out):
         """Padding's rows, which no sequence holds, as zeros."""

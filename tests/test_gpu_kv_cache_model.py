@@ -5,9 +5,9 @@ in other orders: logits within the bar of the generation tests, 0.5%."""
 
 import pytest
 import torch
-from transformers import DynamicCache
+from transformers import DynamicCache, Qwen2ForCausalLM
 
-from talm_amd import engaged, few_tokens, patches, qgroup, qlora_model
+from talm_amd import engaged, few_tokens, patches, qgroup, qlora_model, state
 from talm_amd.kv_cache import QuantizedCache
 
 pytestmark = pytest.mark.gpu
@@ -186,6 +186,44 @@ def test_bfloat16_caches(patched):
     want = _answer(model, QuantizedCache(model.config, 1, 100), ids, mask, pieces)
     got = _answer(model, QuantizedCache(model.config, 1, 100, dtype=torch.bfloat16), ids, mask, pieces)
     assert (got - want).norm() <= 0.02 * want.norm()
+
+
+@pytest.mark.parametrize("held", [torch.float16, torch.bfloat16])
+def test_models_of_another_type_than_the_cache(monkeypatch, patched, held):
+    """Plain bfloat16 weights, no autocast: what the attention returns is of the model's type. One call, which
+    attends to its own keys and values: they, the queries and the output are rounded to the cache's type
+    where transformers rounds to bfloat16 (u = 2^-8 per value and layer: a bar of 2%)."""
+    for fp16_only in ("swiglu", "rmsnorm", "addnorm"):
+        monkeypatch.setitem(state.DISABLED, fp16_only, "a bfloat16 model")
+    config = qlora_model.qwen2_config(vocab_size=1000, hidden_size=512, intermediate_size=1024, num_hidden_layers=2,
+                                      num_attention_heads=4, num_key_value_heads=2, head_dim=128)
+    torch.manual_seed(5)
+    model = Qwen2ForCausalLM(config).to("cuda", torch.bfloat16).eval()
+    patches.apply()
+    ids, mask = _ids(2, 50), _mask(2, 50, (0, 7))
+    with torch.no_grad():
+        want = model(input_ids=ids, attention_mask=mask, past_key_values=DynamicCache(), use_cache=True).logits[:, -1]
+        cache = QuantizedCache(config, 2, 60, dtype=held)
+        out = model(input_ids=ids, attention_mask=mask, past_key_values=cache, use_cache=True).logits
+        again = model(input_ids=ids[:, :1], past_key_values=cache, use_cache=True).logits
+    assert out.dtype == again.dtype == torch.bfloat16 and again.isfinite().all()
+    assert (out[:, -1] - want).float().norm() <= 0.02 * want.float().norm()
+
+
+@pytest.mark.parametrize("overrides", [{}, {"num_attention_heads": 8, "num_key_value_heads": 2, "head_dim": 64}])
+def test_rows_of_padding_are_finite(patched, overrides):
+    """First calls and later ones, in memory that held NaN."""
+    model = _model(**overrides)
+    patches.apply()
+    cache, ids, mask = QuantizedCache(model.config, 2, 60), _ids(2, 60), _mask(2, 40, (0, 33))
+    more = torch.cat((mask, _mask(2, 10, (4, 0))), 1)
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.float16):
+        for n, seen in ((40, mask), (10, more)):
+            junk = [torch.full((size,), float("nan"), device="cuda") for size in (1 << 12, 1 << 16, 1 << 20, 1 << 24)]
+            del junk
+            out = model(input_ids=ids[:, :n], attention_mask=seen, past_key_values=cache, use_cache=True).logits
+            assert out.isfinite().all()
+    assert cache.lengths == [46, 17]
 
 
 def test_calls_that_are_refused(patched):

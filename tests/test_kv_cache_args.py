@@ -35,6 +35,7 @@ def _write(**bad):
     ({"d": 96}, "shape"), ({"dtype": _lib.TALM_F32}, "shape"), ({"kv": 0}, "shape"), ({"kv": 2000}, "shape"),
     ({"rows": -1}, "shape"), ({"rows": 1 << 31}, "shape"), ({"pages": 1 << 31}, "shape"), ({"width": -1}, "shape"),
     ({"width": (1 << 24) + 1}, "shape"), ({"new": -1}, "shape"), ({"nq": -1}, "shape"), ({"seqs": -1}, "shape"),
+    ({"seqs": (1 << 24) + 1}, "shape"),
     ({"sin": None}, "cos"), ({"cos": None, "sin": None}, "cos"), ({"cs": 64}, "cos"), ({"cs": 130}, "cos"),
     ({"k": None}, "null"), ({"tail": None}, "null"), ({"codes": None}, "null"), ({"out": None}, "null"), ({"past": None}, "null"),
     ({"ks": 129}, "strides"), ({"qs": 4}, "strides"), ({"vs": -256}, "strides"), ({"k": PTR + 2}, "16-byte"),
