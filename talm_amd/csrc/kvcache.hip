@@ -40,6 +40,7 @@ constexpr int kBlock = 64;     // tokens of a page
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kSplits = 256;   // the most parts that the keys of a row are split into
+constexpr int kNear = 4;       // tiles beside each other that share a die's L2
 
 struct Cache {
   const uint8_t* codes;   // [pages, 2, kv, 64 D]
@@ -576,13 +577,21 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
   const int head = blockIdx.y;
   int tile = 0, seq = blockIdx.z, split = blockIdx.x;
   if (a.listed) {
-    tile = split / a.splits;
-    split -= tile * a.splits;
+    // kNear tiles beside each other, of the same part, go to the same die
+    const int o = split, slot = o >> 3;
+    if (o < static_cast<int>(gridDim.x & ~(8u * kNear - 1))) split = (slot & ~(kNear - 1)) * 8 + (o & 7) * kNear + (slot & (kNear - 1));
+    tile = split & (kNear - 1);
+    split /= kNear;
+    const int q = split / a.splits;
+    tile += q * kNear;
+    split -= q * a.splits;
   }
   // Workgroups go to the eight dies in turn: without this a die would have the same part of every sequence,
   // and later parts are those that short sequences lack.
-  split += (head + seq + tile) & a.turn;
-  if (split >= a.splits) split -= a.splits;
+  if (!a.listed) {
+    split += (head + seq) & a.turn;
+    if (split >= a.splits) split -= a.splits;
+  }
   // A workgroup begins with a chain of cache misses; all arguments in one, the sequence's numbers and its
   // pages' places (without a window known from the part alone) in the next, then the pages.
   asm volatile("" ::"s"(a.c.codes), "s"(a.c.scales), "s"(a.c.tail), "s"(a.c.table), "s"(a.c.width), "s"(a.c.kv),
@@ -657,7 +666,7 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
   float unit = 1.f;
   u32x4 kw[kLoads], vw[kLoads];
   // what one wavefront alone reads passes by the caches
-  auto load = [&](const u32x4* p) { return kWide == 1 ? __builtin_nontemporal_load(p) : *p; };
+  auto load = [&](const u32x4* p) { return kCol == 16 ? __builtin_nontemporal_load(p) : *p; };
   auto load_k = [&](int page) __attribute__((always_inline)) {
     const u32x4* src = reinterpret_cast<const u32x4*>(
                            a.c.codes + (static_cast<int64_t>(page) * 2 * a.c.kv + head) * (kBlock * D)) +
@@ -1036,26 +1045,22 @@ struct Plan {
   int wide;  // 0: 16 rows a workgroup, one tile a sequence; 1, 2: kWide of 32 each
   int64_t cols, tiles, splits, per;
 };
-Plan plan_of(int64_t n_rows, int64_t n_seqs, int64_t kv, int64_t group, int64_t max_new, int64_t max_len,
-             int64_t window, int64_t sinks) {
+Plan plan_with(int wide, int64_t n_rows, int64_t n_seqs, int64_t kv, int64_t group, int64_t max_new, int64_t max_len,
+               int64_t window, int64_t sinks) {
   Plan p;
   sinks = std::min(sinks, max_len);
-  const int64_t rows = max_new * group, cus = device_cus();
+  p.wide = wide;
+  p.cols = wide ? 32 * wide : 16;
   // a sequence's last tile may be part of one; no more rows than there are
-  auto tiles_of = [&](int64_t cols) {
-    return std::min(n_seqs * ((rows + cols - 1) / cols), (n_rows * group + cols - 1) / cols + n_seqs);
-  };
-  auto visits_of = [&](int64_t cols) {
-    const int64_t all = (max_len + kBlock - 1) / kBlock;
-    return window > 0 ? std::min(all, (window + cols - 1 + kBlock - 1) / kBlock + 1 + (sinks + kBlock - 1) / kBlock)
-                      : all;
-  };
-  // Rows past 16: tiles of 64, whose pages come through the L1 for two wavefronts, where the pages' way from
-  // the L2 sets the time; tiles of 32 below that, which spread over more CUs
-  p.wide = rows <= 16 ? 0 : rows <= 32 || kv * tiles_of(64) * visits_of(64) < 24 * cus ? 1 : 2;
-  p.cols = p.wide ? 32 * p.wide : 16;
-  p.tiles = p.wide ? tiles_of(p.cols) : n_seqs;
-  const int64_t visits = visits_of(p.cols), base = std::max<int64_t>(kv * p.tiles, 1);
+  p.tiles = n_seqs;
+  if (wide) {
+    const int64_t rows = max_new * group, near = kNear;
+    p.tiles = std::min(n_seqs * ((rows + p.cols - 1) / p.cols), (n_rows * group + p.cols - 1) / p.cols + n_seqs);
+    p.tiles = (p.tiles + near - 1) / near * near;
+  }
+  int64_t visits = (max_len + kBlock - 1) / kBlock;
+  if (window > 0)
+    visits = std::min(visits, (window + p.cols - 1 + kBlock - 1) / kBlock + 1 + (sinks + kBlock - 1) / kBlock);
   // Parts cost their join: a launch, and 520 bytes a row written and read again. Two workgroups a CU, parts of
   // at least a page per wavefront. No parts where one's pages in turn take no longer than the join: 16 pages,
   // 32 where 16-row tiles fill half of the CUs, 48 where larger ones fill a quarter (one token of 64
@@ -1064,12 +1069,13 @@ Plan plan_of(int64_t n_rows, int64_t n_seqs, int64_t kv, int64_t group, int64_t 
   // lengths than the longest leave CUs idle at the end (64 sequences of 201 to 8191: 36 us in parts of 10
   // pages, 40 in 32), and long ones where there are many (256 over 2001: 64 in 10, 51 in 32). All within
   // 8192 workgroups (a part that a sequence lacks costs a start) and 128 MB of parts.
+  const int64_t cus = device_cus(), base = std::max<int64_t>(kv * p.tiles, 1);
   const int64_t most = std::min<int64_t>({kSplits, 8192 / base, (int64_t{1} << 27) / (n_rows * kv * group * 520 + 1)});
-  const bool filled = base >= (p.wide ? cus / 4 : cus / 2);
+  const bool filled = base >= (wide ? cus / 4 : cus / 2);
   int64_t want = 2 * cus / base;
-  if (visits <= (!filled ? 16 : p.wide ? 48 : 32)) {
+  if (visits <= (!filled ? 16 : wide ? 48 : 32)) {
     want = 1;
-  } else if (!p.wide) {
+  } else if (!wide) {
     const int64_t pages = base < cus ? 10 : base < 2 * cus ? 32 : 64;
     want = std::max(want, (visits + pages - 1) / pages);
   }
@@ -1077,6 +1083,22 @@ Plan plan_of(int64_t n_rows, int64_t n_seqs, int64_t kv, int64_t group, int64_t 
   p.per = std::max<int64_t>((visits + want - 1) / want, kWaves);
   p.splits = std::max<int64_t>((visits + p.per - 1) / p.per, 1);
   return p;
+}
+// Tiles of 64 rows or of 32, whichever end first: a round of the workgroups takes as long as some 4 pages and
+// its wavefronts' pages, a join 2.5 (one text's 512 rows over 8289 tokens 48 us in tiles of 64, 52 in 32;
+// 1000 rows 90 and 83; 12 texts of 200 to 4000 tokens, 10 to 150 rows each, 54 and 45).
+Plan plan_of(int64_t n_rows, int64_t n_seqs, int64_t kv, int64_t group, int64_t max_new, int64_t max_len,
+             int64_t window, int64_t sinks) {
+  auto with = [&](int wide) { return plan_with(wide, n_rows, n_seqs, kv, group, max_new, max_len, window, sinks); };
+  const int64_t rows = max_new * group;
+  if (rows <= 32) return with(rows <= 16 ? 0 : 1);
+  auto cost = [&](const Plan& p) {
+    const int64_t deep = kWaves / p.wide;
+    const double rounds = std::max(1.0, static_cast<double>(kv * p.tiles * p.splits) / (2.0 * device_cus()));
+    return rounds * static_cast<double>(4 + (p.per + deep - 1) / deep) + (p.splits > 1 ? 2.5 : 0.0);
+  };
+  const Plan one = with(1), two = with(2);
+  return cost(two) < cost(one) ? two : one;
 }
 
 bool cache_shape(int32_t n_kv, int32_t head_dim, int32_t dtype, int32_t n_seqs, int64_t n_pages, int32_t width,

@@ -340,13 +340,25 @@ def test_attention_of_long_sequences(length, dim, dtype):
 @pytest.mark.parametrize("heads,kv,dim,dtype", [
     (16, 8, 64, torch.float16), (16, 8, 128, torch.bfloat16), (12, 2, 128, torch.float16)])
 def test_attention_of_long_pieces(heads, kv, dim, dtype):
-    """Tiles of 64 rows, two sequences, the second without new tokens; masks of windows inside a tile."""
+    """Tiles of 32 rows, and of 64 in parts; a sequence without new tokens; masks of windows inside a tile."""
     c = Case(3, kv, dim, 9400, dtype, heads=heads)
     c.append([2000, 300, 8700])
     new = [130, 0, 650 if kv == 2 else 450]
     c.append(new)
     c.check_attention(new)
     c.check_attention([3, 1, new[2]], window=700, sinks=5)
+
+
+@pytest.mark.parametrize("dim,dtype", [
+    (64, torch.float16), (64, torch.bfloat16), (128, torch.float16), (128, torch.bfloat16)])
+def test_attention_of_prompts(dim, dtype):
+    """Tiles of 64 rows, more than the CUs hold at once, of sequences of other lengths and of none."""
+    c = Case(6, 4, dim, 460, dtype, heads=16)
+    c.append([0, 40, 0, 17, 0, 0])
+    new = [400, 390, 256, 400, 0, 400]
+    c.append(new)
+    c.check_attention(new)
+    c.check_attention(new, window=70, sinks=3)
 
 
 @pytest.mark.parametrize("new", [1, 9])
