@@ -7,7 +7,7 @@ include/talm.h) reached through `torch.ops.talm.*` custom ops, behind the refere
 
 Modules keep the reference's names: qgroup, nf4_dequant, rmsnorm, rope, swiglu, swiglu_inplace,
 mlp_save_up, fused_head, lora, fused_proj, patches, state, engaged. Without a counterpart there: dropout
-(a counter-based generator's masks), few_tokens (a generating model's products on the NF4 codes).
+(a counter-based generator's masks), few_tokens (a generating model's products on the NF4 codes), kv_cache (its keys and values in 8 bits).
 """
 
 __version__ = "0.1.0"

@@ -217,7 +217,13 @@ __device__ __forceinline__ float top_of(const uint32_t (&w)[4], float top) {
 
 // One workgroup: block `j` behind past's of one sequence, one KV head, keys or values. A complete
 // block becomes a page; the workgroup of the first block, the one that reads the tail, then also
-// stores the tokens behind the last complete block into it, so no other touches the tail.
+// stores the tokens behind the last complete block into it, so no other touches the tail. A block has one
+// scale, so its workgroup holds it whole (LDS, where the page's order is made too) and reads it once.
+//
+// Bound by its bytes where it is large: 32001 tokens in bfloat16 with 12 query heads turned, 279 MB, take 58 us
+// (4.8 TB/s; a large copy reaches 5.2), four prompts of 1531 to 4096 tokens in fp16, 111 MB, 22; by the launch
+// and a chain of cache misses (arguments, the sequence's numbers, rows) where it is small: one token 2.9 us, one
+// of each of 64 sequences 6.2, of which those that complete a block first read its 63 others from the tail.
 template <class T, int D, bool kTurn>
 __global__ __launch_bounds__(kThreads) void cache_write_kernel(WriteArgs a) {
   constexpr int kPer = D / 8;  // 16-byte pieces of a row
@@ -395,7 +401,9 @@ __device__ __forceinline__ void held(u32x4 w, float scale, uint32_t (&out)[8]) {
 }
 
 // One workgroup: one block of one sequence, one KV head, keys or values. A lane's 16 keys are one token's
-// columns and go where they belong; its values are 16 tokens of one column and are turned in LDS.
+// columns and go where they belong; its values are 16 tokens of one column and are turned in LDS. Bound by its
+// bytes: 16 sequences of 4000 to 8191 tokens in bfloat16, 153 MB, take 32 us (4.8 TB/s of a copy's 5.2); 8
+// of 100 to 500 with heads of 64, 2 MB, take 4.9.
 template <class T, int D>
 __global__ __launch_bounds__(kThreads) void cache_read_kernel(ReadArgs a) {
   constexpr int kPer = D / 8, kEach = kBlock * D / 16 / kThreads;
@@ -564,6 +572,16 @@ struct Lay {
 // Weights are exp2(c s - ref) of a reference that follows the running maximum only where a score passes it
 // by more than 2^8: they stay below 2^8, far inside fp16, and nearly every page leaves the sums so far as
 // they are.
+//
+// Tiles of 16 rows, for sequences of a token or two: the pages come from memory once, and that is the time. One
+// token of each of 64 sequences of 201 to 8191 tokens, 143 MB, takes 29 us (4.9 TB/s of a copy's 5.2) and 4 for
+// the join; one over 131001, 67 MB, 14 and 4; one over 4001 5.8 and 3.3, where the start is most of it.
+// Tiles of 32 and 64 rows: the VALU's issue is the time. A wavefront's page of 32 rows takes some 500 issue
+// slots of 4 cycles: 128 conversions of codes, 150 for the softmax (an exponential has two), 64 of the 32
+// MFMAs, the loads, and its share of the start and the join. 512 rows of 6 heads each over 8289 tokens 41 us
+// (615 TF/s) and 6 for the join, the next turns of 12 conversations (1 to 300 tokens behind 300 to 3500) 58
+// (565 TF/s). Converted pages shared through LDS, and 64 columns a wavefront on one wavefront a SIMD, were no
+// faster (the same; 62 against 48 us with the join).
 template <class T, int D, int kCol, int kWide>
 __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kernel(AttnArgs a) {
   using L = Lay<D, kCol>;
@@ -577,17 +595,19 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
   const int head = blockIdx.y;
   int tile = 0, seq = blockIdx.z, split = blockIdx.x;
   if (a.listed) {
-    // kNear tiles beside each other, of the same part, go to the same die
-    const int o = split, slot = o >> 3;
-    if (o < static_cast<int>(gridDim.x & ~(8u * kNear - 1))) split = (slot & ~(kNear - 1)) * 8 + (o & 7) * kNear + (slot & (kNear - 1));
+    // Workgroups go to the eight dies in turn. kNear tiles beside each other, of the same part, go to one, whose
+    // L2 then has their pages (20 tokens of each of 40 sequences of 2000: 41 us spread out, 30 so)
+    const int slot = split >> 3;
+    if (split < static_cast<int>(gridDim.x & ~(8u * kNear - 1)))
+      split = (slot & ~(kNear - 1)) * 8 + (split & 7) * kNear + (slot & (kNear - 1));
     tile = split & (kNear - 1);
     split /= kNear;
     const int q = split / a.splits;
     tile += q * kNear;
     split -= q * a.splits;
   }
-  // Workgroups go to the eight dies in turn: without this a die would have the same part of every sequence,
-  // and later parts are those that short sequences lack.
+  // other sequences' parts in turn: a die would have the same part of every one, and later parts are those that
+  // short sequences lack
   if (!a.listed) {
     split += (head + seq) & a.turn;
     if (split >= a.splits) split -= a.splits;
@@ -665,7 +685,8 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
   // stay inside fp32's range whatever follows; bfloat16's do not, and there each page's sums are scaled.
   float unit = 1.f;
   u32x4 kw[kLoads], vw[kLoads];
-  // what one wavefront alone reads passes by the caches
+  // what one wavefront alone reads passes by the caches; the larger tiles' pages are read by their neighbours
+  // too (12 conversations in tiles of 32 rows 82 us past the caches, 61 through them)
   auto load = [&](const u32x4* p) { return kCol == 16 ? __builtin_nontemporal_load(p) : *p; };
   auto load_k = [&](int page) __attribute__((always_inline)) {
     const u32x4* src = reinterpret_cast<const u32x4*>(
@@ -923,7 +944,8 @@ __device__ __forceinline__ float lanes_sum(float x) {
 // The parts of a row and head, joined in their order. kRows = 0: a workgroup has 32 columns of one, its
 // 32 groups of 8 threads take every 32nd part (up to 256). Else a wavefront has all D columns of kRows of
 // them, its groups of D / 4 lanes take every second part (fourth with 64 columns), kEach each. All loads are
-// on their way before the weights are known.
+// on their way before the weights are known. 3 to 4 us, a launch's least and two misses, for one token's 16
+// or 256 parts as for 64 sequences' 13 each; 16 MB of a long piece's parts 5.8.
 template <class T, int D, int kRows, int kEach>
 __global__ __launch_bounds__(kThreads) void cache_join_kernel(AttnArgs a) {
   constexpr bool kWide = kRows == 0;
@@ -974,7 +996,8 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int j = grp + i * kGroups;
-      o[k][i] = j < parts[k] ? *reinterpret_cast<const f32x4*>(p + static_cast<int64_t>(j) * D) : f32x4{0.f, 0.f, 0.f, 0.f};
+      o[k][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (j < parts[k]) o[k][i] = *reinterpret_cast<const f32x4*>(p + static_cast<int64_t>(j) * D);
     }
     // every wavefront takes all weights
 #pragma unroll
@@ -1117,7 +1140,7 @@ using namespace talm;
 
 #define TALM_CACHE_KERNEL(name, grid, args)                                                                   \
   do {                                                                                                        \
-    const dim3 g_(grid), b_(kThreads);                                                 \
+    const dim3 g_(grid), b_(kThreads);                                                                        \
     if (dtype == TALM_F16 && head_dim == 128) name(F16, 128, g_, b_, args);                                   \
     else if (dtype == TALM_F16) name(F16, 64, g_, b_, args);                                                  \
     else if (head_dim == 128) name(BF16, 128, g_, b_, args);                                                  \
