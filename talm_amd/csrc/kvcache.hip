@@ -706,11 +706,23 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
   auto weigh = [&](float c, bool mask, int first, float ratio) __attribute__((always_inline)) {
     c = fmaxf(c, 1e-37f);  // never 0: c times a hidden score's -inf is one
     if (mask) {
+      // the lane's scores are those of the keys base + kStep (i / 4) + i % 4
+      const int base = first + 4 * g, last = place - base;
 #pragma unroll
       for (int i = 0; i < L::kLane; ++i) {
-        const int key = first + L::kStep * (i / 4) + 4 * g + i % 4;
-        const bool seen = (key <= place) & ((a.window == 0) | (place - key < a.window) | (key < a.sinks));
-        st[i / L::kEach][i % L::kEach] = seen ? st[i / L::kEach][i % L::kEach] : -__builtin_inff();
+        const int key = L::kStep * (i / 4) + i % 4;
+        st[i / L::kEach][i % L::kEach] = key <= last ? st[i / L::kEach][i % L::kEach] : -__builtin_inff();
+      }
+      if (a.window > 0) {
+        // (wraps only where every key is behind the row's place and hidden already)
+        const int from = static_cast<int>(static_cast<uint32_t>(last) - static_cast<uint32_t>(a.window));
+        const int sinks = a.sinks - base;
+#pragma unroll
+        for (int i = 0; i < L::kLane; ++i) {
+          const int key = L::kStep * (i / 4) + i % 4;
+          const bool seen = (key > from) | (key < sinks);
+          st[i / L::kEach][i % L::kEach] = seen ? st[i / L::kEach][i % L::kEach] : -__builtin_inff();
+        }
       }
     }
     float top = st[0][0];
@@ -734,6 +746,21 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
       st[i / L::kEach][i % L::kEach] =
           __builtin_amdgcn_exp2f(__builtin_fmaf(st[i / L::kEach][i % L::kEach], c, -base));
     }
+  };
+
+  // the weights in fp16, and their sum
+  auto round = [&](half8 (&p)[L::kPs]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < L::kPs; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const int i = 8 * u + e;
+        const half2_ w = __builtin_convertvector(
+            (f32x2{st[i / L::kEach][i % L::kEach], st[i / L::kEach][i % L::kEach + 1]}), half2_);
+        p[u][e] = w.x;
+        p[u][e + 1] = w.y;
+        l = __builtin_amdgcn_fdot2(w, half2_{static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)}, l, false);
+      }
   };
 
   // 64 of the wavefront's pages at a time: lane l holds the l-th one's place and scales
@@ -784,17 +811,7 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
       // a rounding to 11 bits, and its sum is that of the rounded weights, so a token that has nearly all
       // of it keeps its values exactly.
       half8 p[L::kPs];
-#pragma unroll
-      for (int u = 0; u < L::kPs; ++u)
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const int i0 = 8 * u + e;
-          const half2_ w = __builtin_convertvector(
-              (f32x2{st[i0 / L::kEach][i0 % L::kEach], st[i0 / L::kEach][i0 % L::kEach + 1]}), half2_);
-          p[u][e] = w.x;
-          p[u][e + 1] = w.y;
-          l = __builtin_amdgcn_fdot2(w, half2_{static_cast<_Float16>(1.f), static_cast<_Float16>(1.f)}, l, false);
-        }
+      round(p);
       if (page < 0) {
 #pragma unroll
         for (int k = 0; k < kLoads; ++k) vw[k] = u32x4{0, 0, 0, 0};
@@ -844,13 +861,17 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
     unit = 1.f;
     // the weights in the tail's type; for bfloat16 as two parts, so that they keep 16 bits
     half8 hi[L::kPs], lo[L::kPs];
+    if constexpr (kUnits) {
+      round(hi);
+    } else {
 #pragma unroll
-    for (int i = 0; i < L::kLane; ++i) {
-      const float x = st[i / L::kEach][i % L::kEach];
-      const uint16_t b = T::down(x);
-      hi[i / 8][i % 8] = __builtin_bit_cast(_Float16, b);
-      lo[i / 8][i % 8] = __builtin_bit_cast(_Float16, T::down(x - T::up(b)));
-      l += kUnits ? T::up(b) : x;
+      for (int i = 0; i < L::kLane; ++i) {
+        const float x = st[i / L::kEach][i % L::kEach];
+        const uint16_t b = T::down(x);
+        hi[i / 8][i % 8] = __builtin_bit_cast(_Float16, b);
+        lo[i / 8][i % 8] = __builtin_bit_cast(_Float16, T::down(x - T::up(b)));
+        l += x;
+      }
     }
 #pragma unroll
     for (int n = 0; n < L::kOuts; ++n)
