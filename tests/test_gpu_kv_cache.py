@@ -381,6 +381,19 @@ def test_attention_of_loud_keys_and_quiet_values():
     c.check_attention([1, 5], std=0.1)
 
 
+@pytest.mark.parametrize("dim,dtype,heads", [
+    (128, torch.bfloat16, 4), (64, torch.float16, 12), (128, torch.float16, 16), (64, torch.bfloat16, 16)])
+def test_pieces_over_loud_keys_and_quiet_values(dim, dtype, heads):
+    """The same in tiles of 32 rows, from loud pages to quiet ones and back."""
+    c = Case(2, 2, dim, 1200, dtype, heads=heads)
+    for i in range(11):
+        n, loud = 64 if i % 3 else 50, 5 - abs(i - 5)
+        c.append([n, n], k=c.rows(2 * n, 2, 2.0 ** -loud), v=c.rows(2 * n, 2, 2.0 ** (12 - 3 * (i % 7))))
+    c.append([90, 400])
+    c.check_attention([90, 400], std=0.3)
+    c.check_attention([90, 30], window=100, sinks=70, std=0.3)
+
+
 def test_attention_over_shared_pages():
     """Two sequences with a common beginning whose complete pages are the same."""
     c = Case(2, 1, 128, 300, heads=2)
