@@ -1129,8 +1129,9 @@ Plan plan_with(int wide, int64_t n_rows, int64_t n_seqs, int64_t kv, int64_t gro
   return p;
 }
 // Tiles of 64 rows or of 32, whichever end first: a round of the workgroups takes as long as some 4 pages and
-// its wavefronts' pages, a join 2.5 (one text's 512 rows over 8289 tokens 48 us in tiles of 64, 52 in 32;
-// 1000 rows 90 and 83; 12 texts of 200 to 4000 tokens, 10 to 150 rows each, 54 and 45).
+// its wavefronts' pages, parts and their join 6 (one text's 512 rows over 8289 tokens 48 us in tiles of 64, 52
+// in 32; 1000 rows over 9000 90 and 83, 190 over 1334 17.0 and 14.5; 12 texts of 200 to 4000 tokens, 10 to 150
+// rows each, 54 and 45).
 Plan plan_of(int64_t n_rows, int64_t n_seqs, int64_t kv, int64_t group, int64_t max_new, int64_t max_len,
              int64_t window, int64_t sinks) {
   auto with = [&](int wide) { return plan_with(wide, n_rows, n_seqs, kv, group, max_new, max_len, window, sinks); };
@@ -1139,7 +1140,7 @@ Plan plan_of(int64_t n_rows, int64_t n_seqs, int64_t kv, int64_t group, int64_t 
   auto cost = [&](const Plan& p) {
     const int64_t deep = kWaves / p.wide;
     const double rounds = std::max(1.0, static_cast<double>(kv * p.tiles * p.splits) / (2.0 * device_cus()));
-    return rounds * static_cast<double>(4 + (p.per + deep - 1) / deep) + (p.splits > 1 ? 2.5 : 0.0);
+    return rounds * static_cast<double>(4 + (p.per + deep - 1) / deep) + (p.splits > 1 ? 6.0 : 0.0);
   };
   const Plan one = with(1), two = with(2);
   return cost(two) < cost(one) ? two : one;
