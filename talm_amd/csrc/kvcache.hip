@@ -636,12 +636,13 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
       if (seq >= a.c.n_seqs) return;
       Span mine{0, 0, 0};
       if (seq + lane < a.c.n_seqs) mine = span_of(a.bounds, a.past, seq + lane, a.n_rows, a.max_new, a.max_len);
-      const int count = (mine.n * a.group + kCols - 1) / kCols, size = mine.past + mine.n;
+      const int count = (mine.n * a.group + kCols - 1) / kCols;
+      const int order = (mine.past + mine.n) / kBlock * kWave + kWave - 1 - lane;  // no two alike
       int before = 0, all = 0;
       for (int l = 0; l < min(kWave, a.c.n_seqs - seq); ++l) {
-        const int c = __builtin_amdgcn_readlane(count, l), n = __builtin_amdgcn_readlane(size, l);
+        const int c = __builtin_amdgcn_readlane(count, l);
         all += c;
-        if (n > size || (n == size && l < lane)) before += c;
+        before += __builtin_amdgcn_readlane(order, l) > order ? c : 0;
       }
       if (tile >= all) {
         tile -= all;
@@ -892,31 +893,10 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
       }
   }
 
-  // 4 columns of one row, from its sums over the part
+  // The wavefronts' sums to one reference, and where there is no other part over the sum of the weights; a
+  // row's columns are then only added up.
   const bool only = visits.count <= a.per;
-  auto store = [&](int r, int d, f32x4 o, float top, float sum) __attribute__((always_inline)) {
-    const int token = a.over(r);
-    const int64_t to = static_cast<int64_t>(s.row0 + token) * a.n_q + head * a.group + r - token * a.group;
-    if (only) {
-      const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // a sum that is NaN stays one
-      u32x2 w;
-      w.x = T::down(o[0] * inv) | static_cast<uint32_t>(T::down(o[1] * inv)) << 16;
-      w.y = T::down(o[2] * inv) | static_cast<uint32_t>(T::down(o[3] * inv)) << 16;
-      *reinterpret_cast<u32x2*>(a.out + to * D + d) = w;
-    } else {
-      *reinterpret_cast<f32x4*>(a.part_o + (to * a.splits + split) * D + d) = o;
-      if (d == 0) a.part_ml[to * a.splits + split] = make_float2(top, sum);
-    }
-  };
-  // the i-th four output columns of a lane, of D / (4 wavefronts' lanes a column)
-  auto out4 = [&](int i, float by) __attribute__((always_inline)) {
-    constexpr int kFours = L::kEach / 4;
-    const Tile& o = acc[i / kFours];
-    const int e = i % kFours * 4;
-    return f32x4{o[e] * by, o[e + 1] * by, o[e + 2] * by, o[e + 3] * by};
-  };
-  constexpr int kFours = L::kOuts * L::kEach / 4;
-  auto out_at = [&](int i) { return kCol == 16 ? i * 16 + g * 4 : i * 8 + g * 4; };
+  constexpr int kFours = L::kEach / 4;
   l = L::sum_of(l);
   const int mine = wide * kCol + col;
   if (g == 0) {
@@ -924,29 +904,49 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
     stat[1][deep][mine] = l;
   }
   __syncthreads();
-  float best = stat[0][0][mine];
+  float top = stat[0][0][mine], sum = 0.f;
 #pragma unroll
-  for (int w = 1; w < kDeep; ++w) best = fmaxf(best, stat[0][w][mine]);
-  const float by = ref == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ref - best) * unit;
+  for (int w = 1; w < kDeep; ++w) top = fmaxf(top, stat[0][w][mine]);
 #pragma unroll
-  for (int i = 0; i < kFours; ++i) *reinterpret_cast<f32x4*>(&part[deep][mine][out_at(i)]) = out4(i, by);
+  for (int w = 0; w < kDeep; ++w) {
+    const float x = stat[0][w][mine];
+    sum += x == -__builtin_inff() ? 0.f : stat[1][w][mine] * __builtin_amdgcn_exp2f(x - top);
+  }
+  float by = ref == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(ref - top) * unit;
+  if (only) by *= sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // a sum that is NaN stays one
+#pragma unroll
+  for (int i = 0; i < L::kOuts * kFours; ++i) {
+    const Tile& o = acc[i / kFours];
+    const int e = i % kFours * 4;
+    *reinterpret_cast<f32x4*>(&part[deep][mine][kCol == 16 ? i * 16 + g * 4 : i * 8 + g * 4]) =
+        f32x4{o[e] * by, o[e + 1] * by, o[e + 2] * by, o[e + 3] * by};
+  }
   __syncthreads();
-  for (int i = tid; i < kCols * D / 4; i += kThreads) {
-    const int c = i / (D / 4), d = (i % (D / 4)) * 4, r = r0 + c;
-    if (r >= rows) break;
-    float top = stat[0][0][c], sum = 0.f;
+  if (!only && deep == 0 && g == 0 && r0 + mine < rows) {
+    const int token = a.over(r0 + mine);
+    const int64_t to = static_cast<int64_t>(s.row0 + token) * a.n_q + head * a.group + r0 + mine - token * a.group;
+    a.part_ml[to * a.splits + split] = make_float2(top, sum);
+  }
 #pragma unroll
-    for (int w = 1; w < kDeep; ++w) top = fmaxf(top, stat[0][w][c]);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < kCols * D / 4 / kThreads; ++i) {
+    const int c = (i * kThreads + tid) / (D / 4), d = tid % (D / 4) * 4, r = r0 + c, token = a.over(r);
+    const int64_t to = static_cast<int64_t>(s.row0 + token) * a.n_q + head * a.group + r - token * a.group;
+    f32x4 o = *reinterpret_cast<const f32x4*>(&part[0][c][d]);
 #pragma unroll
-    for (int w = 0; w < kDeep; ++w) {
-      const float x = stat[0][w][c];
-      sum += x == -__builtin_inff() ? 0.f : stat[1][w][c] * __builtin_amdgcn_exp2f(x - top);
+    for (int w = 1; w < kDeep; ++w) {
       const f32x4 y = *reinterpret_cast<const f32x4*>(&part[w][c][d]);
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] += y[e];
     }
-    store(r, d, o, top, sum);
+    if (r >= rows) continue;
+    if (only) {
+      u32x2 w;
+      w.x = T::down(o[0]) | static_cast<uint32_t>(T::down(o[1])) << 16;
+      w.y = T::down(o[2]) | static_cast<uint32_t>(T::down(o[3])) << 16;
+      *reinterpret_cast<u32x2*>(a.out + to * D + d) = w;
+    } else {
+      *reinterpret_cast<f32x4*>(a.part_o + (to * a.splits + split) * D + d) = o;
+    }
   }
 }
 
