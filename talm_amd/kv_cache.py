@@ -94,11 +94,12 @@ class CacheLayer:
 
     def attention(self, query, bounds, past, max_new, max_len, scale, window=None, sinks=0):
         """softmax(scale q K^T) V of query [1, Hq, N, D] over the cache, which holds the rows' own tokens
-        already: the row of token p sees the tokens up to p, in a `window` only the last `window` ones
-        (itself among them) and the sequence's first `sinks`. `max_len` is at least the longest sequence
-        with its new tokens (in a graph: with those of any replay). Values of tokens that a row does not
-        see must be finite, since a weight of 0 does not hide NaN; its keys may be anything. Returns
-        [1, N, Hq, D]; a row that sees nothing is zero, a row that no sequence holds undefined."""
+        already and none behind them (past[b] and b's rows are all that it has): the row of token p sees the
+        tokens up to p, in a `window` only the last `window` ones (itself among them) and the sequence's
+        first `sinks`. `max_len` is at least the longest sequence with its new tokens (in a graph: with those
+        of any replay). Values of tokens that a row does not see must be finite, since a weight of 0 does
+        not hide NaN; its keys may be anything. Returns [1, N, Hq, D]; a row that sees nothing is zero, a row
+        that no sequence holds undefined."""
         if window is not None and window < 1:
             raise ValueError(f"cache_attention: window {window} (at least 1, or None)")
         out = torch.ops.talm.cache_attention(query, bounds, past, max_new, max_len, self.codes, self.scales,

@@ -394,6 +394,65 @@ def test_pieces_over_loud_keys_and_quiet_values(dim, dtype, heads):
     c.check_attention([90, 30], window=100, sinks=70, std=0.3)
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dim,dtype,new", [
+    (128, torch.float16, [1, 60]), (64, torch.bfloat16, [3, 150]), (128, torch.bfloat16, [130, 1]),
+    (64, torch.float16, [1, 1])])
+def test_keys_that_are_not_finite(dim, dtype, new, bad):
+    """A key that is not finite, in a page and in the tail: rows that see it are NaN (an infinity in the tail
+    keeps its sign there: a row whose query turns it into a score of -inf gives it no weight), rows that do
+    not see it have the bits that they have without it, other heads too."""
+    bounds, n = Case(2, 2, dim, 1).spans(new)
+    (_, one), (_, two) = bounds.tolist()
+    q = Case(1, 1, dim, 1, dtype, seed=9).rows(n, 8)
+
+    def spoiled(lo, hi, column, place, total):
+        """[rows, 4] of the second KV head's heads: which rows' outputs are NaN."""
+        held_as_nan = bad != bad or place // 64 < total // 64
+        return torch.ones(hi - lo, 4, dtype=torch.bool) if held_as_nan else (q[0, 4:, lo:hi, column] > 0).T.cpu()
+
+    def both(past, window=None, sinks=0):
+        past = torch.tensor(past, dtype=torch.int32).cuda()
+        return (x.layer.attention(q, bounds, past, max(new), 2300, dim ** -0.5, window, sinks) for x in (c, d))
+
+    def check(got, want, nan):
+        assert want.isfinite().all() and torch.equal(got[:, :, :4], want[:, :, :4])
+        assert torch.equal(got[0, :, 4:].isnan().all(2).cpu(), nan)
+        assert torch.equal(got[0, :, 4:].isnan().any(2).cpu(), nan)
+
+    c, d = (Case(2, 2, dim, 2300, dtype, seed=5, heads=8) for _ in range(2))
+    long = 2170
+    for i, x in enumerate((c, d)):
+        k, v = x.rows(long + 100, 2), x.rows(long + 100, 2)
+        if i == 0:
+            k[0, 1, 40, 7] = k[0, 1, long + 99, 0] = bad
+        x.append([long, 100], k=k, v=v)
+        x.append(new)
+    nan = torch.cat((spoiled(0, one, 7, 40, long + new[0]), spoiled(one, two, 0, 99, 100 + new[1])))
+    check(*both([long, 100]), nan)
+    got, want = both([long, 100], window=200, sinks=3)  # leaves the first sequence's out
+    nan[:one] = False
+    check(got, want, nan)
+    assert torch.equal(got[:, :one], want[:, :one])
+
+    # among the new tokens: the rows in front of it do not see it
+    c, d = (Case(2, 2, dim, 400, dtype, seed=6, heads=8) for _ in range(2))
+    nan = torch.zeros(n, 4, dtype=torch.bool)
+    for i, x in enumerate((c, d)):
+        x.append([130, 100])
+        k, v = x.rows(n, 2), x.rows(n, 2)
+        if i == 0:
+            for (lo, hi), past in zip(bounds.tolist(), (130, 100)):
+                at = (lo + hi) // 2
+                k[0, 1, at, 3] = bad
+                nan[at:hi] = spoiled(at, hi, 3, past + at - lo, past + hi - lo)
+        x.append(new, k=k, v=v)
+    got, want = both([130, 100])
+    check(got, want, nan)
+    for lo, hi in bounds.tolist():
+        assert torch.equal(got[:, lo:(lo + hi) // 2], want[:, lo:(lo + hi) // 2])
+
+
 def test_attention_over_shared_pages():
     """Two sequences with a common beginning whose complete pages are the same."""
     c = Case(2, 1, 128, 300, heads=2)
