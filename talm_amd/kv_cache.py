@@ -201,6 +201,7 @@ class QuantizedCache(Cache):
         outer, unpad._cached.step = getattr(unpad._cached, "step", None), self
         try:
             yield
+            self._settled()
         except BaseException:
             self._broken = True
             raise
@@ -213,12 +214,29 @@ class QuantizedCache(Cache):
             raise RuntimeError("QuantizedCache: outside of a patched Qwen2 model's forward (solution.apply())")
         return self.cache_layers[layer_idx]
 
+    def _settled(self):
+        """The attention of what the last `update` returned must have been asked for here."""
+        if self._step.kept is not None:
+            raise RuntimeError("QuantizedCache: a layer's attention was not of the keys and values that the cache "
+                               "returned to it")
+
     def update(self, key_states, value_states, layer_idx, *args, **kwargs):
         """New keys and values [B, Hkv, T, D] of one layer; returns them (the attention reads the cache)."""
         layer, s = self._layer(layer_idx), self._step
+        self._settled()
         key_states, value_states = key_states.to(self.dtype), value_states.to(self.dtype)
+        if key_states.shape[0] != self.batch or key_states.shape[2] != s.rows:
+            raise ValueError(f"QuantizedCache: keys of {key_states.shape[0]} sequences of {key_states.shape[2]} tokens "
+                             f"in a call of {self.batch} of {s.rows}")
         layer.write(_packed(key_states), _packed(value_states), s.bounds, s.past, s.max_new)
-        return key_states, value_states
+        s.kept = key_states, value_states
+        return s.kept
+
+    def asked(self, key, value):
+        """Whether an attention call is of the keys and values that the last `update` returned: a model that runs
+        inside of this one's call, a probe or a guard, has others."""
+        kept = self._step.kept
+        return kept is not None and key is kept[0] and value is kept[1]
 
     def takes(self, query, tables):
         """Whether `answer` serves the call: not a first one (its keys are needed in 16 bits), of the
@@ -240,6 +258,10 @@ class QuantizedCache(Cache):
             raise ValueError("QuantizedCache: no dropout of attention weights")
         layer, s = self._layer(module.layer_idx), self._step
         b, heads, t, d = query.shape
+        if b != self.batch or t != s.rows:
+            raise ValueError(f"QuantizedCache: queries of {b} sequences of {t} tokens in a call of {self.batch} of "
+                             f"{s.rows}")
+        s.kept = None
         scale = scaling if scaling is not None else d ** -0.5
         sinks = unpad.attention_sinks(module) if window is not None else 0
         q = _packed(query.to(self.dtype))
@@ -266,6 +288,7 @@ class _Step:
     def __init__(self, bounds, past, max_new, max_len, cu, rows, real):
         self.bounds, self.past, self.max_new, self.max_len = bounds, past, max_new, max_len
         self.cu, self.rows, self.real = cu, rows, real
+        self.kept = None  # the keys and values that `update` returned, until their attention
 
 
 def _runs(mask, batch, columns, rows):

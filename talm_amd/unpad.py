@@ -397,7 +397,7 @@ def patch_sdpa_rows():
     def rows_sdpa(module, query, key, value, attention_mask, dropout=0.0, scaling=None,
                   sliding_window=None, **kwargs):
         cache = getattr(_cached, "step", None)
-        if cache is not None:
+        if cache is not None and cache.asked(key, value):
             return cache.attend(module, query, key, value, dropout, scaling, sliding_window), None
         sinks = attention_sinks(module) if sliding_window is not None else 0
         if not _rows or query.shape[0] != 1:
