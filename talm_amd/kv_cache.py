@@ -202,6 +202,9 @@ class QuantizedCache(Cache):
         try:
             yield
             self._settled()
+            if len(self._step.written) != len(self.cache_layers):
+                raise RuntimeError(f"QuantizedCache: layers {sorted(self._step.written)} of {len(self.cache_layers)} "
+                                   "wrote their tokens (a checkpointed layer is not given the cache)")
         except BaseException:
             self._broken = True
             raise
@@ -214,6 +217,15 @@ class QuantizedCache(Cache):
             raise RuntimeError("QuantizedCache: outside of a patched Qwen2 model's forward (solution.apply())")
         return self.cache_layers[layer_idx]
 
+    def _writes(self, layer_idx):
+        """The layer, about to be written in this call."""
+        layer = self._layer(layer_idx)
+        self._settled()
+        if layer_idx in self._step.written:
+            raise RuntimeError(f"QuantizedCache: layer {layer_idx} wrote its tokens already in this call")
+        self._step.written.add(layer_idx)
+        return layer
+
     def _settled(self):
         """The attention of what the last `update` returned must have been asked for here."""
         if self._step.kept is not None:
@@ -222,8 +234,7 @@ class QuantizedCache(Cache):
 
     def update(self, key_states, value_states, layer_idx, *args, **kwargs):
         """New keys and values [B, Hkv, T, D] of one layer; returns them (the attention reads the cache)."""
-        layer, s = self._layer(layer_idx), self._step
-        self._settled()
+        layer, s = self._writes(layer_idx), self._step
         key_states, value_states = key_states.to(self.dtype), value_states.to(self.dtype)
         if key_states.shape[0] != self.batch or key_states.shape[2] != s.rows:
             raise ValueError(f"QuantizedCache: keys of {key_states.shape[0]} sequences of {key_states.shape[2]} tokens "
@@ -247,7 +258,7 @@ class QuantizedCache(Cache):
     def answer(self, query, key, value, layer_idx, tables, scale, window, sinks):
         """Attention of new rows [1, H, N, D] that are not turned yet, tables (cos, sin) float32 [N, D]: written
         with their rotary positions in one launch, then attended. Returns [1, N, Hq, D]."""
-        layer, s = self._layer(layer_idx), self._step
+        layer, s = self._writes(layer_idx), self._step
         turned = layer.write(key, value, s.bounds, s.past, s.max_new, query, tables)
         return self._clean(layer.attention(turned, s.bounds, s.past, s.max_new, s.max_len, scale, window, sinks))
 
@@ -288,6 +299,7 @@ class _Step:
     def __init__(self, bounds, past, max_new, max_len, cu, rows, real):
         self.bounds, self.past, self.max_new, self.max_len = bounds, past, max_new, max_len
         self.cu, self.rows, self.real = cu, rows, real
+        self.written = set()  # the layers that hold the call's tokens
         self.kept = None  # the keys and values that `update` returned, until their attention
 
 

@@ -133,3 +133,37 @@ def test_attention_of_other_keys_than_the_caches_is_refused(patched, monkeypatch
         _answers(model, cache)
     cache.reset()
     assert torch.equal(_answers(model, cache), want)
+
+
+@pytest.mark.parametrize("layers", [(0, 1), (1,)])
+def test_layers_that_leave_the_cache_out_are_refused(patched, layers):
+    """transformers takes the cache from a layer that is checkpointed: its tokens would be missing from then on."""
+    model = _qwen2()
+    cache, want = _cache(model), _answers(model, _cache(model))
+    for i in layers:
+        layer = model.model.layers[i]
+        layer.training, layer.gradient_checkpointing = True, True
+        layer._gradient_checkpointing_func = lambda f, *args: f(*args)
+    with pytest.raises(RuntimeError, match="layers"):
+        _answers(model, cache)
+    for layer in model.model.layers:
+        layer.training = False
+    with pytest.raises(RuntimeError, match="reset"):
+        _answers(model, cache)
+    cache.reset()
+    assert torch.equal(_answers(model, cache), want)
+
+
+def test_layers_that_write_twice_are_refused(patched):
+    """The same tokens again would meet an open block that holds them already."""
+    model = _qwen2()
+    layer = model.model.layers[0]
+    forward = layer.forward
+
+    def twice(*args, **kwargs):
+        forward(*args, **kwargs)
+        return forward(*args, **kwargs)
+
+    layer.forward = twice
+    with pytest.raises(RuntimeError, match="layer 0"):
+        _answers(model, _cache(model))
