@@ -837,7 +837,8 @@ def _attention_block(attn, x, group, adapters, weights, rope, n_tok):
 def _few_attention(attn, x, position_embeddings, attention_mask, past_key_values, plan, kwargs):
     """Qwen2Attention.forward for a few tokens without autograd: q|k|v (+ LoRA) as one product on the
     NF4 codes (few_tokens.py), the rotary embedding in place, then transformers' own steps (the
-    cache, the attention interface, o_proj), or an 8-bit cache's (kv_cache.py). None where the product does not take the layer."""
+    cache, the attention interface, o_proj), or an 8-bit cache's (kv_cache.py). None where the product
+    does not take the layer."""
     from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
     from transformers.models.qwen2 import modeling_qwen2
 
@@ -859,13 +860,14 @@ def _few_attention(attn, x, position_embeddings, attention_mask, past_key_values
             and hd % 2 == 0 and hd <= 512 and cos.shape[1] == lead[-1] and len(lead) == 2 \
             and cos.shape[0] in (1, lead[0]) and "rope" not in DISABLED:
         tables = [t.expand(*lead, hd).reshape(-1, hd) for t in (cos, sin)]
-        if isinstance(past_key_values, QuantizedCache) and past_key_values.takes(rows, tables):
+        if isinstance(past_key_values, QuantizedCache) and past_key_values.takes(rows.dtype, hd):
             # the 8-bit cache turns queries and keys as it writes
             packed = [rows[:, lo:hi].view(-1, (hi - lo) // hd, hd).transpose(0, 1)[None]
                       for lo, hi in ((0, n_q), (n_q, n_q + n_k), (n_q + n_k, rows.shape[1]))]
             window = attn.sliding_window
             y = past_key_values.answer(*packed, attn.layer_idx, tables, attn.scaling, window,
-                                       attention_sinks(attn) if window is not None else 0)
+                                       attention_sinks(attn) if window is not None else 0,
+                                       0.0 if not attn.training else attn.attention_dropout)
             return attn.o_proj(y.view(*lead, -1)), None
         rope_(rows[:, :n_q].view(-1, n_q // hd, hd), rows[:, n_q:n_q + n_k].view(-1, n_k // hd, hd), *tables)
         RAN["rope"] += 1

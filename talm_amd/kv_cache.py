@@ -249,15 +249,17 @@ class QuantizedCache(Cache):
         kept = self._step.kept
         return kept is not None and key is kept[0] and value is kept[1]
 
-    def takes(self, query, tables):
-        """Whether `answer` serves the call: not a first one (its keys are needed in 16 bits), of the
-        cache's type, with tables that the write turns by."""
-        return (self._step is not None and self._step.cu is None and query.dtype == self.dtype
-                and tables[0].shape[-1] == query.shape[-1])
+    def takes(self, dtype, dim):
+        """Whether `answer` serves the call: not a first one (its keys are needed in 16 bits), with heads of
+        the cache's type and size."""
+        return (self._step is not None and self._step.cu is None and dtype == self.dtype
+                and dim == self.cache_layers[0].tail.shape[3] // BLOCK)
 
-    def answer(self, query, key, value, layer_idx, tables, scale, window, sinks):
+    def answer(self, query, key, value, layer_idx, tables, scale, window, sinks, dropout=0.0):
         """Attention of new rows [1, H, N, D] that are not turned yet, tables (cos, sin) float32 [N, D]: written
         with their rotary positions in one launch, then attended. Returns [1, N, Hq, D]."""
+        if dropout:
+            raise ValueError("QuantizedCache: no dropout of attention weights")
         layer, s = self._writes(layer_idx), self._step
         turned = layer.write(key, value, s.bounds, s.past, s.max_new, query, tables)
         return self._clean(layer.attention(turned, s.bounds, s.past, s.max_new, s.max_len, scale, window, sinks))

@@ -45,3 +45,41 @@ def test_other_models_calls_are_their_own(patched):
         h.remove()
     assert len(seen) == 9 and all(torch.equal(x, want) for x in seen)
     assert torch.equal(got, alone)
+
+
+SLIDING = dict(use_sliding_window=True, sliding_window=50, max_window_layers=1, attention_sinks=3)
+
+
+@pytest.mark.parametrize("batch,pads", [(1, (0,)), (4, (0, 69, 13, 64))])
+@pytest.mark.parametrize("overrides", [{}, {"num_attention_heads": 8, "num_key_value_heads": 2, "head_dim": 64}, SLIDING])
+def test_few_tokens_turn_as_they_are_written(monkeypatch, patched, batch, pads, overrides):
+    """Calls of few tokens behind the first go through the write that turns queries and keys: no rotary launch
+    of their own, and the bits that turning them apart gives (rope_ in fp16 rounds as the write does)."""
+    model = _model(**overrides)
+    patches.apply()
+    answer, counts = QuantizedCache.answer, []
+
+    def counted(self, *args):
+        counts.append(args[3])
+        return answer(self, *args)
+
+    monkeypatch.setattr(QuantizedCache, "answer", counted)
+    ids, mask, pieces = _ids(batch, 140), _mask(batch, 120, pads), [120, 1, 1, 5, 3, 1]
+    got = _answer(model, QuantizedCache(model.config, batch, 140), ids, mask, pieces)
+    assert counts == [0, 1, 2] * 5
+    rotary = engaged.RAN["rope"]
+    monkeypatch.setattr(QuantizedCache, "takes", lambda *args: False)
+    want = _answer(model, QuantizedCache(model.config, batch, 140), ids, mask, pieces)
+    assert torch.equal(got, want) and len(counts) == 15
+    assert engaged.RAN["rope"] - rotary == rotary + 15  # the first call's stays
+
+
+def test_few_tokens_refuse_dropout_of_attention_weights(patched):
+    model = _model(attention_dropout=0.1)
+    patches.apply()
+    cache, ids, mask = QuantizedCache(model.config, 2, 30), _ids(2, 21), _mask(2, 20, (0, 0))
+    _answer(model, cache, ids, mask, [20])
+    for layer in model.model.layers:
+        layer.self_attn.training = True
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.float16), pytest.raises(ValueError, match="dropout"):
+        model(input_ids=ids[:, 20:], past_key_values=cache, use_cache=True)
