@@ -789,9 +789,10 @@ int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, const uint8_
  *
  * talm_cache_attn: out [n_rows, n_q, D] dense, row i of sequence b = softmax(scale q K^T) V over the cached tokens
  * j <= past[b] + i, with a window (> 0) only those with past[b] + i - j < window or j < sinks; zeros where it sees
- * none. The cache holds the rows' own tokens already: past[b] + (rows of b) tokens in all, of which max_len at
+ * none. The cache holds the rows' own tokens already: past[b] + (rows of b) tokens in all, max_len at
  * least as many. Codes enter the products exactly; the keys' scale multiplies the fp32 scores, the values' the
- * fp32 sums. Values of tokens that a row does not see must be finite (its keys may be anything). `workspace` holds
+ * fp32 sums, and a mean past the type's largest number is that number. Values of tokens that a row does not
+ * see must be finite (its keys may be anything). `workspace` holds
  * talm_cache_attn_workspace bytes (-1: rejected shape). Deterministic.
  */
 int talm_cache_write(const uint16_t* k, int64_t k_stride_tok, int64_t k_stride_head,

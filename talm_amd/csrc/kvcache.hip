@@ -72,7 +72,10 @@ __device__ __forceinline__ Span span_of(const int32_t* bounds, const int32_t* pa
   return span_of(bounds[2 * seq], bounds[2 * seq + 1], past[seq], static_cast<int>(n_rows), max_new, max_len);
 }
 
+// kMost: the type's largest number. Attention holds sums of values times kUnit: bfloat16's largest values times
+// weights below 2^8 of at most 2^30 tokens would leave fp32 (2^-40 costs results below 2^-100 bits).
 struct F16 {
+  static constexpr float kMost = 65504.f, kUnit = 1.f;
   static __device__ __forceinline__ float up(uint32_t bits) { return h2f(static_cast<uint16_t>(bits)); }
   static __device__ __forceinline__ uint16_t down(float x) { return f2h(x); }
   // 8 e4m3 codes, exactly
@@ -91,6 +94,7 @@ struct F16 {
   }
 };
 struct BF16 {
+  static constexpr float kMost = 0x1.fep127f, kUnit = 0x1p-40f;
   static __device__ __forceinline__ float up(uint32_t bits) { return __builtin_bit_cast(float, bits << 16); }
   static __device__ __forceinline__ uint16_t down(float x) {
     return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
@@ -507,6 +511,22 @@ struct Visits {
   __device__ __forceinline__ int page(int i) const { return i < sinks ? i : i - sinks + first; }
 };
 
+// Four outputs in 16 bits from means of values times kUnit. A mean past the type's largest number (values whose
+// codes were rounded past it) is that number, as those values are where they are read back.
+template <class T>
+__device__ __forceinline__ u32x2 outputs(f32x4 x) {
+  constexpr float kTop = T::kMost * T::kUnit;
+  if (fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))) > kTop) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (fabsf(x[e]) < __builtin_inff()) x[e] = fminf(fmaxf(x[e], -kTop), kTop);
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = T::down(x[e] * (1.f / T::kUnit));
+  return u32x2{w[0] | w[1] << 16, w[2] | w[3] << 16};
+}
+
 // How S^T = K Q^T and O^T = V^T P^T of one page lie in a wavefront with kCol query columns, 16
 // (v_mfma_*_16x16x32) or 32 (v_mfma_*_32x32x16; half as many instructions for the same products, each of
 // which takes the VALU's issue for about 8 cycles). Lane l is column l % kCol, quarter or half g = l / kCol.
@@ -776,7 +796,7 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
         page_l = static_cast<int>(a.c.page(seq, visits.page(mine)));
       if (page_l >= 0) {
         ks_l = a.c.scales[static_cast<int64_t>(page_l) * 2 * a.c.kv + head];
-        vs_l = a.c.scales[(static_cast<int64_t>(page_l) * 2 + 1) * a.c.kv + head];
+        vs_l = a.c.scales[(static_cast<int64_t>(page_l) * 2 + 1) * a.c.kv + head] * T::kUnit;
       }
     }
     const int count = min((code_end - base + kDeep - 1) / kDeep, kWave);
@@ -867,10 +887,10 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
     } else {
 #pragma unroll
       for (int i = 0; i < L::kLane; ++i) {
-        const float x = st[i / L::kEach][i % L::kEach];
-        const uint16_t b = T::down(x);
+        const float x = st[i / L::kEach][i % L::kEach], y = x * T::kUnit;
+        const uint16_t b = T::down(y);
         hi[i / 8][i % 8] = __builtin_bit_cast(_Float16, b);
-        lo[i / 8][i % 8] = __builtin_bit_cast(_Float16, T::down(x - T::up(b)));
+        lo[i / 8][i % 8] = __builtin_bit_cast(_Float16, T::down(y - T::up(b)));
         l += x;
       }
     }
@@ -940,10 +960,7 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
     }
     if (r >= rows) continue;
     if (only) {
-      u32x2 w;
-      w.x = T::down(o[0]) | static_cast<uint32_t>(T::down(o[1])) << 16;
-      w.y = T::down(o[2]) | static_cast<uint32_t>(T::down(o[3])) << 16;
-      *reinterpret_cast<u32x2*>(a.out + to * D + d) = w;
+      *reinterpret_cast<u32x2*>(a.out + to * D + d) = outputs<T>(o);
     } else {
       *reinterpret_cast<f32x4*>(a.part_o + (to * a.splits + split) * D + d) = o;
     }
@@ -1075,10 +1092,9 @@ __global__ __launch_bounds__(kThreads) void cache_join_kernel(AttnArgs a) {
     }
     if (grp == 0) {
       const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
-      u32x2 out;
-      out.x = T::down(total[0] * inv) | static_cast<uint32_t>(T::down(total[1] * inv)) << 16;
-      out.y = T::down(total[2] * inv) | static_cast<uint32_t>(T::down(total[3] * inv)) << 16;
-      *reinterpret_cast<u32x2*>(a.out + to[k] * D + d) = out;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) total[e] *= inv;
+      *reinterpret_cast<u32x2*>(a.out + to[k] * D + d) = outputs<T>(total);
     }
   }
 }

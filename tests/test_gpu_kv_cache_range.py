@@ -1,0 +1,54 @@
+"""The 8-bit cache's attention (kv_cache.CacheLayer) at the ends of its ranges: values as large as their type
+holds, and long sequences whose every part shows in the output. Tolerances are those of
+test_gpu_kv_cache.py unless a test derives its own."""
+
+import pytest
+import torch
+
+from test_gpu_kv_cache import Case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dim,heads,past,new", [
+    (128, 4, [70, 20, 1000], [1, 1, 1]),        # tiles of 16 rows in one part
+    (64, 4, [3000, 500], [1, 2]),               # in parts, which are joined
+    (128, 1, [20000], [1]),                     # in many
+    (128, 6, [300, 2000], [40, 20]),            # tiles of 32 rows
+    (64, 16, [130, 8700], [150, 450])])         # and of 64, in parts
+def test_values_of_the_types_largest_magnitudes(dim, heads, past, new, dtype):
+    """Outputs are means of values and no larger than the type's largest number, also where a code rounds
+    past it (its values read as that number) and sums of many are past float32's."""
+    most = torch.finfo(dtype).max
+    c = Case(len(past), 1, dim, max(p + n for p, n in zip(past, new)), dtype, heads=heads)
+    sign = torch.where(torch.arange(dim) % 3 == 0, -1.0, 1.0)
+
+    def top(n):
+        return (sign.expand(n, dim) * most).to(dtype).cuda()[None, None]
+
+    def loud(n):
+        return ((2 * torch.rand(n, dim, generator=c.g) - 1).double() * most).to(dtype).cuda()[None, None]
+
+    for make in (top, loud):
+        c.tokens = [t[:, :, :0] for t in c.tokens]
+        c.append(past, v=make(sum(past)))
+        c.append(new, v=make(sum(new)))
+        out = c.check_attention(new)
+        assert out.isfinite().all()
+        if make is top:
+            assert (out[0].sign().cpu() == sign).all()
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_infinite_values_stay_infinite(new):
+    """What is not finite in 16 bits is no large number: rows that see it are not finite."""
+    for dtype in (torch.float16, torch.bfloat16):
+        c = Case(1, 1, 64, 200, dtype, heads=2)
+        v = c.rows(100 + new, 1)
+        v[0, 0, 90, 5] = float("inf")
+        c.append([100], v=v[:, :, :100])
+        c.append([new], v=v[:, :, 100:])
+        past = torch.tensor([100], dtype=torch.int32).cuda()
+        out = c.layer.attention(c.rows(new, 2), torch.tensor([[0, new]], dtype=torch.int32).cuda(), past, new, 200, 0.125)
+        assert not out[..., 5].isfinite().any() and out[..., :5].isfinite().all()
