@@ -20,6 +20,7 @@
 #include <ATen/hip/HIPContext.h>
 #include <hipblaslt/hipblaslt-ext.hpp>
 #include <hipblaslt/hipblaslt.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -1060,6 +1061,15 @@ struct CacheSizes {
   int64_t pages, kv, dim, seqs, width;
 };
 
+// The cache's operators have no derivative: a tensor that needs one, backwards or forwards (a dual tensor, which
+// no_grad does not switch off), is refused.
+void cache_constant(const Tensor& t, const char* what) {
+  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()) &&
+                        !(c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()),
+                    "cache: ", what, " requires a gradient, and the cache's operators have none: call them without "
+                    "autograd");
+}
+
 CacheSizes cache_buffers(const Tensor& codes, const Tensor& scales, const Tensor& tail, const Tensor& table) {
   require(codes.is_cuda() && codes.scalar_type() == at::kFloat8_e4m3fn && codes.dim() == 4 && codes.size(1) == 2 &&
               codes.is_contiguous() && (codes.size(3) == 64 * 64 || codes.size(3) == 64 * 128),
@@ -1075,6 +1085,8 @@ CacheSizes cache_buffers(const Tensor& codes, const Tensor& scales, const Tensor
   require(table.device() == codes.device() && table.scalar_type() == at::kInt && table.is_contiguous() &&
               table.dim() == 2 && table.size(0) == tail.size(0),
           "cache: table int32 [sequences, width] on the codes' device, contiguous");
+  cache_constant(scales, "scales");
+  cache_constant(tail, "tail");
   return CacheSizes{codes.size(0), codes.size(2), codes.size(3) / 64, tail.size(0), table.size(1)};
 }
 
@@ -1092,8 +1104,7 @@ Tensor cache_rows(const Tensor& t, const Tensor& tail, int64_t dim, const char* 
   TORCH_CHECK_VALUE(t.device() == tail.device() && t.scalar_type() == tail.scalar_type() && t.dim() == 4 &&
                         t.size(0) == 1 && t.size(3) == dim,
                     "cache: ", what, " must be [1, H, N, ", dim, "] of the tail's type on the cache's device");
-  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()), "cache: ", what,
-                    " requires a gradient, and the cache's operators have none: call them without autograd");
+  cache_constant(t, what);
   return head_rows(t);
 }
 
@@ -1118,6 +1129,7 @@ OptTensor cache_write(const Tensor& key, const Tensor& value, const Tensor& boun
     auto rows = [&](const Tensor& t) {
       require(t.device() == codes.device() && t.scalar_type() == at::kFloat && same_shape(t, n, c.dim),
               "cache_write: cos and sin float32 [N, D] on the cache's device");
+      cache_constant(t, "cos or sin");
       return t;
     };
     cs = rows(*cos);
@@ -1173,6 +1185,7 @@ std::tuple<Tensor, Tensor> cache_read(const Tensor& codes, const Tensor& scales,
     require(out->device() == codes.device() && out->scalar_type() == tail.scalar_type() && out->is_contiguous() &&
                 out->dim() == 3 && out->size(0) == rows && out->size(1) == c.kv && out->size(2) == c.dim,
             "cache_read: out [rows, Hkv, D] of the tail's type on the cache's device, contiguous");
+    cache_constant(*out, "out");
     return out->as_strided(sizes, strides);
   };
   const Tensor key = buffer(out_key), value = buffer(out_value);

@@ -52,3 +52,48 @@ def test_infinite_values_stay_infinite(new):
         past = torch.tensor([100], dtype=torch.int32).cuda()
         out = c.layer.attention(c.rows(new, 2), torch.tensor([[0, new]], dtype=torch.int32).cuda(), past, new, 200, 0.125)
         assert not out[..., 5].isfinite().any() and out[..., :5].isfinite().all()
+
+
+def test_operands_with_derivatives_are_refused():
+    """Whoever wants a derivative, backwards or forwards, gets an error and not a result without one."""
+    import torch.autograd.forward_ad as forward
+
+    c = Case(2, 2, 64, 128, heads=4)
+    c.append([70, 3])
+    bounds, _ = c.spans([1, 1])
+    past, k, q = torch.tensor([70, 3], dtype=torch.int32).cuda(), c.rows(2, 2), c.rows(2, 4)
+    table = torch.zeros(2, 64, device="cuda")
+    out = torch.empty(2, 2, 64, dtype=torch.float16, device="cuda")
+    layer = c.layer
+
+    def write(k=k, v=k, q=q, cos=table, sin=table, **parts):
+        with_parts(parts).write(k, v, bounds, past, 1, q, (cos, sin))
+
+    def attend(q=q, **parts):
+        with_parts(parts).attention(q, bounds, past, 1, 128, 1.0)
+
+    def read(out=out, **parts):
+        with_parts(parts).read(past, bounds, past * 0, 1, 2, (out, out.detach().clone()))
+
+    def with_parts(parts):
+        names = ("codes", "scales", "tail", "table")
+        return type(layer)(**{n: parts.get(n, getattr(layer, n)) for n in names})
+
+    asked = [(write, "k", k), (write, "v", k), (write, "q", q), (write, "cos", table), (write, "sin", table),
+             (attend, "q", q), (read, "out", out)]
+    asked += [(f, n, getattr(layer, n)) for f in (write, attend, read) for n in ("scales", "tail")]
+    for call, name, x in asked:
+        call()
+        wanted = x.detach().clone().requires_grad_()
+        with pytest.raises(ValueError, match="gradient"):
+            call(**{name: wanted})
+        with torch.no_grad():
+            call(**{name: wanted})
+        with forward.dual_level():
+            dual = forward.make_dual(x.detach().clone(), torch.ones_like(x))
+            with pytest.raises(ValueError, match="gradient"):
+                call(**{name: dual})
+            with torch.no_grad(), pytest.raises(ValueError, match="gradient"):
+                call(**{name: dual})
+            with forward._set_fwd_grad_enabled(False):
+                call(**{name: dual})
