@@ -28,6 +28,7 @@ from . import _ops, unpad  # noqa: F401 - _ops registers torch.ops.talm.*
 from .engaged import ON, RAN
 
 BLOCK = 64
+_HALVES = (torch.float16, torch.bfloat16)
 
 
 class CacheLayer:
@@ -55,7 +56,7 @@ class CacheLayer:
     def allocate(cls, sequences, kv_heads, head_dim, capacity, dtype=torch.float16, device="cuda"):
         """Buffers for `sequences` of up to `capacity` tokens, sequence b's pages one behind the other."""
         if min(sequences, kv_heads, capacity) < 0 or head_dim not in (64, 128) \
-                or dtype not in (torch.float16, torch.bfloat16):
+                or dtype not in _HALVES:
             raise ValueError(f"CacheLayer: {sequences} sequences of {capacity} tokens, {kv_heads} KV heads of "
                              f"{head_dim} (64 or 128) in {dtype} (float16 or bfloat16)")
         width = -(-capacity // BLOCK)
@@ -123,19 +124,24 @@ class QuantizedCache(Cache):
     Each call's new tokens are those that its attention mask names, one run per sequence (left-padded
     prompts, as generation has them); padding is neither stored nor attended to. A first call attends to
     its own 16-bit keys and values where the packed rows' kernels take them (fp16 or bfloat16 heads of
-    128), later ones, and first ones of heads of 64, to the cache. It needs solution.apply(), the "sdpa"
+    128), later ones, and first ones of heads of 64, to the cache. `dtype`, of its 16-bit parts and its
+    attention, is by default that of the first call's keys: float32 ones count as autocast's type, and
+    without autocast as bfloat16, which has their range. A named float16 makes numbers past 65504
+    infinite. It needs solution.apply(), the "sdpa"
     attention, and no gradient; it does not reorder, repeat or crop its sequences (beam search, assisted
     generation), and its calls run eagerly (a step to capture in a HIP graph takes CacheLayer)."""
 
     is_compileable = False
 
-    def __init__(self, config, batch, capacity, dtype=torch.float16, device="cuda"):
+    def __init__(self, config, batch, capacity, dtype=None, device="cuda"):
         super().__init__(layers=[])
         heads = config.num_attention_heads
         dim = getattr(config, "head_dim", None) or config.hidden_size // heads
-        self.cache_layers = [CacheLayer.allocate(batch, config.num_key_value_heads, dim, capacity, dtype, device)
+        self.cache_layers = [CacheLayer.allocate(batch, config.num_key_value_heads, dim, capacity,
+                                                 torch.float16 if dtype is None else dtype, device)
                              for _ in range(config.num_hidden_layers)]
-        self.batch, self.capacity, self.dtype = batch, capacity, dtype
+        self.batch, self.capacity = batch, capacity
+        self.named_dtype = self.dtype = dtype
         self.device = torch.device(device)
         self.lengths, self.columns = [0] * batch, 0
         self._step = self._broken = None
@@ -158,6 +164,7 @@ class QuantizedCache(Cache):
         """Empty again, also after a call that failed part-way."""
         self.lengths, self.columns = [0] * self.batch, 0
         self._step = self._broken = None
+        self.dtype = self.named_dtype
 
     def _unsupported(self, *args, **kwargs):
         raise NotImplementedError("QuantizedCache does not reorder, repeat, select, crop or offload its sequences")
@@ -226,6 +233,22 @@ class QuantizedCache(Cache):
         self._step.written.add(layer_idx)
         return layer
 
+    def _take_type(self, key):
+        """The cache's type from its first keys, unless it was named; later ones must be of the same."""
+        if self.named_dtype is not None:
+            return
+        dtype = key.dtype
+        if dtype not in _HALVES:
+            kind = key.device.type
+            dtype = torch.get_autocast_dtype(kind) if torch.is_autocast_enabled(kind) else None
+            dtype = dtype if dtype in _HALVES else torch.bfloat16
+        if self.dtype is None:
+            self.dtype = dtype
+            for layer in self.cache_layers:
+                layer.tail = layer.tail.view(dtype)
+        elif self.dtype != dtype:
+            raise ValueError(f"QuantizedCache: keys of {dtype} behind ones of {self.dtype}: name the cache's dtype")
+
     def _settled(self):
         """The attention of what the last `update` returned must have been asked for here."""
         if self._step.kept is not None:
@@ -235,6 +258,7 @@ class QuantizedCache(Cache):
     def update(self, key_states, value_states, layer_idx, *args, **kwargs):
         """New keys and values [B, Hkv, T, D] of one layer; returns them (the attention reads the cache)."""
         layer, s = self._writes(layer_idx), self._step
+        self._take_type(key_states)
         key_states, value_states = key_states.to(self.dtype), value_states.to(self.dtype)
         if key_states.shape[0] != self.batch or key_states.shape[2] != s.rows:
             raise ValueError(f"QuantizedCache: keys of {key_states.shape[0]} sequences of {key_states.shape[2]} tokens "

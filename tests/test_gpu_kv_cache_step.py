@@ -3,9 +3,9 @@ serve them, in which types, and sliding layers over pages."""
 
 import pytest
 import torch
-from transformers import LlamaConfig, LlamaForCausalLM
+from transformers import LlamaConfig, LlamaForCausalLM, Qwen2ForCausalLM
 
-from talm_amd import engaged, patches, qgroup
+from talm_amd import engaged, patches, qgroup, qlora_model, state
 from talm_amd.kv_cache import QuantizedCache
 from test_gpu_kv_cache_model import _answer, _ids, _mask, _model
 
@@ -83,3 +83,27 @@ def test_few_tokens_refuse_dropout_of_attention_weights(patched):
         layer.self_attn.training = True
     with torch.no_grad(), torch.autocast("cuda", dtype=torch.float16), pytest.raises(ValueError, match="dropout"):
         model(input_ids=ids[:, 20:], past_key_values=cache, use_cache=True)
+
+
+def test_a_bfloat16_model_is_held_in_bfloat16(monkeypatch, patched):
+    """Keys and values past fp16's largest number, in a first call, single tokens, a completed page and a piece."""
+    for fp16_only in ("swiglu", "rmsnorm", "addnorm"):
+        monkeypatch.setitem(state.DISABLED, fp16_only, "a bfloat16 model")
+    config = qlora_model.qwen2_config(vocab_size=1000, hidden_size=512, intermediate_size=1024, num_hidden_layers=2,
+                                      num_attention_heads=4, num_key_value_heads=2, head_dim=128)
+    torch.manual_seed(5)
+    model = Qwen2ForCausalLM(config).to("cuda", torch.bfloat16).eval()
+    with torch.no_grad():
+        for layer in model.model.layers:
+            layer.self_attn.k_proj.bias[3] = 1e5
+            layer.self_attn.v_proj.bias[5] = -2e5
+    patches.apply()
+    ids, cache = _ids(2, 80), QuantizedCache(config, 2, 80)
+    at = 0
+    with torch.no_grad():
+        for n in (60, 1, 9, 10):
+            out = model(input_ids=ids[:, at:at + n], past_key_values=cache, use_cache=True).logits
+            assert out.isfinite().all() and out.dtype == torch.bfloat16
+            at += n
+    assert cache.dtype is torch.bfloat16
+    assert all(layer.tail.dtype is torch.bfloat16 for layer in cache.cache_layers)

@@ -50,7 +50,7 @@ def _qwen2(seed=0, **more):
 
 
 def _cache(model, batch=2, capacity=64, **more):
-    return kv_cache.QuantizedCache(model.config, batch, capacity, device="cpu", **more)
+    return kv_cache.QuantizedCache(model.config, batch, capacity, device="cpu", **{"dtype": torch.float16, **more})
 
 
 def _ids(batch, n, seed=1):
@@ -167,3 +167,50 @@ def test_layers_that_write_twice_are_refused(patched):
     layer.forward = twice
     with pytest.raises(RuntimeError, match="layer 0"):
         _answers(model, _cache(model))
+
+
+@pytest.mark.parametrize("model_type,held", [
+    (torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.bfloat16)])
+def test_a_cache_is_of_the_models_type(patched, model_type, held):
+    """Unless it is named: of the first call's keys, and bfloat16 for float32 ones, whose range it has."""
+    model = _qwen2().to(model_type)
+    cache = _cache(model, dtype=None)
+    assert cache.dtype is None
+    got = _answers(model, cache)
+    assert cache.dtype is held and all(layer.tail.dtype is held for layer in cache.cache_layers)
+    assert torch.equal(got, _answers(model, _cache(model, dtype=held)))
+    other = torch.bfloat16 if held is torch.float16 else torch.float16
+    model.to(other)
+    with pytest.raises(ValueError, match="dtype"), torch.no_grad():
+        model(input_ids=_ids(2, 1), past_key_values=cache, use_cache=True)
+    cache.reset()
+    _answers(model, cache)
+    assert cache.dtype is other
+
+
+def test_autocast_names_the_type_of_float32_keys(patched):
+    model, cache = _qwen2(), None
+    for held in (torch.float16, torch.bfloat16):
+        cache = _cache(model, dtype=None)
+        with torch.autocast("cpu", dtype=held):
+            _answers(model, cache)
+        assert cache.dtype is held
+
+
+@pytest.mark.parametrize("model_type", [torch.bfloat16, torch.float32])
+def test_keys_past_fp16s_range_are_held(patched, model_type):
+    model = _qwen2().to(model_type)
+    with torch.no_grad():
+        for layer in model.model.layers:
+            layer.self_attn.k_proj.bias[3] = 1e5
+            layer.self_attn.v_proj.bias[5] = -2e5
+        want = model(input_ids=_ids(2, 9)).logits
+    got = _answers(model, _cache(model, dtype=None))
+    # loud biases make the softmax one of few keys: only that nothing is infinite, and the values' size
+    assert got.isfinite().all() and 0.5 < got.norm() / want.norm() < 2
+
+
+def test_types_that_are_not_held(patched):
+    for bad in (torch.float32, torch.float64, torch.int8):
+        with pytest.raises(ValueError, match="float16"):
+            _cache(_qwen2(), dtype=bad)
