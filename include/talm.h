@@ -775,8 +775,11 @@ int talm_nf4_gemv(const uint16_t* x, int64_t ldx, int64_t n_tokens, const uint8_
  * i-th of them token past[b] + i. bounds and past lie in device memory; rows outside the operands, past the
  * first max_new of a sequence or behind its width blocks are left out (nothing of them is written). The
  * sequences' rows do not overlap. Two sequences may share complete pages; a page that a call writes belongs to
- * one block of one sequence. n_seqs at most 2^24. Strides in elements, multiples of 8; 16-byte aligned buffers
- * (scales, table, bounds and past 4). Non-finite values are held as NaN in a page.
+ * one block of one sequence. Strides in elements, multiples of 8; 16-byte aligned buffers (scales, table, bounds
+ * and past 4). Non-finite values are held as NaN in a page.
+ * Refused as too many: more than 2^24 sequences; writes and reads of 2^31 or more workgroups, 2 n_seqs n_kv
+ * (max_new / 64 + 2) and those of the turned queries; attention of more than 65535 sequences where max_new
+ * n_q / n_kv <= 16, and of 2^24 or more tiles of 32 or 64 rows of a KV head else.
  *
  * talm_cache_write puts k, v [n_rows, n_kv, D] into the cache. With cos and sin (f32 [n_rows, D], row stride
  * cs_stride, a multiple of 4; NULL both: without) the keys are turned by them first (as talm_rope does, rounded

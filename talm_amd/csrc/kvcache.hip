@@ -39,6 +39,8 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr int kBlock = 64;     // tokens of a page
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
+// the most workgroups of a launch's axis: its threads are counted in 32 bits
+constexpr int64_t kGrid = 0xffffffffll / kThreads;
 constexpr int kSplits = 256;   // the most parts that the keys of a row are split into
 constexpr int kNear = 4;       // tiles beside each other that share a die's L2
 
@@ -141,6 +143,7 @@ struct WriteArgs {
   int n_q;
   uint16_t* q_out;  // [n_rows, n_q, D]
   int64_t kv_items;  // workgroups of the cache; those behind them turn the queries
+  uint32_t first;    // the launch's first workgroup of all
 };
 
 // Columns [d, d + 8) of a row of D, turned (the pair of column d is d + D/2 or d - D/2).
@@ -234,8 +237,9 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(WriteArgs a) {
   __shared__ alignas(16) uint16_t tile[kBlock][D + 2];
   __shared__ float tops[kWaves];
   const int tid = threadIdx.x, lane = tid & 63;
-  if (kTurn && blockIdx.x >= a.kv_items) {
-    const int64_t i = (blockIdx.x - a.kv_items) * kThreads + tid;
+  const uint32_t item = a.first + blockIdx.x;
+  if (kTurn && item >= a.kv_items) {
+    const int64_t i = (item - a.kv_items) * kThreads + tid;
     if (i >= a.n_rows * a.n_q * kPer) return;
     const int d = static_cast<int>(i % kPer) * 8;
     const int64_t rh = i / kPer, row = rh / a.n_q;
@@ -245,8 +249,8 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(WriteArgs a) {
     *reinterpret_cast<u32x4*>(a.q_out + rh * D + d) = u32x4{w[0], w[1], w[2], w[3]};
     return;
   }
-  const int rest = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.chunks));
-  const int j = static_cast<int>(blockIdx.x) - rest * a.chunks;
+  const int rest = static_cast<int>(item / static_cast<unsigned>(a.chunks));
+  const int j = static_cast<int>(item) - rest * a.chunks;
   const int seq = (rest >> 1) / a.c.kv, head = (rest >> 1) - seq * a.c.kv, which = rest & 1;
   // the arguments in one cache miss, the sequence's numbers in the next
   asm volatile("" ::"s"(a.bounds), "s"(a.past), "s"(a.n_rows), "s"(a.max_new), "s"(a.max_len), "s"(a.tail),
@@ -377,6 +381,7 @@ struct ReadArgs {
   int max_new, max_len, chunks;
   uint16_t* k;  // [n_rows, kv, D]
   uint16_t* v;
+  uint32_t first;  // the launch's first workgroup of all
 };
 
 // A lane's 16 codes times their scale in 16 bits. A value near the type's largest number may have been rounded
@@ -413,8 +418,9 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(ReadArgs a) {
   constexpr int kPer = D / 8, kEach = kBlock * D / 16 / kThreads;
   __shared__ alignas(16) uint16_t tile[kBlock][D + 8];
   const int tid = threadIdx.x;
-  const int j = static_cast<int>(blockIdx.x % a.chunks);
-  const int rest = static_cast<int>(blockIdx.x / a.chunks);
+  const uint32_t item = a.first + blockIdx.x;
+  const int j = static_cast<int>(item % a.chunks);
+  const int rest = static_cast<int>(item / a.chunks);
   const int which = rest & 1, head = (rest >> 1) % a.c.kv, seq = (rest >> 1) / a.c.kv;
   const Span s = span_of(a.bounds, a.past, seq, a.n_rows, a.max_new, a.max_len);
   const int len = min(max(a.length[seq], 0), a.max_len);
@@ -1215,7 +1221,7 @@ TALM_API int talm_cache_write(const uint16_t* k, int64_t k_stride_tok, int64_t k
   WriteArgs a{k, k_stride_tok, k_stride_head, v, v_stride_tok, v_stride_head, n_rows, bounds, past, max_new,
               width * kBlock, (max_new + kBlock - 1) / kBlock + 1, codes, scales, tail,
               Cache{codes, scales, tail, table, n_pages, width, n_seqs, n_kv_heads}, cos, sin, cs_stride, q,
-              q_stride_tok, q_stride_head, n_q_heads, q_out, 0};
+              q_stride_tok, q_stride_head, n_q_heads, q_out, 0, 0};
   a.kv_items = some ? static_cast<int64_t>(n_seqs) * n_kv_heads * 2 * a.chunks : 0;
   const int64_t turns = turn ? (n_rows * n_q_heads * (head_dim / 8) + kThreads - 1) / kThreads : 0;
   if (a.kv_items + turns > 0x7fffffff) return fail(TALM_EINVAL, "cache_write: too many tokens");
@@ -1228,9 +1234,13 @@ TALM_API int talm_cache_write(const uint16_t* k, int64_t k_stride_tok, int64_t k
     else                                                                                    \
       hipLaunchKernelGGL((cache_write_kernel<T, D, false>), grid, block, 0, st, args);      \
   } while (0)
-  TALM_CACHE_KERNEL(LAUNCH, static_cast<unsigned>(a.kv_items + turns), a);
+  for (int64_t first = 0; first < a.kv_items + turns; first += kGrid) {
+    a.first = static_cast<uint32_t>(first);
+    TALM_CACHE_KERNEL(LAUNCH, static_cast<unsigned>(std::min(a.kv_items + turns - first, kGrid)), a);
+    if (const int status = check_launch("cache_write")) return status;
+  }
 #undef LAUNCH
-  return check_launch("cache_write");
+  return ok();
 }
 
 TALM_API int talm_cache_read(const uint8_t* codes, const float* scales, const uint16_t* tail, const int32_t* table,
@@ -1247,15 +1257,19 @@ TALM_API int talm_cache_read(const uint8_t* codes, const float* scales, const ui
                         static_cast<const void*>(v)})
     if (!aligned(p, 16)) return fail(TALM_EINVAL, "cache_read: buffers must be 16-byte aligned");
   max_new = static_cast<int32_t>(std::min<int64_t>(max_new, n_rows));
-  const ReadArgs a{Cache{codes, scales, tail, table, n_pages, width, n_seqs, n_kv_heads}, length, bounds, past, n_rows,
-                   max_new, width * kBlock, (max_new + kBlock - 1) / kBlock + 1, k, v};
+  ReadArgs a{Cache{codes, scales, tail, table, n_pages, width, n_seqs, n_kv_heads}, length, bounds, past, n_rows,
+                   max_new, width * kBlock, (max_new + kBlock - 1) / kBlock + 1, k, v, 0};
   const int64_t items = static_cast<int64_t>(n_seqs) * n_kv_heads * 2 * a.chunks;
   if (items > 0x7fffffff) return fail(TALM_EINVAL, "cache_read: too many tokens");
   const hipStream_t st = as_stream(stream);
 #define LAUNCH(T, D, grid, block, args) hipLaunchKernelGGL((cache_read_kernel<T, D>), grid, block, 0, st, args)
-  TALM_CACHE_KERNEL(LAUNCH, static_cast<unsigned>(items), a);
+  for (int64_t first = 0; first < items; first += kGrid) {
+    a.first = static_cast<uint32_t>(first);
+    TALM_CACHE_KERNEL(LAUNCH, static_cast<unsigned>(std::min(items - first, kGrid)), a);
+    if (const int status = check_launch("cache_read")) return status;
+  }
 #undef LAUNCH
-  return check_launch("cache_read");
+  return ok();
 }
 
 namespace {
@@ -1323,7 +1337,11 @@ TALM_API int talm_cache_attn(const uint16_t* q, int64_t q_stride_tok, int64_t q_
              reinterpret_cast<float2*>(part_o ? part_o + n_rows * n_q_heads * p.splits * head_dim : nullptr)};
   const int64_t items = (p.wide ? p.tiles : 1) * p.splits;
   const int64_t joins = p.splits > 1 ? static_cast<int64_t>(n_seqs) * max_new * n_q_heads : 0;
-  if (items > 0x7fffffff || joins * (head_dim / 32) > 0x7fffffff || (!p.wide && n_seqs > 65535))
+  // groups of D / 4 lanes in a wavefront; one row's few parts are too little work for it
+  const int lanes = kWave * 4 / head_dim;
+  const int rows = p.splits <= 2 * lanes ? 4 : p.splits <= 8 * lanes ? 1 : 0;
+  const int64_t groups = rows ? (joins + rows * kWaves - 1) / (rows * kWaves) : joins * (head_dim / 32);
+  if (items > kGrid || joins > 0x7fffffff || groups > kGrid || (!p.wide && n_seqs > 65535))
     return fail(TALM_EINVAL, "cache_attn: too many rows, or more than 65535 sequences of few");
   const hipStream_t st = as_stream(stream);
 #define LAUNCH(T, D, grid, block, args)                                                    \
@@ -1339,10 +1357,6 @@ TALM_API int talm_cache_attn(const uint16_t* q, int64_t q_stride_tok, int64_t q_
 #undef LAUNCH
   if (const int status = check_launch("cache_attn")) return status;
   if (joins == 0) return TALM_OK;
-  // groups of D / 4 lanes in a wavefront; one row's few parts are too little work for it
-  const int lanes = kWave * 4 / head_dim;
-  const int rows = p.splits <= 2 * lanes ? 4 : p.splits <= 8 * lanes ? 1 : 0;
-  const int64_t groups = rows ? (joins + rows * kWaves - 1) / (rows * kWaves) : joins * (head_dim / 32);
 #define LAUNCH(T, D, grid, block, args)                                                   \
   do {                                                                                    \
     if (rows == 4)                                                                        \

@@ -97,3 +97,46 @@ def test_operands_with_derivatives_are_refused():
                 call(**{name: dual})
             with forward._set_fwd_grad_enabled(False):
                 call(**{name: dual})
+
+
+def test_more_workgroups_than_a_launch_takes():
+    """600 sequences of 8 heads, the last of which brings 131072 tokens at once: 19.7 million workgroups of a write,
+    and of a read, most of them of sequences that have one token. The same as that sequence alone."""
+    from talm_amd.kv_cache import CacheLayer
+
+    count, kv, dim, long = 600, 8, 64, 131072
+    width, rows = long // 64 + 1, count - 1 + long
+    i32 = {"dtype": torch.int32, "device": "cuda"}
+    g = torch.Generator("cuda").manual_seed(0)
+    k, v = (torch.randn(rows, kv, dim, generator=g, device="cuda").half().transpose(0, 1)[None] for _ in range(2))
+
+    def layer(sequences, tables, pages):
+        new = CacheLayer.allocate(sequences, kv, dim, 64)
+        new.tail.zero_()
+        return CacheLayer(torch.zeros(pages, 2, kv, 64 * dim, dtype=torch.uint8, device="cuda")
+                          .view(torch.float8_e4m3fn), torch.zeros(pages, 2, kv, device="cuda"), new.tail, tables)
+
+    table = torch.full((count, width), -1, **i32)
+    table[-1] = torch.arange(width, **i32)
+    table[:-1, 0] = width + torch.arange(count - 1, **i32)
+    many = layer(count, table, width + count - 1)
+    alone = layer(1, table[-1:], width)
+    first = torch.arange(count, **i32)
+    bounds, past = torch.stack((first, first + 1), 1), torch.zeros(count, **i32)
+    bounds[-1, 1] = rows
+    past[:-1] = 63  # their one token completes a block of what the tail held
+    many.write(k, v, bounds, past, long)
+    at = bounds[-1:] * 1
+    alone.write(k, v, at, past[-1:], long)
+    assert torch.equal(many.codes.view(torch.uint8)[:width], alone.codes.view(torch.uint8))
+    assert torch.equal(many.scales[:width], alone.scales) and torch.equal(many.tail[-1], alone.tail[0])
+    assert (many.codes.view(torch.uint8)[width:] != 0).flatten(2).any(2).all()
+    length = torch.full((count,), 64, **i32)
+    length[-1] = long
+    got = many.read(length, bounds, past, long, rows)
+    want = alone.read(length[-1:], at - (count - 1), past[-1:], long, long)
+    for x, y, new in zip(got, want, (k, v)):
+        assert torch.equal(x[:, :, count - 1:], y)
+        # the short ones' scale is that of their one token: within half a step of a code
+        few = x[:, :, :count - 1].float() - new[:, :, :count - 1].float()
+        assert (few.abs() <= 2.0 ** -4 * new[:, :, :count - 1].float().abs() + 2.0 ** -17).all()
