@@ -26,6 +26,7 @@ from transformers import Cache
 
 from . import _ops, unpad  # noqa: F401 - _ops registers torch.ops.talm.*
 from .engaged import ON, RAN
+from .state import DISABLED, fallback
 
 BLOCK = 64
 _HALVES = (torch.float16, torch.bfloat16)
@@ -302,16 +303,30 @@ class QuantizedCache(Cache):
         scale = scaling if scaling is not None else d ** -0.5
         sinks = unpad.attention_sinks(module) if window is not None else 0
         q = _packed(query.to(self.dtype))
+        out = None
         if s.cu is not None:
-            k, v = _packed(key), _packed(value)
-            if unpad.window_takes(q, k, v):
-                # without a window: one that no sequence is longer than, or the fp16 kernels of training
-                out = unpad.VarlenAttention.apply(q, k, v, s.cu, s.rows, scale) \
-                    if window is None and q.dtype == torch.float16 \
-                    else unpad.window_attention(q, k, v, s.cu, s.rows, scale, window or s.rows, sinks)
-                return out.view(b, t, heads, d).to(query.dtype)
-        out = layer.attention(q, s.bounds, s.past, s.max_new, s.max_len, scale, window, sinks)
-        return self._clean(out).view(b, t, heads, d).to(query.dtype)
+            out = self._first(q, _packed(key), _packed(value), scale, window, sinks)
+        if out is None:
+            out = self._clean(layer.attention(q, s.bounds, s.past, s.max_new, s.max_len, scale, window, sinks))
+        return out.view(b, t, heads, d).to(query.dtype)
+
+    def _first(self, q, k, v, scale, window, sinks):
+        """A first call's attention to its own keys and values in the packed rows' kernels; None where they do
+        not take it, are off or failed (state.py): the cache answers then."""
+        s = self._step
+        if "varlen_attention" in DISABLED or not unpad.window_takes(q, k, v):
+            return None
+        try:
+            # without a window: the fp16 kernels of training, or a window that no sequence is longer than
+            if window is None and q.dtype == torch.float16:
+                out = unpad.VarlenAttention.apply(q, k, v, s.cu, s.rows, scale)
+                RAN["varlen_attn"] += 1
+                return out
+            return unpad.window_attention(q, k, v, s.cu, s.rows, scale, window or s.rows, sinks)
+        except Exception as exc:  # noqa: BLE001 - state.py convention
+            if not fallback("varlen_attention", exc):
+                raise
+        return None
 
     def _clean(self, out):
         """Padding's rows, which no sequence holds, as zeros."""

@@ -5,7 +5,7 @@ import pytest
 import torch
 from transformers import LlamaConfig, LlamaForCausalLM, Qwen2ForCausalLM
 
-from talm_amd import engaged, patches, qgroup, qlora_model, state
+from talm_amd import engaged, patches, qgroup, qlora_model, state, unpad
 from talm_amd.kv_cache import QuantizedCache
 from test_gpu_kv_cache_model import _answer, _ids, _mask, _model
 
@@ -107,3 +107,47 @@ def test_a_bfloat16_model_is_held_in_bfloat16(monkeypatch, patched):
             at += n
     assert cache.dtype is torch.bfloat16
     assert all(layer.tail.dtype is torch.bfloat16 for layer in cache.cache_layers)
+
+
+PIECES = [70, 1, 1, 12]
+
+
+def test_first_calls_are_counted(patched):
+    model = _model()
+    patches.apply()
+    _answer(model, QuantizedCache(model.config, 2, 90), _ids(2, 90), _mask(2, 70, (0, 5)), PIECES)
+    assert engaged.RAN["varlen_attn"] == 3 and engaged.RAN["cache_attn"] == 9
+
+
+@pytest.mark.parametrize("overrides", [{}, SLIDING])
+def test_first_calls_without_the_packed_rows_kernels(monkeypatch, patched, overrides):
+    """Switched off, or failing: the first call reads the cache as the later ones do, and the cache stays whole."""
+    model = _model(**overrides)
+    patches.apply()
+    ids, mask = _ids(2, 90), _mask(2, 70, (0, 5))
+    with monkeypatch.context() as m:
+        m.setattr(unpad, "window_takes", lambda *args: False)
+        want = _answer(model, QuantizedCache(model.config, 2, 90), ids, mask, PIECES)
+    engaged.reset()
+    with monkeypatch.context() as m:
+        m.setitem(state.DISABLED, "varlen_attention", "off")
+        got = _answer(model, QuantizedCache(model.config, 2, 90), ids, mask, PIECES)
+        assert torch.equal(got, want) and engaged.RAN["cache_attn"] == 12
+        assert engaged.RAN["varlen_attn"] == engaged.RAN["window_attn"] == 0
+
+    def broken(*args):
+        raise KeyError("a kernel fails")
+
+    monkeypatch.setattr(state, "STRICT", False)
+    monkeypatch.setattr(unpad, "window_attention", broken)
+    monkeypatch.setattr(unpad.VarlenAttention, "apply", broken)
+    monkeypatch.delitem(state.DISABLED, "varlen_attention", raising=False)
+    try:
+        got = _answer(model, QuantizedCache(model.config, 2, 90), ids, mask, PIECES)
+        assert "KeyError" in state.DISABLED["varlen_attention"]
+    finally:
+        state.DISABLED.pop("varlen_attention", None)
+    assert torch.equal(got, want)
+    monkeypatch.setattr(state, "STRICT", True)
+    with pytest.raises(KeyError):
+        _answer(model, QuantizedCache(model.config, 2, 90), ids, mask, PIECES)
