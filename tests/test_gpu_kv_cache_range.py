@@ -2,10 +2,13 @@
 holds, and long sequences whose every part shows in the output. Tolerances are those of
 test_gpu_kv_cache.py unless a test derives its own."""
 
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_kv_cache import Case
+from oracle import kv_cache as oracle
+from talm_amd import _lib
+from test_gpu_kv_cache import U, Case
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +143,114 @@ def test_more_workgroups_than_a_launch_takes():
         # the short ones' scale is that of their one token: within half a step of a code
         few = x[:, :, :count - 1].float() - new[:, :, :count - 1].float()
         assert (few.abs() <= 2.0 ** -4 * new[:, :, :count - 1].float().abs() + 2.0 ** -17).all()
+
+
+class Visible:
+    """A sequence of T tokens whose 64-token blocks each have a key of their own, D random signs: a query of the same
+    signs gives its block's tokens scores of 20 and others' about 20 / sqrt(D), so that nearly all of its weight
+    lies there, and an output that lost, doubled or misplaced the block is off by hundreds of tolerances (planted()).
+
+    Tolerance, without terms that grow with T. A wavefront sums n keys of at most one part, with weights relative to a
+    reference of its own that is no larger than its largest score: rounded to fp16 they are off by 2^-11 of themselves,
+    or 2^-25 where they are subnormal, which is n 2^-25 max|V| of an output, since a reference's weight is part of
+    the sum; so is their sum. fp32 sums: n products, 4 wavefronts and at most 256 parts, 2^-24 each. Scores: D 2^-24
+    of the sum of their magnitudes, exponents up to 2^5 twice (a weight's and its part's) 2^-19 each. The output: u."""
+
+    def __init__(self, length, dim, dtype, heads, kv=1, new=1, seed=0):
+        self.c = Case(1, kv, dim, length, dtype, seed=seed, heads=heads)
+        self.blocks, self.length, self.new, g = -(-length // 64), length, new, self.c.g
+        self.sign = torch.where(torch.rand(self.blocks, dim, generator=g) < 0.5, -1.0, 1.0)
+        k = self.sign.repeat_interleave(64, 0)[:length, None].expand(length, kv, dim).to(dtype).cuda().transpose(0, 1)[None]
+        v = self.c.rows(length, kv)
+        for lo, hi in ((0, length - new), (length - new, length)):
+            self.c.append([hi - lo], k=k[:, :, lo:hi], v=v[:, :, lo:hi])
+
+    def parts(self, window=0, sinks=0):
+        c = self.c
+        size = _lib.lib().talm_cache_attn_workspace(self.new, c.heads, c.kv, c.dim, 1, self.new, self.length, window, sinks)
+        return max(1, size // (self.new * c.heads * (c.dim + 2) * 4))
+
+    def attend(self, targets, window=None, sinks=0):
+        """targets [new, heads]: the block that each row and head looks at. Returns (query, output) [new, heads, D]."""
+        c = self.c
+        q = (self.sign[targets] * (20.0 / c.dim ** 0.5)).to(c.dtype).cuda()
+        past = torch.tensor([self.length - self.new], dtype=torch.int32).cuda()
+        bounds = torch.tensor([[0, self.new]], dtype=torch.int32).cuda()
+        out = c.layer.attention(q.transpose(0, 1)[None], bounds, past, self.new, self.length, c.dim ** -0.5, window, sinks)
+        return q.double().cpu().numpy(), out[0].double().cpu().numpy()
+
+    def check(self, q, got, target, past, head=0, window=None, sinks=0):
+        """Rows q, got [n, D] of one KV head that look at blocks `target` [n], at places past, past + 1, .."""
+        c = self.c
+        k, v = (x[head] for x in self.held)
+        scale = c.dim ** -0.5
+        want, size, score = oracle.attention(q, k, v, past, scale, window, sinks)
+        visits = self.blocks if window is None else min(self.blocks, (window + 63) // 64 + 2 + (sinks + 63) // 64)
+        n = 64 * -(-visits // self.parts(window or 0, sinks))
+        rel = 2.0 ** -11 + 2 * (c.dim * 2.0 ** -24 * score + 2.0 ** -18) + (n + 260) * 2.0 ** -24
+        tol = rel * (size + np.abs(want)) + U[c.dtype] * np.abs(want) + 2.0 ** -25 * (n * np.abs(v).max() + 1)
+        worst = float((np.abs(got - want) / tol).max())
+        planted = min(self.planted(x, w, t, k, v, y, p) for x, w, t, y, p in zip(q, want, tol, target, past + np.arange(len(q))))
+        print(f"[case] {self.length} tokens, {self.parts(window or 0, sinks)} parts, D={c.dim} {c.dtype} window={window}: "
+              f"worst {worst:.3f} of its tolerance, a lost block {planted:.0f}", flush=True)
+        assert not np.isnan(got).any() and worst <= 1.0
+        assert planted >= 20
+
+    def planted(self, q, want, tol, k, v, block, place):
+        """How many tolerances the output would be off without the block that the row looks at."""
+        at = slice(64 * block, min(64 * block + 64, place + 1))
+        s = q @ k[at].T * self.c.dim ** -0.5
+        if not len(s):
+            return np.inf
+        # nearly all of the weight is the block's: what is left without it is a mean of the others, taken as 0
+        p = np.exp(s - s.max())
+        return float((np.abs(p @ v[at] / p.sum()) / tol).max())
+
+    @property
+    def held(self):
+        if not hasattr(self, "_held"):
+            self._held = self.c.values(0)
+        return self._held
+
+
+@pytest.mark.parametrize("length,parts", [(1500, 6), (3000, 12), (8999, 36), (65536, 256), (100001, 224)])
+@pytest.mark.parametrize("dim,dtype", [(128, torch.float16), (64, torch.float16), (128, torch.bfloat16), (64, torch.bfloat16)])
+def test_every_part_of_a_long_sequence_shows(length, parts, dim, dtype):
+    """One token's 16 heads, in all of the join's forms; a block of every part, and every wavefront's in turn."""
+    x = Visible(length, dim, dtype, 16)
+    assert x.parts() == parts
+    per = -(-x.blocks // parts)
+    targets = np.array([min(r * per + r % per, x.blocks - 1) for r in range(-(-parts // 16) * 16)])
+    outs = [x.attend(torch.from_numpy(targets[lo:lo + 16])[None]) for lo in range(0, len(targets), 16)]
+    q, got = (np.concatenate([o[i][0] for o in outs]) for i in range(2))
+    # each at the last token's place: as rows behind it they see the same keys
+    x.check(q, got, targets, length - 1)
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, torch.float16), (64, torch.bfloat16)])
+def test_every_part_of_a_long_window_shows(dim, dtype):
+    length, window, sinks = 50001, 30000, 200
+    x = Visible(length, dim, dtype, 16)
+    seen = np.r_[0:3, (length - window) // 64 + 1:x.blocks]  # whole blocks but for the sinks' last and the newest
+    targets = seen[np.linspace(0, len(seen) - 1, 16 * 12).astype(int)]
+    for lo in range(0, len(targets), 16):
+        q, got = x.attend(torch.from_numpy(targets[lo:lo + 16])[None], window, sinks)
+        for h in range(16):
+            x.check(q[:, h], got[:, h], targets[lo + h:lo + h + 1], length - 1, 0, window, sinks)
+
+
+@pytest.mark.parametrize("length,new,heads,kv,dim,dtype", [
+    (9000, 200, 12, 2, 128, torch.float16), (9000, 600, 12, 2, 128, torch.bfloat16), (7001, 20, 8, 2, 64, torch.float16),
+    (700, 300, 4, 2, 64, torch.bfloat16)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (3000, 100)])
+def test_every_block_of_a_piece_shows(length, new, heads, kv, dim, dtype, window, sinks):
+    """Tiles of 32 and 64 rows: every row and head looks at a block that it sees."""
+    x = Visible(length, dim, dtype, heads, kv, new)
+    past, g = length - new, np.random.default_rng(0)
+    place = past + np.arange(new)[:, None]
+    first = np.maximum(place - (window or length) + 1, 0) // 64 + 1  # whole blocks of a window
+    first = np.minimum(first, place // 64)
+    targets = first + (g.random((new, heads)) * (place // 64 - first + 1)).astype(int)
+    q, got = x.attend(torch.from_numpy(targets), window, sinks)
+    for h in range(heads):
+        x.check(q[:, h], got[:, h], targets[:, h], past, h * kv // heads, window, sinks)

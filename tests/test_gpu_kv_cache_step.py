@@ -7,7 +7,7 @@ from transformers import LlamaConfig, LlamaForCausalLM, Qwen2ForCausalLM
 
 from talm_amd import engaged, patches, qgroup, qlora_model, state, unpad
 from talm_amd.kv_cache import QuantizedCache
-from test_gpu_kv_cache_model import _answer, _ids, _mask, _model
+from test_gpu_kv_cache_model import Plain, _answer, _ids, _mask, _model, _near
 
 pytestmark = pytest.mark.gpu
 
@@ -151,3 +151,38 @@ def test_first_calls_without_the_packed_rows_kernels(monkeypatch, patched, overr
     monkeypatch.setattr(state, "STRICT", True)
     with pytest.raises(KeyError):
         _answer(model, QuantizedCache(model.config, 2, 90), ids, mask, PIECES)
+
+
+@pytest.mark.parametrize("batch,pads", [(1, (0,)), (3, (0, 70, 131))])
+@pytest.mark.parametrize("heads", [{}, {"num_attention_heads": 8, "num_key_value_heads": 2, "head_dim": 64}])
+def test_sliding_layers_over_pages(patched, batch, pads, heads):
+    """Windows and sinks over 8-bit pages: a prompt of four blocks, single tokens that complete a block, a piece and
+    a short one, left-padded, against a plain cache that holds what the 8-bit one does under masks that
+    say the window and the sinks."""
+    model = _model(**{**SLIDING, **heads, "sliding_window": 90, "attention_sinks": 5})
+    patches.apply()
+    pieces = [250, 1, 1, 1, 1, 1, 1, 45, 5, 1]
+    ids, mask = _ids(batch, sum(pieces)), _mask(batch, 250, pads)
+    got = _answer(model, QuantizedCache(model.config, batch, 320), ids, mask, pieces)
+    model.config.attention_sinks = 0  # the masks hold them
+    cache, outs, at = Plain(rounded_at_first=bool(heads)), [], 0
+    for n in pieces:
+        seen = torch.cat((mask, mask.new_ones(batch, max(0, at + n - 250))), 1)[:, :at + n]
+        place = (seen.cumsum(1) - 1).clamp_min(0)
+        key, row = place[:, None], place[:, at:at + n, None]
+        column = torch.arange(at + n, device="cuda")
+        full = (column <= column[at:at + n, None]) & (seen[:, None] > 0)
+        slide = full & ((row - key < 90) | (key < 5))
+        # rows of padding look at themselves: no row is empty
+        own = (column == column[at:at + n, None])[None]
+        masks = {"full_attention": (full | own)[:, None], "sliding_attention": (slide | own)[:, None]}
+        cache.mask = seen
+        with torch.no_grad(), torch.autocast("cuda", dtype=torch.float16):
+            hidden = model.model(input_ids=ids[:, at:at + n], attention_mask=masks, position_ids=place[:, at:at + n],
+                                 past_key_values=cache, use_cache=True).last_hidden_state
+            outs.append(model.lm_head(hidden[:, -1]).float())
+        at += n
+    _near(got, torch.stack(outs))
+    # and the masks matter: without the sinks the answers are others
+    other = _answer(model, QuantizedCache(model.config, batch, 320), ids, mask, pieces)
+    assert (other - got).norm() > 5e-3 * got.norm()
