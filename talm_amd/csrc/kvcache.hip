@@ -729,8 +729,8 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) vw[i] = load(src + L::value_at(i));
   };
-  // Weights of a page's (or the tail's) scores; the sums so far follow a new reference and unit.
-  auto weigh = [&](float c, bool mask, int first, float ratio) __attribute__((always_inline)) {
+  // Weights of a page's (or the tail's, times 2^-low) scores; the sums so far follow a new reference and unit.
+  auto weigh = [&](float c, bool mask, int first, float ratio, float low) __attribute__((always_inline)) {
     c = fmaxf(c, 1e-37f);  // never 0: c times a hidden score's -inf is one
     if (mask) {
       // the lane's scores are those of the keys base + kStep (i / 4) + i % 4
@@ -767,7 +767,7 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
 #pragma unroll
         for (int e = 0; e < L::kEach; ++e) acc[n][e] *= grow * ratio;
     }
-    const float base = ref == -__builtin_inff() ? 0.f : ref;  // its weights are exp2(-inf - 0) = 0
+    const float base = ref == -__builtin_inff() ? 0.f : ref + low;  // its weights are exp2(-inf - 0) = 0
 #pragma unroll
     for (int i = 0; i < L::kLane; ++i) {
       st[i / L::kEach][i % L::kEach] =
@@ -832,7 +832,8 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
       __builtin_amdgcn_sched_barrier(0);
       const bool all = page >= 0 && first + kBlock - 1 <= lo_place &&
                        (a.window == 0 || hi_place - first < a.window || first + kBlock <= a.sinks);
-      weigh(a.scale_log2 * k_scale, !all, page >= 0 ? first : 0x7fff0000, kUnits ? unit * inverse(v_scale) : 1.f);
+      weigh(a.scale_log2 * k_scale, !all, page >= 0 ? first : 0x7fff0000, kUnits ? unit * inverse(v_scale) : 1.f,
+            0.f);
       if constexpr (kUnits) unit = v_scale;
       // P in fp16 whatever the operands' type: the values' codes are exact in it. The error is that of
       // a rounding to 11 bits, and its sum is that of the rounded weights, so a token that has nearly all
@@ -884,21 +885,23 @@ __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kerne
       for (int f = 0; f < L::kFrags; ++f)
         st[t] = T::mfma(*reinterpret_cast<const half8*>(tk + (t * kCol + col) * D + L::column(f, g)), q[f], st[t]);
     }
-    weigh(a.scale_log2, true, first, unit);
+    weigh(a.scale_log2, true, first, unit, kUnits ? 0.f : 40.f);
     unit = 1.f;
     // the weights in the tail's type; for bfloat16 as two parts, so that they keep 16 bits
     half8 hi[L::kPs], lo[L::kPs];
     if constexpr (kUnits) {
       round(hi);
     } else {
+      float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < L::kLane; ++i) {
-        const float x = st[i / L::kEach][i % L::kEach], y = x * T::kUnit;
-        const uint16_t b = T::down(y);
+        const float x = st[i / L::kEach][i % L::kEach];
+        const uint16_t b = T::down(x);
         hi[i / 8][i % 8] = __builtin_bit_cast(_Float16, b);
-        lo[i / 8][i % 8] = __builtin_bit_cast(_Float16, T::down(y - T::up(b)));
-        l += x;
+        lo[i / 8][i % 8] = __builtin_bit_cast(_Float16, T::down(x - T::up(b)));
+        sum += x;
       }
+      l += sum * (1.f / T::kUnit);
     }
 #pragma unroll
     for (int n = 0; n < L::kOuts; ++n)
