@@ -602,12 +602,13 @@ struct Lay {
 // Tiles of 16 rows, for sequences of a token or two: the pages come from memory once, and that is the time. One
 // token of each of 64 sequences of 201 to 8191 tokens, 143 MB, takes 29 us (4.9 TB/s of a copy's 5.2) and 4 for
 // the join; one over 131001, 67 MB, 14 and 4; one over 4001 5.6 and 3.2, where the start is most of it.
-// Tiles of 32 and 64 rows: the VALU's issue is the time. A wavefront's page of 32 rows takes some 500 issue
-// slots of 4 cycles: 128 conversions of codes, 150 for the softmax (an exponential has two), 64 of the 32
-// MFMAs, the loads, and its share of the start and the join. 512 rows of 6 heads each over 8289 tokens 39
-// us (648 TF/s) and 6 for the join, the next turns of 12 conversations (1 to 300 tokens behind 300 to 3500) 55
-// (590 TF/s). Converted pages shared through LDS, and 64 columns a wavefront on one wavefront a SIMD, were no
-// faster (the same; 62 against 48 us with the join).
+// Tiles of 32 and 64 rows: issue is the largest share of the time. A wavefront's page of 32 rows takes some 485
+// issue slots of 4 cycles (bfloat16 535): 128 conversions of codes, 150 for the softmax (an exponential has two),
+// 64 of the 32 MFMAs, the loads, and its share of the start and the join. 512 rows of 6 heads each over 8289
+// tokens 40 us (630 TF/s) and 6 for the join: 25 of issue at the clock of this load, 4.4 until all workgroups
+// run, and ends that spread over 14. The next turns of 12 conversations (1 to 300 tokens behind 300 to 3500) 56 us
+// (580 TF/s), 35 of them issue. Converted pages shared through LDS, and 64 columns a wavefront on one wavefront
+// a SIMD, were no faster (the same; 62 against 48 us with the join).
 template <class T, int D, int kCol, int kWide>
 __global__ __launch_bounds__(kThreads, kCol == 16 ? 3 : 2) void cache_attn_kernel(AttnArgs a) {
   using L = Lay<D, kCol>;

@@ -46,8 +46,8 @@ class CacheLayer:
     bounds[b, 1] - 1, its tokens past[b], past[b] + 1, ..; `bounds` int32 [sequences, 2] and `past` int32
     [sequences] lie on the device, `max_new` is at least the largest count of rows. Rows that no sequence
     holds, that lie past max_new or do not fit the table are not written. The operators run on the
-    current stream, wait for nothing and can be captured in a HIP graph; they have no gradient and
-    refuse operands that need one. A row belongs to one sequence, and a page that a call writes to one
+    current stream, wait for nothing and can be captured in a HIP graph; they have no derivative and
+    refuse operands that need one (that require a gradient, or are dual). A row belongs to one sequence, and a page that a call writes to one
     block of one sequence."""
 
     def __init__(self, codes, scales, tail, table):
@@ -100,8 +100,8 @@ class CacheLayer:
         tokens up to p, in a `window` only the last `window` ones (itself among them) and the sequence's
         first `sinks`. `max_len` is at least the longest sequence with its new tokens (in a graph: with those
         of any replay). Values of tokens that a row does not see must be finite, since a weight of 0 does
-        not hide NaN; its keys may be anything. Returns [1, N, Hq, D]; a row that sees nothing is zero, a row
-        that no sequence holds undefined."""
+        not hide NaN; its keys may be anything. Returns [1, N, Hq, D], means of values and none past the
+        type's largest number; a row that sees nothing is zero, a row that no sequence holds undefined."""
         if window is not None and window < 1:
             raise ValueError(f"cache_attention: window {window} (at least 1, or None)")
         out = torch.ops.talm.cache_attention(query, bounds, past, max_new, max_len, self.codes, self.scales,
@@ -128,8 +128,8 @@ class QuantizedCache(Cache):
     128), later ones, and first ones of heads of 64, to the cache. `dtype`, of its 16-bit parts and its
     attention, is by default that of the first call's keys: float32 ones count as autocast's type, and
     without autocast as bfloat16, which has their range. A named float16 makes numbers past 65504
-    infinite. It needs solution.apply(), the "sdpa"
-    attention, and no gradient; it does not reorder, repeat or crop its sequences (beam search, assisted
+    infinite. Models that run inside of its calls (a hook's) are answered on their own. It needs
+    solution.apply(), the "sdpa" attention, no gradient, and every layer's call (no checkpointed ones); it does not reorder, repeat or crop its sequences (beam search, assisted
     generation), and its calls run eagerly (a step to capture in a HIP graph takes CacheLayer)."""
 
     is_compileable = False
