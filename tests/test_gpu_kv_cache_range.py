@@ -254,3 +254,26 @@ def test_every_block_of_a_piece_shows(length, new, heads, kv, dim, dtype, window
     q, got = x.attend(torch.from_numpy(targets), window, sinks)
     for h in range(heads):
         x.check(q[:, h], got[:, h], targets[:, h], past, h * kv // heads, window, sinks)
+
+
+@pytest.mark.parametrize("dim,heads,length", [(64, 4, 300), (128, 16, 300), (64, 16, 3000), (128, 6, 5000), (64, 2, 40)])
+def test_single_tokens_weights_are_of_32_bits(dim, heads, length):
+    """Weights of a single token's rows are no coarser than fp32 sums: keys and queries of few bits, whose scores are
+    exact, leave exponents below 2^4 with a product's and a subtraction's rounding (2^-20 of a weight, with exp2), two
+    parts of 11 bits (2^-22, or 2^-25 of a reference's weight), sums of at most 128 tokens a wavefront, 4 of them and
+    a few parts (256 2^-24 in all), and the output's half step."""
+    c = Case(1, 1, dim, length, heads=heads)
+    few = torch.tensor([-1.0, -0.5, 0.0, 0.5, 1.0])
+    k = few[torch.randint(5, (length, dim), generator=c.g)].half().cuda()[None, None]
+    c.append([length - 1], k=k[:, :, :-1])
+    c.append([1], k=k[:, :, -1:])
+    q = (torch.randint(-8, 9, (1, heads, 1, dim), generator=c.g) / 4).half().cuda()
+    past = torch.tensor([length - 1], dtype=torch.int32).cuda()
+    out = c.layer.attention(q, torch.tensor([[0, 1]], dtype=torch.int32).cuda(), past, 1, length, 0.125)
+    (k,), (v,) = c.values(0)
+    want, size, _ = oracle.attention(q[0, :, 0].double().cpu().numpy(), k, v, length - 1, 0.125)
+    rel = 2.0 ** -20 + 2.0 ** -22 + 256 * 2.0 ** -24
+    tol = rel * (size + np.abs(want)) + 2.0 ** -11 * np.abs(want) + 2.0 ** -25 * (128 * 2.0 ** -8 * np.abs(v).max() + 1)
+    worst = (np.abs(out[0, 0].double().cpu().numpy() - want) / tol).max()
+    print(f"[case] D={dim} {length} tokens: worst {worst:.3f} of its tolerance", flush=True)
+    assert worst <= 1.0
