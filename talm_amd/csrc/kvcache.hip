@@ -600,8 +600,8 @@ struct Lay {
 // they are.
 //
 // Tiles of 16 rows, for sequences of a token or two: the pages come from memory once, and that is the time. One
-// token of each of 64 sequences of 201 to 8191 tokens, 143 MB, takes 29 us (4.9 TB/s of a copy's 5.2) and 4 for
-// the join; one over 131001, 67 MB, 14 and 4; one over 4001 5.6 and 3.2, where the start is most of it.
+// token of each of 64 sequences of 201 to 8191 tokens, 143 MB, takes 30 us (4.8 TB/s of a copy's 5.2) and 4 for
+// the join; one over 131001, 67 MB, 14.5 and 4; one over 4001 5.8 and 3.3, where the start is most of it.
 // Tiles of 32 and 64 rows: issue is the largest share of the time. A wavefront's page of 32 rows takes some 485
 // issue slots of 4 cycles (bfloat16 535): 128 conversions of codes, 150 for the softmax (an exponential has two),
 // 64 of the 32 MFMAs, the loads, and its share of the start and the join. 512 rows of 6 heads each over 8289

@@ -47,8 +47,8 @@ class CacheLayer:
     [sequences] lie on the device, `max_new` is at least the largest count of rows. Rows that no sequence
     holds, that lie past max_new or do not fit the table are not written. The operators run on the
     current stream, wait for nothing and can be captured in a HIP graph; they have no derivative and
-    refuse operands that need one (that require a gradient, or are dual). A row belongs to one sequence, and a page that a call writes to one
-    block of one sequence."""
+    refuse operands that need one (that require a gradient, or are dual). A row belongs to one sequence,
+    and a page that a call writes to one block of one sequence."""
 
     def __init__(self, codes, scales, tail, table):
         self.codes, self.scales, self.tail, self.table = codes, scales, tail, table
@@ -128,9 +128,11 @@ class QuantizedCache(Cache):
     128), later ones, and first ones of heads of 64, to the cache. `dtype`, of its 16-bit parts and its
     attention, is by default that of the first call's keys: float32 ones count as autocast's type, and
     without autocast as bfloat16, which has their range. A named float16 makes numbers past 65504
-    infinite. Models that run inside of its calls (a hook's) are answered on their own. It needs
-    solution.apply(), the "sdpa" attention, no gradient, and every layer's call (no checkpointed ones); it does not reorder, repeat or crop its sequences (beam search, assisted
-    generation), and its calls run eagerly (a step to capture in a HIP graph takes CacheLayer)."""
+    infinite. Models that run inside of its calls (a hook's) are answered on their own.
+
+    It needs solution.apply(), the "sdpa" attention, no gradient, and every layer's call (no checkpointed
+    ones); it does not reorder, repeat or crop its sequences (beam search, assisted generation), and its
+    calls run eagerly (a step to capture in a HIP graph takes CacheLayer)."""
 
     is_compileable = False
 
